@@ -99,6 +99,55 @@ int nsv_verify_attention_tile_refs(
     size_t workspace_bytes, void* stream);
 
 /*
+ * Paged attention of a few rows per sequence with a sliding window and a few
+ * first tokens that stay visible.  No reference counterpart (its attention
+ * sees every key).  As nsv_verify_attention, but the row at position p sees
+ * key j only if j > p - window or j < sinks (window > 0, sinks >= 0).  K/V of
+ * keys that no row of the sequence sees are not read, nor their block-table
+ * entries used.  Rows that see no key are written as zeros.
+ * Supported: D in {64, 128}; H % Hkv == 0; max_q_len <= 64; block_size a
+ * power of two; q, out and the caches on 16 bytes; fewer than 2^31 cached
+ * keys.
+ * Workspace: nsv_window_attention_workspace_size() bytes on 16 bytes, of any
+ * content; calls that share one must not run concurrently.
+ */
+size_t nsv_window_attention_workspace_size(int B, int H, int Hkv, int D,
+                                           int block_size, int max_blocks,
+                                           int max_q_len, int dtype,
+                                           int window, int sinks);
+int nsv_window_attention(void* out, const void* q, const void* k_cache,
+                         const void* v_cache, const int32_t* block_tables,
+                         const int64_t* context_lens,
+                         const int32_t* cu_seqlens_q, const int64_t* positions,
+                         float scale, int B, int T, int H, int Hkv, int D,
+                         int block_size, int max_blocks, int max_q_len,
+                         int dtype, int window, int sinks, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/*
+ * nsv_verify_attention that adds every key's attention weight, summed over
+ * the rows and over the query heads of its kv head, to
+ *   key_weights  [num_blocks, Hkv, block_size] fp32, paged as the caches are
+ * The place of a key at or behind the position of its sequence's first row
+ * is set, an older key's added to; places of keys past the last row and of
+ * unmapped pages keep their value.  Rows with positions[r] < 0 add nothing.
+ * No reference counterpart.  Shapes and workspace as nsv_window_attention's.
+ */
+size_t nsv_weights_attention_workspace_size(int B, int H, int Hkv, int D,
+                                            int block_size, int max_blocks,
+                                            int max_q_len, int dtype);
+int nsv_weights_attention(void* out, const void* q, const void* k_cache,
+                          const void* v_cache, float* key_weights,
+                          const int32_t* block_tables,
+                          const int64_t* context_lens,
+                          const int32_t* cu_seqlens_q,
+                          const int64_t* positions, float scale, int B, int T,
+                          int H, int Hkv, int D, int block_size,
+                          int max_blocks, int max_q_len, int dtype,
+                          void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/*
  * Causal prefill attention (bf16): rows of several prompts attend keys 0 ..
  * their position.
  * Replaces layers/attention.py:123-363 (the varlen and the paged prefill

@@ -9,6 +9,7 @@ operator raises.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -47,6 +48,12 @@ SIGNATURES: dict[str, tuple] = {
     "nsv_prefill_tiles": (_c_int, [_c_vp] * 2 + [_c_int] * 5 + [_c_vp, _c_i64, _c_vp]),
     "nsv_prefill_attention": (
         _c_int, [_c_vp] * 6 + [_c_int] * 2 + [_c_vp, _c_int, _c_f32] + [_c_int] * 5 + [_c_vp] * 2),
+    "nsv_window_attention_workspace_size": (_c_size, [_c_int] * 10),
+    "nsv_window_attention": (
+        _c_int, [_c_vp] * 8 + [_c_f32] + [_c_int] * 11 + [_c_vp, _c_size, _c_vp]),
+    "nsv_weights_attention_workspace_size": (_c_size, [_c_int] * 8),
+    "nsv_weights_attention": (
+        _c_int, [_c_vp] * 9 + [_c_f32] + [_c_int] * 9 + [_c_vp, _c_size, _c_vp]),
     "nsv_verify_attention_load_floor": (_c_int, [_c_vp] * 4 + [_c_int] * 6 + [_c_vp, _c_vp]),
     "nsv_stream_read": (_c_int, [_c_vp, _c_size, _c_int, _c_vp, _c_vp]),
     "nsv_store_kv": (_c_int, [_c_vp] * 5 + [_c_int] * 5 + [_c_vp]),
@@ -135,6 +142,15 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
+
+
+_no_guard = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """Makes ``device`` the current one for a launch, where it is not (a
+    kernel runs on the current device, whatever device its stream is of)."""
+    return _no_guard if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -1,0 +1,840 @@
+// Paged attention of a few query rows per sequence (verify rows, decode
+// steps) over a bounded cache, for gfx950:
+//   * with a sliding window and a few first tokens that stay visible;
+//   * with the attention weight of every key added to a paged table.
+//
+//   row r at position p sees key j  <=>  j <= p, j < context, its page is
+//   mapped, and (with a window W) j > p - W or j < sinks
+//   out_r = sum_j 2^(s_rj - m_r) v_j / l_r,  s_rj = scale log2(e) q_r . k_j
+//   weight of (kv head, key j) = sum_r sum_(heads of the group) 2^(s_rj - m_r) / l_r
+//
+// What bounds it: the K/V bytes of the keys that some row of a sequence
+// sees.  Those are one or two runs of keys (the first ones, the windows'
+// union), numbered through as virtual keys; a workgroup takes a part of one
+// (sequence, kv head) pair's virtual keys for up to 64 query rows (the pair's
+// group heads x rows; further heads in workgroups of their own), so no byte
+// is read for a key that no row sees.  Its four waves take tiles of keys in
+// turn, each wave from its own LDS: K and V rows go from memory straight to
+// LDS two tiles deep, with no barrier in the loop.
+//
+// Products: S^T = K Q^T puts a row's scores into four lanes (16-lane group g
+// holds keys 4 g + i), which is the operand layout of O^T = V^T P^T, so
+// weights move through no shuffle.  bf16: v_mfma_f32_16x16x32_bf16, V^T from
+// the transposing LDS reads; fp32: v_mfma_f32_16x16x4_f32, whose terms are
+// numbered so that 16-byte LDS reads feed them.  Maxima, sums and outputs are
+// held in fp32; the weights P are rounded to bf16 for the second product (at
+// an exponent reference of every tile's maximum), never for the key weights.
+
+#include "common.h"
+
+#include <algorithm>
+
+namespace {
+
+constexpr int kWaves = 4;         // waves per workgroup
+constexpr int kMaxPages = 2048;   // block-table entries of a workgroup's keys held in LDS
+constexpr int kMaxSplits = 64;
+constexpr float kNegInf = -__builtin_inff();
+
+enum Mode { kAttend, kAttendScores, kWeights };
+
+struct RowArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const int32_t* block_tables;
+  const int64_t* context_lens;
+  const int32_t* cu_seqlens_q;
+  const int64_t* positions;
+  float2* part_ml;    // [npairs * subsets][S][R]: (maximum, log2 domain; sum)
+  float* part_o;      // [npairs * subsets][S][R][D], unnormalised
+  float* scores;      // [npairs][R][score_keys], log2 domain, -inf where masked (kAttendScores)
+  float* key_weights; // [num_blocks][Hkv][block_size]
+  float scale_log2;
+  int H, Hkv, G, subsets;  // query heads, kv heads, query heads of a kv head that a workgroup serves, how often
+  int bs_log2, max_blocks, QL, R, S, npairs;  // R = G * QL
+  int window, sinks;  // window 0: every key up to the row
+  int score_keys;
+  int first_subset;   // kWeights: the subset this launch adds
+};
+
+typedef short i16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+
+__device__ __forceinline__ bf16x8 as_bf16x8(u32x4 v) { return __builtin_bit_cast(bf16x8, v); }
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ uint2 lds_read_tr(const unsigned char* p) {
+  const i16x4 v = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4*)(p));
+  return __builtin_bit_cast(uint2, v);
+}
+
+// over the four 16-lane groups' values of the same lane
+__device__ __forceinline__ float groups_max(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float groups_sum(float v) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The keys of a sequence that some row of the call sees, numbered 0 .. total
+// - 1: the first `head` keys, then those from head + gap on.
+struct Span {
+  int total, head, gap;
+  int pos_min, pos_max;  // of the sequence's rows that are no padding
+  __device__ int key(int v) const { return v < head ? v : v + gap; }
+};
+
+// (every lane of the wave; the sequence's rows are q0 .. q0 + qlen - 1)
+__device__ __forceinline__ Span make_span(const RowArgs& a, int b, int q0, int qlen, int& my_pos) {
+  const int lane = threadIdx.x & 63;
+  const int64_t cap = (int64_t)a.max_blocks << a.bs_log2;
+  const int64_t len = a.context_lens[b];
+  const int ctx = uniform((int)(len < 0 ? 0 : (len < cap ? len : cap)));
+  int64_t p64 = -1;
+  if (lane < qlen) p64 = a.positions[q0 + lane];
+  my_pos = p64 < 0 ? -1 : (int)(p64 < 0x3fffffff ? p64 : 0x3fffffff);
+  int lo = my_pos < 0 ? 0x7fffffff : my_pos, hi = my_pos;
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) {
+    lo = min(lo, __shfl_xor(lo, d, 64));
+    hi = max(hi, __shfl_xor(hi, d, 64));
+  }
+  Span s;
+  s.pos_min = uniform(lo);
+  s.pos_max = uniform(hi);
+  s.total = s.head = min(ctx, s.pos_max + 1);  // (no row at all: 0)
+  s.gap = 0;
+  if (a.window > 0 && s.pos_max >= 0) {
+    const int first = max(0, s.pos_min - a.window + 1);  // of the windows' union
+    const int head = min(a.sinks, s.total);
+    if (first > head) {
+      s.head = head;
+      s.gap = first - head;
+      s.total = head + max(0, s.total - first);
+    }
+  }
+  return s;
+}
+
+// Keys per split: the span spread evenly over S splits, in whole turns of
+// the workgroup's waves where that leaves none of them short.
+template <int TK>
+__device__ __forceinline__ int split_keys(int total, int S) {
+  const int per = (total + S - 1) / S;
+  return max((per + TK - 1) / TK * TK, TK * kWaves);
+}
+
+template <typename T, int DH>
+struct Shape {
+  static constexpr bool kBf16 = sizeof(T) == 2;
+  static constexpr int TK = kBf16 ? 32 : 16;          // keys per tile
+  static constexpr int ROWB = DH * (int)sizeof(T);    // bytes per row
+  static constexpr int CPR = ROWB / 16;               // 16-byte chunks per row
+  static constexpr int RPI = 64 / CPR;                // rows one load instruction fills
+  static constexpr int J = TK / RPI;                  // load instructions per K (or V) tile
+  static constexpr int TILEB = TK * ROWB;
+  static constexpr int KT = TK / 16;                  // 16-key score tiles
+  static constexpr int QV = DH / (kBf16 ? 32 : 16);   // 16-byte query pieces per lane
+  // the slot of a row's chunk: the 16 rows (K) and the 8 or 4 rows (V) that
+  // one read's lanes touch fall into different banks
+  static __device__ __forceinline__ int kswz(int r) { return r & (CPR < 16 ? CPR - 1 : 15); }
+  static __device__ __forceinline__ int vswz(int r) {
+    if constexpr (!kBf16) return 0;  // (16 lanes read 256 consecutive bytes)
+    else return CPR >= 16 ? (r & 7) << 1 : ((r >> 1) & 3) << 1;
+  }
+};
+
+template <typename T, int MT, int DH, int MODE>
+__global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a) {
+  using S_ = Shape<T, DH>;
+  constexpr bool BF16 = S_::kBf16;
+  constexpr int TK = S_::TK, KT = S_::KT, J = S_::J, ROWB = S_::ROWB, CPR = S_::CPR, RPI = S_::RPI;
+  constexpr int NT = kWaves * 64, MP = MT * 16;
+  constexpr int DT = DH / 16;
+  constexpr bool V = MODE != kWeights;
+  constexpr int BUFS = 2;
+  constexpr int WAVEB = BUFS * 2 * S_::TILEB;  // one wave's tiles; later its rows of O
+  static_assert(WAVEB >= MP * DH * 4 || !V, "a wave's tiles hold its output rows");
+  struct __attribute__((aligned(16))) Lds {
+    unsigned char tiles[kWaves][V ? WAVEB : WAVEB / 2];
+    int pages[kMaxPages];
+    float2 ml[kWaves][MP];
+    float2 row[MP];
+    int holes, mapped;
+  };
+  __shared__ Lds lds;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int w = uniform(tid >> 6);
+  const int g = lane >> 4, c = lane & 15;
+  const int pair = blockIdx.x % a.npairs;
+  const int rest = blockIdx.x / a.npairs;
+  const int sub = MODE == kWeights ? a.first_subset : rest % a.subsets;
+  const int split = MODE == kWeights ? rest : rest / a.subsets;
+  const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
+  const int head0 = hk * (a.G * a.subsets) + sub * a.G;  // first query head
+  const int q0 = uniform(a.cu_seqlens_q[b]);
+  const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
+  int my_pos;
+  const Span sp = make_span(a, b, q0, qlen, my_pos);
+  const int per = split_keys<TK>(sp.total, a.S);
+  const int v0 = split * per;
+  const int v1 = min(sp.total, v0 + per);
+  const int64_t part = ((int64_t)(pair * a.subsets + sub) * a.S + split) * a.R;
+  if (v0 >= v1 && split > 0) {  // uniform: this sequence has fewer splits
+    if (V && tid < a.R) a.part_ml[part + tid] = make_float2(kNegInf, 0.f);
+    return;
+  }
+
+  // ---- query rows m = head * QL + t: the B operand of S^T, lane (g, c) holds row c
+  u32x4 q[MT][S_::QV];
+  int pos[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int m = mt * 16 + c;
+    const int gh = m / a.QL, t = m - gh * a.QL;
+    const int p = __shfl(my_pos, t & 63, 64);
+    const bool live = m < a.R && t < qlen;
+    pos[mt] = live ? p : -1;
+    const T* src = (const T*)a.q + ((int64_t)(q0 + (live ? t : 0)) * a.H + head0 + (live ? gh : 0)) * DH + g * (16 / (int)sizeof(T));
+#pragma unroll
+    for (int j = 0; j < S_::QV; ++j) {
+      u32x4 x = {0u, 0u, 0u, 0u};
+      if (pos[mt] >= 0) x = *reinterpret_cast<const u32x4*>(src + j * (64 / (int)sizeof(T)));
+      q[mt][j] = x;
+    }
+  }
+
+  // ---- the block-table entries of this split's keys: the head run's pages, then the window run's
+  const int bs_mask = (1 << a.bs_log2) - 1;
+  const int32_t* bt = a.block_tables + (int64_t)b * a.max_blocks;
+  const int headn = min(v1, sp.head);                      // end of the head run
+  const int pg_a = v0 >> a.bs_log2;
+  const int na = headn > v0 ? ((headn - 1) >> a.bs_log2) - pg_a + 1 : 0;
+  const int win0 = max(v0, sp.head) + sp.gap, win1 = v1 + sp.gap;  // the window run's keys
+  const int pg_b = win0 >> a.bs_log2;
+  const int nb = v1 > sp.head && win1 > win0 ? ((win1 - 1) >> a.bs_log2) - pg_b + 1 : 0;
+  if (tid == 0) {
+    lds.holes = 0;
+    lds.mapped = 0x7fffffff;
+  }
+  __syncthreads();
+  for (int i = tid; i < na + nb; i += NT) {
+    const int p = bt[i < na ? pg_a + i : pg_b + i - na];
+    if (i < kMaxPages) lds.pages[i] = p;
+    if (p < 0) lds.holes = 1;
+  }
+  // (the query rows are waited for here, not behind the tiles loading ahead)
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int j = 0; j < S_::QV; ++j) __asm__ volatile("" ::"v"(q[mt][j]));
+  __syncthreads();
+  auto page = [&](int key, bool head) {
+    const int i = head ? (key >> a.bs_log2) - pg_a : (key >> a.bs_log2) - pg_b + na;
+    return i < kMaxPages ? lds.pages[i] : bt[key >> a.bs_log2];
+  };
+  const bool holes = uniform(lds.holes) != 0;
+  int n_keys = v1 - v0;
+  int spare = 0;  // the cache row that an unmapped key reads: one of a key that the split has
+  if (holes) {    // uniform
+    for (int i = tid; i < na + nb; i += NT)
+      if (bt[i < na ? pg_a + i : pg_b + i - na] >= 0) atomicMin(&lds.mapped, i);
+    __syncthreads();
+    const int i = uniform(lds.mapped);
+    if (i >= na + nb) {
+      n_keys = 0;  // no key at all
+    } else {
+      const int key = i < na ? max((pg_a + i) << a.bs_log2, v0) : max((pg_b + i - na) << a.bs_log2, win0);
+      spare = (bt[key >> a.bs_log2] << a.bs_log2) + (key & bs_mask);
+    }
+  }
+
+  // ---- K/V rows straight to LDS: instruction j fills rows j RPI .., the lane
+  // picking the chunk that its slot holds; rows past the last key read it again
+  const uint32_t row_bytes = (uint32_t)a.Hkv * ROWB;
+  const char* kbase = (const char*)a.k + (int64_t)hk * ROWB;
+  const char* vbase = (const char*)a.v + (int64_t)hk * ROWB;
+  unsigned char* mine = lds.tiles[w];
+  auto load_lds = [&](const char* src, unsigned char* dst) {
+    const uint32_t at = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)dst);
+    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(src) : "memory", "m0");
+  };
+  const int ntiles = (n_keys + TK - 1) / TK;
+  auto ktile = [&](int buf) { return mine + buf * (V ? 2 : 1) * S_::TILEB; };
+  auto vtile = [&](int buf) { return mine + (buf * 2 + 1) * S_::TILEB; };
+  auto issue = [&](int buf, int tile) {
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+      const int r = j * RPI + lane / CPR, slot = lane % CPR;
+      const int v = min(v0 + tile * TK + r, v1 - 1);
+      const int key = sp.key(v);
+      const int p = page(key, v < sp.head);
+      const uint32_t row = p >= 0 ? (uint32_t)((p << a.bs_log2) + (key & bs_mask)) : (uint32_t)spare;
+      const uint64_t off = (uint64_t)row * row_bytes;
+      load_lds(kbase + off + ((slot ^ S_::kswz(r)) << 4), ktile(buf) + j * 1024);
+      if constexpr (V) load_lds(vbase + off + ((slot ^ S_::vswz(r)) << 4), vtile(buf) + j * 1024);
+    }
+  };
+  auto landed = [&](bool ahead) {
+    constexpr int N = J * (V ? 2 : 1);
+    if (ahead) __asm__ volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    else __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  };
+
+  // ---- running state
+  constexpr int NACC = V ? DT : 1;
+  f32x4 acc[MT][NACC];
+  float m_run[MT], l_run[MT];
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    m_run[mt] = kNegInf;
+    l_run[mt] = 0.f;
+#pragma unroll
+    for (int d = 0; d < NACC; ++d) acc[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  float row_m[MT], row_inv[MT];  // kWeights: the rows' final statistics
+  if constexpr (MODE == kWeights) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      const int m = mt * 16 + c;
+      float M = kNegInf, L = 0.f;
+      if (pos[mt] >= 0) {
+        const float2* ml = a.part_ml + (int64_t)(pair * a.subsets + sub) * a.S * a.R + m;
+        for (int s = 0; s < a.S; ++s) M = fmaxf(M, ml[(int64_t)s * a.R].x);
+        if (M > kNegInf)
+          for (int s = 0; s < a.S; ++s) {
+            const float2 x = ml[(int64_t)s * a.R];
+            L += x.y * __builtin_amdgcn_exp2f(x.x - M);
+          }
+      }
+      row_m[mt] = M == kNegInf ? 0.f : M;
+      row_inv[mt] = L > 0.f ? 1.f / L : 0.f;
+      __asm__ volatile("" ::"v"(row_m[mt]), "v"(row_inv[mt]));
+    }
+  }
+
+  // scores of a tile: element i of s[mt][u] is key 16 u + 4 g + i, row c
+  f32x4 s[MT][KT];
+  auto scores = [&](const unsigned char* kt) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int u = 0; u < KT; ++u) s[mt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int u = 0; u < KT; ++u) {
+      const int r = u * 16 + c;
+      u32x4 ka[S_::QV];
+#pragma unroll
+      for (int j = 0; j < S_::QV; ++j)
+        ka[j] = *reinterpret_cast<const u32x4*>(kt + r * ROWB + (((j * 4 + g) ^ S_::kswz(r)) << 4));
+#pragma unroll
+      for (int j = 0; j < S_::QV; ++j)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          if constexpr (BF16) {
+            s[mt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(ka[j]), as_bf16x8(q[mt][j]), s[mt][u], 0, 0, 0);
+          } else {
+            const f32x4 kf = __builtin_bit_cast(f32x4, ka[j]), qf = __builtin_bit_cast(f32x4, q[mt][j]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[mt][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], s[mt][u], 0, 0, 0);
+          }
+        }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int u = 0; u < KT; ++u) s[mt][u] *= a.scale_log2;
+  };
+  auto mask = [&](int tile) {
+    const int vt = v0 + tile * TK;
+    const int k_first = sp.key(vt), k_last = sp.key(min(vt + TK, v1) - 1);
+    // uniform: every key exists and every row sees it
+    const bool all = vt + TK <= v1 && k_last <= sp.pos_min &&
+                     (a.window == 0 || k_last < a.sinks || k_first > sp.pos_max - a.window);
+    if (!all) {
+#pragma unroll
+      for (int u = 0; u < KT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int v = vt + u * 16 + g * 4 + i;
+          const int key = sp.key(v);
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const bool on = v < v1 && key <= pos[mt] && (a.window == 0 || key > pos[mt] - a.window || key < a.sinks);
+            s[mt][u][i] = on ? s[mt][u][i] : kNegInf;
+          }
+        }
+    }
+    if (holes) {  // uniform
+      const int v = min(vt + (lane & (TK - 1)), v1 - 1);
+      const uint64_t mapped = __ballot(page(sp.key(v), v < sp.head) >= 0);
+#pragma unroll
+      for (int u = 0; u < KT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            s[mt][u][i] = (mapped >> (u * 16 + g * 4 + i)) & 1 ? s[mt][u][i] : kNegInf;
+    }
+  };
+  auto attend = [&](const unsigned char* vt) {
+    u32x4 pB[MT];  // bf16: the weights as the B operand (elements 0..3 keys 4 g + i, 4..7 keys 16 + 4 g + i)
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float mx = kNegInf;
+#pragma unroll
+      for (int u = 0; u < KT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[mt][u][i]);
+      const float m_new = fmaxf(m_run[mt], groups_max(mx));
+      const float ref = m_new == kNegInf ? 0.f : m_new;
+      const float alpha = __builtin_amdgcn_exp2f(m_run[mt] - ref);  // (from -inf: 0)
+      m_run[mt] = m_new;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < KT; ++u)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[mt][u][i] = __builtin_amdgcn_exp2f(s[mt][u][i] - ref);
+          sum += s[mt][u][i];
+        }
+      l_run[mt] = fmaf(l_run[mt], alpha, sum);
+      if (__ballot(alpha != 1.f)) {
+#pragma unroll
+        for (int d = 0; d < NACC; ++d) acc[mt][d] *= alpha;
+      }
+      if constexpr (BF16) {
+        pB[mt] = u32x4{pack_bf16x2(s[mt][0][0], s[mt][0][1]), pack_bf16x2(s[mt][0][2], s[mt][0][3]),
+                       pack_bf16x2(s[mt][KT - 1][0], s[mt][KT - 1][1]), pack_bf16x2(s[mt][KT - 1][2], s[mt][KT - 1][3])};
+      }
+    }
+    if constexpr (BF16) {
+      // V^T: 16-lane group g reads rows 4 g .. (and 16 + 4 g ..), dims 16 dt .. + 15
+      const int r = g * 4 + (c >> 2);
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        const unsigned char* src = vt + r * ROWB + (((dt * 2 + ((c & 3) >> 1)) ^ S_::vswz(r)) << 4) + (c & 1) * 8;
+        const uint2 lo = lds_read_tr(src), hi = lds_read_tr(src + 16 * ROWB);  // (vswz(r + 16) == vswz(r))
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y}),
+                                                                as_bf16x8(pB[mt]), acc[mt][dt], 0, 0, 0);
+      }
+    } else {
+      // step i takes keys 4 g + i: V[key][64 h + 4 c + e] feeds tile (h, e), whose row c is dim 64 h + 4 c + e
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < DH / 64; ++h) {
+          const f32x4 x = *reinterpret_cast<const f32x4*>(vt + (g * 4 + i) * ROWB + (h * 16 + c) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+              acc[mt][h * 4 + e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], s[mt][0][i], acc[mt][h * 4 + e], 0, 0, 0);
+        }
+    }
+  };
+
+  if (w < ntiles) {
+    issue(0, w);
+    if (w + kWaves < ntiles) issue(1, w + kWaves);
+    int buf = 0;
+    for (int t = w; t < ntiles; t += kWaves) {
+      landed(t + kWaves < ntiles);
+      scores(ktile(buf));
+      mask(t);
+      if constexpr (MODE == kAttendScores) {
+        const int vt = v0 + t * TK;
+#pragma unroll
+        for (int u = 0; u < KT; ++u)
+          if (c < a.R) {
+            float* dst = a.scores + ((int64_t)pair * a.R + c) * a.score_keys + vt + u * 16 + g * 4;
+            *reinterpret_cast<f32x4*>(dst) = s[0][u];  // (score_keys is a whole number of tiles; v0 too)
+          }
+      }
+      if constexpr (V) {
+        attend(vtile(buf));
+      } else {
+        // weights of 16 u + 4 g + i summed over the rows: a register sum over the
+        // row tiles, then over the group's 16 lanes
+        float x[KT * 4];
+#pragma unroll
+        for (int u = 0; u < KT; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float y = 0.f;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+              y = pos[mt] >= 0 ? fmaf(__builtin_amdgcn_exp2f(s[mt][u][i] - row_m[mt]), row_inv[mt], y) : y;
+            y += dpp_f32<kDppXor1>(y);
+            y += dpp_f32<kDppXor2>(y);
+            y += dpp_f32<kDppHalfMirror>(y);
+            x[u * 4 + i] = y + dpp_f32<kDppMirror>(y);
+          }
+        float y = x[0];
+#pragma unroll
+        for (int e = 1; e < KT * 4; ++e) y = c == e ? x[e] : y;
+        const int v = v0 + t * TK + (c >> 2) * 16 + g * 4 + (c & 3);
+        if (c < KT * 4 && v < v1) {
+          const int p = page(v, true);
+          if (p >= 0) {
+            float* dst = a.key_weights + ((int64_t)p * a.Hkv + hk) * (bs_mask + 1) + (v & bs_mask);
+            if (v >= sp.pos_min && sub == 0) *dst = y;
+            else unsafeAtomicAdd(dst, y);
+          }
+        }
+      }
+      if (t + 2 * kWaves < ntiles) {
+        __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its buffer may be filled again
+        issue(buf, t + 2 * kWaves);
+      }
+      buf ^= 1;
+    }
+  }
+  if constexpr (!V) return;
+
+  // ---- the waves' rows combined through LDS
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    l_run[mt] = groups_sum(l_run[mt]);
+    if (pos[mt] < 0) {  // padding: no key, whatever an unmasked tile gave it
+      m_run[mt] = kNegInf;
+      l_run[mt] = 0.f;
+    }
+    if (g == 0) lds.ml[w][mt * 16 + c] = make_float2(m_run[mt], l_run[mt]);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+    const int m = mt * 16 + c;
+    float M = kNegInf, L = 0.f;
+#pragma unroll
+    for (int ww = 0; ww < kWaves; ++ww) M = fmaxf(M, lds.ml[ww][m].x);
+    const float ref = M == kNegInf ? 0.f : M;
+#pragma unroll
+    for (int ww = 0; ww < kWaves; ++ww) L += lds.ml[ww][m].y * __builtin_amdgcn_exp2f(lds.ml[ww][m].x - ref);
+    const float f = __builtin_amdgcn_exp2f(m_run[mt] - ref);
+    if (w == 0 && g == 0) lds.row[m] = make_float2(M, L);
+    // (row m of a wave's O as DH floats; its 16-byte pieces rotated by the row, for the banks)
+    float* dst = reinterpret_cast<float*>(mine) + m * DH;
+#pragma unroll
+    for (int d = 0; d < DT; ++d) {
+      f32x4 x;
+      int ch;
+      if constexpr (BF16) {
+        x = acc[mt][d];
+        ch = d * 4 + g;  // dims 16 d + 4 g ..
+      } else {
+        const int h = d >> 2, i = d & 3;  // dims 64 h + 16 g + 4 i ..
+        x = f32x4{acc[mt][h * 4][i], acc[mt][h * 4 + 1][i], acc[mt][h * 4 + 2][i], acc[mt][h * 4 + 3][i]};
+        ch = h * 16 + g * 4 + i;
+      }
+      *reinterpret_cast<f32x4*>(dst + ((ch + m) & (DH / 4 - 1)) * 4) = f > 0.f ? x * f : f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  __syncthreads();
+  for (int idx = tid; idx < a.R * (DH / 4); idx += NT) {
+    const int m = idx / (DH / 4), ch = idx % (DH / 4);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ww = 0; ww < kWaves; ++ww)
+      o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds.tiles[ww]) + m * DH + ((ch + m) & (DH / 4 - 1)) * 4);
+    const float2 ml = lds.row[m];
+    if (ch == 0) a.part_ml[part + m] = ml;
+    if (a.S > 1) {
+      *reinterpret_cast<f32x4*>(a.part_o + (part + m) * DH + ch * 4) = o;
+      continue;
+    }
+    const int gh = m / a.QL, t = m - gh * a.QL;
+    if (t >= qlen) continue;
+    o = ml.y > 0.f ? o * (1.f / ml.y) : f32x4{0.f, 0.f, 0.f, 0.f};
+    T* dst = (T*)a.out + ((int64_t)(q0 + t) * a.H + head0 + gh) * DH + ch * 4;
+    if constexpr (BF16) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    else *reinterpret_cast<f32x4*>(dst) = o;
+  }
+}
+
+// ---------------------------------------------------------------------------
+// The splits joined: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, in
+// split order; one workgroup per 256 / (D / 4) rows of a (pair, head subset).
+// A split without a key of the row (maximum -inf) holds no output.
+// ---------------------------------------------------------------------------
+template <typename T, int DH>
+__global__ __launch_bounds__(256) void row_merge_kernel(RowArgs a) {
+  constexpr int C4 = DH / 4;
+  const int ps = blockIdx.x;  // pair * subsets + sub
+  const int m = blockIdx.y * (256 / C4) + threadIdx.x / C4, ch = threadIdx.x % C4;
+  const int pair = ps / a.subsets, sub = ps - pair * a.subsets;
+  const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
+  if (m >= a.R) return;
+  const int q0 = a.cu_seqlens_q[b], qlen = a.cu_seqlens_q[b + 1] - q0;
+  const int gh = m / a.QL, t = m - gh * a.QL;
+  if (t >= qlen) return;
+  const int64_t base = (int64_t)ps * a.S * a.R + m;
+  constexpr int CH = 4;  // splits per round trip
+  float M = kNegInf, den = 0.f;
+  f32x4 num = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = 0; s0 < a.S; s0 += CH) {
+    float2 ml[CH];
+    f32x4 o[CH];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int64_t r = base + (int64_t)min(s0 + k, a.S - 1) * a.R;
+      ml[k] = a.part_ml[r];
+      o[k] = *reinterpret_cast<const f32x4*>(a.part_o + r * DH + ch * 4);
+    }
+    float Mn = M;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) Mn = fmaxf(Mn, ml[k].x);
+    if (Mn == kNegInf) continue;
+    const float w0 = __builtin_amdgcn_exp2f(M - Mn);
+    den *= w0;
+    num *= w0;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const bool on = s0 + k < a.S && ml[k].x > kNegInf;
+      const float wk = on ? __builtin_amdgcn_exp2f(ml[k].x - Mn) : 0.f;
+      den += on ? ml[k].y * wk : 0.f;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) num[e] = on ? fmaf(o[k][e], wk, num[e]) : num[e];
+    }
+    M = Mn;
+  }
+  num = den > 0.f ? num * (1.f / den) : f32x4{0.f, 0.f, 0.f, 0.f};
+  T* dst = (T*)a.out + ((int64_t)(q0 + t) * a.H + hk * (a.G * a.subsets) + sub * a.G + gh) * DH + ch * 4;
+  if constexpr (sizeof(T) == 2)
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(num[0], num[1]), pack_bf16x2(num[2], num[3]));
+  else *reinterpret_cast<f32x4*>(dst) = num;
+}
+
+// ---------------------------------------------------------------------------
+// Key weights from stored scores: one thread per key of a pair, the rows'
+// statistics in LDS.  A weight of a key at or behind the sequence's first row
+// is set, an older one's added to (one thread adds to a place; an atomic add,
+// so that sequences which share a page lose nothing).
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void row_weights_kernel(RowArgs a) {
+  __shared__ float2 stat[16];  // maximum and 1 / sum
+  const int pair = blockIdx.x, b = pair / a.Hkv, hk = pair - b * a.Hkv;
+  const int q0 = uniform(a.cu_seqlens_q[b]);
+  const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
+  int my_pos;
+  const Span sp = make_span(a, b, q0, qlen, my_pos);
+  const int key = blockIdx.y * 256 + threadIdx.x;
+  if ((int)blockIdx.y * 256 >= sp.total) return;  // uniform
+  if (threadIdx.x < a.R) {
+    const float2* ml = a.part_ml + (int64_t)pair * a.S * a.R + threadIdx.x;
+    float M = kNegInf, L = 0.f;
+    for (int s = 0; s < a.S; ++s) M = fmaxf(M, ml[(int64_t)s * a.R].x);
+    if (M > kNegInf)
+      for (int s = 0; s < a.S; ++s) {
+        const float2 x = ml[(int64_t)s * a.R];
+        L += x.y * __builtin_amdgcn_exp2f(x.x - M);
+      }
+    stat[threadIdx.x] = make_float2(M == kNegInf ? 0.f : M, L > 0.f ? 1.f / L : 0.f);
+  }
+  __syncthreads();
+  if (key >= sp.total) return;
+  const int p = a.block_tables[(int64_t)b * a.max_blocks + (key >> a.bs_log2)];
+  if (p < 0) return;
+  const float* src = a.scores + (int64_t)pair * a.R * a.score_keys + key;
+  float y = 0.f;
+  for (int m = 0; m < a.R; ++m) {
+    const float inv = stat[m].y;  // 0: a row that sees nothing
+    const float s = src[(int64_t)m * a.score_keys];
+    y = inv > 0.f ? fmaf(__builtin_amdgcn_exp2f(s - stat[m].x), inv, y) : y;
+  }
+  float* dst = a.key_weights + (((int64_t)p * a.Hkv + hk) << a.bs_log2) + (key & ((1 << a.bs_log2) - 1));
+  if (key >= sp.pos_min) *dst = y;
+  else unsafeAtomicAdd(dst, y);
+}
+
+// ---------------------------------------------------------------------------
+// Host
+// ---------------------------------------------------------------------------
+struct RowPlan {
+  int G, subsets, R, MT, S;
+  bool stored;     // key weights: from stored scores, else from the keys again
+  int score_keys;
+  size_t ml_bytes, o_bytes, score_bytes;
+};
+
+size_t align256(size_t x) { return (x + 255) & ~(size_t)255; }
+
+int make_row_plan(int B, int H, int Hkv, int D, int block_size, int max_blocks, int max_q_len, int dtype, int window,
+                  int sinks, bool weights, RowPlan* p) {
+  if (B < 0 || H <= 0 || Hkv <= 0 || max_blocks <= 0 || max_q_len <= 0 || window < 0 || sinks < 0) return NSV_ERR_ARG;
+  if (dtype != NSV_F32 && dtype != NSV_BF16) return NSV_ERR_ARG;
+  if (H % Hkv || (D != 64 && D != 128) || max_q_len > 64) return NSV_ERR_UNSUPPORTED;
+  if (block_size <= 0 || (block_size & (block_size - 1))) return NSV_ERR_UNSUPPORTED;
+  const int64_t cap = (int64_t)max_blocks * block_size;
+  if (cap > (int64_t)1 << 30) return NSV_ERR_UNSUPPORTED;
+  const int group = H / Hkv;
+  p->G = group;
+  while (p->G * max_q_len > 64) {
+    int g = p->G - 1;
+    while (group % g) --g;
+    p->G = g;
+  }
+  p->subsets = group / p->G;
+  p->R = p->G * max_q_len;
+  p->MT = (p->R + 15) / 16;
+  const int64_t pairs = (int64_t)B * Hkv;
+  // the most keys that some row of a sequence of consecutive rows sees
+  int64_t keys = cap;
+  if (window > 0) keys = std::min<int64_t>(cap, (int64_t)window + sinks + max_q_len - 1);
+  const int tile = dtype == NSV_BF16 ? 32 : 16;
+  int64_t S = pairs > 0 ? (512 + pairs * p->subsets - 1) / (pairs * p->subsets) : 1;
+  S = std::min<int64_t>({S, (keys + tile * kWaves - 1) / (tile * kWaves), (int64_t)kMaxSplits});
+  p->S = (int)std::max<int64_t>(1, S);
+  p->score_keys = (int)((cap + 31) / 32 * 32);
+  p->score_bytes = weights ? (size_t)pairs * p->R * p->score_keys * sizeof(float) : 0;
+  p->stored = weights && p->MT == 1 && p->subsets == 1 && p->score_bytes <= ((size_t)256 << 20);
+  if (!p->stored) p->score_bytes = 0;
+  const size_t rows = (size_t)pairs * p->subsets * p->S * p->R;
+  p->ml_bytes = align256(rows * sizeof(float2));
+  p->o_bytes = p->S > 1 ? align256(rows * (size_t)D * sizeof(float)) : 0;
+  if (pairs * p->subsets * p->S > 0x7fffffff) return NSV_ERR_UNSUPPORTED;
+  return NSV_OK;
+}
+
+template <typename T, int DH, int MODE>
+void launch_rows(const RowArgs& a, int MT, dim3 grid, hipStream_t s) {
+  const dim3 block(kWaves * 64);
+  if constexpr (MODE == kAttendScores) {
+    hipLaunchKernelGGL((row_attention_kernel<T, 1, DH, MODE>), grid, block, 0, s, a);
+  } else {
+    switch (MT) {
+      case 1: hipLaunchKernelGGL((row_attention_kernel<T, 1, DH, MODE>), grid, block, 0, s, a); break;
+      case 2: hipLaunchKernelGGL((row_attention_kernel<T, 2, DH, MODE>), grid, block, 0, s, a); break;
+      case 3: hipLaunchKernelGGL((row_attention_kernel<T, 3, DH, MODE>), grid, block, 0, s, a); break;
+      default: hipLaunchKernelGGL((row_attention_kernel<T, 4, DH, MODE>), grid, block, 0, s, a); break;
+    }
+  }
+}
+
+template <typename T, int DH>
+int launch_call(RowArgs& a, const RowPlan& p, hipStream_t s) {
+  const dim3 grid((unsigned)(a.npairs * p.subsets * p.S));
+  if (p.stored) launch_rows<T, DH, kAttendScores>(a, p.MT, grid, s);
+  else launch_rows<T, DH, kAttend>(a, p.MT, grid, s);
+  int rc = nsv_launch_status();
+  if (rc != NSV_OK) return rc;
+  if (p.S > 1) {
+    constexpr int rows = 256 / (DH / 4);
+    hipLaunchKernelGGL((row_merge_kernel<T, DH>), dim3(a.npairs * p.subsets, (p.R + rows - 1) / rows), dim3(256), 0, s, a);
+    rc = nsv_launch_status();
+    if (rc != NSV_OK) return rc;
+  }
+  if (!a.key_weights) return NSV_OK;
+  if (p.stored) {
+    hipLaunchKernelGGL(row_weights_kernel, dim3(a.npairs, (p.score_keys + 255) / 256), dim3(256), 0, s, a);
+    return nsv_launch_status();
+  }
+  for (a.first_subset = 0; a.first_subset < p.subsets; ++a.first_subset) {
+    launch_rows<T, DH, kWeights>(a, p.MT, dim3((unsigned)(a.npairs * p.S)), s);
+    rc = nsv_launch_status();
+    if (rc != NSV_OK) return rc;
+  }
+  return NSV_OK;
+}
+
+int row_attention(void* out, const void* q, const void* k_cache, const void* v_cache, float* key_weights,
+                  const int32_t* block_tables, const int64_t* context_lens, const int32_t* cu_seqlens_q,
+                  const int64_t* positions, float scale, int B, int T, int H, int Hkv, int D, int block_size,
+                  int max_blocks, int max_q_len, int dtype, int window, int sinks, bool weights, void* workspace,
+                  size_t workspace_bytes, void* stream) {
+  if (T < 0) return NSV_ERR_ARG;
+  RowPlan p;
+  const int rc = make_row_plan(B, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, window, sinks, weights, &p);
+  if (rc != NSV_OK) return rc;
+  if (B == 0 || T == 0) return NSV_OK;
+  if (!out || !q || !k_cache || !v_cache || !block_tables || !context_lens || !cu_seqlens_q || !positions ||
+      (weights && !key_weights))
+    return NSV_ERR_ARG;
+  if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16) return NSV_ERR_ARG;
+  if (!workspace || workspace_bytes < p.ml_bytes + p.o_bytes + p.score_bytes) return NSV_ERR_WORKSPACE;
+  RowArgs a;
+  a.q = q;
+  a.k = k_cache;
+  a.v = v_cache;
+  a.out = out;
+  a.block_tables = block_tables;
+  a.context_lens = context_lens;
+  a.cu_seqlens_q = cu_seqlens_q;
+  a.positions = positions;
+  a.part_ml = (float2*)workspace;
+  a.part_o = (float*)((char*)workspace + p.ml_bytes);
+  a.scores = (float*)((char*)workspace + p.ml_bytes + p.o_bytes);
+  a.key_weights = weights ? key_weights : nullptr;
+  a.scale_log2 = scale * 1.44269504088896340736f;
+  a.H = H;
+  a.Hkv = Hkv;
+  a.G = p.G;
+  a.subsets = p.subsets;
+  a.bs_log2 = __builtin_ctz((unsigned)block_size);
+  a.max_blocks = max_blocks;
+  a.QL = max_q_len;
+  a.R = p.R;
+  a.S = p.S;
+  a.npairs = B * Hkv;
+  a.window = window;
+  a.sinks = sinks;
+  a.score_keys = p.score_keys;
+  a.first_subset = 0;
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == NSV_BF16) return D == 128 ? launch_call<bf16_t, 128>(a, p, s) : launch_call<bf16_t, 64>(a, p, s);
+  return D == 128 ? launch_call<float, 128>(a, p, s) : launch_call<float, 64>(a, p, s);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t nsv_window_attention_workspace_size(int B, int H, int Hkv, int D, int block_size, int max_blocks, int max_q_len,
+                                           int dtype, int window, int sinks) {
+  RowPlan p;
+  if (window <= 0 || make_row_plan(B, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, window, sinks, false, &p) != NSV_OK)
+    return 0;
+  return p.ml_bytes + p.o_bytes;
+}
+
+int nsv_window_attention(void* out, const void* q, const void* k_cache, const void* v_cache,
+                         const int32_t* block_tables, const int64_t* context_lens, const int32_t* cu_seqlens_q,
+                         const int64_t* positions, float scale, int B, int T, int H, int Hkv, int D, int block_size,
+                         int max_blocks, int max_q_len, int dtype, int window, int sinks, void* workspace,
+                         size_t workspace_bytes, void* stream) {
+  if (window <= 0) return NSV_ERR_ARG;
+  return row_attention(out, q, k_cache, v_cache, nullptr, block_tables, context_lens, cu_seqlens_q, positions, scale, B,
+                       T, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, window, sinks, false, workspace,
+                       workspace_bytes, stream);
+}
+
+size_t nsv_weights_attention_workspace_size(int B, int H, int Hkv, int D, int block_size, int max_blocks, int max_q_len,
+                                            int dtype) {
+  RowPlan p;
+  if (make_row_plan(B, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, 0, 0, true, &p) != NSV_OK) return 0;
+  return p.ml_bytes + p.o_bytes + p.score_bytes;
+}
+
+int nsv_weights_attention(void* out, const void* q, const void* k_cache, const void* v_cache, float* key_weights,
+                          const int32_t* block_tables, const int64_t* context_lens, const int32_t* cu_seqlens_q,
+                          const int64_t* positions, float scale, int B, int T, int H, int Hkv, int D, int block_size,
+                          int max_blocks, int max_q_len, int dtype, void* workspace, size_t workspace_bytes,
+                          void* stream) {
+  return row_attention(out, q, k_cache, v_cache, key_weights, block_tables, context_lens, cu_seqlens_q, positions, scale,
+                       B, T, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, 0, 0, true, workspace, workspace_bytes,
+                       stream);
+}
+
+}  // extern "C"

@@ -10,6 +10,7 @@ PyTorch fallback.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 import torch.nn as nn
@@ -161,6 +162,171 @@ def paged_attention_verify(
         max_num_blocks, qlen_bound, code, kv_split_tokens,
         _lib.ptr(ws), ws_bytes, stream)
     _lib.check(rc, "paged_attention_verify")
+    return out
+
+
+def _check_few_rows(query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads: int,
+                    num_kv_heads: int, head_dim: int, block_size: int, out, what: str) -> tuple:
+    """The checks of the few-row operators over a paged cache; returns the
+    index tensors in the kernels' types and the output."""
+    if not query.is_cuda:
+        raise ValueError(f"{what} runs on the GPU; query is on the CPU")
+    if query.dim() != 3 or query.shape[1] != num_heads or query.shape[2] != head_dim:
+        raise ValueError(f"query must be (T, {num_heads}, {head_dim}), got {tuple(query.shape)}")
+    nb, bs, hkv, d = _check_cache(k_cache, "k_cache")
+    if v_cache.shape != k_cache.shape or not v_cache.is_contiguous():
+        raise ValueError("k_cache and v_cache must have the same contiguous shape")
+    if bs != block_size or hkv != num_kv_heads or d != head_dim:
+        raise ValueError("cache shape disagrees with block_size / num_kv_heads / head_dim")
+    if query.dtype != k_cache.dtype or v_cache.dtype != k_cache.dtype:
+        raise ValueError("query and caches must share one dtype")
+    if nb * bs > 0x7fffffff:
+        raise ValueError(f"{what} addresses fewer than 2^31 cached keys, got {nb} pages of {bs}")
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise ValueError("k_cache and v_cache must start on 16 bytes")
+    dev = query.device
+    for name, t in (("k_cache", k_cache), ("v_cache", v_cache), ("block_tables", block_tables),
+                    ("context_lens", context_lens), ("cu_seqlens_q", cu_seqlens_q), ("positions", positions)):
+        if t.device != dev:
+            raise ValueError(f"{name} is on {t.device}, query on {dev}")
+    if block_tables.dim() != 2:
+        raise ValueError(f"block_tables must be (B, max_num_blocks), got {tuple(block_tables.shape)}")
+    B, T = block_tables.shape[0], query.shape[0]
+    if tuple(context_lens.shape) != (B,) or tuple(cu_seqlens_q.shape) != (B + 1,) or tuple(positions.shape) != (T,):
+        raise ValueError(f"context_lens, cu_seqlens_q and positions must have {B}, {B + 1} and {T} entries, got "
+                         f"{tuple(context_lens.shape)}, {tuple(cu_seqlens_q.shape)} and {tuple(positions.shape)}")
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=dev)
+    elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
+        raise ValueError(f"out must be a contiguous {query.dtype} tensor of shape {tuple(query.shape)} on {dev}")
+    return (_aligned(query.contiguous()), _as(block_tables, "block_tables"), _as(context_lens, "context_lens"),
+            _as(cu_seqlens_q, "cu_seqlens_q"), _as(positions, "positions"), out)
+
+
+def _check_key_weights(key_weights: torch.Tensor, k_cache: torch.Tensor) -> None:
+    nb, bs, hkv, _ = k_cache.shape
+    if (tuple(key_weights.shape) != (nb, hkv, bs) or key_weights.dtype != torch.float32
+            or key_weights.device != k_cache.device or not key_weights.is_contiguous()):
+        raise ValueError(f"key_weights must be a contiguous fp32 tensor of shape {(nb, hkv, bs)} on {k_cache.device}, got "
+                         f"{key_weights.dtype} {tuple(key_weights.shape)} on {key_weights.device}")
+
+
+@functools.lru_cache(maxsize=512)
+def _window_workspace_bytes(*shape: int) -> int:
+    return int(_lib.lib().nsv_window_attention_workspace_size(*shape))
+
+
+@functools.lru_cache(maxsize=512)
+def _weights_workspace_bytes(*shape: int) -> int:
+    return int(_lib.lib().nsv_weights_attention_workspace_size(*shape))
+
+
+def _int_arg(value, name: str, least: int) -> int:
+    """A host integer of at least ``least``, capped where it means no bound
+    to the kernels (no table holds 2^30 keys)."""
+    if int(value) != value or value < least:
+        raise ValueError(f"{name} must be an integer of at least {least}, got {value}")
+    return min(int(value), 1 << 30)
+
+
+def paged_attention_window(
+    query: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    positions: torch.Tensor,
+    scale: float,
+    num_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    block_size: int,
+    block_m: int,
+    *,
+    window: int,
+    sinks: int = 0,
+    max_q_len: int | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """paged_attention_verify with a sliding window: the row at position p
+    sees the keys j <= p with j > p - window or j < sinks (a few first tokens
+    that stay visible); bfloat16 and float32, up to 64 rows per sequence.
+
+    Only keys that some row of their sequence sees are read, so the pages
+    between the sinks and the windows may be given to other sequences (their
+    entries any value, -1 included).  A row that sees no key, and a row at
+    position -1, comes back as zeros.  Scratch comes from torch's allocator,
+    so calls on several streams, and captured ones, share nothing.
+    No counterpart in the reference, whose attention sees every key."""
+    window, sinks = _int_arg(window, "window", 1), _int_arg(sinks, "sinks", 0)
+    query, block_tables, context_lens, cu_seqlens_q, positions, out = _check_few_rows(
+        query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads, num_kv_heads, head_dim,
+        block_size, out, "paged_attention_window")
+    B, max_blocks = block_tables.shape
+    shape = (num_heads, num_kv_heads, head_dim, block_size, max_blocks, int(block_m if max_q_len is None else max_q_len),
+             _lib.dtype_code(query.dtype), window, sinks)
+    dev = query.device
+    with _lib.on_device(dev):
+        ws_bytes = _window_workspace_bytes(B, *shape)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        rc = _lib.lib().nsv_window_attention(
+            out.data_ptr(), query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+            context_lens.data_ptr(), cu_seqlens_q.data_ptr(), positions.data_ptr(), scale, B, query.shape[0], *shape,
+            ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+    _lib.check(rc, "paged_attention_window")
+    return out
+
+
+def paged_attention_weights(
+    query: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    key_weights: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    positions: torch.Tensor,
+    scale: float,
+    num_heads: int,
+    num_kv_heads: int,
+    head_dim: int,
+    block_size: int,
+    block_m: int,
+    *,
+    max_q_len: int | None = None,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """paged_attention_verify that also keeps score of the keys:
+    ``key_weights`` (num_blocks, num_kv_heads, block_size) fp32, paged as the
+    cache is, holds for every (key, kv head) the attention weights that the
+    key got, summed over rows and over the query heads of its kv head.
+
+    A call adds its rows' weights to the keys before the position of the
+    sequence's first row; those from there on are new, and their places are
+    set (so nothing has to be cleared when a page is handed out).  Rows at
+    position -1 see nothing and add nothing.  Places of keys past the last
+    row, and of unmapped pages, keep what they hold.  evict_kvcache reads the
+    table; prefill_key_weights adds a prompt's rows.  bfloat16 and float32, up
+    to 64 rows per sequence.  A page that several sequences of a call share
+    gets the sum of theirs, in no fixed order.  Scratch comes from torch's
+    allocator.  No counterpart in the reference."""
+    query, block_tables, context_lens, cu_seqlens_q, positions, out = _check_few_rows(
+        query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads, num_kv_heads, head_dim,
+        block_size, out, "paged_attention_weights")
+    _check_key_weights(key_weights, k_cache)
+    B, max_blocks = block_tables.shape
+    shape = (num_heads, num_kv_heads, head_dim, block_size, max_blocks, int(block_m if max_q_len is None else max_q_len),
+             _lib.dtype_code(query.dtype))
+    dev = query.device
+    with _lib.on_device(dev):
+        ws_bytes = _weights_workspace_bytes(B, *shape)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        rc = _lib.lib().nsv_weights_attention(
+            out.data_ptr(), query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), key_weights.data_ptr(),
+            block_tables.data_ptr(), context_lens.data_ptr(), cu_seqlens_q.data_ptr(), positions.data_ptr(), scale, B,
+            query.shape[0], *shape, ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+    _lib.check(rc, "paged_attention_weights")
     return out
 
 
