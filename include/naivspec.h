@@ -195,6 +195,79 @@ int nsv_prefill_tiles(const int64_t* seqlens_q, const int64_t* seqlens_k,
                       int32_t* out, int64_t capacity, int32_t* counts);
 
 /*
+ * The same two with a sliding window and a few first keys that stay visible
+ * (window > 0, sinks >= 0; window 0: every key up to the row), as
+ * nsv_window_attention's, and with the rows' softmax statistics.  No
+ * reference counterpart.  The list and the kernel take the same window and
+ * sinks; a tile's key range counts the keys that some row of it sees: the
+ * first `sinks`, then those from its first row's window on (all of them, where
+ * the two meet).  K/V of keys that no row of a tile sees are not read.
+ *   stats   NULL, or [rows, H, 2] fp32: with a row's entry (m, l) the weight of
+ *           a key of score s = scale * log2(e) * q.k is 2^(s - m) / l (l 0: the
+ *           row sees no key)
+ */
+int nsv_prefill_window_tiles(const int64_t* seqlens_q,
+                             const int64_t* seqlens_k, int n, int H, int Hkv,
+                             int block_size, int cus, int window, int sinks,
+                             int32_t* out, int64_t capacity, int32_t* counts);
+int nsv_prefill_window_attention(
+    void* out, const void* q, const void* k, const void* v,
+    const int32_t* block_tables, const int32_t* tiles, int ntiles,
+    int tile_rows, const int32_t* merges, int nmerges, float scale, int H,
+    int Hkv, int D, int block_size, int max_blocks, int window, int sinks,
+    float* stats, void* partials, void* stream);
+
+/*
+ * Attention weights of a prefill step's rows (bf16), summed per key into the
+ * paged key_weights of nsv_weights_attention: for each (key, kv head) over
+ * the rows at or behind the key and the kv head's query heads.  Keys of the
+ * step itself (at or behind a sequence's first row) are set, older ones added
+ * to.  No reference counterpart.
+ *   q        [rows, H, D], the sequences' rows back to back
+ *   stats    what nsv_prefill_window_attention (window 0) left for the same q,
+ *            K and scale
+ *   units    [nunits, 8] and sums [nsums, 6] int32, device memory: the list of
+ *            nsv_key_weights_units for the same sequences (at most max_blocks
+ *            * block_size keys each), heads and a device with `cus` compute
+ *            units; written there to `out` (host memory, `capacity` words),
+ *            units first, with counts[0] = nunits and counts[1] = nsums
+ *            (NSV_ERR_WORKSPACE with them set when `capacity` is too small)
+ *   partials [nunits, Hkv, 256] fp32
+ * Supported: D in {64, 128}; H % Hkv == 0; block_size a power of two.
+ */
+int nsv_key_weights_units(const int64_t* seqlens_q, const int64_t* seqlens_k,
+                          int n, int H, int Hkv, int cus, int32_t* out,
+                          int64_t capacity, int32_t* counts);
+int nsv_prefill_key_weights(const void* q, const void* k_cache,
+                            float* key_weights, const float* stats,
+                            const int32_t* block_tables, const int32_t* units,
+                            int nunits, const int32_t* sums, int nsums,
+                            float scale, int H, int Hkv, int D, int block_size,
+                            int max_blocks, void* partials, void* stream);
+
+/*
+ * Eviction from a paged cache by accumulated attention weight.  No reference
+ * counterpart.  Of each (sequence, kv head) with more than `budget` keys, the
+ * first `sinks`, the last `recent` and the rest's heaviest stay (equal
+ * weights: the lower position first; NaN as -inf), budget in all.  Their rows
+ * of k_cache, v_cache [num_blocks, block_size, Hkv, D] and key_weights
+ * [num_blocks, Hkv, block_size] move to places 0 .. budget - 1, in the order of their
+ * positions, of block_tables, or of out_block_tables [B, out_blocks] when it
+ * is not NULL (sequences of up to `budget` keys too, then).
+ *   lens  [B] int64: min(context_lens[b], max_blocks * block_size, budget)
+ *   kept  [B, Hkv, budget] int32: the positions that stay, ascending, then -1
+ * Every page of a context must be mapped, and out_block_tables holds no page
+ * of block_tables at another place.  Supported: rows of a multiple of 64
+ * bytes; block_size a power of two; sinks + recent <= budget.
+ */
+int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights,
+                 const int32_t* block_tables, const int64_t* context_lens,
+                 const int32_t* out_block_tables, int64_t* lens, int32_t* kept,
+                 int B, int Hkv, int D, int block_size, int max_blocks,
+                 int out_blocks, int dtype, int budget, int sinks, int recent,
+                 void* stream);
+
+/*
  * Load-only measurement kernels, no reference counterpart (the ceilings
  * against which bench.py --ceiling reads the verify-attention kernels).
  * nsv_verify_attention_load_floor reads exactly the K/V bytes of a bf16,

@@ -34,6 +34,7 @@
 #include <algorithm>
 #include <array>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 namespace {
@@ -63,9 +64,11 @@ struct PrefillArgs {
   const int32_t* tiles;         // [ntiles][kTileWords]: sequence, first row, rows, first position, first K/V row,
                                 // first key, end key, partial slot (-1: the tile's only part)
   float* part;                  // [slots][H][tile_rows][DH + 2]: unnormalised rows, then (max, sum) pairs
+  float2* stats;                // null, or [rows][H]: a row's exponent reference (log2 domain) and sum
   int tile_rows;
   float scale_log2;
   int H, Hkv, bs_log2, max_blocks;
+  int window, sinks;            // WIN kernels only
   int hw;                       // query heads of a kv head one workgroup serves
   int hgroups;                  // workgroups per (tile, kv head): (H / Hkv) / hw
 };
@@ -87,7 +90,22 @@ __device__ __forceinline__ float half_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-template <int DH, int NW>
+// WIN: a sliding window and a few first keys that stay visible.  The keys that
+// some row of a tile sees, the first ones and the windows' union, are numbered
+// through (tile_span); keys, a record's key range and the rows' positions are
+// in these numbers from there on, in which the row at position p sees key j iff
+// p - window < j <= p or j < min(sinks, p + 1): one shift, and no load or
+// product is spent on the keys between.
+struct TileSpan {
+  int64_t head, gap, total;  // key j is key j of the sequence below head, j + gap from there on
+};
+__host__ __device__ inline TileSpan tile_span(int64_t pos0, int64_t nrows, int64_t window, int64_t sinks) {
+  const int64_t end = pos0 + nrows, first = pos0 - window + 1;
+  if (window <= 0 || first <= sinks) return {0, 0, end};
+  return {sinks, first - sinks, end - (first - sinks)};
+}
+
+template <int DH, int NW, bool WIN>
 __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a) {
   constexpr int NT = NW * 64;
   constexpr int CPR = DH / 8;              // 16-byte chunks per row
@@ -119,7 +137,15 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
   const int rest = blockIdx.x / a.Hkv;
   const int hg = rest % a.hgroups;
   const int32_t* rec = a.tiles + (int64_t)(rest / a.hgroups) * kTileWords;
-  const int seq = rec[0], row0 = rec[1], nrows = rec[2], pos0 = rec[3], kv0 = rec[4];
+  const int seq = rec[0], row0 = rec[1], nrows = rec[2], kv0 = rec[4];
+  int pos0 = rec[3], head_keys = 0, gap = 0;
+  if constexpr (WIN) {
+    const TileSpan span = tile_span(pos0, nrows, a.window, a.sinks);
+    head_keys = (int)span.head;
+    gap = (int)span.gap;
+    pos0 -= gap;
+  }
+  auto real_key = [&](int key) { return WIN && key >= head_keys ? key + gap : key; };
   const int key_begin = rec[5], slot = rec[7];
   const int wph = NW / a.hw;               // waves per head
   const int head = hk * (a.H / a.Hkv) + hg * a.hw + w / wph;
@@ -127,7 +153,10 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
   const bool paged = a.block_tables != nullptr;
   const int bs_mask = (1 << a.bs_log2) - 1;
   int key_end = min(rec[6], pos0 + nrows);  // (keys past the tile's last row are never attended)
-  if (paged) key_end = min(key_end, a.max_blocks << a.bs_log2);  // the table's width
+  if (paged) {  // the table's width
+    const int width = a.max_blocks << a.bs_log2;
+    key_end = min(key_end, WIN ? max(width - gap, min(width, head_keys)) : width);
+  }
   const int64_t tok = (int64_t)a.Hkv * DH; // elements between consecutive keys
 
   // query rows as the B operand of S^T: lane (h, col) holds row col, dims 16 ks + 8 h .. + 7
@@ -145,9 +174,22 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
   // Block-table entries in LDS: entry i from the first page on at slot i mod
   // kMaxPages, the first kMaxPages here, the rest half a ring at a time once
   // the loop has left the half they replace.
+  // (WIN: the pages of the first keys, then those of the window)
   const int pg0 = key_begin >> a.bs_log2;
-  const int npg = ((key_end + bs_mask) >> a.bs_log2) - pg0;
+  int npg = ((key_end + bs_mask) >> a.bs_log2) - pg0;
   const int32_t* bt = paged ? a.block_tables + (int64_t)seq * a.max_blocks + pg0 : nullptr;
+  int head_pgs = 0, win_pg = 0;  // entries of the first keys; the window's first entry, less pg0
+  if constexpr (WIN) {
+    const int head_end = min(key_end, head_keys), win0 = max(key_begin, head_keys);
+    head_pgs = head_end > key_begin ? ((head_end - 1) >> a.bs_log2) - pg0 + 1 : 0;
+    win_pg = ((win0 + gap) >> a.bs_log2) - pg0;
+    npg = head_pgs + (key_end > win0 ? ((key_end + gap - 1) >> a.bs_log2) - pg0 - win_pg + 1 : 0);
+  }
+  auto entry = [&](int i) { return bt[!WIN || i < head_pgs ? i : i - head_pgs + win_pg]; };
+  auto entry_of = [&](int key) {  // of a key of the tile
+    const int i = (real_key(key) >> a.bs_log2) - pg0;
+    return !WIN || key < head_keys ? i : i - win_pg + head_pgs;
+  };
   int staged = kMaxPages;
   if (paged) {
     if (tid == 0) {
@@ -156,34 +198,39 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
     }
     __syncthreads();
     for (int i = tid; i < npg; i += NT) {
-      const int p = bt[i];
+      const int p = entry(i);
       if (i < kMaxPages) lds.pages[i] = p;
       if (p < 0) lds.holes = 1;
     }
     __syncthreads();
   }
-  auto page = [&](int key) { return lds.pages[((key >> a.bs_log2) - pg0) & (kMaxPages - 1)]; };
+  auto page = [&](int key) { return lds.pages[entry_of(key) & (kMaxPages - 1)]; };
   // the ring's next half, at the start of key tile n0's step (by every wave;
   // the waves a step behind still read tile n0 - kKeys, the loads ahead reach
   // 4 tiles, 256 pages at most, past that one: its first use is behind the
   // step's barrier)
   auto turn_pages = [&](int n0) {
     if (!paged || staged >= npg) return;  // uniform
-    const int low = (max(n0 - kKeys, key_begin) >> a.bs_log2) - pg0;
+    const int low = entry_of(max(n0 - kKeys, key_begin));
     if (low < staged - kMaxPages / 2) return;  // uniform
     const int end = min(staged + kMaxPages / 2, npg);
-    for (int i = staged + tid; i < end; i += NT) lds.pages[i & (kMaxPages - 1)] = bt[i];
+    for (int i = staged + tid; i < end; i += NT) lds.pages[i & (kMaxPages - 1)] = entry(i);
     staged += kMaxPages / 2;
   };
   const bool holes = paged && __builtin_amdgcn_readfirstlane(lds.holes) != 0;
   int64_t spare = 0;  // the row an unmapped key reads instead (of a key that exists; its weight is zero)
   if (holes) {        // uniform
     for (int i = tid; i < npg; i += NT)
-      if (bt[i] >= 0) atomicMin(&lds.first, i);
+      if (entry(i) >= 0) atomicMin(&lds.first, i);
     __syncthreads();
     const int first = __builtin_amdgcn_readfirstlane(lds.first);
     if (first >= npg) key_end = key_begin;  // no key at all
-    else spare = (int64_t)bt[first] << a.bs_log2;
+    else spare = (int64_t)entry(first) << a.bs_log2;
+    if constexpr (WIN) {  // (the page's first key may lie before the window: the first that the tile has)
+      const int from = first < head_pgs ? key_begin : max(key_begin, head_keys) + gap;
+      const int pg = pg0 + (first < head_pgs ? first : first - head_pgs + win_pg);
+      spare += max(from - (pg << a.bs_log2), 0);
+    }
   }
 
   // K/V rows of a tile go from memory straight to LDS (no registers, no LDS
@@ -205,10 +252,11 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
       const int r0j = (w * J + j) * RPI;
       const int r = r0j + lane / CPR, sl = lane % CPR;
       const int kc = min(n0 + r, key_end - 1);
-      int64_t row = kv0 + kc;
+      const int real = real_key(kc);
+      int64_t row = kv0 + real;
       if (paged) {
         const int p = page(kc);
-        row = p >= 0 ? ((int64_t)p << a.bs_log2) + (kc & bs_mask) : spare;
+        row = p >= 0 ? ((int64_t)p << a.bs_log2) + (real & bs_mask) : spare;
       }
       const int64_t off = row * tok + hk * DH;
       load_lds(a.k + off + ((sl ^ (r & (CPR - 1))) << 3), &lds.kt[kb][r0j * ROWB]);
@@ -231,9 +279,13 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
   const float sc = a.scale_log2;
 
   f32x16 s[2];
-  // scores of a tile (every key of a skipped tile lies past this wave's rows)
+  // uniform: every key of the tile lies past this wave's rows, or before their windows
+  auto unseen = [&](int n0) {
+    return n0 > pos_last || (WIN && n0 >= a.sinks && n0 + kKeys - 1 <= pos_first - a.window);
+  };
+  // scores of a tile
   auto scores = [&](int kb, int n0) {
-    if (n0 > pos_last) return;  // uniform
+    if (unseen(n0)) return;
     const unsigned char* kt = lds.kt[kb];
     // K operands KH steps at a time, both 32-key halves, the next group's
     // reads in flight while one is multiplied (left to itself the compiler
@@ -265,7 +317,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
     __builtin_amdgcn_sched_barrier(0);
   };
   auto values = [&](int vb, int n0) {  // softmax of the tile's scores, O^T += V^T P^T
-    if (n0 > pos_last) return;  // uniform
+    if (unseen(n0)) return;
     const unsigned char* vt = lds.vt[vb];
     // lane (h, col), element i of tile t: key n0 + 32 t + 8 (i / 4) + 4 h + i % 4, row col
     if (n0 + kKeys - 1 > pos_first) {  // uniform: some key lies past the wave's first row
@@ -275,6 +327,16 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
         for (int i = 0; i < 16; ++i) {
           const int key = t * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
           s[t][i] = key <= pos - n0 ? s[t][i] : kNegInf;
+        }
+    }
+    // uniform: some key lies before the last row's window
+    if (WIN && n0 <= pos_last - a.window && n0 + kKeys > a.sinks) {
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = n0 + t * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
+          s[t][i] = key > pos - a.window || key < a.sinks ? s[t][i] : kNegInf;
         }
     }
     if (holes) {  // uniform
@@ -450,6 +512,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
     return;
   }
   if (r < nrows) {
+    if (a.stats && h == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(m_ref * sc, L);
     bf16_t* dst = a.out + ((int64_t)(row0 + r) * a.H + head) * DH + h * 4;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -467,6 +530,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
 //   out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, in part order.
 struct PrefillMergeArgs {
   bf16_t* out;
+  float2* stats;  // as PrefillArgs'
   const float* part;
   const int32_t* merges;  // [nmerge][4]: first slot, parts, first row, rows
   int H, tile_rows;
@@ -510,6 +574,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillMergeArgs a) 
     M = Mn;
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
+  if (a.stats && c4 == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(M, den);
   bf16_t* dst = a.out + ((int64_t)(row0 + r) * a.H + head) * DH + c4 * 4;
   *reinterpret_cast<uint2*>(dst) =
       make_uint2(pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv));
@@ -542,7 +607,8 @@ struct Tiling {
   int rows, slots;
 };
 
-Tiling make_tiles(const int64_t* ql, const int64_t* kl, int n, int H, int Hkv, int block_size, int cus) {
+Tiling make_tiles(const int64_t* ql, const int64_t* kl, int n, int H, int Hkv, int block_size, int cus, int window,
+                  int sinks) {
   const int hw = (H / Hkv) % 2 == 0 ? 2 : 1;
   auto key_tiles = [](int64_t end) { return (end + kKeys - 1) / kKeys; };
   auto count = [&](int rows, int64_t& tiles, int64_t& keys) {
@@ -550,7 +616,7 @@ Tiling make_tiles(const int64_t* ql, const int64_t* kl, int n, int H, int Hkv, i
     for (int b = 0; b < n; ++b)
       for (int64_t r = 0; r < ql[b]; r += rows) {
         ++tiles;
-        keys += key_tiles(kl[b] - ql[b] + std::min(r + rows, ql[b]));
+        keys += key_tiles(tile_span(kl[b] - ql[b] + r, std::min<int64_t>(rows, ql[b] - r), window, sinks).total);
       }
   };
   Tiling t{{}, {}, 8 * kWaveRows / hw, 0};
@@ -566,7 +632,8 @@ Tiling make_tiles(const int64_t* ql, const int64_t* kl, int n, int H, int Hkv, i
   int64_t q0 = 0, k0 = 0;
   for (int b = 0; b < n; ++b) {
     for (int64_t r = 0; r < ql[b]; r += t.rows) {
-      const int64_t nr = std::min<int64_t>(t.rows, ql[b] - r), pos = kl[b] - ql[b] + r, end = pos + nr, nt = key_tiles(end);
+      const int64_t nr = std::min<int64_t>(t.rows, ql[b] - r), pos = kl[b] - ql[b] + r;
+      const int64_t end = tile_span(pos, nr, window, sinks).total, nt = key_tiles(end);
       int64_t parts = tiles * units <= cus && 2 * nt > 3 * target ? (nt + target - 1) / target : 1;
       const int64_t per = (nt + parts - 1) / parts;
       parts = (nt + per - 1) / per;
@@ -590,7 +657,12 @@ extern "C" {
 
 int nsv_prefill_tiles(const int64_t* seqlens_q, const int64_t* seqlens_k, int n, int H, int Hkv, int block_size,
                       int cus, int32_t* out, int64_t capacity, int32_t* counts) {
-  if (n < 0 || H <= 0 || Hkv <= 0 || H % Hkv || block_size < 0 || cus <= 0 || capacity < 0 || !counts) return NSV_ERR_ARG;
+  return nsv_prefill_window_tiles(seqlens_q, seqlens_k, n, H, Hkv, block_size, cus, 0, 0, out, capacity, counts);
+}
+
+int nsv_prefill_window_tiles(const int64_t* seqlens_q, const int64_t* seqlens_k, int n, int H, int Hkv, int block_size,
+                             int cus, int window, int sinks, int32_t* out, int64_t capacity, int32_t* counts) {
+  if (window < 0 || sinks < 0 || n < 0 || H <= 0 || Hkv <= 0 || H % Hkv || block_size < 0 || cus <= 0 || capacity < 0 || !counts) return NSV_ERR_ARG;
   if (n > 0 && (!seqlens_q || !seqlens_k || !out)) return NSV_ERR_ARG;
   int64_t rows = 0, keys = 0;
   for (int b = 0; b < n; ++b) {
@@ -600,7 +672,7 @@ int nsv_prefill_tiles(const int64_t* seqlens_q, const int64_t* seqlens_k, int n,
   }
   if (rows > 0x7fffffff || keys > 0x7fffffff) return NSV_ERR_UNSUPPORTED;
   try {
-    const Tiling t = make_tiles(seqlens_q, seqlens_k, n, H, Hkv, block_size, cus);
+    const Tiling t = make_tiles(seqlens_q, seqlens_k, n, H, Hkv, block_size, cus, window, sinks);
     counts[0] = (int32_t)t.tiles.size();
     counts[1] = (int32_t)t.merges.size();
     counts[2] = t.rows;
@@ -618,6 +690,15 @@ int nsv_prefill_attention(void* out, const void* q, const void* k, const void* v
                           const int32_t* tiles, int ntiles, int tile_rows, const int32_t* merges, int nmerges,
                           float scale, int H, int Hkv, int D, int block_size, int max_blocks, void* partials,
                           void* stream) {
+  return nsv_prefill_window_attention(out, q, k, v, block_tables, tiles, ntiles, tile_rows, merges, nmerges, scale, H, Hkv,
+                                      D, block_size, max_blocks, 0, 0, nullptr, partials, stream);
+}
+
+int nsv_prefill_window_attention(void* out, const void* q, const void* k, const void* v, const int32_t* block_tables,
+                                 const int32_t* tiles, int ntiles, int tile_rows, const int32_t* merges, int nmerges,
+                                 float scale, int H, int Hkv, int D, int block_size, int max_blocks, int window,
+                                 int sinks, float* stats, void* partials, void* stream) {
+  if (window < 0 || window > (1 << 30) || sinks < 0 || sinks > (1 << 30)) return NSV_ERR_ARG;
   if (ntiles < 0 || nmerges < 0 || H <= 0 || Hkv <= 0) return NSV_ERR_ARG;
   if (H % Hkv || (D != 64 && D != 128)) return NSV_ERR_UNSUPPORTED;
   const int G = H / Hkv, hw = G % 2 == 0 ? 2 : 1;
@@ -650,19 +731,28 @@ int nsv_prefill_attention(void* out, const void* q, const void* k, const void* v
   a.hgroups = G / hw;
   a.part = (float*)partials;
   a.tile_rows = tile_rows;
+  a.stats = (float2*)stats;
+  a.window = window;
+  a.sinks = sinks;
   hipStream_t s = (hipStream_t)stream;
   const dim3 g((unsigned)grid), b(nw * 64);
-  if (D == 128) {
-    if (nw == 8) hipLaunchKernelGGL((prefill_attn_kernel<128, 8>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((prefill_attn_kernel<128, 4>), g, b, 0, s, a);
-  } else {
-    if (nw == 8) hipLaunchKernelGGL((prefill_attn_kernel<64, 8>), g, b, 0, s, a);
-    else hipLaunchKernelGGL((prefill_attn_kernel<64, 4>), g, b, 0, s, a);
-  }
+  auto launch = [&](auto win) {
+    constexpr bool WIN = decltype(win)::value;
+    if (D == 128) {
+      if (nw == 8) hipLaunchKernelGGL((prefill_attn_kernel<128, 8, WIN>), g, b, 0, s, a);
+      else hipLaunchKernelGGL((prefill_attn_kernel<128, 4, WIN>), g, b, 0, s, a);
+    } else {
+      if (nw == 8) hipLaunchKernelGGL((prefill_attn_kernel<64, 8, WIN>), g, b, 0, s, a);
+      else hipLaunchKernelGGL((prefill_attn_kernel<64, 4, WIN>), g, b, 0, s, a);
+    }
+  };
+  if (window > 0) launch(std::true_type{});
+  else launch(std::false_type{});
   const int rc = nsv_launch_status();
   if (rc || nmerges == 0) return rc;
   PrefillMergeArgs m;
   m.out = (bf16_t*)out;
+  m.stats = (float2*)stats;
   m.part = (const float*)partials;
   m.merges = merges;
   m.H = H;

@@ -373,24 +373,34 @@ def _prefill_lengths(seqlens_q, seqlens_k) -> tuple[list[int], list[int]]:
     return seqlens_q, seqlens_k
 
 
-def _prefill_work(seqlens_q, seqlens_k, num_heads: int, num_kv_heads: int, block_size: int | None, cus: int,
-                  pinned: bool) -> tuple[torch.Tensor, list[int]]:
-    """nsv_prefill_tiles into a host tensor; returns (its words, [tiles,
-    merges, tile_rows, slots])."""
+def _host_list(build, seqlens_q, seqlens_k, words_of, pinned: bool, what: str) -> tuple[torch.Tensor, list[int]]:
+    """A native work list of the sequences in a host tensor: build(seqlens_q,
+    seqlens_k, n, its address, its words, counts) fills it, and says
+    (words_of(counts)) how many words it has.  Returns (the words, counts)."""
     seqlens_q, seqlens_k = _prefill_lengths(seqlens_q, seqlens_k)
     n = len(seqlens_q)
     q, k, counts = (ctypes.c_int64 * n)(*seqlens_q), (ctypes.c_int64 * n)(*seqlens_k), (ctypes.c_int32 * 4)()
     words = 4096
     while True:
         buf = torch.empty(words, dtype=torch.int32, pin_memory=pinned)
-        rc = _lib.lib().nsv_prefill_tiles(q, k, n, num_heads, num_kv_heads, block_size or 0, cus, buf.data_ptr(),
-                                          words, counts)
-        need = 8 * counts[0] + 4 * counts[1]
+        rc = build(q, k, n, buf.data_ptr(), words, counts)
+        need = words_of(counts)
         if rc == 0 or need <= words:
             break
         words = need
-    _lib.check(rc, "prefill_tiles")
+    _lib.check(rc, what)
     return buf[:need], list(counts)
+
+
+def _prefill_work(seqlens_q, seqlens_k, num_heads: int, num_kv_heads: int, block_size: int | None, cus: int,
+                  window: int, sinks: int, pinned: bool) -> tuple[torch.Tensor, list[int]]:
+    """nsv_prefill_window_tiles into a host tensor; returns (its words,
+    [tiles, merges, tile_rows, slots])."""
+    def build(q, k, n, at, words, counts):
+        return _lib.lib().nsv_prefill_window_tiles(q, k, n, num_heads, num_kv_heads, block_size or 0, cus, window, sinks,
+                                                   at, words, counts)
+
+    return _host_list(build, seqlens_q, seqlens_k, lambda c: 8 * c[0] + 4 * c[1], pinned, "prefill_tiles")
 
 
 def prefill_tiles(seqlens_q, seqlens_k, num_heads: int, num_kv_heads: int, block_size: int | None, cus: int):
@@ -398,7 +408,7 @@ def prefill_tiles(seqlens_q, seqlens_k, num_heads: int, num_kv_heads: int, block
     ending seqlens_k keys each (nsv_prefill_tiles); block_size None: K/V are
     the sequences' keys back to back.  Host only.
     Returns (tiles [n, 8] int32, merges [m, 4] int32, tile_rows, slots)."""
-    work, (nt, nm, rows, slots) = _prefill_work(seqlens_q, seqlens_k, num_heads, num_kv_heads, block_size, cus, False)
+    work, (nt, nm, rows, slots) = _prefill_work(seqlens_q, seqlens_k, num_heads, num_kv_heads, block_size, cus, 0, 0, False)
     return work[:8 * nt].view(nt, 8).numpy(), work[8 * nt:].view(nm, 4).numpy(), rows, slots
 
 
@@ -436,15 +446,36 @@ def _send_ahead() -> bool:
 
 
 class PrefillPlan(_StepList):
-    """The prefill kernel's work list of one step on the device."""
+    """The prefill kernel's work list of one step on the device.  window and
+    sinks: every row sees its last ``window`` keys and its sequence's first
+    ``sinks`` (window 0: all keys up to it)."""
 
-    def __init__(self, seqlens_q, seqlens_k, num_heads: int, num_kv_heads: int, block_size: int | None, device):
+    def __init__(self, seqlens_q, seqlens_k, num_heads: int, num_kv_heads: int, block_size: int | None, device,
+                 window: int = 0, sinks: int = 0):
+        self.window, self.sinks = _int_arg(window, "window", 0), _int_arg(sinks, "sinks", 0)
         cus = torch.cuda.get_device_properties(device).multi_processor_count
         ahead = _send_ahead()
         work, (self.ntiles, self.nmerges, self.tile_rows, self.slots) = _prefill_work(
-            seqlens_q, seqlens_k, num_heads, num_kv_heads, block_size, cus, ahead)
+            seqlens_q, seqlens_k, num_heads, num_kv_heads, block_size, cus, self.window, self.sinks, ahead)
         self.num_heads, self.num_kv_heads, self.block_size = num_heads, num_kv_heads, block_size
         self.sequences, self.rows, self.keys = len(seqlens_q), int(sum(seqlens_q)), int(sum(seqlens_k))
+        self._send(work, device, ahead)
+
+
+class KeyWeightsPlan(_StepList):
+    """The work list of prefill_key_weights of one step on the device."""
+
+    def __init__(self, seqlens_q, seqlens_k, num_heads: int, num_kv_heads: int, block_size: int, device):
+        cus = torch.cuda.get_device_properties(device).multi_processor_count
+        ahead = _send_ahead()
+
+        def build(q, k, n, at, words, counts):
+            return _lib.lib().nsv_key_weights_units(q, k, n, num_heads, num_kv_heads, cus, at, words, counts)
+
+        work, (self.nunits, self.nsums, _, _) = _host_list(build, seqlens_q, seqlens_k, lambda c: 8 * c[0] + 6 * c[1],
+                                                           ahead, "key_weights_units")
+        self.num_heads, self.num_kv_heads, self.block_size = num_heads, num_kv_heads, block_size
+        self.sequences, self.rows, self.longest = len(seqlens_q), int(sum(seqlens_q)), int(max(seqlens_k, default=0))
         self._send(work, device, ahead)
 
 
@@ -504,10 +535,15 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 
 def prefill_attention(query: torch.Tensor, k: torch.Tensor, v: torch.Tensor, plan: PrefillPlan, scale: float,
-                      head_dim: int, block_tables: torch.Tensor | None = None) -> torch.Tensor:
+                      head_dim: int, block_tables: torch.Tensor | None = None, *,
+                      stats: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of a prefill step's rows (bf16): query [rows, H, D];
     k, v the step's own [keys, Hkv, D], or with block_tables the paged caches
-    [num_blocks, block_size, Hkv, D] (layers/attention.py:123-363)."""
+    [num_blocks, block_size, Hkv, D] (layers/attention.py:123-363).  With a
+    window in the plan every row sees that many keys and the first ``sinks``
+    (no reference counterpart), and keys that no row sees are not read.
+    ``stats``: an fp32 [rows, H, 2] that takes the rows' softmax statistics,
+    for prefill_key_weights (not written where the plan has a window)."""
     H, Hkv = plan.num_heads, plan.num_kv_heads
     if not query.is_cuda:
         raise ValueError("prefill_attention runs on the GPU; query is on the CPU")
@@ -533,6 +569,10 @@ def prefill_attention(query: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pla
     query = query.contiguous()
     if (query.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
         query, k, v = _aligned(query), _aligned(k), _aligned(v)
+    if stats is not None:
+        if plan.window:
+            raise ValueError("stats are of attention without a window")
+        _check_stats(stats, plan.rows, H, query.device)
     out = torch.empty_like(query)
     # (the plan's list is the only memory that calls on several streams or
     # threads share, and they only read it)
@@ -541,12 +581,123 @@ def prefill_attention(query: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pla
     part = torch.empty(plan.slots * H * plan.tile_rows * (head_dim + 2), dtype=torch.float32,
                        device=query.device) if plan.slots else None
     tiles = plan.work.data_ptr()
-    rc = _lib.lib().nsv_prefill_attention(
+    rc = _lib.lib().nsv_prefill_window_attention(
         out.data_ptr(), query.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(block_tables), tiles, plan.ntiles,
         plan.tile_rows, tiles + plan.ntiles * 32, plan.nmerges, float(scale), H, Hkv, head_dim,
-        plan.block_size or 1, max_blocks, _lib.ptr(part), stream.cuda_stream)
+        plan.block_size or 1, max_blocks, plan.window, plan.sinks, _lib.ptr(stats), _lib.ptr(part), stream.cuda_stream)
     _lib.check(rc, "prefill_attention")
     return out
+
+
+def _check_stats(stats: torch.Tensor, rows: int, num_heads: int, device) -> None:
+    if (stats.dim() != 3 or stats.shape[0] < rows or tuple(stats.shape[1:]) != (num_heads, 2)
+            or stats.dtype != torch.float32 or stats.device != device or not stats.is_contiguous()):
+        raise ValueError(f"stats must be a contiguous fp32 tensor of (at least {rows}, {num_heads}, 2) on {device}, got "
+                         f"{stats.dtype} {tuple(stats.shape)} on {stats.device}")
+
+
+def prefill_key_weights(query: torch.Tensor, k_cache: torch.Tensor, key_weights: torch.Tensor, plan: KeyWeightsPlan,
+                        stats: torch.Tensor, scale: float, head_dim: int, block_tables: torch.Tensor) -> None:
+    """Adds the attention weights of a prefill step's rows (bf16) to the paged
+    ``key_weights`` (num_blocks, num_kv_heads, block_size) fp32: for every
+    (key, kv head) the weights it gets from the rows at or behind it, summed
+    over them and over the kv head's query heads.  ``query`` and ``scale`` are
+    those of the step's prefill_attention call over the same paged K, which
+    left ``stats``.  The places of the step's own keys are set, those of keys
+    before its first row added to.  A page that several sequences of the step
+    share gets the sum of theirs, in no fixed order.  No counterpart in the
+    reference."""
+    H, Hkv = plan.num_heads, plan.num_kv_heads
+    if not query.is_cuda:
+        raise ValueError("prefill_key_weights runs on the GPU; query is on the CPU")
+    if query.dtype != torch.bfloat16 or k_cache.dtype != torch.bfloat16:
+        raise ValueError("query and k_cache must be bfloat16")
+    if query.dim() != 3 or tuple(query.shape[1:]) != (H, head_dim) or query.shape[0] < plan.rows:
+        raise ValueError(f"query must be (at least {plan.rows}, {H}, {head_dim}), got {tuple(query.shape)}")
+    if _check_cache(k_cache, "k_cache")[1:] != (plan.block_size, Hkv, head_dim):
+        raise ValueError("cache shape disagrees with block_size / num_kv_heads / head_dim")
+    if k_cache.device != query.device or block_tables.device != query.device:
+        raise ValueError(f"query is on {query.device}, k_cache on {k_cache.device}, block_tables on {block_tables.device}")
+    if k_cache.data_ptr() % 16:
+        raise ValueError("k_cache must start on 16 bytes")
+    _check_key_weights(key_weights, k_cache)
+    _check_stats(stats, plan.rows, H, query.device)
+    block_tables = _as(block_tables, "block_tables")
+    if block_tables.dim() != 2 or block_tables.shape[0] < plan.sequences:
+        raise ValueError(f"{plan.sequences} sequences but block tables of {tuple(block_tables.shape)}")
+    if block_tables.shape[1] * plan.block_size < plan.longest:
+        raise ValueError(f"block tables of {block_tables.shape[1]} pages for sequences of up to {plan.longest} keys")
+    query = _aligned(query.contiguous())
+    stream = torch.cuda.current_stream(query.device)
+    with _lib.on_device(query.device):
+        plan.use_on(stream)
+        part = torch.empty(plan.nunits * Hkv * 256, dtype=torch.float32, device=query.device)
+        units = plan.work.data_ptr()
+        rc = _lib.lib().nsv_prefill_key_weights(
+            query.data_ptr(), k_cache.data_ptr(), key_weights.data_ptr(), stats.data_ptr(), block_tables.data_ptr(), units,
+            plan.nunits, units + plan.nunits * 32, plan.nsums, float(scale), H, Hkv, head_dim, plan.block_size,
+            block_tables.shape[1], part.data_ptr(), stream.cuda_stream)
+    _lib.check(rc, "prefill_key_weights")
+
+
+def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch.Tensor, block_tables: torch.Tensor,
+                  context_lens: torch.Tensor, budget: int, *, sinks: int = 0, recent: int = 0,
+                  out_block_tables: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Cuts every sequence's cache to at most ``budget`` keys by the weights
+    that paged_attention_weights and prefill_key_weights left.
+
+    For each (sequence, kv head) with more keys than that, the first ``sinks``
+    and the last ``recent`` stay, and of the rest those with the most weight
+    (of equal ones the lower position; NaN counts as -inf).  Their rows of
+    ``k_cache``, ``v_cache`` (num_blocks, block_size, Hkv, D; bfloat16 or
+    float32) and ``key_weights`` (num_blocks, Hkv, block_size) move, in the
+    order of their positions, to the first places of the sequence's table, or
+    of its row of ``out_block_tables`` (which also gets the sequences that are
+    short enough; their old pages keep what they hold, so it is the form for
+    pages that other sequences share).  Every page of the context must be
+    mapped; pages of out_block_tables must be no other pages of block_tables.
+
+    Returns (lens (B,) int64: min(length, budget); kept (B, Hkv, budget)
+    int32: the positions that stay, ascending, -1 behind the last).  Keys hold
+    their rotary embedding, so later queries keep their true positions for
+    that, and use their places in the cache (lens, lens + 1, ..) as the
+    ``positions`` and context lengths of the attention.  No counterpart in the
+    reference."""
+    if not k_cache.is_cuda:
+        raise ValueError("evict_kvcache runs on the GPU; k_cache is on the CPU")
+    nb, bs, hkv, d = _check_cache(k_cache, "k_cache")
+    if v_cache.shape != k_cache.shape or not v_cache.is_contiguous() or v_cache.dtype != k_cache.dtype:
+        raise ValueError("k_cache and v_cache must have the same contiguous shape and dtype")
+    _check_key_weights(key_weights, k_cache)
+    dev = k_cache.device
+    tables = [block_tables] + ([] if out_block_tables is None else [out_block_tables])
+    if any(t.device != dev for t in (v_cache, context_lens, *tables)):
+        raise ValueError(f"the caches, the block tables and context_lens must be on {dev}")
+    if any(t.dim() != 2 or t.shape[0] != block_tables.shape[0] for t in tables):
+        raise ValueError("block_tables and out_block_tables must be (B, pages)")
+    B, max_blocks = block_tables.shape
+    if tuple(context_lens.shape) != (B,):
+        raise ValueError(f"context_lens must have {B} entries, got {tuple(context_lens.shape)}")
+    budget, sinks, recent = _int_arg(budget, "budget", 1), _int_arg(sinks, "sinks", 0), _int_arg(recent, "recent", 0)
+    if sinks + recent > budget:
+        raise ValueError(f"{sinks} sinks and {recent} recent keys exceed the budget of {budget}")
+    if out_block_tables is not None and out_block_tables.shape[1] * bs < min(budget, max_blocks * bs):
+        raise ValueError(f"out_block_tables of {out_block_tables.shape[1]} pages do not hold {budget} keys")
+    if nb * bs > 0x7fffffff:
+        raise ValueError(f"evict_kvcache addresses fewer than 2^31 cached keys, got {nb} pages of {bs}")
+    block_tables, context_lens = _as(block_tables, "block_tables"), _as(context_lens, "context_lens")
+    if out_block_tables is not None:
+        out_block_tables = _as(out_block_tables, "block_tables")
+    lens = torch.empty(B, dtype=torch.int64, device=dev)
+    kept = torch.empty((B, hkv, budget), dtype=torch.int32, device=dev)
+    with _lib.on_device(dev):
+        rc = _lib.lib().nsv_evict_kv(
+            k_cache.data_ptr(), v_cache.data_ptr(), key_weights.data_ptr(), block_tables.data_ptr(),
+            context_lens.data_ptr(), _lib.ptr(out_block_tables), lens.data_ptr(), kept.data_ptr(), B, hkv, d, bs,
+            max_blocks, 0 if out_block_tables is None else out_block_tables.shape[1], _lib.dtype_code(k_cache.dtype),
+            budget, sinks, recent, _lib.stream_ptr(dev))
+    _lib.check(rc, "evict_kvcache")
+    return lens, kept
 
 
 _prefill_plan: tuple = (None, None)  # (the Context it was built for, its tensors)
