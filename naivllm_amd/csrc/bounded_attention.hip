@@ -212,50 +212,54 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     }
   }
 
-  // ---- the block-table entries of this split's keys: the head run's pages, then the window run's
+  // ---- the block-table entries of a run of this split's keys, c0 .. c1 - 1, in
+  // LDS: the head run's pages, then the window run's.  (Nothing else loads
+  // pages: a load that the compiler knows of among those below would make it
+  // wait for all of them.)  One run, unless pages are small and many.
   const int bs_mask = (1 << a.bs_log2) - 1;
   const int32_t* bt = a.block_tables + (int64_t)b * a.max_blocks;
-  const int headn = min(v1, sp.head);                      // end of the head run
-  const int pg_a = v0 >> a.bs_log2;
-  const int na = headn > v0 ? ((headn - 1) >> a.bs_log2) - pg_a + 1 : 0;
-  const int win0 = max(v0, sp.head) + sp.gap, win1 = v1 + sp.gap;  // the window run's keys
-  const int pg_b = win0 >> a.bs_log2;
-  const int nb = v1 > sp.head && win1 > win0 ? ((win1 - 1) >> a.bs_log2) - pg_b + 1 : 0;
-  if (tid == 0) {
-    lds.holes = 0;
-    lds.mapped = 0x7fffffff;
-  }
-  __syncthreads();
-  for (int i = tid; i < na + nb; i += NT) {
-    const int p = bt[i < na ? pg_a + i : pg_b + i - na];
-    if (i < kMaxPages) lds.pages[i] = p;
-    if (p < 0) lds.holes = 1;
-  }
-  // (the query rows are waited for here, not behind the tiles loading ahead)
+  // (a run's two ends may lie inside pages, on both sides of the gap)
+  const int run = (int)min((int64_t)1 << 30, ((int64_t)(kMaxPages - 4) << a.bs_log2) / TK * TK);
+  int c0 = v0, c1 = v0;
+  int pg_a, na, pg_b;
+  bool holes;
+  int spare;  // the cache row that an unmapped key reads: one of a key that the run has
+  auto stage_pages = [&]() {  // the run's keys that count (0: none is mapped)
+    const int headn = min(c1, sp.head);                      // end of the head run
+    pg_a = c0 >> a.bs_log2;
+    na = headn > c0 ? ((headn - 1) >> a.bs_log2) - pg_a + 1 : 0;
+    const int win0 = max(c0, sp.head) + sp.gap, win1 = c1 + sp.gap;  // the window run's keys
+    pg_b = win0 >> a.bs_log2;
+    const int nb = c1 > sp.head && win1 > win0 ? ((win1 - 1) >> a.bs_log2) - pg_b + 1 : 0;
+    if (tid == 0) {
+      lds.holes = 0;
+      lds.mapped = 0x7fffffff;
+    }
+    __syncthreads();
+    for (int i = tid; i < na + nb; i += NT) {
+      const int p = bt[i < na ? pg_a + i : pg_b + i - na];
+      lds.pages[i] = p;
+      if (p < 0) lds.holes = 1;
+    }
+    // (the query rows are waited for here, not behind the tiles loading ahead)
 #pragma unroll
-  for (int mt = 0; mt < MT; ++mt)
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int j = 0; j < S_::QV; ++j) __asm__ volatile("" ::"v"(q[mt][j]));
-  __syncthreads();
-  auto page = [&](int key, bool head) {
-    const int i = head ? (key >> a.bs_log2) - pg_a : (key >> a.bs_log2) - pg_b + na;
-    return i < kMaxPages ? lds.pages[i] : bt[key >> a.bs_log2];
-  };
-  const bool holes = uniform(lds.holes) != 0;
-  int n_keys = v1 - v0;
-  int spare = 0;  // the cache row that an unmapped key reads: one of a key that the split has
-  if (holes) {    // uniform
+      for (int j = 0; j < S_::QV; ++j) __asm__ volatile("" ::"v"(q[mt][j]));
+    __syncthreads();
+    holes = uniform(lds.holes) != 0;
+    spare = 0;
+    if (!holes) return c1 - c0;  // uniform
     for (int i = tid; i < na + nb; i += NT)
-      if (bt[i < na ? pg_a + i : pg_b + i - na] >= 0) atomicMin(&lds.mapped, i);
+      if (lds.pages[i] >= 0) atomicMin(&lds.mapped, i);
     __syncthreads();
     const int i = uniform(lds.mapped);
-    if (i >= na + nb) {
-      n_keys = 0;  // no key at all
-    } else {
-      const int key = i < na ? max((pg_a + i) << a.bs_log2, v0) : max((pg_b + i - na) << a.bs_log2, win0);
-      spare = (bt[key >> a.bs_log2] << a.bs_log2) + (key & bs_mask);
-    }
-  }
+    if (i >= na + nb) return 0;
+    const int key = i < na ? max((pg_a + i) << a.bs_log2, c0) : max((pg_b + i - na) << a.bs_log2, win0);
+    spare = (lds.pages[i] << a.bs_log2) + (key & bs_mask);
+    return c1 - c0;
+  };
+  auto page = [&](int key, bool head) { return lds.pages[(key >> a.bs_log2) - (head ? pg_a : pg_b - na)]; };
 
   // ---- K/V rows straight to LDS: instruction j fills rows j RPI .., the lane
   // picking the chunk that its slot holds; rows past the last key read it again
@@ -267,14 +271,13 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     const uint32_t at = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)dst);
     __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(src) : "memory", "m0");
   };
-  const int ntiles = (n_keys + TK - 1) / TK;
   auto ktile = [&](int buf) { return mine + buf * (V ? 2 : 1) * S_::TILEB; };
   auto vtile = [&](int buf) { return mine + (buf * 2 + 1) * S_::TILEB; };
   auto issue = [&](int buf, int tile) {
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int r = j * RPI + lane / CPR, slot = lane % CPR;
-      const int v = min(v0 + tile * TK + r, v1 - 1);
+      const int v = min(c0 + tile * TK + r, c1 - 1);
       const int key = sp.key(v);
       const int p = page(key, v < sp.head);
       const uint32_t row = p >= 0 ? (uint32_t)((p << a.bs_log2) + (key & bs_mask)) : (uint32_t)spare;
@@ -355,10 +358,10 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       for (int u = 0; u < KT; ++u) s[mt][u] *= a.scale_log2;
   };
   auto mask = [&](int tile) {
-    const int vt = v0 + tile * TK;
-    const int k_first = sp.key(vt), k_last = sp.key(min(vt + TK, v1) - 1);
+    const int vt = c0 + tile * TK;
+    const int k_first = sp.key(vt), k_last = sp.key(min(vt + TK, c1) - 1);
     // uniform: every key exists and every row sees it
-    const bool all = vt + TK <= v1 && k_last <= sp.pos_min &&
+    const bool all = vt + TK <= c1 && k_last <= sp.pos_min &&
                      (a.window == 0 || k_last < a.sinks || k_first > sp.pos_max - a.window);
     if (!all) {
 #pragma unroll
@@ -369,13 +372,13 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
           const int key = sp.key(v);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) {
-            const bool on = v < v1 && key <= pos[mt] && (a.window == 0 || key > pos[mt] - a.window || key < a.sinks);
+            const bool on = v < c1 && key <= pos[mt] && (a.window == 0 || key > pos[mt] - a.window || key < a.sinks);
             s[mt][u][i] = on ? s[mt][u][i] : kNegInf;
           }
         }
     }
     if (holes) {  // uniform
-      const int v = min(vt + (lane & (TK - 1)), v1 - 1);
+      const int v = min(vt + (lane & (TK - 1)), c1 - 1);
       const uint64_t mapped = __ballot(page(sp.key(v), v < sp.head) >= 0);
 #pragma unroll
       for (int u = 0; u < KT; ++u)
@@ -445,8 +448,11 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     }
   };
 
-  if (w < ntiles) {
-    issue(0, w);
+  do {
+    c0 = c1;
+    c1 = min(v1, c0 + run);
+    const int ntiles = (stage_pages() + TK - 1) / TK;
+    if (w < ntiles) issue(0, w);
     if (w + kWaves < ntiles) issue(1, w + kWaves);
     int buf = 0;
     for (int t = w; t < ntiles; t += kWaves) {
@@ -454,12 +460,12 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       scores(ktile(buf));
       mask(t);
       if constexpr (MODE == kAttendScores) {
-        const int vt = v0 + t * TK;
+        const int vt = c0 + t * TK;
 #pragma unroll
         for (int u = 0; u < KT; ++u)
           if (c < a.R) {
             float* dst = a.scores + ((int64_t)pair * a.R + c) * a.score_keys + vt + u * 16 + g * 4;
-            *reinterpret_cast<f32x4*>(dst) = s[0][u];  // (score_keys is a whole number of tiles; v0 too)
+            *reinterpret_cast<f32x4*>(dst) = s[0][u];  // (score_keys is a whole number of tiles; c0 too)
           }
       }
       if constexpr (V) {
@@ -484,8 +490,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
         float y = x[0];
 #pragma unroll
         for (int e = 1; e < KT * 4; ++e) y = c == e ? x[e] : y;
-        const int v = v0 + t * TK + (c >> 2) * 16 + g * 4 + (c & 3);
-        if (c < KT * 4 && v < v1) {
+        const int v = c0 + t * TK + (c >> 2) * 16 + g * 4 + (c & 3);
+        if (c < KT * 4 && v < c1) {
           const int p = page(v, true);
           if (p >= 0) {
             float* dst = a.key_weights + ((int64_t)p * a.Hkv + hk) * (bs_mask + 1) + (v & bs_mask);
@@ -500,7 +506,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       }
       buf ^= 1;
     }
-  }
+    if (c1 < v1) __syncthreads();  // (uniform) the run's pages are read
+  } while (c1 < v1);
   if constexpr (!V) return;
 
   // ---- the waves' rows combined through LDS
