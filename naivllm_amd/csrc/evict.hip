@@ -6,20 +6,26 @@
 // and weight rows move to the front, in the order of their positions, of the
 // sequence's own table or of another.
 //
-// Selection (evict_select_kernel), one workgroup per (sequence, kv head): the
-// weights as unsigned words of the same order; the need-th largest found by
-// four passes over 8 bits each (a histogram per wave, so that equal words
-// cost few collisions); then one pass per wave over a run of its own counts
-// what lies above that word and what equals it, and a second one writes the
-// kept positions in order.  Bound by the latency of its passes over weights
-// that stay in L2.
+// Selection (evict_select_kernel), one workgroup of 16 waves per (sequence, kv
+// head): the weights are read once into registers, four neighbours per load
+// (beyond 32,768 keys they are read again in every pass), and compared as
+// unsigned words of the same order, in which the keys that stay anyway are the
+// largest.  The budget-th largest word comes from three passes over 11, 11
+// and 10 bits (four histograms; a wave whose words share a digit adds once,
+// so that equal weights cost no collisions); then each wave counts, per load, what lies
+// above that word and what equals it, a scan over those counts gives every
+// kept key its place, and key and weight are written there.  Bound by the
+// latency of its passes: one round trip and 15 barriers.
 //
 // Moving (evict_move_kernel): every kept row read and written once.  Within a
 // table rows move forward only: row i comes from kept[i] >= i.  A workgroup
-// owns one 64-byte column of one (sequence, kv head, K or V) and takes its
-// rows in ascending chunks, each read whole before it is written, so what a
-// chunk overwrites no later chunk reads, and no other workgroup touches the
-// column.  Bound by the rows' bytes.
+// owns a column of one (sequence, kv head, K or V), all of the row or 64 or
+// 128 bytes of it where there are few sequences, and takes its rows in
+// ascending chunks, each read whole before it is written and the next one's
+// reads under way: what a chunk overwrites no later chunk reads, and no other
+// workgroup touches the column.  Between tables apart nothing can be
+// overwritten, and the rows are dealt to many workgroups.  Bound by the rows'
+// bytes.
 
 #include "common.h"
 
@@ -29,8 +35,10 @@ namespace {
 
 constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
-constexpr int kMoveThreads = 256;
-constexpr int kMoveUnroll = 8;   // rows per lane and chunk
+constexpr int kSelLoads = 8;     // loads of four weights that a thread holds: 32,768 keys in all
+constexpr int kBins = 2048, kCopies = 4;
+constexpr int kMoveThreads = 512;
+constexpr int kMoveUnroll = 8;   // 16-byte pieces per lane and chunk
 
 struct EvictArgs {
   char* k;
@@ -42,6 +50,7 @@ struct EvictArgs {
   int64_t* lens;                 // [B]
   int32_t* kept;                 // [B][Hkv][budget]
   int Hkv, row_bytes, bs_log2, max_blocks, out_blocks, budget, sinks, recent;
+  int vector;                    // four weights of a page in one load
 };
 
 __device__ __forceinline__ int clamp_len(const EvictArgs& a, int b) {
@@ -57,155 +66,301 @@ __device__ __forceinline__ uint32_t ordered(float f) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
+// The wave's loads have returned (a barrier alone orders their issue).
+__device__ __forceinline__ void loads_back() { __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// HELD: every weight of a context fits the workgroup's registers.
+template <bool HELD>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
-  __shared__ int hist[kSelWaves][256];
-  __shared__ int above[256];
-  __shared__ int wave_gt[kSelWaves], wave_eq[kSelWaves];
+  constexpr int STEP = kSelThreads * 4;  // keys per load of the workgroup
+  __shared__ __attribute__((aligned(16))) int hist[kCopies][kBins];
+  __shared__ int wave_sum[kSelWaves];
   __shared__ int digit, rest;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / a.Hkv, h = blockIdx.x - b * a.Hkv;
-  const int n = clamp_len(a, b);
+  const int n = clamp_len(a, b), got = min(n, a.budget);
   const int bs_mask = (1 << a.bs_log2) - 1;
   const int32_t* bt = a.block_tables + (int64_t)b * a.max_blocks;
+  const int32_t* ot = a.out_tables + (int64_t)b * a.out_blocks;
+  const bool apart = a.out_tables != a.block_tables;
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
   auto place = [&](const int32_t* table, int key) -> int64_t {  // of a key's weight; -1: no page
     const int p = table[key >> a.bs_log2];
     return p < 0 ? -1 : ((((int64_t)p * a.Hkv + h) << a.bs_log2) + (key & bs_mask));
   };
-  auto word = [&](int key) {
-    const int64_t at = place(bt, key);
-    return at < 0 ? 0u : ordered(a.weights[at]);
-  };
-  if (tid == 0 && h == 0) a.lens[b] = min(n, a.budget);
-  const int got = min(n, a.budget);
+  if (tid == 0 && h == 0) a.lens[b] = got;
   for (int i = got + tid; i < a.budget; i += kSelThreads) kept[i] = -1;
-  if (n <= a.budget) {  // uniform: all of them stay
+  if (n <= a.budget && !apart) {  // uniform: nothing moves
     for (int i = tid; i < n; i += kSelThreads) kept[i] = i;
-  } else {
-    const int lo = a.sinks, hi = n - a.recent;      // the keys that compete
-    const int need = a.budget - a.sinks - a.recent; // how many of them stay
-    uint32_t prefix = 0;                            // the leading bits of the need-th largest word
-    int want = need;                                // which of the words with that prefix it is, from the top
-    for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-      for (int i = tid; i < kSelWaves * 256; i += kSelThreads) (&hist[0][0])[i] = 0;
-      __syncthreads();
-      for (int key = lo + tid; key < hi; key += kSelThreads) {
-        const uint32_t u = word(key);
-        if (shift == 24 || (u >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[w][(u >> shift) & 255], 1);
+    return;
+  }
+
+  // keys key .. key + 3 (key a multiple of 4); past the context and in unmapped pages: whatever
+  auto load4 = [&](int key) {
+    f32x4 x = {0.f, 0.f, 0.f, 0.f};
+    if (key >= n) return x;
+    if (a.vector) {  // uniform: pages of four keys or more, on 16 bytes
+      const int64_t at = place(bt, key);
+      if (at >= 0) x = *reinterpret_cast<const f32x4*>(a.weights + at);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t at = key + j < n ? place(bt, key + j) : -1;
+        if (at >= 0) x[j] = a.weights[at];
       }
+    }
+    return x;
+  };
+  auto word = [&](int key, float x) { return key < a.sinks || key >= n - a.recent ? 0xffffffffu : ordered(x); };
+  const int loads = (n + STEP - 1) / STEP;
+  f32x4 held[HELD ? kSelLoads : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int e = 0; e < kSelLoads; ++e)
+      if (e < loads) held[e] = load4(e * STEP + tid * 4);  // uniform
+  }
+  auto each = [&](auto f) {  // f(e, first key, weights) for every load
+    if constexpr (HELD) {
+#pragma unroll
+      for (int e = 0; e < kSelLoads; ++e)
+        if (e < loads) {  // uniform
+          // (nothing derived from these is kept from one use to the next: registers)
+          int key = e * STEP + tid * 4;
+          __asm__ volatile("" : "+v"(held[e]), "+v"(key));
+          f(e, key, held[e]);
+        }
+    } else {
+      for (int e = 0; e < loads; ++e) f(e, e * STEP + tid * 4, load4(e * STEP + tid * 4));
+    }
+  };
+
+  // ---- the got-th largest word, and how many of the words equal to it stay
+  uint32_t prefix = 0;
+  int want = got;
+  if (n > a.budget) {  // uniform
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
+      for (int i = tid; i < kCopies * kBins / 4; i += kSelThreads)
+        reinterpret_cast<u32x4*>(&hist[0][0])[i] = u32x4{0u, 0u, 0u, 0u};
       __syncthreads();
-      if (tid < 256) {
-        int s = 0;
-        for (int ww = 0; ww < kSelWaves; ++ww) s += hist[ww][tid];
-        above[tid] = s;
+      each([&](int, int key, f32x4 x) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t u = word(key + j, x[j]);
+          const bool on = key + j < n && (pass == 0 || (u >> (shift + bits)) == (prefix >> (shift + bits)));
+          const int d = (int)(u >> shift) & ((1 << bits) - 1);
+          const uint64_t active = __ballot(on);
+          if (!active) continue;  // uniform
+          const int leader = __builtin_ctzll(active);
+          const int d0 = __builtin_amdgcn_readlane(d, leader);
+          if (__ballot(on && d != d0) == 0) {  // uniform: one digit
+            if (lane == leader) atomicAdd(&hist[w & (kCopies - 1)][d], __popcll(active));
+          } else if (on) {
+            atomicAdd(&hist[w & (kCopies - 1)][d], 1);
+          }
+        }
+      });
+      __syncthreads();
+      // two bins per thread, from the top: what lies above them
+      const int top = kBins - 1 - 2 * tid;
+      int c1 = 0, c0 = 0;
+#pragma unroll
+      for (int k = 0; k < kCopies; ++k) {
+        c1 += hist[k][top];
+        c0 += hist[k][top - 1];
       }
+      int sum = c1 + c0;
+#pragma unroll
+      for (int d = 1; d < 64; d *= 2) {
+        const int y = __shfl_up(sum, d, 64);
+        sum += lane >= d ? y : 0;
+      }
+      if (lane == 63) wave_sum[w] = sum;
       __syncthreads();
-      if (tid == 0) {
-        int d = 255, left = want;
-        while (d > 0 && above[d] < left) left -= above[d--];
-        digit = d;
-        rest = left;
+      int above = sum - c1 - c0;
+      for (int ww = 0; ww < w; ++ww) above += wave_sum[ww];
+      if (above < want && above + c1 + c0 >= want) {  // one thread
+        const bool first = above + c1 >= want;
+        digit = first ? top : top - 1;
+        rest = first ? want - above : want - above - c1;
       }
       __syncthreads();
       prefix |= (uint32_t)digit << shift;
       want = rest;
+    }
+  }
+  // (a context that is short enough: every word is above 0 or, unmapped or
+  // not, equal to it, and stays)
+
+  // ---- places: the kept keys before each wave's four-key groups of each load, by a scan over counts in LDS
+  int* count_gt = &hist[0][0];  // [load][wave]
+  int* count_eq = &hist[1][0];
+  auto emit = [&](int e, int key, f32x4 x, int at_gt, int at_eq) {
+    // the wave's counts before this lane, then this lane's keys in order
+    uint64_t gt[4], eq[4];
+    int g = at_gt, q = at_eq;
+    const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t u = word(key + j, x[j]);
+      gt[j] = __ballot(key + j < n && u > prefix);
+      eq[j] = __ballot(key + j < n && u == prefix);
+      g += __popcll(gt[j] & below);
+      q += __popcll(eq[j] & below);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const bool is_gt = (gt[j] >> lane) & 1, is_eq = (eq[j] >> lane) & 1;
+      if (is_gt || (is_eq && q < want)) {
+        const int i = g + min(q, want);
+        kept[i] = key + j;
+        if constexpr (HELD) {  // (every weight of the context is in registers: places may be overwritten)
+          const int64_t to = place(bt, key + j) < 0 ? -1 : place(ot, i);
+          if (to >= 0) a.weights[to] = x[j];
+        }
+      }
+      g += is_gt;
+      q += is_eq;
+    }
+  };
+  auto tally = [&](int key, f32x4 x, int& g, int& q) {
+    g = q = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t u = word(key + j, x[j]);
+      g += __popcll(__ballot(key + j < n && u > prefix));
+      q += __popcll(__ballot(key + j < n && u == prefix));
+    }
+  };
+  constexpr int GROUP = kBins / kSelWaves;  // loads whose counts fit at a time
+  int base_gt = 0, base_eq = 0;
+  for (int e0 = 0; e0 < loads; e0 += GROUP) {  // (one turn up to 524,288 keys)
+    __syncthreads();
+    each([&](int e, int key, f32x4 x) {
+      if (e < e0 || e >= e0 + GROUP) return;  // uniform
+      int g, q;
+      tally(key, x, g, q);
+      if (lane == 0) {
+        count_gt[(e - e0) * kSelWaves + w] = g;
+        count_eq[(e - e0) * kSelWaves + w] = q;
+      }
+    });
+    __syncthreads();
+    const int m = min(GROUP, loads - e0) * kSelWaves;
+    if (w == 0) {  // exclusive scan of the counts, 64 at a time
+      int run_gt = base_gt, run_eq = base_eq;
+      for (int i0 = 0; i0 < m; i0 += 64) {
+        const int i = i0 + lane;
+        const int g = i < m ? count_gt[i] : 0, q = i < m ? count_eq[i] : 0;
+        int sg = g, sq = q;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const int yg = __shfl_up(sg, d, 64), yq = __shfl_up(sq, d, 64);
+          sg += lane >= d ? yg : 0;
+          sq += lane >= d ? yq : 0;
+        }
+        if (i < m) {
+          count_gt[i] = run_gt + sg - g;
+          count_eq[i] = run_eq + sq - q;
+        }
+        run_gt += __shfl(sg, 63, 64);
+        run_eq += __shfl(sq, 63, 64);
+      }
+      if (lane == 0) {
+        wave_sum[0] = run_gt;
+        wave_sum[1] = run_eq;
+      }
+    }
+    __syncthreads();
+    base_gt = wave_sum[0];
+    base_eq = wave_sum[1];
+    each([&](int e, int key, f32x4 x) {
+      if (e < e0 || e >= e0 + GROUP) return;  // uniform
+      emit(e, key, x, count_gt[(e - e0) * kSelWaves + w], count_eq[(e - e0) * kSelWaves + w]);
+    });
+  }
+  if constexpr (!HELD) {
+    // the weights themselves, a chunk at a time: every read of a chunk before its first write
+    __syncthreads();
+    for (int i0 = 0; i0 < got; i0 += kSelThreads) {
+      const int i = i0 + tid;
+      const int64_t at = i < got ? place(bt, kept[i]) : -1;
+      const float x = at >= 0 ? a.weights[at] : 0.f;
+      loads_back();
+      __syncthreads();
+      const int64_t to = at >= 0 ? place(ot, i) : -1;
+      if (to >= 0) a.weights[to] = x;
       __syncthreads();
     }
-    // words above `prefix` stay, and of those equal to it the first `want`
-    const int per = ((hi - lo + kSelWaves - 1) / kSelWaves + 63) & ~63;  // a wave's run
-    const int r0 = lo + w * per, r1 = min(hi, r0 + per);
-    int gt = 0, eq = 0;
-    if (need > 0) {
-      for (int key = r0 + lane; key - lane < r1; key += 64) {
-        const uint32_t u = key < r1 ? word(key) : 0u;
-        gt += __popcll(__ballot(key < r1 && u > prefix));
-        eq += __popcll(__ballot(key < r1 && u == prefix));
-      }
-    }
-    if (lane == 0) {
-      wave_gt[w] = gt;
-      wave_eq[w] = eq;
-    }
-    __syncthreads();
-    int at_gt = 0, at_eq = 0;
-    for (int ww = 0; ww < w; ++ww) {
-      at_gt += wave_gt[ww];
-      at_eq += wave_eq[ww];
-    }
-    if (need > 0) {
-      const uint64_t below = (1ull << lane) - 1;
-      for (int key = r0 + lane; key - lane < r1; key += 64) {
-        const uint32_t u = key < r1 ? word(key) : 0u;
-        const bool is_gt = key < r1 && u > prefix, is_eq = key < r1 && u == prefix;
-        const uint64_t bg = __ballot(is_gt), be = __ballot(is_eq);
-        const int g = at_gt + __popcll(bg & below), e = at_eq + __popcll(be & below);
-        if (is_gt || (is_eq && e < want)) kept[a.sinks + g + min(e, want)] = key;
-        at_gt += __popcll(bg);
-        at_eq += __popcll(be);
-      }
-    }
-    for (int i = tid; i < a.sinks; i += kSelThreads) kept[i] = i;
-    for (int i = tid; i < a.recent; i += kSelThreads) kept[a.budget - a.recent + i] = hi + i;
-  }
-  if (n <= a.budget && a.out_tables == a.block_tables) return;
-  // the weights themselves, a chunk at a time: every read of a chunk before its first write
-  __syncthreads();
-  const int32_t* ot = a.out_tables + (int64_t)b * a.out_blocks;
-  for (int i0 = 0; i0 < got; i0 += kSelThreads) {
-    const int i = i0 + tid;
-    float x = 0.f;
-    bool on = false;
-    if (i < got) {
-      const int64_t at = place(bt, kept[i]);
-      on = at >= 0;
-      if (on) x = a.weights[at];
-    }
-    __syncthreads();
-    if (on) {
-      const int64_t to = place(ot, i);
-      if (to >= 0) a.weights[to] = x;
-    }
-    __syncthreads();
   }
 }
 
-__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a) {
-  constexpr int ROWS = kMoveThreads / 4;  // rows a step of the workgroup takes: four lanes of 16 bytes each
-  const int slices = a.row_bytes / 64;
-  const int slice = blockIdx.x % slices, rest = blockIdx.x / slices;
+// grid: (sequence, kv head, column) x (K, V) x rows (1 workgroup in place)
+__global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, int lanes_log2) {
+  const int lanes = 1 << lanes_log2;               // 16-byte pieces per row and column
+  const int rows = kMoveThreads >> lanes_log2;     // rows that a step of the workgroup takes
+  const int columns = a.row_bytes / (16 * lanes);
+  const int column = blockIdx.x % columns, rest = blockIdx.x / columns;
   const int h = rest % a.Hkv, b = rest / a.Hkv;
   const int n = clamp_len(a, b), got = min(n, a.budget);
-  if (n <= a.budget && a.out_tables == a.block_tables) return;  // uniform: nothing moves
+  const bool apart = a.out_tables != a.block_tables;
+  if (n <= a.budget && !apart) return;  // uniform: nothing moves
   const int bs_mask = (1 << a.bs_log2) - 1;
   const int32_t* bt = a.block_tables + (int64_t)b * a.max_blocks;
   const int32_t* ot = a.out_tables + (int64_t)b * a.out_blocks;
   const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + h) * a.budget;
-  char* base = (blockIdx.y ? a.v : a.k) + (int64_t)h * a.row_bytes + slice * 64 + (threadIdx.x & 3) * 16;
+  char* base = (blockIdx.y ? a.v : a.k) + (int64_t)h * a.row_bytes + (column * lanes + (threadIdx.x & (lanes - 1))) * 16;
   const int64_t stride = (int64_t)a.Hkv * a.row_bytes;
-  const int r = threadIdx.x >> 2;
+  const int r = threadIdx.x >> lanes_log2;
   auto row = [&](const int32_t* table, int key) -> char* {
     const int p = table[key >> a.bs_log2];
     return p < 0 ? nullptr : base + (((int64_t)p << a.bs_log2) + (key & bs_mask)) * stride;
   };
-  for (int i0 = 0; i0 < got; i0 += ROWS * kMoveUnroll) {
+  const int chunk = rows * kMoveUnroll;
+  struct Chunk {
     u32x4 x[kMoveUnroll];
     bool on[kMoveUnroll];
+  };
+  auto read = [&](Chunk& c, int i0) {
+    const char* src[kMoveUnroll];
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
-      const int i = i0 + u * ROWS + r;
-      const char* src = i < got ? row(bt, kept[i]) : nullptr;
-      on[u] = src != nullptr;
-      x[u] = u32x4{0u, 0u, 0u, 0u};
-      if (on[u]) x[u] = load16_stream(src);
+      const int i = i0 + u * rows + r;
+      src[u] = i < got ? row(bt, kept[i]) : nullptr;
     }
-    __syncthreads();
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
-      const int i = i0 + u * ROWS + r;
-      char* dst = on[u] ? row(ot, i) : nullptr;
-      if (dst) *reinterpret_cast<u32x4*>(dst) = x[u];
+      c.on[u] = src[u] != nullptr;
+      c.x[u] = u32x4{0u, 0u, 0u, 0u};
+      if (c.on[u]) c.x[u] = load16_stream(src[u]);
     }
+  };
+  auto write = [&](const Chunk& c, int i0) {
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) {
+      const int i = i0 + u * rows + r;
+      char* dst = c.on[u] ? row(ot, i) : nullptr;
+      if (dst) __builtin_nontemporal_store(c.x[u], reinterpret_cast<u32x4*>(dst));
+    }
+  };
+  Chunk c;
+  if (apart) {
+    for (int i0 = blockIdx.z * chunk; i0 < got; i0 += gridDim.z * chunk) {
+      read(c, i0);
+      write(c, i0);
+    }
+    return;
+  }
+  // (the next chunk's sources lie behind this chunk's destinations; the barrier
+  // puts every read of a chunk before its first write)
+  read(c, 0);
+  for (int i0 = 0; i0 < got; i0 += chunk) {
+    Chunk next;
+    loads_back();
     __syncthreads();
+    if (i0 + chunk < got) read(next, i0 + chunk);
+    write(c, i0);
+    c = next;
   }
 }
 
@@ -232,12 +387,25 @@ int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights, const int32_t
   while ((1 << bs_log2) < block_size) ++bs_log2;
   EvictArgs a{(char*)k_cache, (char*)v_cache, key_weights, block_tables, out_block_tables ? out_block_tables : block_tables,
               context_lens, lens, kept, Hkv, row_bytes, bs_log2, max_blocks, out_block_tables ? out_blocks : max_blocks,
-              budget, sinks, recent};
+              budget, sinks, recent, bs_log2 >= 2 && (uintptr_t)key_weights % 16 == 0};
   hipStream_t s = (hipStream_t)stream;
-  hipLaunchKernelGGL(evict_select_kernel, dim3(B * Hkv), dim3(kSelThreads), 0, s, a);
+  if (cap <= (int64_t)kSelThreads * 4 * kSelLoads)
+    hipLaunchKernelGGL(evict_select_kernel<true>, dim3(B * Hkv), dim3(kSelThreads), 0, s, a);
+  else
+    hipLaunchKernelGGL(evict_select_kernel<false>, dim3(B * Hkv), dim3(kSelThreads), 0, s, a);
   const int rc = nsv_launch_status();
   if (rc) return rc;
-  hipLaunchKernelGGL(evict_move_kernel, dim3(B * Hkv * (row_bytes / 64), 2), dim3(kMoveThreads), 0, s, a);
+  // a row's pieces to one workgroup where the (sequence, head, K or V)s fill the chip (whole lines, one read of the
+  // page and position lists), else down to 64 bytes
+  int lanes_log2 = 2;
+  while (lanes_log2 < 5 && row_bytes % (32 << lanes_log2) == 0 &&
+         (a.out_tables != block_tables || (int64_t)B * Hkv * 2 * (row_bytes / (32 << lanes_log2)) >= 256))
+    ++lanes_log2;
+  const int columns = row_bytes / (16 << lanes_log2);
+  const int chunk = (kMoveThreads >> lanes_log2) * kMoveUnroll;
+  const int64_t most = std::min<int64_t>(cap, budget);
+  const int z = a.out_tables != block_tables ? (int)std::min<int64_t>((most + chunk - 1) / chunk, 64) : 1;
+  hipLaunchKernelGGL(evict_move_kernel, dim3(B * Hkv * columns, 2, z), dim3(kMoveThreads), 0, s, a, lanes_log2);
   return nsv_launch_status();
 }
 
