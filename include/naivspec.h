@@ -202,8 +202,8 @@ int nsv_prefill_tiles(const int64_t* seqlens_q, const int64_t* seqlens_k,
  * sinks; a tile's key range counts the keys that some row of it sees: the
  * first `sinks`, then those from its first row's window on (all of them, where
  * the two meet).  K/V of keys that no row of a tile sees are not read.
- *   stats   NULL, or [rows, H, 2] fp32: with a row's entry (m, l) the weight of
- *           a key of score s = scale * log2(e) * q.k is 2^(s - m) / l (l 0: the
+ *   stats   NULL, or [rows, H, 2] fp32: with a row's entry (m, r) the weight of
+ *           a key of score s = scale * log2(e) * q.k is 2^(s - m) * r (r 0: the
  *           row sees no key)
  */
 int nsv_prefill_window_tiles(const int64_t* seqlens_q,

@@ -148,7 +148,10 @@ def dtype_code(dtype: torch.dtype) -> int:
 
 
 def stream_ptr(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    """The current stream of a CUDA device (the raw handle, without making a
+    Stream object of it: 0.1 us instead of 2)."""
+    index = device.index
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if index is None else index)
 
 
 _no_guard = contextlib.nullcontext()

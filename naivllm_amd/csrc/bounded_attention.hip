@@ -56,6 +56,7 @@ struct RowArgs {
   int bs_log2, max_blocks, QL, R, S, npairs;  // R = G * QL
   int window, sinks;  // window 0: every key up to the row
   int score_keys;
+  int weight_splits;  // kWeights: workgroups that a pair's keys are dealt to
   int first_subset;   // kWeights: the subset this launch adds
 };
 
@@ -131,6 +132,32 @@ __device__ __forceinline__ int split_keys(int total, int S) {
   return max((per + TK - 1) / TK * TK, TK * kWaves);
 }
 
+// A row's maximum and 1 / sum over its splits, for `rows` rows from (pair, head
+// subset) ps on, into LDS (a barrier follows): a lane per split.  A row that
+// sees nothing: 0 and 0.
+__device__ __forceinline__ void join_stats(const RowArgs& a, int ps, int rows, float2* stat) {
+  constexpr int CH = 4;  // rows per round trip of a wave
+  const int lane = threadIdx.x & 63;
+  for (int m0 = threadIdx.x >> 6; m0 < rows; m0 += CH * kWaves) {
+    float2 x[CH];
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int m = min(m0 + k * kWaves, rows - 1);
+      const int sub = m / a.R;  // (rows may run on into the pair's next subsets)
+      x[k] = a.part_ml[((int64_t)(ps + sub) * a.S + min(lane, a.S - 1)) * a.R + m - sub * a.R];
+    }
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const int m = m0 + k * kWaves;
+      if (m >= rows) break;  // uniform
+      const float M = wave_max(x[k].x);
+      const float ref = M == kNegInf ? 0.f : M;
+      const float L = wave_sum(lane < a.S ? x[k].y * __builtin_amdgcn_exp2f(x[k].x - ref) : 0.f);
+      if (lane == 0) stat[m] = make_float2(ref, L > 0.f ? 1.f / L : 0.f);
+    }
+  }
+}
+
 template <typename T, int DH>
 struct Shape {
   static constexpr bool kBf16 = sizeof(T) == 2;
@@ -184,10 +211,10 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
   const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
   int my_pos;
   const Span sp = make_span(a, b, q0, qlen, my_pos);
-  const int per = split_keys<TK>(sp.total, a.S);
+  const int per = split_keys<TK>(sp.total, MODE == kWeights ? a.weight_splits : a.S);
   const int v0 = split * per;
   const int v1 = min(sp.total, v0 + per);
-  const int64_t part = ((int64_t)(pair * a.subsets + sub) * a.S + split) * a.R;
+  const int64_t part = ((int64_t)(pair * a.subsets + sub) * a.S + split) * a.R;  // (unused by kWeights)
   if (v0 >= v1 && split > 0) {  // uniform: this sequence has fewer splits
     if (V && tid < a.R) a.part_ml[part + tid] = make_float2(kNegInf, 0.f);
     return;
@@ -267,13 +294,17 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
   const char* kbase = (const char*)a.k + (int64_t)hk * ROWB;
   const char* vbase = (const char*)a.v + (int64_t)hk * ROWB;
   unsigned char* mine = lds.tiles[w];
-  auto load_lds = [&](const char* src, unsigned char* dst) {
-    const uint32_t at = uniform((uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)dst);
-    __asm__ volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), "v"(src) : "memory", "m0");
+  auto lds_at = [](const void* p) {
+    return (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
   };
+#define NSV_LOAD_LDS(at, offset, src)                                                                 \
+  __asm__ volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), \
+                   "v"(src), "n"(offset)                                                              \
+                   : "memory", "m0", "scc")
   auto ktile = [&](int buf) { return mine + buf * (V ? 2 : 1) * S_::TILEB; };
   auto vtile = [&](int buf) { return mine + (buf * 2 + 1) * S_::TILEB; };
   auto issue = [&](int buf, int tile) {
+    const uint32_t kt = lds_at(ktile(buf)), vt = V ? lds_at(vtile(buf)) : 0u;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const int r = j * RPI + lane / CPR, slot = lane % CPR;
@@ -282,8 +313,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       const int p = page(key, v < sp.head);
       const uint32_t row = p >= 0 ? (uint32_t)((p << a.bs_log2) + (key & bs_mask)) : (uint32_t)spare;
       const uint64_t off = (uint64_t)row * row_bytes;
-      load_lds(kbase + off + ((slot ^ S_::kswz(r)) << 4), ktile(buf) + j * 1024);
-      if constexpr (V) load_lds(vbase + off + ((slot ^ S_::vswz(r)) << 4), vtile(buf) + j * 1024);
+      NSV_LOAD_LDS(kt, j * 1024, kbase + off + ((slot ^ S_::kswz(r)) << 4));
+      if constexpr (V) NSV_LOAD_LDS(vt, j * 1024, vbase + off + ((slot ^ S_::vswz(r)) << 4));
     }
   };
   auto landed = [&](bool ahead) {
@@ -303,24 +334,16 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
 #pragma unroll
     for (int d = 0; d < NACC; ++d) acc[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  float row_m[MT], row_inv[MT];  // kWeights: the rows' final statistics
+  float row_m[MT], row_inv[MT];  // kWeights: the rows' maxima and 1 / their sums (0: a row that sees nothing)
   if constexpr (MODE == kWeights) {
+    join_stats(a, pair * a.subsets + sub, a.R, lds.row);
+    __syncthreads();
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       const int m = mt * 16 + c;
-      float M = kNegInf, L = 0.f;
-      if (pos[mt] >= 0) {
-        const float2* ml = a.part_ml + (int64_t)(pair * a.subsets + sub) * a.S * a.R + m;
-        for (int s = 0; s < a.S; ++s) M = fmaxf(M, ml[(int64_t)s * a.R].x);
-        if (M > kNegInf)
-          for (int s = 0; s < a.S; ++s) {
-            const float2 x = ml[(int64_t)s * a.R];
-            L += x.y * __builtin_amdgcn_exp2f(x.x - M);
-          }
-      }
-      row_m[mt] = M == kNegInf ? 0.f : M;
-      row_inv[mt] = L > 0.f ? 1.f / L : 0.f;
-      __asm__ volatile("" ::"v"(row_m[mt]), "v"(row_inv[mt]));
+      const float2 x = m < a.R ? lds.row[m] : make_float2(0.f, 0.f);
+      row_m[mt] = x.x;
+      row_inv[mt] = x.y;
     }
   }
 
@@ -463,10 +486,12 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
         const int vt = c0 + t * TK;
 #pragma unroll
         for (int u = 0; u < KT; ++u)
-          if (c < a.R) {
-            float* dst = a.scores + ((int64_t)pair * a.R + c) * a.score_keys + vt + u * 16 + g * 4;
-            *reinterpret_cast<f32x4*>(dst) = s[0][u];  // (score_keys is a whole number of tiles; c0 too)
-          }
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+            if (mt * 16 + c < a.R) {
+              float* dst = a.scores + ((int64_t)(pair * a.subsets + sub) * a.R + mt * 16 + c) * a.score_keys + vt + u * 16 + g * 4;
+              *reinterpret_cast<f32x4*>(dst) = s[mt][u];  // (score_keys is a whole number of tiles; c0 too)
+            }
       }
       if constexpr (V) {
         attend(vtile(buf));
@@ -572,51 +597,65 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
 }
 
 // ---------------------------------------------------------------------------
-// The splits joined: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s, in
-// split order; one workgroup per 256 / (D / 4) rows of a (pair, head subset).
-// A split without a key of the row (maximum -inf) holds no output.
+// The splits joined, and the key weights from stored scores.
+//
+// Workgroups y < merges: out = sum_s 2^(m_s - M) o_s / sum_s 2^(m_s - M) l_s of
+// a (pair, head subset)'s rows, one after another; the splits of a row are
+// dealt to `1 << sg_log2` groups of D / 4 lanes (a call of few pairs has up to
+// 64 of them, 14 us one after another), whose parts are added in order.  A split
+// without a key of the row (maximum -inf) holds no output.
+//
+// Workgroups behind them: 256 keys of a pair, one per thread, for all its
+// rows, whose statistics they join themselves.  A weight of a key at or behind
+// the sequence's first row is set, an older one's added to (one thread adds to
+// a place; an atomic add, so that sequences which share a page lose nothing).
 // ---------------------------------------------------------------------------
 template <typename T, int DH>
-__global__ __launch_bounds__(256) void row_merge_kernel(RowArgs a) {
-  constexpr int C4 = DH / 4;
-  const int ps = blockIdx.x;  // pair * subsets + sub
-  const int m = blockIdx.y * (256 / C4) + threadIdx.x / C4, ch = threadIdx.x % C4;
+__device__ __forceinline__ void merge_rows(const RowArgs& a, int ps, int block, int sg_log2) {
+  constexpr int C4 = DH / 4, GROUPS = 256 / C4;
+  __shared__ __attribute__((aligned(16))) f32x4 nums[GROUPS][C4];
+  __shared__ float2 mls[GROUPS];
+  const int grp = threadIdx.x / C4, ch = threadIdx.x % C4;
+  const int sg = 1 << sg_log2, si = grp & (sg - 1);
+  const int m = block * (GROUPS >> sg_log2) + (grp >> sg_log2);
   const int pair = ps / a.subsets, sub = ps - pair * a.subsets;
   const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
-  if (m >= a.R) return;
   const int q0 = a.cu_seqlens_q[b], qlen = a.cu_seqlens_q[b + 1] - q0;
   const int gh = m / a.QL, t = m - gh * a.QL;
-  if (t >= qlen) return;
-  const int64_t base = (int64_t)ps * a.S * a.R + m;
+  const bool row = m < a.R && t < qlen;
+  const int64_t base = (int64_t)ps * a.S * a.R + (row ? m : 0);
   constexpr int CH = 4;  // splits per round trip
   float M = kNegInf, den = 0.f;
   f32x4 num = {0.f, 0.f, 0.f, 0.f};
-  for (int s0 = 0; s0 < a.S; s0 += CH) {
+  auto add = [&](float2 ml, f32x4 o) {  // (in order: what is there, then this)
+    if (!(ml.x > kNegInf)) return;      // no key (its output may hold anything)
+    const float Mn = fmaxf(M, ml.x);
+    const float w0 = __builtin_amdgcn_exp2f(M - Mn), w1 = __builtin_amdgcn_exp2f(ml.x - Mn);
+    den = fmaf(ml.y, w1, den * w0);
+    num = num * w0 + o * w1;
+    M = Mn;
+  };
+  for (int s0 = si; s0 < a.S; s0 += sg * CH) {
     float2 ml[CH];
     f32x4 o[CH];
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
-      const int64_t r = base + (int64_t)min(s0 + k, a.S - 1) * a.R;
+      const int64_t r = base + (int64_t)min(s0 + k * sg, a.S - 1) * a.R;
       ml[k] = a.part_ml[r];
       o[k] = *reinterpret_cast<const f32x4*>(a.part_o + r * DH + ch * 4);
     }
-    float Mn = M;
 #pragma unroll
-    for (int k = 0; k < CH; ++k) Mn = fmaxf(Mn, ml[k].x);
-    if (Mn == kNegInf) continue;
-    const float w0 = __builtin_amdgcn_exp2f(M - Mn);
-    den *= w0;
-    num *= w0;
-#pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const bool on = s0 + k < a.S && ml[k].x > kNegInf;
-      const float wk = on ? __builtin_amdgcn_exp2f(ml[k].x - Mn) : 0.f;
-      den += on ? ml[k].y * wk : 0.f;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) num[e] = on ? fmaf(o[k][e], wk, num[e]) : num[e];
-    }
-    M = Mn;
+    for (int k = 0; k < CH; ++k)
+      if (s0 + k * sg < a.S) add(ml[k], o[k]);
   }
+  if (sg > 1) {  // uniform
+    nums[grp][ch] = num;
+    if (ch == 0) mls[grp] = make_float2(M, den);
+    __syncthreads();
+    if (si != 0) return;
+    for (int k = 1; k < sg; ++k) add(mls[grp + k], nums[grp + k][ch]);
+  }
+  if (!row) return;
   num = den > 0.f ? num * (1.f / den) : f32x4{0.f, 0.f, 0.f, 0.f};
   T* dst = (T*)a.out + ((int64_t)(q0 + t) * a.H + hk * (a.G * a.subsets) + sub * a.G + gh) * DH + ch * 4;
   if constexpr (sizeof(T) == 2)
@@ -624,51 +663,78 @@ __global__ __launch_bounds__(256) void row_merge_kernel(RowArgs a) {
   else *reinterpret_cast<f32x4*>(dst) = num;
 }
 
-// ---------------------------------------------------------------------------
-// Key weights from stored scores: one thread per key of a pair, the rows'
-// statistics in LDS.  A weight of a key at or behind the sequence's first row
-// is set, an older one's added to (one thread adds to a place; an atomic add,
-// so that sequences which share a page lose nothing).
-// ---------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void row_weights_kernel(RowArgs a) {
-  __shared__ float2 stat[16];  // maximum and 1 / sum
-  const int pair = blockIdx.x, b = pair / a.Hkv, hk = pair - b * a.Hkv;
+constexpr int kMaxStoredRows = 64;
+
+__device__ __forceinline__ void stored_weights(const RowArgs& a, int pair, int block) {
+  __shared__ float2 stat[kMaxStoredRows];  // maximum and 1 / sum
+  const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
   const int q0 = uniform(a.cu_seqlens_q[b]);
   const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
   int my_pos;
   const Span sp = make_span(a, b, q0, qlen, my_pos);
-  const int key = blockIdx.y * 256 + threadIdx.x;
-  if ((int)blockIdx.y * 256 >= sp.total) return;  // uniform
-  if (threadIdx.x < a.R) {
-    const float2* ml = a.part_ml + (int64_t)pair * a.S * a.R + threadIdx.x;
-    float M = kNegInf, L = 0.f;
-    for (int s = 0; s < a.S; ++s) M = fmaxf(M, ml[(int64_t)s * a.R].x);
-    if (M > kNegInf)
-      for (int s = 0; s < a.S; ++s) {
-        const float2 x = ml[(int64_t)s * a.R];
-        L += x.y * __builtin_amdgcn_exp2f(x.x - M);
-      }
-    stat[threadIdx.x] = make_float2(M == kNegInf ? 0.f : M, L > 0.f ? 1.f / L : 0.f);
-  }
+  if (block * 256 >= sp.total) return;  // uniform
+  const int key = block * 256 + threadIdx.x, rows = a.R * a.subsets;
+  const int p = key < sp.total ? a.block_tables[(int64_t)b * a.max_blocks + (key >> a.bs_log2)] : -1;
+  // (a chunk of rows' scores per round trip, the first beside the statistics'; behind the last key: key 0's again)
+  constexpr int CH = 16;
+  const float* src = a.scores + (int64_t)pair * rows * a.score_keys + (p < 0 ? 0 : key);
+  float s[CH];
+  auto read = [&](int m0) {
+#pragma unroll
+    for (int k = 0; k < CH; ++k) s[k] = m0 + k < rows ? src[(int64_t)(m0 + k) * a.score_keys] : 0.f;  // (uniform)
+  };
+  read(0);
+  join_stats(a, pair * a.subsets, rows, stat);
   __syncthreads();
-  if (key >= sp.total) return;
-  const int p = a.block_tables[(int64_t)b * a.max_blocks + (key >> a.bs_log2)];
   if (p < 0) return;
-  const float* src = a.scores + (int64_t)pair * a.R * a.score_keys + key;
   float y = 0.f;
-  for (int m = 0; m < a.R; ++m) {
-    const float inv = stat[m].y;  // 0: a row that sees nothing
-    const float s = src[(int64_t)m * a.score_keys];
-    y = inv > 0.f ? fmaf(__builtin_amdgcn_exp2f(s - stat[m].x), inv, y) : y;
+  for (int m0 = 0; m0 < rows; m0 += CH) {
+    if (m0 > 0) read(m0);
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const float2 x = stat[min(m0 + k, rows - 1)];
+      y = m0 + k < rows && x.y > 0.f ? fmaf(__builtin_amdgcn_exp2f(s[k] - x.x), x.y, y) : y;
+    }
   }
   float* dst = a.key_weights + (((int64_t)p * a.Hkv + hk) << a.bs_log2) + (key & ((1 << a.bs_log2) - 1));
   if (key >= sp.pos_min) *dst = y;
   else unsafeAtomicAdd(dst, y);
 }
 
+template <typename T, int DH>
+__global__ __launch_bounds__(256) void row_finish_kernel(RowArgs a, int merges, int sg_log2) {
+  if ((int)blockIdx.y < merges) {
+    const int pair = blockIdx.x / a.subsets;  // (x: pairs x subsets for these, the rest of the grid's rows use pairs)
+    if (pair < a.npairs) merge_rows<T, DH>(a, blockIdx.x, blockIdx.y, sg_log2);
+  } else if ((int)blockIdx.x < a.npairs) {
+    stored_weights(a, blockIdx.x, blockIdx.y - merges);
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Host
 // ---------------------------------------------------------------------------
+constexpr int kStoredMiB = 32;
+constexpr int kCus = 256;        // compute units of an MI355X
+constexpr int kOverheadKeys = 256;
+
+// Splits per pair: the rounds of resident workgroups that a count takes, each as long as
+// its keys and a workgroup's start and end, which take as long as
+// kOverheadKeys keys.
+int choose_splits(int64_t units, int64_t keys, int tile, int resident) {
+  const int64_t most = std::min<int64_t>(kMaxSplits, (keys + tile * kWaves - 1) / (tile * kWaves));
+  int64_t best = 1, best_cost = INT64_MAX;
+  for (int64_t s = 1; s <= most; ++s) {
+    const int64_t rounds = (units * s + resident - 1) / resident;
+    const int64_t cost = rounds * ((keys + s - 1) / s + kOverheadKeys);
+    if (cost < best_cost) {
+      best = s;
+      best_cost = cost;
+    }
+  }
+  return (int)best;
+}
+
 struct RowPlan {
   int G, subsets, R, MT, S;
   bool stored;     // key weights: from stored scores, else from the keys again
@@ -701,12 +767,10 @@ int make_row_plan(int B, int H, int Hkv, int D, int block_size, int max_blocks, 
   int64_t keys = cap;
   if (window > 0) keys = std::min<int64_t>(cap, (int64_t)window + sinks + max_q_len - 1);
   const int tile = dtype == NSV_BF16 ? 32 : 16;
-  int64_t S = pairs > 0 ? (512 + pairs * p->subsets - 1) / (pairs * p->subsets) : 1;
-  S = std::min<int64_t>({S, (keys + tile * kWaves - 1) / (tile * kWaves), (int64_t)kMaxSplits});
-  p->S = (int)std::max<int64_t>(1, S);
+  p->S = choose_splits(pairs * p->subsets, keys, tile, D == 64 ? 2 * kCus : kCus);
   p->score_keys = (int)((cap + 31) / 32 * 32);
-  p->score_bytes = weights ? (size_t)pairs * p->R * p->score_keys * sizeof(float) : 0;
-  p->stored = weights && p->MT == 1 && p->subsets == 1 && p->score_bytes <= ((size_t)256 << 20);
+  p->score_bytes = weights ? (size_t)pairs * p->subsets * p->R * p->score_keys * sizeof(float) : 0;
+  p->stored = weights && p->R * p->subsets <= kMaxStoredRows && p->score_bytes <= ((size_t)kStoredMiB << 20);
   if (!p->stored) p->score_bytes = 0;
   const size_t rows = (size_t)pairs * p->subsets * p->S * p->R;
   p->ml_bytes = align256(rows * sizeof(float2));
@@ -718,15 +782,11 @@ int make_row_plan(int B, int H, int Hkv, int D, int block_size, int max_blocks, 
 template <typename T, int DH, int MODE>
 void launch_rows(const RowArgs& a, int MT, dim3 grid, hipStream_t s) {
   const dim3 block(kWaves * 64);
-  if constexpr (MODE == kAttendScores) {
-    hipLaunchKernelGGL((row_attention_kernel<T, 1, DH, MODE>), grid, block, 0, s, a);
-  } else {
-    switch (MT) {
-      case 1: hipLaunchKernelGGL((row_attention_kernel<T, 1, DH, MODE>), grid, block, 0, s, a); break;
-      case 2: hipLaunchKernelGGL((row_attention_kernel<T, 2, DH, MODE>), grid, block, 0, s, a); break;
-      case 3: hipLaunchKernelGGL((row_attention_kernel<T, 3, DH, MODE>), grid, block, 0, s, a); break;
-      default: hipLaunchKernelGGL((row_attention_kernel<T, 4, DH, MODE>), grid, block, 0, s, a); break;
-    }
+  switch (MT) {
+    case 1: hipLaunchKernelGGL((row_attention_kernel<T, 1, DH, MODE>), grid, block, 0, s, a); break;
+    case 2: hipLaunchKernelGGL((row_attention_kernel<T, 2, DH, MODE>), grid, block, 0, s, a); break;
+    case 3: hipLaunchKernelGGL((row_attention_kernel<T, 3, DH, MODE>), grid, block, 0, s, a); break;
+    default: hipLaunchKernelGGL((row_attention_kernel<T, 4, DH, MODE>), grid, block, 0, s, a); break;
   }
 }
 
@@ -737,19 +797,23 @@ int launch_call(RowArgs& a, const RowPlan& p, hipStream_t s) {
   else launch_rows<T, DH, kAttend>(a, p.MT, grid, s);
   int rc = nsv_launch_status();
   if (rc != NSV_OK) return rc;
-  if (p.S > 1) {
-    constexpr int rows = 256 / (DH / 4);
-    hipLaunchKernelGGL((row_merge_kernel<T, DH>), dim3(a.npairs * p.subsets, (p.R + rows - 1) / rows), dim3(256), 0, s, a);
+  constexpr int groups = 256 / (DH / 4);
+  int sg_log2 = 0;
+  while ((1 << sg_log2) < groups && (4 << sg_log2) < p.S) ++sg_log2;  // a group takes four splits in a round trip
+  const int per = groups >> sg_log2;
+  const int merges = p.S > 1 ? (p.R + per - 1) / per : 0, blocks = p.stored ? (p.score_keys + 255) / 256 : 0;
+  if (merges + blocks > 0) {
+    const dim3 fgrid(a.npairs * (merges ? p.subsets : 1), merges + blocks);
+    hipLaunchKernelGGL((row_finish_kernel<T, DH>), fgrid, dim3(256), 0, s, a, merges, sg_log2);
     rc = nsv_launch_status();
     if (rc != NSV_OK) return rc;
   }
-  if (!a.key_weights) return NSV_OK;
-  if (p.stored) {
-    hipLaunchKernelGGL(row_weights_kernel, dim3(a.npairs, (p.score_keys + 255) / 256), dim3(256), 0, s, a);
-    return nsv_launch_status();
-  }
+  if (!a.key_weights || p.stored) return NSV_OK;
+  // (no V tiles: twice as many workgroups fit a compute unit, and no split leaves anything to join)
+  a.weight_splits = choose_splits(a.npairs, (int64_t)a.max_blocks << a.bs_log2, sizeof(T) == 2 ? 32 : 16,
+                                  2 * (DH == 64 ? 2 * kCus : kCus));
   for (a.first_subset = 0; a.first_subset < p.subsets; ++a.first_subset) {
-    launch_rows<T, DH, kWeights>(a, p.MT, dim3((unsigned)(a.npairs * p.S)), s);
+    launch_rows<T, DH, kWeights>(a, p.MT, dim3((unsigned)(a.npairs * a.weight_splits)), s);
     rc = nsv_launch_status();
     if (rc != NSV_OK) return rc;
   }
@@ -798,6 +862,7 @@ int row_attention(void* out, const void* q, const void* k_cache, const void* v_c
   a.window = window;
   a.sinks = sinks;
   a.score_keys = p.score_keys;
+  a.weight_splits = 1;
   a.first_subset = 0;
   hipStream_t s = (hipStream_t)stream;
   if (dtype == NSV_BF16) return D == 128 ? launch_call<bf16_t, 128>(a, p, s) : launch_call<bf16_t, 64>(a, p, s);

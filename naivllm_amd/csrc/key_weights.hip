@@ -3,7 +3,7 @@
 //   weight of (kv head, key j) = sum_(rows r at or behind j) sum_(heads of the
 //   group) 2^(s_rj - m_r) / l_r,   s_rj = scale log2(e) q_r . k_j
 //
-// with the statistics (m_r, l_r) that nsv_prefill_window_attention leaves.
+// with the statistics (m_r, 1 / l_r) that nsv_prefill_window_attention leaves.
 //
 // What bounds it: one matrix product of 2 D flops per (row, key) pair and an
 // exponential, two fused multiply-adds and a select, of which the exponential
@@ -21,6 +21,7 @@
 #include <algorithm>
 #include <array>
 #include <new>
+#include <type_traits>
 #include <vector>
 
 namespace {
@@ -30,6 +31,9 @@ constexpr int kRows = 64;         // rows per tile
 constexpr int kUnitWords = 8;     // int32 words of a unit record
 constexpr int kSumWords = 6;      // and of a sum record
 constexpr int kStages = 3;        // row tiles in LDS
+// rounds of the chip that the parts make: 8,192 rows of 32/8 heads 392 us with one,
+// 325 with two, 320 with four (1,206 rows of 16/8: no difference)
+constexpr int64_t kRounds = 4;
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -54,7 +58,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs a) {
   constexpr int J = kRows / RPI / 4;       // row loads per wave and tile
   struct __attribute__((aligned(16))) Lds {
     unsigned char q[kStages][kRows * ROWB];
-    float stat[kStages][2][kRows];         // maximum, sum
+    float stat[kStages][2][kRows];         // maximum, 1 / sum
   };
   __shared__ Lds lds;
   const int tid = threadIdx.x, lane = tid & 63;
@@ -109,11 +113,100 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs a) {
                        : "memory", "m0");
   };
 
-  f32x16 sum[2];
+  f32x16 sum[2], s[2];  // s[t]: scores of a half of 32 rows and of the wave's keys 32 t ..
 #pragma unroll
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int i = 0; i < 16; ++i) sum[t][i] = 0.f;
+
+  // 32 rows and 32 keys at a time: while the products of one such square are
+  // made, the exponentials of the one before it are (a quarter-rate operation
+  // each, so together longer than the products: what the loop is bound by).
+  u32x4 qb[KS];
+  auto read = [&](int buf, int half) {
+    const int r = half * 32 + col;
+    const unsigned char* src = lds.q[buf] + r * ROWB;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qb[ks] = *reinterpret_cast<const u32x4*>(src + (((ks * 2 + h) ^ (r & (CPR - 1))) << 4));
+  };
+  struct Rows {   // this lane's row of a half
+    float nb, inv;
+    int pos;
+    bool full;    // uniform: every row sees every key of the wave
+  };
+  auto row_of = [&](int buf, int half, int r0) {
+    const int r = half * 32 + col;
+    Rows x;
+    x.inv = r0 + r < nrows ? lds.stat[buf][1][r] : 0.f;
+    x.nb = x.inv > 0.f ? -lds.stat[buf][0][r] : -__builtin_inff();  // (a row that sees nothing: weights 0)
+    x.pos = pos0 + r0 + r;
+    x.full = pos0 + r0 + half * 32 >= wkey + 63;
+    return x;
+  };
+  auto weight = [&](float score, const Rows& x, float before) {
+    return fmaf(__builtin_amdgcn_exp2f(fmaf(score, a.scale_log2, x.nb)), x.inv, before);
+  };
+  auto add_masked = [&](int t, const Rows& x) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int key = wkey + t * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
+      const float y = weight(s[t][i], x, sum[t][i]);
+      sum[t][i] = key <= x.pos ? y : sum[t][i];
+    }
+  };
+  // the products of square t, and meanwhile square 1 - t (of rows x) added
+  auto square = [&](auto slot, const Rows& x) {
+    constexpr int t = decltype(slot)::value;
+    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    // (in three stages, so that nothing waits for the operation before it: an
+    // element's argument, its exponential and its addition fall beside three
+    // products in turn)
+    constexpr int PER = 16 / KS;
+    auto argument = [&](int i) { s[1 - t][i] = fmaf(s[1 - t][i], a.scale_log2, x.nb); };
+#pragma unroll
+    for (int i = 0; i < 2 * PER; ++i) argument(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(ka[t][ks]), as_bf16x8(qb[ks]), ks == 0 ? zero : s[t], 0, 0, 0);
+#pragma unroll
+      for (int i = ks * PER; i < (ks + 1) * PER; ++i) {
+        s[1 - t][i] = __builtin_amdgcn_exp2f(s[1 - t][i]);
+        if (i + 2 * PER < 16) argument(i + 2 * PER);
+        if (i >= PER) sum[1 - t][i - PER] = fmaf(s[1 - t][i - PER], x.inv, sum[1 - t][i - PER]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+#pragma unroll
+    for (int i = 16 - PER; i < 16; ++i) sum[1 - t][i] = fmaf(s[1 - t][i], x.inv, sum[1 - t][i]);
+  };
+  auto multiply = [&](int t) {
+    const f32x16 zero = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(ka[t][ks]), as_bf16x8(qb[ks]), ks == 0 ? zero : s[t], 0, 0, 0);
+  };
+  bool open = false;  // uniform: square 1 of the half before is multiplied and not yet added
+  Rows last;
+  auto step = [&](int buf, int half, int r0) {
+    read(buf, half);
+    const Rows x = row_of(buf, half, r0);
+    if (open && last.full) {  // uniform
+      square(std::integral_constant<int, 0>{}, last);
+    } else {
+      if (open) add_masked(1, last);
+      multiply(0);
+    }
+    if (x.full) {  // uniform
+      square(std::integral_constant<int, 1>{}, x);
+    } else {
+      multiply(1);
+      add_masked(0, x);
+    }
+    last = x;
+    open = true;
+  };
 
   if (t_begin < t_end) issue(0, t_begin);
   if (t_begin + 1 < t_end) issue(1, t_begin + 1);
@@ -127,49 +220,12 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs a) {
     if (tt + 2 < t_end) issue(buf + 2 >= kStages ? buf + 2 - kStages : buf + 2, tt + 2);
     const int g = tt / tiles, r0 = first + (tt - g * tiles) * kRows;
     if (pos0 + r0 + kRows - 1 >= wkey) {  // uniform: some row sees one of this wave's keys
-#pragma unroll
-      for (int half = 0; half < kRows / 32; ++half) {
-        const int r = half * 32 + col;
-        const unsigned char* src = lds.q[buf] + r * ROWB;
-        f32x16 s[2];
-        u32x4 qb[KS];
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          qb[ks] = *reinterpret_cast<const u32x4*>(src + (((ks * 2 + h) ^ (r & (CPR - 1))) << 4));
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[t][i] = 0.f;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-            s[t] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(as_bf16x8(ka[t][ks]), as_bf16x8(qb[ks]), s[t], 0, 0, 0);
-        // this lane's row: its weights are 2^(s - m) * inv, all of them 0 for a row that is not there or sees nothing
-        const float m = lds.stat[buf][0][r], l = lds.stat[buf][1][r];
-        const bool live = r0 + r < nrows && l > 0.f;
-        const float inv = live ? 1.f / l : 0.f, nb = live ? -m : -__builtin_inff();
-        const int pos = pos0 + r0 + r;
-        if (pos0 + r0 + half * 32 >= wkey + 63) {  // uniform: every row sees every key
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              sum[t][i] = fmaf(__builtin_amdgcn_exp2f(fmaf(s[t][i], a.scale_log2, nb)), inv, sum[t][i]);
-        } else {
-#pragma unroll
-          for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const int key = wkey + t * 32 + (i >> 2) * 8 + h * 4 + (i & 3);
-              const float x = fmaf(__builtin_amdgcn_exp2f(fmaf(s[t][i], a.scale_log2, nb)), inv, sum[t][i]);
-              sum[t][i] = key <= pos ? x : sum[t][i];
-            }
-        }
-      }
+      step(buf, 0, r0);
+      step(buf, 1, r0);
     }
     buf = buf + 1 == kStages ? 0 : buf + 1;
   }
+  if (open) add_masked(1, last);
 
   // over the 32 rows of a half-wave, in a fixed order; lane col 0 of each half holds the keys' sums
   float* dst = a.part + ((int64_t)unit * a.Hkv + hk) * kBlockKeys + w * 64;
@@ -214,6 +270,7 @@ __global__ __launch_bounds__(kBlockKeys) void key_sum_kernel(KeySumArgs a) {
   const int p = a.block_tables[(int64_t)seq * a.max_blocks + (key >> a.bs_log2)];
   const float* src = a.part + ((int64_t)unit * a.Hkv + hk) * kBlockKeys + threadIdx.x;
   float y = 0.f;
+#pragma unroll 8
   for (int u = 0; u < units; ++u) y += src[(int64_t)u * a.Hkv * kBlockKeys];
   if (p < 0) return;
   float* dst = a.key_weights + (((int64_t)p * a.Hkv + hk) << a.bs_log2) + (key & ((1 << a.bs_log2) - 1));
@@ -232,11 +289,25 @@ KeyTiling make_key_units(const int64_t* ql, const int64_t* kl, int n, int H, int
     const int64_t first = std::max<int64_t>(0, key0 - (kl[b] - ql[b]));
     return G * ((ql[b] - first + kRows - 1) / kRows);
   };
-  int64_t total = 0;
-  for (int b = 0; b < n; ++b)
-    for (int64_t k = 0; k < kl[b]; k += kBlockKeys) total += tiles_of(b, k);
-  // two workgroups fit a compute unit; about three rounds of them, none shorter than two row tiles
-  const int64_t target = std::max<int64_t>(2, total * Hkv / (6 * (int64_t)cus));
+  // tiles per part: the fewest (at least two) with which the workgroups, of
+  // which two fit a compute unit, make at most kRounds full rounds of the chip (a
+  // round of a few of them more would take as long as a full one)
+  auto units_of = [&](int64_t target) {
+    int64_t units = 0;
+    for (int b = 0; b < n; ++b)
+      for (int64_t k = 0; k < kl[b]; k += kBlockKeys) units += (tiles_of(b, k) + target - 1) / target;
+    return units * Hkv;
+  };
+  int64_t target = 2, above = 2;
+  while (units_of(above) > kRounds * 2 * (int64_t)cus && above < ((int64_t)1 << 40)) {
+    target = above + 1;
+    above *= 2;
+  }
+  while (target < above) {
+    const int64_t mid = (target + above) / 2;
+    if (units_of(mid) > kRounds * 2 * (int64_t)cus) target = mid + 1;
+    else above = mid;
+  }
   KeyTiling t;
   int64_t row0 = 0;
   for (int b = 0; b < n; ++b) {

@@ -64,7 +64,7 @@ struct PrefillArgs {
   const int32_t* tiles;         // [ntiles][kTileWords]: sequence, first row, rows, first position, first K/V row,
                                 // first key, end key, partial slot (-1: the tile's only part)
   float* part;                  // [slots][H][tile_rows][DH + 2]: unnormalised rows, then (max, sum) pairs
-  float2* stats;                // null, or [rows][H]: a row's exponent reference (log2 domain) and sum
+  float2* stats;                // null, or [rows][H]: a row's exponent reference (log2 domain) and 1 / sum (0: no key)
   int tile_rows;
   float scale_log2;
   int H, Hkv, bs_log2, max_blocks;
@@ -512,7 +512,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
     return;
   }
   if (r < nrows) {
-    if (a.stats && h == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(m_ref * sc, L);
+    if (a.stats && h == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(m_ref * sc, inv);
     bf16_t* dst = a.out + ((int64_t)(row0 + r) * a.H + head) * DH + h * 4;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillMergeArgs a) 
     M = Mn;
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
-  if (a.stats && c4 == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(M, den);
+  if (a.stats && c4 == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(M, inv);
   bf16_t* dst = a.out + ((int64_t)(row0 + r) * a.H + head) * DH + c4 * 4;
   *reinterpret_cast<uint2*>(dst) =
       make_uint2(pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv));

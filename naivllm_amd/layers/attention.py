@@ -165,6 +165,30 @@ def paged_attention_verify(
     return out
 
 
+def _few_rows(query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads: int,
+              num_kv_heads: int, head_dim: int, block_size: int, out, what: str) -> tuple:
+    """The checks of the few-row operators over a paged cache; returns query,
+    the index tensors in the kernels' types, and the output.  What a serving
+    loop passes goes through one condition; everything else is told apart,
+    converted or refused, in _check_few_rows."""
+    dev, kshape = query.get_device(), k_cache.shape
+    B, T = context_lens.numel(), positions.numel()
+    if not (dev >= 0 and query.shape == (T, num_heads, head_dim) and v_cache.shape == kshape
+            and kshape[1:] == (block_size, num_kv_heads, head_dim) and kshape[0] * block_size <= 0x7fffffff
+            and query.dtype == k_cache.dtype == v_cache.dtype and query.is_contiguous() and k_cache.is_contiguous()
+            and v_cache.is_contiguous() and (query.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0
+            and k_cache.get_device() == v_cache.get_device() == block_tables.get_device() == context_lens.get_device()
+            == cu_seqlens_q.get_device() == positions.get_device() == dev
+            and block_tables.dtype == cu_seqlens_q.dtype == torch.int32 and block_tables.is_contiguous()
+            and context_lens.dtype == positions.dtype == torch.int64 and context_lens.is_contiguous()
+            and positions.is_contiguous() and cu_seqlens_q.is_contiguous() and block_tables.dim() == 2
+            and block_tables.shape[0] == B and context_lens.dim() == cu_seqlens_q.dim() == positions.dim() == 1
+            and cu_seqlens_q.numel() == B + 1 and out is None):
+        return _check_few_rows(query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads,
+                               num_kv_heads, head_dim, block_size, out, what)
+    return query, block_tables, context_lens, cu_seqlens_q, positions, torch.empty_like(query)
+
+
 def _check_few_rows(query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads: int,
                     num_kv_heads: int, head_dim: int, block_size: int, out, what: str) -> tuple:
     """The checks of the few-row operators over a paged cache; returns the
@@ -260,7 +284,7 @@ def paged_attention_window(
     so calls on several streams, and captured ones, share nothing.
     No counterpart in the reference, whose attention sees every key."""
     window, sinks = _int_arg(window, "window", 1), _int_arg(sinks, "sinks", 0)
-    query, block_tables, context_lens, cu_seqlens_q, positions, out = _check_few_rows(
+    query, block_tables, context_lens, cu_seqlens_q, positions, out = _few_rows(
         query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads, num_kv_heads, head_dim,
         block_size, out, "paged_attention_window")
     B, max_blocks = block_tables.shape
@@ -311,7 +335,7 @@ def paged_attention_weights(
     to 64 rows per sequence.  A page that several sequences of a call share
     gets the sum of theirs, in no fixed order.  Scratch comes from torch's
     allocator.  No counterpart in the reference."""
-    query, block_tables, context_lens, cu_seqlens_q, positions, out = _check_few_rows(
+    query, block_tables, context_lens, cu_seqlens_q, positions, out = _few_rows(
         query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads, num_kv_heads, head_dim,
         block_size, out, "paged_attention_weights")
     _check_key_weights(key_weights, k_cache)
