@@ -551,6 +551,20 @@ def verify_serves_prefill(seqlens_q, seqlens_k, num_heads: int, num_kv_heads: in
     return pairs >= 8 and key_split and group > 2 and longest >= 1536
 
 
+def few_rows_serve_prefill(seqlens_q, num_heads: int, num_kv_heads: int) -> bool:
+    """Whether a paged bf16 prefill step with a window, or with key weights,
+    runs on the few-row kernels (paged_attention_window / _weights), one block
+    of rows per sequence, and not on the prefill kernels: up to 48 packed rows
+    (query heads of a kv head x rows).  MI355X, graph-replayed, prefill kernels
+    -> few-row ones, us per layer: a window of 1,024 behind 4,096 keys, 16/8
+    heads, one sequence of 9 rows 15.7 -> 11.5, eight 18.2 -> 16.2, of 32 21.7 ->
+    24.0 (64 packed rows: the prefill kernels), 32/8 heads, eight of 9 23.8 ->
+    19.8, of 16 25.2 -> 23.8; behind 256 keys 15.3 -> 14.1, of 16 15.8 -> 16.9.
+    Key weights of the same: 29.6 -> 17.7, 87.6 -> 47.1, 90.3 -> 66.5, 135.7 ->
+    55.4; behind 256 keys 23.4 -> 21.8, of 16 23.9 -> 29.8."""
+    return 1 <= num_heads // num_kv_heads * max(seqlens_q, default=0) <= 48
+
+
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """t on 16 bytes, as the loads of the prefill kernel that go straight to
     LDS need it: a view at an odd offset is copied (what torch allocates is
@@ -791,17 +805,62 @@ class Attention(nn.Module):
         the verify kernel over causal blocks of rows (``_prefill_rows``);
       * decode (neither flag): one query row per sequence attending its
         whole context (:759-767), served by the same verify kernel with
-        each row at position context_lens - 1."""
+        each row at position context_lens - 1.
+
+    A layer over a bounded cache (no reference counterpart):
+      * ``window`` > 0: every row sees its last ``window`` keys and its
+        sequence's first ``sinks`` only, in all three kinds of steps;
+      * ``key_weights`` set to an fp32 (num_blocks, num_kv_heads, block_size)
+        table beside the caches: every step adds its rows' attention weights
+        to their keys' places (a prefill step needs block tables then), for
+        evict_kvcache to cut the cache by."""
 
     def __init__(self, num_heads: int, head_dim: int, scale: float = 1.0, num_kv_heads: int | None = None,
-                 block_size: int = 16):
+                 block_size: int = 16, window: int = 0, sinks: int = 0):
         super().__init__()
+        self.window, self.sinks = _int_arg(window, "window", 0), _int_arg(sinks, "sinks", 0)
         self.num_heads = num_heads
         self.head_dim = head_dim
         self.scale = scale
         self.num_kv_heads = num_kv_heads if num_kv_heads is not None else num_heads
         self.block_size = block_size
         self.k_cache = self.v_cache = torch.tensor([])
+        self.key_weights: torch.Tensor | None = None
+
+    def _few(self, q, tables, context_lens, cu_seqlens_q, positions, scale: float, max_q_len: int,
+             out: torch.Tensor | None = None) -> torch.Tensor:
+        """A few rows per sequence over the paged cache: with the layer's
+        window, with its key weights, or as the verify round does."""
+        shape = (tables, context_lens, cu_seqlens_q, positions, scale, self.num_heads, self.num_kv_heads, self.head_dim,
+                 self.block_size, max(16, 1 << (max_q_len - 1).bit_length()))
+        if self.window:
+            return paged_attention_window(q, self.k_cache, self.v_cache, *shape, window=self.window, sinks=self.sinks,
+                                          max_q_len=max_q_len, out=out)
+        if self.key_weights is not None:
+            return paged_attention_weights(q, self.k_cache, self.v_cache, self.key_weights, *shape, max_q_len=max_q_len,
+                                           out=out)
+        return paged_attention_verify(q, self.k_cache, self.v_cache, *shape, max_q_len=max_q_len, out=out)
+
+    def _prefill_f32_weights(self, context, q, scale: float) -> torch.Tensor:
+        """An fp32 prefill step with key weights: causal blocks of rows as
+        ``_prefill_rows`` cuts them, one block of every sequence per call (two
+        blocks of a sequence in one call would add to the same places)."""
+        tables, lens, cu, positions, q_block = _prefill_rows(context, self.num_heads, self.num_kv_heads, q.device)
+        out, cu, first = torch.empty_like(q), cu.tolist(), 0
+        blocks: list[list[int]] = []  # per turn: the entries of _prefill_rows' batch
+        for n in context.seqlens_q:
+            count = -(-n // q_block)
+            for i in range(count):
+                if i == len(blocks):
+                    blocks.append([])
+                blocks[i].append(first + i)
+            first += count
+        for entries in blocks:
+            rows = torch.cat([torch.arange(cu[e], cu[e + 1]) for e in entries]).to(q.device)
+            starts = torch.tensor([0] + [cu[e + 1] - cu[e] for e in entries]).cumsum(0).to(q.device, torch.int32)
+            at = torch.tensor(entries, device=q.device)
+            out[rows] = self._few(q[rows], tables[at], lens[at], starts, positions[rows], scale, q_block)
+        return out
 
     def _prefill_bf16(self, context, q, k, v, scale: float) -> torch.Tensor:
         """The prefill branch on the prefill kernel, or on the verify kernel
@@ -813,13 +872,29 @@ class Attention(nn.Module):
         bs = self.block_size if paged else None
         key = (self.num_heads, self.num_kv_heads, bs, q.device)
         plans = context.__dict__.setdefault("prefill_plans", {})
-        if paged and verify_serves_prefill(context.seqlens_q, context.seqlens_k, self.num_heads, self.num_kv_heads, bs,
-                                           context.block_tables.shape[1]):
+        if self.window or self.key_weights is not None:
+            few = paged and few_rows_serve_prefill(context.seqlens_q, self.num_heads, self.num_kv_heads)
+        else:
+            few = paged and verify_serves_prefill(context.seqlens_q, context.seqlens_k, self.num_heads, self.num_kv_heads,
+                                                  bs, context.block_tables.shape[1])
+        if few:
             return self._prefill_few(context, plans, q, scale)
+        if self.window:
+            key += (self.window, self.sinks)
         plan = plans.get(key)
         if plan is None:
             plan = plans[key] = PrefillPlan(context.seqlens_q, context.seqlens_k, self.num_heads, self.num_kv_heads,
-                                            bs, q.device)
+                                            bs, q.device, self.window, self.sinks)
+        if paged and self.key_weights is not None:
+            adder = plans.get((*key, "weights"))
+            if adder is None:
+                adder = plans[(*key, "weights")] = KeyWeightsPlan(context.seqlens_q, context.seqlens_k, self.num_heads,
+                                                                  self.num_kv_heads, bs, q.device)
+            tables = context.block_tables.to(q.device)
+            stats = torch.empty((plan.rows, self.num_heads, 2), dtype=torch.float32, device=q.device)
+            out = prefill_attention(q, self.k_cache, self.v_cache, plan, scale, self.head_dim, tables, stats=stats)
+            prefill_key_weights(q, self.k_cache, self.key_weights, adder, stats, scale, self.head_dim, tables)
+            return out
         if paged:
             return prefill_attention(q, self.k_cache, self.v_cache, plan, scale, self.head_dim,
                                      context.block_tables.to(q.device))
@@ -837,6 +912,11 @@ class Attention(nn.Module):
         if tables.shape[0] < rows.sequences:
             raise ValueError(f"{rows.sequences} sequences but {tables.shape[0]} block-table rows")
         rows.use_on(torch.cuda.current_stream(q.device))
+        if self.window or self.key_weights is not None:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)  # (rows past the step's: unwritten)
+            self._few(q[:rows.rows], tables[:rows.sequences], rows.context_lens, rows.cu_seqlens_q, rows.positions, scale,
+                      rows.max_q_len, out[:rows.rows])
+            return out
         return paged_attention_verify(
             q, self.k_cache, self.v_cache, tables[:rows.sequences], rows.context_lens, rows.cu_seqlens_q, rows.positions,
             scale, self.num_heads, self.num_kv_heads, self.head_dim, self.block_size, 64, max_q_len=rows.max_q_len,
@@ -845,6 +925,11 @@ class Attention(nn.Module):
     def forward(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
         context = get_context()
         k_cache, v_cache = self.k_cache, self.v_cache
+        if self.key_weights is not None:
+            if self.window:
+                raise ValueError("a layer has a window or key weights, not both")
+            if context.block_tables is None:
+                raise ValueError("a layer with key weights needs context.block_tables: the weights are paged")
         if k_cache.numel() > 0 and v_cache.numel() > 0 and context.slot_mapping is not None:
             store_kvcache(k.reshape(-1, self.num_kv_heads, self.head_dim),
                           v.reshape(-1, self.num_kv_heads, self.head_dim),
@@ -857,6 +942,9 @@ class Attention(nn.Module):
             if q.dtype == torch.bfloat16:
                 o = self._prefill_bf16(context, q, k, v, scale)
                 return o.reshape(o.shape[0], self.num_heads * self.head_dim)
+            if self.key_weights is not None:
+                o = self._prefill_f32_weights(context, q, scale)
+                return o.reshape(o.shape[0], self.num_heads * self.head_dim)
             bt, lens, cu, positions, q_block = _prefill_rows(context, self.num_heads, self.num_kv_heads, q.device)
             if context.block_tables is not None:
                 kc, vc, bs = k_cache, v_cache, self.block_size
@@ -864,8 +952,13 @@ class Attention(nn.Module):
                 kc = k.reshape(-1, 1, self.num_kv_heads, self.head_dim).contiguous()
                 vc = v.reshape(-1, 1, self.num_kv_heads, self.head_dim).contiguous()
                 bs = 1
-            o = paged_attention_verify(q, kc, vc, bt, lens, cu, positions, scale, self.num_heads, self.num_kv_heads,
-                                       self.head_dim, bs, max(16, q_block), max_q_len=q_block)
+            shape = (bt, lens, cu, positions, scale, self.num_heads, self.num_kv_heads, self.head_dim, bs, max(16, q_block))
+            if self.window:
+                rows, o = positions.numel(), torch.empty_like(q, memory_format=torch.contiguous_format)
+                paged_attention_window(q[:rows], kc, vc, *shape, window=self.window, sinks=self.sinks, max_q_len=q_block,
+                                       out=o[:rows])
+            else:
+                o = paged_attention_verify(q, kc, vc, *shape, max_q_len=q_block)
             return o.reshape(o.shape[0], self.num_heads * self.head_dim)
         if context.is_verify:
             max_q_len = max(context.seqlens_q)
@@ -875,8 +968,5 @@ class Attention(nn.Module):
             max_q_len = 1
             cu = torch.arange(0, q.shape[0] + 1, dtype=torch.int32, device=q.device)
             positions = context.context_lens.to(torch.int64) - 1
-        block_m = max(16, 1 << (max_q_len - 1).bit_length())
-        o = paged_attention_verify(
-            q, k_cache, v_cache, context.block_tables, context.context_lens, cu, positions, scale,
-            self.num_heads, self.num_kv_heads, self.head_dim, self.block_size, block_m, max_q_len=max_q_len)
+        o = self._few(q, context.block_tables, context.context_lens, cu, positions, scale, max_q_len)
         return o.reshape(o.shape[0], self.num_heads * self.head_dim)
