@@ -69,13 +69,14 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 // The wave's loads have returned (a barrier alone orders their issue).
 __device__ __forceinline__ void loads_back() { __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// HELD: every weight of a context fits the workgroup's registers.
+// HELD: every weight of a context fits the workgroup's registers, and so do
+// their words.
 template <bool HELD>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
   constexpr int STEP = kSelThreads * 4;  // keys per load of the workgroup
-  __shared__ __attribute__((aligned(16))) int hist[kCopies][kBins];
-  __shared__ int wave_sum[kSelWaves];
-  __shared__ int digit, rest;
+  __shared__ __attribute__((aligned(16))) int hist[3][kCopies][kBins];  // one per pass
+  __shared__ __attribute__((aligned(16))) int wave_sum[kSelWaves];
+  __shared__ int digit, rest, share;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / a.Hkv, h = blockIdx.x - b * a.Hkv;
   const int n = clamp_len(a, b), got = min(n, a.budget);
@@ -111,52 +112,72 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     }
     return x;
   };
-  auto word = [&](int key, float x) { return key < a.sinks || key >= n - a.recent ? 0xffffffffu : ordered(x); };
+  // words of keys key .. key + 3: the largest for keys that stay anyway, 0 (less than every weight's) past the context
+  auto words = [&](int key, f32x4 x) {
+    u32x4 u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      u[j] = key + j < a.sinks || key + j >= n - a.recent ? 0xffffffffu : ordered(x[j]);
+      u[j] = key + j < n ? u[j] : 0u;
+    }
+    return u;
+  };
   const int loads = (n + STEP - 1) / STEP;
   f32x4 held[HELD ? kSelLoads : 1];
+  u32x4 word[HELD ? kSelLoads : 1];
   if constexpr (HELD) {
 #pragma unroll
     for (int e = 0; e < kSelLoads; ++e)
       if (e < loads) held[e] = load4(e * STEP + tid * 4);  // uniform
   }
-  auto each = [&](auto f) {  // f(e, first key, weights) for every load
+  for (int i = tid; i < 3 * kCopies * kBins / 4; i += kSelThreads)  // (while the weights are under way)
+    reinterpret_cast<u32x4*>(&hist[0][0][0])[i] = u32x4{0u, 0u, 0u, 0u};
+  if constexpr (HELD) {
+#pragma unroll
+    for (int e = 0; e < kSelLoads; ++e)
+      if (e < loads) word[e] = words(e * STEP + tid * 4, held[e]);
+  }
+  auto each = [&](auto f) {  // f(e, first key, weights, words) for every load
     if constexpr (HELD) {
 #pragma unroll
       for (int e = 0; e < kSelLoads; ++e)
         if (e < loads) {  // uniform
           // (nothing derived from these is kept from one use to the next: registers)
           int key = e * STEP + tid * 4;
-          __asm__ volatile("" : "+v"(held[e]), "+v"(key));
-          f(e, key, held[e]);
+          __asm__ volatile("" : "+v"(word[e]), "+v"(key));
+          f(e, key, held[e], word[e]);
         }
     } else {
-      for (int e = 0; e < loads; ++e) f(e, e * STEP + tid * 4, load4(e * STEP + tid * 4));
+      for (int e = 0; e < loads; ++e) {
+        const int key = e * STEP + tid * 4;
+        const f32x4 x = load4(key);
+        f(e, key, x, words(key, x));
+      }
     }
   };
+  __syncthreads();
 
-  // ---- the got-th largest word, and how many of the words equal to it stay
+  // ---- the got-th largest word: its leading bits `prefix` down to bit `low`,
+  // and how many of the words that share them stay (all of them, if low > 0)
   uint32_t prefix = 0;
-  int want = got;
+  int want = n > a.budget ? got : 0, low = 0;
   if (n > a.budget) {  // uniform
+    int above_bits = 32;  // leading bits not yet told apart end here
     for (int pass = 0; pass < 3; ++pass) {
-      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = pass == 2 ? 10 : 11;
-      for (int i = tid; i < kCopies * kBins / 4; i += kSelThreads)
-        reinterpret_cast<u32x4*>(&hist[0][0])[i] = u32x4{0u, 0u, 0u, 0u};
-      __syncthreads();
-      each([&](int, int key, f32x4 x) {
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = above_bits - shift;
+      int* mine = hist[pass][w & (kCopies - 1)];
+      const uint32_t head = pass == 0 ? 0u : prefix >> above_bits;
+      each([&](int, int, f32x4, u32x4 u) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const uint32_t u = word(key + j, x[j]);
-          const bool on = key + j < n && (pass == 0 || (u >> (shift + bits)) == (prefix >> (shift + bits)));
-          const int d = (int)(u >> shift) & ((1 << bits) - 1);
-          const uint64_t active = __ballot(on);
-          if (!active) continue;  // uniform
-          const int leader = __builtin_ctzll(active);
-          const int d0 = __builtin_amdgcn_readlane(d, leader);
-          if (__ballot(on && d != d0) == 0) {  // uniform: one digit
-            if (lane == leader) atomicAdd(&hist[w & (kCopies - 1)][d], __popcll(active));
-          } else if (on) {
-            atomicAdd(&hist[w & (kCopies - 1)][d], 1);
+          if (pass > 0 && (u[j] >> above_bits) != head) continue;
+          const int d = (int)(u[j] >> shift) & ((1 << bits) - 1);
+          const int d0 = __builtin_amdgcn_readfirstlane(d);
+          const uint64_t active = __ballot(true);
+          if (__ballot(d != d0) == 0) {  // uniform: one digit
+            if (lane == __builtin_ctzll(active)) atomicAdd(&mine[d0], __popcll(active));
+          } else {
+            atomicAdd(&mine[d], 1);
           }
         }
       });
@@ -166,8 +187,9 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       int c1 = 0, c0 = 0;
 #pragma unroll
       for (int k = 0; k < kCopies; ++k) {
-        c1 += hist[k][top];
-        c0 += hist[k][top - 1];
+        const int2 c = *reinterpret_cast<const int2*>(&hist[pass][k][top - 1]);
+        c0 += c.x;
+        c1 += c.y;
       }
       int sum = c1 + c0;
 #pragma unroll
@@ -178,39 +200,47 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       if (lane == 63) wave_sum[w] = sum;
       __syncthreads();
       int above = sum - c1 - c0;
-      for (int ww = 0; ww < w; ++ww) above += wave_sum[ww];
+#pragma unroll
+      for (int ww = 0; ww < kSelWaves; ww += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(&wave_sum[ww]);
+        above += (ww < w ? x.x : 0) + (ww + 1 < w ? x.y : 0) + (ww + 2 < w ? x.z : 0) + (ww + 3 < w ? x.w : 0);
+      }
       if (above < want && above + c1 + c0 >= want) {  // one thread
         const bool first = above + c1 >= want;
         digit = first ? top : top - 1;
         rest = first ? want - above : want - above - c1;
+        share = first ? c1 : c0;
       }
       __syncthreads();
       prefix |= (uint32_t)digit << shift;
       want = rest;
+      above_bits = shift;
+      if (want == share) {  // uniform: every word that shares them stays
+        low = shift;
+        break;
+      }
     }
   }
-  // (a context that is short enough: every word is above 0 or, unmapped or
-  // not, equal to it, and stays)
+  // (a context that is short enough: every weight's word is above 0, and stays)
 
   // ---- places: the kept keys before each wave's four-key groups of each load, by a scan over counts in LDS
-  int* count_gt = &hist[0][0];  // [load][wave]
-  int* count_eq = &hist[1][0];
-  auto emit = [&](int e, int key, f32x4 x, int at_gt, int at_eq) {
+  const uint32_t mark = prefix >> low;
+  int* count_gt = &hist[0][0][0];  // [load][wave]
+  int* count_eq = &hist[1][0][0];
+  auto below = [](uint64_t m) {  // of a wave's mask, the bits before this lane's
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+  };
+  auto emit = [&](int key, f32x4 x, u32x4 u, int at_gt, int at_eq) {
     // the wave's counts before this lane, then this lane's keys in order
-    uint64_t gt[4], eq[4];
     int g = at_gt, q = at_eq;
-    const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t u = word(key + j, x[j]);
-      gt[j] = __ballot(key + j < n && u > prefix);
-      eq[j] = __ballot(key + j < n && u == prefix);
-      g += __popcll(gt[j] & below);
-      q += __popcll(eq[j] & below);
+      g += below(__ballot((u[j] >> low) > mark));
+      q += below(__ballot((u[j] >> low) == mark));
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const bool is_gt = (gt[j] >> lane) & 1, is_eq = (eq[j] >> lane) & 1;
+      const bool is_gt = (u[j] >> low) > mark, is_eq = (u[j] >> low) == mark;
       if (is_gt || (is_eq && q < want)) {
         const int i = g + min(q, want);
         kept[i] = key + j;
@@ -223,23 +253,18 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       q += is_eq;
     }
   };
-  auto tally = [&](int key, f32x4 x, int& g, int& q) {
-    g = q = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t u = word(key + j, x[j]);
-      g += __popcll(__ballot(key + j < n && u > prefix));
-      q += __popcll(__ballot(key + j < n && u == prefix));
-    }
-  };
   constexpr int GROUP = kBins / kSelWaves;  // loads whose counts fit at a time
   int base_gt = 0, base_eq = 0;
   for (int e0 = 0; e0 < loads; e0 += GROUP) {  // (one turn up to 524,288 keys)
     __syncthreads();
-    each([&](int e, int key, f32x4 x) {
+    each([&](int e, int, f32x4, u32x4 u) {
       if (e < e0 || e >= e0 + GROUP) return;  // uniform
-      int g, q;
-      tally(key, x, g, q);
+      int g = 0, q = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        g += __popcll(__ballot((u[j] >> low) > mark));
+        q += __popcll(__ballot((u[j] >> low) == mark));
+      }
       if (lane == 0) {
         count_gt[(e - e0) * kSelWaves + w] = g;
         count_eq[(e - e0) * kSelWaves + w] = q;
@@ -274,9 +299,9 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     __syncthreads();
     base_gt = wave_sum[0];
     base_eq = wave_sum[1];
-    each([&](int e, int key, f32x4 x) {
+    each([&](int e, int key, f32x4 x, u32x4 u) {
       if (e < e0 || e >= e0 + GROUP) return;  // uniform
-      emit(e, key, x, count_gt[(e - e0) * kSelWaves + w], count_eq[(e - e0) * kSelWaves + w]);
+      emit(key, x, u, count_gt[(e - e0) * kSelWaves + w], count_eq[(e - e0) * kSelWaves + w]);
     });
   }
   if constexpr (!HELD) {
