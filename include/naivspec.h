@@ -110,6 +110,11 @@ int nsv_verify_attention_tile_refs(
  * keys.
  * Workspace: nsv_window_attention_workspace_size() bytes on 16 bytes, of any
  * content; calls that share one must not run concurrently.
+ * counters: NULL, or 64 KiB of device memory, zero before their first call;
+ * every call leaves them zero, and calls that share them must not run
+ * concurrently (so a graph that may run beside other work needs NULL or its
+ * own).  With them a call of up to 8 splits per sequence is one kernel, whose
+ * last split to finish joins them; without, two.
  */
 size_t nsv_window_attention_workspace_size(int B, int H, int Hkv, int D,
                                            int block_size, int max_blocks,
@@ -121,8 +126,8 @@ int nsv_window_attention(void* out, const void* q, const void* k_cache,
                          const int32_t* cu_seqlens_q, const int64_t* positions,
                          float scale, int B, int T, int H, int Hkv, int D,
                          int block_size, int max_blocks, int max_q_len,
-                         int dtype, int window, int sinks, void* workspace,
-                         size_t workspace_bytes, void* stream);
+                         int dtype, int window, int sinks, void* counters,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * nsv_verify_attention that adds every key's attention weight, summed over

@@ -57,7 +57,7 @@ SIGNATURES: dict[str, tuple] = {
     "nsv_evict_kv": (_c_int, [_c_vp] * 8 + [_c_int] * 10 + [_c_vp]),
     "nsv_window_attention_workspace_size": (_c_size, [_c_int] * 10),
     "nsv_window_attention": (
-        _c_int, [_c_vp] * 8 + [_c_f32] + [_c_int] * 11 + [_c_vp, _c_size, _c_vp]),
+        _c_int, [_c_vp] * 8 + [_c_f32] + [_c_int] * 11 + [_c_vp, _c_vp, _c_size, _c_vp]),
     "nsv_weights_attention_workspace_size": (_c_size, [_c_int] * 8),
     "nsv_weights_attention": (
         _c_int, [_c_vp] * 9 + [_c_f32] + [_c_int] * 9 + [_c_vp, _c_size, _c_vp]),
@@ -165,6 +165,21 @@ def on_device(device: torch.device):
 
 def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
+
+
+_counters: dict = {}
+
+
+def stream_counters(device: torch.device, stream: int) -> int | None:
+    """64 KiB of arrival counters for the calls enqueued on ``stream`` outside
+    a capture, zero between them: their address.  None inside a capture: its
+    graph may be replayed beside any stream's work, or another graph's."""
+    if torch.cuda.is_current_stream_capturing():
+        return None
+    buf = _counters.get((device.index, stream))
+    if buf is None:
+        buf = _counters[device.index, stream] = torch.zeros(16384, dtype=torch.int32, device=device)
+    return buf.data_ptr()
 
 
 def upload(x, device: torch.device) -> torch.Tensor:

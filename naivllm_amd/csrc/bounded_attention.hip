@@ -28,13 +28,20 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
 constexpr int kWaves = 4;         // waves per workgroup
 constexpr int kMaxPages = 2048;   // block-table entries of a workgroup's keys held in LDS
 constexpr int kMaxSplits = 64;
+constexpr int kJoinedSplits = 8;  // the most that the kernel joins itself
+constexpr int kCounters = 16384;  // words of the arrival counters
 constexpr float kNegInf = -__builtin_inff();
+
+// The word of a (pair, head subset): the first 256 have a 256-byte line each
+// (device-scope atomics on one line wait for one another).
+__device__ __forceinline__ int counter_slot(int unit) { return ((unit & 255) << 6) | (unit >> 8); }
 
 enum Mode { kAttend, kAttendScores, kWeights };
 
@@ -49,6 +56,7 @@ struct RowArgs {
   const int64_t* positions;
   float2* part_ml;    // [npairs * subsets][S][R]: (maximum, log2 domain; sum)
   float* part_o;      // [npairs * subsets][S][R][D], unnormalised
+  unsigned* counters; // null, or splits of a (pair, head subset) done so far, 0 between calls (kAttend)
   float* scores;      // [npairs][R][score_keys], log2 domain, -inf where masked (kAttendScores)
   float* key_weights; // [num_blocks][Hkv][block_size]
   float scale_log2;
@@ -215,8 +223,10 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
   const int v0 = split * per;
   const int v1 = min(sp.total, v0 + per);
   const int64_t part = ((int64_t)(pair * a.subsets + sub) * a.S + split) * a.R;  // (unused by kWeights)
+  const bool joins = MODE == kAttend && a.counters != nullptr;  // uniform: the last split to finish joins them all
+  const int nsplit = max(1, (sp.total + per - 1) / per);        // those of this sequence
   if (v0 >= v1 && split > 0) {  // uniform: this sequence has fewer splits
-    if (V && tid < a.R) a.part_ml[part + tid] = make_float2(kNegInf, 0.f);
+    if (V && !joins && tid < a.R) a.part_ml[part + tid] = make_float2(kNegInf, 0.f);
     return;
   }
 
@@ -535,6 +545,14 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
   } while (c1 < v1);
   if constexpr (!V) return;
 
+  auto store_row = [&](int m, int ch, f32x4 o) {  // a 16-byte piece of row m's output
+    const int gh = m / a.QL, t = m - gh * a.QL;
+    if (t >= qlen) return;
+    T* dst = (T*)a.out + ((int64_t)(q0 + t) * a.H + head0 + gh) * DH + ch * 4;
+    if constexpr (BF16) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    else *reinterpret_cast<f32x4*>(dst) = o;
+  };
+
   // ---- the waves' rows combined through LDS
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -575,6 +593,8 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     }
   }
   __syncthreads();
+  const bool whole = a.S == 1 || (joins && nsplit == 1);  // uniform: nothing to join
+  const __amdgpu_buffer_rsrc_t prs = block_rsrc(a.part_o + part * DH);
   for (int idx = tid; idx < a.R * (DH / 4); idx += NT) {
     const int m = idx / (DH / 4), ch = idx % (DH / 4);
     f32x4 o = {0.f, 0.f, 0.f, 0.f};
@@ -582,18 +602,77 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     for (int ww = 0; ww < kWaves; ++ww)
       o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds.tiles[ww]) + m * DH + ((ch + m) & (DH / 4 - 1)) * 4);
     const float2 ml = lds.row[m];
-    if (ch == 0) a.part_ml[part + m] = ml;
-    if (a.S > 1) {
+    if (whole) {
+      if (MODE != kAttend && ch == 0) a.part_ml[part + m] = ml;
+      store_row(m, ch, ml.y > 0.f ? o * (1.f / ml.y) : f32x4{0.f, 0.f, 0.f, 0.f});
+    } else if (joins) {
+      store16_agent(prs, (unsigned)(m * DH + ch * 4) * 4u, o);
+      if (ch == 0)
+        __hip_atomic_store(reinterpret_cast<uint64_t*>(a.part_ml + part + m),
+                           (uint64_t)__float_as_uint(ml.x) | ((uint64_t)__float_as_uint(ml.y) << 32), __ATOMIC_RELAXED,
+                           __HIP_MEMORY_SCOPE_AGENT);
+    } else {
+      if (ch == 0) a.part_ml[part + m] = ml;
       *reinterpret_cast<f32x4*>(a.part_o + (part + m) * DH + ch * 4) = o;
-      continue;
     }
-    const int gh = m / a.QL, t = m - gh * a.QL;
-    if (t >= qlen) continue;
-    o = ml.y > 0.f ? o * (1.f / ml.y) : f32x4{0.f, 0.f, 0.f, 0.f};
-    T* dst = (T*)a.out + ((int64_t)(q0 + t) * a.H + head0 + gh) * DH + ch * 4;
-    if constexpr (BF16) *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
-    else *reinterpret_cast<f32x4*>(dst) = o;
   }
+  if (whole || !joins) return;
+
+  // ---- the splits joined by the last of them to finish.  As the verify
+  // kernel's: partials are written through to the device's point of coherence
+  // (sc1), every thread waits for its stores' acknowledgement before the barrier
+  // ahead of the arrival's count, and the workgroup that counts last loads them
+  // from there, after the count came back; no cache is written back or
+  // invalidated.  Joined in split order, whichever comes last.
+  __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  unsigned* counter = a.counters + counter_slot(pair * a.subsets + sub);
+  if (tid == 0)
+    lds.holes = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(nsplit - 1);
+  __syncthreads();
+  if (!uniform(lds.holes)) return;
+  if (tid == 0) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  const int64_t first = part - (int64_t)split * a.R;  // row 0 of split 0
+  const __amdgpu_buffer_rsrc_t ors = block_rsrc(a.part_o + first * DH), mrs = block_rsrc(a.part_ml + first);
+  auto join = [&](auto width) {
+    constexpr int CW = decltype(width)::value;            // splits loaded in a round trip: all of them
+    constexpr int IG = CW == 4 ? 3 : 2;                   // items of a thread at a time
+    const int items = a.R * (DH / 4);
+    for (int i0 = tid; i0 < items; i0 += IG * NT) {
+      float2 ml[IG][CW];
+      f32x4 o[IG][CW];
+#pragma unroll
+      for (int k = 0; k < CW; ++k) {
+        const unsigned rows = (unsigned)(uniform(k < nsplit ? k : 0) * a.R);
+#pragma unroll
+        for (int i = 0; i < IG; ++i) {
+          const int idx = min(i0 + i * NT, items - 1);
+          ml[i][k] = load8_agent(mrs, (unsigned)(idx / (DH / 4)) * 8u, rows * 8u);
+          o[i][k] = load16_agent(ors, (unsigned)idx * 16u, rows * (DH * 4u));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < IG; ++i) {
+        const int idx = i0 + i * NT;
+        if (idx >= items) break;
+        float M = kNegInf, den = 0.f;
+        f32x4 num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < CW; ++k) M = fmaxf(M, k < nsplit ? ml[i][k].x : kNegInf);
+        const float ref = M == kNegInf ? 0.f : M;
+#pragma unroll
+        for (int k = 0; k < CW; ++k) {
+          const float wk = k < nsplit ? __builtin_amdgcn_exp2f(ml[i][k].x - ref) : 0.f;
+          den = fmaf(ml[i][k].y, wk, den);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) num[e] = fmaf(o[i][k][e], wk, num[e]);
+        }
+        store_row(idx / (DH / 4), idx % (DH / 4), den > 0.f ? num * (1.f / den) : f32x4{0.f, 0.f, 0.f, 0.f});
+      }
+    }
+  };
+  if (nsplit <= 4) join(std::integral_constant<int, 4>{});  // uniform
+  else join(std::integral_constant<int, kJoinedSplits>{});
 }
 
 // ---------------------------------------------------------------------------
@@ -624,17 +703,9 @@ __device__ __forceinline__ void merge_rows(const RowArgs& a, int ps, int block, 
   const int gh = m / a.QL, t = m - gh * a.QL;
   const bool row = m < a.R && t < qlen;
   const int64_t base = (int64_t)ps * a.S * a.R + (row ? m : 0);
-  constexpr int CH = 4;  // splits per round trip
+  constexpr int CH = kJoinedSplits;  // splits per round trip: what the attention kernel joins, joined alike, bit for bit
   float M = kNegInf, den = 0.f;
   f32x4 num = {0.f, 0.f, 0.f, 0.f};
-  auto add = [&](float2 ml, f32x4 o) {  // (in order: what is there, then this)
-    if (!(ml.x > kNegInf)) return;      // no key (its output may hold anything)
-    const float Mn = fmaxf(M, ml.x);
-    const float w0 = __builtin_amdgcn_exp2f(M - Mn), w1 = __builtin_amdgcn_exp2f(ml.x - Mn);
-    den = fmaf(ml.y, w1, den * w0);
-    num = num * w0 + o * w1;
-    M = Mn;
-  };
   for (int s0 = si; s0 < a.S; s0 += sg * CH) {
     float2 ml[CH];
     f32x4 o[CH];
@@ -644,16 +715,37 @@ __device__ __forceinline__ void merge_rows(const RowArgs& a, int ps, int block, 
       ml[k] = a.part_ml[r];
       o[k] = *reinterpret_cast<const f32x4*>(a.part_o + r * DH + ch * 4);
     }
+    float Mn = M;
 #pragma unroll
-    for (int k = 0; k < CH; ++k)
-      if (s0 + k * sg < a.S) add(ml[k], o[k]);
+    for (int k = 0; k < CH; ++k) Mn = fmaxf(Mn, s0 + k * sg < a.S ? ml[k].x : kNegInf);
+    const float ref = Mn == kNegInf ? 0.f : Mn;
+    const float w0 = __builtin_amdgcn_exp2f(M - ref);  // (from -inf: 0)
+    den *= w0;
+    num *= w0;
+#pragma unroll
+    for (int k = 0; k < CH; ++k) {
+      const bool on = s0 + k * sg < a.S && ml[k].x > kNegInf;  // (else its output may hold anything)
+      const float wk = on ? __builtin_amdgcn_exp2f(ml[k].x - ref) : 0.f;
+      den = fmaf(on ? ml[k].y : 0.f, wk, den);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) num[e] = on ? fmaf(o[k][e], wk, num[e]) : num[e];
+    }
+    M = Mn;
   }
   if (sg > 1) {  // uniform
     nums[grp][ch] = num;
     if (ch == 0) mls[grp] = make_float2(M, den);
     __syncthreads();
     if (si != 0) return;
-    for (int k = 1; k < sg; ++k) add(mls[grp + k], nums[grp + k][ch]);
+    for (int k = 1; k < sg; ++k) {
+      const float2 x = mls[grp + k];
+      if (!(x.x > kNegInf)) continue;
+      const float Mn = fmaxf(M, x.x);
+      const float w0 = __builtin_amdgcn_exp2f(M - Mn), w1 = __builtin_amdgcn_exp2f(x.x - Mn);
+      den = fmaf(x.y, w1, den * w0);
+      num = num * w0 + nums[grp + k][ch] * w1;
+      M = Mn;
+    }
   }
   if (!row) return;
   num = den > 0.f ? num * (1.f / den) : f32x4{0.f, 0.f, 0.f, 0.f};
@@ -718,15 +810,19 @@ constexpr int kStoredMiB = 32;
 constexpr int kCus = 256;        // compute units of an MI355X
 constexpr int kOverheadKeys = 256;
 
-// Splits per pair: the rounds of resident workgroups that a count takes, each as long as
-// its keys and a workgroup's start and end, which take as long as
-// kOverheadKeys keys.
+// Splits per pair: the rounds of resident workgroups that a count takes, each
+// as long as its keys and a workgroup's start and end, which take as long as
+// kOverheadKeys keys (64 to 1,024: no difference), and 128 keys more where the
+// splits are too many for the kernel to join.  Whole rounds: 64 pairs of 4,108
+// keys in 4 splits (256 workgroups) 35 us, 6 48, 8 47, 12 54; 64 pairs of 1,250
+// keys 15 us in 4, 19 in 6 and 8; 24 pairs of 1,009 keys in fp32 9.5 us in 8
+// splits, 10.5 in 16.
 int choose_splits(int64_t units, int64_t keys, int tile, int resident) {
   const int64_t most = std::min<int64_t>(kMaxSplits, (keys + tile * kWaves - 1) / (tile * kWaves));
   int64_t best = 1, best_cost = INT64_MAX;
   for (int64_t s = 1; s <= most; ++s) {
     const int64_t rounds = (units * s + resident - 1) / resident;
-    const int64_t cost = rounds * ((keys + s - 1) / s + kOverheadKeys);
+    const int64_t cost = rounds * ((keys + s - 1) / s + kOverheadKeys) + (s > kJoinedSplits ? 128 : 0);
     if (cost < best_cost) {
       best = s;
       best_cost = cost;
@@ -799,9 +895,9 @@ int launch_call(RowArgs& a, const RowPlan& p, hipStream_t s) {
   if (rc != NSV_OK) return rc;
   constexpr int groups = 256 / (DH / 4);
   int sg_log2 = 0;
-  while ((1 << sg_log2) < groups && (4 << sg_log2) < p.S) ++sg_log2;  // a group takes four splits in a round trip
+  while ((1 << sg_log2) < groups && (kJoinedSplits << sg_log2) < p.S) ++sg_log2;  // a group takes eight splits in a round trip
   const int per = groups >> sg_log2;
-  const int merges = p.S > 1 ? (p.R + per - 1) / per : 0, blocks = p.stored ? (p.score_keys + 255) / 256 : 0;
+  const int merges = p.S > 1 && !a.counters ? (p.R + per - 1) / per : 0, blocks = p.stored ? (p.score_keys + 255) / 256 : 0;
   if (merges + blocks > 0) {
     const dim3 fgrid(a.npairs * (merges ? p.subsets : 1), merges + blocks);
     hipLaunchKernelGGL((row_finish_kernel<T, DH>), fgrid, dim3(256), 0, s, a, merges, sg_log2);
@@ -823,8 +919,8 @@ int launch_call(RowArgs& a, const RowPlan& p, hipStream_t s) {
 int row_attention(void* out, const void* q, const void* k_cache, const void* v_cache, float* key_weights,
                   const int32_t* block_tables, const int64_t* context_lens, const int32_t* cu_seqlens_q,
                   const int64_t* positions, float scale, int B, int T, int H, int Hkv, int D, int block_size,
-                  int max_blocks, int max_q_len, int dtype, int window, int sinks, bool weights, void* workspace,
-                  size_t workspace_bytes, void* stream) {
+                  int max_blocks, int max_q_len, int dtype, int window, int sinks, bool weights, unsigned* counters,
+                  void* workspace, size_t workspace_bytes, void* stream) {
   if (T < 0) return NSV_ERR_ARG;
   RowPlan p;
   const int rc = make_row_plan(B, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, window, sinks, weights, &p);
@@ -833,7 +929,7 @@ int row_attention(void* out, const void* q, const void* k_cache, const void* v_c
   if (!out || !q || !k_cache || !v_cache || !block_tables || !context_lens || !cu_seqlens_q || !positions ||
       (weights && !key_weights))
     return NSV_ERR_ARG;
-  if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache) % 16) return NSV_ERR_ARG;
+  if (((uintptr_t)out | (uintptr_t)q | (uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)counters) % 16) return NSV_ERR_ARG;
   if (!workspace || workspace_bytes < p.ml_bytes + p.o_bytes + p.score_bytes) return NSV_ERR_WORKSPACE;
   RowArgs a;
   a.q = q;
@@ -847,6 +943,7 @@ int row_attention(void* out, const void* q, const void* k_cache, const void* v_c
   a.part_ml = (float2*)workspace;
   a.part_o = (float*)((char*)workspace + p.ml_bytes);
   a.scores = (float*)((char*)workspace + p.ml_bytes + p.o_bytes);
+  a.counters = !weights && p.S <= kJoinedSplits && (int64_t)B * Hkv * p.subsets <= kCounters ? counters : nullptr;
   a.key_weights = weights ? key_weights : nullptr;
   a.scale_log2 = scale * 1.44269504088896340736f;
   a.H = H;
@@ -884,11 +981,11 @@ size_t nsv_window_attention_workspace_size(int B, int H, int Hkv, int D, int blo
 int nsv_window_attention(void* out, const void* q, const void* k_cache, const void* v_cache,
                          const int32_t* block_tables, const int64_t* context_lens, const int32_t* cu_seqlens_q,
                          const int64_t* positions, float scale, int B, int T, int H, int Hkv, int D, int block_size,
-                         int max_blocks, int max_q_len, int dtype, int window, int sinks, void* workspace,
-                         size_t workspace_bytes, void* stream) {
+                         int max_blocks, int max_q_len, int dtype, int window, int sinks, void* counters,
+                         void* workspace, size_t workspace_bytes, void* stream) {
   if (window <= 0) return NSV_ERR_ARG;
   return row_attention(out, q, k_cache, v_cache, nullptr, block_tables, context_lens, cu_seqlens_q, positions, scale, B,
-                       T, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, window, sinks, false, workspace,
+                       T, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, window, sinks, false, (unsigned*)counters, workspace,
                        workspace_bytes, stream);
 }
 
@@ -905,8 +1002,8 @@ int nsv_weights_attention(void* out, const void* q, const void* k_cache, const v
                           int max_blocks, int max_q_len, int dtype, void* workspace, size_t workspace_bytes,
                           void* stream) {
   return row_attention(out, q, k_cache, v_cache, key_weights, block_tables, context_lens, cu_seqlens_q, positions, scale,
-                       B, T, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, 0, 0, true, workspace, workspace_bytes,
-                       stream);
+                       B, T, H, Hkv, D, block_size, max_blocks, max_q_len, dtype, 0, 0, true, nullptr, workspace,
+                       workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -281,7 +281,8 @@ def paged_attention_window(
     between the sinks and the windows may be given to other sequences (their
     entries any value, -1 included).  A row that sees no key, and a row at
     position -1, comes back as zeros.  Scratch comes from torch's allocator,
-    so calls on several streams, and captured ones, share nothing.
+    arrival counters are the stream's own (a captured call uses none): calls
+    on several streams, and captured ones, share nothing.
     No counterpart in the reference, whose attention sees every key."""
     window, sinks = _int_arg(window, "window", 1), _int_arg(sinks, "sinks", 0)
     query, block_tables, context_lens, cu_seqlens_q, positions, out = _few_rows(
@@ -294,10 +295,11 @@ def paged_attention_window(
     with _lib.on_device(dev):
         ws_bytes = _window_workspace_bytes(B, *shape)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        stream = _lib.stream_ptr(dev)
         rc = _lib.lib().nsv_window_attention(
             out.data_ptr(), query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
             context_lens.data_ptr(), cu_seqlens_q.data_ptr(), positions.data_ptr(), scale, B, query.shape[0], *shape,
-            ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+            _lib.stream_counters(dev, stream), ws.data_ptr(), ws_bytes, stream)
     _lib.check(rc, "paged_attention_window")
     return out
 

@@ -17,7 +17,7 @@ def test_row_attention_codes():
 
     def window(B=2, T=2, H=16, Hkv=8, D=128, bs=16, mb=4, mq=1, dt=1, window=8, sinks=0, ws=None, size=0, ptr=16):
         return h.nsv_window_attention(ptr, ptr, ptr, ptr, ptr, ptr, ptr, ptr, 0.1, B, T, H, Hkv, D, bs, mb, mq, dt, window,
-                                      sinks, ws, size, None)
+                                      sinks, None, ws, size, None)
 
     def weights(B=2, T=2, H=16, Hkv=8, D=128, bs=16, mb=4, mq=1, dt=1, w=16, ws=None, size=0):
         return h.nsv_weights_attention(16, 16, 16, 16, w, 16, 16, 16, 16, 0.1, B, T, H, Hkv, D, bs, mb, mq, dt, ws, size,
