@@ -344,17 +344,27 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
 #pragma unroll
     for (int d = 0; d < NACC; ++d) acc[mt][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  float row_m[MT], row_inv[MT];  // kWeights: the rows' maxima and 1 / their sums (0: a row that sees nothing)
+  // kWeights: S = Q K^T instead, so that a lane holds one key (c) and rows
+  // 16 mt + 4 g + i, which it adds up in registers; the rows' maxima, 1 / their
+  // sums (+inf and 0: a row that sees nothing, whose weights are then 0) and
+  // positions
+  float row_m[MT][4], row_inv[MT][4];
+  int row_pos[MT][4];
   if constexpr (MODE == kWeights) {
     join_stats(a, pair * a.subsets + sub, a.R, lds.row);
     __syncthreads();
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      const int m = mt * 16 + c;
-      const float2 x = m < a.R ? lds.row[m] : make_float2(0.f, 0.f);
-      row_m[mt] = x.x;
-      row_inv[mt] = x.y;
-    }
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int m = mt * 16 + g * 4 + i;
+        const float2 x = m < a.R ? lds.row[m] : make_float2(0.f, 0.f);
+        const int t = m - m / a.QL * a.QL;
+        const int p = __shfl(my_pos, t & 63, 64);
+        row_pos[mt][i] = m < a.R && t < qlen ? p : -1;
+        row_inv[mt][i] = x.y;
+        row_m[mt][i] = x.y > 0.f ? x.x : __builtin_inff();
+      }
   }
 
   // scores of a tile: element i of s[mt][u] is key 16 u + 4 g + i, row c
@@ -375,20 +385,23 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       for (int j = 0; j < S_::QV; ++j)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
+          const u32x4 x = V ? ka[j] : q[mt][j], y = V ? q[mt][j] : ka[j];
           if constexpr (BF16) {
-            s[mt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(ka[j]), as_bf16x8(q[mt][j]), s[mt][u], 0, 0, 0);
+            s[mt][u] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(x), as_bf16x8(y), s[mt][u], 0, 0, 0);
           } else {
-            const f32x4 kf = __builtin_bit_cast(f32x4, ka[j]), qf = __builtin_bit_cast(f32x4, q[mt][j]);
+            const f32x4 xf = __builtin_bit_cast(f32x4, x), yf = __builtin_bit_cast(f32x4, y);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              s[mt][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[e], qf[e], s[mt][u], 0, 0, 0);
+              s[mt][u] = __builtin_amdgcn_mfma_f32_16x16x4f32(xf[e], yf[e], s[mt][u], 0, 0, 0);
           }
         }
     }
+    if constexpr (V) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-      for (int u = 0; u < KT; ++u) s[mt][u] *= a.scale_log2;
+        for (int u = 0; u < KT; ++u) s[mt][u] *= a.scale_log2;
+    }
   };
   auto mask = [&](int tile) {
     const int vt = c0 + tile * TK;
@@ -491,7 +504,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     for (int t = w; t < ntiles; t += kWaves) {
       landed(t + kWaves < ntiles);
       scores(ktile(buf));
-      mask(t);
+      if constexpr (V) mask(t);
       if constexpr (MODE == kAttendScores) {
         const int vt = c0 + t * TK;
 #pragma unroll
@@ -506,29 +519,28 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       if constexpr (V) {
         attend(vtile(buf));
       } else {
-        // weights of 16 u + 4 g + i summed over the rows: a register sum over the
-        // row tiles, then over the group's 16 lanes
-        float x[KT * 4];
+        const int vt = c0 + t * TK;
+        // uniform: every row sees every key (a key past the run's last, or unmapped, is not written)
+        const bool all = min(vt + TK, c1) - 1 <= sp.pos_min;
+        float sum[KT];
 #pragma unroll
-        for (int u = 0; u < KT; ++u)
+        for (int u = 0; u < KT; ++u) {
+          sum[u] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            float y = 0.f;
+          for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-              y = pos[mt] >= 0 ? fmaf(__builtin_amdgcn_exp2f(s[mt][u][i] - row_m[mt]), row_inv[mt], y) : y;
-            y += dpp_f32<kDppXor1>(y);
-            y += dpp_f32<kDppXor2>(y);
-            y += dpp_f32<kDppHalfMirror>(y);
-            x[u * 4 + i] = y + dpp_f32<kDppMirror>(y);
-          }
-        float y = x[0];
-#pragma unroll
-        for (int e = 1; e < KT * 4; ++e) y = c == e ? x[e] : y;
-        const int v = c0 + t * TK + (c >> 2) * 16 + g * 4 + (c & 3);
-        if (c < KT * 4 && v < c1) {
+            for (int i = 0; i < 4; ++i) {
+              const float e = __builtin_amdgcn_exp2f(fmaf(s[mt][u][i], a.scale_log2, -row_m[mt][i]));
+              const float y = fmaf(e, row_inv[mt][i], sum[u]);
+              sum[u] = all || vt + u * 16 + c <= row_pos[mt][i] ? y : sum[u];
+            }
+          sum[u] = groups_sum(sum[u]);
+        }
+        const int v = vt + g * 16 + c;  // lane (g, c) of the first KT groups writes the key of tile g
+        if (g < KT && v < c1) {
           const int p = page(v, true);
           if (p >= 0) {
+            const float y = KT == 1 || g == 0 ? sum[0] : sum[KT - 1];
             float* dst = a.key_weights + ((int64_t)p * a.Hkv + hk) * (bs_mask + 1) + (v & bs_mask);
             if (v >= sp.pos_min && sub == 0) *dst = y;
             else unsafeAtomicAdd(dst, y);
