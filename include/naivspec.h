@@ -264,13 +264,18 @@ int nsv_prefill_key_weights(const void* q, const void* k_cache,
  * Every page of a context must be mapped, and out_block_tables holds no page
  * of block_tables at another place.  Supported: rows of a multiple of 64
  * bytes; block_size a power of two; sinks + recent <= budget.
+ * Workspace: nsv_evict_workspace_size() bytes on 16 bytes (0: none; apart:
+ * whether out_block_tables will be another table), of any content.
  */
+size_t nsv_evict_workspace_size(int B, int Hkv, int D, int block_size,
+                                int max_blocks, int apart, int dtype,
+                                int budget);
 int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights,
                  const int32_t* block_tables, const int64_t* context_lens,
                  const int32_t* out_block_tables, int64_t* lens, int32_t* kept,
                  int B, int Hkv, int D, int block_size, int max_blocks,
                  int out_blocks, int dtype, int budget, int sinks, int recent,
-                 void* stream);
+                 void* workspace, size_t workspace_bytes, void* stream);
 
 /*
  * Load-only measurement kernels, no reference counterpart (the ceilings

@@ -54,7 +54,8 @@ SIGNATURES: dict[str, tuple] = {
     "nsv_key_weights_units": (_c_int, [_c_vp] * 2 + [_c_int] * 4 + [_c_vp, _c_i64, _c_vp]),
     "nsv_prefill_key_weights": (
         _c_int, [_c_vp] * 6 + [_c_int, _c_vp, _c_int, _c_f32] + [_c_int] * 5 + [_c_vp] * 2),
-    "nsv_evict_kv": (_c_int, [_c_vp] * 8 + [_c_int] * 10 + [_c_vp]),
+    "nsv_evict_workspace_size": (_c_size, [_c_int] * 8),
+    "nsv_evict_kv": (_c_int, [_c_vp] * 8 + [_c_int] * 10 + [_c_vp, _c_size, _c_vp]),
     "nsv_window_attention_workspace_size": (_c_size, [_c_int] * 10),
     "nsv_window_attention": (
         _c_int, [_c_vp] * 8 + [_c_f32] + [_c_int] * 11 + [_c_vp, _c_vp, _c_size, _c_vp]),

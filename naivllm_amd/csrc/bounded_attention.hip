@@ -140,30 +140,34 @@ __device__ __forceinline__ int split_keys(int total, int S) {
   return max((per + TK - 1) / TK * TK, TK * kWaves);
 }
 
-// A row's maximum and 1 / sum over its splits, for `rows` rows from (pair, head
-// subset) ps on, into LDS (a barrier follows): a lane per split.  A row that
-// sees nothing: 0 and 0.
+// A row's maximum and 1 / sum over its splits, for `rows` <= 64 rows from (pair,
+// head subset) ps on, into LDS (a barrier follows): four neighbouring lanes per
+// row, each with every fourth split, all of them loaded in one round trip (a
+// wave per row and a lane per split took 14 us for 64 rows).  A row that sees
+// nothing: 0 and 0.
 __device__ __forceinline__ void join_stats(const RowArgs& a, int ps, int rows, float2* stat) {
-  constexpr int CH = 4;  // rows per round trip of a wave
-  const int lane = threadIdx.x & 63;
-  for (int m0 = threadIdx.x >> 6; m0 < rows; m0 += CH * kWaves) {
-    float2 x[CH];
+  constexpr int N = kMaxSplits / 4;
+  const int j = threadIdx.x & 3, m = threadIdx.x >> 2;
+  const int row = min(m, rows - 1), sub = row / a.R;  // (rows may run on into the pair's next subsets)
+  const float2* src = a.part_ml + (int64_t)(ps + sub) * a.S * a.R + row - sub * a.R;
+  float2 x[N];
 #pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const int m = min(m0 + k * kWaves, rows - 1);
-      const int sub = m / a.R;  // (rows may run on into the pair's next subsets)
-      x[k] = a.part_ml[((int64_t)(ps + sub) * a.S + min(lane, a.S - 1)) * a.R + m - sub * a.R];
-    }
-#pragma unroll
-    for (int k = 0; k < CH; ++k) {
-      const int m = m0 + k * kWaves;
-      if (m >= rows) break;  // uniform
-      const float M = wave_max(x[k].x);
-      const float ref = M == kNegInf ? 0.f : M;
-      const float L = wave_sum(lane < a.S ? x[k].y * __builtin_amdgcn_exp2f(x[k].x - ref) : 0.f);
-      if (lane == 0) stat[m] = make_float2(ref, L > 0.f ? 1.f / L : 0.f);
-    }
+  for (int k = 0; k < N; ++k) {
+    x[k] = make_float2(kNegInf, 0.f);
+    if (4 * k < a.S) x[k] = src[(int64_t)min(4 * k + j, a.S - 1) * a.R];  // uniform
   }
+  float M = kNegInf, L = 0.f;
+#pragma unroll
+  for (int k = 0; k < N; ++k) M = fmaxf(M, x[k].x);  // (a split read twice changes nothing here)
+  M = fmaxf(M, dpp_f32<kDppXor1>(M));
+  M = fmaxf(M, dpp_f32<kDppXor2>(M));
+  const float ref = M == kNegInf ? 0.f : M;
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    if (4 * k < a.S) L += 4 * k + j < a.S ? x[k].y * __builtin_amdgcn_exp2f(x[k].x - ref) : 0.f;
+  L += dpp_f32<kDppXor1>(L);
+  L += dpp_f32<kDppXor2>(L);
+  if (j == 0 && m < rows) stat[m] = make_float2(ref, L > 0.f ? 1.f / L : 0.f);
 }
 
 template <typename T, int DH>
@@ -769,28 +773,30 @@ __device__ __forceinline__ void merge_rows(const RowArgs& a, int ps, int block, 
 
 constexpr int kMaxStoredRows = 64;
 
+// CH: rows whose scores are loaded in a round trip.
+template <int CH>
 __device__ __forceinline__ void stored_weights(const RowArgs& a, int pair, int block) {
   __shared__ float2 stat[kMaxStoredRows];  // maximum and 1 / sum
   const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
-  const int q0 = uniform(a.cu_seqlens_q[b]);
-  const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
-  int my_pos;
-  const Span sp = make_span(a, b, q0, qlen, my_pos);
-  if (block * 256 >= sp.total) return;  // uniform
+  if (block * 256 >= a.context_lens[b]) return;  // uniform
+  // the scores, the page and the statistics, in one round trip beside the sequence's rows' positions
   const int key = block * 256 + threadIdx.x, rows = a.R * a.subsets;
-  const int p = key < sp.total ? a.block_tables[(int64_t)b * a.max_blocks + (key >> a.bs_log2)] : -1;
-  // (a chunk of rows' scores per round trip, the first beside the statistics'; behind the last key: key 0's again)
-  constexpr int CH = 16;
-  const float* src = a.scores + (int64_t)pair * rows * a.score_keys + (p < 0 ? 0 : key);
+  const float* src = a.scores + (int64_t)pair * rows * a.score_keys + min(key, a.score_keys - 1);
   float s[CH];
   auto read = [&](int m0) {
 #pragma unroll
-    for (int k = 0; k < CH; ++k) s[k] = m0 + k < rows ? src[(int64_t)(m0 + k) * a.score_keys] : 0.f;  // (uniform)
+    for (int k = 0; k < CH; ++k) s[k] = src[(int64_t)min(m0 + k, rows - 1) * a.score_keys];
   };
   read(0);
+  const int entry = min(key >> a.bs_log2, a.max_blocks - 1);
+  const int p = a.block_tables[(int64_t)b * a.max_blocks + entry];
+  const int q0 = uniform(a.cu_seqlens_q[b]);
+  const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
   join_stats(a, pair * a.subsets, rows, stat);
+  int my_pos;
+  const Span sp = make_span(a, b, q0, qlen, my_pos);
   __syncthreads();
-  if (p < 0) return;
+  if (key >= sp.total || p < 0) return;
   float y = 0.f;
   for (int m0 = 0; m0 < rows; m0 += CH) {
     if (m0 > 0) read(m0);
@@ -811,7 +817,8 @@ __global__ __launch_bounds__(256) void row_finish_kernel(RowArgs a, int merges, 
     const int pair = blockIdx.x / a.subsets;  // (x: pairs x subsets for these, the rest of the grid's rows use pairs)
     if (pair < a.npairs) merge_rows<T, DH>(a, blockIdx.x, blockIdx.y, sg_log2);
   } else if ((int)blockIdx.x < a.npairs) {
-    stored_weights(a, blockIdx.x, blockIdx.y - merges);
+    if (a.R * a.subsets <= 4) stored_weights<4>(a, blockIdx.x, blockIdx.y - merges);  // uniform
+    else stored_weights<32>(a, blockIdx.x, blockIdx.y - merges);
   }
 }
 

@@ -24,7 +24,8 @@
 // ascending chunks, each read whole before it is written and the next one's
 // reads under way: what a chunk overwrites no later chunk reads, and no other
 // workgroup touches the column.  Between tables apart nothing can be
-// overwritten, and the rows are dealt to many workgroups.  Bound by the rows'
+// overwritten, and the rows are dealt to many workgroups; so they are where few
+// sequences have long rows to move, by way of staging rows.  Bound by the rows'
 // bytes.
 
 #include "common.h"
@@ -51,6 +52,7 @@ struct EvictArgs {
   int32_t* kept;                 // [B][Hkv][budget]
   int Hkv, row_bytes, bs_log2, max_blocks, out_blocks, budget, sinks, recent;
   int vector;                    // four weights of a page in one load
+  char* staged;                  // null, or [B][Hkv][2][budget] rows: K, V by way of it
 };
 
 __device__ __forceinline__ int clamp_len(const EvictArgs& a, int b) {
@@ -320,7 +322,11 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   }
 }
 
-// grid: (sequence, kv head, column) x (K, V) x rows (1 workgroup in place)
+// grid: (sequence, kv head, column) x (K, V) x rows (1 workgroup in place).
+// TO_STAGED: kept rows to the staging rows; FROM_STAGED: those to the table;
+// neither: at once.
+enum Move { kAtOnce, kToStaged, kFromStaged };
+template <Move MOVE>
 __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, int lanes_log2) {
   const int lanes = 1 << lanes_log2;               // 16-byte pieces per row and column
   const int rows = kMoveThreads >> lanes_log2;     // rows that a step of the workgroup takes
@@ -334,7 +340,9 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
   const int32_t* bt = a.block_tables + (int64_t)b * a.max_blocks;
   const int32_t* ot = a.out_tables + (int64_t)b * a.out_blocks;
   const int32_t* kept = a.kept + ((int64_t)b * a.Hkv + h) * a.budget;
-  char* base = (blockIdx.y ? a.v : a.k) + (int64_t)h * a.row_bytes + (column * lanes + (threadIdx.x & (lanes - 1))) * 16;
+  const int piece = (column * lanes + (threadIdx.x & (lanes - 1))) * 16;
+  char* base = (blockIdx.y ? a.v : a.k) + (int64_t)h * a.row_bytes + piece;
+  char* staged = a.staged + (((int64_t)b * a.Hkv + h) * 2 + blockIdx.y) * a.budget * a.row_bytes + piece;
   const int64_t stride = (int64_t)a.Hkv * a.row_bytes;
   const int r = threadIdx.x >> lanes_log2;
   auto row = [&](const int32_t* table, int key) -> char* {
@@ -351,7 +359,8 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
       const int i = i0 + u * rows + r;
-      src[u] = i < got ? row(bt, kept[i]) : nullptr;
+      src[u] = i < got ? row(bt, kept[i]) : nullptr;  // (a row without a page does not move)
+      if (MOVE == kFromStaged && src[u]) src[u] = staged + (int64_t)i * a.row_bytes;
     }
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
@@ -364,12 +373,13 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
       const int i = i0 + u * rows + r;
-      char* dst = c.on[u] ? row(ot, i) : nullptr;
+      char* dst = nullptr;
+      if (c.on[u]) dst = MOVE == kToStaged ? staged + (int64_t)i * a.row_bytes : row(ot, i);
       if (dst) __builtin_nontemporal_store(c.x[u], reinterpret_cast<u32x4*>(dst));
     }
   };
   Chunk c;
-  if (apart) {
+  if (apart || MOVE != kAtOnce) {
     for (int i0 = blockIdx.z * chunk; i0 < got; i0 += gridDim.z * chunk) {
       read(c, i0);
       write(c, i0);
@@ -389,48 +399,97 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
   }
 }
 
+// How the rows move: `lanes_log2` of a column; rows staged, or at once; grid z.
+struct MovePlan {
+  int lanes_log2, z;
+  size_t staged;
+};
+
+MovePlan plan_move(int B, int Hkv, int row_bytes, int64_t cap, int budget, bool apart) {
+  const int64_t most = std::min<int64_t>(cap, budget), units = (int64_t)B * Hkv * 2;
+  MovePlan p{2, 1, 0};
+  // a row's pieces to one workgroup where the (sequence, head, K or V)s fill the
+  // chip (whole lines, one read of the page and position lists), or the rows
+  // are dealt to several; else down to 64 bytes
+  auto widen = [&](int64_t least) {
+    while (p.lanes_log2 < 5 && row_bytes % (32 << p.lanes_log2) == 0 && units * (row_bytes / (32 << p.lanes_log2)) >= least)
+      ++p.lanes_log2;
+  };
+  auto chunk = [&] { return (int64_t)(kMoveThreads >> p.lanes_log2) * kMoveUnroll; };
+  widen(apart ? 0 : 256);
+  // In place, few workgroups take many chunks one after another, each a chain
+  // of three round trips: past two chunks by way of staging rows, which any
+  // number of workgroups may fill and empty (twice the bytes, a third launch).
+  // 3 sequences of 8 heads, 4,205 rows of 128 bytes: 44 us at once.  Not where
+  // the workgroups fill the chip.
+  const int64_t columns = row_bytes / (16 << p.lanes_log2);
+  if (!apart && units * columns < 256 && most > 2 * chunk()) {
+    p.staged = (size_t)units * budget * row_bytes;
+    widen(0);
+  }
+  if (apart || p.staged) p.z = (int)std::min<int64_t>((most + chunk() - 1) / chunk(), 64);
+  return p;
+}
+
+int64_t evict_cap(int block_size, int max_blocks) { return (int64_t)max_blocks * block_size; }
+
+int evict_args(int B, int Hkv, int D, int block_size, int max_blocks, int out_blocks, bool apart, int dtype, int budget,
+               int sinks, int recent) {
+  if (B < 0 || Hkv <= 0 || D <= 0 || max_blocks <= 0 || budget <= 0 || sinks < 0 || recent < 0) return NSV_ERR_ARG;
+  if (dtype != NSV_F32 && dtype != NSV_BF16) return NSV_ERR_ARG;
+  if ((int64_t)sinks + recent > budget || (apart && out_blocks <= 0)) return NSV_ERR_ARG;
+  const int64_t row_bytes = (int64_t)D * (dtype == NSV_BF16 ? 2 : 4), cap = evict_cap(block_size, max_blocks);
+  if (block_size <= 0 || (block_size & (block_size - 1)) || row_bytes % 64 || row_bytes > 65536) return NSV_ERR_UNSUPPORTED;
+  if (cap > (int64_t)1 << 30 || (int64_t)B * Hkv * (row_bytes / 64) > 0x7fffffff) return NSV_ERR_UNSUPPORTED;
+  if (apart && (int64_t)out_blocks * block_size < std::min<int64_t>(cap, budget)) return NSV_ERR_ARG;
+  return NSV_OK;
+}
+
 }  // namespace
 
 extern "C" {
 
+size_t nsv_evict_workspace_size(int B, int Hkv, int D, int block_size, int max_blocks, int apart, int dtype, int budget) {
+  if (evict_args(B, Hkv, D, block_size, max_blocks, max_blocks, false, dtype, budget, 0, 0) != NSV_OK) return 0;
+  return plan_move(B, Hkv, D * (dtype == NSV_BF16 ? 2 : 4), evict_cap(block_size, max_blocks), budget, apart != 0).staged;
+}
+
 int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights, const int32_t* block_tables,
                  const int64_t* context_lens, const int32_t* out_block_tables, int64_t* lens, int32_t* kept, int B,
                  int Hkv, int D, int block_size, int max_blocks, int out_blocks, int dtype, int budget, int sinks,
-                 int recent, void* stream) {
-  if (B < 0 || Hkv <= 0 || D <= 0 || max_blocks <= 0 || budget <= 0 || sinks < 0 || recent < 0) return NSV_ERR_ARG;
-  if (dtype != NSV_F32 && dtype != NSV_BF16) return NSV_ERR_ARG;
-  if ((int64_t)sinks + recent > budget || (out_block_tables && out_blocks <= 0)) return NSV_ERR_ARG;
-  const int row_bytes = D * (dtype == NSV_BF16 ? 2 : 4);
-  if (block_size <= 0 || (block_size & (block_size - 1)) || row_bytes % 64) return NSV_ERR_UNSUPPORTED;
-  const int64_t cap = (int64_t)max_blocks * block_size;
-  if (cap > (int64_t)1 << 30 || (int64_t)B * Hkv * (row_bytes / 64) > 0x7fffffff) return NSV_ERR_UNSUPPORTED;
-  if (out_block_tables && (int64_t)out_blocks * block_size < std::min<int64_t>(cap, budget)) return NSV_ERR_ARG;
+                 int recent, void* workspace, size_t workspace_bytes, void* stream) {
+  const bool apart = out_block_tables && out_block_tables != block_tables;
+  const int bad = evict_args(B, Hkv, D, block_size, max_blocks, out_blocks, out_block_tables != nullptr, dtype, budget, sinks,
+                             recent);
+  if (bad != NSV_OK) return bad;
   if (B == 0) return NSV_OK;
   if (!k_cache || !v_cache || !key_weights || !block_tables || !context_lens || !lens || !kept) return NSV_ERR_ARG;
-  if (((uintptr_t)k_cache | (uintptr_t)v_cache) % 16) return NSV_ERR_ARG;
+  if (((uintptr_t)k_cache | (uintptr_t)v_cache | (uintptr_t)workspace) % 16) return NSV_ERR_ARG;
+  const int row_bytes = D * (dtype == NSV_BF16 ? 2 : 4);
+  const int64_t cap = evict_cap(block_size, max_blocks);
+  const MovePlan p = plan_move(B, Hkv, row_bytes, cap, budget, apart);
+  if (p.staged && (!workspace || workspace_bytes < p.staged)) return NSV_ERR_WORKSPACE;
   int bs_log2 = 0;
   while ((1 << bs_log2) < block_size) ++bs_log2;
-  EvictArgs a{(char*)k_cache, (char*)v_cache, key_weights, block_tables, out_block_tables ? out_block_tables : block_tables,
-              context_lens, lens, kept, Hkv, row_bytes, bs_log2, max_blocks, out_block_tables ? out_blocks : max_blocks,
-              budget, sinks, recent, bs_log2 >= 2 && (uintptr_t)key_weights % 16 == 0};
+  EvictArgs a{(char*)k_cache, (char*)v_cache, key_weights, block_tables, apart ? out_block_tables : block_tables,
+              context_lens, lens, kept, Hkv, row_bytes, bs_log2, max_blocks, apart ? out_blocks : max_blocks,
+              budget, sinks, recent, bs_log2 >= 2 && (uintptr_t)key_weights % 16 == 0, (char*)workspace};
   hipStream_t s = (hipStream_t)stream;
   if (cap <= (int64_t)kSelThreads * 4 * kSelLoads)
     hipLaunchKernelGGL(evict_select_kernel<true>, dim3(B * Hkv), dim3(kSelThreads), 0, s, a);
   else
     hipLaunchKernelGGL(evict_select_kernel<false>, dim3(B * Hkv), dim3(kSelThreads), 0, s, a);
-  const int rc = nsv_launch_status();
+  int rc = nsv_launch_status();
   if (rc) return rc;
-  // a row's pieces to one workgroup where the (sequence, head, K or V)s fill the chip (whole lines, one read of the
-  // page and position lists), else down to 64 bytes
-  int lanes_log2 = 2;
-  while (lanes_log2 < 5 && row_bytes % (32 << lanes_log2) == 0 &&
-         (a.out_tables != block_tables || (int64_t)B * Hkv * 2 * (row_bytes / (32 << lanes_log2)) >= 256))
-    ++lanes_log2;
-  const int columns = row_bytes / (16 << lanes_log2);
-  const int chunk = (kMoveThreads >> lanes_log2) * kMoveUnroll;
-  const int64_t most = std::min<int64_t>(cap, budget);
-  const int z = a.out_tables != block_tables ? (int)std::min<int64_t>((most + chunk - 1) / chunk, 64) : 1;
-  hipLaunchKernelGGL(evict_move_kernel, dim3(B * Hkv * columns, 2, z), dim3(kMoveThreads), 0, s, a, lanes_log2);
+  const dim3 grid(B * Hkv * (row_bytes / (16 << p.lanes_log2)), 2, p.z);
+  if (p.staged) {
+    hipLaunchKernelGGL(evict_move_kernel<kToStaged>, grid, dim3(kMoveThreads), 0, s, a, p.lanes_log2);
+    rc = nsv_launch_status();
+    if (rc) return rc;
+    hipLaunchKernelGGL(evict_move_kernel<kFromStaged>, grid, dim3(kMoveThreads), 0, s, a, p.lanes_log2);
+  } else {
+    hipLaunchKernelGGL(evict_move_kernel<kAtOnce>, grid, dim3(kMoveThreads), 0, s, a, p.lanes_log2);
+  }
   return nsv_launch_status();
 }
 

@@ -241,6 +241,11 @@ def _window_workspace_bytes(*shape: int) -> int:
 
 
 @functools.lru_cache(maxsize=512)
+def _evict_workspace_bytes(*shape: int) -> int:
+    return int(_lib.lib().nsv_evict_workspace_size(*shape))
+
+
+@functools.lru_cache(maxsize=512)
 def _weights_workspace_bytes(*shape: int) -> int:
     return int(_lib.lib().nsv_weights_attention_workspace_size(*shape))
 
@@ -730,12 +735,15 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: tor
         out_block_tables = _as(out_block_tables, "block_tables")
     lens = torch.empty(B, dtype=torch.int64, device=dev)
     kept = torch.empty((B, hkv, budget), dtype=torch.int32, device=dev)
+    code = _lib.dtype_code(k_cache.dtype)
     with _lib.on_device(dev):
+        ws_bytes = _evict_workspace_bytes(B, hkv, d, bs, max_blocks, int(out_block_tables is not None), code, budget)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         rc = _lib.lib().nsv_evict_kv(
             k_cache.data_ptr(), v_cache.data_ptr(), key_weights.data_ptr(), block_tables.data_ptr(),
             context_lens.data_ptr(), _lib.ptr(out_block_tables), lens.data_ptr(), kept.data_ptr(), B, hkv, d, bs,
-            max_blocks, 0 if out_block_tables is None else out_block_tables.shape[1], _lib.dtype_code(k_cache.dtype),
-            budget, sinks, recent, _lib.stream_ptr(dev))
+            max_blocks, 0 if out_block_tables is None else out_block_tables.shape[1], code, budget, sinks, recent,
+            _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
     _lib.check(rc, "evict_kvcache")
     return lens, kept
 

@@ -38,14 +38,19 @@ def test_row_attention_codes():
 def test_evict_codes():
     h = _lib.lib()
 
-    def evict(B=1, Hkv=2, D=64, bs=16, mb=4, ob=0, dt=1, budget=8, sinks=0, recent=0, out=None, k=16):
-        return h.nsv_evict_kv(k, 16, 16, 16, 16, out, 16, 16, B, Hkv, D, bs, mb, ob, dt, budget, sinks, recent, None)
+    def evict(B=1, Hkv=2, D=64, bs=16, mb=4, ob=0, dt=1, budget=8, sinks=0, recent=0, out=None, k=16, ws=None):
+        return h.nsv_evict_kv(k, 16, 16, 16, 16, out, 16, 16, B, Hkv, D, bs, mb, ob, dt, budget, sinks, recent, ws, 64,
+                              None)
 
     assert evict(B=0) == 0
     assert evict(B=-1) == evict(budget=0) == evict(sinks=-1) == evict(recent=-1) == evict(dt=3) == evict(k=None) == -1
     assert evict(sinks=5, recent=4) == evict(k=24) == -1
     assert evict(out=16, ob=0) == evict(out=16, ob=1, budget=40) == -1  # no room for what stays
     assert evict(D=40) == evict(bs=24) == evict(mb=1 << 27) == -2
+    assert evict(mb=600, budget=8192) == evict(mb=600, budget=8192, ws=16) == -3  # rows by way of a workspace
+    assert h.nsv_evict_workspace_size(1, 2, 64, 16, 600, 0, 1, 8192) == 2 * 2 * 8192 * 128
+    assert h.nsv_evict_workspace_size(1, 2, 64, 16, 600, 1, 1, 8192) == 0
+    assert h.nsv_evict_workspace_size(16, 8, 128, 256, 128, 0, 1, 2048) == 0
 
 
 def test_prefill_key_weights_codes():

@@ -89,6 +89,13 @@ def test_pages_apart_leave_the_old_ones():
     _check(k, v, w, tables, lens, 200, 4, 30, out)
 
 
+@pytest.mark.parametrize("Hkv,D", [(2, 64), (1, 128)])
+def test_many_rows_of_few_sequences(Hkv, D):
+    print(f"case: evict by way of staging rows {Hkv} {D}", flush=True)
+    lens = [9000, 5000, 8193]
+    _check(*_case(78, lens, Hkv, D, 64)[:4], lens, 5000, 4, 100)
+
+
 def test_a_long_context():
     print("case: evict 70000 keys", flush=True)
     lens = [70000, 40000]
