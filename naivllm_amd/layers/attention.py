@@ -469,6 +469,13 @@ class _StepList:
             stream.wait_event(self.ready)
         self.work.record_stream(stream)
 
+    def use_here(self, device: torch.device) -> int:
+        """use_on the device's current stream; returns its handle."""
+        stream = _lib.stream_ptr(device)
+        if stream != self.stream:
+            self.use_on(torch.cuda.current_stream(device))
+        return stream
+
 
 def _send_ahead() -> bool:
     """As _lib.upload: a step's transfer is not waited for, except inside a
@@ -621,15 +628,15 @@ def prefill_attention(query: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pla
     out = torch.empty_like(query)
     # (the plan's list is the only memory that calls on several streams or
     # threads share, and they only read it)
-    stream = torch.cuda.current_stream(query.device)
-    plan.use_on(stream)
-    part = torch.empty(plan.slots * H * plan.tile_rows * (head_dim + 2), dtype=torch.float32,
-                       device=query.device) if plan.slots else None
-    tiles = plan.work.data_ptr()
-    rc = _lib.lib().nsv_prefill_window_attention(
-        out.data_ptr(), query.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(block_tables), tiles, plan.ntiles,
-        plan.tile_rows, tiles + plan.ntiles * 32, plan.nmerges, float(scale), H, Hkv, head_dim,
-        plan.block_size or 1, max_blocks, plan.window, plan.sinks, _lib.ptr(stats), _lib.ptr(part), stream.cuda_stream)
+    with _lib.on_device(query.device):
+        stream = plan.use_here(query.device)
+        part = torch.empty(plan.slots * H * plan.tile_rows * (head_dim + 2), dtype=torch.float32,
+                           device=query.device) if plan.slots else None
+        tiles = plan.work.data_ptr()
+        rc = _lib.lib().nsv_prefill_window_attention(
+            out.data_ptr(), query.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(block_tables), tiles, plan.ntiles,
+            plan.tile_rows, tiles + plan.ntiles * 32, plan.nmerges, float(scale), H, Hkv, head_dim,
+            plan.block_size or 1, max_blocks, plan.window, plan.sinks, _lib.ptr(stats), _lib.ptr(part), stream)
     _lib.check(rc, "prefill_attention")
     return out
 
@@ -673,15 +680,14 @@ def prefill_key_weights(query: torch.Tensor, k_cache: torch.Tensor, key_weights:
     if block_tables.shape[1] * plan.block_size < plan.longest:
         raise ValueError(f"block tables of {block_tables.shape[1]} pages for sequences of up to {plan.longest} keys")
     query = _aligned(query.contiguous())
-    stream = torch.cuda.current_stream(query.device)
     with _lib.on_device(query.device):
-        plan.use_on(stream)
+        stream = plan.use_here(query.device)
         part = torch.empty(plan.nunits * Hkv * 256, dtype=torch.float32, device=query.device)
         units = plan.work.data_ptr()
         rc = _lib.lib().nsv_prefill_key_weights(
             query.data_ptr(), k_cache.data_ptr(), key_weights.data_ptr(), stats.data_ptr(), block_tables.data_ptr(), units,
             plan.nunits, units + plan.nunits * 32, plan.nsums, float(scale), H, Hkv, head_dim, plan.block_size,
-            block_tables.shape[1], part.data_ptr(), stream.cuda_stream)
+            block_tables.shape[1], part.data_ptr(), stream)
     _lib.check(rc, "prefill_key_weights")
 
 
