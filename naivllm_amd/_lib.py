@@ -178,8 +178,8 @@ def stream_counters(device: torch.device, stream: int) -> int | None:
     if torch.cuda.is_current_stream_capturing():
         return None
     buf = _counters.get((device.index, stream))
-    if buf is None:
-        buf = _counters[device.index, stream] = torch.zeros(16384, dtype=torch.int32, device=device)
+    if buf is None:  # (two threads at once: the first one's stays)
+        buf = _counters.setdefault((device.index, stream), torch.zeros(16384, dtype=torch.int32, device=device))
     return buf.data_ptr()
 
 

@@ -423,7 +423,7 @@ MovePlan plan_move(int B, int Hkv, int row_bytes, int64_t cap, int budget, bool 
   // 3 sequences of 8 heads, 4,205 rows of 128 bytes: 44 us at once.  Not where
   // the workgroups fill the chip.
   const int64_t columns = row_bytes / (16 << p.lanes_log2);
-  if (!apart && units * columns < 256 && most > 2 * chunk()) {
+  if (!apart && budget < cap && units * columns < 256 && most > 2 * chunk()) {
     p.staged = (size_t)units * budget * row_bytes;
     widen(0);
   }

@@ -298,11 +298,8 @@ KeyTiling make_key_units(const int64_t* ql, const int64_t* kl, int n, int H, int
       for (int64_t k = 0; k < kl[b]; k += kBlockKeys) units += (tiles_of(b, k) + target - 1) / target;
     return units * Hkv;
   };
-  int64_t target = 2, above = 2;
-  while (units_of(above) > kRounds * 2 * (int64_t)cus && above < ((int64_t)1 << 40)) {
-    target = above + 1;
-    above *= 2;
-  }
+  int64_t target = 2, above = 2;  // (above: a block's most tiles, a part per block)
+  for (int b = 0; b < n; ++b) above = std::max(above, tiles_of(b, 0));
   while (target < above) {
     const int64_t mid = (target + above) / 2;
     if (units_of(mid) > kRounds * 2 * (int64_t)cus) target = mid + 1;

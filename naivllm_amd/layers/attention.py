@@ -223,6 +223,10 @@ def _check_few_rows(query, k_cache, v_cache, block_tables, context_lens, cu_seql
         out = torch.empty(query.shape, dtype=query.dtype, device=dev)
     elif out.shape != query.shape or out.dtype != query.dtype or out.device != dev or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {query.dtype} tensor of shape {tuple(query.shape)} on {dev}")
+    elif out.data_ptr() % 16:
+        raise ValueError("out must start on 16 bytes")
+    elif out.numel() and abs(out.data_ptr() - query.data_ptr()) < out.numel() * out.element_size():
+        raise ValueError("out must not overlap query")
     return (_aligned(query.contiguous()), _as(block_tables, "block_tables"), _as(context_lens, "context_lens"),
             _as(cu_seqlens_q, "cu_seqlens_q"), _as(positions, "positions"), out)
 
@@ -284,8 +288,9 @@ def paged_attention_window(
 
     Only keys that some row of their sequence sees are read, so the pages
     between the sinks and the windows may be given to other sequences (their
-    entries any value, -1 included).  A row that sees no key, and a row at
-    position -1, comes back as zeros.  Scratch comes from torch's allocator,
+    entries any value, -1 included), and what they hold (NaN, say) reaches no
+    result; a key that one row sees and another does not must be finite.  A row
+    that sees no key, and a row at position -1, comes back as zeros.  Scratch comes from torch's allocator,
     arrival counters are the stream's own (a captured call uses none): calls
     on several streams, and captured ones, share nothing.
     No counterpart in the reference, whose attention sees every key."""

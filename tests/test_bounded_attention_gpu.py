@@ -117,6 +117,27 @@ def test_window_positions_apart_and_contexts_short_of_them():
     _check_window(vb, 64, 2)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_sequences_without_rows(dtype):
+    print(f"case: sequences without rows {dtype}", flush=True)
+    vb = synth.verify_batch(40, [300, 50, 77, 10], [3, 0, 2, 0], dtype=dtype, block_size=16)
+    _check_window(vb, 40, 4)
+    _check_weights(vb)
+
+
+def test_scales_of_every_sign():
+    print("case: scales", flush=True)
+    vb = synth.verify_batch(44, [300], [3], dtype="f32", block_size=16)
+    t = to_device(vb)
+    for scale in (0.0, -0.09, 2.0):
+        want, want_abs, mag, _ = ob.attention(vb.q, vb.k_cache, vb.v_cache, vb.block_tables, vb.context_lens,
+                                              vb.cu_seqlens_q, vb.positions, scale, vb.num_kv_heads, 50, 2)
+        meta = _args(vb, t)
+        out = paged_attention_window(t["query"], t["k_cache"], t["v_cache"], *meta[:4], scale, *meta[5:], window=50,
+                                     sinks=2, max_q_len=3)
+        check_attention(out, want, want_abs, np.abs(mag), "f32", 60, f"scale {scale}")
+
+
 def test_window_rows_behind_the_last_sequence_stay():
     vb = synth.verify_batch(38, [100], [3], dtype="bf16", block_size=16)
     t = to_device(vb)

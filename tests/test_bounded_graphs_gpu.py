@@ -201,6 +201,10 @@ def test_refusals_on_the_gpu():
     refused("entries", window, meta[0], meta[1][:-1], *meta[2:])
     refused("on cpu", window, meta[0].cpu(), *meta[1:])
     refused("out must be", window, out=torch.empty_like(q, dtype=torch.float32))
+    refused("overlap", window, out=q)
+    refused("overlap", paged_attention_weights, q, k, v, w, *meta, out=q)
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device="cuda")[1:].view(q.shape)
+    refused("16 bytes", window, out=odd)
     refused("unsupported", window, max_q_len=65)
     refused("unsupported dtype", window, query=q.half(), kc=k.half(), vc=v.half())
     refused("key_weights must be", paged_attention_weights, q, k, v, w.double(), *meta)
