@@ -27,6 +27,12 @@
 // overwritten, and the rows are dealt to many workgroups; so they are where few
 // sequences have long rows to move, by way of staging rows.  Bound by the rows'
 // bytes.
+//
+// Measured on MI355X: one sequence, 1,250 -> 512 keys of 8 heads, bf16, D 128,
+// to pages apart: 10.5 us of selection, 5.5 of moving; 16 sequences of 16k-32k
+// -> 2,048 keys in place: 36 and 62 (268 MB read and written, 4.3 TB/s; a large
+// copy 4.8).  Before the words were held and the histograms cleared ahead the
+// selection took 13 and 50, with one serial scan per pass 43 and 128.
 
 #include "common.h"
 

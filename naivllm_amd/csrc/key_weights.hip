@@ -15,6 +15,13 @@
 // three deep.  The (head, row tile) list of a key block is cut into parts so
 // that the grid fills the chip; a second kernel adds the parts in their order
 // (no atomics between them: the sums do not depend on which part ends first).
+//
+// Measured on MI355X: 8,192 rows of 32/8 heads 320 us (860 TFLOP/s of the one
+// product; the products alone, without the sums, 163, the exponentials and sums
+// alone 267: they overlap in part only), 1,206 rows of 16/8 heads 14 + 4.  Not
+// better: both squares of 32 keys multiplied in turn (spills), 32 rows' operands
+// read a half ahead, units ordered by their rows for the L2, one workgroup per
+// compute unit (522).
 
 #include "common.h"
 

@@ -96,6 +96,9 @@ __device__ __forceinline__ float half_sum(float v) {
 // in these numbers from there on, in which the row at position p sees key j iff
 // p - window < j <= p or j < min(sinks, p + 1): one shift, and no load or
 // product is spent on the keys between.
+// MI355X: 8 prompts of 650-1,300 tokens, 16/8 heads, window 512, 48 us (513
+// TFLOP/s of visible pairs; all keys 66), chunks of 2,900-4,050 rows behind 4,096
+// keys, 32/8 heads, window 2,048, 359 us (752; all keys 895).
 struct TileSpan {
   int64_t head, gap, total;  // key j is key j of the sequence below head, j + gap from there on
 };
