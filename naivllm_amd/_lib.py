@@ -168,19 +168,30 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
-_counters: dict = {}
+_stream_scratch: dict = {}
 
 
-def stream_counters(device: torch.device, stream: int) -> int | None:
-    """64 KiB of arrival counters for the calls enqueued on ``stream`` outside
-    a capture, zero between them: their address.  None inside a capture: its
-    graph may be replayed beside any stream's work, or another graph's."""
+def stream_scratch(device: torch.device, stream: int, nbytes: int) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """(scratch of at least nbytes, 64 KiB of arrival counters) for a call
+    that is enqueued on ``stream``, the device's current one.
+
+    Outside a capture they are the stream's own, used again by its next call
+    (the stream orders them) and grown on demand (a replaced buffer goes back
+    to the allocator, which gives it to later work of that stream only); the
+    counters are zero between calls.  Inside a capture the scratch is a new
+    tensor of the graph's, and there are no counters: the graph may be
+    replayed beside any stream's work, or another graph's."""
     if torch.cuda.is_current_stream_capturing():
-        return None
-    buf = _counters.get((device.index, stream))
-    if buf is None:  # (two threads at once: the first one's stays)
-        buf = _counters.setdefault((device.index, stream), torch.zeros(16384, dtype=torch.int32, device=device))
-    return buf.data_ptr()
+        return torch.empty(nbytes, dtype=torch.uint8, device=device), None
+    key = (device.index, stream)
+    got = _stream_scratch.get(key)
+    if got is None:  # (two threads at once: the first one's counters stay)
+        got = _stream_scratch.setdefault(key, [torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device),
+                                               torch.zeros(16384, dtype=torch.int32, device=device)])
+    buf = got[0]
+    if buf.numel() < nbytes:
+        buf = got[0] = torch.empty(nbytes + nbytes // 2, dtype=torch.uint8, device=device)
+    return buf, got[1]
 
 
 def upload(x, device: torch.device) -> torch.Tensor:

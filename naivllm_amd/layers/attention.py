@@ -290,9 +290,9 @@ def paged_attention_window(
     between the sinks and the windows may be given to other sequences (their
     entries any value, -1 included), and what they hold (NaN, say) reaches no
     result; a key that one row sees and another does not must be finite.  A row
-    that sees no key, and a row at position -1, comes back as zeros.  Scratch comes from torch's allocator,
-    arrival counters are the stream's own (a captured call uses none): calls
-    on several streams, and captured ones, share nothing.
+    that sees no key, and a row at position -1, comes back as zeros.  Scratch
+    and arrival counters are the stream's own (a captured call's scratch its
+    graph's): calls on several streams, and captured ones, share nothing.
     No counterpart in the reference, whose attention sees every key."""
     window, sinks = _int_arg(window, "window", 1), _int_arg(sinks, "sinks", 0)
     query, block_tables, context_lens, cu_seqlens_q, positions, out = _few_rows(
@@ -303,13 +303,12 @@ def paged_attention_window(
              _lib.dtype_code(query.dtype), window, sinks)
     dev = query.device
     with _lib.on_device(dev):
-        ws_bytes = _window_workspace_bytes(B, *shape)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
         stream = _lib.stream_ptr(dev)
+        ws, counters = _lib.stream_scratch(dev, stream, _window_workspace_bytes(B, *shape))
         rc = _lib.lib().nsv_window_attention(
             out.data_ptr(), query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
             context_lens.data_ptr(), cu_seqlens_q.data_ptr(), positions.data_ptr(), scale, B, query.shape[0], *shape,
-            _lib.stream_counters(dev, stream), ws.data_ptr(), ws_bytes, stream)
+            _lib.ptr(counters), ws.data_ptr(), ws.numel(), stream)
     _lib.check(rc, "paged_attention_window")
     return out
 
@@ -345,8 +344,8 @@ def paged_attention_weights(
     row, and of unmapped pages, keep what they hold.  evict_kvcache reads the
     table; prefill_key_weights adds a prompt's rows.  bfloat16 and float32, up
     to 64 rows per sequence.  A page that several sequences of a call share
-    gets the sum of theirs, in no fixed order.  Scratch comes from torch's
-    allocator.  No counterpart in the reference."""
+    gets the sum of theirs, in no fixed order.  Scratch as
+    paged_attention_window's.  No counterpart in the reference."""
     query, block_tables, context_lens, cu_seqlens_q, positions, out = _few_rows(
         query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads, num_kv_heads, head_dim,
         block_size, out, "paged_attention_weights")
@@ -356,12 +355,12 @@ def paged_attention_weights(
              _lib.dtype_code(query.dtype))
     dev = query.device
     with _lib.on_device(dev):
-        ws_bytes = _weights_workspace_bytes(B, *shape)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+        stream = _lib.stream_ptr(dev)
+        ws, _ = _lib.stream_scratch(dev, stream, _weights_workspace_bytes(B, *shape))
         rc = _lib.lib().nsv_weights_attention(
             out.data_ptr(), query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), key_weights.data_ptr(),
             block_tables.data_ptr(), context_lens.data_ptr(), cu_seqlens_q.data_ptr(), positions.data_ptr(), scale, B,
-            query.shape[0], *shape, ws.data_ptr(), ws_bytes, _lib.stream_ptr(dev))
+            query.shape[0], *shape, ws.data_ptr(), ws.numel(), stream)
     _lib.check(rc, "paged_attention_weights")
     return out
 
@@ -725,11 +724,10 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: tor
     if v_cache.shape != k_cache.shape or not v_cache.is_contiguous() or v_cache.dtype != k_cache.dtype:
         raise ValueError("k_cache and v_cache must have the same contiguous shape and dtype")
     _check_key_weights(key_weights, k_cache)
-    dev = k_cache.device
-    tables = [block_tables] + ([] if out_block_tables is None else [out_block_tables])
-    if any(t.device != dev for t in (v_cache, context_lens, *tables)):
+    dev, out_tables = k_cache.device, block_tables if out_block_tables is None else out_block_tables
+    if not v_cache.device == context_lens.device == block_tables.device == out_tables.device == dev:
         raise ValueError(f"the caches, the block tables and context_lens must be on {dev}")
-    if any(t.dim() != 2 or t.shape[0] != block_tables.shape[0] for t in tables):
+    if block_tables.dim() != 2 or out_tables.dim() != 2 or out_tables.shape[0] != block_tables.shape[0]:
         raise ValueError("block_tables and out_block_tables must be (B, pages)")
     B, max_blocks = block_tables.shape
     if tuple(context_lens.shape) != (B,):
@@ -748,13 +746,14 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: tor
     kept = torch.empty((B, hkv, budget), dtype=torch.int32, device=dev)
     code = _lib.dtype_code(k_cache.dtype)
     with _lib.on_device(dev):
+        stream = _lib.stream_ptr(dev)
         ws_bytes = _evict_workspace_bytes(B, hkv, d, bs, max_blocks, int(out_block_tables is not None), code, budget)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None  # (too large to keep)
         rc = _lib.lib().nsv_evict_kv(
             k_cache.data_ptr(), v_cache.data_ptr(), key_weights.data_ptr(), block_tables.data_ptr(),
             context_lens.data_ptr(), _lib.ptr(out_block_tables), lens.data_ptr(), kept.data_ptr(), B, hkv, d, bs,
             max_blocks, 0 if out_block_tables is None else out_block_tables.shape[1], code, budget, sinks, recent,
-            _lib.ptr(ws), ws_bytes, _lib.stream_ptr(dev))
+            _lib.ptr(ws), ws_bytes, stream)
     _lib.check(rc, "evict_kvcache")
     return lens, kept
 
