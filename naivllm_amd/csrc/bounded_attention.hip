@@ -182,7 +182,7 @@ __device__ __forceinline__ void join_stats(const RowArgs& a, int ps, int rows, f
     if (4 * k < a.S) L += 4 * k + j < a.S ? x[k].y * __builtin_amdgcn_exp2f(x[k].x - ref) : 0.f;
   L += dpp_f32<kDppXor1>(L);
   L += dpp_f32<kDppXor2>(L);
-  if (j == 0 && m < rows) stat[m] = make_float2(ref, L > 0.f ? 1.f / L : 0.f);
+  if (j == 0 && m < rows) stat[m] = make_float2(ref, L == 0.f ? 0.f : 1.f / L);
 }
 
 template <typename T, int DH>
@@ -382,7 +382,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
         const int p = __shfl(my_pos, t & 63, 64);
         row_pos[mt][i] = m < a.R && t < qlen ? p : -1;
         row_inv[mt][i] = x.y;
-        row_m[mt][i] = x.y > 0.f ? x.x : __builtin_inff();
+        row_m[mt][i] = x.y == 0.f ? __builtin_inff() : x.x;
       }
   }
 
@@ -605,7 +605,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
 #pragma unroll
     for (int ww = 0; ww < kWaves; ++ww) L += lds.ml[ww][m].y * __builtin_amdgcn_exp2f(lds.ml[ww][m].x - ref);
     const float f = __builtin_amdgcn_exp2f(m_run[mt] - ref);
-    if (w == 0 && g == 0) lds.row[m] = make_float2(M, L);
+    if (w == 0 && g == 0) lds.row[m] = make_float2(L != L ? ref : M, L);  // (a sum that is NaN stays with its row)
     // (row m of a wave's O as DH floats; its 16-byte pieces rotated by the row, for the banks)
     float* dst = reinterpret_cast<float*>(mine) + m * DH;
 #pragma unroll
@@ -635,7 +635,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     const float2 ml = lds.row[m];
     if (whole) {
       if (MODE != kAttend && ch == 0) a.part_ml[part + m] = ml;
-      store_row(m, ch, ml.y > 0.f ? o * (1.f / ml.y) : f32x4{0.f, 0.f, 0.f, 0.f});
+      store_row(m, ch, ml.y == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * (1.f / ml.y));
     } else if (joins) {
       store16_agent(prs, (unsigned)(m * DH + ch * 4) * 4u, o);
       if (ch == 0)
@@ -698,7 +698,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
 #pragma unroll
           for (int e = 0; e < 4; ++e) num[e] = fmaf(o[i][k][e], wk, num[e]);
         }
-        store_row(idx / (DH / 4), idx % (DH / 4), den > 0.f ? num * (1.f / den) : f32x4{0.f, 0.f, 0.f, 0.f});
+        store_row(idx / (DH / 4), idx % (DH / 4), den == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : num * (1.f / den));
       }
     }
   };
@@ -779,7 +779,7 @@ __device__ __forceinline__ void merge_rows(const RowArgs& a, int ps, int block, 
     }
   }
   if (!row) return;
-  num = den > 0.f ? num * (1.f / den) : f32x4{0.f, 0.f, 0.f, 0.f};
+  num = den == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : num * (1.f / den);
   T* dst = (T*)a.out + ((int64_t)(q0 + t) * a.H + hk * (a.G * a.subsets) + sub * a.G + gh) * DH + ch * 4;
   if constexpr (sizeof(T) == 2)
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(num[0], num[1]), pack_bf16x2(num[2], num[3]));
@@ -818,7 +818,8 @@ __device__ __forceinline__ void stored_weights(const RowArgs& a, int pair, int b
 #pragma unroll
     for (int k = 0; k < CH; ++k) {
       const float2 x = stat[min(m0 + k, rows - 1)];
-      y = m0 + k < rows && x.y > 0.f ? fmaf(__builtin_amdgcn_exp2f(s[k] - x.x), x.y, y) : y;
+      const bool on = m0 + k < rows && x.y != 0.f && s[k] != kNegInf;  // (a masked key of a row that is NaN stays out of it)
+      y = on ? fmaf(__builtin_amdgcn_exp2f(s[k] - x.x), x.y, y) : y;
     }
   }
   float* dst = a.key_weights + (((int64_t)p * a.Hkv + hk) << a.bs_log2) + (key & ((1 << a.bs_log2) - 1));

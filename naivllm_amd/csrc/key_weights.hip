@@ -146,7 +146,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs a) {
     const int r = half * 32 + col;
     Rows x;
     x.inv = r0 + r < nrows ? lds.stat[buf][1][r] : 0.f;
-    x.nb = x.inv > 0.f ? -lds.stat[buf][0][r] : -__builtin_inff();  // (a row that sees nothing: weights 0)
+    x.nb = x.inv == 0.f ? -__builtin_inff() : -lds.stat[buf][0][r];  // (a row that sees nothing: weights 0)
     x.pos = pos0 + r0 + r;
     x.full = pos0 + r0 + half * 32 >= wkey + 63;
     return x;

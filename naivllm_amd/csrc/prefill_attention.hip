@@ -544,7 +544,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
     return;
   }
   if (r < nrows) {
-    if (a.stats && h == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(m_ref * sc, inv);
+    if (a.stats && h == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(m_ref * sc, L == 0.f ? 0.f : 1.f / L);
     bf16_t* dst = a.out + ((int64_t)(row0 + r) * a.H + head) * DH + h * 4;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -606,7 +606,7 @@ __global__ __launch_bounds__(256) void prefill_merge_kernel(PrefillMergeArgs a) 
     M = Mn;
   }
   const float inv = den > 0.f ? 1.f / den : 0.f;
-  if (a.stats && c4 == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(M, inv);
+  if (a.stats && c4 == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(M, den == 0.f ? 0.f : 1.f / den);
   bf16_t* dst = a.out + ((int64_t)(row0 + r) * a.H + head) * DH + c4 * 4;
   *reinterpret_cast<uint2*>(dst) =
       make_uint2(pack_bf16x2(num[0] * inv, num[1] * inv), pack_bf16x2(num[2] * inv, num[3] * inv));

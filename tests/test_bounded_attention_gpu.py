@@ -222,3 +222,36 @@ def test_weights_rows_behind_the_last_sequence_and_other_places_stay():
     vb = synth.verify_batch(43, [100], [3], dtype="bf16", block_size=16)
     vb.context_lens[0] = 500  # a table wider than the rows reach: keys past the last row keep their place's value
     _check_weights(vb)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,H", [(2, 16), (9, 32)])
+def test_a_row_of_nan_stays_alone(dtype, rows, H):
+    """A NaN query row: NaN for itself and for the weights of the keys it
+    sees, nothing for other rows, heads and keys; in a padding row, nothing."""
+    print(f"case: a NaN row {dtype} {rows} {H}", flush=True)
+    vb = synth.verify_batch(45, [700, 300], [rows, rows], num_heads=H, dtype=dtype, block_size=16, pad_rows=[1, 0])
+    t = to_device(vb)
+    want = paged_attention_window(t["query"], t["k_cache"], t["v_cache"], *_args(vb, t), window=200, sinks=4, max_q_len=rows)
+    w_want = torch.rand((vb.k_cache.shape[0], 8, 16), device="cuda")
+    w = w_want.clone()
+    every = paged_attention_weights(t["query"], t["k_cache"], t["v_cache"], w_want, *_args(vb, t), max_q_len=rows)
+    t["query"][rows - 1] = float("nan")        # padding
+    t["query"][rows, 5 * H // 16] = float("nan")    # the second sequence's first row, one head
+    out = paged_attention_window(t["query"], t["k_cache"], t["v_cache"], *_args(vb, t), window=200, sinks=4, max_q_len=rows)
+    out_w = paged_attention_weights(t["query"], t["k_cache"], t["v_cache"], w, *_args(vb, t), max_q_len=rows)
+    for got, good in ((out, want), (out_w, every)):
+        assert got[rows, 5 * H // 16].isnan().all()
+        good[rows, 5 * H // 16] = 0
+        got[rows, 5 * H // 16] = 0
+        assert torch.equal(got, good)
+    head = 5 * H // 16 // (H // 8)
+    seen = 300 - rows + 1                      # keys that the row sees
+    for b, n in enumerate((700 - (1 if rows > 1 else 0), 300)):
+        j = np.arange(n)
+        at = (torch.from_numpy(vb.block_tables[b, j // 16]).long().cuda(), slice(None), torch.from_numpy(j % 16).cuda())
+        got, good = w[at], w_want[at]
+        if b == 1:
+            assert got[:seen, head].isnan().all()
+            got[:seen, head] = good[:seen, head] = 0
+        assert torch.equal(got, good)

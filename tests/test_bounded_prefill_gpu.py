@@ -145,3 +145,27 @@ def test_key_weights_unmapped_pages():
     vb.block_tables[0, [0, 9, 18]] = -1
     vb.block_tables[1, :] = -1
     _check_key_weights(vb)
+
+
+def test_a_row_of_nan_stays_alone():
+    print("case: prompt, a NaN row", flush=True)
+    vb = _batch(61, [200, 50], [100, 0], 4, 2, 128, 16)
+    scale, tables = 1.0 / np.sqrt(128), None
+    results = []
+    for bad in (False, True):
+        t = to_device(vb)
+        tables = t["block_tables"]
+        if bad:
+            t["query"][150, 3] = float("nan")
+        plan, adder = (PrefillPlan([200, 50], [300, 50], 4, 2, 16, DEV), KeyWeightsPlan([200, 50], [300, 50], 4, 2, 16, DEV))
+        stats = torch.empty((250, 4, 2), device="cuda")
+        out = prefill_attention(t["query"], t["k_cache"], t["v_cache"], plan, scale, 128, tables, stats=stats)
+        w = torch.ones((vb.k_cache.shape[0], 2, 16), device="cuda")
+        prefill_key_weights(t["query"], t["k_cache"], w, adder, stats, scale, 128, tables)
+        j = np.arange(300)
+        results.append((out, w[torch.from_numpy(vb.block_tables[0, j // 16]).long().cuda(), :, torch.from_numpy(j % 16).cuda()]))
+    (good, w_good), (got, w_got) = results
+    assert got[150, 3].isnan().all() and w_got[:251, 1].isnan().all()
+    got[150, 3] = good[150, 3] = 0
+    w_got[:251, 1] = w_good[:251, 1] = 0
+    assert torch.equal(got, good) and torch.equal(w_got, w_good)
