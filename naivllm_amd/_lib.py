@@ -12,6 +12,7 @@ from __future__ import annotations
 import contextlib
 import ctypes
 import os
+import threading
 
 import torch  # noqa: F401  (must be imported before the library is loaded)
 
@@ -168,30 +169,44 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+class StreamScratch:
+    """Scratch of a stream's calls, used while ``lock`` is held: a call may be
+    several launches, which another thread's call on the same stream must not
+    come between.  ``counters``: 64 KiB of arrival counters, zero between
+    calls, or None."""
+
+    __slots__ = ("lock", "counters", "_buf", "_device")
+
+    def __init__(self, device: torch.device, counters: torch.Tensor | None, nbytes: int):
+        self.lock, self.counters, self._device = threading.Lock(), counters, device
+        self._buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+    def take(self, nbytes: int) -> torch.Tensor:
+        """At least nbytes, grown on demand: a replaced buffer goes back to the
+        allocator, which gives it to later work of that stream only."""
+        if self._buf.numel() < nbytes:
+            spare = nbytes // 2 if self._buf.numel() else 0  # (a capture's: as much as its call needs)
+            self._buf = torch.empty(nbytes + spare, dtype=torch.uint8, device=self._device)
+        return self._buf
+
+
 _stream_scratch: dict = {}
 
 
-def stream_scratch(device: torch.device, stream: int, nbytes: int) -> tuple[torch.Tensor, torch.Tensor | None]:
-    """(scratch of at least nbytes, 64 KiB of arrival counters) for a call
-    that is enqueued on ``stream``, the device's current one.
-
-    Outside a capture they are the stream's own, used again by its next call
-    (the stream orders them) and grown on demand (a replaced buffer goes back
-    to the allocator, which gives it to later work of that stream only); the
-    counters are zero between calls.  Inside a capture the scratch is a new
-    tensor of the graph's, and there are no counters: the graph may be
-    replayed beside any stream's work, or another graph's."""
+def stream_scratch(device: torch.device, stream: int) -> StreamScratch:
+    """The scratch for calls that are enqueued on ``stream``, the device's
+    current one: the stream's own, used again by its next call (the stream
+    orders them).  Inside a capture it is new, the graph's, and without
+    counters: the graph may be replayed beside any stream's work, or another
+    graph's."""
     if torch.cuda.is_current_stream_capturing():
-        return torch.empty(nbytes, dtype=torch.uint8, device=device), None
+        return StreamScratch(device, None, 0)
     key = (device.index, stream)
     got = _stream_scratch.get(key)
-    if got is None:  # (two threads at once: the first one's counters stay)
-        got = _stream_scratch.setdefault(key, [torch.empty(max(nbytes, 1 << 20), dtype=torch.uint8, device=device),
-                                               torch.zeros(16384, dtype=torch.int32, device=device)])
-    buf = got[0]
-    if buf.numel() < nbytes:
-        buf = got[0] = torch.empty(nbytes + nbytes // 2, dtype=torch.uint8, device=device)
-    return buf, got[1]
+    if got is None:  # (two threads at once: the first one's stays)
+        got = _stream_scratch.setdefault(
+            key, StreamScratch(device, torch.zeros(16384, dtype=torch.int32, device=device), 1 << 20))
+    return got
 
 
 def upload(x, device: torch.device) -> torch.Tensor:

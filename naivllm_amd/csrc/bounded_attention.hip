@@ -72,7 +72,7 @@ struct RowArgs {
   float2* part_ml;    // [npairs * subsets][S][R]: (maximum, log2 domain; sum)
   float* part_o;      // [npairs * subsets][S][R][D], unnormalised
   unsigned* counters; // null, or splits of a (pair, head subset) done so far, 0 between calls (kAttend)
-  float* scores;      // [npairs][R][score_keys], log2 domain, -inf where masked (kAttendScores)
+  float* scores;      // [npairs * subsets][R][score_keys], log2 domain, -inf where masked (kAttendScores)
   float* key_weights; // [num_blocks][Hkv][block_size]
   float scale_log2;
   int H, Hkv, G, subsets;  // query heads, kv heads, query heads of a kv head that a workgroup serves, how often

@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs a) {
   const int first = max(0, key0 - pos0);              // the first row that sees a key of the block
   const int tiles = (nrows - first + kRows - 1) / kRows;  // per head
 
-  // the keys: lane (h, col) holds key 32 t + col, dims 16 ks + 8 h ..; a key that is not there reads the block's first
+  // the keys: lane (h, col) holds key 32 t + col, dims 16 ks + 8 h ..; a key that is not there reads the block's last
   const int wkey = key0 + w * 64;
   u32x4 ka[2][KS];
 #pragma unroll

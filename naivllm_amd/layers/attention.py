@@ -304,11 +304,13 @@ def paged_attention_window(
     dev = query.device
     with _lib.on_device(dev):
         stream = _lib.stream_ptr(dev)
-        ws, counters = _lib.stream_scratch(dev, stream, _window_workspace_bytes(B, *shape))
-        rc = _lib.lib().nsv_window_attention(
-            out.data_ptr(), query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
-            context_lens.data_ptr(), cu_seqlens_q.data_ptr(), positions.data_ptr(), scale, B, query.shape[0], *shape,
-            _lib.ptr(counters), ws.data_ptr(), ws.numel(), stream)
+        scratch = _lib.stream_scratch(dev, stream)
+        with scratch.lock:
+            ws = scratch.take(_window_workspace_bytes(B, *shape))
+            rc = _lib.lib().nsv_window_attention(
+                out.data_ptr(), query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_tables.data_ptr(),
+                context_lens.data_ptr(), cu_seqlens_q.data_ptr(), positions.data_ptr(), scale, B, query.shape[0], *shape,
+                _lib.ptr(scratch.counters), ws.data_ptr(), ws.numel(), stream)
     _lib.check(rc, "paged_attention_window")
     return out
 
@@ -356,11 +358,13 @@ def paged_attention_weights(
     dev = query.device
     with _lib.on_device(dev):
         stream = _lib.stream_ptr(dev)
-        ws, _ = _lib.stream_scratch(dev, stream, _weights_workspace_bytes(B, *shape))
-        rc = _lib.lib().nsv_weights_attention(
-            out.data_ptr(), query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), key_weights.data_ptr(),
-            block_tables.data_ptr(), context_lens.data_ptr(), cu_seqlens_q.data_ptr(), positions.data_ptr(), scale, B,
-            query.shape[0], *shape, ws.data_ptr(), ws.numel(), stream)
+        scratch = _lib.stream_scratch(dev, stream)
+        with scratch.lock:
+            ws = scratch.take(_weights_workspace_bytes(B, *shape))
+            rc = _lib.lib().nsv_weights_attention(
+                out.data_ptr(), query.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), key_weights.data_ptr(),
+                block_tables.data_ptr(), context_lens.data_ptr(), cu_seqlens_q.data_ptr(), positions.data_ptr(), scale, B,
+                query.shape[0], *shape, ws.data_ptr(), ws.numel(), stream)
     _lib.check(rc, "paged_attention_weights")
     return out
 

@@ -1,10 +1,14 @@
 """The bounded cache's operators captured, replayed, on several streams at
 once, and over pages that sequences share."""
 
+import threading
+import time
+
 import numpy as np
 import pytest
 import torch
 
+from naivllm_amd import _lib
 from naivllm_amd.layers.attention import (KeyWeightsPlan, PrefillPlan, evict_kvcache, paged_attention_weights,
                                           paged_attention_window, prefill_attention, prefill_key_weights)
 from naivllm_amd.utils import synth
@@ -132,6 +136,56 @@ def test_two_streams_at_once():
         torch.cuda.synchronize()
         for got, want in zip(results, wants):
             assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+
+
+@pytest.mark.parametrize("name,native", [("window", "nsv_window_attention"), ("key_weights", "nsv_weights_attention")])
+def test_two_threads_on_one_stream(name, native, monkeypatch):
+    """A call's launches, which share the stream's scratch, stay together: the
+    second thread's begin when the first's are all enqueued."""
+    print(f"case: two threads {name}", flush=True)
+    calls = [_calls(101)[name], _calls(104)[name]]
+    wants = []
+    for make in calls:
+        state, step = make()
+        wants.append(step() + state)
+    torch.cuda.synchronize()
+    real, inside, most = _lib.lib(), [], []
+
+    class Watched:
+        def __getattr__(self, attr):
+            call = getattr(real, attr)
+            if attr != native:
+                return call
+
+            def watched(*args):
+                inside.append(1)
+                most.append(len(inside))
+                time.sleep(0.02)
+                rc = call(*args)
+                inside.pop()
+                return rc
+            return watched
+
+    monkeypatch.setattr(_lib, "lib", lambda: Watched())
+    made, results, start = [make() for make in calls], [None, None], threading.Barrier(2)
+    torch.cuda.synchronize()
+
+    def work(i):
+        start.wait()
+        for _ in range(3):
+            got = made[i][1]()
+            if results[i] is None:
+                results[i] = [x.clone() for x in got + made[i][0]]
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for x in threads:
+        x.start()
+    for x in threads:
+        x.join(60)
+    torch.cuda.synchronize()
+    assert len(most) == 6 and max(most) == 1
+    for got, want in zip(results, wants):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 def test_a_shared_page_gets_the_weights_of_every_sequence():
