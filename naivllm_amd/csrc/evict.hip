@@ -8,14 +8,16 @@
 //
 // Selection (evict_select_kernel), one workgroup of 16 waves per (sequence, kv
 // head): the weights are read once into registers, four neighbours per load
-// (beyond 32,768 keys they are read again in every pass), and compared as
-// unsigned words of the same order, in which the keys that stay anyway are the
-// largest.  The budget-th largest word comes from three passes over 11, 11
-// and 10 bits (four histograms; a wave whose words share a digit adds once,
-// so that equal weights cost no collisions); then each wave counts, per load, what lies
-// above that word and what equals it, a scan over those counts gives every
-// kept key its place, and key and weight are written there.  Bound by the
-// latency of its passes: one round trip and 15 barriers.
+// (beyond 32,768 keys, and of pages of fewer than four keys, they are read again
+// in every pass), and compared as unsigned words of the same order, in which the
+// keys that stay anyway are the largest.  The budget-th largest word comes from
+// three passes over 11, 11 and 10 bits (four histograms, taken by a wave's lanes
+// in turn: weights share few leading digits, and equal adds wait for one
+// another); then each wave counts, per load, what lies above that word and
+// what equals it, a scan over those counts gives every kept key its place, and
+// keys and weights go there by way of LDS, so that they are written by full
+// waves.  Bound by its passes' latency (two round trips, some 15 barriers) and
+// above 10,000 keys by the histograms' adds and the words' comparisons.
 //
 // Moving (evict_move_kernel): every kept row read and written once.  Within a
 // table rows move forward only: row i comes from kept[i] >= i.  A workgroup
@@ -29,10 +31,12 @@
 // bytes.
 //
 // Measured on MI355X: one sequence, 1,250 -> 512 keys of 8 heads, bf16, D 128,
-// to pages apart: 10.5 us of selection, 5.5 of moving; 16 sequences of 16k-32k
-// -> 2,048 keys in place: 36 and 62 (268 MB read and written, 4.3 TB/s; a large
-// copy 4.8).  Before the words were held and the histograms cleared ahead the
-// selection took 13 and 50, with one serial scan per pass 43 and 128.
+// to pages apart: 9.0 us of selection, 5.5 of moving; 16 sequences of 16k-32k
+// -> 2,048 keys in place: 23 and 60 (268 MB read and written, 4.4 TB/s; a large
+// copy 4.8).  The selection took 36 of the latter with every page looked up
+// before its weights and again at each kept key's place, kept keys written from
+// where they were found, and one histogram per wave; 50 with the words made
+// anew in each pass, 128 with one serial scan per pass.
 
 #include "common.h"
 
@@ -44,6 +48,7 @@ constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kSelLoads = 8;     // loads of four weights that a thread holds: 32,768 keys in all
 constexpr int kBins = 2048, kCopies = 4;
+constexpr int kOutPages = 4096;  // entries of the destination's table held in LDS
 constexpr int kMoveThreads = 512;
 constexpr int kMoveUnroll = 8;   // 16-byte pieces per lane and chunk
 
@@ -77,13 +82,24 @@ __device__ __forceinline__ uint32_t ordered(float f) {
 // The wave's loads have returned (a barrier alone orders their issue).
 __device__ __forceinline__ void loads_back() { __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
+__device__ __forceinline__ int wave_scan(int v) {  // the sum over the lanes up to this one
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // row_shr:1
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // row_shr:2
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // row_shr:4
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // row_shr:8
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+  return v;
+}
+
 // HELD: every weight of a context fits the workgroup's registers, and so do
 // their words.
 template <bool HELD>
 __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) {
   constexpr int STEP = kSelThreads * 4;  // keys per load of the workgroup
-  __shared__ __attribute__((aligned(16))) int hist[3][kCopies][kBins];  // one per pass
+  __shared__ __attribute__((aligned(16))) int hist[3][kBins][kCopies];  // one per pass
   __shared__ __attribute__((aligned(16))) int wave_sum[kSelWaves];
+  __shared__ int out_page[HELD ? kOutPages : 1];
   __shared__ int digit, rest, share;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int b = blockIdx.x / a.Hkv, h = blockIdx.x - b * a.Hkv;
@@ -133,17 +149,34 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   const int loads = (n + STEP - 1) / STEP;
   f32x4 held[HELD ? kSelLoads : 1];
   u32x4 word[HELD ? kSelLoads : 1];
-  if constexpr (HELD) {
+  uint32_t mapped = 0;  // HELD: bit e: load e has a page
+  if constexpr (HELD) {  // every page in one round trip, then every weight (a.vector holds)
+    int page[kSelLoads];
 #pragma unroll
     for (int e = 0; e < kSelLoads; ++e)
-      if (e < loads) held[e] = load4(e * STEP + tid * 4);  // uniform
+      if (e < loads) page[e] = bt[min(e * STEP + tid * 4, n - 1) >> a.bs_log2];  // uniform
+#pragma unroll
+    for (int e = 0; e < kSelLoads; ++e)
+      if (e < loads) {  // (past the context the last key's group, of a hole page 0: a load under a condition would be waited for)
+        const int key = min(e * STEP + tid * 4, (n - 1) & ~3);
+        held[e] = *reinterpret_cast<const f32x4*>(a.weights + ((((int64_t)max(page[e], 0) * a.Hkv + h) << a.bs_log2) + (key & bs_mask)));
+        mapped |= page[e] >= 0 ? 1u << e : 0u;
+      }
+  }
+  if constexpr (HELD) {
+    const int pages = got > 0 ? ((got - 1) >> a.bs_log2) + 1 : 0;
+    for (int i = tid; i < min(pages, kOutPages); i += kSelThreads) out_page[i] = ot[i];
   }
   for (int i = tid; i < 3 * kCopies * kBins / 4; i += kSelThreads)  // (while the weights are under way)
     reinterpret_cast<u32x4*>(&hist[0][0][0])[i] = u32x4{0u, 0u, 0u, 0u};
   if constexpr (HELD) {
 #pragma unroll
     for (int e = 0; e < kSelLoads; ++e)
-      if (e < loads) word[e] = words(e * STEP + tid * 4, held[e]);
+      if (e < loads) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) held[e][j] = (mapped >> e) & 1 ? held[e][j] : 0.f;
+        word[e] = words(e * STEP + tid * 4, held[e]);
+      }
   }
   auto each = [&](auto f) {  // f(e, first key, weights, words) for every load
     if constexpr (HELD) {
@@ -171,22 +204,16 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   int want = n > a.budget ? got : 0, low = 0;
   if (n > a.budget) {  // uniform
     int above_bits = 32;  // leading bits not yet told apart end here
+#pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0), bits = above_bits - shift;
-      int* mine = hist[pass][w & (kCopies - 1)];
+      int* mine = hist[pass][0] + (lane & (kCopies - 1));
       const uint32_t head = pass == 0 ? 0u : prefix >> above_bits;
       each([&](int, int, f32x4, u32x4 u) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           if (pass > 0 && (u[j] >> above_bits) != head) continue;
-          const int d = (int)(u[j] >> shift) & ((1 << bits) - 1);
-          const int d0 = __builtin_amdgcn_readfirstlane(d);
-          const uint64_t active = __ballot(true);
-          if (__ballot(d != d0) == 0) {  // uniform: one digit
-            if (lane == __builtin_ctzll(active)) atomicAdd(&mine[d0], __popcll(active));
-          } else {
-            atomicAdd(&mine[d], 1);
-          }
+          atomicAdd(&mine[((u[j] >> shift) & ((1u << bits) - 1)) * kCopies], 1);
         }
       });
       __syncthreads();
@@ -194,17 +221,13 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       const int top = kBins - 1 - 2 * tid;
       int c1 = 0, c0 = 0;
 #pragma unroll
-      for (int k = 0; k < kCopies; ++k) {
-        const int2 c = *reinterpret_cast<const int2*>(&hist[pass][k][top - 1]);
-        c0 += c.x;
-        c1 += c.y;
+      for (int k = 0; k < kCopies; k += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(&hist[pass][top - 1][k]);
+        const int4 y = *reinterpret_cast<const int4*>(&hist[pass][top][k]);
+        c0 += x.x + x.y + x.z + x.w;
+        c1 += y.x + y.y + y.z + y.w;
       }
-      int sum = c1 + c0;
-#pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int y = __shfl_up(sum, d, 64);
-        sum += lane >= d ? y : 0;
-      }
+      const int sum = wave_scan(c1 + c0);
       if (lane == 63) wave_sum[w] = sum;
       __syncthreads();
       int above = sum - c1 - c0;
@@ -232,50 +255,39 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   // (a context that is short enough: every weight's word is above 0, and stays)
 
   // ---- places: the kept keys before each wave's four-key groups of each load, by a scan over counts in LDS
-  const uint32_t mark = prefix >> low;
+  const uint32_t least = prefix, most = prefix | ((1u << low) - 1);  // (low < 32) words that tie: least .. most
   int* count_gt = &hist[0][0][0];  // [load][wave]
-  int* count_eq = &hist[1][0][0];
-  auto below = [](uint64_t m) {  // of a wave's mask, the bits before this lane's
-    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0u));
+  int* count_eq = &hist[0][kBins / 2][0];
+  // of a lane's four words: those above the tie, and from it up (<< 16)
+  auto counts = [&](u32x4 u) {
+    int c = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c += (u[j] > most ? 1 : 0) + (u[j] >= least ? 1 << 16 : 0);
+    return c;
   };
-  auto emit = [&](int key, f32x4 x, u32x4 u, int at_gt, int at_eq) {
-    // the wave's counts before this lane, then this lane's keys in order
-    int g = at_gt, q = at_eq;
+  // f(j, place) for those of a lane's keys that stay, after the wave's at_gt above the tie and at_eq tied ones
+  auto emit = [&](u32x4 u, int at_gt, int at_eq, int before, auto f) {
+    int g = at_gt + (before & 0xffff), q = at_eq + (before >> 16) - (before & 0xffff);
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      g += below(__ballot((u[j] >> low) > mark));
-      q += below(__ballot((u[j] >> low) == mark));
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const bool is_gt = (u[j] >> low) > mark, is_eq = (u[j] >> low) == mark;
-      if (is_gt || (is_eq && q < want)) {
-        const int i = g + min(q, want);
-        kept[i] = key + j;
-        if constexpr (HELD) {  // (every weight of the context is in registers: places may be overwritten)
-          const int64_t to = place(bt, key + j) < 0 ? -1 : place(ot, i);
-          if (to >= 0) a.weights[to] = x[j];
-        }
-      }
-      g += is_gt;
-      q += is_eq;
+      const bool gt = u[j] > most, eq = u[j] >= least && !gt;
+      if (gt || (eq && q < want)) f(j, g + min(q, want));
+      g += gt;
+      q += eq;
     }
   };
   constexpr int GROUP = kBins / kSelWaves;  // loads whose counts fit at a time
   int base_gt = 0, base_eq = 0;
+  int before[HELD ? kSelLoads : 1];  // the wave's counts of a load before this lane's keys
   for (int e0 = 0; e0 < loads; e0 += GROUP) {  // (one turn up to 524,288 keys)
     __syncthreads();
     each([&](int e, int, f32x4, u32x4 u) {
       if (e < e0 || e >= e0 + GROUP) return;  // uniform
-      int g = 0, q = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        g += __popcll(__ballot((u[j] >> low) > mark));
-        q += __popcll(__ballot((u[j] >> low) == mark));
-      }
-      if (lane == 0) {
-        count_gt[(e - e0) * kSelWaves + w] = g;
-        count_eq[(e - e0) * kSelWaves + w] = q;
+      const int own = counts(u), upto = wave_scan(own);
+      if constexpr (HELD) before[e] = upto - own;
+      if (lane == 63) {
+        count_gt[(e - e0) * kSelWaves + w] = upto & 0xffff;
+        count_eq[(e - e0) * kSelWaves + w] = (upto >> 16) - (upto & 0xffff);
       }
     });
     __syncthreads();
@@ -285,19 +297,13 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
       for (int i0 = 0; i0 < m; i0 += 64) {
         const int i = i0 + lane;
         const int g = i < m ? count_gt[i] : 0, q = i < m ? count_eq[i] : 0;
-        int sg = g, sq = q;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const int yg = __shfl_up(sg, d, 64), yq = __shfl_up(sq, d, 64);
-          sg += lane >= d ? yg : 0;
-          sq += lane >= d ? yq : 0;
-        }
+        const int sg = wave_scan(g), sq = wave_scan(q);
         if (i < m) {
           count_gt[i] = run_gt + sg - g;
           count_eq[i] = run_eq + sq - q;
         }
-        run_gt += __shfl(sg, 63, 64);
-        run_eq += __shfl(sq, 63, 64);
+        run_gt += __builtin_amdgcn_readlane(sg, 63);
+        run_eq += __builtin_amdgcn_readlane(sq, 63);
       }
       if (lane == 0) {
         wave_sum[0] = run_gt;
@@ -307,10 +313,37 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     __syncthreads();
     base_gt = wave_sum[0];
     base_eq = wave_sum[1];
-    each([&](int e, int key, f32x4 x, u32x4 u) {
-      if (e < e0 || e >= e0 + GROUP) return;  // uniform
-      emit(key, x, u, count_gt[(e - e0) * kSelWaves + w], count_eq[(e - e0) * kSelWaves + w]);
-    });
+    if constexpr (!HELD) {
+      each([&](int e, int key, f32x4, u32x4 u) {
+        if (e < e0 || e >= e0 + GROUP) return;  // uniform
+        const int at = (e - e0) * kSelWaves + w, own = counts(u);
+        emit(u, count_gt[at], count_eq[at], wave_scan(own) - own, [&](int j, int i) { kept[i] = key + j; });
+      });
+    }
+  }
+  if constexpr (HELD) {
+    // By way of LDS, kPlaces at a time, so that the lanes that write are all
+    // busy: few of a load's keys stay.  (Every weight of the context is in
+    // registers: places may be overwritten.)
+    constexpr int kPlaces = 2 * kCopies * kBins / 2;  // (two histograms, two words a place)
+    int2* list = reinterpret_cast<int2*>(&hist[1][0][0]);  // (key, or ~key where it has no page; weight)
+    for (int i0 = 0; i0 < got; i0 += kPlaces) {
+      each([&](int e, int key, f32x4 x, u32x4 u) {
+        emit(u, count_gt[e * kSelWaves + w], count_eq[e * kSelWaves + w], before[e], [&](int j, int i) {
+          if ((unsigned)(i - i0) < (unsigned)kPlaces)
+            list[i - i0] = make_int2((mapped >> e) & 1 ? key + j : ~(key + j), __float_as_int(x[j]));
+        });
+      });
+      __syncthreads();
+      for (int i = i0 + tid; i < min(got, i0 + kPlaces); i += kSelThreads) {
+        const int2 x = list[i - i0];
+        kept[i] = x.x < 0 ? ~x.x : x.x;
+        const int pi = i >> a.bs_log2;
+        const int p = pi < kOutPages ? out_page[pi] : ot[pi];
+        if (x.x >= 0 && p >= 0) a.weights[(((int64_t)p * a.Hkv + h) << a.bs_log2) + (i & bs_mask)] = __int_as_float(x.y);
+      }
+      if (i0 + kPlaces < got) __syncthreads();
+    }
   }
   if constexpr (!HELD) {
     // the weights themselves, a chunk at a time: every read of a chunk before its first write
@@ -481,7 +514,7 @@ int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights, const int32_t
               context_lens, lens, kept, Hkv, row_bytes, bs_log2, max_blocks, apart ? out_blocks : max_blocks,
               budget, sinks, recent, bs_log2 >= 2 && (uintptr_t)key_weights % 16 == 0, (char*)workspace};
   hipStream_t s = (hipStream_t)stream;
-  if (cap <= (int64_t)kSelThreads * 4 * kSelLoads)
+  if (cap <= (int64_t)kSelThreads * 4 * kSelLoads && a.vector)
     hipLaunchKernelGGL(evict_select_kernel<true>, dim3(B * Hkv), dim3(kSelThreads), 0, s, a);
   else
     hipLaunchKernelGGL(evict_select_kernel<false>, dim3(B * Hkv), dim3(kSelThreads), 0, s, a);

@@ -106,3 +106,30 @@ def test_a_table_narrower_than_the_context():
     lens = [400]
     k, v, w, tables, _ = _case(77, lens)
     _check(k, v, w, tables[:, :20].copy(), lens, 100, 4, 10)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+def test_many_keys_stay_on_small_pages(apart):
+    """More places than the workgroup lists at a time, more pages than it holds."""
+    print(f"case: evict 25000 of 30000 keys, pages of 4, apart {apart}", flush=True)
+    lens = [30000, 8193, 25001]
+    k, v, w, tables, free = _case(79, lens, 1, 32, 4, levels=1000, spare=6250 * 3)
+    out = free[:6250 * 3].reshape(3, 6250).copy() if apart else None
+    _check(k, v, w, tables, lens, 25000, 4, 100, out)
+
+
+def test_weights_off_their_alignment():
+    print("case: evict, weights at an odd address", flush=True)
+    k, v, w, tables, _ = _case(80, [3000, 700])
+    odd = torch.empty(w.numel() + 1, device="cuda")[1:].view(w.shape)
+    odd.copy_(w)
+    aligned = w.cuda()
+    results = []
+    for weights in (aligned, odd):
+        gk, gv = k.cuda(), v.cuda()
+        _, kept = evict_kvcache(gk, gv, weights, torch.from_numpy(tables).cuda(),
+                                torch.tensor([3000, 700], device="cuda"), 333, sinks=3, recent=40)
+        results.append((gk, gv, weights, kept))
+    torch.cuda.synchronize()
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
