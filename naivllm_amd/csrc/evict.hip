@@ -31,7 +31,7 @@
 // bytes.
 //
 // Measured on MI355X: one sequence, 1,250 -> 512 keys of 8 heads, bf16, D 128,
-// to pages apart: 9.0 us of selection, 5.5 of moving; 16 sequences of 16k-32k
+// to pages apart: 9.0 us of selection, 3.5 of moving; 16 sequences of 16k-32k
 // -> 2,048 keys in place: 23 and 60 (268 MB read and written, 4.4 TB/s; a large
 // copy 4.8).  The selection took 36 of the latter with every page looked up
 // before its weights and again at each kept key's place, kept keys written from
@@ -374,7 +374,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
   const int h = rest % a.Hkv, b = rest / a.Hkv;
   const int n = clamp_len(a, b), got = min(n, a.budget);
   const bool apart = a.out_tables != a.block_tables;
-  if (n <= a.budget && !apart) return;  // uniform: nothing moves
+  if (got == 0 || (n <= a.budget && !apart)) return;  // uniform: nothing moves
   const int bs_mask = (1 << a.bs_log2) - 1;
   const int32_t* bt = a.block_tables + (int64_t)b * a.max_blocks;
   const int32_t* ot = a.out_tables + (int64_t)b * a.out_blocks;
@@ -384,37 +384,38 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
   char* staged = a.staged + (((int64_t)b * a.Hkv + h) * 2 + blockIdx.y) * a.budget * a.row_bytes + piece;
   const int64_t stride = (int64_t)a.Hkv * a.row_bytes;
   const int r = threadIdx.x >> lanes_log2;
-  auto row = [&](const int32_t* table, int key) -> char* {
-    const int p = table[key >> a.bs_log2];
-    return p < 0 ? nullptr : base + (((int64_t)p << a.bs_log2) + (key & bs_mask)) * stride;
-  };
   const int chunk = rows * kMoveUnroll;
   struct Chunk {
     u32x4 x[kMoveUnroll];
-    bool on[kMoveUnroll];
+    int to[kMoveUnroll];   // the page that a row goes to; -1: the row does not move (a hole, or past the last)
   };
+  // (rows past the last read it again and those of a hole page 0, so that no
+  // load is under a condition: it would be waited for there)
   auto read = [&](Chunk& c, int i0) {
-    const char* src[kMoveUnroll];
+    int key[kMoveUnroll], p[kMoveUnroll];
+#pragma unroll
+    for (int u = 0; u < kMoveUnroll; ++u) key[u] = kept[min(i0 + u * rows + r, got - 1)];
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
-      const int i = i0 + u * rows + r;
-      src[u] = i < got ? row(bt, kept[i]) : nullptr;  // (a row without a page does not move)
-      if (MOVE == kFromStaged && src[u]) src[u] = staged + (int64_t)i * a.row_bytes;
+      p[u] = bt[key[u] >> a.bs_log2];
+      c.to[u] = MOVE == kToStaged ? 0 : ot[min(i0 + u * rows + r, got - 1) >> a.bs_log2];
     }
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
-      c.on[u] = src[u] != nullptr;
-      c.x[u] = u32x4{0u, 0u, 0u, 0u};
-      if (c.on[u]) c.x[u] = load16_stream(src[u]);
+      const int i = min(i0 + u * rows + r, got - 1);
+      if (i0 + u * rows + r >= got || p[u] < 0) c.to[u] = -1;
+      const char* src = MOVE == kFromStaged ? staged + (int64_t)i * a.row_bytes
+                                            : base + (((int64_t)max(p[u], 0) << a.bs_log2) + (key[u] & bs_mask)) * stride;
+      c.x[u] = load16_stream(src);
     }
   };
   auto write = [&](const Chunk& c, int i0) {
 #pragma unroll
     for (int u = 0; u < kMoveUnroll; ++u) {
       const int i = i0 + u * rows + r;
-      char* dst = nullptr;
-      if (c.on[u]) dst = MOVE == kToStaged ? staged + (int64_t)i * a.row_bytes : row(ot, i);
-      if (dst) __builtin_nontemporal_store(c.x[u], reinterpret_cast<u32x4*>(dst));
+      char* dst = MOVE == kToStaged ? staged + (int64_t)i * a.row_bytes
+                                    : base + (((int64_t)c.to[u] << a.bs_log2) + (i & bs_mask)) * stride;
+      if (c.to[u] >= 0) __builtin_nontemporal_store(c.x[u], reinterpret_cast<u32x4*>(dst));
     }
   };
   Chunk c;
