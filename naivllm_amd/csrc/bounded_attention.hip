@@ -33,10 +33,10 @@
 // 714 us against 503), or over K again, whose products are made anew.
 //
 // Measured on MI355X, us per call, bytes that it cannot do without per second:
-// window 512 + 4 sinks, 1 row of 16/8 heads 8.0 (latency: the metadata's,
+// window 512 + 4 sinks, 1 row of 16/8 heads 7.7 (latency: the metadata's,
 // the table's and the tiles' round trips); window 4,096, 8 sequences of 9 rows,
-// 32/8 heads, 35 (3.9 TB/s; loads alone 33); fp32, 3 sequences, window 999, 9.5;
-// key weights of 8 sequences of 1,250 keys, 1 row, 15.7 (2.6 TB/s); of 16
+// 32/8 heads, 35 (3.9 TB/s; loads alone 33); fp32, 3 sequences, window 999, 9.2;
+// key weights of 8 sequences of 1,250 keys, 1 row, 15.1 (2.7 TB/s); of 16
 // sequences of 16k-32k keys, 9 rows of 32/8 heads, 500: 309 for the attention
 // (5.2 TB/s), 184 for K again (4.4 TB/s; its loads alone 171).
 
@@ -107,6 +107,19 @@ __device__ __forceinline__ float groups_sum(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// over the wave
+template <typename F>
+__device__ __forceinline__ int wave_reduce(int v, F f) {
+  v = f(v, (int)dpp_u32<kDppXor1>((uint32_t)v));
+  v = f(v, (int)dpp_u32<kDppXor2>((uint32_t)v));
+  v = f(v, (int)dpp_u32<kDppHalfMirror>((uint32_t)v));
+  v = f(v, (int)dpp_u32<kDppMirror>((uint32_t)v));
+  auto r = __builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false);
+  v = f((int)r[0], (int)r[1]);
+  r = __builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false);
+  return uniform(f((int)r[0], (int)r[1]));
+}
+
 // The keys of a sequence that some row of the call sees, numbered 0 .. total
 // - 1: the first `head` keys, then those from head + gap on.
 struct Span {
@@ -115,24 +128,18 @@ struct Span {
   __device__ int key(int v) const { return v < head ? v : v + gap; }
 };
 
-// (every lane of the wave; the sequence's rows are q0 .. q0 + qlen - 1)
-__device__ __forceinline__ Span make_span(const RowArgs& a, int b, int q0, int qlen, int& my_pos) {
+// (every lane of the wave; the sequence's rows are q0 .. q0 + qlen - 1, its
+// context length, loaded beside them, is len)
+__device__ __forceinline__ Span make_span(const RowArgs& a, int64_t len, int q0, int qlen, int& my_pos) {
   const int lane = threadIdx.x & 63;
   const int64_t cap = (int64_t)a.max_blocks << a.bs_log2;
-  const int64_t len = a.context_lens[b];
   const int ctx = uniform((int)(len < 0 ? 0 : (len < cap ? len : cap)));
   int64_t p64 = -1;
   if (lane < qlen) p64 = a.positions[q0 + lane];
   my_pos = p64 < 0 ? -1 : (int)(p64 < 0x3fffffff ? p64 : 0x3fffffff);
-  int lo = my_pos < 0 ? 0x7fffffff : my_pos, hi = my_pos;
-#pragma unroll
-  for (int d = 1; d < 64; d *= 2) {
-    lo = min(lo, __shfl_xor(lo, d, 64));
-    hi = max(hi, __shfl_xor(hi, d, 64));
-  }
   Span s;
-  s.pos_min = uniform(lo);
-  s.pos_max = uniform(hi);
+  s.pos_min = wave_reduce(my_pos < 0 ? 0x7fffffff : my_pos, [](int x, int y) { return min(x, y); });
+  s.pos_max = wave_reduce(my_pos, [](int x, int y) { return max(x, y); });
   s.total = s.head = min(ctx, s.pos_max + 1);  // (no row at all: 0)
   s.gap = 0;
   if (a.window > 0 && s.pos_max >= 0) {
@@ -234,10 +241,11 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
   const int split = MODE == kWeights ? rest : rest / a.subsets;
   const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
   const int head0 = hk * (a.G * a.subsets) + sub * a.G;  // first query head
+  const int64_t len = a.context_lens[b];
   const int q0 = uniform(a.cu_seqlens_q[b]);
   const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
   int my_pos;
-  const Span sp = make_span(a, b, q0, qlen, my_pos);
+  const Span sp = make_span(a, len, q0, qlen, my_pos);
   const int per = split_keys<TK>(sp.total, MODE == kWeights ? a.weight_splits : a.S);
   const int v0 = split * per;
   const int v1 = min(sp.total, v0 + per);
@@ -793,7 +801,8 @@ template <int CH>
 __device__ __forceinline__ void stored_weights(const RowArgs& a, int pair, int block) {
   __shared__ float2 stat[kMaxStoredRows];  // maximum and 1 / sum
   const int b = pair / a.Hkv, hk = pair - b * a.Hkv;
-  if (block * 256 >= a.context_lens[b]) return;  // uniform
+  const int64_t len = a.context_lens[b];
+  if (block * 256 >= len) return;  // uniform
   // the scores, the page and the statistics, in one round trip beside the sequence's rows' positions
   const int key = block * 256 + threadIdx.x, rows = a.R * a.subsets;
   const float* src = a.scores + (int64_t)pair * rows * a.score_keys + min(key, a.score_keys - 1);
@@ -809,7 +818,7 @@ __device__ __forceinline__ void stored_weights(const RowArgs& a, int pair, int b
   const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
   join_stats(a, pair * a.subsets, rows, stat);
   int my_pos;
-  const Span sp = make_span(a, b, q0, qlen, my_pos);
+  const Span sp = make_span(a, len, q0, qlen, my_pos);
   __syncthreads();
   if (key >= sp.total || p < 0) return;
   float y = 0.f;
