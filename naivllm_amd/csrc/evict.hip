@@ -460,8 +460,9 @@ MovePlan plan_move(int B, int Hkv, int row_bytes, int64_t cap, int budget, bool 
   // In place, few workgroups take many chunks one after another, each a chain
   // of three round trips: past two chunks by way of staging rows, which any
   // number of workgroups may fill and empty (twice the bytes, a third launch).
-  // 3 sequences of 8 heads, 4,205 rows of 128 bytes: 44 us at once.  Not where
-  // the workgroups fill the chip.
+  // Whole calls, at once against staged: 12,000 -> 4,205 keys of 8 heads, 3
+  // sequences of 128-byte rows 49 and 42 us, 1 of 256 bytes 46 and 34; 4,000 ->
+  // 1,000 (one chunk) 18.1 and 19.8.  Not where the workgroups fill the chip.
   const int64_t columns = row_bytes / (16 << p.lanes_log2);
   if (!apart && budget < cap && units * columns < 256 && most > 2 * chunk()) {
     p.staged = (size_t)units * budget * row_bytes;
