@@ -642,7 +642,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       o += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds.tiles[ww]) + m * DH + ((ch + m) & (DH / 4 - 1)) * 4);
     const float2 ml = lds.row[m];
     if (whole) {
-      if (MODE != kAttend && ch == 0) a.part_ml[part + m] = ml;
+      if (a.key_weights && ch == 0) a.part_ml[part + m] = ml;  // (uniform) for the weights, however these are made
       store_row(m, ch, ml.y == 0.f ? f32x4{0.f, 0.f, 0.f, 0.f} : o * (1.f / ml.y));
     } else if (joins) {
       store16_agent(prs, (unsigned)(m * DH + ch * 4) * 4u, o);

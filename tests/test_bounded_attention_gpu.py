@@ -218,6 +218,17 @@ def test_weights_lengths_holes_and_padding(dtype, block_size):
     _check_weights(vb)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("lens,rows,H,Hkv,D", [([60, 41, 9], 9, 40, 1, 64), ([64, 30], 33, 4, 2, 64),
+                                              ([1100] * 30 + [900, 33], 9, 32, 8, 128)])
+def test_weights_of_whole_sequences_and_keys_read_again(dtype, lens, rows, H, Hkv, D):
+    """No split to join and too many scores to store: by the rows of a kv
+    head, or by the call's."""
+    print(f"case: weights unsplit, {len(lens)} sequences {rows} rows {H}/{Hkv} {dtype}", flush=True)
+    _check_weights(synth.verify_batch(43, lens, [rows] * len(lens) if rows <= 9 else [rows, 30], num_heads=H,
+                                      num_kv_heads=Hkv, head_dim=D, dtype=dtype, block_size=16))
+
+
 def test_weights_rows_behind_the_last_sequence_and_other_places_stay():
     vb = synth.verify_batch(43, [100], [3], dtype="bf16", block_size=16)
     vb.context_lens[0] = 500  # a table wider than the rows reach: keys past the last row keep their place's value
