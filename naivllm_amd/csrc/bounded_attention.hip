@@ -30,15 +30,15 @@
 // over the scores, which the first one stores where a call has few of them
 // (up to 64 rows of a kv head and 32 MiB: 64 pairs, 2 rows, 1,250 keys 15 us
 // against 26 from the keys again; 36 rows over 16k-32k keys, 604 MB of scores,
-// 714 us against 503), or over K again, whose products are made anew.
+// 714 us against 490), or over K again, whose products are made anew.
 //
 // Measured on MI355X, us per call, bytes that it cannot do without per second:
 // window 512 + 4 sinks, 1 row of 16/8 heads 7.7 (latency: the metadata's,
 // the table's and the tiles' round trips); window 4,096, 8 sequences of 9 rows,
 // 32/8 heads, 35 (3.9 TB/s; loads alone 33); fp32, 3 sequences, window 999, 9.2;
 // key weights of 8 sequences of 1,250 keys, 1 row, 15.1 (2.7 TB/s); of 16
-// sequences of 16k-32k keys, 9 rows of 32/8 heads, 500: 309 for the attention
-// (5.2 TB/s), 184 for K again (4.4 TB/s; its loads alone 171).
+// sequences of 16k-32k keys, 9 rows of 32/8 heads, 490: 318 for the attention
+// (5.0 TB/s), 166 for K again (4.8 TB/s).
 
 #include "common.h"
 
@@ -58,7 +58,7 @@ constexpr float kNegInf = -__builtin_inff();
 // (device-scope atomics on one line wait for one another).
 __device__ __forceinline__ int counter_slot(int unit) { return ((unit & 255) << 6) | (unit >> 8); }
 
-enum Mode { kAttend, kAttendScores, kWeights };
+enum Mode { kAttend, kAttendScores, kAttendFirst, kWeights };  // kAttendFirst: kWeights follows
 
 struct RowArgs {
   const void* q;
@@ -334,9 +334,9 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
   auto lds_at = [](const void* p) {
     return (uint32_t)uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p);
   };
-#define NSV_LOAD_LDS(at, offset, src)                                                                 \
-  __asm__ volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off nt" ::"s"(at), \
-                   "v"(src), "n"(offset)                                                              \
+#define NSV_LOAD_LDS(at, offset, src, policy)                                                       \
+  __asm__ volatile("s_add_u32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" policy ::"s"(at), \
+                   "v"(src), "n"(offset)                                                            \
                    : "memory", "m0", "scc")
   auto ktile = [&](int buf) { return mine + buf * (V ? 2 : 1) * S_::TILEB; };
   auto vtile = [&](int buf) { return mine + (buf * 2 + 1) * S_::TILEB; };
@@ -350,8 +350,10 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       const int p = page(key, v < sp.head);
       const uint32_t row = p >= 0 ? (uint32_t)((p << a.bs_log2) + (key & bs_mask)) : (uint32_t)spare;
       const uint64_t off = (uint64_t)row * row_bytes;
-      NSV_LOAD_LDS(kt, j * 1024, kbase + off + ((slot ^ S_::kswz(r)) << 4));
-      if constexpr (V) NSV_LOAD_LDS(vt, j * 1024, vbase + off + ((slot ^ S_::vswz(r)) << 4));
+      const char* ksrc = kbase + off + ((slot ^ S_::kswz(r)) << 4);
+      if constexpr (MODE == kAttendFirst) NSV_LOAD_LDS(kt, j * 1024, ksrc, "");
+      else NSV_LOAD_LDS(kt, j * 1024, ksrc, " nt");
+      if constexpr (V) NSV_LOAD_LDS(vt, j * 1024, vbase + off + ((slot ^ S_::vswz(r)) << 4), " nt");
     }
   };
   auto landed = [&](bool ahead) {
@@ -525,8 +527,12 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     c0 = c1;
     c1 = min(v1, c0 + run);
     const int ntiles = (stage_pages() + TK - 1) / TK;
-    if (w < ntiles) issue(0, w);
-    if (w + kWaves < ntiles) issue(1, w + kWaves);
+    // (kWeights from the last tile back: with K read without the streaming policy
+    // by kAttendFirst, its end is still in the last-level cache.  36 rows over 4,
+    // 8 and 16 sequences of 16k-32k keys: 142, 254 and 492 us -> 135, 241 and 485.)
+    auto at = [&](int t) { return MODE == kWeights ? ntiles - 1 - t : t; };
+    if (w < ntiles) issue(0, at(w));
+    if (w + kWaves < ntiles) issue(1, at(w + kWaves));
     int buf = 0;
     for (int t = w; t < ntiles; t += kWaves) {
       landed(t + kWaves < ntiles);
@@ -546,7 +552,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       if constexpr (V) {
         attend(vtile(buf));
       } else {
-        const int vt = c0 + t * TK;
+        const int vt = c0 + at(t) * TK;
         // uniform: every row sees every key (a key past the run's last, or unmapped, is not written)
         const bool all = min(vt + TK, c1) - 1 <= sp.pos_min;
         float sum[KT];
@@ -576,7 +582,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
       }
       if (t + 2 * kWaves < ntiles) {
         __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the tile is read: its buffer may be filled again
-        issue(buf, t + 2 * kWaves);
+        issue(buf, at(t + 2 * kWaves));
       }
       buf ^= 1;
     }
@@ -934,6 +940,7 @@ template <typename T, int DH>
 int launch_call(RowArgs& a, const RowPlan& p, hipStream_t s) {
   const dim3 grid((unsigned)(a.npairs * p.subsets * p.S));
   if (p.stored) launch_rows<T, DH, kAttendScores>(a, p.MT, grid, s);
+  else if (a.key_weights) launch_rows<T, DH, kAttendFirst>(a, p.MT, grid, s);
   else launch_rows<T, DH, kAttend>(a, p.MT, grid, s);
   int rc = nsv_launch_status();
   if (rc != NSV_OK) return rc;
