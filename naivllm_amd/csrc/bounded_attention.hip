@@ -36,7 +36,7 @@
 // window 512 + 4 sinks, 1 row of 16/8 heads 7.7 (latency: the metadata's,
 // the table's and the tiles' round trips); window 4,096, 8 sequences of 9 rows,
 // 32/8 heads, 35 (3.9 TB/s; loads alone 33); fp32, 3 sequences, window 999, 9.2;
-// key weights of 8 sequences of 1,250 keys, 1 row, 15.1 (2.7 TB/s); of 16
+// key weights of 8 sequences of 1,250 keys, 1 row, 14.6 (2.8 TB/s); of 16
 // sequences of 16k-32k keys, 9 rows of 32/8 heads, 490: 318 for the attention
 // (5.0 TB/s), 166 for K again (4.8 TB/s).
 
@@ -128,15 +128,19 @@ struct Span {
   __device__ int key(int v) const { return v < head ? v : v + gap; }
 };
 
-// (every lane of the wave; the sequence's rows are q0 .. q0 + qlen - 1, its
-// context length, loaded beside them, is len)
-__device__ __forceinline__ Span make_span(const RowArgs& a, int64_t len, int q0, int qlen, int& my_pos) {
+// The position of the sequence's row `lane` (whatever behind the last of them:
+// a load under a condition would be waited for there).
+__device__ __forceinline__ int64_t row_position(const RowArgs& a, int q0, int qlen) {
+  return a.positions[max(q0 + min((int)(threadIdx.x & 63), qlen - 1), 0)];  // (T > 0)
+}
+
+// (every lane of the wave; the sequence's rows are q0 .. q0 + qlen - 1, p64
+// their positions, len its context length)
+__device__ __forceinline__ Span make_span(const RowArgs& a, int64_t len, int qlen, int64_t p64, int& my_pos) {
   const int lane = threadIdx.x & 63;
   const int64_t cap = (int64_t)a.max_blocks << a.bs_log2;
   const int ctx = uniform((int)(len < 0 ? 0 : (len < cap ? len : cap)));
-  int64_t p64 = -1;
-  if (lane < qlen) p64 = a.positions[q0 + lane];
-  my_pos = p64 < 0 ? -1 : (int)(p64 < 0x3fffffff ? p64 : 0x3fffffff);
+  my_pos = lane >= qlen || p64 < 0 ? -1 : (int)(p64 < 0x3fffffff ? p64 : 0x3fffffff);
   Span s;
   s.pos_min = wave_reduce(my_pos < 0 ? 0x7fffffff : my_pos, [](int x, int y) { return min(x, y); });
   s.pos_max = wave_reduce(my_pos, [](int x, int y) { return max(x, y); });
@@ -167,17 +171,14 @@ __device__ __forceinline__ int split_keys(int total, int S) {
 // row, each with every fourth split, all of them loaded in one round trip (a
 // wave per row and a lane per split took 14 us for 64 rows).  A row that sees
 // nothing: 0 and 0.
-__device__ __forceinline__ void join_stats(const RowArgs& a, int ps, int rows, float2* stat) {
-  constexpr int N = kMaxSplits / 4;
+template <int N>  // 4 N >= a.S
+__device__ __forceinline__ void join_stats_of(const RowArgs& a, int ps, int rows, float2* stat) {
   const int j = threadIdx.x & 3, m = threadIdx.x >> 2;
   const int row = min(m, rows - 1), sub = row / a.R;  // (rows may run on into the pair's next subsets)
   const float2* src = a.part_ml + (int64_t)(ps + sub) * a.S * a.R + row - sub * a.R;
   float2 x[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) {
-    x[k] = make_float2(kNegInf, 0.f);
-    if (4 * k < a.S) x[k] = src[(int64_t)min(4 * k + j, a.S - 1) * a.R];  // uniform
-  }
+  for (int k = 0; k < N; ++k) x[k] = src[(int64_t)min(4 * k + j, a.S - 1) * a.R];
   float M = kNegInf, L = 0.f;
 #pragma unroll
   for (int k = 0; k < N; ++k) M = fmaxf(M, x[k].x);  // (a split read twice changes nothing here)
@@ -185,11 +186,17 @@ __device__ __forceinline__ void join_stats(const RowArgs& a, int ps, int rows, f
   M = fmaxf(M, dpp_f32<kDppXor2>(M));
   const float ref = M == kNegInf ? 0.f : M;
 #pragma unroll
-  for (int k = 0; k < N; ++k)
-    if (4 * k < a.S) L += 4 * k + j < a.S ? x[k].y * __builtin_amdgcn_exp2f(x[k].x - ref) : 0.f;
+  for (int k = 0; k < N; ++k) L += 4 * k + j < a.S ? x[k].y * __builtin_amdgcn_exp2f(x[k].x - ref) : 0.f;
   L += dpp_f32<kDppXor1>(L);
   L += dpp_f32<kDppXor2>(L);
   if (j == 0 && m < rows) stat[m] = make_float2(ref, L == 0.f ? 0.f : 1.f / L);
+}
+
+__device__ __forceinline__ void join_stats(const RowArgs& a, int ps, int rows, float2* stat) {
+  static_assert(kMaxSplits == 64, "four lanes take every split");
+  if (a.S <= 4) join_stats_of<1>(a, ps, rows, stat);  // uniform
+  else if (a.S <= 8) join_stats_of<2>(a, ps, rows, stat);
+  else join_stats_of<16>(a, ps, rows, stat);
 }
 
 template <typename T, int DH>
@@ -245,7 +252,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
   const int q0 = uniform(a.cu_seqlens_q[b]);
   const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
   int my_pos;
-  const Span sp = make_span(a, len, q0, qlen, my_pos);
+  const Span sp = make_span(a, len, qlen, row_position(a, q0, qlen), my_pos);
   const int per = split_keys<TK>(sp.total, MODE == kWeights ? a.weight_splits : a.S);
   const int v0 = split * per;
   const int v1 = min(sp.total, v0 + per);
@@ -822,9 +829,10 @@ __device__ __forceinline__ void stored_weights(const RowArgs& a, int pair, int b
   const int p = a.block_tables[(int64_t)b * a.max_blocks + entry];
   const int q0 = uniform(a.cu_seqlens_q[b]);
   const int qlen = min(uniform(a.cu_seqlens_q[b + 1]) - q0, a.QL);
+  const int64_t p64 = row_position(a, q0, qlen);
   join_stats(a, pair * a.subsets, rows, stat);
   int my_pos;
-  const Span sp = make_span(a, len, q0, qlen, my_pos);
+  const Span sp = make_span(a, len, qlen, p64, my_pos);
   __syncthreads();
   if (key >= sp.total || p < 0) return;
   float y = 0.f;
