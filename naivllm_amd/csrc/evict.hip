@@ -9,7 +9,7 @@
 // Selection (evict_select_kernel), one workgroup of 16 waves per (sequence, kv
 // head): the weights are read once into registers, four neighbours per load
 // (beyond 32,768 keys, and of pages of fewer than four keys, they are read again
-// in every pass), and compared as unsigned words of the same order, in which the
+// in every pass: 131,072 keys of 8 heads 135 us), and compared as unsigned words of the same order, in which the
 // keys that stay anyway are the largest.  The budget-th largest word comes from
 // three passes over 11, 11 and 10 bits (four histograms, taken by a wave's lanes
 // in turn: weights share few leading digits, and equal adds wait for one
@@ -41,6 +41,7 @@
 #include "common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace {
 
@@ -48,6 +49,7 @@ constexpr int kSelThreads = 1024;
 constexpr int kSelWaves = kSelThreads / 64;
 constexpr int kSelLoads = 8;     // loads of four weights that a thread holds: 32,768 keys in all
 constexpr int kBins = 2048, kCopies = 4;
+constexpr int kAgain = 4;        // loads in a round trip where the weights are read again
 constexpr int kOutPages = 4096;  // entries of the destination's table held in LDS
 constexpr int kMoveThreads = 512;
 constexpr int kMoveUnroll = 8;   // 16-byte pieces per lane and chunk
@@ -109,9 +111,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   const int32_t* ot = a.out_tables + (int64_t)b * a.out_blocks;
   const bool apart = a.out_tables != a.block_tables;
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
-  auto place = [&](const int32_t* table, int key) -> int64_t {  // of a key's weight; -1: no page
-    const int p = table[key >> a.bs_log2];
-    return p < 0 ? -1 : ((((int64_t)p * a.Hkv + h) << a.bs_log2) + (key & bs_mask));
+  auto at = [&](int page, int key) {  // the weight of a key there (of a hole: page 0's)
+    return a.weights + ((((int64_t)max(page, 0) * a.Hkv + h) << a.bs_log2) + (key & bs_mask));
   };
   if (tid == 0 && h == 0) a.lens[b] = got;
   for (int i = got + tid; i < a.budget; i += kSelThreads) kept[i] = -1;
@@ -120,21 +121,37 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     return;
   }
 
-  // keys key .. key + 3 (key a multiple of 4); past the context and in unmapped pages: whatever
-  auto load4 = [&](int key) {
-    f32x4 x = {0.f, 0.f, 0.f, 0.f};
-    if (key >= n) return x;
+  // The weights of keys key[u] .. key[u] + 3 (multiples of 4), 0 in a hole, past
+  // the context whatever: every page in one round trip, then every weight.  (Past
+  // the context the last key's are loaded, of a hole page 0's: a load under a
+  // condition would be waited for there.)
+  auto fetch = [&](const auto& key, auto& x, auto count) {
+    constexpr int U = decltype(count)::value;
     if (a.vector) {  // uniform: pages of four keys or more, on 16 bytes
-      const int64_t at = place(bt, key);
-      if (at >= 0) x = *reinterpret_cast<const f32x4*>(a.weights + at);
-    } else {
+      int page[U];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int64_t at = key + j < n ? place(bt, key + j) : -1;
-        if (at >= 0) x[j] = a.weights[at];
-      }
+      for (int u = 0; u < U; ++u) page[u] = bt[min(key[u], n - 1) >> a.bs_log2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = *reinterpret_cast<const f32x4*>(at(page[u], min(key[u], (n - 1) & ~3)));
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[u][j] = page[u] >= 0 ? x[u][j] : 0.f;
+    } else {
+      int page[U][4];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) page[u][j] = bt[min(key[u] + j, n - 1) >> a.bs_log2];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[u][j] = *at(page[u][j], min(key[u] + j, n - 1));
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[u][j] = page[u][j] >= 0 ? x[u][j] : 0.f;
     }
-    return x;
   };
   // words of keys key .. key + 3: the largest for keys that stay anyway, 0 (less than every weight's) past the context
   auto words = [&](int key, f32x4 x) {
@@ -159,7 +176,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     for (int e = 0; e < kSelLoads; ++e)
       if (e < loads) {  // (past the context the last key's group, of a hole page 0: a load under a condition would be waited for)
         const int key = min(e * STEP + tid * 4, (n - 1) & ~3);
-        held[e] = *reinterpret_cast<const f32x4*>(a.weights + ((((int64_t)max(page[e], 0) * a.Hkv + h) << a.bs_log2) + (key & bs_mask)));
+        held[e] = *reinterpret_cast<const f32x4*>(at(page[e], key));
         mapped |= page[e] >= 0 ? 1u << e : 0u;
       }
   }
@@ -189,10 +206,15 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
           f(e, key, held[e], word[e]);
         }
     } else {
-      for (int e = 0; e < loads; ++e) {
-        const int key = e * STEP + tid * 4;
-        const f32x4 x = load4(key);
-        f(e, key, x, words(key, x));
+      for (int e0 = 0; e0 < loads; e0 += kAgain) {
+        int key[kAgain];
+        f32x4 x[kAgain];
+#pragma unroll
+        for (int u = 0; u < kAgain; ++u) key[u] = (e0 + u) * STEP + tid * 4;
+        fetch(key, x, std::integral_constant<int, kAgain>{});
+#pragma unroll
+        for (int u = 0; u < kAgain; ++u)
+          if (e0 + u < loads) f(e0 + u, key[u], x[u], words(key[u], x[u]));  // uniform
       }
     }
   };
@@ -316,8 +338,8 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
     if constexpr (!HELD) {
       each([&](int e, int key, f32x4, u32x4 u) {
         if (e < e0 || e >= e0 + GROUP) return;  // uniform
-        const int at = (e - e0) * kSelWaves + w, own = counts(u);
-        emit(u, count_gt[at], count_eq[at], wave_scan(own) - own, [&](int j, int i) { kept[i] = key + j; });
+        const int c = (e - e0) * kSelWaves + w, own = counts(u);
+        emit(u, count_gt[c], count_eq[c], wave_scan(own) - own, [&](int j, int i) { kept[i] = key + j; });
       });
     }
   }
@@ -340,7 +362,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
         kept[i] = x.x < 0 ? ~x.x : x.x;
         const int pi = i >> a.bs_log2;
         const int p = pi < kOutPages ? out_page[pi] : ot[pi];
-        if (x.x >= 0 && p >= 0) a.weights[(((int64_t)p * a.Hkv + h) << a.bs_log2) + (i & bs_mask)] = __int_as_float(x.y);
+        if (x.x >= 0 && p >= 0) *at(p, i) = __int_as_float(x.y);
       }
       if (i0 + kPlaces < got) __syncthreads();
     }
@@ -348,14 +370,25 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   if constexpr (!HELD) {
     // the weights themselves, a chunk at a time: every read of a chunk before its first write
     __syncthreads();
-    for (int i0 = 0; i0 < got; i0 += kSelThreads) {
-      const int i = i0 + tid;
-      const int64_t at = i < got ? place(bt, kept[i]) : -1;
-      const float x = at >= 0 ? a.weights[at] : 0.f;
+    for (int i0 = 0; i0 < got; i0 += kSelThreads * kMoveUnroll) {
+      int key[kMoveUnroll], from[kMoveUnroll], to[kMoveUnroll];
+      float x[kMoveUnroll];
+#pragma unroll
+      for (int u = 0; u < kMoveUnroll; ++u) key[u] = kept[min(i0 + u * kSelThreads + tid, got - 1)];
+#pragma unroll
+      for (int u = 0; u < kMoveUnroll; ++u) {
+        from[u] = bt[key[u] >> a.bs_log2];
+        to[u] = ot[min(i0 + u * kSelThreads + tid, got - 1) >> a.bs_log2];
+      }
+#pragma unroll
+      for (int u = 0; u < kMoveUnroll; ++u) x[u] = *at(from[u], key[u]);
       loads_back();
       __syncthreads();
-      const int64_t to = at >= 0 ? place(ot, i) : -1;
-      if (to >= 0) a.weights[to] = x;
+#pragma unroll
+      for (int u = 0; u < kMoveUnroll; ++u) {
+        const int i = i0 + u * kSelThreads + tid;
+        if (i < got && from[u] >= 0 && to[u] >= 0) *at(to[u], i) = x[u];
+      }
       __syncthreads();
     }
   }

@@ -133,3 +133,12 @@ def test_weights_off_their_alignment():
     torch.cuda.synchronize()
     for a, b in zip(*results):
         assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("block_size,apart", [(64, False), (16, True), (2, False)])
+def test_long_contexts_of_many_kept_keys(block_size, apart):
+    print(f"case: evict 50000 -> 20001 keys, pages of {block_size}, apart {apart}", flush=True)
+    lens = [50000, 33000, 20002]
+    pages = -(-20001 // block_size)
+    k, v, w, tables, free = _case(81, lens, 1, 32, block_size, levels=500, spare=3 * pages)
+    _check(k, v, w, tables, lens, 20001, 4, 100, free[:3 * pages].reshape(3, pages).copy() if apart else None)
