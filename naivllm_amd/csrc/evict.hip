@@ -25,10 +25,12 @@
 // 128 bytes of it where there are few sequences, and takes its rows in
 // ascending chunks, each read whole before it is written and the next one's
 // reads under way: what a chunk overwrites no later chunk reads, and no other
-// workgroup touches the column.  Between tables apart nothing can be
-// overwritten, and the rows are dealt to many workgroups; so they are where few
-// sequences have long rows to move, by way of staging rows.  Bound by the rows'
-// bytes.
+// workgroup touches the column.  Between tables that share no page nothing can
+// be overwritten, and the rows are dealt to many workgroups; so they are where
+// few sequences have long rows to move, by way of staging rows.  A second table
+// may also be a copy of the first, or keep some of its pages at their places:
+// every workgroup compares the two, and such a sequence is moved as in place.
+// Bound by the rows' bytes.
 //
 // Measured on MI355X: one sequence, 1,250 -> 512 keys of 8 heads, bf16, D 128,
 // to pages apart: 9.0 us of selection, 3.5 of moving; 16 sequences of 16k-32k
@@ -452,8 +454,31 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
     }
   };
   Chunk c;
-  if (apart || MOVE != kAtOnce) {
+  if (MOVE != kAtOnce) {
     for (int i0 = blockIdx.z * chunk; i0 < got; i0 += gridDim.z * chunk) {
+      read(c, i0);
+      write(c, i0);
+    }
+    return;
+  }
+  const int first = blockIdx.z * chunk;  // (in place: 0)
+  if (first >= got) return;  // uniform
+  const int pages = ((got - 1) >> a.bs_log2) + 1, mine = min((int)threadIdx.x, pages - 1);
+  const int from = bt[mine], into = ot[mine];
+  read(c, first);
+  bool ordered = !apart;
+  if (apart && n > a.budget) {  // uniform
+    // Another table may hold pages of this one at their places, in which rows
+    // move as they do in place: one workgroup takes the column then.  (Its
+    // entries are looked up beside the first chunk, and before any write.)
+    int same = from >= 0 && from == into;
+    for (int i = kMoveThreads + threadIdx.x; i < pages; i += kMoveThreads) same |= bt[i] >= 0 && bt[i] == ot[i];
+    ordered = __syncthreads_or(same) != 0;
+    if (ordered && blockIdx.z > 0) return;  // uniform
+  }
+  if (!ordered) {
+    write(c, first);
+    for (int i0 = first + gridDim.z * chunk; i0 < got; i0 += gridDim.z * chunk) {
       read(c, i0);
       write(c, i0);
     }
@@ -461,7 +486,6 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
   }
   // (the next chunk's sources lie behind this chunk's destinations; the barrier
   // puts every read of a chunk before its first write)
-  read(c, 0);
   for (int i0 = 0; i0 < got; i0 += chunk) {
     Chunk next;
     loads_back();

@@ -712,9 +712,12 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: tor
     float32) and ``key_weights`` (num_blocks, Hkv, block_size) move, in the
     order of their positions, to the first places of the sequence's table, or
     of its row of ``out_block_tables`` (which also gets the sequences that are
-    short enough; their old pages keep what they hold, so it is the form for
-    pages that other sequences share).  Every page of the context must be
-    mapped; pages of out_block_tables must be no other pages of block_tables.
+    short enough; pages of the old table that the new one does not hold keep
+    what they hold, so it is the form for pages that other sequences share).
+    Every page of the context must be mapped.  A sequence's new row may hold
+    pages of its old one at the same places (a copy of the table, its first
+    columns), but no page of ``block_tables`` at another place or of another
+    sequence.
 
     Returns (lens (B,) int64: min(length, budget); kept (B, Hkv, budget)
     int32: the positions that stay, ascending, -1 behind the last).  Keys hold
