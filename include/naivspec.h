@@ -266,7 +266,8 @@ int nsv_prefill_key_weights(const void* q, const void* k_cache,
  * its first columns), but nowhere else in block_tables.  Supported: rows of a
  * multiple of 64 bytes; block_size a power of two; sinks + recent <= budget.
  * Workspace: nsv_evict_workspace_size() bytes on 16 bytes (0: none; apart:
- * whether out_block_tables will be another table), of any content.
+ * whether out_block_tables will be another table: not NULL, and at another
+ * address or of another width), of any content.
  */
 size_t nsv_evict_workspace_size(int B, int Hkv, int D, int block_size,
                                 int max_blocks, int apart, int dtype,

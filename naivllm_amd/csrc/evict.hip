@@ -61,12 +61,13 @@ struct EvictArgs {
   char* v;
   float* weights;                // [num_blocks][Hkv][block_size]
   const int32_t* block_tables;
-  const int32_t* out_tables;     // = block_tables: in place
+  const int32_t* out_tables;
   const int64_t* context_lens;
   int64_t* lens;                 // [B]
   int32_t* kept;                 // [B][Hkv][budget]
   int Hkv, row_bytes, bs_log2, max_blocks, out_blocks, budget, sinks, recent;
   int vector;                    // four weights of a page in one load
+  int apart;                     // out_tables is another table
   char* staged;                  // null, or [B][Hkv][2][budget] rows: K, V by way of it
 };
 
@@ -111,7 +112,7 @@ __global__ __launch_bounds__(kSelThreads) void evict_select_kernel(EvictArgs a) 
   const int bs_mask = (1 << a.bs_log2) - 1;
   const int32_t* bt = a.block_tables + (int64_t)b * a.max_blocks;
   const int32_t* ot = a.out_tables + (int64_t)b * a.out_blocks;
-  const bool apart = a.out_tables != a.block_tables;
+  const bool apart = a.apart != 0;
   int32_t* kept = a.kept + (int64_t)blockIdx.x * a.budget;
   auto at = [&](int page, int key) {  // the weight of a key there (of a hole: page 0's)
     return a.weights + ((((int64_t)max(page, 0) * a.Hkv + h) << a.bs_log2) + (key & bs_mask));
@@ -408,7 +409,7 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
   const int column = blockIdx.x % columns, rest = blockIdx.x / columns;
   const int h = rest % a.Hkv, b = rest / a.Hkv;
   const int n = clamp_len(a, b), got = min(n, a.budget);
-  const bool apart = a.out_tables != a.block_tables;
+  const bool apart = a.apart != 0;
   if (got == 0 || (n <= a.budget && !apart)) return;  // uniform: nothing moves
   const int bs_mask = (1 << a.bs_log2) - 1;
   const int32_t* bt = a.block_tables + (int64_t)b * a.max_blocks;
@@ -556,7 +557,7 @@ int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights, const int32_t
                  const int64_t* context_lens, const int32_t* out_block_tables, int64_t* lens, int32_t* kept, int B,
                  int Hkv, int D, int block_size, int max_blocks, int out_blocks, int dtype, int budget, int sinks,
                  int recent, void* workspace, size_t workspace_bytes, void* stream) {
-  const bool apart = out_block_tables && out_block_tables != block_tables;
+  const bool apart = out_block_tables && (out_block_tables != block_tables || out_blocks != max_blocks);
   const int bad = evict_args(B, Hkv, D, block_size, max_blocks, out_blocks, out_block_tables != nullptr, dtype, budget, sinks,
                              recent);
   if (bad != NSV_OK) return bad;
@@ -571,7 +572,7 @@ int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights, const int32_t
   while ((1 << bs_log2) < block_size) ++bs_log2;
   EvictArgs a{(char*)k_cache, (char*)v_cache, key_weights, block_tables, apart ? out_block_tables : block_tables,
               context_lens, lens, kept, Hkv, row_bytes, bs_log2, max_blocks, apart ? out_blocks : max_blocks,
-              budget, sinks, recent, bs_log2 >= 2 && (uintptr_t)key_weights % 16 == 0, (char*)workspace};
+              budget, sinks, recent, bs_log2 >= 2 && (uintptr_t)key_weights % 16 == 0, apart, (char*)workspace};
   hipStream_t s = (hipStream_t)stream;
   if (cap <= (int64_t)kSelThreads * 4 * kSelLoads && a.vector)
     hipLaunchKernelGGL(evict_select_kernel<true>, dim3(B * Hkv), dim3(kSelThreads), 0, s, a);

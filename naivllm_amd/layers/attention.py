@@ -699,6 +699,16 @@ def prefill_key_weights(query: torch.Tensor, k_cache: torch.Tensor, key_weights:
     _lib.check(rc, "prefill_key_weights")
 
 
+def _evict_tables(block_tables: torch.Tensor, out_block_tables: torch.Tensor | None) -> tuple:
+    """The two tables in the kernel's type, the second None where it is the
+    first one itself (an eviction in place)."""
+    tables = _as(block_tables, "block_tables")
+    if out_block_tables is None or out_block_tables is block_tables:
+        return tables, None
+    out = _as(out_block_tables, "block_tables")
+    return tables, None if out.data_ptr() == tables.data_ptr() and out.shape == tables.shape else out
+
+
 def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: torch.Tensor, block_tables: torch.Tensor,
                   context_lens: torch.Tensor, budget: int, *, sinks: int = 0, recent: int = 0,
                   out_block_tables: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
@@ -746,9 +756,8 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: tor
         raise ValueError(f"out_block_tables of {out_block_tables.shape[1]} pages do not hold {budget} keys")
     if nb * bs > 0x7fffffff:
         raise ValueError(f"evict_kvcache addresses fewer than 2^31 cached keys, got {nb} pages of {bs}")
-    block_tables, context_lens = _as(block_tables, "block_tables"), _as(context_lens, "context_lens")
-    if out_block_tables is not None:
-        out_block_tables = _as(out_block_tables, "block_tables")
+    block_tables, out_block_tables = _evict_tables(block_tables, out_block_tables)
+    context_lens = _as(context_lens, "context_lens")
     lens = torch.empty(B, dtype=torch.int64, device=dev)
     kept = torch.empty((B, hkv, budget), dtype=torch.int32, device=dev)
     code = _lib.dtype_code(k_cache.dtype)

@@ -41,6 +41,14 @@ SHAPES = [dict(lens=[700, 150, 20], budget=300, Hkv=2, D=64, block_size=16),
 
 
 @pytest.mark.parametrize("shape", SHAPES, ids=["short", "staged", "long"])
+@pytest.mark.parametrize("index", [torch.int32, torch.int64])
+def test_the_table_itself_is_in_place(shape, index):
+    print(f"case: evict to the same table {shape} {index}", flush=True)
+    case = _case(121, shape["lens"], shape["Hkv"], shape["D"], shape["block_size"])
+    _check(case, shape["lens"], shape["budget"], lambda t: t, index=index)
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=["short", "staged", "long"])
 @pytest.mark.parametrize("how", ["clone", "narrow"])
 def test_copies_of_the_table(shape, how):
     print(f"case: evict to a {how} of the table {shape}", flush=True)
@@ -48,6 +56,12 @@ def test_copies_of_the_table(shape, how):
     pages = -(-shape["budget"] // shape["block_size"])
     out = case[3] if how == "clone" else np.ascontiguousarray(case[3][:, :pages])
     _check(case, shape["lens"], shape["budget"], lambda t: t.clone() if how == "clone" else t[:, :pages].clone(), out)
+
+
+def test_a_narrower_view_of_one_sequence():
+    print("case: evict to a view at the table's own address", flush=True)
+    case = _case(123, [700], 2, 64, 16)
+    _check(case, [700], 300, lambda t: t[:, :19], np.ascontiguousarray(case[3][:, :19]))
 
 
 @pytest.mark.parametrize("block_size", [1, 16])
