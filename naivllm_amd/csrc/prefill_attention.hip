@@ -514,6 +514,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
     if (h == 0) *reinterpret_cast<float2*>(base + a.tile_rows * DH + 2 * r) = make_float2(m_ref * sc, L);
     return;
   }
+  if (a.stats && h == 0 && r < nrows) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(m_ref * sc, L == 0.f ? 0.f : 1.f / L);
   if constexpr (WIN && NW == 4) {
     // Short ranges of keys, where the ends of a workgroup weigh: the wave's rows
     // through LDS (its own part of the tiles, once every wave is done with
@@ -544,7 +545,6 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
     return;
   }
   if (r < nrows) {
-    if (a.stats && h == 0) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(m_ref * sc, L == 0.f ? 0.f : 1.f / L);
     bf16_t* dst = a.out + ((int64_t)(row0 + r) * a.H + head) * DH + h * 4;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)

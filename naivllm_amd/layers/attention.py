@@ -603,7 +603,7 @@ def prefill_attention(query: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pla
     window in the plan every row sees that many keys and the first ``sinks``
     (no reference counterpart), and keys that no row sees are not read.
     ``stats``: an fp32 [rows, H, 2] that takes the rows' softmax statistics,
-    for prefill_key_weights (not written where the plan has a window)."""
+    for prefill_key_weights (a plan with a window is refused then)."""
     H, Hkv = plan.num_heads, plan.num_kv_heads
     if not query.is_cuda:
         raise ValueError("prefill_attention runs on the GPU; query is on the CPU")

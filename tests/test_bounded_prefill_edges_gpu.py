@@ -1,0 +1,72 @@
+"""The prompts' bounded operators at their edges."""
+
+import numpy as np
+import pytest
+import torch
+
+from naivllm_amd import _lib
+from naivllm_amd.layers.attention import PrefillPlan
+from naivllm_amd.utils import synth
+from oracle import bounded as ob
+from tests.bounded_util import EPS32, check_attention, weight_error
+from tests.gpu_util import to_device
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+def _batch(seed, new, prefix, H=4, Hkv=2, D=128, block_size=64):
+    return synth.verify_batch(seed, [p + n for p, n in zip(prefix, new)], new, num_heads=H, num_kv_heads=Hkv, head_dim=D,
+                              block_size=block_size)
+
+
+def _lse2(vb, scale, window, sinks):
+    """log2 of every row's sum of exponentials [T, H], and the scores' magnitudes."""
+    lse, mag = np.full((len(vb.q), vb.num_heads), -np.inf), np.zeros((len(vb.q), vb.num_heads))
+    G = vb.num_heads // vb.num_kv_heads
+    for b, n in enumerate(vb.context_lens):
+        j, rows = np.arange(n), slice(vb.cu_seqlens_q[b], vb.cu_seqlens_q[b + 1])
+        seen = ob.visible(vb.positions[rows], j, window or None, sinks)
+        page = vb.block_tables[b, j // vb.block_size]
+        for h in range(vb.num_heads):
+            K = vb.k_cache[page, j % vb.block_size, h // G]
+            s = np.where(seen, vb.q[rows, h] @ K.T * scale, -np.inf) * np.log2(np.e)
+            top = s.max(1)
+            lse[rows, h] = top + np.log2(np.exp2(s - top[:, None]).sum(1))
+            mag[rows, h] = (np.abs(vb.q[rows, h]) @ np.abs(K).T * seen).max(1) * abs(scale)
+    return lse, mag
+
+
+@pytest.mark.parametrize("new,prefix,H,Hkv,window,sinks,waves,cut", [
+    ([500, 1, 77, 130], [0, 0, 300, 65], 4, 2, 100, 4, 4, False),
+    ([40], [1500], 2, 1, 900, 3, 4, True),         # keys cut over workgroups
+    ([1100] * 4, [2200] * 4, 16, 8, 1700, 4, 8, False),
+    ([900], [3000], 2, 1, 1700, 70, 8, True),
+    ([300, 90], [0, 200], 3, 1, 0, 0, 4, False)])  # no window
+def test_statistics_of_the_library_entry(new, prefix, H, Hkv, window, sinks, waves, cut):
+    """nsv_prefill_window_attention leaves every row's (m, r), under a window
+    as without one, beside its outputs."""
+    print(f"case: statistics {new} window {window}", flush=True)
+    vb = _batch(101, new, prefix, H, Hkv)
+    t = to_device(vb)
+    ends, scale = vb.context_lens.tolist(), 1.0 / np.sqrt(128)
+    plan = PrefillPlan(new, ends, H, Hkv, 64, DEV, window=window, sinks=sinks)
+    assert (plan.nmerges > 0) == cut and plan.tile_rows * (2 if H // Hkv % 2 == 0 else 1) == 32 * waves
+    out = torch.empty_like(t["query"])
+    stats = torch.full((sum(new), H, 2), float("nan"), device="cuda")
+    part = torch.empty(max(1, plan.slots) * H * plan.tile_rows * 130, device="cuda")
+    at = plan.work.data_ptr()
+    rc = _lib.lib().nsv_prefill_window_attention(
+        out.data_ptr(), t["query"].data_ptr(), t["k_cache"].data_ptr(), t["v_cache"].data_ptr(),
+        t["block_tables"].data_ptr(), at, plan.ntiles, plan.tile_rows, at + plan.ntiles * 32, plan.nmerges, scale, H, Hkv,
+        128, 64, vb.block_tables.shape[1], window, sinks, stats.data_ptr(), part.data_ptr(),
+        torch.cuda.current_stream().cuda_stream)
+    torch.cuda.synchronize()
+    assert rc == 0
+    check_attention(out, *ob.attention(vb.q, vb.k_cache, vb.v_cache, vb.block_tables, vb.context_lens, vb.cu_seqlens_q,
+                                       vb.positions, scale, Hkv, window or None, sinks)[:3], "bf16", max(ends))
+    want, mag = _lse2(vb, scale, window, sinks)
+    m, r = stats.cpu().numpy().astype(np.float64).transpose(2, 0, 1)
+    # the sum's relative error is a weight's; m is rounded once, r twice (its sum's and its own)
+    bound = np.log2(np.e) * (weight_error(mag, max(ends), 128) + 4 * EPS32) + EPS32 * (np.abs(m) + mag * np.log2(np.e))
+    assert (np.abs(m - np.log2(r) - want) <= bound).all()
