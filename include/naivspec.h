@@ -136,6 +136,8 @@ int nsv_window_attention(void* out, const void* q, const void* k_cache,
  * The place of a key at or behind the position of its sequence's first row
  * is set, an older key's added to; places of keys past the last row and of
  * unmapped pages keep their value.  Rows with positions[r] < 0 add nothing.
+ * A place of several sequences (a page that they share) gets the sum of
+ * theirs, in no fixed order, set where one of them says set.
  * No reference counterpart.  Shapes and workspace as nsv_window_attention's.
  */
 size_t nsv_weights_attention_workspace_size(int B, int H, int Hkv, int D,
@@ -227,7 +229,8 @@ int nsv_prefill_window_attention(
  * paged key_weights of nsv_weights_attention: for each (key, kv head) over
  * the rows at or behind the key and the kv head's query heads.  Keys of the
  * step itself (at or behind a sequence's first row) are set, older ones added
- * to.  No reference counterpart.
+ * to; a place of several sequences as nsv_weights_attention's.  No reference
+ * counterpart.
  *   q        [rows, H, D], the sequences' rows back to back
  *   stats    what nsv_prefill_window_attention (window 0) left for the same q,
  *            K and scale

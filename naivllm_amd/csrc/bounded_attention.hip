@@ -534,6 +534,17 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     c0 = c1;
     c1 = min(v1, c0 + run);
     const int ntiles = (stage_pages() + TK - 1) / TK;
+    // The call's new keys start from zero, to which the launches behind this one
+    // add: another sequence may have the same page behind it (a prefix that one
+    // sequence of the step computes and the next shares).
+    if constexpr (MODE == kAttendScores || MODE == kAttendFirst) {
+      if (sub == 0 && ntiles > 0 && sp.pos_min < c1) {  // uniform
+        for (int v = max(c0, sp.pos_min) + tid; v < c1; v += NT) {
+          const int p = page(v, true);
+          if (p >= 0) a.key_weights[((int64_t)p * a.Hkv + hk) * (bs_mask + 1) + (v & bs_mask)] = 0.f;
+        }
+      }
+    }
     // (kWeights from the last tile back: with K read without the streaming policy
     // by kAttendFirst, its end is still in the last-level cache.  36 rows over 4,
     // 8 and 16 sequences of 16k-32k keys: 142, 254 and 492 us -> 135, 241 and 485.)
@@ -581,9 +592,7 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
           const int p = page(v, true);
           if (p >= 0) {
             const float y = KT == 1 || g == 0 ? sum[0] : sum[KT - 1];
-            float* dst = a.key_weights + ((int64_t)p * a.Hkv + hk) * (bs_mask + 1) + (v & bs_mask);
-            if (v >= sp.pos_min && sub == 0) *dst = y;
-            else unsafeAtomicAdd(dst, y);
+            unsafeAtomicAdd(a.key_weights + ((int64_t)p * a.Hkv + hk) * (bs_mask + 1) + (v & bs_mask), y);
           }
         }
       }
@@ -737,9 +746,9 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
 // without a key of the row (maximum -inf) holds no output.
 //
 // Workgroups behind them: 256 keys of a pair, one per thread, for all its
-// rows, whose statistics they join themselves.  A weight of a key at or behind
-// the sequence's first row is set, an older one's added to (one thread adds to
-// a place; an atomic add, so that sequences which share a page lose nothing).
+// rows, whose statistics they join themselves.  One thread adds to a place (of a
+// key at or behind the sequence's first row: to the zero that the attention left
+// there), by an atomic add, so that sequences which share a page lose nothing.
 // ---------------------------------------------------------------------------
 template <typename T, int DH>
 __device__ __forceinline__ void merge_rows(const RowArgs& a, int ps, int block, int sg_log2) {
@@ -845,9 +854,7 @@ __device__ __forceinline__ void stored_weights(const RowArgs& a, int pair, int b
       y = on ? fmaf(__builtin_amdgcn_exp2f(s[k] - x.x), x.y, y) : y;
     }
   }
-  float* dst = a.key_weights + (((int64_t)p * a.Hkv + hk) << a.bs_log2) + (key & ((1 << a.bs_log2) - 1));
-  if (key >= sp.pos_min) *dst = y;
-  else unsafeAtomicAdd(dst, y);
+  unsafeAtomicAdd(a.key_weights + (((int64_t)p * a.Hkv + hk) << a.bs_log2) + (key & ((1 << a.bs_log2) - 1)), y);
 }
 
 template <typename T, int DH>

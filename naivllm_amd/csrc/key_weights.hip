@@ -52,6 +52,7 @@ struct KeyWeightsArgs {
   const int32_t* units;         // [n][kUnitWords]: sequence, first key, keys, row of q of the sequence's first, rows,
                                 // position of that row, first (head, row tile), end
   float* part;                  // [units][Hkv][kBlockKeys]
+  float* key_weights;           // [num_blocks][Hkv][block_size]
   float scale_log2;
   int H, Hkv, bs_log2, max_blocks;
 };
@@ -78,6 +79,15 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs a) {
   const int G = a.H / a.Hkv;
   const int first = max(0, key0 - pos0);              // the first row that sees a key of the block
   const int tiles = (nrows - first + kRows - 1) / kRows;  // per head
+
+  // the step's own keys start from zero, to which key_sum_kernel adds: another
+  // sequence may have the same page behind it (a prefix that one sequence of the
+  // step computes and the next shares)
+  if (t_begin == 0 && tid < nkeys && key0 + tid >= pos0) {  // (one unit per block of keys begins at 0)
+    const int key = key0 + tid, entry = key >> a.bs_log2;
+    const int p = entry < a.max_blocks ? a.block_tables[(int64_t)seq * a.max_blocks + entry] : -1;
+    if (p >= 0) a.key_weights[(((int64_t)p * a.Hkv + hk) << a.bs_log2) + (key & ((1 << a.bs_log2) - 1))] = 0.f;
+  }
 
   // the keys: lane (h, col) holds key 32 t + col, dims 16 ks + 8 h ..; a key that is not there reads the block's last
   const int wkey = key0 + w * 64;
@@ -258,9 +268,9 @@ __global__ __launch_bounds__(256, 2) void key_weights_kernel(KeyWeightsArgs a) {
   }
 }
 
-// The parts of a key block added in order, and that to the paged table: set
-// for the keys of the step itself (those at or behind its first row), added
-// for older ones.  One workgroup per (block, kv head).
+// The parts of a key block added in order, and that to the paged table, where
+// the keys of the step itself (those at or behind its first row) are zero by
+// now.  One workgroup per (block, kv head).
 struct KeySumArgs {
   const float* part;
   const int32_t* sums;  // [n][kSumWords]: sequence, first key, keys, first unit, units, position of the first row
@@ -271,7 +281,7 @@ struct KeySumArgs {
 
 __global__ __launch_bounds__(kBlockKeys) void key_sum_kernel(KeySumArgs a) {
   const int32_t* rec = a.sums + (int64_t)blockIdx.x * kSumWords;
-  const int seq = rec[0], key0 = rec[1], nkeys = rec[2], unit = rec[3], units = rec[4], fresh = rec[5];
+  const int seq = rec[0], key0 = rec[1], nkeys = rec[2], unit = rec[3], units = rec[4];
   const int hk = blockIdx.y, key = key0 + threadIdx.x;
   if ((int)threadIdx.x >= nkeys || (key >> a.bs_log2) >= a.max_blocks) return;
   const int p = a.block_tables[(int64_t)seq * a.max_blocks + (key >> a.bs_log2)];
@@ -280,9 +290,8 @@ __global__ __launch_bounds__(kBlockKeys) void key_sum_kernel(KeySumArgs a) {
 #pragma unroll 8
   for (int u = 0; u < units; ++u) y += src[(int64_t)u * a.Hkv * kBlockKeys];
   if (p < 0) return;
-  float* dst = a.key_weights + (((int64_t)p * a.Hkv + hk) << a.bs_log2) + (key & ((1 << a.bs_log2) - 1));
-  if (key >= fresh) *dst = y;
-  else unsafeAtomicAdd(dst, y);
+  // (an atomic add: sequences may share a page)
+  unsafeAtomicAdd(a.key_weights + (((int64_t)p * a.Hkv + hk) << a.bs_log2) + (key & ((1 << a.bs_log2) - 1)), y);
 }
 
 struct KeyTiling {
@@ -372,7 +381,7 @@ int nsv_prefill_key_weights(const void* q, const void* k_cache, float* key_weigh
   int bs_log2 = 0;
   while ((1 << bs_log2) < block_size) ++bs_log2;
   KeyWeightsArgs a{(const bf16_t*)q, (const bf16_t*)k_cache, (const float2*)stats, block_tables, units, (float*)partials,
-                   scale * 1.44269504088896340736f, H, Hkv, bs_log2, max_blocks};
+                   key_weights, scale * 1.44269504088896340736f, H, Hkv, bs_log2, max_blocks};
   hipStream_t s = (hipStream_t)stream;
   const dim3 grid((unsigned)((int64_t)nunits * Hkv));
   if (D == 128) hipLaunchKernelGGL(key_weights_kernel<128>, grid, dim3(256), 0, s, a);

@@ -346,8 +346,9 @@ def paged_attention_weights(
     row, and of unmapped pages, keep what they hold.  evict_kvcache reads the
     table; prefill_key_weights adds a prompt's rows.  bfloat16 and float32, up
     to 64 rows per sequence.  A page that several sequences of a call share
-    gets the sum of theirs, in no fixed order.  Scratch as
-    paged_attention_window's.  No counterpart in the reference."""
+    gets the sum of theirs, in no fixed order, on top of nothing where the key
+    is new to one of them.  Scratch as paged_attention_window's.  No
+    counterpart in the reference."""
     query, block_tables, context_lens, cu_seqlens_q, positions, out = _few_rows(
         query, k_cache, v_cache, block_tables, context_lens, cu_seqlens_q, positions, num_heads, num_kv_heads, head_dim,
         block_size, out, "paged_attention_weights")
@@ -665,8 +666,8 @@ def prefill_key_weights(query: torch.Tensor, k_cache: torch.Tensor, key_weights:
     those of the step's prefill_attention call over the same paged K, which
     left ``stats``.  The places of the step's own keys are set, those of keys
     before its first row added to.  A page that several sequences of the step
-    share gets the sum of theirs, in no fixed order.  No counterpart in the
-    reference."""
+    share (a prefix that one computes and another has behind it) gets the sum
+    of theirs, in no fixed order.  No counterpart in the reference."""
     H, Hkv = plan.num_heads, plan.num_kv_heads
     if not query.is_cuda:
         raise ValueError("prefill_key_weights runs on the GPU; query is on the CPU")

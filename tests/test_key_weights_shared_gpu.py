@@ -1,0 +1,74 @@
+"""Key weights of pages that one sequence of a call fills and others read: a
+step's prompts may share a prefix that the first of them computes."""
+
+import numpy as np
+import pytest
+import torch
+
+from naivllm_amd.layers.attention import (KeyWeightsPlan, PrefillPlan, paged_attention_weights, prefill_attention,
+                                          prefill_key_weights)
+from naivllm_amd.utils import synth
+from oracle import bounded as ob
+from tests.bounded_util import as_device, weight_error
+from tests.gpu_util import to_device
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+def _shared(seed, lens, rows, owner, pages, **kw):
+    """Every sequence's first pages are those of sequence ``owner``."""
+    vb = synth.verify_batch(seed, lens, rows, block_size=16, **kw)
+    for b in range(len(lens)):
+        vb.block_tables[b, :pages] = vb.block_tables[owner, :pages]
+    return vb
+
+
+def _check(vb, owner, add, seed=5):
+    """add(tensors, weights) against the oracle's sums, the owner's first."""
+    first = [int(vb.positions[vb.cu_seqlens_q[b]]) for b in range(len(vb.context_lens))]
+    _, _, mag, sums = ob.attention(vb.q, vb.k_cache, vb.v_cache, vb.block_tables, vb.context_lens, vb.cu_seqlens_q,
+                                   vb.positions, 1.0 / np.sqrt(vb.head_dim), vb.num_kv_heads)
+    order = [owner] + [b for b in sums if b != owner]
+    nb, bs = vb.k_cache.shape[:2]
+    old = synth.normal(seed, 3, nb * vb.num_kv_heads * bs).reshape(nb, vb.num_kv_heads, bs).astype(np.float32) ** 2
+    want = ob.add_weights(old, {b: sums[b] for b in order}, vb.block_tables, first)
+    got = as_device(old)
+    add(to_device(vb), got)
+    torch.cuda.synchronize()
+    rows = int(np.diff(vb.cu_seqlens_q).max()) * vb.num_heads // vb.num_kv_heads
+    # a weight's own error, the additions of a sequence's rows, one addition per sequence
+    share = weight_error(mag.max(), int(vb.context_lens.max()), vb.head_dim) + (rows + len(first) + 2) * 2.0 ** -24
+    assert (np.abs(got.cpu().numpy() - want) <= share * want + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("owner", [0, 5])
+@pytest.mark.parametrize("H,Hkv,rows", [(16, 8, 9), (40, 1, 2)])  # stored scores; keys read again
+def test_few_rows(dtype, owner, H, Hkv, rows):
+    print(f"case: shared new keys {dtype} {H}/{Hkv} owner {owner}", flush=True)
+    lens = [120 + 7 * b for b in range(6)]
+    lens[owner] = 32                              # two pages, its rows' own keys in the second
+    vb = _shared(131, lens, [rows] * 6, owner, 2, num_heads=H, num_kv_heads=Hkv, dtype=dtype)
+    _check(vb, owner, lambda t, w: paged_attention_weights(
+        t["query"], t["k_cache"], t["v_cache"], w, t["block_tables"], t["context_lens"], t["cu_seqlens_q"], t["positions"],
+        1 / np.sqrt(128), H, Hkv, 128, 16, 64, max_q_len=rows))
+
+
+@pytest.mark.parametrize("owner", [0, 3])
+def test_prompts(owner):
+    print(f"case: prompts behind a prefix of the same step, owner {owner}", flush=True)
+    new, prefix = [60, 300, 33, 70], [192] * 4
+    new[owner], prefix[owner] = 400, 0
+    vb = _shared(132, [n + p for n, p in zip(new, prefix)], new, owner, 12, num_heads=4, num_kv_heads=2)
+
+    def add(t, w):
+        ends = vb.context_lens.tolist()
+        stats = torch.empty((sum(new), 4, 2), device="cuda")
+        scale = 1 / np.sqrt(128)
+        prefill_attention(t["query"], t["k_cache"], t["v_cache"], PrefillPlan(new, ends, 4, 2, 16, DEV), scale, 128,
+                          t["block_tables"], stats=stats)
+        prefill_key_weights(t["query"], t["k_cache"], w, KeyWeightsPlan(new, ends, 4, 2, 16, DEV), stats, scale, 128,
+                            t["block_tables"])
+
+    _check(vb, owner, add)
