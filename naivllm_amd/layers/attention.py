@@ -880,19 +880,20 @@ class Attention(nn.Module):
 
     def _prefill_f32_weights(self, context, q, scale: float) -> torch.Tensor:
         """An fp32 prefill step with key weights: causal blocks of rows as
-        ``_prefill_rows`` cuts them, one block of every sequence per call (two
-        blocks of a sequence in one call would add to the same places)."""
+        ``_prefill_rows`` cuts them, in turns of one call each: a sequence's
+        blocks in several, in their order (two in one call would add to the
+        same places), and every sequence's by the block's first position, so
+        that a prefix that one of them computes is set before the others that
+        have it behind them add to it."""
         tables, lens, cu, positions, q_block = _prefill_rows(context, self.num_heads, self.num_kv_heads, q.device)
         out, cu, first = torch.empty_like(q), cu.tolist(), 0
-        blocks: list[list[int]] = []  # per turn: the entries of _prefill_rows' batch
-        for n in context.seqlens_q:
+        turns: dict[int, list[int]] = {}  # the entries of _prefill_rows' batch
+        for n, end in zip(context.seqlens_q, context.seqlens_k):
             count = -(-n // q_block)
             for i in range(count):
-                if i == len(blocks):
-                    blocks.append([])
-                blocks[i].append(first + i)
+                turns.setdefault((end - n) // q_block + i, []).append(first + i)
             first += count
-        for entries in blocks:
+        for _, entries in sorted(turns.items()):
             rows = torch.cat([torch.arange(cu[e], cu[e + 1]) for e in entries]).to(q.device)
             starts = torch.tensor([0] + [cu[e + 1] - cu[e] for e in entries]).cumsum(0).to(q.device, torch.int32)
             at = torch.tensor(entries, device=q.device)

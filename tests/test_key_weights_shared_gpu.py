@@ -5,9 +5,10 @@ import numpy as np
 import pytest
 import torch
 
-from naivllm_amd.layers.attention import (KeyWeightsPlan, PrefillPlan, paged_attention_weights, prefill_attention,
+from naivllm_amd.layers.attention import (Attention, KeyWeightsPlan, PrefillPlan, paged_attention_weights, prefill_attention,
                                           prefill_key_weights)
 from naivllm_amd.utils import synth
+from naivllm_amd.utils.context import reset_context, set_context
 from oracle import bounded as ob
 from tests.bounded_util import as_device, weight_error
 from tests.gpu_util import to_device
@@ -70,5 +71,31 @@ def test_prompts(owner):
                           t["block_tables"], stats=stats)
         prefill_key_weights(t["query"], t["k_cache"], w, KeyWeightsPlan(new, ends, 4, 2, 16, DEV), stats, scale, 128,
                             t["block_tables"])
+
+    _check(vb, owner, add)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("owner", [0, 2])
+def test_the_layer_over_a_step_that_shares_its_prefix(dtype, owner):
+    """One prompt computes a prefix, two of the same step have it behind them."""
+    print(f"case: layer, shared prefix {dtype} owner {owner}", flush=True)
+    new, prefix = [33, 90, 100], [128] * 3
+    new[owner], prefix[owner] = 300, 0
+    vb = _shared(133, [n + p for n, p in zip(new, prefix)], new, owner, 8, num_heads=4, num_kv_heads=2, dtype=dtype)
+    layer = Attention(4, 128, 1.0, 2, 16)
+
+    def add(t, w):
+        layer.k_cache, layer.v_cache, layer.key_weights = t["k_cache"], t["v_cache"], w
+        at = torch.from_numpy(np.concatenate([
+            vb.block_tables[b, np.arange(p, p + n) // 16].astype(np.int64) * 16 + np.arange(p, p + n) % 16
+            for b, (n, p) in enumerate(zip(new, prefix))])).cuda()
+        k, v = t["k_cache"].flatten(0, 1)[at], t["v_cache"].flatten(0, 1)[at]
+        set_context(True, cu_seqlens_q=t["cu_seqlens_q"], slot_mapping=at, context_lens=t["context_lens"],
+                    block_tables=t["block_tables"], seqlens_q=new, seqlens_k=vb.context_lens.tolist())
+        try:
+            layer(t["query"], k, v)
+        finally:
+            reset_context()
 
     _check(vb, owner, add)
