@@ -544,6 +544,50 @@ class PrefillRows(_StepList):
         self.cu_seqlens_q = self.work[n + rows:].view(torch.int32)[:n + 1]
 
 
+class _WeightTurns(_StepList):
+    """The calls of an fp32 prefill step with key weights, in one transfer:
+    causal blocks of up to ``q_block`` rows, a sequence's in turns of their own
+    (two in one call would add to the same places), every sequence's by the
+    block's first position, so that a prefix that one of them computes is set
+    before the others that have it behind them add to it.  ``turns``: (rows, or
+    the first and last + 1 of neighbours; block tables, context_lens,
+    cu_seqlens_q, positions)."""
+
+    def __init__(self, seqlens_q, seqlens_k, block_tables: torch.Tensor, q_block: int, device):
+        ql, kl = _prefill_lengths(seqlens_q, seqlens_k)
+        if block_tables.shape[0] < len(ql):
+            raise ValueError(f"{len(ql)} sequences but {block_tables.shape[0]} block-table rows")
+        tables = block_tables.to("cpu", torch.int32)  # (waits, once per step)
+        blocks: dict[int, list[tuple[int, int, int, int]]] = {}  # turn -> (sequence, first row, rows, first position)
+        row0 = 0
+        for b, (n, end) in enumerate(zip(ql, kl)):
+            for r in range(0, n, q_block):
+                first = end - n + r
+                blocks.setdefault(first // q_block, []).append((b, row0 + r, min(q_block, n - r), first))
+            row0 += n
+        words: list[torch.Tensor] = []  # int64: per turn rows, lens, positions, then cu and the tables in halves of words
+        cuts, at = [], 0
+        for _, turn in sorted(blocks.items()):
+            rows = torch.cat([torch.arange(r, r + n) for _, r, n, _ in turn])
+            lens = torch.tensor([p + n for _, _, n, p in turn])
+            positions = torch.cat([torch.arange(p, p + n) for _, _, n, p in turn])
+            half = torch.cat([torch.tensor([0] + [n for _, _, n, _ in turn]).cumsum(0).to(torch.int32),
+                              tables[[b for b, *_ in turn]].flatten()])
+            half = torch.cat([half, half.new_zeros(half.numel() % 2)]).view(torch.int64)
+            words += [rows, lens, positions, half]
+            cuts.append((at, rows.numel(), len(turn), (int(rows[0]), int(rows[-1]) + 1) if len(turn) == 1 else None))
+            at += 2 * rows.numel() + lens.numel() + half.numel()
+        ahead = _send_ahead()
+        work = torch.cat(words)
+        self._send(work.pin_memory() if ahead else work, device, ahead)
+        self.rows, self.turns = row0, []
+        for at, n, count, whole in cuts:
+            rows, lens, positions = self.work[at:at + n], self.work[at + n:at + n + count], self.work[at + n + count:at + 2 * n + count]
+            half = self.work[at + 2 * n + count:].view(torch.int32)
+            self.turns.append((whole or rows, half[count + 1:count + 1 + count * tables.shape[1]].view(count, -1), lens,
+                               half[:count + 1], positions))
+
+
 def verify_serves_prefill(seqlens_q, seqlens_k, num_heads: int, num_kv_heads: int, block_size: int,
                           max_num_blocks: int) -> bool:
     """Whether a paged bf16 prefill step runs on the verify kernel, one block
@@ -879,25 +923,25 @@ class Attention(nn.Module):
         return paged_attention_verify(q, self.k_cache, self.v_cache, *shape, max_q_len=max_q_len, out=out)
 
     def _prefill_f32_weights(self, context, q, scale: float) -> torch.Tensor:
-        """An fp32 prefill step with key weights: causal blocks of rows as
-        ``_prefill_rows`` cuts them, in turns of one call each: a sequence's
-        blocks in several, in their order (two in one call would add to the
-        same places), and every sequence's by the block's first position, so
-        that a prefix that one of them computes is set before the others that
-        have it behind them add to it."""
-        tables, lens, cu, positions, q_block = _prefill_rows(context, self.num_heads, self.num_kv_heads, q.device)
-        out, cu, first = torch.empty_like(q), cu.tolist(), 0
-        turns: dict[int, list[int]] = {}  # the entries of _prefill_rows' batch
-        for n, end in zip(context.seqlens_q, context.seqlens_k):
-            count = -(-n // q_block)
-            for i in range(count):
-                turns.setdefault((end - n) // q_block + i, []).append(first + i)
-            first += count
-        for _, entries in sorted(turns.items()):
-            rows = torch.cat([torch.arange(cu[e], cu[e + 1]) for e in entries]).to(q.device)
-            starts = torch.tensor([0] + [cu[e + 1] - cu[e] for e in entries]).cumsum(0).to(q.device, torch.int32)
-            at = torch.tensor(entries, device=q.device)
-            out[rows] = self._few(q[rows], tables[at], lens[at], starts, positions[rows], scale, q_block)
+        """An fp32 prefill step with key weights: causal blocks of rows in
+        several calls (_WeightTurns, built by the step's first layer)."""
+        if context.seqlens_q is None or context.seqlens_k is None:
+            raise ValueError("a prefill step needs context.seqlens_q and context.seqlens_k")
+        q_block = max(1, 64 // (self.num_heads // self.num_kv_heads))
+        plans, key = context.__dict__.setdefault("prefill_plans", {}), ("turns", q_block, q.device)
+        plan = plans.get(key)
+        if plan is None:
+            plan = plans[key] = _WeightTurns(context.seqlens_q, context.seqlens_k, context.block_tables, q_block, q.device)
+        if q.shape[0] < plan.rows:
+            raise ValueError(f"query must have at least {plan.rows} rows, got {q.shape[0]}")
+        plan.use_on(torch.cuda.current_stream(q.device))
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)  # (rows past the step's: unwritten)
+        for rows, *meta in plan.turns:
+            if isinstance(rows, tuple):
+                at = slice(*rows)
+                self._few(q[at], *meta, scale, q_block, out[at])
+            else:
+                out.index_copy_(0, rows, self._few(q.index_select(0, rows), *meta, scale, q_block))
         return out
 
     def _prefill_bf16(self, context, q, k, v, scale: float) -> torch.Tensor:

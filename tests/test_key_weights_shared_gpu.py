@@ -99,3 +99,43 @@ def test_the_layer_over_a_step_that_shares_its_prefix(dtype, owner):
             reset_context()
 
     _check(vb, owner, add)
+
+
+@pytest.mark.parametrize("new", [[100], [100, 40, 70]])
+def test_a_layer_of_a_step_waits_for_nothing_and_can_be_captured(new):
+    """fp32: the step's lists are made by its first layer."""
+    print(f"case: fp32 layer captured {new}", flush=True)
+    vb = synth.verify_batch(134, new, new, block_size=16, num_heads=4, num_kv_heads=2, dtype="f32")
+    t = to_device(vb)
+    layers = [Attention(4, 128, 1.0, 2, 16) for _ in range(2)]
+    for layer in layers:
+        layer.k_cache, layer.v_cache = t["k_cache"], t["v_cache"]
+        layer.key_weights = torch.full((vb.k_cache.shape[0], 2, 16), float("nan"), device="cuda")
+    k = v = torch.empty((sum(new), 2, 128), device="cuda")
+    set_context(True, cu_seqlens_q=t["cu_seqlens_q"], context_lens=t["context_lens"], block_tables=t["block_tables"],
+                seqlens_q=new, seqlens_k=new)
+    try:
+        want = layers[0](t["query"], k, v)
+        torch.cuda.synchronize()
+        torch.cuda.set_sync_debug_mode("error")
+        try:
+            out = layers[1](t["query"], k, v)
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+        assert torch.equal(out, want)
+        weights = layers[1].key_weights.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = layers[1](t["query"], k, v)
+        for _ in range(3):
+            layers[1].key_weights.fill_(3.0)
+            out.zero_()
+            graph.replay()
+            layers[0](t["query"], k, v)  # eager work between the replays
+            torch.cuda.synchronize()
+            assert torch.equal(out, want)
+            at = ~weights.isnan()        # (a prompt of its own: every key of it is set)
+            assert torch.equal(layers[1].key_weights[at], weights[at])
+            assert (layers[1].key_weights[~at] == 3.0).all()
+    finally:
+        reset_context()
