@@ -66,7 +66,8 @@ struct PrefillArgs {
   float* part;                  // [slots][H][tile_rows][DH + 2]: unnormalised rows, then (max, sum) pairs
   float2* stats;                // null, or [rows][H]: a row's exponent reference (log2 domain) and 1 / sum (0: no key)
   int tile_rows;
-  float scale_log2;
+  float scale_log2;             // > 0 (or NaN): scores are masked before they are scaled
+  uint32_t q_keep, q_flip;      // bits of a pair of query elements that stay, and change: a scale's sign, or its zero
   int H, Hkv, bs_log2, max_blocks;
   int window, sinks;            // WIN kernels only
   int hw;                       // query heads of a kv head one workgroup serves
@@ -452,6 +453,10 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
     const int last = key_begin + (key_end - 1 - key_begin) / kKeys * kKeys;  // the last tile's first key
     issue(0, 0, key_begin);
     if (DIST == 2 && key_begin < last) issue(1, 1, key_begin + kKeys);
+    if (~a.q_keep | a.q_flip) {  // uniform
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) qB[ks] = as_bf16x8((__builtin_bit_cast(u32x4, qB[ks]) & a.q_keep) ^ a.q_flip);
+    }
     // (the query operands are waited for here: a wait for them inside the loop
     // would wait for the tiles loading ahead)
 #pragma unroll
@@ -754,7 +759,12 @@ int nsv_prefill_window_attention(void* out, const void* q, const void* k, const 
   a.out = (bf16_t*)out;
   a.block_tables = block_tables;
   a.tiles = tiles;
-  a.scale_log2 = scale * 1.44269504088896340736f;
+  // A scale below zero goes to the queries' signs, a scale of zero to queries of
+  // zero: the largest product of the kernel's is the largest score then, and a
+  // masked one (-inf) scaled is still one.
+  a.scale_log2 = scale == 0.f ? 1.f : fabsf(scale) * 1.44269504088896340736f;
+  a.q_keep = scale == 0.f ? 0u : 0xffffffffu;
+  a.q_flip = scale < 0.f ? 0x80008000u : 0u;
   a.H = H;
   a.Hkv = Hkv;
   a.bs_log2 = bs_log2;

@@ -5,10 +5,10 @@ import pytest
 import torch
 
 from naivllm_amd import _lib
-from naivllm_amd.layers.attention import PrefillPlan
+from naivllm_amd.layers.attention import KeyWeightsPlan, PrefillPlan, prefill_attention, prefill_key_weights
 from naivllm_amd.utils import synth
 from oracle import bounded as ob
-from tests.bounded_util import EPS32, check_attention, weight_error
+from tests.bounded_util import EPS32, as_device, check_attention, weight_error
 from tests.gpu_util import to_device
 
 pytestmark = pytest.mark.gpu
@@ -70,3 +70,31 @@ def test_statistics_of_the_library_entry(new, prefix, H, Hkv, window, sinks, wav
     # the sum's relative error is a weight's; m is rounded once, r twice (its sum's and its own)
     bound = np.log2(np.e) * (weight_error(mag, max(ends), 128) + 4 * EPS32) + EPS32 * (np.abs(m) + mag * np.log2(np.e))
     assert (np.abs(m - np.log2(r) - want) <= bound).all()
+
+
+@pytest.mark.parametrize("window,sinks", [(0, 0), (60, 3)])
+@pytest.mark.parametrize("scale", [0.0, -0.09, 2.0])
+def test_scales_of_every_sign(window, sinks, scale):
+    """As the few-row operators': at 0 a row's keys weigh the same, below it
+    the smallest products weigh most."""
+    print(f"case: prompt scale {scale} window {window}", flush=True)
+    vb = _batch(102, [300, 40, 5], [0, 900, 33])
+    vb.block_tables[0, 1] = -1
+    t = to_device(vb)
+    want, want_abs, mag, sums = ob.attention(vb.q, vb.k_cache, vb.v_cache, vb.block_tables, vb.context_lens,
+                                             vb.cu_seqlens_q, vb.positions, scale, 2, window or None, sinks)
+    mag = np.abs(mag)
+    new, ends = [300, 40, 5], vb.context_lens.tolist()
+    plan = PrefillPlan(new, ends, 4, 2, 64, DEV, window=window, sinks=sinks)
+    stats = None if window else torch.empty((345, 4, 2), device="cuda")
+    out = prefill_attention(t["query"], t["k_cache"], t["v_cache"], plan, scale, 128, t["block_tables"], stats=stats)
+    check_attention(out, want, want_abs, mag, "bf16", max(ends), f"scale {scale}")
+    if window:
+        return
+    old = synth.normal(9, 3, vb.k_cache.shape[0] * 2 * 64).reshape(-1, 2, 64).astype(np.float32) ** 2
+    weights = as_device(old)
+    prefill_key_weights(t["query"], t["k_cache"], weights, KeyWeightsPlan(new, ends, 4, 2, 64, DEV), stats, scale, 128,
+                        t["block_tables"])
+    want_w = ob.add_weights(old, sums, vb.block_tables, [0, 900, 33])
+    bound = (weight_error(mag.max(), max(ends), 128) + (300 * 2 + 2) * EPS32) * np.abs(want_w) + 1e-30
+    assert (np.abs(weights.cpu().numpy() - want_w) <= bound).all()
