@@ -516,7 +516,9 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
       for (int q = 0; q < 4; ++q)
         *reinterpret_cast<f32x4*>(dst + dt * 32 + q * 8) =
             f32x4{acc[dt][4 * q], acc[dt][4 * q + 1], acc[dt][4 * q + 2], acc[dt][4 * q + 3]};
-    if (h == 0) *reinterpret_cast<float2*>(base + a.tile_rows * DH + 2 * r) = make_float2(m_ref * sc, L);
+    // (a row whose every score is NaN has no maximum; its sum is NaN, and -inf would drop it)
+    const float m = L != L && m_ref == kNegInf ? 0.f : m_ref * sc;
+    if (h == 0) *reinterpret_cast<float2*>(base + a.tile_rows * DH + 2 * r) = make_float2(m, L);
     return;
   }
   if (a.stats && h == 0 && r < nrows) a.stats[(int64_t)(row0 + r) * a.H + head] = make_float2(m_ref * sc, L == 0.f ? 0.f : 1.f / L);

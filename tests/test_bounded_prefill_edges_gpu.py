@@ -98,3 +98,29 @@ def test_scales_of_every_sign(window, sinks, scale):
     want_w = ob.add_weights(old, sums, vb.block_tables, [0, 900, 33])
     bound = (weight_error(mag.max(), max(ends), 128) + (300 * 2 + 2) * EPS32) * np.abs(want_w) + 1e-30
     assert (np.abs(weights.cpu().numpy() - want_w) <= bound).all()
+
+
+def test_a_row_of_nan_whose_keys_are_cut():
+    """NaN for the row, its statistics and the weights of the keys it sees,
+    also where several workgroups share its keys; nothing for other rows."""
+    print("case: prompt, a NaN row over cut keys", flush=True)
+    vb = _batch(103, [40], [1500], 2, 1)
+    plan = PrefillPlan([40], [1540], 2, 1, 64, DEV)
+    assert plan.nmerges > 0
+    results = []
+    for bad in (False, True):
+        t = to_device(vb)
+        if bad:
+            t["query"][17, 1] = float("nan")
+        stats, w = torch.empty((40, 2, 2), device="cuda"), torch.ones((vb.k_cache.shape[0], 1, 64), device="cuda")
+        out = prefill_attention(t["query"], t["k_cache"], t["v_cache"], plan, 0.09, 128, t["block_tables"], stats=stats)
+        prefill_key_weights(t["query"], t["k_cache"], w, KeyWeightsPlan([40], [1540], 2, 1, 64, DEV), stats, 0.09, 128,
+                            t["block_tables"])
+        j = np.arange(1540)
+        results.append((out, w[torch.from_numpy(vb.block_tables[0, j // 64]).long().cuda(), 0,
+                               torch.from_numpy(j % 64).cuda()], stats))
+    (good, w_good, s_good), (got, w_got, s_got) = results
+    assert s_got[17, 1, 1].isnan() and got[17, 1].isnan().all() and w_got[:1518].isnan().all()
+    got[17, 1] = good[17, 1] = 0
+    s_got[17, 1] = s_good[17, 1] = 0
+    assert torch.equal(got, good) and torch.equal(s_got, s_good) and torch.equal(w_got[1518:], w_good[1518:])
