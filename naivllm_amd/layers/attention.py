@@ -654,6 +654,7 @@ def prefill_attention(query: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pla
         raise ValueError("prefill_attention runs on the GPU; query is on the CPU")
     if query.dtype != torch.bfloat16 or k.dtype != query.dtype or v.dtype != query.dtype:
         raise ValueError("query, k and v must be bfloat16")
+    _check_devices(query, plan, k=k, v=v, block_tables=block_tables)
     if query.dim() != 3 or tuple(query.shape[1:]) != (H, head_dim) or query.shape[0] < plan.rows:
         raise ValueError(f"query must be (at least {plan.rows}, {H}, {head_dim}), got {tuple(query.shape)}")
     max_blocks = 0
@@ -694,6 +695,13 @@ def prefill_attention(query: torch.Tensor, k: torch.Tensor, v: torch.Tensor, pla
     return out
 
 
+def _check_devices(query: torch.Tensor, plan: _StepList, **others: torch.Tensor | None) -> None:
+    dev = query.get_device()
+    for name, t in (*others.items(), ("the plan", plan.work)):
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{name} is on {t.device}, query on {query.device}")
+
+
 def _check_stats(stats: torch.Tensor, rows: int, num_heads: int, device) -> None:
     if (stats.dim() != 3 or stats.shape[0] < rows or tuple(stats.shape[1:]) != (num_heads, 2)
             or stats.dtype != torch.float32 or stats.device != device or not stats.is_contiguous()):
@@ -721,8 +729,7 @@ def prefill_key_weights(query: torch.Tensor, k_cache: torch.Tensor, key_weights:
         raise ValueError(f"query must be (at least {plan.rows}, {H}, {head_dim}), got {tuple(query.shape)}")
     if _check_cache(k_cache, "k_cache")[1:] != (plan.block_size, Hkv, head_dim):
         raise ValueError("cache shape disagrees with block_size / num_kv_heads / head_dim")
-    if k_cache.device != query.device or block_tables.device != query.device:
-        raise ValueError(f"query is on {query.device}, k_cache on {k_cache.device}, block_tables on {block_tables.device}")
+    _check_devices(query, plan, k_cache=k_cache, block_tables=block_tables)
     if k_cache.data_ptr() % 16:
         raise ValueError("k_cache must start on 16 bytes")
     _check_key_weights(key_weights, k_cache)
