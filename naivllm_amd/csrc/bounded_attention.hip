@@ -22,9 +22,11 @@
 // weights move through no shuffle.  bf16: v_mfma_f32_16x16x32_bf16, V^T from
 // the transposing LDS reads; fp32: v_mfma_f32_16x16x4_f32, whose terms are
 // numbered so that 16-byte LDS reads feed them.  Maxima, sums and outputs are
-// held in fp32; the weights P are rounded to bf16 for the second product (at
-// the running maximum as exponent reference: the outputs' error against 64
-// bits is that of one final rounding, 1.7e-3), never for the key weights.
+// held in fp32.  For the second product a weight of P is the sum of two bf16
+// numbers (16 bits; one bf16 number left the outputs up to 1.86e-3 from 64 bits,
+// two leave the final rounding's 1.7e-3), in two products: 4% of the time where
+// a kv head has 36 rows (35.0 -> 36.3 us), nothing at fewer or on long contexts.
+// The key weights are never rounded.
 //
 // Key weights need every row's final statistics, so they are a second pass:
 // over the scores, which the first one stores where a call has few of them
@@ -472,7 +474,9 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
     }
   };
   auto attend = [&](const unsigned char* vt) {
-    u32x4 pB[MT];  // bf16: the weights as the B operand (elements 0..3 keys 4 g + i, 4..7 keys 16 + 4 g + i)
+    // bf16: the weights as the B operand (elements 0..3 keys 4 g + i, 4..7 keys
+    // 16 + 4 g + i), each as the sum of two bf16 numbers
+    u32x4 pB[MT], pL[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       float mx = kNegInf;
@@ -498,8 +502,12 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
         for (int d = 0; d < NACC; ++d) acc[mt][d] *= alpha;
       }
       if constexpr (BF16) {
-        pB[mt] = u32x4{pack_bf16x2(s[mt][0][0], s[mt][0][1]), pack_bf16x2(s[mt][0][2], s[mt][0][3]),
-                       pack_bf16x2(s[mt][KT - 1][0], s[mt][KT - 1][1]), pack_bf16x2(s[mt][KT - 1][2], s[mt][KT - 1][3])};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = s[mt][e < 2 ? 0 : KT - 1][2 * (e & 1)], y = s[mt][e < 2 ? 0 : KT - 1][2 * (e & 1) + 1];
+          pB[mt][e] = pack_bf16x2(x, y);
+          pL[mt][e] = pack_bf16x2(x - __uint_as_float(pB[mt][e] << 16), y - __uint_as_float(pB[mt][e] & 0xffff0000u));
+        }
       }
     }
     if constexpr (BF16) {
@@ -513,6 +521,10 @@ __global__ __launch_bounds__(kWaves * 64, 1) void row_attention_kernel(RowArgs a
         for (int mt = 0; mt < MT; ++mt)
           acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y}),
                                                                 as_bf16x8(pB[mt]), acc[mt][dt], 0, 0, 0);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+          acc[mt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf16x8(u32x4{lo.x, lo.y, hi.x, hi.y}),
+                                                                as_bf16x8(pL[mt]), acc[mt][dt], 0, 0, 0);
       }
     } else {
       // step i takes keys 4 g + i: V[key][64 h + 4 c + e] feeds tile (h, e), whose row c is dim 64 h + 4 c + e
