@@ -101,6 +101,7 @@ def test_the_layer_over_a_step_that_shares_its_prefix(dtype, owner):
     _check(vb, owner, add)
 
 
+@pytest.mark.filterwarnings("ignore:Synchronization debug mode")
 @pytest.mark.parametrize("new", [[100], [100, 40, 70]])
 def test_a_layer_of_a_step_waits_for_nothing_and_can_be_captured(new):
     """fp32: the step's lists are made by its first layer."""
