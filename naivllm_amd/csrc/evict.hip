@@ -462,38 +462,43 @@ __global__ __launch_bounds__(kMoveThreads) void evict_move_kernel(EvictArgs a, i
     }
     return;
   }
-  const int first = blockIdx.z * chunk;  // (in place: 0)
+  // (the next chunk's sources lie behind this chunk's destinations; the barrier
+  // puts every read of a chunk before its first write)
+  auto in_order = [&] {
+    for (int i0 = 0; i0 < got; i0 += chunk) {
+      Chunk next;
+      loads_back();
+      __syncthreads();
+      if (i0 + chunk < got) read(next, i0 + chunk);
+      write(c, i0);
+      c = next;
+    }
+  };
+  if (!apart) {
+    read(c, 0);
+    in_order();
+    return;
+  }
+  const int first = blockIdx.z * chunk;
   if (first >= got) return;  // uniform
   const int pages = ((got - 1) >> a.bs_log2) + 1, mine = min((int)threadIdx.x, pages - 1);
   const int from = bt[mine], into = ot[mine];
   read(c, first);
-  bool ordered = !apart;
-  if (apart && n > a.budget) {  // uniform
+  if (n > a.budget) {  // uniform
     // Another table may hold pages of this one at their places, in which rows
     // move as they do in place: one workgroup takes the column then.  (Its
     // entries are looked up beside the first chunk, and before any write.)
     int same = from >= 0 && from == into;
     for (int i = kMoveThreads + threadIdx.x; i < pages; i += kMoveThreads) same |= bt[i] >= 0 && bt[i] == ot[i];
-    ordered = __syncthreads_or(same) != 0;
-    if (ordered && blockIdx.z > 0) return;  // uniform
-  }
-  if (!ordered) {
-    write(c, first);
-    for (int i0 = first + gridDim.z * chunk; i0 < got; i0 += gridDim.z * chunk) {
-      read(c, i0);
-      write(c, i0);
+    if (__syncthreads_or(same)) {  // uniform
+      if (blockIdx.z == 0) in_order();
+      return;
     }
-    return;
   }
-  // (the next chunk's sources lie behind this chunk's destinations; the barrier
-  // puts every read of a chunk before its first write)
-  for (int i0 = 0; i0 < got; i0 += chunk) {
-    Chunk next;
-    loads_back();
-    __syncthreads();
-    if (i0 + chunk < got) read(next, i0 + chunk);
+  write(c, first);
+  for (int i0 = first + gridDim.z * chunk; i0 < got; i0 += gridDim.z * chunk) {
+    read(c, i0);
     write(c, i0);
-    c = next;
   }
 }
 
