@@ -257,7 +257,11 @@ def _weights_workspace_bytes(*shape: int) -> int:
 def _int_arg(value, name: str, least: int) -> int:
     """A host integer of at least ``least``, capped where it means no bound
     to the kernels (no table holds 2^30 keys)."""
-    if int(value) != value or value < least:
+    try:
+        whole = int(value) == value and value >= least
+    except (OverflowError, TypeError, ValueError):  # (infinite; no number; NaN)
+        whole = False
+    if not whole:
         raise ValueError(f"{name} must be an integer of at least {least}, got {value}")
     return min(int(value), 1 << 30)
 
