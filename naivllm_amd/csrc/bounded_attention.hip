@@ -24,8 +24,9 @@
 // numbered so that 16-byte LDS reads feed them.  Maxima, sums and outputs are
 // held in fp32.  For the second product a weight of P is the sum of two bf16
 // numbers (16 bits; one bf16 number left the outputs up to 1.86e-3 from 64 bits,
-// two leave the final rounding's 1.7e-3), in two products: 4% of the time where
-// a kv head has 36 rows (35.0 -> 36.3 us), nothing at fewer or on long contexts.
+// two leave the final rounding's 1.7e-3), in two products: 4% of the time at 36
+// rows of a kv head over 4,096 keys (34.7 -> 36.3 us), nothing measurable at 2 rows
+// or where 36 read 16k keys and more.
 // The key weights are never rounded.
 //
 // Key weights need every row's final statistics, so they are a second pass:
@@ -34,13 +35,13 @@
 // against 26 from the keys again; 36 rows over 16k-32k keys, 604 MB of scores,
 // 714 us against 490), or over K again, whose products are made anew.
 //
-// Measured on MI355X, us per call, bytes that it cannot do without per second:
-// window 512 + 4 sinks, 1 row of 16/8 heads 7.7 (latency: the metadata's,
-// the table's and the tiles' round trips); window 4,096, 8 sequences of 9 rows,
-// 32/8 heads, 35 (3.9 TB/s; loads alone 33); fp32, 3 sequences, window 999, 9.2;
-// key weights of 8 sequences of 1,250 keys, 1 row, 14.6 (2.8 TB/s); of 16
-// sequences of 16k-32k keys, 9 rows of 32/8 heads, 490: 318 for the attention
-// (5.0 TB/s), 166 for K again (4.8 TB/s).
+// Measured on MI355X, us, bytes that it cannot do without per second: window
+// 512 + 4 sinks, 1 row of 16/8 heads 7.6 (latency: the metadata's, the table's
+// and the tiles' round trips); window 4,096, 8 sequences of 9 rows, 32/8 heads,
+// 36.5 (3.7 TB/s; loads alone 33); fp32, 3 sequences, window 999, 9.3; key weights
+// of 8 sequences of 1,250 keys, 1 row, 15.1 (2.7 TB/s); of 16 sequences of
+// 16k-32k keys, 9 rows of 32/8 heads, 492: 322 for the attention (5.4 TB/s), 167
+// for K again (5.2 TB/s).
 
 #include "common.h"
 

@@ -97,9 +97,10 @@ __device__ __forceinline__ float half_sum(float v) {
 // in these numbers from there on, in which the row at position p sees key j iff
 // p - window < j <= p or j < min(sinks, p + 1): one shift, and no load or
 // product is spent on the keys between.
-// MI355X: 8 prompts of 650-1,300 tokens, 16/8 heads, window 512, 48 us (513
-// TFLOP/s of visible pairs; all keys 66), chunks of 2,900-4,050 rows behind 4,096
-// keys, 32/8 heads, window 2,048, 359 us (752; all keys 895).
+// MI355X, calls one after another: 8 prompts of 650-1,300 tokens, 16/8 heads,
+// window 512, 48.8 us (515 TFLOP/s of visible pairs; all keys 66; replayed from a
+// graph or traced 55 to 58), chunks of 2,900-4,050 rows behind 4,096 keys, 32/8
+// heads, window 2,048, 357 us (755; all keys 895).
 struct TileSpan {
   int64_t head, gap, total;  // key j is key j of the sequence below head, j + gap from there on
 };
@@ -526,7 +527,7 @@ __global__ __launch_bounds__(NW * 64, 2) void prefill_attn_kernel(PrefillArgs a)
     // Short ranges of keys, where the ends of a workgroup weigh: the wave's rows
     // through LDS (its own part of the tiles, once every wave is done with
     // them), so that whole rows of 16-byte pieces are written instead of 8
-    // bytes per lane and row.  8 prompts of 650-1,300 tokens, 16/8 heads: window
+    // bytes per lane and row.  Traced, 8 prompts of 650-1,300 tokens, 16/8 heads: window
     // 128 42.6 -> 36.9 us, 512 60.6 -> 56.1, 2 prompts of 2,900-4,050 behind 4,096,
     // 32/8 heads, window 512 140 -> 131; the 8-wave kernel, of longer ranges,
     // loses 1% by it.

@@ -294,7 +294,8 @@ def paged_attention_window(
     between the sinks and the windows may be given to other sequences (their
     entries any value, -1 included), and what they hold (NaN, say) reaches no
     result; a key that one row sees and another does not must be finite.  A row
-    that sees no key, and a row at position -1, comes back as zeros.  Scratch
+    that sees no key, and a row at position -1, comes back as zeros; rows behind
+    the last sequence (cu_seqlens_q[-1]) are not written.  Scratch
     and arrival counters are the stream's own (a captured call's scratch its
     graph's): calls on several streams, and captured ones, share nothing.
     No counterpart in the reference, whose attention sees every key."""
@@ -783,7 +784,9 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: tor
     Every page of the context must be mapped.  A sequence's new row may hold
     pages of its old one at the same places (a copy of the table, its first
     columns), but no page of ``block_tables`` at another place or of another
-    sequence.
+    sequence.  What rows go to is rewritten: a prefix cache must not serve
+    those pages by their old tokens.  In place, few sequences of many kept rows
+    go by way of scratch as large as those rows of K and V.
 
     Returns (lens (B,) int64: min(length, budget); kept (B, Hkv, budget)
     int32: the positions that stay, ascending, -1 behind the last).  Keys hold
