@@ -264,10 +264,11 @@ int nsv_prefill_key_weights(const void* q, const void* k_cache,
  * is not NULL (sequences of up to `budget` keys too, then).
  *   lens  [B] int64: min(context_lens[b], max_blocks * block_size, budget)
  *   kept  [B, Hkv, budget] int32: the positions that stay, ascending, then -1
- * Every page of a context must be mapped.  A page of a row of out_block_tables
- * may stand at the same place in that row of block_tables (a copy of the table,
- * its first columns), but nowhere else in block_tables.  Supported: rows of a
- * multiple of 64 bytes; block_size a power of two; sinks + recent <= budget.
+ * Every page of a context must be mapped.  A row of out_block_tables may hold
+ * pages of the sequence's context at the same places as block_tables (a copy of
+ * the table, its first columns), but none of a context's pages at another place
+ * or of another sequence.  Supported: rows of a multiple of 64 bytes; block_size
+ * a power of two; sinks + recent <= budget.
  * Workspace: nsv_evict_workspace_size() bytes on 16 bytes (0: none; apart:
  * whether out_block_tables will be another table: not NULL, and at another
  * address or of another width), of any content.

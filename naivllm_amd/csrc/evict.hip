@@ -34,7 +34,7 @@
 //
 // Measured on MI355X: one sequence, 1,250 -> 512 keys of 8 heads, bf16, D 128,
 // to pages apart: 9.0 us of selection, 3.5 of moving; 16 sequences of 16k-32k
-// -> 2,048 keys in place: 23 and 57 (268 MB read and written, 4.7 TB/s; a large
+// -> 2,048 keys in place: 23.5 and 56 (268 MB read and written, 4.8 TB/s; a large
 // copy 4.8).  The selection took 36 of the latter with every page looked up
 // before its weights and again at each kept key's place, kept keys written from
 // where they were found, and one histogram per wave; 50 with the words made

@@ -7,11 +7,12 @@
 //
 // What bounds it: one matrix product of 2 D flops per (row, key) pair, an
 // exponential (quarter rate) and two fused multiply-adds, at the diagonal a
-// select: at 8,192 rows the vector units are busy for 57% of the SIMDs' cycles and
-// the matrix cores for 37%, and the two overlap little.  The keys stay, the rows stream: a wave holds 64 keys in
-// registers as the A operand of S^T = K Q^T (v_mfma_f32_32x32x16_bf16), so a
-// lane's 32 scores of a 32-row tile are added into 32 registers of its own and
-// the sum over the lanes is taken once, at the end.  A workgroup's four waves
+// select: at 8,192 rows the vector units are busy for 57% of the SIMDs' cycles
+// and the matrix cores for 37%, and the two overlap little.  The keys stay, the
+// rows stream: a wave holds 64 keys in registers as the A operand of S^T = K Q^T
+// (v_mfma_f32_32x32x16_bf16), so a lane's 32 scores of a 32-row tile are added
+// into 32 registers of its own and the sum over the lanes is taken once, at the
+// end.  A workgroup's four waves
 // (256 keys) read the row tiles from one LDS copy, loaded straight from memory
 // three deep.  The (head, row tile) list of a key block is cut into parts so
 // that the grid fills the chip; a second kernel adds the parts in their order
@@ -20,9 +21,10 @@
 // Measured on MI355X: 8,192 rows of 32/8 heads 316 us at 2.0 GHz (870 TFLOP/s of
 // the one product; without the sums 163, without the products 267, where the
 // vector operations' issue alone takes about 200: the rest is the operands' reads
-// and the waits for tiles), 1,206 rows of 16/8 heads 13.6 + 3.8.  Not better: both squares of 32 keys multiplied in turn (spills), 32 rows' operands
-// read a half ahead, units ordered by their rows for the L2, one workgroup per
-// compute unit (522).
+// and the waits for tiles), 1,206 rows of 16/8 heads 13.6 + 3.8.  Not better:
+// both squares of 32 keys multiplied in turn (spills), 32 rows' operands read a
+// half ahead, units ordered by their rows for the L2, one workgroup per compute
+// unit (522).
 
 #include "common.h"
 

@@ -782,8 +782,8 @@ def evict_kvcache(k_cache: torch.Tensor, v_cache: torch.Tensor, key_weights: tor
     short enough; pages of the old table that the new one does not hold keep
     what they hold, so it is the form for pages that other sequences share).
     Every page of the context must be mapped.  A sequence's new row may hold
-    pages of its old one at the same places (a copy of the table, its first
-    columns), but no page of ``block_tables`` at another place or of another
+    pages of its context at the same places (a copy of the table, its first
+    columns), but none of a context's pages at another place or of another
     sequence.  What rows go to is rewritten: a prefix cache must not serve
     those pages by their old tokens.  In place, few sequences of many kept rows
     go by way of scratch as large as those rows of K and V.
