@@ -440,6 +440,62 @@ int nsv_sample(const void* logits, int64_t row_stride, const float* temperature,
                size_t workspace_bytes, void* stream);
 
 /*
+ * Sampling and acceptance under a temperature, top-k, top-p and min-p, from
+ * one uniform number per draw.  No reference counterpart (its sampler and its
+ * acceptance have a temperature only).
+ *
+ * Of a row x of V logits with maximum M: temperature <= 1e-6 (or NaN), and any
+ * row with a NaN or with nothing above -inf, leave the argmax alone (first
+ * maximum; NaN above all).  Otherwise w = exp((x - M) / temperature), 1 where
+ * x == M and 0 where x == -inf; the tokens are ordered by falling x, equal ones
+ * by rising index, and each filter leaves a beginning of the order:
+ *   top_k  the first top_k (<= 0 or >= V: all)
+ *   top_p  the fewest (one at least) whose sum of w reaches top_p times the sum
+ *          of what top_k left (>= 1 or NaN: all)
+ *   min_p  those with w >= min_p, every maximum at least (<= 0 or NaN: all)
+ * What all three leave has the sum W; p(token) = w / W in it, 0 outside.  The
+ * sample of u is the first token of the order whose running sum exceeds u W.
+ * Sums are exact to 2^-44 of the largest weight per token.  top_k, top_p and
+ * min_p are [B] and may be NULL (all stay); uniforms are in [0, 1).
+ * V <= 2^20, B <= 65,535; K <= 63.
+ *
+ * nsv_sample_filtered: row b at b * row_stride elements (any row_stride >= V),
+ *   temperature and uniforms [B] fp32; the token goes to
+ *   out_tokens[b * out_stride]; kept [B] int32 (nullable): how many tokens the
+ *   filters left.
+ *
+ * nsv_accept_filtered: target and draft rows, drafts, num_drafts, draft_mode,
+ *   out_tokens and out_len as nsv_accept_stochastic's (entries past a
+ *   sequence's tokens are not written); temperature and filters [B], the same
+ *   for a sequence's target and draft rows; uniforms [B, K + 1].  A sequence
+ *   with draft rows and temperature > 1e-6 keeps draft i if
+ *   uniforms[i] * p_draft(d_i) < p_target(d_i); at the first that it does not,
+ *   the token is the first index whose running sum of
+ *   max(p_target - p_draft, 0) exceeds uniforms[K] times their sum (of
+ *   p_target where that sum is 0); behind kept drafts it is the sample of
+ *   uniforms[K] of row num_drafts.  Any other sequence takes the sample of
+ *   uniforms[r] of every row r, and keeps drafts while they equal it.
+ *   A draft outside [0, V) has probability 0.  Workspace:
+ *   nsv_accept_filtered_workspace_size() bytes on 16 bytes, of any content.
+ */
+int nsv_sample_filtered(const void* logits, int64_t row_stride,
+                        const float* temperature, const int32_t* top_k,
+                        const float* top_p, const float* min_p,
+                        const float* uniforms, int B, int V, int dtype,
+                        int32_t* out_tokens, int64_t out_stride,
+                        int32_t* kept, void* stream);
+size_t nsv_accept_filtered_workspace_size(int B, int K, int V);
+int nsv_accept_filtered(const void* target_logits, int64_t target_seq_stride,
+                        const void* draft_logits, int64_t draft_seq_stride,
+                        int64_t draft_row_stride, const int32_t* draft_mode,
+                        const int32_t* drafts, const int32_t* num_drafts,
+                        const float* temperature, const int32_t* top_k,
+                        const float* top_p, const float* min_p,
+                        const float* uniforms, int B, int K, int V, int dtype,
+                        int32_t* out_tokens, int32_t* out_len,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * N-gram (prompt-lookup) drafting on a device-resident token history.
  * Replaces src/myvllm/spec_engine/drafters.py:63-83 (NgramDrafter._lookup,
  * a bytes.rfind over the big-endian uint32 encoding of the history) and the

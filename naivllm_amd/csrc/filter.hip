@@ -1,0 +1,718 @@
+// Sampling and acceptance of drafts under a temperature, top-k, top-p and
+// min-p, for gfx950.  No reference counterpart (its sampler has a temperature
+// only); the operators stand beside nsv_sample and nsv_accept_stochastic.
+//
+// Of a row x with maximum M and temperature T the weights are
+// w = exp((x - M) / T) (1 where x = M, 0 where x = -inf), and its tokens are
+// ordered by falling x, equal ones by rising index.  Each filter leaves a
+// beginning of that order: top-k its first k; top-p the fewest whose sum
+// reaches p times the sum that top-k left; min-p those with w >= min_p.  So
+// what all of them leave is described by its last token: a value, and an index
+// among the tokens of that value.  The sample of u is the first token whose
+// running sum along the order exceeds u W, W the sum of what is left: one
+// uniform number per row, and no noise of the vocabulary's size to draw and
+// read.  T <= 1e-6, and rows with a NaN or without a value above -inf, leave
+// the argmax alone (first maximum, NaN above all, torch's rule).
+//
+// filter_rows_kernel works one row out per workgroup.  A value is found by
+// radix descent over its order-preserving bits: per level a histogram in LDS
+// of the row's tokens below the prefix so far, counts and weights, and a scan
+// of its bins.  Weights are added up as 64-bit integers, w 2^s rounded, so
+// sums do not depend on the order of the additions; s leaves room for the
+// vocabulary (44 bits for 2^18 tokens), each weight off by 2^-45 of the
+// largest, where fp32 sums would move the sample of one row in a hundred.
+
+#include "common.h"
+#include "exp_f64.h"
+
+namespace {
+
+constexpr int kRowThreads = 1024;
+constexpr int kRowWaves = kRowThreads / 64;
+constexpr int kBins = 2048;
+constexpr int kVec = 8;                          // elements a thread takes at a time
+constexpr int kStep = kRowThreads * kVec;        // elements a workgroup takes at a time
+constexpr int kMaxVocab = 1 << 20;
+constexpr int kMaxSteps = kMaxVocab / kStep + 1; // (a row that starts off a 16-byte boundary)
+constexpr int kMaxDrafts = 63;                   // K + 1 rows fit one 64-lane ballot
+constexpr int kChunkThreads = 256;
+constexpr int kChunk = kChunkThreads * kVec;     // of the residual passes
+
+template <typename T> struct Elem;
+template <> struct Elem<uint16_t> {  // bf16 bits
+  __device__ static float get(uint16_t v) { return bf16_bits_to_f32(v); }
+  __device__ static float unpack(const u32x4& w, int e) {
+    return bf16_bits_to_f32((e & 1) ? (w[e >> 1] >> 16) : (w[e >> 1] & 0xffffu));
+  }
+};
+template <> struct Elem<float> {
+  __device__ static float get(float v) { return v; }
+  __device__ static float unpack(const u32x4& w, int e) { return __uint_as_float(w[e]); }
+};
+
+// What the filters leave of a row: tokens of x > cut, and of x == cut up to
+// the index `last`; top: the row's maximum; total: W; kept: how many.  kept 1
+// is `token` alone, whatever the row holds.
+struct RowCut {
+  float top, cut;
+  int32_t last, kept, token, pad;
+  double total;
+};
+
+struct FilterArgs {
+  const void* target;      // row r of sequence b at b * t_seq + r * t_row elements
+  int64_t t_seq, t_row;
+  const void* draft;       // nullable; row i of sequence b at (b * d_seq + i * d_row) * V
+  int64_t d_seq, d_row;
+  int B, K, V;             // K -1: the sampler (one row per sequence, one uniform)
+  int shift;               // weights are held as integers, w 2^shift
+  const float* temperature;
+  const int32_t* top_k;    // nullable
+  const float* top_p;      // nullable
+  const float* min_p;      // nullable
+  const float* uniforms;   // [B, K + 1]
+  const int32_t* drafts;   // [B, K]
+  const int32_t* num_drafts;
+  const int32_t* mode;     // nullable; 0: sequence b has no draft rows
+  RowCut* cuts;            // [B, 2K + 1]: target rows 0..K, then draft rows
+  double* probs;           // [B, 2K + 1]: the probability of the row's draft
+  double* parts;           // [B, chunks, 2]: sums of the residual and of p_target
+  int chunks;
+  int32_t* tokens;         // sampler: row b's at b * out_stride
+  int64_t out_stride;
+  int32_t* kept;           // sampler, nullable
+  int32_t* out_tokens;     // [B, K + 1]
+  int32_t* out_len;
+};
+
+__device__ __forceinline__ bool is_greedy(float T) { return !(T > 1e-6f); }
+// u of the sample's goal u W: what is no number in [0, 1] is taken to its end
+__device__ __forceinline__ double unit(float u) { return fmin(fmax((double)u, 0.0), 1.0); }
+// sequence b's drafts are decided by their probabilities
+__device__ __forceinline__ bool by_rows(const FilterArgs& a, int b) {
+  return a.draft && !(a.mode && a.mode[b] == 0) && !is_greedy(a.temperature[b]);
+}
+__device__ __forceinline__ int draft_count(const FilterArgs& a, int b) { return min(max(a.num_drafts[b], 0), a.K); }
+__device__ __forceinline__ int64_t draft_at(const FilterArgs& a, int b, int i) {
+  return ((int64_t)b * a.d_seq + (int64_t)i * a.d_row) * a.V;
+}
+
+// order-preserving bits, complemented: rising along the order of the tokens;
+// -0 as +0
+__device__ __forceinline__ uint32_t order_bits(float x) {
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return (u & 0x80000000u) ? u : ~(u | 0x80000000u);
+}
+__device__ __forceinline__ float order_value(uint32_t k) {
+  return __uint_as_float((k & 0x80000000u) ? k : ~(k | 0x80000000u));
+}
+
+__device__ __forceinline__ double weight_of(float x, float top, double inv_t, const double* tab) {
+  return x == top ? 1.0 : nsv_exp_nonpos(((double)x - (double)top) * inv_t, tab);
+}
+// w 2^shift, rounded: added to 2^52 it lies in the low bits of the sum
+__device__ __forceinline__ uint64_t fixed_weight(double w, double scale) {
+  return (uint64_t)__double_as_longlong(fma(w, scale, 0x1p52)) & 0x000fffffffffffffull;
+}
+
+// elements base .. base + 7 of a row, those past its end -inf
+template <typename T>
+__device__ __forceinline__ void load_vec(const T* row, int64_t base, int V, float (&x)[kVec]) {
+  constexpr int PER = 16 / sizeof(T);
+  if (((uintptr_t)row & 15) == 0 && base + kVec <= V) {
+    u32x4 w[kVec / PER];
+#pragma unroll
+    for (int l = 0; l < kVec / PER; ++l) w[l] = *reinterpret_cast<const u32x4*>(row + base + l * PER);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x[e] = Elem<T>::unpack(w[e / PER], e % PER);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) x[e] = base + e < V ? Elem<T>::get(row[base + e]) : -__builtin_inff();
+  }
+}
+
+// f(index, x) of every element of a row, a workgroup's threads together
+template <typename T, typename F>
+__device__ __forceinline__ void each(const T* row, int V, F f) {
+  for (int64_t lo = 0; lo < V; lo += kStep) {
+    const int64_t base = lo + kVec * threadIdx.x;
+    if (base >= V) continue;
+    float x[kVec];
+    load_vec<T>(row, base, V, x);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e)
+      if (base + e < V) f((int)(base + e), x[e]);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {  // inclusive
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const T o = __shfl_up(v, d);
+    if (lane >= d) v += o;
+  }
+  return v;
+}
+
+struct RowLds {
+  uint32_t count[kBins];
+  unsigned long long mass[kBins];
+  uint32_t found[kMaxSteps * kRowWaves];
+  uint64_t red[kRowWaves];
+  uint64_t red2[kRowWaves];
+  double tab[256];
+  int hit;
+  uint64_t hit_mass, hit_before;
+  uint32_t hit_count, hit_cbefore;
+};
+
+__device__ __forceinline__ uint64_t block_max(uint64_t v, RowLds& s) {
+  v = wave_max_u64_dpp(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) s.red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  uint64_t r = s.red[0];
+  for (int i = 1; i < kRowWaves; ++i) r = s.red[i] > r ? s.red[i] : r;
+  return r;
+}
+__device__ __forceinline__ uint64_t block_sum(uint64_t v, RowLds& s) {
+  v = wave_scan(v);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 63) s.red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  uint64_t r = 0;
+  for (int i = 0; i < kRowWaves; ++i) r += s.red[i];
+  return r;
+}
+
+// A place in the order: the tokens of one value, what lies before them, and
+// the weight of each.
+struct Spot {
+  uint32_t key;            // order_bits of the value
+  uint32_t before, count;  // tokens
+  uint64_t mass;           // weights before
+  uint64_t weight;
+};
+enum Seek { kByCount, kReach, kBeyond };
+
+// The last value with: tokens before it < goal (kByCount); weights before it
+// < goal (kReach) or <= goal (kBeyond), and a weight of its own.
+template <typename T>
+__device__ Spot seek(Seek kind, double goal, const T* row, int V, float top, double inv_t, double scale, RowLds& s) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Spot at{0u, 0u, 0u, 0ull, 0ull};
+  constexpr int kShift[3] = {21, 10, 0}, kWidth[3] = {11, 11, 10};
+  for (int level = 0; level < 3; ++level) {
+    const int sh = kShift[level], bits = kWidth[level];
+    __syncthreads();
+    for (int i = tid; i < kBins; i += kRowThreads) {
+      s.count[i] = 0;
+      s.mass[i] = 0;
+    }
+    if (tid == 0) s.hit = -1;
+    __syncthreads();
+    each<T>(row, V, [&](int, float x) {
+      const uint32_t k = order_bits(x);
+      if (level && (k >> (sh + bits)) != (at.key >> (sh + bits))) return;
+      const uint32_t bin = (k >> sh) & ((1u << bits) - 1);
+      atomicAdd(&s.count[bin], 1u);
+      const uint64_t q = fixed_weight(weight_of(x, top, inv_t, s.tab), scale);
+      if (q) atomicAdd(&s.mass[bin], (unsigned long long)q);
+    });
+    __syncthreads();
+    const uint32_t c0 = s.count[2 * tid], c1 = s.count[2 * tid + 1];
+    const uint64_t m0 = s.mass[2 * tid], m1 = s.mass[2 * tid + 1];
+    const uint32_t c = wave_scan(c0 + c1);
+    const uint64_t m = wave_scan(m0 + m1);
+    if (lane == 63) {
+      s.red[wave] = c;
+      s.red2[wave] = m;
+    }
+    __syncthreads();
+    uint32_t cb = at.before + c - c0 - c1;
+    uint64_t mb = at.mass + m - m0 - m1;
+    for (int i = 0; i < wave; ++i) {
+      cb += (uint32_t)s.red[i];
+      mb += s.red2[i];
+    }
+    auto fits = [&](uint32_t n, uint64_t w, uint32_t before, uint64_t mass) {
+      if (kind == kByCount) return n > 0 && (double)before < goal;
+      return w > 0 && (kind == kReach ? (double)mass < goal : (double)mass <= goal);
+    };
+    int best = -1;
+    if (fits(c0, m0, cb, mb)) best = 2 * tid;
+    if (fits(c1, m1, cb + c0, mb + m0)) best = 2 * tid + 1;
+    if (best >= 0) atomicMax(&s.hit, best);
+    __syncthreads();
+    if (best >= 0 && best == s.hit) {
+      const bool second = best & 1;
+      s.hit_cbefore = cb + (second ? c0 : 0);
+      s.hit_before = mb + (second ? m0 : 0);
+      s.hit_count = second ? c1 : c0;
+      s.hit_mass = second ? m1 : m0;
+    }
+    __syncthreads();
+    at.key |= (uint32_t)max(s.hit, 0) << sh;
+    at.before = s.hit_cbefore;
+    at.mass = s.hit_before;
+    at.count = s.hit_count;
+    at.weight = s.hit_mass;
+  }
+  at.weight /= at.count;  // (equal values have equal weights)
+  return at;
+}
+
+// index of the token with j of its value before it
+template <typename T>
+__device__ int index_of(float value, uint32_t j, const T* row, int V, RowLds& s) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int steps = (V + kStep - 1) / kStep;
+  __syncthreads();
+  for (int it = 0; it < steps; ++it) {
+    const int64_t base = (int64_t)it * kStep + kVec * threadIdx.x;
+    float x[kVec];
+    int n = 0;
+    if (base < V) {
+      load_vec<T>(row, base, V, x);
+      for (int e = 0; e < kVec; ++e) n += base + e < V && x[e] == value;
+    }
+    n = (int)wave_scan((uint32_t)n);
+    if (lane == 63) s.found[it * kRowWaves + wave] = n;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    uint32_t left = j;
+    int g = 0;
+    while (g < steps * kRowWaves - 1 && left >= s.found[g]) left -= s.found[g++];
+    s.hit = g;
+    s.hit_count = left;
+  }
+  __syncthreads();
+  const int g = s.hit;
+  const uint32_t left = s.hit_count;
+  if (wave == g % kRowWaves) {
+    const int64_t base = (int64_t)(g / kRowWaves) * kStep + kVec * threadIdx.x;
+    float x[kVec];
+    uint32_t n = 0;
+    if (base < V) {
+      load_vec<T>(row, base, V, x);
+      for (int e = 0; e < kVec; ++e) n += base + e < V && x[e] == value;
+    }
+    uint32_t before = wave_scan(n) - n;
+    if (base < V)
+      for (int e = 0; e < kVec; ++e)
+        if (base + e < V && x[e] == value) {
+          if (before == left) s.hit_cbefore = (uint32_t)(base + e);
+          ++before;
+        }
+  }
+  __syncthreads();
+  return (int)s.hit_cbefore;
+}
+
+// What the filters leave of a row, and its sample of u where one is wanted.
+template <typename T>
+__device__ RowCut filter_row(const FilterArgs& a, int b, const T* row, bool sampled, float u, bool ends, RowLds& s) {
+  const int V = a.V;
+  const float T_ = a.temperature[b];
+  RowCut out;
+  // the argmax: NaN above all, equal values by the lower index
+  uint64_t best = 0;
+  each<T>(row, V, [&](int i, float x) {
+    const uint32_t k = x != x ? 0xffffffffu : ~order_bits(x);
+    const uint64_t key = ((uint64_t)k << 32) | (uint32_t)~i;
+    best = key > best ? key : best;
+  });
+  best = block_max(best, s);
+  const int first = (int)~(uint32_t)best;
+  const bool nan = (uint32_t)(best >> 32) == 0xffffffffu;
+  out.top = nan ? __builtin_nanf("") : order_value(~(uint32_t)(best >> 32));
+  out.cut = out.top;
+  out.last = out.token = first;
+  out.kept = 1;
+  out.pad = 0;
+  out.total = 1.0;
+  if (is_greedy(T_) || nan || out.top == -__builtin_inff()) return out;  // uniform
+
+  const double inv_t = 1.0 / (double)T_, scale = (double)(1ull << a.shift);
+  const float top = out.top;
+  if (threadIdx.x < 256) s.tab[threadIdx.x] = kExp2Frac256[threadIdx.x];
+  const int k = a.top_k ? a.top_k[b] : 0;
+  const double p = a.top_p ? (double)a.top_p[b] : 1.0, m = a.min_p ? (double)a.min_p[b] : 0.0;
+  out.kept = V;
+  out.cut = -__builtin_inff();
+  out.last = V - 1;
+  __syncthreads();
+  uint64_t total;
+  if (k > 0 && k < V) {
+    const Spot at = seek<T>(kByCount, (double)k, row, V, top, inv_t, scale, s);
+    out.kept = k;
+    out.cut = order_value(at.key);
+    out.last = (uint32_t)k - at.before == at.count ? V - 1 : -(int)((uint32_t)k - at.before);  // (negative: to be looked up)
+    total = at.mass + (uint64_t)((uint32_t)k - at.before) * at.weight;
+  } else {
+    uint64_t sum = 0;
+    each<T>(row, V, [&](int, float x) { sum += fixed_weight(weight_of(x, top, inv_t, s.tab), scale); });
+    total = block_sum(sum, s);
+  }
+  if (p < 1.0) {
+    const double goal = fmax(p * (double)total, 0.5);  // (the first token stays)
+    const Spot at = seek<T>(kReach, goal, row, V, top, inv_t, scale, s);
+    const double need = ceil((goal - (double)at.mass) / (double)at.weight);
+    const uint32_t n = (uint32_t)fmin(fmax(need, 1.0), (double)at.count);
+    if ((int)(at.before + n) < out.kept) {
+      out.kept = (int)(at.before + n);
+      out.cut = order_value(at.key);
+      out.last = n == at.count ? V - 1 : -(int)n;
+      total = at.mass + (uint64_t)n * at.weight;
+    }
+  }
+  if (m > 0.0) {
+    uint64_t sum = 0, count = 0, low = 0;  // low: the furthest key along the order
+    each<T>(row, V, [&](int, float x) {
+      const double w = weight_of(x, top, inv_t, s.tab);
+      if (x != top && !(w >= m)) return;
+      sum += fixed_weight(w, scale);
+      ++count;
+      const uint64_t key = order_bits(x);
+      low = key > low ? key : low;
+    });
+    count = block_sum(count, s);
+    if ((int)count < out.kept) {
+      out.kept = (int)count;
+      out.last = V - 1;
+      total = block_sum(sum, s);
+      out.cut = order_value((uint32_t)block_max(low, s));
+    }
+  }
+  out.total = (double)total / scale;
+  if (sampled) {
+    const double goal = unit(u) * (double)total;
+    const Spot at = seek<T>(kBeyond, goal, row, V, top, inv_t, scale, s);
+    double j = floor((goal - (double)at.mass) / (double)at.weight);
+    j = fmin(fmax(j, 0.0), (double)(at.count - 1));
+    j = fmin(j, (double)(out.kept - 1 - (int)at.before));
+    out.token = index_of<T>(order_value(at.key), (uint32_t)j, row, V, s);
+  }
+  if (out.last < 0) out.last = ends ? index_of<T>(out.cut, (uint32_t)(-out.last - 1), row, V, s) : V - 1;
+  return out;
+}
+
+// probability of token i of logit x
+__device__ __forceinline__ double prob_of(const RowCut& c, float x, int i, double inv_t, const double* tab) {
+  if (c.kept == 1) return i == c.token ? 1.0 : 0.0;
+  const bool in = x > c.cut || (x == c.cut && i <= c.last);
+  return in ? weight_of(x, c.top, inv_t, tab) / c.total : 0.0;
+}
+
+// grid (rows per sequence, B): target rows, then draft rows
+template <typename T>
+__global__ __launch_bounds__(kRowThreads) void filter_rows_kernel(FilterArgs a) {
+  __shared__ RowLds s;
+  const int b = blockIdx.y, r = blockIdx.x;
+  if (a.K < 0) {
+    const RowCut c = filter_row<T>(a, b, (const T*)a.target + (int64_t)b * a.t_seq, true, a.uniforms[b], false, s);
+    if (threadIdx.x == 0) {
+      a.tokens[(int64_t)b * a.out_stride] = c.token;
+      if (a.kept) a.kept[b] = c.kept;
+    }
+    return;
+  }
+  const int kb = draft_count(a, b);
+  const bool rows = by_rows(a, b), is_draft = r > a.K;
+  const int i = is_draft ? r - a.K - 1 : r;
+  if (is_draft ? !rows || i >= kb : i > kb) return;  // uniform
+  const T* row = is_draft ? (const T*)a.draft + draft_at(a, b, i)
+                          : (const T*)a.target + (int64_t)b * a.t_seq + (int64_t)i * a.t_row;
+  const bool sampled = !rows || i == kb;
+  const float u = a.uniforms[(int64_t)b * (a.K + 1) + (rows ? a.K : i)];
+  const RowCut c = filter_row<T>(a, b, row, sampled, u, !sampled, s);
+  if (threadIdx.x != 0) return;
+  const int64_t at = (int64_t)b * (2 * a.K + 1) + r;
+  a.cuts[at] = c;
+  if (rows && i < kb) {
+    const int32_t d = a.drafts[(int64_t)b * a.K + i];
+    const bool in = d >= 0 && d < a.V;  // a token outside the vocabulary has probability 0
+    const double inv_t = 1.0 / (double)a.temperature[b];
+    a.probs[at] = in ? prob_of(c, Elem<T>::get(row[d]), d, inv_t, kExp2Frac256) : 0.0;
+  }
+}
+
+// drafts accepted before the first refused (a whole wave)
+__device__ __forceinline__ int accepted_by_rows(const FilterArgs& a, int b, int kb) {
+  const int i = threadIdx.x & 63;
+  bool refused = false;
+  if (i < kb) {
+    const double pt = a.probs[(int64_t)b * (2 * a.K + 1) + i], pd = a.probs[(int64_t)b * (2 * a.K + 1) + a.K + 1 + i];
+    refused = !((double)a.uniforms[(int64_t)b * (a.K + 1) + i] * pd < pt);
+  }
+  const uint64_t no = __ballot(refused);
+  return no ? __ffsll((long long)no) - 1 : kb;
+}
+
+// a thread's residuals max(p_target - p_draft, 0) and p_target of a chunk
+template <typename T>
+__device__ __forceinline__ void residuals(const FilterArgs& a, int b, int r, int ch, const double* tab, double (&left)[kVec],
+                                          double (&pt)[kVec]) {
+  const T* t = (const T*)a.target + (int64_t)b * a.t_seq + (int64_t)r * a.t_row;
+  const T* d = (const T*)a.draft + draft_at(a, b, r);
+  const RowCut ct = a.cuts[(int64_t)b * (2 * a.K + 1) + r], cd = a.cuts[(int64_t)b * (2 * a.K + 1) + a.K + 1 + r];
+  const double inv_t = 1.0 / (double)a.temperature[b];
+  const int64_t base = (int64_t)ch * kChunk + kVec * threadIdx.x;
+  float xt[kVec], xd[kVec];
+  if (base < a.V) {
+    load_vec<T>(t, base, a.V, xt);
+    load_vec<T>(d, base, a.V, xd);
+  }
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    left[e] = pt[e] = 0.0;
+    if (base + e >= a.V) continue;
+    pt[e] = prob_of(ct, xt[e], (int)(base + e), inv_t, tab);
+    if (pt[e] > 0.0) left[e] = fmax(pt[e] - prob_of(cd, xd[e], (int)(base + e), inv_t, tab), 0.0);
+  }
+}
+
+// grid (chunks, B): chunk sums of the refused row's residuals
+template <typename T>
+__global__ __launch_bounds__(kChunkThreads) void filter_residual_kernel(FilterArgs a) {
+  __shared__ double tab[256], red[2 * kChunkThreads / 64];
+  const int b = blockIdx.y, ch = blockIdx.x;
+  if (!by_rows(a, b)) return;  // uniform
+  const int kb = draft_count(a, b), n = accepted_by_rows(a, b, kb);
+  if (n == kb) return;  // uniform: every draft stays
+  tab[threadIdx.x] = kExp2Frac256[threadIdx.x];
+  __syncthreads();
+  double left[kVec], pt[kVec], sl = 0.0, sp = 0.0;
+  residuals<T>(a, b, n, ch, tab, left, pt);
+  for (int e = 0; e < kVec; ++e) {
+    sl += left[e];
+    sp += pt[e];
+  }
+  sl = wave_sum_dpp(sl);
+  sp = wave_sum_dpp(sp);
+  if ((threadIdx.x & 63) == 0) {
+    red[2 * (threadIdx.x >> 6)] = sl;
+    red[2 * (threadIdx.x >> 6) + 1] = sp;
+  }
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    double r = 0.0;
+    for (int w = 0; w < kChunkThreads / 64; ++w) r += red[2 * w + threadIdx.x];
+    a.parts[((int64_t)b * a.chunks + ch) * 2 + threadIdx.x] = r;
+  }
+}
+
+// grid B: the sequence's tokens
+template <typename T>
+__global__ __launch_bounds__(kChunkThreads) void filter_finish_kernel(FilterArgs a) {
+  __shared__ double tab[256], red[kChunkThreads / 64], goal_s, before_s;
+  __shared__ int which, use_pt, token;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int K = a.K, kb = draft_count(a, b);
+  const RowCut* cuts = a.cuts + (int64_t)b * (2 * K + 1);
+  int32_t* out = a.out_tokens + (int64_t)b * (K + 1);
+  const int32_t d = lane < kb ? a.drafts[(int64_t)b * K + lane] : -1;
+  if (!by_rows(a, b)) {  // uniform: every row was sampled
+    if (wave) return;
+    const int32_t t = lane <= kb ? cuts[lane].token : 0;
+    const uint64_t no = __ballot(lane < kb && t != d);
+    const int n = no ? __ffsll((long long)no) - 1 : kb;
+    if (lane <= n) out[lane] = t;
+    if (lane == 0) a.out_len[b] = n + 1;
+    return;
+  }
+  const int n = accepted_by_rows(a, b, kb);
+  if (wave == 0 && lane < n) out[lane] = d;
+  if (tid == 0) a.out_len[b] = n + 1;
+  if (n == kb) {  // uniform: the bonus token
+    if (tid == 0) out[n] = cuts[n].token;
+    return;
+  }
+  tab[tid] = kExp2Frac256[tid];
+  // the chunk that holds the token: the last with any weight whose sums before it do not exceed the goal
+  const double* parts = a.parts + (int64_t)b * a.chunks * 2;
+  if (wave == 0) {
+    double sl = 0.0;
+    for (int c = lane; c < a.chunks; c += 64) sl += parts[2 * c];
+    const int col = wave_sum_dpp(sl) > 0.0 ? 0 : 1;  // no residual: the target row itself
+    double total = 0.0;
+    for (int c0 = 0; c0 < a.chunks; c0 += 64) {
+      const double v = wave_scan(c0 + lane < a.chunks ? parts[2 * (c0 + lane) + col] : 0.0);
+      total += __shfl(v, 63);
+    }
+    const double goal = unit(a.uniforms[(int64_t)b * (K + 1) + K]) * total;
+    double run = 0.0, before = 0.0;
+    int at = 0;
+    for (int c0 = 0; c0 < a.chunks; c0 += 64) {
+      const double mine = c0 + lane < a.chunks ? parts[2 * (c0 + lane) + col] : 0.0;
+      const double v = wave_scan(mine);
+      double prev = __shfl_up(v, 1);
+      if (lane == 0) prev = 0.0;
+      const uint64_t yes = __ballot(mine > 0.0 && run + prev <= goal);
+      if (yes) {
+        const int l = 63 - __clzll((long long)yes);
+        at = c0 + l;
+        before = run + __shfl(prev, l);
+      }
+      run += __shfl(v, 63);
+    }
+    if (lane == 0) {
+      which = at;
+      use_pt = col;
+      goal_s = goal;
+      before_s = before;
+      token = -1;
+    }
+  }
+  __syncthreads();
+  double left[kVec], pt[kVec];
+  residuals<T>(a, b, n, which, tab, left, pt);
+  double mine = 0.0;
+  for (int e = 0; e < kVec; ++e) {
+    if (use_pt) left[e] = pt[e];
+    mine += left[e];
+  }
+  const double v = wave_scan(mine);
+  double run = __shfl_up(v, 1);
+  if (lane == 0) run = 0.0;
+  if (lane == 63) red[wave] = v;
+  __syncthreads();
+  double before = before_s;
+  for (int w = 0; w < wave; ++w) before += red[w];
+  run += before;
+  // the last element with any weight whose sums before it do not exceed the goal
+  int best = -1;
+  for (int e = 0; e < kVec; ++e) {
+    if (left[e] > 0.0 && run <= goal_s) best = which * kChunk + kVec * tid + e;
+    run += left[e];
+  }
+  if (best >= 0) atomicMax(&token, best);
+  __syncthreads();
+  if (tid == 0) out[n] = token;
+}
+
+bool bad_rows(int B, int V, int dtype) { return B < 0 || V <= 0 || (dtype != NSV_F32 && dtype != NSV_BF16); }
+
+// weights as integers: V of them, each at most 2^shift, stay below 2^62
+int weight_shift(int V) {
+  int bits = 0;
+  while ((1 << bits) < V) ++bits;
+  const int s = 62 - bits;
+  return s > 50 ? 50 : s;
+}
+
+size_t a256(size_t x) { return (x + 255) & ~(size_t)255; }
+int residual_chunks(int V) { return (V + kChunk - 1) / kChunk; }
+
+struct Layout {
+  size_t cuts, probs, parts, total;
+};
+Layout layout(int B, int K, int V) {
+  Layout L;
+  const size_t rows = (size_t)B * (2 * (size_t)K + 1);
+  L.cuts = 0;
+  L.probs = a256(rows * sizeof(RowCut));
+  L.parts = L.probs + a256(rows * sizeof(double));
+  L.total = L.parts + a256((size_t)B * residual_chunks(V) * 2 * sizeof(double));
+  return L;
+}
+
+void launch_rows(const FilterArgs& a, int rows, int dtype, hipStream_t s) {
+  const dim3 grid(rows, a.B);
+  if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_rows_kernel<uint16_t>, grid, dim3(kRowThreads), 0, s, a);
+  else hipLaunchKernelGGL(filter_rows_kernel<float>, grid, dim3(kRowThreads), 0, s, a);
+}
+
+}  // namespace
+
+extern "C" {
+
+int nsv_sample_filtered(const void* logits, int64_t row_stride, const float* temperature, const int32_t* top_k,
+                        const float* top_p, const float* min_p, const float* uniforms, int B, int V, int dtype,
+                        int32_t* out_tokens, int64_t out_stride, int32_t* kept, void* stream) {
+  if (bad_rows(B, V, dtype) || row_stride < V || out_stride < 1) return NSV_ERR_ARG;
+  if (V > kMaxVocab || B > 65535) return NSV_ERR_UNSUPPORTED;
+  if (B == 0) return NSV_OK;
+  if (!logits || !temperature || !uniforms || !out_tokens) return NSV_ERR_ARG;
+  FilterArgs a{};
+  a.target = logits;
+  a.t_seq = row_stride;
+  a.B = B;
+  a.K = -1;
+  a.V = V;
+  a.shift = weight_shift(V);
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.uniforms = uniforms;
+  a.tokens = out_tokens;
+  a.out_stride = out_stride;
+  a.kept = kept;
+  launch_rows(a, 1, dtype, (hipStream_t)stream);
+  return nsv_launch_status();
+}
+
+size_t nsv_accept_filtered_workspace_size(int B, int K, int V) {
+  if (B < 0 || K < 0 || K > kMaxDrafts || V <= 0) return 0;
+  return layout(B, K, V).total;
+}
+
+int nsv_accept_filtered(const void* target_logits, int64_t target_seq_stride, const void* draft_logits,
+                        int64_t draft_seq_stride, int64_t draft_row_stride, const int32_t* draft_mode,
+                        const int32_t* drafts, const int32_t* num_drafts, const float* temperature, const int32_t* top_k,
+                        const float* top_p, const float* min_p, const float* uniforms, int B, int K, int V, int dtype,
+                        int32_t* out_tokens, int32_t* out_len, void* workspace, size_t workspace_bytes, void* stream) {
+  if (bad_rows(B, V, dtype) || K < 0 || K > kMaxDrafts || target_seq_stride < K + 1) return NSV_ERR_ARG;
+  if (draft_logits && (draft_row_stride < 1 || draft_seq_stride < 0)) return NSV_ERR_ARG;
+  if (draft_mode && !draft_logits) return NSV_ERR_ARG;
+  if (V > kMaxVocab || B > 65535) return NSV_ERR_UNSUPPORTED;
+  if (B == 0) return NSV_OK;
+  if (!target_logits || (!drafts && K > 0) || !num_drafts || !temperature || !uniforms || !out_tokens || !out_len)
+    return NSV_ERR_ARG;
+  const Layout L = layout(B, K, V);
+  if (!workspace || workspace_bytes < L.total) return NSV_ERR_WORKSPACE;
+  FilterArgs a{};
+  a.target = target_logits;
+  a.t_seq = target_seq_stride * V;
+  a.t_row = V;
+  a.draft = K > 0 ? draft_logits : nullptr;
+  a.d_seq = draft_seq_stride;
+  a.d_row = draft_row_stride;
+  a.B = B;
+  a.K = K;
+  a.V = V;
+  a.shift = weight_shift(V);
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.uniforms = uniforms;
+  a.drafts = drafts;
+  a.num_drafts = num_drafts;
+  a.mode = draft_mode;
+  a.cuts = (RowCut*)((char*)workspace + L.cuts);
+  a.probs = (double*)((char*)workspace + L.probs);
+  a.parts = (double*)((char*)workspace + L.parts);
+  a.chunks = residual_chunks(V);
+  a.out_tokens = out_tokens;
+  a.out_len = out_len;
+  hipStream_t s = (hipStream_t)stream;
+  launch_rows(a, a.draft ? 2 * K + 1 : K + 1, dtype, s);
+  int rc = nsv_launch_status();
+  if (rc) return rc;
+  if (a.draft) {
+    const dim3 grid(a.chunks, B);
+    if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_residual_kernel<uint16_t>, grid, dim3(kChunkThreads), 0, s, a);
+    else hipLaunchKernelGGL(filter_residual_kernel<float>, grid, dim3(kChunkThreads), 0, s, a);
+    if ((rc = nsv_launch_status())) return rc;
+  }
+  if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_finish_kernel<uint16_t>, dim3(B), dim3(kChunkThreads), 0, s, a);
+  else hipLaunchKernelGGL(filter_finish_kernel<float>, dim3(B), dim3(kChunkThreads), 0, s, a);
+  return nsv_launch_status();
+}
+
+}  // extern "C"

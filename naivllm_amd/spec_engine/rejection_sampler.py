@@ -14,6 +14,10 @@ rows (n-gram drafts) from ``generator``.  torch's multinomial(p, 1) is
 argmax(p / q) with q = empty_like(p).exponential_(1) drawn from the same
 generator, so ``draw_randomness`` draws u and q in exactly that order and
 the kernels reproduce the reference's samples from them.
+
+``sample_filtered`` and ``accept_filtered`` sample and accept under a
+temperature, top-k, top-p and min-p (the reference has a temperature only),
+from one uniform number per draw.
 """
 
 from __future__ import annotations
@@ -190,6 +194,171 @@ def sample(logits: torch.Tensor, temperature: torch.Tensor, noise: torch.Tensor,
                       out.stride(0) if B > 1 else 1, _lib.ptr(ws), nbytes, _lib.stream_ptr(dev))
     _lib.check(rc, "sample")
     return out
+
+
+def _per_row(x, rows: int, dtype: torch.dtype, device, name: str) -> torch.Tensor | None:
+    """A row's setting as a (rows,) tensor of the device: None stays None (the
+    filter is off), a number is every row's."""
+    if x is None:
+        return None
+    whole = dtype == torch.int32
+    if not isinstance(x, torch.Tensor):
+        if isinstance(x, bool) or not isinstance(x, int if whole else (int, float)):
+            raise ValueError(f"{name} must be a tensor or {'an integer' if whole else 'a number'}, got {x!r}")
+        return torch.full((rows,), min(x, 0x7fffffff) if whole else float(x), dtype=dtype, device=device)
+    if tuple(x.shape) != (rows,):
+        raise ValueError(f"{name} must have {rows} entries, got {tuple(x.shape)}")
+    if x.dtype != dtype:
+        if x.dtype == torch.bool or (whole and x.dtype.is_floating_point) or x.dtype.is_complex:
+            raise ValueError(f"{name}: unsupported dtype {x.dtype}")
+        if whole and x.dtype == torch.int64:
+            x = x.clamp(-1, 0x7fffffff)
+        x = x.to(dtype)
+    if x.device != device:
+        x = x.to(device)
+    return x if x.is_contiguous() else x.contiguous()
+
+
+def _check_out(t: torch.Tensor, shape: tuple, device, name: str, strided: bool = False) -> None:
+    if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device:
+        raise ValueError(f"{name} must be an int32 {shape} tensor on {device}")
+    if not t.is_contiguous() and not (strided and t.stride(0) >= 1):
+        raise ValueError(f"{name} must be contiguous")
+
+
+def sample_filtered(logits: torch.Tensor, temperature, uniforms: torch.Tensor, top_k=None, top_p=None, min_p=None,
+                    out: torch.Tensor | None = None, kept: torch.Tensor | None = None) -> torch.Tensor:
+    """Samples a token of every row under a temperature, top-k, top-p and
+    min-p, from one uniform number in [0, 1) per row.
+
+    logits (B, V) bfloat16 or float32 (rows contiguous, any pitch); V at most
+    2^20.  temperature, top_k, top_p and min_p are (B,) tensors, or numbers
+    for every row; None leaves a filter off, as do top_k <= 0, top_p >= 1 and
+    min_p <= 0.  uniforms (B,) float32.
+
+    Of a row's tokens in falling order of their logits (equal ones by rising
+    index) top-k leaves the first k, top-p the fewest whose probabilities
+    reach p of what top-k left, min-p those of at least min_p times the
+    largest probability.  The sample is the first token, in that order, whose
+    running sum exceeds the uniform number times the sum of what is left.
+    temperature <= 1e-6 takes the argmax, and so does a row with a NaN or
+    with no logit above -inf.
+
+    Returns / writes int32 tokens (B,) (``out`` may be a strided column of a
+    draft buffer); ``kept`` (B,) int32, when given, gets how many tokens the
+    filters left.  No counterpart in the reference."""
+    _check_logits(logits, "logits")
+    if logits.dim() != 2:
+        raise ValueError("logits must be (batch, vocab)")
+    B, V = logits.shape
+    dev = logits.device
+    pitch = logits.stride(0) if B > 1 else V
+    if pitch < V:
+        raise ValueError("logits rows must not overlap")
+    temperature = _per_row(temperature, B, torch.float32, dev, "temperature")
+    if temperature is None or uniforms is None:
+        raise ValueError("sample_filtered needs a temperature and uniforms")
+    uniforms = _per_row(uniforms, B, torch.float32, dev, "uniforms")
+    top_k = _per_row(top_k, B, torch.int32, dev, "top_k")
+    top_p = _per_row(top_p, B, torch.float32, dev, "top_p")
+    min_p = _per_row(min_p, B, torch.float32, dev, "min_p")
+    if out is None:
+        out = torch.empty(B, dtype=torch.int32, device=dev)
+    else:
+        _check_out(out, (B,), dev, "out", strided=True)
+    if kept is not None:
+        _check_out(kept, (B,), dev, "kept")
+    with _lib.on_device(dev):
+        rc = _lib.lib().nsv_sample_filtered(
+            logits.data_ptr(), pitch, temperature.data_ptr(), _lib.ptr(top_k), _lib.ptr(top_p), _lib.ptr(min_p),
+            uniforms.data_ptr(), B, V, _lib.dtype_code(logits.dtype), out.data_ptr(), out.stride(0) if B > 1 else 1,
+            _lib.ptr(kept), _lib.stream_ptr(dev))
+    _lib.check(rc, "sample_filtered")
+    return out
+
+
+def accept_filtered(target_logits: torch.Tensor, drafts: torch.Tensor, num_drafts: torch.Tensor, temperature,
+                    uniforms: torch.Tensor, draft_logits: torch.Tensor | None = None, top_k=None, top_p=None, min_p=None,
+                    target_seq_stride: int | None = None, draft_seq_stride: int = 0, draft_row_stride: int = 1,
+                    draft_mode: torch.Tensor | None = None, out_tokens: torch.Tensor | None = None,
+                    out_len: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Batched acceptance of drafts under the filters of sample_filtered,
+    which hold for a sequence's target and draft rows alike: the accepted
+    tokens are distributed as the filtered target's samples.
+
+    Rows, drafts, draft_mode and outputs as accept_stochastic's; temperature
+    and the filters (B,) tensors, numbers, or None.  uniforms (B, K + 1)
+    float32.  With draft rows and a temperature above 1e-6 a draft stays if
+    its uniform number times its draft probability is below its target
+    probability; at the first that does not, the last uniform number draws
+    from max(p_target - p_draft, 0) in the order of the indices; behind kept
+    drafts it samples the bonus row.  Otherwise uniform number r samples row
+    r, and drafts stay while they equal the samples.  Returns (tokens
+    (B, K + 1) int32, lengths (B,) int32) on the device; entries past a
+    sequence's tokens are not written.  No counterpart in the reference."""
+    _check_logits(target_logits, "target_logits")
+    dev = target_logits.device
+    V = target_logits.shape[-1]
+    if drafts.dim() != 2:
+        raise ValueError("drafts must be (batch, drafts)")
+    B, K = drafts.shape
+    if target_seq_stride is None:
+        target_seq_stride = K + 1
+    if target_seq_stride < K + 1:
+        raise ValueError("target_seq_stride must be at least K + 1 rows")
+    if not target_logits.is_contiguous():
+        raise ValueError("target_logits must be contiguous")
+    if B:
+        _check_extent(target_logits, ((B - 1) * target_seq_stride + K + 1) * V, "target_logits")
+    if draft_mode is not None and draft_logits is None:
+        raise ValueError("draft_mode selects per-sequence draft rows; draft_logits is missing")
+    if draft_logits is not None:
+        _check_logits(draft_logits, "draft_logits")
+        if draft_logits.dtype != target_logits.dtype or draft_logits.device != dev or draft_logits.shape[-1] != V:
+            raise ValueError("draft and target logits must share dtype, device and vocabulary")
+        if draft_row_stride < 1 or draft_seq_stride < 0:
+            raise ValueError("bad draft strides")
+        if B and K:
+            _check_extent(draft_logits, ((B - 1) * draft_seq_stride + (K - 1) * draft_row_stride + 1) * V, "draft_logits")
+        if draft_mode is not None:
+            draft_mode = _i32(draft_mode, dev)
+            if draft_mode.numel() != B:
+                raise ValueError("draft_mode must hold one flag per sequence")
+    if uniforms is None or tuple(uniforms.shape) != (B, K + 1):
+        raise ValueError(f"uniforms must be ({B}, {K + 1})")
+    uniforms = uniforms.to(device=dev, dtype=torch.float32).contiguous()
+    temperature = _per_row(temperature, B, torch.float32, dev, "temperature")
+    if temperature is None:
+        raise ValueError("accept_filtered needs a temperature")
+    top_k = _per_row(top_k, B, torch.int32, dev, "top_k")
+    top_p = _per_row(top_p, B, torch.float32, dev, "top_p")
+    min_p = _per_row(min_p, B, torch.float32, dev, "min_p")
+    drafts = _i32(drafts, dev)
+    num_drafts = _i32(num_drafts, dev)
+    if num_drafts.numel() != B:
+        raise ValueError("num_drafts must hold one count per sequence")
+    if out_tokens is None:
+        out_tokens = torch.empty(B, K + 1, dtype=torch.int32, device=dev)
+    else:
+        _check_out(out_tokens, (B, K + 1), dev, "out_tokens")
+    if out_len is None:
+        out_len = torch.empty(B, dtype=torch.int32, device=dev)
+    else:
+        _check_out(out_len, (B,), dev, "out_len")
+    h = _lib.lib()
+    nbytes = int(h.nsv_accept_filtered_workspace_size(B, K, V))
+    with _lib.on_device(dev):
+        stream = _lib.stream_ptr(dev)
+        scratch = _lib.stream_scratch(dev, stream)
+        with scratch.lock:
+            ws = scratch.take(nbytes)
+            rc = h.nsv_accept_filtered(
+                target_logits.data_ptr(), target_seq_stride, _lib.ptr(draft_logits), draft_seq_stride, draft_row_stride,
+                _lib.ptr(draft_mode), drafts.data_ptr(), num_drafts.data_ptr(), temperature.data_ptr(), _lib.ptr(top_k),
+                _lib.ptr(top_p), _lib.ptr(min_p), uniforms.data_ptr(), B, K, V, _lib.dtype_code(target_logits.dtype),
+                out_tokens.data_ptr(), out_len.data_ptr(), ws.data_ptr(), nbytes, stream)
+    _lib.check(rc, "accept_filtered")
+    return out_tokens, out_len
 
 
 def draw_randomness(num_drafts: list[int], V: int, dtype: torch.dtype, device, with_draft_rows: bool,
