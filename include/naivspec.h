@@ -284,6 +284,67 @@ int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights,
                  void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Pages of a paged cache copied, forked and compacted.  No reference
+ * counterpart.  One page numbering serves several pools (K and V of every
+ * layer, key weights): page i of a pool is `segments` runs of block_size keys
+ * of key_bytes each, at base + i * segments * block_size * key_bytes (K/V
+ * [num_blocks, block_size, Hkv, D]: one segment of Hkv * D elements per key;
+ * key weights [num_blocks, Hkv, block_size]: Hkv segments of 4 bytes).
+ * `pools` is a host array, read before the call returns.  key_bytes and base
+ * even; num_blocks <= 524,288; pages under 2^30 bytes.  A table entry outside
+ * [0, num_blocks) is unmapped.  held [num_blocks] bytes (nullable): a page
+ * with a nonzero byte is somebody else's and neither given out nor moved.
+ *
+ * nsv_copy_pages: page src[i] to page dst[i] (device int32), its first
+ *   keys[i] keys, or whole ones where keys is NULL; a pair with an id outside
+ *   the pools is left out.  No page may be the target of two pairs, nor a
+ *   target and a source.
+ *
+ * nsv_fork_pages: row b of the new tables goes on from row parents[b] of the
+ *   old (-1, or outside [0, B): the row ends and is empty).  Of its parent's
+ *   pages it shares those that the parent's keys fill.  The others, partly
+ *   filled or kept for later keys, stay with the parent's first child, the
+ *   lowest b; each later child gets free pages for them and a copy of the
+ *   partly filled one's keys.  Free is what no new row keeps and nobody holds;
+ *   the lowest ids go first, row by row, column by column.  Where they run
+ *   out, a row that lacks one is empty; *lacking is how many were short (0:
+ *   every row is there).  B <= 4,096.  The new tables [B, max_blocks] and
+ *   lengths [B] may not overlap the old.
+ *
+ * nsv_compact_pages: of the pages in block_tables that nobody holds, the
+ *   highest goes to the lowest free one while that lies before it.
+ *   new_ids [num_blocks]: where a page in use or held is now, -1 for others;
+ *   *top: the pages before it are all that are in use or held.
+ *   out_block_tables: the tables with the new ids (block_tables itself, or
+ *   apart from it).
+ *
+ * Workspaces: of any content; calls that share one must not run concurrently.
+ */
+typedef struct nsv_pool {
+  void* base;
+  int32_t segments;
+  int32_t key_bytes;
+} nsv_pool;
+int nsv_copy_pages(const nsv_pool* pools, int npools, int num_blocks,
+                   int block_size, const int32_t* src, const int32_t* dst,
+                   const int32_t* keys, int moves, void* stream);
+size_t nsv_fork_pages_workspace_size(int B, int max_blocks, int num_blocks);
+int nsv_fork_pages(const nsv_pool* pools, int npools, int num_blocks,
+                   int block_size, const int32_t* block_tables,
+                   const int64_t* context_lens, const int32_t* parents,
+                   const uint8_t* held, int B, int max_blocks,
+                   int32_t* out_block_tables, int64_t* out_context_lens,
+                   int32_t* lacking, void* workspace, size_t workspace_bytes,
+                   void* stream);
+size_t nsv_compact_pages_workspace_size(int num_blocks);
+int nsv_compact_pages(const nsv_pool* pools, int npools, int num_blocks,
+                      int block_size, const int32_t* block_tables,
+                      const uint8_t* held, int B, int max_blocks,
+                      int32_t* out_block_tables, int32_t* new_ids,
+                      int32_t* top, void* workspace, size_t workspace_bytes,
+                      void* stream);
+
+/*
  * Load-only measurement kernels, no reference counterpart (the ceilings
  * against which bench.py --ceiling reads the verify-attention kernels).
  * nsv_verify_attention_load_floor reads exactly the K/V bytes of a bf16,

@@ -80,6 +80,13 @@ SIGNATURES: dict[str, tuple] = {
     "nsv_accept_filtered": (
         _c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_i64] + [_c_vp] * 8 + [_c_int] * 4
         + [_c_vp, _c_vp, _c_vp, _c_size, _c_vp]),
+    "nsv_copy_pages": (_c_int, [_c_vp] + [_c_int] * 3 + [_c_vp] * 3 + [_c_int, _c_vp]),
+    "nsv_fork_pages_workspace_size": (_c_size, [_c_int] * 3),
+    "nsv_fork_pages": (
+        _c_int, [_c_vp] + [_c_int] * 3 + [_c_vp] * 4 + [_c_int] * 2 + [_c_vp] * 4 + [_c_size, _c_vp]),
+    "nsv_compact_pages_workspace_size": (_c_size, [_c_int]),
+    "nsv_compact_pages": (
+        _c_int, [_c_vp] + [_c_int] * 3 + [_c_vp] * 2 + [_c_int] * 2 + [_c_vp] * 4 + [_c_size, _c_vp]),
     "nsv_prepare_draft": (
         _c_int, [_c_vp, _c_i64, _c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_int, _c_int] + [_c_vp] * 7),
     "nsv_ngram_draft": (_c_int, [_c_vp, _c_vp, _c_i64] + [_c_int] * 4 + [_c_vp, _c_vp, _c_vp]),
