@@ -14,13 +14,20 @@
 // read.  T <= 1e-6, and rows with a NaN or without a value above -inf, leave
 // the argmax alone (first maximum, NaN above all, torch's rule).
 //
-// filter_rows_kernel works one row out per workgroup.  A value is found by
-// radix descent over its order-preserving bits: per level a histogram in LDS
-// of the row's tokens below the prefix so far, counts and weights, and a scan
-// of its bins.  Weights are added up as 64-bit integers, w 2^s rounded, so
-// sums do not depend on the order of the additions; s leaves room for the
-// vocabulary (44 bits for 2^18 tokens), each weight off by 2^-45 of the
-// largest, where fp32 sums would move the sample of one row in a hundred.
+// filter_rows_kernel works one row out per workgroup.
+//   bf16 (count_row): a row has few distinct values, so one pass counts the
+//     tokens of each of the 65,536 in LDS (16 bits each), and everything else
+//     comes from the counts: a value's tokens weigh count * w, one exponential
+//     per value that occurs (some 3,000) instead of one per token.  The row
+//     stays in registers, where the sampled token is found by its value and
+//     its rank among the tokens of that value.
+//   fp32 (filter_row): a value is found by radix descent over its
+//     order-preserving bits: per level a histogram in LDS of the row's tokens
+//     below the prefix so far, counts and weights, and a scan of its bins.
+//     Weights are added up as 64-bit integers, w 2^s rounded, so sums do not
+//     depend on the order of the additions; s leaves room for the vocabulary
+//     (44 bits for 2^18 tokens), each weight off by 2^-45 of the largest, where
+//     fp32 sums would move the sample of one row in a hundred.
 
 #include "common.h"
 #include "exp_f64.h"
@@ -195,7 +202,7 @@ struct Spot {
   uint64_t mass;           // weights before
   uint64_t weight;
 };
-enum Seek { kByCount, kReach, kBeyond };
+enum Seek { kByCount, kReach, kAbove, kBeyond };
 
 // The last value with: tokens before it < goal (kByCount); weights before it
 // < goal (kReach) or <= goal (kBeyond), and a weight of its own.
@@ -400,6 +407,490 @@ __device__ RowCut filter_row(const FilterArgs& a, int b, const T* row, bool samp
   return out;
 }
 
+
+// ---------------------------------------------------------------------------
+// bf16 rows by counts
+// ---------------------------------------------------------------------------
+constexpr int kHold = 19;      // 16-byte vectors a thread keeps (76 of its 128 registers): rows up to 155,648
+constexpr int kGroups = 512;   // of 128 values each, along the order of the tokens: 64 words of two counts
+constexpr int kSafeSteps = 7;  // steps whose 57,344 tokens fit a 16-bit count beside ..
+constexpr uint32_t kFull = 65536 - kSafeSteps * kStep;  // .. fewer than these
+constexpr int kMaxHeavy = kRowWaves + kMaxVocab / kFull + 1;
+
+struct CountLds {
+  uint32_t bin[32768];         // counts of values 2i (low half) and 2i + 1
+  double mass[kGroups];        // weights of a group, first of its first value's
+  double before[kGroups];      // weights before a group
+  uint32_t count[kGroups];
+  uint32_t cbefore[kGroups];
+  uint32_t ref[kGroups];       // bits of a group's first value that occurs
+  uint32_t found[kMaxSteps * kRowWaves];
+  double tab[256];
+  uint32_t heavy[kMaxHeavy], heavy_count[kMaxHeavy];  // counts beside the bins
+  int heavies;
+  uint32_t slots;              // tokens counted
+  int nan, index;
+  // what wave 0 decides
+  float top, cut;
+  int kept, rank, cut_rank;    // rank -1: no token is looked up; cut_rank -1: no index is
+  uint32_t value, cut_value;   // bits
+  double total;
+};
+
+// Vector g of a row: its elements 8 g - skew .. + 7, `skew` the elements from a
+// 16-byte boundary to its start.
+__device__ __forceinline__ bool whole_vec(int skew, int V, int g) {
+  const int64_t e0 = (int64_t)8 * g - skew;
+  return e0 >= 0 && e0 + 8 <= V;
+}
+__device__ __forceinline__ u32x4 load_whole(const uint16_t* row, int skew, int g) {
+  return load16_stream(row + ((int64_t)8 * g - skew));
+}
+// one of the row's ends: -inf where the row has no element
+__device__ __forceinline__ u32x4 load_edge(const uint16_t* row, int skew, int V, int g) {
+  const int64_t e0 = (int64_t)8 * g - skew;
+  u32x4 v;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t a = e0 + 2 * i, b = a + 1;
+    const uint32_t lo = a >= 0 && a < V ? row[a] : 0xff80u, hi = b >= 0 && b < V ? row[b] : 0xff80u;
+    v[i] = lo | (hi << 16);
+  }
+  return v;
+}
+__device__ __forceinline__ u32x4 load_bits(const uint16_t* row, int skew, int V, int g) {
+  return whole_vec(skew, V, g) ? load_whole(row, skew, g) : load_edge(row, skew, V, g);
+}
+
+__device__ __forceinline__ void count_value(uint32_t* bin, uint32_t bits) {
+  atomicAdd(&bin[bits >> 1], 1u << ((bits & 1) << 4));
+}
+
+// The tokens of a vector counted.  A value that many of a wave's lanes hold
+// (a mask's) would be 64 additions to one address one after another: the
+// wave's first such value is added up beside the bins.
+__device__ __forceinline__ void count_vec(uint32_t* bin, const u32x4& v, uint32_t& heavy, uint32_t& many) {
+  const uint32_t some = (uint32_t)__builtin_amdgcn_readfirstlane((int)(v[0] & 0xffffu));
+  if (__popcll(__ballot((v[0] & 0xffffu) == some)) >= 16 && (heavy == some || heavy == ~0u)) {  // uniform
+    heavy = some;
+    u32x4 w = v;
+#pragma unroll 1
+    for (int i = 0; i < 4; ++i) {  // (rarely run: small)
+      const uint32_t lo = w[0] & 0xffffu, hi = w[0] >> 16;
+      many += __popcll(__ballot(lo == some)) + __popcll(__ballot(hi == some));
+      if (lo != some) count_value(bin, lo);
+      if (hi != some) count_value(bin, hi);
+      w = u32x4{w[1], w[2], w[3], w[0]};
+    }
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) count_value(bin, (e & 1) ? v[e >> 1] >> 16 : v[e >> 1] & 0xffffu);
+}
+
+// Counts that another kSafeSteps might carry over 16 bits, beside the bins.
+__device__ __forceinline__ void flush_full(CountLds& s) {
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < 32768; i += kRowThreads) {
+    uint32_t w = s.bin[i];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t c = (w >> (16 * half)) & 0xffffu;
+      if (c < kFull) continue;
+      const int at = atomicAdd(&s.heavies, 1);
+      s.heavy[at] = 2 * i + half;
+      s.heavy_count[at] = c;
+      w -= c << (16 * half);
+    }
+    s.bin[i] = w;
+  }
+  __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t heavy_of(const CountLds& s, uint32_t value) {
+  uint32_t c = 0;
+  for (int i = 0; i < s.heavies; ++i)
+    if (s.heavy[i] == value) c += s.heavy_count[i];
+  return c;
+}
+
+// The two values of a lane in a group, in order, and their counts; -0 counts as +0.
+struct Pair {
+  uint32_t v1, v2, c1, c2;
+};
+__device__ __forceinline__ Pair pair_of(const CountLds& s, int g) {
+  const int lane = threadIdx.x & 63;
+  const bool neg = g >= kGroups / 2;
+  const uint32_t w = neg ? 64 * g + lane : 64 * (kGroups / 2 - 1 - g) + 63 - lane;
+  const uint32_t both = s.bin[w], lo = both & 0xffffu, hi = both >> 16;
+  Pair p{2 * w + !neg, 2 * w + neg, neg ? lo : hi, neg ? hi : lo};
+  if (s.heavies) {  // uniform
+    p.c1 += heavy_of(s, p.v1);
+    p.c2 += heavy_of(s, p.v2);
+  }
+  if (g == kGroups / 2 && lane == 0) p.c1 = 0;
+  if (w == 0) p.c2 += (s.bin[0x4000] & 0xffffu) + heavy_of(s, 0x8000u);
+  return p;
+}
+
+struct Place {
+  uint32_t value;          // bits
+  uint32_t before, count;  // tokens
+  double mass, weight;     // weights before; of one token
+};
+
+// As seek, from the counts, by one wave.  kAbove: the last value of weight >= goal.
+__device__ __forceinline__ Place seek_counts(int kind, double goal, const CountLds& s, float top, double inv_t) {
+  const int lane = threadIdx.x & 63;
+  int g = -1;
+#pragma unroll 1
+  for (int i = kGroups / 64 - 1; i >= 0 && g < 0; --i) {
+    const int mine = 64 * i + lane;
+    const uint32_t c = s.count[mine];
+    bool fits = c > 0;
+    if (kind == kByCount) fits = fits && (double)s.cbefore[mine] < goal;
+    else if (kind == kAbove) fits = fits && weight_of(bf16_bits_to_f32(s.ref[mine]), top, inv_t, s.tab) >= goal;
+    else fits = fits && s.mass[mine] > 0.0 && (kind == kReach ? s.before[mine] < goal : s.before[mine] <= goal);
+    const uint64_t yes = __ballot(fits);
+    if (yes) g = 64 * i + 63 - __clzll((long long)yes);
+  }
+  g = max(g, 0);
+  const Pair p = pair_of(s, g);
+  const double w1 = p.c1 ? weight_of(bf16_bits_to_f32(p.v1), top, inv_t, s.tab) : 0.0;
+  const double w2 = p.c2 ? weight_of(bf16_bits_to_f32(p.v2), top, inv_t, s.tab) : 0.0;
+  const double m1 = p.c1 * w1, m = m1 + p.c2 * w2;
+  double before = __shfl_up(wave_scan(m), 1);
+  if (lane == 0) before = 0.0;
+  before += s.before[g];
+  const uint32_t cbefore = s.cbefore[g] + wave_scan(p.c1 + p.c2) - p.c1 - p.c2;
+  auto fits = [&](uint32_t c, double w, uint32_t cb, double mb) {
+    if (kind == kByCount) return c && (double)cb < goal;
+    if (kind == kAbove) return c && w >= goal;
+    return c && w > 0.0 && (kind == kReach ? mb < goal : mb <= goal);
+  };
+  const uint64_t y1 = __ballot(fits(p.c1, w1, cbefore, before)), y2 = __ballot(fits(p.c2, w2, cbefore + p.c1, before + m1));
+  const int l1 = y1 ? 63 - __clzll((long long)y1) : -1, l2 = y2 ? 63 - __clzll((long long)y2) : -1;
+  const bool second = l2 >= l1;
+  const int l = max(max(l1, l2), 0);
+  Place at;
+  at.value = (uint32_t)__shfl((int)(second ? p.v2 : p.v1), l);
+  at.count = (uint32_t)__shfl((int)(second ? p.c2 : p.c1), l);
+  at.before = (uint32_t)__shfl((int)(second ? cbefore + p.c1 : cbefore), l);
+  at.mass = __shfl(second ? before + m1 : before, l);
+  at.weight = __shfl(second ? w2 : w1, l);
+  return at;
+}
+
+// how many of a vector's tokens have the value (`both`: twice its bits, under `mask`)
+__device__ __forceinline__ uint32_t matches(const u32x4& v, uint32_t both, uint32_t mask) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 n = {0, 0};  // others
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    n += __builtin_elementwise_min(__builtin_bit_cast(u16x2, (v[i] & mask) ^ both), (u16x2){1, 1});
+  return 8u - n[0] - n[1];
+}
+
+// s.index = the index of the token of bits `value` with `rank` of them before it
+__device__ __forceinline__ void find_token(const u32x4 (&held)[kHold], const uint16_t* row, int skew, int V, int vecs, int steps,
+                                           uint32_t value, uint32_t rank, CountLds& s) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t mask = value ? ~0u : 0x7fff7fffu, both = value | (value << 16);  // (+0: -0 too)
+  auto note = [&](int it, uint32_t n) {
+    uint32_t all = 0;
+    if (__ballot(n > 0)) {
+#pragma unroll
+      for (int b = 0; b < 4; ++b) all += __popcll(__ballot((n >> b) & 1)) << b;
+    }
+    if (lane == 0) s.found[it * kRowWaves + wave] = all;
+  };
+  int mine_end = (vecs - tid + kRowThreads - 1) / kRowThreads;
+  asm volatile("" : "+v"(mine_end));  // (compared anew: the conditions of the loads would be kept in, and spilled from, 38 SGPRs)
+#pragma unroll
+  for (int it = 0; it < kHold; ++it)
+    if (it < steps) note(it, it < mine_end ? matches(held[it], both, mask) : 0u);
+#pragma unroll 1
+  for (int it = kHold; it < steps; ++it) {
+    const int g = it * kRowThreads + tid;
+    uint32_t n = 0;
+    if (g < vecs) n = matches(load_bits(row, skew, V, g), both, mask);
+    note(it, n);
+  }
+  __syncthreads();
+  // the (step, wave) that holds it: every wave looks, one goes on
+  const int entries = steps * kRowWaves, per = (entries + 63) / 64;
+  uint32_t mine = 0;
+#pragma unroll 1
+  for (int i = 0; i < per; ++i)
+    if (lane * per + i < entries) mine += s.found[lane * per + i];
+  const uint32_t upto = wave_scan(mine);
+  const uint64_t yes = __ballot(upto > rank);
+  const int l = yes ? __ffsll((long long)yes) - 1 : 63;
+  uint32_t left = rank - (uint32_t)__shfl((int)(upto - mine), l);
+  int at = l * per;
+  while (at < min(entries, (l + 1) * per) - 1 && left >= s.found[at]) left -= s.found[at++];
+  at = __builtin_amdgcn_readfirstlane(min(at, entries - 1));
+  if (wave == at % kRowWaves) {  // uniform
+    const int it = at / kRowWaves, g = it * kRowThreads + tid;
+    u32x4 v{};
+    if (it < kHold) {
+#pragma unroll
+      for (int i = 0; i < kHold; ++i)
+        if (i == it) v = held[i];
+    } else if (g < vecs) {
+      v = load_bits(row, skew, V, g);
+    }
+    const uint32_t n = g < vecs ? matches(v, both, mask) : 0u;
+    const uint32_t before = wave_scan(n) - n;
+    if (n && left >= before && left < before + n) {
+      uint32_t k = before;
+      int e = 0;
+      for (; e < 7; ++e) {
+        const bool hit = ((v[0] ^ both) & mask & 0xffffu) == 0;
+        if (hit && k == left) break;
+        k += hit;
+        if (e & 1) v = u32x4{v[1], v[2], v[3], v[0]};
+        else v[0] >>= 16;
+      }
+      s.index = 8 * g - skew + e;
+    }
+  }
+  __syncthreads();
+}
+
+// filter_row for bf16.
+__device__ __forceinline__ RowCut count_row(const FilterArgs& a, int b, const uint16_t* row, bool sampled, float u, bool ends,
+                                            CountLds& s) {
+  const int V = a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int skew = (int)(((uintptr_t)row & 15) >> 1);
+  const int vecs = (V + skew + 7) / 8, steps = (vecs + kRowThreads - 1) / kRowThreads;
+  u32x4 held[kHold];
+#pragma unroll
+  for (int it = 0; it < kHold; ++it) {
+    const int g = it * kRowThreads + tid;
+    held[it] = u32x4{0u, 0u, 0u, 0u};
+    if (g < vecs && whole_vec(skew, V, g)) held[it] = load_whole(row, skew, g);
+  }
+  const float T = a.temperature[b];
+  const int k = a.top_k ? a.top_k[b] : 0;
+  const float p = a.top_p ? a.top_p[b] : 1.f, least = a.min_p ? a.min_p[b] : 0.f;
+  for (int i = tid; i < 32768 / 4; i += kRowThreads) reinterpret_cast<u32x4*>(s.bin)[i] = u32x4{0u, 0u, 0u, 0u};
+  if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
+  if (tid == 0) {
+    s.nan = s.heavies = 0;
+    s.slots = 0;
+  }
+  // the row's first and last vector, where they are no whole ones
+#pragma unroll 1
+  for (int e = 0; e < 2; ++e) {
+    const int g = e ? vecs - 1 : 0;
+    if (g >= kHold * kRowThreads || tid != g % kRowThreads || whole_vec(skew, V, g)) continue;
+    const u32x4 v = load_edge(row, skew, V, g);
+#pragma unroll
+    for (int it = 0; it < kHold; ++it)
+      if (it == g / kRowThreads) held[it] = v;
+  }
+  lds_barrier();  // (the row's loads stay in flight)
+  const bool greedy = is_greedy(T);
+  const double inv_t = greedy ? 1.0 : 1.0 / (double)T;
+  uint32_t heavy = ~0u, many = 0;
+  int mine = (vecs - tid + kRowThreads - 1) / kRowThreads;
+  asm volatile("" : "+v"(mine));
+#pragma unroll
+  for (int it = 0; it < kHold; ++it)
+    if (it < mine) count_vec(s.bin, held[it], heavy, many);
+#pragma unroll 1
+  for (int it = kHold; it < steps; ++it) {
+    const int g = it * kRowThreads + tid;
+    if (g < vecs) count_vec(s.bin, load_bits(row, skew, V, g), heavy, many);
+  }
+  // A bin runs over only where one value has more than 65,535 tokens: the
+  // counts then miss some, and are taken again with the full ones put aside
+  // in between.
+#pragma unroll 1
+  for (int careful = 0; careful < 2; ++careful) {
+    if (careful) {
+      heavy = ~0u;
+      many = 0;
+#pragma unroll 1
+      for (int it = 0; it < steps; ++it) {
+        const int g = it * kRowThreads + tid;
+        if (g < vecs) count_vec(s.bin, load_bits(row, skew, V, g), heavy, many);
+        if (it % kSafeSteps == kSafeSteps - 1) flush_full(s);
+      }
+    }
+    // (a wave's lanes count alike, but those without a last vector)
+    heavy = (uint32_t)__builtin_amdgcn_readfirstlane((int)heavy);
+    many = (uint32_t)__builtin_amdgcn_readfirstlane((int)many);
+    if (lane == 0 && many) {
+      const int at = atomicAdd(&s.heavies, 1);
+      s.heavy[at] = heavy;
+      s.heavy_count[at] = many;
+    }
+    __syncthreads();
+    // groups, taken by the waves in turn: values that occur lie in few of them, next to each other
+    uint32_t slots = 0;
+#pragma unroll 1
+    for (int g = wave; g < kGroups; g += kRowWaves) {
+      const Pair q = pair_of(s, g);
+      const uint32_t c = q.c1 + q.c2;
+      if (!__ballot(c > 0)) {  // uniform
+        if (lane == 0) s.count[g] = 0;
+        continue;
+      }
+      if ((q.c1 && (q.v1 & 0x7fffu) > 0x7f80u) || (q.c2 && (q.v2 & 0x7fffu) > 0x7f80u)) s.nan = 1;
+      const uint64_t y1 = __ballot(q.c1 > 0), y2 = __ballot(q.c2 > 0);
+      const int l1 = y1 ? __ffsll((long long)y1) - 1 : 64, l2 = y2 ? __ffsll((long long)y2) - 1 : 64;
+      const uint32_t ref = (uint32_t)__shfl((int)(l1 <= l2 ? q.v1 : q.v2), min(l1, l2));
+      const float rv = bf16_bits_to_f32(ref);
+      double m = 0.0;
+      if (q.c1) m = q.c1 * weight_of(bf16_bits_to_f32(q.v1), rv, inv_t, s.tab);
+      if (q.c2) m += q.c2 * weight_of(bf16_bits_to_f32(q.v2), rv, inv_t, s.tab);
+      m = wave_sum_dpp(m);
+      const uint32_t all = (uint32_t)__shfl((int)wave_scan(c), 63);
+      slots += all;
+      if (lane == 0) {
+        s.count[g] = all;
+        s.mass[g] = m;
+        s.ref[g] = ref;
+      }
+    }
+    if (lane == 0) atomicAdd(&s.slots, slots);
+    __syncthreads();
+    if (s.slots == 8u * (uint32_t)vecs) break;  // uniform
+    __syncthreads();
+    for (int i = tid; i < 32768 / 4; i += kRowThreads) reinterpret_cast<u32x4*>(s.bin)[i] = u32x4{0u, 0u, 0u, 0u};
+    if (tid == 0) {
+      s.heavies = 0;
+      s.slots = 0;
+    }
+    __syncthreads();
+  }
+  RowCut out;
+  out.last = V - 1;
+  out.token = 0;
+  out.pad = 0;
+  if (s.nan) {  // uniform: the first NaN
+    if (tid == 0) s.index = V;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < V; i += kRowThreads)
+      if ((row[i] & 0x7fffu) > 0x7f80u) atomicMin(&s.index, i);
+    __syncthreads();
+    out.top = out.cut = __builtin_nanf("");
+    out.kept = 1;
+    out.token = out.last = s.index;
+    out.total = 1.0;
+    return out;
+  }
+  if (wave == 0) {
+    // the maximum: the first group's first value
+    int g0 = 0;
+#pragma unroll 1
+    for (int i = kGroups / 64 - 1; i >= 0; --i) {
+      const uint64_t yes = __ballot(s.count[64 * i + lane] > 0);
+      if (yes) g0 = 64 * i + __ffsll((long long)yes) - 1;
+    }
+    const uint32_t top_bits = s.ref[g0];
+    const float top = bf16_bits_to_f32(top_bits);
+    uint32_t cut = top_bits, value = top_bits;
+    int kept = 1, rank = 0, cut_rank = -1;
+    double total = 1.0;
+    if (!greedy && top != -__builtin_inff()) {  // uniform
+      // weights and tokens before each group
+      double f = 0.0;
+      uint32_t n = 0;
+#pragma unroll 1
+      for (int g = 8 * lane; g < 8 * lane + 8; ++g) {
+        const uint32_t c = s.count[g];
+        const double m = c ? s.mass[g] * weight_of(bf16_bits_to_f32(s.ref[g]), top, inv_t, s.tab) : 0.0;
+        s.mass[g] = m;
+        s.before[g] = f;
+        s.cbefore[g] = n;
+        f += m;
+        n += c;
+      }
+      const double upto = wave_scan(f);
+      double fb = __shfl_up(upto, 1);
+      if (lane == 0) fb = 0.0;
+      const uint32_t nb = wave_scan(n) - n;
+#pragma unroll 1
+      for (int g = 8 * lane; g < 8 * lane + 8; ++g) {
+        s.before[g] += fb;
+        s.cbefore[g] += nb;
+      }
+      total = __shfl(upto, 63);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
+      kept = V;
+      cut = 0xff80u;
+#pragma unroll 1
+      for (int kind = 0; kind < 4; ++kind) {
+        double goal = 0.0;
+        if (kind == kByCount) {
+          if (k <= 0 || k >= V) continue;
+          goal = (double)k;
+        } else if (kind == kReach) {
+          if (!(p < 1.f)) continue;
+          goal = fmax((double)p * total, 0x1p-1000);  // (the first token stays)
+        } else if (kind == kAbove) {
+          if (!(least > 0.f)) continue;
+          goal = fmin((double)least, 1.0);
+        } else {
+          if (!sampled || kept == 1) continue;
+          goal = unit(u) * total;
+        }
+        const Place at = seek_counts(kind, goal, s, top, inv_t);
+        if (kind == kBeyond) {
+          const double j = fmin(floor((goal - at.mass) / at.weight), (double)min((int)at.count, kept - (int)at.before) - 1.0);
+          value = at.value;
+          rank = (int)fmax(j, 0.0);
+          continue;
+        }
+        uint32_t stay = at.count;  // tokens of the value that do
+        if (kind == kByCount) stay = (uint32_t)k - at.before;
+        if (kind == kReach) stay = (uint32_t)fmin(fmax(ceil((goal - at.mass) / at.weight), 1.0), (double)at.count);
+        if ((int)(at.before + stay) >= kept) continue;
+        kept = (int)(at.before + stay);
+        cut = at.value;
+        cut_rank = stay < at.count ? (int)stay - 1 : -1;
+        total = at.mass + stay * at.weight;
+      }
+      if (!sampled && kept > 1) rank = -1;
+      // (a cut among tokens of weight 0 cuts nothing; a lone token is looked up as the sample)
+      if (!ends || kept == 1 || cut == 0xff80u) cut_rank = -1;
+    }
+    if (lane == 0) {
+      s.top = top;
+      s.cut = bf16_bits_to_f32(cut);
+      s.cut_value = cut;
+      s.kept = kept;
+      s.total = total;
+      s.value = value;
+      s.rank = rank;
+      s.cut_rank = cut_rank;
+    }
+  }
+  __syncthreads();
+  out.top = s.top;
+  out.cut = s.cut;
+  out.kept = s.kept;
+  out.total = s.total;
+  const int rank = s.rank, cut_rank = s.cut_rank;
+  const bool empty = s.top == -__builtin_inff();  // nothing above it: the first token
+  const uint32_t value = s.value, cut_value = s.cut_value;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int r = which ? cut_rank : rank;
+    if (r < 0 || empty) continue;  // uniform
+    find_token(held, row, skew, V, vecs, steps, which ? cut_value : value, (uint32_t)r, s);
+    if (which) out.last = s.index;
+    else out.token = s.index;
+  }
+  if (out.kept == 1) out.last = out.token;
+  return out;
+}
+
 // probability of token i of logit x
 __device__ __forceinline__ double prob_of(const RowCut& c, float x, int i, double inv_t, const double* tab) {
   if (c.kept == 1) return i == c.token ? 1.0 : 0.0;
@@ -407,13 +898,30 @@ __device__ __forceinline__ double prob_of(const RowCut& c, float x, int i, doubl
   return in ? weight_of(x, c.top, inv_t, tab) / c.total : 0.0;
 }
 
+template <typename T> union RowScratch;
+template <> union RowScratch<float> {
+  RowLds radix;
+};
+template <> union RowScratch<uint16_t> {
+  CountLds counts;
+};
+
+__device__ __forceinline__ RowCut work_out(const FilterArgs& a, int b, const float* row, bool sampled, float u, bool ends,
+                                           RowScratch<float>& s) {
+  return filter_row<float>(a, b, row, sampled, u, ends, s.radix);
+}
+__device__ __forceinline__ RowCut work_out(const FilterArgs& a, int b, const uint16_t* row, bool sampled, float u, bool ends,
+                                           RowScratch<uint16_t>& s) {
+  return count_row(a, b, row, sampled, u, ends, s.counts);
+}
+
 // grid (rows per sequence, B): target rows, then draft rows
 template <typename T>
 __global__ __launch_bounds__(kRowThreads) void filter_rows_kernel(FilterArgs a) {
-  __shared__ RowLds s;
+  __shared__ RowScratch<T> s;
   const int b = blockIdx.y, r = blockIdx.x;
   if (a.K < 0) {
-    const RowCut c = filter_row<T>(a, b, (const T*)a.target + (int64_t)b * a.t_seq, true, a.uniforms[b], false, s);
+    const RowCut c = work_out(a, b, (const T*)a.target + (int64_t)b * a.t_seq, true, a.uniforms[b], false, s);
     if (threadIdx.x == 0) {
       a.tokens[(int64_t)b * a.out_stride] = c.token;
       if (a.kept) a.kept[b] = c.kept;
@@ -428,7 +936,7 @@ __global__ __launch_bounds__(kRowThreads) void filter_rows_kernel(FilterArgs a) 
                           : (const T*)a.target + (int64_t)b * a.t_seq + (int64_t)i * a.t_row;
   const bool sampled = !rows || i == kb;
   const float u = a.uniforms[(int64_t)b * (a.K + 1) + (rows ? a.K : i)];
-  const RowCut c = filter_row<T>(a, b, row, sampled, u, !sampled, s);
+  const RowCut c = work_out(a, b, row, sampled, u, !sampled, s);
   if (threadIdx.x != 0) return;
   const int64_t at = (int64_t)b * (2 * a.K + 1) + r;
   a.cuts[at] = c;
