@@ -152,15 +152,38 @@ __device__ __forceinline__ void each(const T* row, int V, F f) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {  // inclusive
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const T o = __shfl_up(v, d);
-    if (lane >= d) v += o;
+// Inclusive scan over a wave's 64 lanes on the VALU: within rows of 16 by
+// shifts of 1, 2, 4 and 8 lanes, then the last lane of row 0 and 2 to the row
+// behind it, and of row 1 to rows 2 and 3 (what has no source adds 0).  A
+// sixth of the shuffles' time, whose every step is a round trip through LDS.
+template <int CTRL, int ROWS, typename T>
+__device__ __forceinline__ T dpp_or_zero(T v) {
+  if constexpr (sizeof(T) == 4) {
+    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
+  } else {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(T, ((uint64_t)hi << 32) | lo);
   }
+}
+template <typename T>
+__device__ __forceinline__ T wave_scan(T v) {
+  v += dpp_or_zero<0x111, 0xf>(v);
+  v += dpp_or_zero<0x112, 0xf>(v);
+  v += dpp_or_zero<0x114, 0xf>(v);
+  v += dpp_or_zero<0x118, 0xf>(v);
+  v += dpp_or_zero<0x142, 0xa>(v);
+  v += dpp_or_zero<0x143, 0xc>(v);
   return v;
+}
+// lane l's value (l uniform), and the lane's before a lane's own
+__device__ __forceinline__ double lane_f64(double v, int l) {
+  return __longlong_as_double((long long)lane_u64((uint64_t)__double_as_longlong(v), l));
+}
+template <typename T>
+__device__ __forceinline__ T lane_before(T v) {
+  return dpp_or_zero<0x138, 0xf>(v);  // the whole wave one lane up, 0 into the first
 }
 
 struct RowLds {
@@ -419,11 +442,13 @@ constexpr int kMaxHeavy = kRowWaves + kMaxVocab / kFull + 1;
 
 struct CountLds {
   uint32_t bin[32768];         // counts of values 2i (low half) and 2i + 1
+  uint32_t occurs[kGroups / 32];
+  // groups that occur, along the order
   double mass[kGroups];        // weights of a group, first of its first value's
   double before[kGroups];      // weights before a group
   uint32_t count[kGroups];
   uint32_t cbefore[kGroups];
-  uint32_t ref[kGroups];       // bits of a group's first value that occurs
+  uint32_t ref[kGroups];       // group << 16 | bits of its first value that occurs
   uint32_t found[kMaxSteps * kRowWaves];
   double tab[256];
   uint32_t heavy[kMaxHeavy], heavy_count[kMaxHeavy];  // counts beside the bins
@@ -508,29 +533,33 @@ __device__ __forceinline__ void flush_full(CountLds& s) {
   __syncthreads();
 }
 
-__device__ __forceinline__ uint32_t heavy_of(const CountLds& s, uint32_t value) {
+__device__ __forceinline__ uint32_t heavy_of(const CountLds& s, int heavies, uint32_t value) {
   uint32_t c = 0;
-  for (int i = 0; i < s.heavies; ++i)
+  for (int i = 0; i < heavies; ++i)
     if (s.heavy[i] == value) c += s.heavy_count[i];
   return c;
+}
+
+// a lane's word of a group
+__device__ __forceinline__ uint32_t word_of(int g) {
+  const int lane = threadIdx.x & 63;
+  return g >= kGroups / 2 ? 64 * g + lane : 64 * (kGroups / 2 - 1 - g) + 63 - lane;
 }
 
 // The two values of a lane in a group, in order, and their counts; -0 counts as +0.
 struct Pair {
   uint32_t v1, v2, c1, c2;
 };
-__device__ __forceinline__ Pair pair_of(const CountLds& s, int g) {
-  const int lane = threadIdx.x & 63;
+__device__ __forceinline__ Pair pair_of(const CountLds& s, int heavies, int g) {
   const bool neg = g >= kGroups / 2;
-  const uint32_t w = neg ? 64 * g + lane : 64 * (kGroups / 2 - 1 - g) + 63 - lane;
-  const uint32_t both = s.bin[w], lo = both & 0xffffu, hi = both >> 16;
+  const uint32_t w = word_of(g), both = s.bin[w], lo = both & 0xffffu, hi = both >> 16;
   Pair p{2 * w + !neg, 2 * w + neg, neg ? lo : hi, neg ? hi : lo};
-  if (s.heavies) {  // uniform
-    p.c1 += heavy_of(s, p.v1);
-    p.c2 += heavy_of(s, p.v2);
+  if (heavies) {  // uniform
+    p.c1 += heavy_of(s, heavies, p.v1);
+    p.c2 += heavy_of(s, heavies, p.v2);
   }
-  if (g == kGroups / 2 && lane == 0) p.c1 = 0;
-  if (w == 0) p.c2 += (s.bin[0x4000] & 0xffffu) + heavy_of(s, 0x8000u);
+  if (w == 0x4000u) p.c1 = 0;
+  if (w == 0) p.c2 += (s.bin[0x4000] & 0xffffu) + heavy_of(s, heavies, 0x8000u);
   return p;
 }
 
@@ -540,30 +569,29 @@ struct Place {
   double mass, weight;     // weights before; of one token
 };
 
-// As seek, from the counts, by one wave.  kAbove: the last value of weight >= goal.
-__device__ __forceinline__ Place seek_counts(int kind, double goal, const CountLds& s, float top, double inv_t) {
+// As seek, from the counts of `groups` groups, by one wave.  kAbove: the last
+// value of weight >= goal.
+__device__ __forceinline__ Place seek_counts(int kind, double goal, const CountLds& s, int groups, int heavies, float top,
+                                             double inv_t) {
   const int lane = threadIdx.x & 63;
-  int g = -1;
+  int at_group = -1;
 #pragma unroll 1
-  for (int i = kGroups / 64 - 1; i >= 0 && g < 0; --i) {
-    const int mine = 64 * i + lane;
-    const uint32_t c = s.count[mine];
-    bool fits = c > 0;
-    if (kind == kByCount) fits = fits && (double)s.cbefore[mine] < goal;
-    else if (kind == kAbove) fits = fits && weight_of(bf16_bits_to_f32(s.ref[mine]), top, inv_t, s.tab) >= goal;
-    else fits = fits && s.mass[mine] > 0.0 && (kind == kReach ? s.before[mine] < goal : s.before[mine] <= goal);
-    const uint64_t yes = __ballot(fits);
-    if (yes) g = 64 * i + 63 - __clzll((long long)yes);
+  for (int i = (groups - 1) >> 6; i >= 0 && at_group < 0; --i) {
+    const int mine = min(64 * i + lane, groups - 1);
+    bool fits;
+    if (kind == kByCount) fits = (double)s.cbefore[mine] < goal;
+    else if (kind == kAbove) fits = weight_of(bf16_bits_to_f32(s.ref[mine] & 0xffffu), top, inv_t, s.tab) >= goal;
+    else fits = s.mass[mine] > 0.0 && (kind == kReach ? s.before[mine] < goal : s.before[mine] <= goal);
+    const uint64_t yes = __ballot(fits && s.count[mine] > 0 && 64 * i + lane < groups);  // (a group of -0 alone is empty)
+    if (yes) at_group = 64 * i + 63 - __clzll((long long)yes);
   }
-  g = max(g, 0);
-  const Pair p = pair_of(s, g);
+  at_group = max(at_group, 0);
+  const Pair p = pair_of(s, heavies, (int)(s.ref[at_group] >> 16));
   const double w1 = p.c1 ? weight_of(bf16_bits_to_f32(p.v1), top, inv_t, s.tab) : 0.0;
   const double w2 = p.c2 ? weight_of(bf16_bits_to_f32(p.v2), top, inv_t, s.tab) : 0.0;
   const double m1 = p.c1 * w1, m = m1 + p.c2 * w2;
-  double before = __shfl_up(wave_scan(m), 1);
-  if (lane == 0) before = 0.0;
-  before += s.before[g];
-  const uint32_t cbefore = s.cbefore[g] + wave_scan(p.c1 + p.c2) - p.c1 - p.c2;
+  const double before = lane_before(wave_scan(m)) + s.before[at_group];
+  const uint32_t cbefore = s.cbefore[at_group] + wave_scan(p.c1 + p.c2) - p.c1 - p.c2;
   auto fits = [&](uint32_t c, double w, uint32_t cb, double mb) {
     if (kind == kByCount) return c && (double)cb < goal;
     if (kind == kAbove) return c && w >= goal;
@@ -574,11 +602,11 @@ __device__ __forceinline__ Place seek_counts(int kind, double goal, const CountL
   const bool second = l2 >= l1;
   const int l = max(max(l1, l2), 0);
   Place at;
-  at.value = (uint32_t)__shfl((int)(second ? p.v2 : p.v1), l);
-  at.count = (uint32_t)__shfl((int)(second ? p.c2 : p.c1), l);
-  at.before = (uint32_t)__shfl((int)(second ? cbefore + p.c1 : cbefore), l);
-  at.mass = __shfl(second ? before + m1 : before, l);
-  at.weight = __shfl(second ? w2 : w1, l);
+  at.value = lane_u32(second ? p.v2 : p.v1, l);
+  at.count = lane_u32(second ? p.c2 : p.c1, l);
+  at.before = lane_u32(second ? cbefore + p.c1 : cbefore, l);
+  at.mass = lane_f64(second ? before + m1 : before, l);
+  at.weight = lane_f64(second ? w2 : w1, l);
   return at;
 }
 
@@ -592,14 +620,25 @@ __device__ __forceinline__ uint32_t matches(const u32x4& v, uint32_t both, uint3
   return 8u - n[0] - n[1];
 }
 
+// whether a vector has a token of the value
+__device__ __forceinline__ bool has_value(const u32x4& v, uint32_t both, uint32_t mask) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 d[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) d[i] = __builtin_bit_cast(u16x2, (v[i] & mask) ^ both);
+  const u16x2 m = __builtin_elementwise_min(__builtin_elementwise_min(d[0], d[1]), __builtin_elementwise_min(d[2], d[3]));
+  return m[0] == 0 || m[1] == 0;
+}
+
 // s.index = the index of the token of bits `value` with `rank` of them before it
 __device__ __forceinline__ void find_token(const u32x4 (&held)[kHold], const uint16_t* row, int skew, int V, int vecs, int steps,
                                            uint32_t value, uint32_t rank, CountLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t mask = value ? ~0u : 0x7fff7fffu, both = value | (value << 16);  // (+0: -0 too)
-  auto note = [&](int it, uint32_t n) {
+  auto note = [&](int it, const u32x4& v, bool in) {
     uint32_t all = 0;
-    if (__ballot(n > 0)) {
+    if (__ballot(in && has_value(v, both, mask))) {
+      const uint32_t n = in ? matches(v, both, mask) : 0u;
 #pragma unroll
       for (int b = 0; b < 4; ++b) all += __popcll(__ballot((n >> b) & 1)) << b;
     }
@@ -609,13 +648,13 @@ __device__ __forceinline__ void find_token(const u32x4 (&held)[kHold], const uin
   asm volatile("" : "+v"(mine_end));  // (compared anew: the conditions of the loads would be kept in, and spilled from, 38 SGPRs)
 #pragma unroll
   for (int it = 0; it < kHold; ++it)
-    if (it < steps) note(it, it < mine_end ? matches(held[it], both, mask) : 0u);
+    if (it < steps) note(it, held[it], it < mine_end);
 #pragma unroll 1
   for (int it = kHold; it < steps; ++it) {
     const int g = it * kRowThreads + tid;
-    uint32_t n = 0;
-    if (g < vecs) n = matches(load_bits(row, skew, V, g), both, mask);
-    note(it, n);
+    u32x4 v{};
+    if (g < vecs) v = load_bits(row, skew, V, g);
+    note(it, v, g < vecs);
   }
   __syncthreads();
   // the (step, wave) that holds it: every wave looks, one goes on
@@ -627,8 +666,9 @@ __device__ __forceinline__ void find_token(const u32x4 (&held)[kHold], const uin
   const uint32_t upto = wave_scan(mine);
   const uint64_t yes = __ballot(upto > rank);
   const int l = yes ? __ffsll((long long)yes) - 1 : 63;
-  uint32_t left = rank - (uint32_t)__shfl((int)(upto - mine), l);
+  uint32_t left = rank - lane_u32(upto - mine, l);
   int at = l * per;
+#pragma unroll 1
   while (at < min(entries, (l + 1) * per) - 1 && left >= s.found[at]) left -= s.found[at++];
   at = __builtin_amdgcn_readfirstlane(min(at, entries - 1));
   if (wave == at % kRowWaves) {  // uniform
@@ -672,9 +712,12 @@ __device__ __forceinline__ RowCut count_row(const FilterArgs& a, int b, const ui
     held[it] = u32x4{0u, 0u, 0u, 0u};
     if (g < vecs && whole_vec(skew, V, g)) held[it] = load_whole(row, skew, g);
   }
-  const float T = a.temperature[b];
-  const int k = a.top_k ? a.top_k[b] : 0;
-  const float p = a.top_p ? a.top_p[b] : 1.f, least = a.min_p ? a.min_p[b] : 0.f;
+  // (as vector loads: scalar ones would be waited for with the LDS writes)
+  int at_b = b;
+  asm volatile("" : "+v"(at_b));
+  const float T = a.temperature[at_b];
+  const int k = a.top_k ? a.top_k[at_b] : 0;
+  const float p = a.top_p ? a.top_p[at_b] : 1.f, least = a.min_p ? a.min_p[at_b] : 0.f;
   for (int i = tid; i < 32768 / 4; i += kRowThreads) reinterpret_cast<u32x4*>(s.bin)[i] = u32x4{0u, 0u, 0u, 0u};
   if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
   if (tid == 0) {
@@ -695,6 +738,7 @@ __device__ __forceinline__ RowCut count_row(const FilterArgs& a, int b, const ui
   const bool greedy = is_greedy(T);
   const double inv_t = greedy ? 1.0 : 1.0 / (double)T;
   uint32_t heavy = ~0u, many = 0;
+  int heavies = 0, groups = 0;
   int mine = (vecs - tid + kRowThreads - 1) / kRowThreads;
   asm volatile("" : "+v"(mine));
 #pragma unroll
@@ -729,31 +773,52 @@ __device__ __forceinline__ RowCut count_row(const FilterArgs& a, int b, const ui
       s.heavy_count[at] = many;
     }
     __syncthreads();
-    // groups, taken by the waves in turn: values that occur lie in few of them, next to each other
+    // which groups have values: 32 each wave
+    heavies = s.heavies;
+    uint32_t has = 0;
+#pragma unroll 1
+    for (int i = 0; i < 32; i += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = s.bin[word_of(32 * wave + i + j)];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) has |= (__ballot(w[j] != 0) ? 1u : 0u) << (i + j);
+    }
+    for (int i = 0; i < heavies; ++i) {  // (group of bits v: the order is falling for v < 0x8000)
+      const uint32_t v = s.heavy[i], g = v & 0x8000u ? v >> 7 : kGroups / 2 - 1 - (v >> 7);
+      if (g >> 5 == (uint32_t)wave) has |= 1u << (g & 31);
+    }
+    // (-0 counts with +0, the last value of the positive ones)
+    if (lane == 0) s.occurs[wave] = has;
+    __syncthreads();
+    const uint32_t occurs = lane < kGroups / 32 ? s.occurs[lane] | (lane == kGroups / 64 - 1 && (s.occurs[kGroups / 64] & 1) ? 1u << 31 : 0u) : 0u;
+    const uint32_t upto = wave_scan((uint32_t)__popc(occurs));
+    groups = (int)lane_u32(upto, 63);
+    // their counts and weights, the waves in turn
     uint32_t slots = 0;
 #pragma unroll 1
-    for (int g = wave; g < kGroups; g += kRowWaves) {
-      const Pair q = pair_of(s, g);
+    for (int n = wave; n < groups; n += kRowWaves) {
+      const int l = __ffsll((long long)__ballot(upto > (uint32_t)n)) - 1;
+      const uint32_t word = lane_u32(occurs, l), skip = n - (lane_u32(upto, l) - __popc(word));
+      const bool me = lane < 32 && ((word >> lane) & 1) && __popc(word & ((1u << (lane & 31)) - 1)) == skip;
+      const int g = 32 * l + __ffsll((long long)__ballot(me)) - 1;
+      const Pair q = pair_of(s, heavies, g);
       const uint32_t c = q.c1 + q.c2;
-      if (!__ballot(c > 0)) {  // uniform
-        if (lane == 0) s.count[g] = 0;
-        continue;
-      }
       if ((q.c1 && (q.v1 & 0x7fffu) > 0x7f80u) || (q.c2 && (q.v2 & 0x7fffu) > 0x7f80u)) s.nan = 1;
       const uint64_t y1 = __ballot(q.c1 > 0), y2 = __ballot(q.c2 > 0);
       const int l1 = y1 ? __ffsll((long long)y1) - 1 : 64, l2 = y2 ? __ffsll((long long)y2) - 1 : 64;
-      const uint32_t ref = (uint32_t)__shfl((int)(l1 <= l2 ? q.v1 : q.v2), min(l1, l2));
+      const uint32_t ref = lane_u32(l1 <= l2 ? q.v1 : q.v2, min(min(l1, l2), 63));
       const float rv = bf16_bits_to_f32(ref);
       double m = 0.0;
       if (q.c1) m = q.c1 * weight_of(bf16_bits_to_f32(q.v1), rv, inv_t, s.tab);
       if (q.c2) m += q.c2 * weight_of(bf16_bits_to_f32(q.v2), rv, inv_t, s.tab);
       m = wave_sum_dpp(m);
-      const uint32_t all = (uint32_t)__shfl((int)wave_scan(c), 63);
+      const uint32_t all = lane_u32(wave_scan(c), 63);
       slots += all;
       if (lane == 0) {
-        s.count[g] = all;
-        s.mass[g] = m;
-        s.ref[g] = ref;
+        s.count[n] = all;
+        s.mass[n] = m;
+        s.ref[n] = ((uint32_t)g << 16) | ref;
       }
     }
     if (lane == 0) atomicAdd(&s.slots, slots);
@@ -785,14 +850,8 @@ __device__ __forceinline__ RowCut count_row(const FilterArgs& a, int b, const ui
     return out;
   }
   if (wave == 0) {
-    // the maximum: the first group's first value
-    int g0 = 0;
-#pragma unroll 1
-    for (int i = kGroups / 64 - 1; i >= 0; --i) {
-      const uint64_t yes = __ballot(s.count[64 * i + lane] > 0);
-      if (yes) g0 = 64 * i + __ffsll((long long)yes) - 1;
-    }
-    const uint32_t top_bits = s.ref[g0];
+    // the maximum: the first value
+    const uint32_t top_bits = s.ref[0] & 0xffffu;
     const float top = bf16_bits_to_f32(top_bits);
     uint32_t cut = top_bits, value = top_bits;
     int kept = 1, rank = 0, cut_rank = -1;
@@ -802,25 +861,22 @@ __device__ __forceinline__ RowCut count_row(const FilterArgs& a, int b, const ui
       double f = 0.0;
       uint32_t n = 0;
 #pragma unroll 1
-      for (int g = 8 * lane; g < 8 * lane + 8; ++g) {
-        const uint32_t c = s.count[g];
-        const double m = c ? s.mass[g] * weight_of(bf16_bits_to_f32(s.ref[g]), top, inv_t, s.tab) : 0.0;
-        s.mass[g] = m;
-        s.before[g] = f;
-        s.cbefore[g] = n;
-        f += m;
-        n += c;
+      for (int i = 0; i < groups; i += 64) {
+        const int g = min(i + lane, groups - 1);
+        const bool in = i + lane < groups;
+        const double m = in ? s.mass[g] * weight_of(bf16_bits_to_f32(s.ref[g] & 0xffffu), top, inv_t, s.tab) : 0.0;
+        const uint32_t c = in ? s.count[g] : 0u;
+        const double fu = wave_scan(m);
+        const uint32_t nu = wave_scan(c);
+        if (in) {
+          s.mass[g] = m;
+          s.before[g] = f + lane_before(fu);
+          s.cbefore[g] = n + nu - c;
+        }
+        f += lane_f64(fu, 63);
+        n += lane_u32(nu, 63);
       }
-      const double upto = wave_scan(f);
-      double fb = __shfl_up(upto, 1);
-      if (lane == 0) fb = 0.0;
-      const uint32_t nb = wave_scan(n) - n;
-#pragma unroll 1
-      for (int g = 8 * lane; g < 8 * lane + 8; ++g) {
-        s.before[g] += fb;
-        s.cbefore[g] += nb;
-      }
-      total = __shfl(upto, 63);
+      total = f;
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
       kept = V;
       cut = 0xff80u;
@@ -840,7 +896,7 @@ __device__ __forceinline__ RowCut count_row(const FilterArgs& a, int b, const ui
           if (!sampled || kept == 1) continue;
           goal = unit(u) * total;
         }
-        const Place at = seek_counts(kind, goal, s, top, inv_t);
+        const Place at = seek_counts(kind, goal, s, groups, heavies, top, inv_t);
         if (kind == kBeyond) {
           const double j = fmin(floor((goal - at.mass) / at.weight), (double)min((int)at.count, kept - (int)at.before) - 1.0);
           value = at.value;

@@ -118,6 +118,28 @@ def test_masks(V, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_values_of_most_tokens(dtype):
+    """More than 65,535 tokens of one value: all over the row, in stretches one
+    after another, and where no wave's first lane holds it."""
+    print(f"case: sample_filtered crowded values {dtype}", flush=True)
+    V = 300001
+    x = logits(1, 6, V, dtype)
+    x[0, :90000] = -1.0
+    x[0, 100000:190000] = 1.0
+    x[0, 200000:] = -1.0
+    x[1, torch.arange(V) % 512 != 0] = 0.5
+    x[2, torch.arange(V) % 8 != 0] = 3.0
+    x[3, ::2] = -0.0
+    x[3, 1::2] = 0.0
+    x[4, torch.arange(V) % 3 > 0] = 20.0
+    x[5, torch.arange(V) % 512 != 0] = -0.0
+    f = dict(temperature=np.full(6, 0.8, np.float32))
+    for n, more in enumerate((dict(), dict(top_p=np.full(6, 0.7, np.float32)), dict(top_k=np.full(6, 150000, np.int32)),
+                              dict(min_p=np.full(6, 0.01, np.float32)))):
+        assert _check(x, dict(f, **more), _uniforms(n, 6)) == 6
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("V,pitch,offset", [(1000, 1001, 0), (1000, 1003, 3), (4096, 4096, 1), (8190, 8197, 5), (24593, 30000, 7)])
 def test_pitches_and_outputs(V, pitch, offset, dtype):
     """Rows off 16-byte boundaries; a strided column of drafts; neighbours untouched."""
