@@ -523,7 +523,8 @@ int nsv_sample(const void* logits, int64_t row_stride, const float* temperature,
  * nsv_sample_filtered: row b at b * row_stride elements (any row_stride >= V),
  *   temperature and uniforms [B] fp32; the token goes to
  *   out_tokens[b * out_stride]; kept [B] int32 (nullable): how many tokens the
- *   filters left.
+ *   filters left.  Workspace: nsv_sample_filtered_workspace_size() bytes on 16
+ *   bytes (0: none), of any content.
  *
  * nsv_accept_filtered: target and draft rows, drafts, num_drafts, draft_mode,
  *   out_tokens and out_len as nsv_accept_stochastic's (entries past a
@@ -538,14 +539,17 @@ int nsv_sample(const void* logits, int64_t row_stride, const float* temperature,
  *   uniforms[r] of every row r, and keeps drafts while they equal it.
  *   A draft outside [0, V) has probability 0.  Workspace:
  *   nsv_accept_filtered_workspace_size() bytes on 16 bytes, of any content.
+ * Calls that share a workspace must not run concurrently.
  */
+size_t nsv_sample_filtered_workspace_size(int B, int V, int dtype);
 int nsv_sample_filtered(const void* logits, int64_t row_stride,
                         const float* temperature, const int32_t* top_k,
                         const float* top_p, const float* min_p,
                         const float* uniforms, int B, int V, int dtype,
                         int32_t* out_tokens, int64_t out_stride,
-                        int32_t* kept, void* stream);
-size_t nsv_accept_filtered_workspace_size(int B, int K, int V);
+                        int32_t* kept, void* workspace, size_t workspace_bytes,
+                        void* stream);
+size_t nsv_accept_filtered_workspace_size(int B, int K, int V, int dtype);
 int nsv_accept_filtered(const void* target_logits, int64_t target_seq_stride,
                         const void* draft_logits, int64_t draft_seq_stride,
                         int64_t draft_row_stride, const int32_t* draft_mode,

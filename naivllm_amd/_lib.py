@@ -75,8 +75,9 @@ SIGNATURES: dict[str, tuple] = {
     "nsv_sample_workspace_size": (_c_size, [_c_int] * 3),
     "nsv_sample": (_c_int, [_c_vp, _c_i64, _c_vp, _c_vp] + [_c_int] * 3 + [_c_vp, _c_i64, _c_vp, _c_size, _c_vp]),
     "nsv_sample_filtered": (
-        _c_int, [_c_vp, _c_i64] + [_c_vp] * 5 + [_c_int] * 3 + [_c_vp, _c_i64, _c_vp, _c_vp]),
-    "nsv_accept_filtered_workspace_size": (_c_size, [_c_int] * 3),
+        _c_int, [_c_vp, _c_i64] + [_c_vp] * 5 + [_c_int] * 3 + [_c_vp, _c_i64, _c_vp, _c_vp, _c_size, _c_vp]),
+    "nsv_sample_filtered_workspace_size": (_c_size, [_c_int] * 3),
+    "nsv_accept_filtered_workspace_size": (_c_size, [_c_int] * 4),
     "nsv_accept_filtered": (
         _c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_i64] + [_c_vp] * 8 + [_c_int] * 4
         + [_c_vp, _c_vp, _c_vp, _c_size, _c_vp]),

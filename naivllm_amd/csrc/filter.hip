@@ -45,6 +45,7 @@ constexpr int kMaxDrafts = 63;                   // K + 1 rows fit one 64-lane b
 constexpr int kChunkThreads = 256;
 constexpr int kChunk = kChunkThreads * kVec;     // of the residual passes
 
+struct Part;
 template <typename T> struct Elem;
 template <> struct Elem<uint16_t> {  // bf16 bits
   __device__ static float get(uint16_t v) { return bf16_bits_to_f32(v); }
@@ -83,6 +84,8 @@ struct FilterArgs {
   const int32_t* mode;     // nullable; 0: sequence b has no draft rows
   RowCut* cuts;            // [B, 2K + 1]: target rows 0..K, then draft rows
   double* probs;           // [B, 2K + 1]: the probability of the row's draft
+  Part* row_parts;         // [B, rows per sequence, split]
+  int split;
   double* parts;           // [B, chunks, 2]: sums of the residual and of p_target
   int chunks;
   int32_t* tokens;         // sampler: row b's at b * out_stride
@@ -434,11 +437,13 @@ __device__ RowCut filter_row(const FilterArgs& a, int b, const T* row, bool samp
 // ---------------------------------------------------------------------------
 // bf16 rows by counts
 // ---------------------------------------------------------------------------
-constexpr int kHold = 19;      // 16-byte vectors a thread keeps (76 of its 128 registers): rows up to 155,648
 constexpr int kGroups = 512;   // of 128 values each, along the order of the tokens: 64 words of two counts
+constexpr int kAhead = 4;      // vectors a thread loads ahead of those it counts
 constexpr int kSafeSteps = 7;  // steps whose 57,344 tokens fit a 16-bit count beside ..
 constexpr uint32_t kFull = 65536 - kSafeSteps * kStep;  // .. fewer than these
 constexpr int kMaxHeavy = kRowWaves + kMaxVocab / kFull + 1;
+constexpr int kMaxParts = 32;  // of a row, counted by a workgroup each ..
+constexpr int kMaxSplit = 8;  // .. for speed this many
 
 struct CountLds {
   uint32_t bin[32768];         // counts of values 2i (low half) and 2i + 1
@@ -452,6 +457,7 @@ struct CountLds {
   uint32_t found[kMaxSteps * kRowWaves];
   double tab[256];
   uint32_t heavy[kMaxHeavy], heavy_count[kMaxHeavy];  // counts beside the bins
+  uint32_t part_occurs[kMaxParts * kGroups / 32];
   int heavies;
   uint32_t slots;              // tokens counted
   int nan, index;
@@ -462,29 +468,53 @@ struct CountLds {
   double total;
 };
 
-// Vector g of a row: its elements 8 g - skew .. + 7, `skew` the elements from a
-// 16-byte boundary to its start.
-__device__ __forceinline__ bool whole_vec(int skew, int V, int g) {
-  const int64_t e0 = (int64_t)8 * g - skew;
-  return e0 >= 0 && e0 + 8 <= V;
-}
-__device__ __forceinline__ u32x4 load_whole(const uint16_t* row, int skew, int g) {
-  return load16_stream(row + ((int64_t)8 * g - skew));
-}
-// one of the row's ends: -inf where the row has no element
-__device__ __forceinline__ u32x4 load_edge(const uint16_t* row, int skew, int V, int g) {
-  const int64_t e0 = (int64_t)8 * g - skew;
-  u32x4 v;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t a = e0 + 2 * i, b = a + 1;
-    const uint32_t lo = a >= 0 && a < V ? row[a] : 0xff80u, hi = b >= 0 && b < V ? row[b] : 0xff80u;
-    v[i] = lo | (hi << 16);
+// A row as vectors of 8 elements on 16 bytes: vector g holds elements 8 g -
+// skew .. + 7; what lies outside the row counts as -inf.
+struct Row {
+  const uint16_t* at;
+  int V, skew, vecs;
+  __device__ Row(const uint16_t* row, int V_) : at(row), V(V_), skew((int)(((uintptr_t)row & 15) >> 1)) {
+    vecs = (V + skew + 7) / 8;
   }
-  return v;
-}
-__device__ __forceinline__ u32x4 load_bits(const uint16_t* row, int skew, int V, int g) {
-  return whole_vec(skew, V, g) ? load_whole(row, skew, g) : load_edge(row, skew, V, g);
+  __device__ __forceinline__ u32x4 load(int g) const {
+    const int64_t e0 = (int64_t)8 * g - skew;
+    if (e0 >= 0 && e0 + 8 <= V) return *reinterpret_cast<const u32x4*>(at + e0);
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t a = e0 + 2 * i, b = a + 1;
+      const uint32_t lo = a >= 0 && a < V ? at[a] : 0xff80u, hi = b >= 0 && b < V ? at[b] : 0xff80u;
+      v[i] = lo | (hi << 16);
+    }
+    return v;
+  }
+};
+
+// f(step, vector, whether there is one) of the vectors lo .. hi - 1, a
+// workgroup's threads together, kAhead of them loaded ahead.  The loop stays
+// rolled: a row kept in registers (one unrolled body per vector) saved its
+// second reading, and cost more in instructions fetched once.
+template <typename F>
+__device__ __forceinline__ void each_vec(const Row& row, int lo, int hi, F f) {
+  const int steps = (hi - lo + kRowThreads - 1) / kRowThreads;
+  u32x4 v[kAhead];
+  int g = lo + threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) v[j] = row.load(min(g + j * kRowThreads, hi - 1));
+#pragma unroll 1
+  for (int it = 0; it < steps; it += kAhead) {
+    u32x4 w[kAhead];
+    if (it + kAhead < steps) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) w[j] = row.load(min(g + (kAhead + j) * kRowThreads, hi - 1));
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (it + j < steps) f(it + j, v[j], g + j * kRowThreads < hi);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) v[j] = w[j];
+    g += kAhead * kRowThreads;
+  }
 }
 
 __device__ __forceinline__ void count_value(uint32_t* bin, uint32_t bits) {
@@ -513,6 +543,10 @@ __device__ __forceinline__ void count_vec(uint32_t* bin, const u32x4& v, uint32_
   for (int e = 0; e < 8; ++e) count_value(bin, (e & 1) ? v[e >> 1] >> 16 : v[e >> 1] & 0xffffu);
 }
 
+__device__ __forceinline__ void clear_bins(uint32_t* bin) {
+  for (int i = threadIdx.x; i < 32768 / 4; i += kRowThreads) reinterpret_cast<u32x4*>(bin)[i] = u32x4{0u, 0u, 0u, 0u};
+}
+
 // Counts that another kSafeSteps might carry over 16 bits, beside the bins.
 __device__ __forceinline__ void flush_full(CountLds& s) {
   __syncthreads();
@@ -533,17 +567,51 @@ __device__ __forceinline__ void flush_full(CountLds& s) {
   __syncthreads();
 }
 
+// a lane's word of a group
+__device__ __forceinline__ uint32_t word_of(int g) {
+  const int lane = threadIdx.x & 63;
+  return g >= kGroups / 2 ? 64 * g + lane : 64 * (kGroups / 2 - 1 - g) + 63 - lane;
+}
+__device__ __forceinline__ int group_of(uint32_t value) {
+  return value & 0x8000u ? (int)(value >> 7) : kGroups / 2 - 1 - (int)(value >> 7);
+}
+
+// Which of a wave's 32 groups have values, as bits; f(group, a lane's word) of
+// each that has.
+template <typename F>
+__device__ __forceinline__ uint32_t own_groups(const uint32_t* bin, F f) {
+  const int wave = threadIdx.x >> 6;
+  uint32_t has = 0;
+#pragma unroll 1
+  for (int i = 0; i < 32; i += 8) {
+    uint32_t w[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) w[j] = bin[word_of(32 * wave + i + j)];
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (__ballot(w[j] != 0)) {  // uniform
+        has |= 1u << (i + j);
+        f(32 * wave + i + j, w[j]);
+      }
+  }
+  return has;
+}
+
+// The n-th group that occurs; lanes 0..15 hold the words of bits in `occurs`
+// and their running counts in `upto`.
+__device__ __forceinline__ int nth_group(int n, uint32_t occurs, uint32_t upto) {
+  const int lane = threadIdx.x & 63;
+  const int l = __ffsll((long long)__ballot(upto > (uint32_t)n)) - 1;
+  const uint32_t word = lane_u32(occurs, l), skip = n - (lane_u32(upto, l) - __popc(word));
+  const bool me = lane < 32 && ((word >> lane) & 1) && __popc(word & ((1u << (lane & 31)) - 1)) == skip;
+  return 32 * l + __ffsll((long long)__ballot(me)) - 1;
+}
+
 __device__ __forceinline__ uint32_t heavy_of(const CountLds& s, int heavies, uint32_t value) {
   uint32_t c = 0;
   for (int i = 0; i < heavies; ++i)
     if (s.heavy[i] == value) c += s.heavy_count[i];
   return c;
-}
-
-// a lane's word of a group
-__device__ __forceinline__ uint32_t word_of(int g) {
-  const int lane = threadIdx.x & 63;
-  return g >= kGroups / 2 ? 64 * g + lane : 64 * (kGroups / 2 - 1 - g) + 63 - lane;
 }
 
 // The two values of a lane in a group, in order, and their counts; -0 counts as +0.
@@ -561,6 +629,16 @@ __device__ __forceinline__ Pair pair_of(const CountLds& s, int heavies, int g) {
   if (w == 0x4000u) p.c1 = 0;
   if (w == 0) p.c2 += (s.bin[0x4000] & 0xffffu) + heavy_of(s, heavies, 0x8000u);
   return p;
+}
+
+// weights of a pair's values against the value `top` (0 where a value does not
+// occur), without a branch: the two chains run beside each other
+__device__ __forceinline__ void pair_weights(const Pair& p, float top, double inv_t, const double* tab, double& w1, double& w2) {
+  const float x1 = bf16_bits_to_f32(p.c1 ? p.v1 : 0xff80u), x2 = bf16_bits_to_f32(p.c2 ? p.v2 : 0xff80u);
+  const double e1 = nsv_exp_nonpos(((double)x1 - (double)top) * inv_t, tab);
+  const double e2 = nsv_exp_nonpos(((double)x2 - (double)top) * inv_t, tab);
+  w1 = x1 == top ? 1.0 : e1;
+  w2 = x2 == top ? 1.0 : e2;
 }
 
 struct Place {
@@ -587,8 +665,8 @@ __device__ __forceinline__ Place seek_counts(int kind, double goal, const CountL
   }
   at_group = max(at_group, 0);
   const Pair p = pair_of(s, heavies, (int)(s.ref[at_group] >> 16));
-  const double w1 = p.c1 ? weight_of(bf16_bits_to_f32(p.v1), top, inv_t, s.tab) : 0.0;
-  const double w2 = p.c2 ? weight_of(bf16_bits_to_f32(p.v2), top, inv_t, s.tab) : 0.0;
+  double w1, w2;
+  pair_weights(p, top, inv_t, s.tab, w1, w2);
   const double m1 = p.c1 * w1, m = m1 + p.c2 * w2;
   const double before = lane_before(wave_scan(m)) + s.before[at_group];
   const uint32_t cbefore = s.cbefore[at_group] + wave_scan(p.c1 + p.c2) - p.c1 - p.c2;
@@ -610,19 +688,17 @@ __device__ __forceinline__ Place seek_counts(int kind, double goal, const CountL
   return at;
 }
 
-// how many of a vector's tokens have the value (`both`: twice its bits, under `mask`)
+// how many of a vector's tokens have the value (`both`: twice its bits, under
+// `mask`), and whether any has
+typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ uint32_t matches(const u32x4& v, uint32_t both, uint32_t mask) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   u16x2 n = {0, 0};  // others
 #pragma unroll
   for (int i = 0; i < 4; ++i)
     n += __builtin_elementwise_min(__builtin_bit_cast(u16x2, (v[i] & mask) ^ both), (u16x2){1, 1});
   return 8u - n[0] - n[1];
 }
-
-// whether a vector has a token of the value
 __device__ __forceinline__ bool has_value(const u32x4& v, uint32_t both, uint32_t mask) {
-  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   u16x2 d[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) d[i] = __builtin_bit_cast(u16x2, (v[i] & mask) ^ both);
@@ -630,12 +706,12 @@ __device__ __forceinline__ bool has_value(const u32x4& v, uint32_t both, uint32_
   return m[0] == 0 || m[1] == 0;
 }
 
-// s.index = the index of the token of bits `value` with `rank` of them before it
-__device__ __forceinline__ void find_token(const u32x4 (&held)[kHold], const uint16_t* row, int skew, int V, int vecs, int steps,
-                                           uint32_t value, uint32_t rank, CountLds& s) {
+// s.index = the index of the token of bits `value` with `rank` of them before
+// it among the vectors lo .. hi - 1
+__device__ __forceinline__ void find_token(const Row& row, int lo, int hi, uint32_t value, uint32_t rank, CountLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t mask = value ? ~0u : 0x7fff7fffu, both = value | (value << 16);  // (+0: -0 too)
-  auto note = [&](int it, const u32x4& v, bool in) {
+  each_vec(row, lo, hi, [&](int it, const u32x4& v, bool in) {
     uint32_t all = 0;
     if (__ballot(in && has_value(v, both, mask))) {
       const uint32_t n = in ? matches(v, both, mask) : 0u;
@@ -643,22 +719,10 @@ __device__ __forceinline__ void find_token(const u32x4 (&held)[kHold], const uin
       for (int b = 0; b < 4; ++b) all += __popcll(__ballot((n >> b) & 1)) << b;
     }
     if (lane == 0) s.found[it * kRowWaves + wave] = all;
-  };
-  int mine_end = (vecs - tid + kRowThreads - 1) / kRowThreads;
-  asm volatile("" : "+v"(mine_end));  // (compared anew: the conditions of the loads would be kept in, and spilled from, 38 SGPRs)
-#pragma unroll
-  for (int it = 0; it < kHold; ++it)
-    if (it < steps) note(it, held[it], it < mine_end);
-#pragma unroll 1
-  for (int it = kHold; it < steps; ++it) {
-    const int g = it * kRowThreads + tid;
-    u32x4 v{};
-    if (g < vecs) v = load_bits(row, skew, V, g);
-    note(it, v, g < vecs);
-  }
+  });
   __syncthreads();
   // the (step, wave) that holds it: every wave looks, one goes on
-  const int entries = steps * kRowWaves, per = (entries + 63) / 64;
+  const int entries = (hi - lo + kRowThreads - 1) / kRowThreads * kRowWaves, per = (entries + 63) / 64;
   uint32_t mine = 0;
 #pragma unroll 1
   for (int i = 0; i < per; ++i)
@@ -672,16 +736,10 @@ __device__ __forceinline__ void find_token(const u32x4 (&held)[kHold], const uin
   while (at < min(entries, (l + 1) * per) - 1 && left >= s.found[at]) left -= s.found[at++];
   at = __builtin_amdgcn_readfirstlane(min(at, entries - 1));
   if (wave == at % kRowWaves) {  // uniform
-    const int it = at / kRowWaves, g = it * kRowThreads + tid;
+    const int g = lo + at / kRowWaves * kRowThreads + tid;
     u32x4 v{};
-    if (it < kHold) {
-#pragma unroll
-      for (int i = 0; i < kHold; ++i)
-        if (i == it) v = held[i];
-    } else if (g < vecs) {
-      v = load_bits(row, skew, V, g);
-    }
-    const uint32_t n = g < vecs ? matches(v, both, mask) : 0u;
+    if (g < hi) v = row.load(g);
+    const uint32_t n = g < hi ? matches(v, both, mask) : 0u;
     const uint32_t before = wave_scan(n) - n;
     if (n && left >= before && left < before + n) {
       uint32_t k = before;
@@ -693,76 +751,204 @@ __device__ __forceinline__ void find_token(const u32x4 (&held)[kHold], const uin
         if (e & 1) v = u32x4{v[1], v[2], v[3], v[0]};
         else v[0] >>= 16;
       }
-      s.index = 8 * g - skew + e;
+      s.index = 8 * g - row.skew + e;
     }
   }
   __syncthreads();
 }
 
-// filter_row for bf16.
-__device__ __forceinline__ RowCut count_row(const FilterArgs& a, int b, const uint16_t* row, bool sampled, float u, bool ends,
-                                            CountLds& s) {
-  const int V = a.V, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int skew = (int)(((uintptr_t)row & 15) >> 1);
-  const int vecs = (V + skew + 7) / 8, steps = (vecs + kRowThreads - 1) / kRowThreads;
-  u32x4 held[kHold];
-#pragma unroll
-  for (int it = 0; it < kHold; ++it) {
-    const int g = it * kRowThreads + tid;
-    held[it] = u32x4{0u, 0u, 0u, 0u};
-    if (g < vecs && whole_vec(skew, V, g)) held[it] = load_whole(row, skew, g);
+struct Settings {
+  float T, p, least, u;
+  int k;
+  bool sampled, ends;
+  double inv_t;
+};
+// (as vector loads: scalar ones would be waited for with the LDS writes)
+__device__ __forceinline__ Settings settings_of(const FilterArgs& a, int b, bool sampled, int64_t at_u, bool ends) {
+  int vb = b;
+  int64_t vu = at_u;
+  asm volatile("" : "+v"(vb), "+v"(vu));
+  Settings f;
+  f.T = a.temperature[vb];
+  f.k = a.top_k ? a.top_k[vb] : 0;
+  f.p = a.top_p ? a.top_p[vb] : 1.f;
+  f.least = a.min_p ? a.min_p[vb] : 0.f;
+  f.u = a.uniforms[vu];
+  f.sampled = sampled;
+  f.ends = ends;
+  return f;
+}
+
+// Counts and weights of the groups that occur, the waves in turn; their number.
+__device__ __forceinline__ int weigh_groups(double inv_t, int heavies, CountLds& s) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  uint32_t occurs = lane < kGroups / 32 ? s.occurs[lane] : 0u;
+  // (-0 counts with +0, the last value of the positive ones)
+  if (lane == kGroups / 64 - 1 && (s.occurs[kGroups / 64] & 1)) occurs |= 1u << 31;
+  const uint32_t upto = wave_scan((uint32_t)__popc(occurs));
+  const int groups = (int)lane_u32(upto, 63);
+  uint32_t slots = 0;
+#pragma unroll 1
+  for (int n = wave; n < groups; n += kRowWaves) {
+    const int g = nth_group(n, occurs, upto);
+    const Pair q = pair_of(s, heavies, g);
+    if ((q.c1 && (q.v1 & 0x7fffu) > 0x7f80u) || (q.c2 && (q.v2 & 0x7fffu) > 0x7f80u)) s.nan = 1;
+    const uint64_t y1 = __ballot(q.c1 > 0), y2 = __ballot(q.c2 > 0);
+    const int l1 = y1 ? __ffsll((long long)y1) - 1 : 64, l2 = y2 ? __ffsll((long long)y2) - 1 : 64;
+    const uint32_t ref = lane_u32(l1 <= l2 ? q.v1 : q.v2, min(min(l1, l2), 63));
+    double w1, w2;
+    pair_weights(q, bf16_bits_to_f32(ref), inv_t, s.tab, w1, w2);
+    const double m = wave_sum_dpp(q.c1 * w1 + q.c2 * w2);
+    const uint32_t all = lane_u32(wave_scan(q.c1 + q.c2), 63);
+    slots += all;
+    if (lane == 0) {
+      s.count[n] = all;
+      s.mass[n] = m;
+      s.ref[n] = ((uint32_t)g << 16) | ref;
+    }
   }
-  // (as vector loads: scalar ones would be waited for with the LDS writes)
-  int at_b = b;
-  asm volatile("" : "+v"(at_b));
-  const float T = a.temperature[at_b];
-  const int k = a.top_k ? a.top_k[at_b] : 0;
-  const float p = a.top_p ? a.top_p[at_b] : 1.f, least = a.min_p ? a.min_p[at_b] : 0.f;
-  for (int i = tid; i < 32768 / 4; i += kRowThreads) reinterpret_cast<u32x4*>(s.bin)[i] = u32x4{0u, 0u, 0u, 0u};
+  if (lane == 0) atomicAdd(&s.slots, slots);
+  return groups;
+}
+
+// What the filters leave, from the weighed groups, by one wave: into s.
+__device__ __forceinline__ void decide(const Settings& f, int V, int groups, int heavies, CountLds& s) {
+  const int lane = threadIdx.x & 63;
+  const uint32_t top_bits = s.ref[0] & 0xffffu;  // the maximum: the first value
+  const float top = bf16_bits_to_f32(top_bits);
+  uint32_t cut = top_bits, value = top_bits;
+  int kept = 1, rank = 0, cut_rank = -1;
+  double total = 1.0;
+  if (!is_greedy(f.T) && top != -__builtin_inff()) {  // uniform
+    // weights and tokens before each group
+    total = 0.0;
+    uint32_t n = 0;
+#pragma unroll 1
+    for (int i = 0; i < groups; i += 64) {
+      const int g = min(i + lane, groups - 1);
+      const bool in = i + lane < groups;
+      const double m = in ? s.mass[g] * weight_of(bf16_bits_to_f32(s.ref[g] & 0xffffu), top, f.inv_t, s.tab) : 0.0;
+      const uint32_t c = in ? s.count[g] : 0u;
+      const double fu = wave_scan(m);
+      const uint32_t nu = wave_scan(c);
+      if (in) {
+        s.mass[g] = m;
+        s.before[g] = total + lane_before(fu);
+        s.cbefore[g] = n + nu - c;
+      }
+      total += lane_f64(fu, 63);
+      n += lane_u32(nu, 63);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");  // (this wave's own)
+    kept = V;
+    cut = 0xff80u;
+#pragma unroll 1
+    for (int kind = 0; kind < 4; ++kind) {
+      double goal = 0.0;
+      if (kind == kByCount) {
+        if (f.k <= 0 || f.k >= V) continue;
+        goal = (double)f.k;
+      } else if (kind == kReach) {
+        if (!(f.p < 1.f)) continue;
+        goal = fmax((double)f.p * total, 0x1p-1000);  // (the first token stays)
+      } else if (kind == kAbove) {
+        if (!(f.least > 0.f)) continue;
+        goal = fmin((double)f.least, 1.0);
+      } else {
+        if (!f.sampled || kept == 1) continue;
+        goal = unit(f.u) * total;
+      }
+      const Place at = seek_counts(kind, goal, s, groups, heavies, top, f.inv_t);
+      if (kind == kBeyond) {
+        const double j = fmin(floor((goal - at.mass) / at.weight), (double)min((int)at.count, kept - (int)at.before) - 1.0);
+        value = at.value;
+        rank = (int)fmax(j, 0.0);
+        continue;
+      }
+      uint32_t stay = at.count;  // tokens of the value that do
+      if (kind == kByCount) stay = (uint32_t)f.k - at.before;
+      if (kind == kReach) stay = (uint32_t)fmin(fmax(ceil((goal - at.mass) / at.weight), 1.0), (double)at.count);
+      if ((int)(at.before + stay) >= kept) continue;
+      kept = (int)(at.before + stay);
+      cut = at.value;
+      cut_rank = stay < at.count ? (int)stay - 1 : -1;
+      total = at.mass + stay * at.weight;
+    }
+    if (!f.sampled && kept > 1) rank = -1;
+    // (a cut among tokens of weight 0 cuts nothing; a lone token is looked up as the sample)
+    if (!f.ends || kept == 1 || cut == 0xff80u) cut_rank = -1;
+  }
+  if (lane == 0) {
+    s.top = top;
+    s.cut = bf16_bits_to_f32(cut);
+    s.cut_value = cut;
+    s.kept = kept;
+    s.total = total;
+    s.value = value;
+    s.rank = rank;
+    s.cut_rank = cut_rank;
+  }
+}
+
+// The first NaN of a row that has one.
+__device__ __forceinline__ RowCut nan_row(const Row& row, CountLds& s) {
+  if (threadIdx.x == 0) s.index = row.V;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < row.V; i += kRowThreads)
+    if ((row.at[i] & 0x7fffu) > 0x7f80u) atomicMin(&s.index, i);
+  __syncthreads();
+  return RowCut{__builtin_nanf(""), __builtin_nanf(""), s.index, 1, s.index, 0, 1.0};
+}
+
+// find(value, rank) -> s.index, for what decide() wants looked up
+template <typename F>
+__device__ __forceinline__ RowCut look_up(int V, const CountLds& s, F find) {
+  RowCut out{s.top, s.cut, V - 1, s.kept, 0, 0, s.total};
+  const int rank = s.rank, cut_rank = s.cut_rank;
+  const uint32_t value = s.value, cut_value = s.cut_value;
+  if (out.top == -__builtin_inff()) {  // uniform: nothing above it, the first token
+    out.last = 0;
+    return out;
+  }
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    const int r = which ? cut_rank : rank;
+    if (r < 0) continue;  // uniform
+    find(which ? cut_value : value, (uint32_t)r);
+    if (which) out.last = s.index;
+    else out.token = s.index;
+  }
+  if (out.kept == 1) out.last = out.token;
+  return out;
+}
+
+// filter_row for bf16, by one workgroup.
+__device__ __forceinline__ RowCut count_row(const Row& row, Settings f, CountLds& s) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  clear_bins(s.bin);
   if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
   if (tid == 0) {
     s.nan = s.heavies = 0;
     s.slots = 0;
   }
-  // the row's first and last vector, where they are no whole ones
-#pragma unroll 1
-  for (int e = 0; e < 2; ++e) {
-    const int g = e ? vecs - 1 : 0;
-    if (g >= kHold * kRowThreads || tid != g % kRowThreads || whole_vec(skew, V, g)) continue;
-    const u32x4 v = load_edge(row, skew, V, g);
-#pragma unroll
-    for (int it = 0; it < kHold; ++it)
-      if (it == g / kRowThreads) held[it] = v;
-  }
-  lds_barrier();  // (the row's loads stay in flight)
-  const bool greedy = is_greedy(T);
-  const double inv_t = greedy ? 1.0 : 1.0 / (double)T;
-  uint32_t heavy = ~0u, many = 0;
-  int heavies = 0, groups = 0;
-  int mine = (vecs - tid + kRowThreads - 1) / kRowThreads;
-  asm volatile("" : "+v"(mine));
-#pragma unroll
-  for (int it = 0; it < kHold; ++it)
-    if (it < mine) count_vec(s.bin, held[it], heavy, many);
-#pragma unroll 1
-  for (int it = kHold; it < steps; ++it) {
-    const int g = it * kRowThreads + tid;
-    if (g < vecs) count_vec(s.bin, load_bits(row, skew, V, g), heavy, many);
-  }
+  lds_barrier();
+  f.inv_t = is_greedy(f.T) ? 1.0 : 1.0 / (double)f.T;
   // A bin runs over only where one value has more than 65,535 tokens: the
   // counts then miss some, and are taken again with the full ones put aside
   // in between.
+  int groups = 0, heavies = 0;
 #pragma unroll 1
   for (int careful = 0; careful < 2; ++careful) {
-    if (careful) {
-      heavy = ~0u;
-      many = 0;
+    uint32_t heavy = ~0u, many = 0;
+    const int whole = (row.vecs + kRowThreads - 1) / kRowThreads * kRowThreads;
+    const int run = careful ? kSafeSteps * kRowThreads : whole;
 #pragma unroll 1
-      for (int it = 0; it < steps; ++it) {
-        const int g = it * kRowThreads + tid;
-        if (g < vecs) count_vec(s.bin, load_bits(row, skew, V, g), heavy, many);
-        if (it % kSafeSteps == kSafeSteps - 1) flush_full(s);
-      }
+    for (int lo = 0; lo < row.vecs; lo += run) {
+      each_vec(row, lo, min(lo + run, row.vecs), [&](int, const u32x4& v, bool in) {
+        if (in) count_vec(s.bin, v, heavy, many);
+      });
+      if (careful) flush_full(s);
     }
     // (a wave's lanes count alike, but those without a last vector)
     heavy = (uint32_t)__builtin_amdgcn_readfirstlane((int)heavy);
@@ -773,178 +959,134 @@ __device__ __forceinline__ RowCut count_row(const FilterArgs& a, int b, const ui
       s.heavy_count[at] = many;
     }
     __syncthreads();
-    // which groups have values: 32 each wave
     heavies = s.heavies;
-    uint32_t has = 0;
-#pragma unroll 1
-    for (int i = 0; i < 32; i += 8) {
-      uint32_t w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = s.bin[word_of(32 * wave + i + j)];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) has |= (__ballot(w[j] != 0) ? 1u : 0u) << (i + j);
+    uint32_t has = own_groups(s.bin, [](int, uint32_t) {});
+    for (int i = 0; i < heavies; ++i) {
+      const int g = group_of(s.heavy[i]);
+      if (g >> 5 == wave) has |= 1u << (g & 31);
     }
-    for (int i = 0; i < heavies; ++i) {  // (group of bits v: the order is falling for v < 0x8000)
-      const uint32_t v = s.heavy[i], g = v & 0x8000u ? v >> 7 : kGroups / 2 - 1 - (v >> 7);
-      if (g >> 5 == (uint32_t)wave) has |= 1u << (g & 31);
-    }
-    // (-0 counts with +0, the last value of the positive ones)
     if (lane == 0) s.occurs[wave] = has;
     __syncthreads();
-    const uint32_t occurs = lane < kGroups / 32 ? s.occurs[lane] | (lane == kGroups / 64 - 1 && (s.occurs[kGroups / 64] & 1) ? 1u << 31 : 0u) : 0u;
-    const uint32_t upto = wave_scan((uint32_t)__popc(occurs));
-    groups = (int)lane_u32(upto, 63);
-    // their counts and weights, the waves in turn
-    uint32_t slots = 0;
-#pragma unroll 1
-    for (int n = wave; n < groups; n += kRowWaves) {
-      const int l = __ffsll((long long)__ballot(upto > (uint32_t)n)) - 1;
-      const uint32_t word = lane_u32(occurs, l), skip = n - (lane_u32(upto, l) - __popc(word));
-      const bool me = lane < 32 && ((word >> lane) & 1) && __popc(word & ((1u << (lane & 31)) - 1)) == skip;
-      const int g = 32 * l + __ffsll((long long)__ballot(me)) - 1;
-      const Pair q = pair_of(s, heavies, g);
-      const uint32_t c = q.c1 + q.c2;
-      if ((q.c1 && (q.v1 & 0x7fffu) > 0x7f80u) || (q.c2 && (q.v2 & 0x7fffu) > 0x7f80u)) s.nan = 1;
-      const uint64_t y1 = __ballot(q.c1 > 0), y2 = __ballot(q.c2 > 0);
-      const int l1 = y1 ? __ffsll((long long)y1) - 1 : 64, l2 = y2 ? __ffsll((long long)y2) - 1 : 64;
-      const uint32_t ref = lane_u32(l1 <= l2 ? q.v1 : q.v2, min(min(l1, l2), 63));
-      const float rv = bf16_bits_to_f32(ref);
-      double m = 0.0;
-      if (q.c1) m = q.c1 * weight_of(bf16_bits_to_f32(q.v1), rv, inv_t, s.tab);
-      if (q.c2) m += q.c2 * weight_of(bf16_bits_to_f32(q.v2), rv, inv_t, s.tab);
-      m = wave_sum_dpp(m);
-      const uint32_t all = lane_u32(wave_scan(c), 63);
-      slots += all;
-      if (lane == 0) {
-        s.count[n] = all;
-        s.mass[n] = m;
-        s.ref[n] = ((uint32_t)g << 16) | ref;
-      }
-    }
-    if (lane == 0) atomicAdd(&s.slots, slots);
+    groups = weigh_groups(f.inv_t, heavies, s);
     __syncthreads();
-    if (s.slots == 8u * (uint32_t)vecs) break;  // uniform
+    if (s.slots == 8u * (uint32_t)row.vecs) break;  // uniform
     __syncthreads();
-    for (int i = tid; i < 32768 / 4; i += kRowThreads) reinterpret_cast<u32x4*>(s.bin)[i] = u32x4{0u, 0u, 0u, 0u};
+    clear_bins(s.bin);
     if (tid == 0) {
       s.heavies = 0;
       s.slots = 0;
     }
     __syncthreads();
   }
-  RowCut out;
-  out.last = V - 1;
-  out.token = 0;
-  out.pad = 0;
-  if (s.nan) {  // uniform: the first NaN
-    if (tid == 0) s.index = V;
-    __syncthreads();
-#pragma unroll 1
-    for (int i = tid; i < V; i += kRowThreads)
-      if ((row[i] & 0x7fffu) > 0x7f80u) atomicMin(&s.index, i);
-    __syncthreads();
-    out.top = out.cut = __builtin_nanf("");
-    out.kept = 1;
-    out.token = out.last = s.index;
-    out.total = 1.0;
-    return out;
-  }
-  if (wave == 0) {
-    // the maximum: the first value
-    const uint32_t top_bits = s.ref[0] & 0xffffu;
-    const float top = bf16_bits_to_f32(top_bits);
-    uint32_t cut = top_bits, value = top_bits;
-    int kept = 1, rank = 0, cut_rank = -1;
-    double total = 1.0;
-    if (!greedy && top != -__builtin_inff()) {  // uniform
-      // weights and tokens before each group
-      double f = 0.0;
-      uint32_t n = 0;
-#pragma unroll 1
-      for (int i = 0; i < groups; i += 64) {
-        const int g = min(i + lane, groups - 1);
-        const bool in = i + lane < groups;
-        const double m = in ? s.mass[g] * weight_of(bf16_bits_to_f32(s.ref[g] & 0xffffu), top, inv_t, s.tab) : 0.0;
-        const uint32_t c = in ? s.count[g] : 0u;
-        const double fu = wave_scan(m);
-        const uint32_t nu = wave_scan(c);
-        if (in) {
-          s.mass[g] = m;
-          s.before[g] = f + lane_before(fu);
-          s.cbefore[g] = n + nu - c;
-        }
-        f += lane_f64(fu, 63);
-        n += lane_u32(nu, 63);
-      }
-      total = f;
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "local");
-      kept = V;
-      cut = 0xff80u;
-#pragma unroll 1
-      for (int kind = 0; kind < 4; ++kind) {
-        double goal = 0.0;
-        if (kind == kByCount) {
-          if (k <= 0 || k >= V) continue;
-          goal = (double)k;
-        } else if (kind == kReach) {
-          if (!(p < 1.f)) continue;
-          goal = fmax((double)p * total, 0x1p-1000);  // (the first token stays)
-        } else if (kind == kAbove) {
-          if (!(least > 0.f)) continue;
-          goal = fmin((double)least, 1.0);
-        } else {
-          if (!sampled || kept == 1) continue;
-          goal = unit(u) * total;
-        }
-        const Place at = seek_counts(kind, goal, s, groups, heavies, top, inv_t);
-        if (kind == kBeyond) {
-          const double j = fmin(floor((goal - at.mass) / at.weight), (double)min((int)at.count, kept - (int)at.before) - 1.0);
-          value = at.value;
-          rank = (int)fmax(j, 0.0);
-          continue;
-        }
-        uint32_t stay = at.count;  // tokens of the value that do
-        if (kind == kByCount) stay = (uint32_t)k - at.before;
-        if (kind == kReach) stay = (uint32_t)fmin(fmax(ceil((goal - at.mass) / at.weight), 1.0), (double)at.count);
-        if ((int)(at.before + stay) >= kept) continue;
-        kept = (int)(at.before + stay);
-        cut = at.value;
-        cut_rank = stay < at.count ? (int)stay - 1 : -1;
-        total = at.mass + stay * at.weight;
-      }
-      if (!sampled && kept > 1) rank = -1;
-      // (a cut among tokens of weight 0 cuts nothing; a lone token is looked up as the sample)
-      if (!ends || kept == 1 || cut == 0xff80u) cut_rank = -1;
-    }
-    if (lane == 0) {
-      s.top = top;
-      s.cut = bf16_bits_to_f32(cut);
-      s.cut_value = cut;
-      s.kept = kept;
-      s.total = total;
-      s.value = value;
-      s.rank = rank;
-      s.cut_rank = cut_rank;
-    }
+  if (s.nan) return nan_row(row, s);  // uniform
+  if (wave == 0) decide(f, row.V, groups, heavies, s);
+  __syncthreads();
+  return look_up(row.V, s, [&](uint32_t value, uint32_t rank) { find_token(row, 0, row.vecs, value, rank, s); });
+}
+
+// A row in parts, each counted by a workgroup of its own (at most kSafeSteps
+// steps, so that 16 bits hold every count): which groups occur, and the words
+// of those that do.
+struct Part {
+  uint32_t occurs[kGroups / 32];
+  uint32_t word[kGroups * 64];
+};
+
+__device__ __forceinline__ int part_vecs(const Row& row, int parts) { return (row.vecs + parts - 1) / parts; }
+
+__device__ __forceinline__ void count_part(const Row& row, int part, int parts, uint32_t* bin, Part* out) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int per = part_vecs(row, parts), lo = part * per, hi = min(lo + per, row.vecs);
+  clear_bins(bin);
+  lds_barrier();
+  uint32_t heavy = ~0u, many = 0;
+  if (lo < hi)
+    each_vec(row, lo, hi, [&](int, const u32x4& v, bool in) {
+      if (in) count_vec(bin, v, heavy, many);
+    });
+  heavy = (uint32_t)__builtin_amdgcn_readfirstlane((int)heavy);
+  many = (uint32_t)__builtin_amdgcn_readfirstlane((int)many);
+  if (lane == 0 && many) atomicAdd(&bin[heavy >> 1], many << ((heavy & 1) << 4));
+  __syncthreads();
+  const uint32_t has = own_groups(bin, [&](int g, uint32_t w) { out->word[64 * g + lane] = w; });
+  if (lane == 0) out->occurs[wave] = has;
+}
+
+// filter_row for bf16, from the counts of a row's parts.
+__device__ __forceinline__ RowCut merge_row(const Row& row, Settings f, const Part* in, int parts, CountLds& s) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid < kGroups / 32 * parts) s.part_occurs[tid] = in[tid / (kGroups / 32)].occurs[tid % (kGroups / 32)];
+  if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
+  if (tid == 0) {
+    s.nan = s.heavies = 0;
+    s.slots = 0;
+    s.bin[0x4000] = 0;  // (read with the word of +0, whether its own group occurs or not)
   }
   __syncthreads();
-  out.top = s.top;
-  out.cut = s.cut;
-  out.kept = s.kept;
-  out.total = s.total;
-  const int rank = s.rank, cut_rank = s.cut_rank;
-  const bool empty = s.top == -__builtin_inff();  // nothing above it: the first token
-  const uint32_t value = s.value, cut_value = s.cut_value;
-#pragma unroll 1
-  for (int which = 0; which < 2; ++which) {
-    const int r = which ? cut_rank : rank;
-    if (r < 0 || empty) continue;  // uniform
-    find_token(held, row, skew, V, vecs, steps, which ? cut_value : value, (uint32_t)r, s);
-    if (which) out.last = s.index;
-    else out.token = s.index;
+  uint32_t occurs = 0;
+  if (lane < kGroups / 32) {
+#pragma unroll 8
+    for (int c = 0; c < parts; ++c) occurs |= s.part_occurs[c * (kGroups / 32) + lane];
   }
-  if (out.kept == 1) out.last = out.token;
-  return out;
+  if (wave == 0 && lane < kGroups / 32) s.occurs[lane] = occurs;
+  if (lane == kGroups / 64 - 1 && (lane_u32(occurs, kGroups / 64) & 1)) occurs |= 1u << 31;  // (+0's group where there is -0)
+  const uint32_t upto = wave_scan((uint32_t)__popc(occurs));
+  const int groups = (int)lane_u32(upto, 63);
+#pragma unroll 1
+  for (int n = wave; n < groups; n += kRowWaves) {
+    const int g = nth_group(n, occurs, upto);
+    // parts that have it (the word of one that has not is whatever the memory held)
+    const uint64_t have = __ballot(lane < parts && ((s.part_occurs[min(lane, parts - 1) * (kGroups / 32) + (g >> 5)] >> (g & 31)) & 1));
+    uint32_t lo = 0, hi = 0;
+#pragma unroll 1
+    for (int c0 = 0; c0 < parts; c0 += 8) {
+      uint32_t w[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = in[min(c0 + j, parts - 1)].word[64 * g + lane];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool has = (have >> (c0 + j)) & 1;
+        lo += has ? w[j] & 0xffffu : 0u;
+        hi += has ? w[j] >> 16 : 0u;
+      }
+    }
+    const int64_t word = g >= kGroups / 2 ? 64 * g + lane : 64 * (kGroups / 2 - 1 - g) + 63 - lane;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t& c = half ? hi : lo;
+      if (c < 65536) continue;  // (rows of one value mostly)
+      const int at = atomicAdd(&s.heavies, 1);
+      s.heavy[at] = 2 * (uint32_t)word + half;
+      s.heavy_count[at] = c;
+      c = 0;
+    }
+    s.bin[word] = lo | (hi << 16);
+  }
+  f.inv_t = is_greedy(f.T) ? 1.0 : 1.0 / (double)f.T;
+  __syncthreads();
+  const int heavies = s.heavies;
+  weigh_groups(f.inv_t, heavies, s);
+  __syncthreads();
+  if (s.nan) return nan_row(row, s);  // uniform
+  if (wave == 0) decide(f, row.V, groups, heavies, s);
+  __syncthreads();
+  return look_up(row.V, s, [&](uint32_t value, uint32_t rank) {
+    // the part that holds the token, by its counts of the value
+    uint32_t c = 0;
+    auto count = [&](uint32_t v) {
+      const int g = group_of(v);
+      if (lane >= parts || !((s.part_occurs[lane * (kGroups / 32) + (g >> 5)] >> (g & 31)) & 1)) return;
+      const uint32_t w = v >> 1, at = g >= kGroups / 2 ? w & 63 : 63 - (w & 63);
+      const uint32_t both = in[lane].word[64 * g + at];
+      c += (v & 1) ? both >> 16 : both & 0xffffu;
+    };
+    count(value);
+    if (value == 0) count(0x8000u);
+    const uint32_t upto_c = wave_scan(c);
+    const int part = max(__ffsll((long long)__ballot(upto_c > rank)) - 1, 0);
+    const int per = part_vecs(row, parts), lo = part * per;
+    find_token(row, lo, min(lo + per, row.vecs), value, rank - lane_u32(upto_c - c, part), s);
+  });
 }
 
 // probability of token i of logit x
@@ -954,54 +1096,84 @@ __device__ __forceinline__ double prob_of(const RowCut& c, float x, int i, doubl
   return in ? weight_of(x, c.top, inv_t, tab) / c.total : 0.0;
 }
 
-template <typename T> union RowScratch;
-template <> union RowScratch<float> {
-  RowLds radix;
+// The row of workgroup (r, b): where it lies, and what is wanted of it.
+struct Job {
+  int64_t at;       // elements, from `target` or `draft`
+  int64_t u;        // its number among the uniforms
+  bool active, is_draft, sampled, ends;
+  int draft;        // the draft that its probability is wanted of; -1: none
 };
-template <> union RowScratch<uint16_t> {
-  CountLds counts;
-};
-
-__device__ __forceinline__ RowCut work_out(const FilterArgs& a, int b, const float* row, bool sampled, float u, bool ends,
-                                           RowScratch<float>& s) {
-  return filter_row<float>(a, b, row, sampled, u, ends, s.radix);
-}
-__device__ __forceinline__ RowCut work_out(const FilterArgs& a, int b, const uint16_t* row, bool sampled, float u, bool ends,
-                                           RowScratch<uint16_t>& s) {
-  return count_row(a, b, row, sampled, u, ends, s.counts);
-}
-
-// grid (rows per sequence, B): target rows, then draft rows
-template <typename T>
-__global__ __launch_bounds__(kRowThreads) void filter_rows_kernel(FilterArgs a) {
-  __shared__ RowScratch<T> s;
-  const int b = blockIdx.y, r = blockIdx.x;
-  if (a.K < 0) {
-    const RowCut c = work_out(a, b, (const T*)a.target + (int64_t)b * a.t_seq, true, a.uniforms[b], false, s);
-    if (threadIdx.x == 0) {
-      a.tokens[(int64_t)b * a.out_stride] = c.token;
-      if (a.kept) a.kept[b] = c.kept;
-    }
-    return;
-  }
+__device__ __forceinline__ Job job_of(const FilterArgs& a, int r, int b) {
+  if (a.K < 0) return Job{(int64_t)b * a.t_seq, b, true, false, true, false, -1};
   const int kb = draft_count(a, b);
   const bool rows = by_rows(a, b), is_draft = r > a.K;
   const int i = is_draft ? r - a.K - 1 : r;
-  if (is_draft ? !rows || i >= kb : i > kb) return;  // uniform
-  const T* row = is_draft ? (const T*)a.draft + draft_at(a, b, i)
-                          : (const T*)a.target + (int64_t)b * a.t_seq + (int64_t)i * a.t_row;
-  const bool sampled = !rows || i == kb;
-  const float u = a.uniforms[(int64_t)b * (a.K + 1) + (rows ? a.K : i)];
-  const RowCut c = work_out(a, b, row, sampled, u, !sampled, s);
+  Job j;
+  j.at = is_draft ? draft_at(a, b, i) : (int64_t)b * a.t_seq + (int64_t)i * a.t_row;
+  j.u = (int64_t)b * (a.K + 1) + (rows ? a.K : i);
+  j.active = is_draft ? rows && i < kb : i <= kb;
+  j.is_draft = is_draft;
+  j.sampled = !rows || i == kb;
+  j.ends = !j.sampled;
+  j.draft = rows && i < kb ? i : -1;
+  return j;
+}
+
+template <typename T>
+__device__ __forceinline__ void put_row(const FilterArgs& a, int r, int b, const Job& j, const T* row, const RowCut& c) {
   if (threadIdx.x != 0) return;
+  if (a.K < 0) {
+    a.tokens[(int64_t)b * a.out_stride] = c.token;
+    if (a.kept) a.kept[b] = c.kept;
+    return;
+  }
   const int64_t at = (int64_t)b * (2 * a.K + 1) + r;
   a.cuts[at] = c;
-  if (rows && i < kb) {
-    const int32_t d = a.drafts[(int64_t)b * a.K + i];
+  if (j.draft >= 0) {
+    const int32_t d = a.drafts[(int64_t)b * a.K + j.draft];
     const bool in = d >= 0 && d < a.V;  // a token outside the vocabulary has probability 0
     const double inv_t = 1.0 / (double)a.temperature[b];
     a.probs[at] = in ? prob_of(c, Elem<T>::get(row[d]), d, inv_t, kExp2Frac256) : 0.0;
   }
+}
+
+// grid (rows per sequence, B): target rows, then draft rows
+__global__ __launch_bounds__(kRowThreads) void filter_rows_f32_kernel(FilterArgs a) {
+  __shared__ RowLds s;
+  const int r = blockIdx.x, b = blockIdx.y;
+  const Job j = job_of(a, r, b);
+  if (!j.active) return;  // uniform
+  const float* row = (const float*)(j.is_draft ? a.draft : a.target) + j.at;
+  put_row(a, r, b, j, row, filter_row<float>(a, b, row, j.sampled, a.uniforms[j.u], j.ends, s));
+}
+
+__global__ __launch_bounds__(kRowThreads) void filter_rows_bf16_kernel(FilterArgs a) {
+  __shared__ CountLds s;
+  const int r = blockIdx.x, b = blockIdx.y;
+  const Job j = job_of(a, r, b);
+  if (!j.active) return;  // uniform
+  const uint16_t* row = (const uint16_t*)(j.is_draft ? a.draft : a.target) + j.at;
+  put_row(a, r, b, j, row, count_row(Row(row, a.V), settings_of(a, b, j.sampled, j.u, j.ends), s));
+}
+
+// grid (parts, rows per sequence, B)
+__global__ __launch_bounds__(kRowThreads) void filter_parts_kernel(FilterArgs a) {
+  __shared__ uint32_t bin[32768];
+  const int r = blockIdx.y, b = blockIdx.z;
+  const Job j = job_of(a, r, b);
+  if (!j.active) return;  // uniform
+  const uint16_t* row = (const uint16_t*)(j.is_draft ? a.draft : a.target) + j.at;
+  count_part(Row(row, a.V), blockIdx.x, gridDim.x, bin, a.row_parts + ((int64_t)b * gridDim.y + r) * gridDim.x + blockIdx.x);
+}
+// grid (rows per sequence, B)
+__global__ __launch_bounds__(kRowThreads) void filter_merge_kernel(FilterArgs a) {
+  __shared__ CountLds s;
+  const int r = blockIdx.x, b = blockIdx.y;
+  const Job j = job_of(a, r, b);
+  if (!j.active) return;  // uniform
+  const uint16_t* row = (const uint16_t*)(j.is_draft ? a.draft : a.target) + j.at;
+  const Part* in = a.row_parts + ((int64_t)b * gridDim.x + r) * a.split;
+  put_row(a, r, b, j, row, merge_row(Row(row, a.V), settings_of(a, b, j.sampled, j.u, j.ends), in, a.split, s));
 }
 
 // drafts accepted before the first refused (a whole wave)
@@ -1171,36 +1343,72 @@ int weight_shift(int V) {
 size_t a256(size_t x) { return (x + 255) & ~(size_t)255; }
 int residual_chunks(int V) { return (V + kChunk - 1) / kChunk; }
 
+// Workgroups that count a bf16 row, each a part of it; 1: one workgroup does
+// the whole row.  Up to 256 workgroups share few rows (one row of 151,936
+// TIME1), as long as the parts' counts stay under 64 MiB.
+int row_split(int rows, int V, int dtype) {
+  if (dtype != NSV_BF16 || rows <= 0) return 1;
+  const int least = (V + 7 + kSafeSteps * kStep - 1) / (kSafeSteps * kStep);
+  int n = kMaxSplit;
+  while (n > 1 && (rows * n > 256 || V < n * kStep)) n >>= 1;
+  if (n < least) n = least;
+  return n > 1 && rows * n <= 512 && n <= kMaxParts ? n : 1;
+}
+size_t parts_bytes(int rows, int V, int dtype) {
+  const int n = row_split(rows, V, dtype);
+  return n > 1 ? (size_t)rows * n * sizeof(Part) : 0;
+}
+
 struct Layout {
-  size_t cuts, probs, parts, total;
+  size_t cuts, probs, parts, row_parts, total;
 };
-Layout layout(int B, int K, int V) {
+Layout layout(int B, int K, int V, int dtype, bool draft_rows) {
   Layout L;
   const size_t rows = (size_t)B * (2 * (size_t)K + 1);
   L.cuts = 0;
   L.probs = a256(rows * sizeof(RowCut));
   L.parts = L.probs + a256(rows * sizeof(double));
-  L.total = L.parts + a256((size_t)B * residual_chunks(V) * 2 * sizeof(double));
+  L.row_parts = L.parts + a256((size_t)B * residual_chunks(V) * 2 * sizeof(double));
+  L.total = L.row_parts + parts_bytes(B * (draft_rows ? 2 * K + 1 : K + 1), V, dtype);
   return L;
 }
 
-void launch_rows(const FilterArgs& a, int rows, int dtype, hipStream_t s) {
-  const dim3 grid(rows, a.B);
-  if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_rows_kernel<uint16_t>, grid, dim3(kRowThreads), 0, s, a);
-  else hipLaunchKernelGGL(filter_rows_kernel<float>, grid, dim3(kRowThreads), 0, s, a);
+int launch_rows(FilterArgs& a, int rows, int dtype, char* row_parts, hipStream_t s) {
+  a.split = row_split(rows * a.B, a.V, dtype);
+  a.row_parts = (Part*)row_parts;
+  const dim3 grid(rows, a.B), block(kRowThreads);
+  if (dtype == NSV_F32) {
+    hipLaunchKernelGGL(filter_rows_f32_kernel, grid, block, 0, s, a);
+  } else if (a.split == 1) {
+    hipLaunchKernelGGL(filter_rows_bf16_kernel, grid, block, 0, s, a);
+  } else {
+    hipLaunchKernelGGL(filter_parts_kernel, dim3(a.split, rows, a.B), block, 0, s, a);
+    const int rc = nsv_launch_status();
+    if (rc) return rc;
+    hipLaunchKernelGGL(filter_merge_kernel, grid, block, 0, s, a);
+  }
+  return nsv_launch_status();
 }
 
 }  // namespace
 
 extern "C" {
 
+size_t nsv_sample_filtered_workspace_size(int B, int V, int dtype) {
+  if (bad_rows(B, V, dtype) || V > kMaxVocab || B > 65535) return 0;
+  return parts_bytes(B, V, dtype);
+}
+
 int nsv_sample_filtered(const void* logits, int64_t row_stride, const float* temperature, const int32_t* top_k,
                         const float* top_p, const float* min_p, const float* uniforms, int B, int V, int dtype,
-                        int32_t* out_tokens, int64_t out_stride, int32_t* kept, void* stream) {
+                        int32_t* out_tokens, int64_t out_stride, int32_t* kept, void* workspace, size_t workspace_bytes,
+                        void* stream) {
   if (bad_rows(B, V, dtype) || row_stride < V || out_stride < 1) return NSV_ERR_ARG;
   if (V > kMaxVocab || B > 65535) return NSV_ERR_UNSUPPORTED;
   if (B == 0) return NSV_OK;
   if (!logits || !temperature || !uniforms || !out_tokens) return NSV_ERR_ARG;
+  const size_t need = parts_bytes(B, V, dtype);
+  if (need && (!workspace || workspace_bytes < need)) return NSV_ERR_WORKSPACE;
   FilterArgs a{};
   a.target = logits;
   a.t_seq = row_stride;
@@ -1216,13 +1424,13 @@ int nsv_sample_filtered(const void* logits, int64_t row_stride, const float* tem
   a.tokens = out_tokens;
   a.out_stride = out_stride;
   a.kept = kept;
-  launch_rows(a, 1, dtype, (hipStream_t)stream);
-  return nsv_launch_status();
+  return launch_rows(a, 1, dtype, (char*)workspace, (hipStream_t)stream);
 }
 
-size_t nsv_accept_filtered_workspace_size(int B, int K, int V) {
-  if (B < 0 || K < 0 || K > kMaxDrafts || V <= 0) return 0;
-  return layout(B, K, V).total;
+size_t nsv_accept_filtered_workspace_size(int B, int K, int V, int dtype) {
+  if (bad_rows(B, V, dtype) || K < 0 || K > kMaxDrafts || V > kMaxVocab || B > 65535) return 0;
+  const size_t x = layout(B, K, V, dtype, false).total, y = layout(B, K, V, dtype, true).total;
+  return x > y ? x : y;  // (with draft rows or without)
 }
 
 int nsv_accept_filtered(const void* target_logits, int64_t target_seq_stride, const void* draft_logits,
@@ -1237,8 +1445,8 @@ int nsv_accept_filtered(const void* target_logits, int64_t target_seq_stride, co
   if (B == 0) return NSV_OK;
   if (!target_logits || (!drafts && K > 0) || !num_drafts || !temperature || !uniforms || !out_tokens || !out_len)
     return NSV_ERR_ARG;
-  const Layout L = layout(B, K, V);
-  if (!workspace || workspace_bytes < L.total) return NSV_ERR_WORKSPACE;
+  const Layout L = layout(B, K, V, dtype, K > 0 && draft_logits);
+  if (!workspace || workspace_bytes < nsv_accept_filtered_workspace_size(B, K, V, dtype)) return NSV_ERR_WORKSPACE;
   FilterArgs a{};
   a.target = target_logits;
   a.t_seq = target_seq_stride * V;
@@ -1265,8 +1473,7 @@ int nsv_accept_filtered(const void* target_logits, int64_t target_seq_stride, co
   a.out_tokens = out_tokens;
   a.out_len = out_len;
   hipStream_t s = (hipStream_t)stream;
-  launch_rows(a, a.draft ? 2 * K + 1 : K + 1, dtype, s);
-  int rc = nsv_launch_status();
+  int rc = launch_rows(a, a.draft ? 2 * K + 1 : K + 1, dtype, (char*)workspace + L.row_parts, s);
   if (rc) return rc;
   if (a.draft) {
     const dim3 grid(a.chunks, B);

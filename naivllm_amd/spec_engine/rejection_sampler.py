@@ -22,6 +22,8 @@ from one uniform number per draw.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from naivllm_amd import _lib
@@ -226,6 +228,16 @@ def _check_out(t: torch.Tensor, shape: tuple, device, name: str, strided: bool =
         raise ValueError(f"{name} must be contiguous")
 
 
+@functools.lru_cache(maxsize=256)
+def _sample_filtered_bytes(*shape: int) -> int:
+    return int(_lib.lib().nsv_sample_filtered_workspace_size(*shape))
+
+
+@functools.lru_cache(maxsize=256)
+def _accept_filtered_bytes(*shape: int) -> int:
+    return int(_lib.lib().nsv_accept_filtered_workspace_size(*shape))
+
+
 def sample_filtered(logits: torch.Tensor, temperature, uniforms: torch.Tensor, top_k=None, top_p=None, min_p=None,
                     out: torch.Tensor | None = None, kept: torch.Tensor | None = None) -> torch.Tensor:
     """Samples a token of every row under a temperature, top-k, top-p and
@@ -268,11 +280,17 @@ def sample_filtered(logits: torch.Tensor, temperature, uniforms: torch.Tensor, t
         _check_out(out, (B,), dev, "out", strided=True)
     if kept is not None:
         _check_out(kept, (B,), dev, "kept")
+    h, code = _lib.lib(), _lib.dtype_code(logits.dtype)
+    nbytes = _sample_filtered_bytes(B, V, code)
     with _lib.on_device(dev):
-        rc = _lib.lib().nsv_sample_filtered(
-            logits.data_ptr(), pitch, temperature.data_ptr(), _lib.ptr(top_k), _lib.ptr(top_p), _lib.ptr(min_p),
-            uniforms.data_ptr(), B, V, _lib.dtype_code(logits.dtype), out.data_ptr(), out.stride(0) if B > 1 else 1,
-            _lib.ptr(kept), _lib.stream_ptr(dev))
+        stream = _lib.stream_ptr(dev)
+        scratch = _lib.stream_scratch(dev, stream)
+        with scratch.lock:
+            ws = scratch.take(nbytes)
+            rc = h.nsv_sample_filtered(
+                logits.data_ptr(), pitch, temperature.data_ptr(), _lib.ptr(top_k), _lib.ptr(top_p), _lib.ptr(min_p),
+                uniforms.data_ptr(), B, V, code, out.data_ptr(), out.stride(0) if B > 1 else 1, _lib.ptr(kept),
+                ws.data_ptr(), nbytes, stream)
     _lib.check(rc, "sample_filtered")
     return out
 
@@ -345,8 +363,8 @@ def accept_filtered(target_logits: torch.Tensor, drafts: torch.Tensor, num_draft
         out_len = torch.empty(B, dtype=torch.int32, device=dev)
     else:
         _check_out(out_len, (B,), dev, "out_len")
-    h = _lib.lib()
-    nbytes = int(h.nsv_accept_filtered_workspace_size(B, K, V))
+    h, code = _lib.lib(), _lib.dtype_code(target_logits.dtype)
+    nbytes = _accept_filtered_bytes(B, K, V, code)
     with _lib.on_device(dev):
         stream = _lib.stream_ptr(dev)
         scratch = _lib.stream_scratch(dev, stream)
@@ -355,7 +373,7 @@ def accept_filtered(target_logits: torch.Tensor, drafts: torch.Tensor, num_draft
             rc = h.nsv_accept_filtered(
                 target_logits.data_ptr(), target_seq_stride, _lib.ptr(draft_logits), draft_seq_stride, draft_row_stride,
                 _lib.ptr(draft_mode), drafts.data_ptr(), num_drafts.data_ptr(), temperature.data_ptr(), _lib.ptr(top_k),
-                _lib.ptr(top_p), _lib.ptr(min_p), uniforms.data_ptr(), B, K, V, _lib.dtype_code(target_logits.dtype),
+                _lib.ptr(top_p), _lib.ptr(min_p), uniforms.data_ptr(), B, K, V, code,
                 out_tokens.data_ptr(), out_len.data_ptr(), ws.data_ptr(), nbytes, stream)
     _lib.check(rc, "accept_filtered")
     return out_tokens, out_len

@@ -12,9 +12,10 @@ P = ctypes.c_void_p(0x1000)  # any address: refused calls touch nothing
 ARG, UNSUPPORTED, WORKSPACE = -1, -2, -3
 
 
-def _sample(logits=P, pitch=100, temperature=P, uniforms=P, B=2, V=100, dtype=1, out=P, stride=1):
+def _sample(logits=P, pitch=100, temperature=P, uniforms=P, B=2, V=100, dtype=1, out=P, stride=1,
+            ws=P, ws_bytes=1 << 30):
     return _lib.lib().nsv_sample_filtered(logits, pitch, temperature, None, None, None, uniforms, B, V, dtype, out, stride,
-                                          None, None)
+                                          None, ws, ws_bytes, None)
 
 
 def _accept(target=P, t_stride=4, draft=P, d_seq=3, d_row=1, mode=None, drafts=P, live=P, temperature=P, uniforms=P, B=2,
@@ -33,6 +34,10 @@ def test_sample_shapes():
     assert _sample(V=(1 << 20) + 1, pitch=1 << 21) == UNSUPPORTED
     assert _sample(B=65536) == UNSUPPORTED
     assert _sample(B=0) == 0
+    size = _lib.lib().nsv_sample_filtered_workspace_size
+    need = size(2, 151936, 1)
+    assert need > 0 and size(2, 151936, 0) == size(2, (1 << 20) + 1, 1) == size(-1, 100, 1) == 0
+    assert _sample(V=151936, pitch=151936, ws=None) == _sample(V=151936, pitch=151936, ws_bytes=need - 1) == WORKSPACE
 
 
 @pytest.mark.parametrize("bad", [dict(target=None), dict(drafts=None), dict(live=None), dict(temperature=None),
@@ -47,9 +52,9 @@ def test_accept_shapes_and_workspace():
     h = _lib.lib()
     assert _accept(V=(1 << 20) + 1) == UNSUPPORTED and _accept(B=65536) == UNSUPPORTED
     assert _accept(B=0) == 0
-    need = h.nsv_accept_filtered_workspace_size(2, 3, 100)
+    need = h.nsv_accept_filtered_workspace_size(2, 3, 100, 1)
     assert need > 0 and _accept(ws_bytes=need - 1) == WORKSPACE and _accept(ws=None) == WORKSPACE
-    assert h.nsv_accept_filtered_workspace_size(2, 64, 100) == 0 and h.nsv_accept_filtered_workspace_size(-1, 3, 100) == 0
+    assert h.nsv_accept_filtered_workspace_size(2, 64, 100, 1) == 0 and h.nsv_accept_filtered_workspace_size(-1, 3, 100, 1) == 0
 
 
 def test_tensors_on_the_cpu_are_refused():

@@ -137,6 +137,20 @@ def test_values_of_most_tokens(dtype):
     for n, more in enumerate((dict(), dict(top_p=np.full(6, 0.7, np.float32)), dict(top_k=np.full(6, 150000, np.int32)),
                               dict(min_p=np.full(6, 0.01, np.float32)))):
         assert _check(x, dict(f, **more), _uniforms(n, 6)) == 6
+        # so many rows that one workgroup does a whole one
+        f15 = on_gpu({k: np.tile(v, 15) for k, v in dict(f, **more).items()})
+        kept = torch.zeros(90, dtype=torch.int32, device="cuda")
+        got = sample_filtered(x.cuda().repeat(15, 1), uniforms=torch.from_numpy(np.tile(_uniforms(n, 6), 15)).cuda(), kept=kept, **f15)
+        assert (got.view(15, 6) == got[:6]).all() and (kept.view(15, 6) == kept[:6]).all()
+        assert _check(x, dict(f, **more), _uniforms(n, 6), got[:6], kept[:6]) == 6
+
+
+@pytest.mark.parametrize("B,V", [(33, 16384), (65, 20011), (129, 20011), (300, 9001), (260, 70001)])
+def test_many_rows(B, V):
+    """Rows counted in parts, and whole ones."""
+    print(f"case: sample_filtered {B} rows of {V}", flush=True)
+    for shape in ("peaked", "levels"):
+        assert _check(logits(B, B, V, "bf16", shape), settings(B, B), _uniforms(B, B)) == B
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
