@@ -1,145 +1,33 @@
-// Sampling and acceptance of drafts under a temperature, top-k, top-p and
-// min-p, for gfx950.  No reference counterpart (its sampler has a temperature
-// only); the operators stand beside nsv_sample and nsv_accept_stochastic.
+// Rows under a temperature, top-k, top-p and min-p (filter.h): what the filters
+// leave of each, and its sample, for gfx950.
 //
-// Of a row x with maximum M and temperature T the weights are
-// w = exp((x - M) / T) (1 where x = M, 0 where x = -inf), and its tokens are
-// ordered by falling x, equal ones by rising index.  Each filter leaves a
-// beginning of that order: top-k its first k; top-p the fewest whose sum
-// reaches p times the sum that top-k left; min-p those with w >= min_p.  So
-// what all of them leave is described by its last token: a value, and an index
-// among the tokens of that value.  The sample of u is the first token whose
-// running sum along the order exceeds u W, W the sum of what is left: one
-// uniform number per row, and no noise of the vocabulary's size to draw and
-// read.  T <= 1e-6, and rows with a NaN or without a value above -inf, leave
-// the argmax alone (first maximum, NaN above all, torch's rule).
-//
-// filter_rows_kernel works one row out per workgroup.
-//   bf16 (count_row): a row has few distinct values, so one pass counts the
-//     tokens of each of the 65,536 in LDS (16 bits each), and everything else
-//     comes from the counts: a value's tokens weigh count * w, one exponential
-//     per value that occurs (some 3,000) instead of one per token.  The row
-//     stays in registers, where the sampled token is found by its value and
-//     its rank among the tokens of that value.
-//   fp32 (filter_row): a value is found by radix descent over its
-//     order-preserving bits: per level a histogram in LDS of the row's tokens
-//     below the prefix so far, counts and weights, and a scan of its bins.
-//     Weights are added up as 64-bit integers, w 2^s rounded, so sums do not
-//     depend on the order of the additions; s leaves room for the vocabulary
-//     (44 bits for 2^18 tokens), each weight off by 2^-45 of the largest, where
-//     fp32 sums would move the sample of one row in a hundred.
+// Two kernels.  The first cuts a row into parts, a workgroup each, and leaves
+// what a part holds of each value, or of each narrow range of values; the
+// second, a workgroup per row, adds the parts up, finds the cuts and the
+// sample's value along the order, and the sample's index in the row.
+//   bf16: a row has few distinct values, so the first kernel counts the tokens
+//     of each of the 65,536 in LDS (16 bits each), and everything else comes
+//     from the counts: a value's tokens weigh count * w, one exponential per
+//     value that occurs (some 3,000) instead of one per token.  The sampled
+//     token is found by its value and its rank among the tokens of that value,
+//     in the part that holds it.
+//   fp32: 8,192 bins of equal leading bits, counts and weights.  Weights are
+//     added up as 64-bit integers, w 2^s rounded, so sums do not depend on the
+//     order of the additions; s leaves room for the vocabulary (44 bits for
+//     2^18 tokens), each weight off by 2^-45 of the largest, where fp32 sums
+//     would move the sample of one row in a hundred.  The second kernel lists
+//     the tokens of the few bins that matter and looks at those.  A row whose
+//     list is too long (many equal values) or that holds a NaN goes by radix
+//     descent over its order-preserving bits, a pass over the row per level.
 
-#include "common.h"
-#include "exp_f64.h"
+#include "filter.h"
+
+using namespace nsv_filter;
 
 namespace {
 
-constexpr int kRowThreads = 1024;
-constexpr int kRowWaves = kRowThreads / 64;
 constexpr int kBins = 2048;
-constexpr int kVec = 8;                          // elements a thread takes at a time
-constexpr int kStep = kRowThreads * kVec;        // elements a workgroup takes at a time
-constexpr int kMaxVocab = 1 << 20;
 constexpr int kMaxSteps = kMaxVocab / kStep + 1; // (a row that starts off a 16-byte boundary)
-constexpr int kMaxDrafts = 63;                   // K + 1 rows fit one 64-lane ballot
-constexpr int kChunkThreads = 256;
-constexpr int kChunk = kChunkThreads * kVec;     // of the residual passes
-
-struct Part;
-template <typename T> struct Elem;
-template <> struct Elem<uint16_t> {  // bf16 bits
-  __device__ static float get(uint16_t v) { return bf16_bits_to_f32(v); }
-  __device__ static float unpack(const u32x4& w, int e) {
-    return bf16_bits_to_f32((e & 1) ? (w[e >> 1] >> 16) : (w[e >> 1] & 0xffffu));
-  }
-};
-template <> struct Elem<float> {
-  __device__ static float get(float v) { return v; }
-  __device__ static float unpack(const u32x4& w, int e) { return __uint_as_float(w[e]); }
-};
-
-// What the filters leave of a row: tokens of x > cut, and of x == cut up to
-// the index `last`; top: the row's maximum; total: W; kept: how many.  kept 1
-// is `token` alone, whatever the row holds.
-struct RowCut {
-  float top, cut;
-  int32_t last, kept, token, pad;
-  double total;
-};
-
-struct FilterArgs {
-  const void* target;      // row r of sequence b at b * t_seq + r * t_row elements
-  int64_t t_seq, t_row;
-  const void* draft;       // nullable; row i of sequence b at (b * d_seq + i * d_row) * V
-  int64_t d_seq, d_row;
-  int B, K, V;             // K -1: the sampler (one row per sequence, one uniform)
-  int shift;               // weights are held as integers, w 2^shift
-  const float* temperature;
-  const int32_t* top_k;    // nullable
-  const float* top_p;      // nullable
-  const float* min_p;      // nullable
-  const float* uniforms;   // [B, K + 1]
-  const int32_t* drafts;   // [B, K]
-  const int32_t* num_drafts;
-  const int32_t* mode;     // nullable; 0: sequence b has no draft rows
-  RowCut* cuts;            // [B, 2K + 1]: target rows 0..K, then draft rows
-  double* probs;           // [B, 2K + 1]: the probability of the row's draft
-  Part* row_parts;         // [B, rows per sequence, split]
-  int split;
-  double* parts;           // [B, chunks, 2]: sums of the residual and of p_target
-  int chunks;
-  int32_t* tokens;         // sampler: row b's at b * out_stride
-  int64_t out_stride;
-  int32_t* kept;           // sampler, nullable
-  int32_t* out_tokens;     // [B, K + 1]
-  int32_t* out_len;
-};
-
-__device__ __forceinline__ bool is_greedy(float T) { return !(T > 1e-6f); }
-// u of the sample's goal u W: what is no number in [0, 1] is taken to its end
-__device__ __forceinline__ double unit(float u) { return fmin(fmax((double)u, 0.0), 1.0); }
-// sequence b's drafts are decided by their probabilities
-__device__ __forceinline__ bool by_rows(const FilterArgs& a, int b) {
-  return a.draft && !(a.mode && a.mode[b] == 0) && !is_greedy(a.temperature[b]);
-}
-__device__ __forceinline__ int draft_count(const FilterArgs& a, int b) { return min(max(a.num_drafts[b], 0), a.K); }
-__device__ __forceinline__ int64_t draft_at(const FilterArgs& a, int b, int i) {
-  return ((int64_t)b * a.d_seq + (int64_t)i * a.d_row) * a.V;
-}
-
-// order-preserving bits, complemented: rising along the order of the tokens;
-// -0 as +0
-__device__ __forceinline__ uint32_t order_bits(float x) {
-  const uint32_t u = __float_as_uint(x + 0.f);
-  return (u & 0x80000000u) ? u : ~(u | 0x80000000u);
-}
-__device__ __forceinline__ float order_value(uint32_t k) {
-  return __uint_as_float((k & 0x80000000u) ? k : ~(k | 0x80000000u));
-}
-
-__device__ __forceinline__ double weight_of(float x, float top, double inv_t, const double* tab) {
-  return x == top ? 1.0 : nsv_exp_nonpos(((double)x - (double)top) * inv_t, tab);
-}
-// w 2^shift, rounded: added to 2^52 it lies in the low bits of the sum
-__device__ __forceinline__ uint64_t fixed_weight(double w, double scale) {
-  return (uint64_t)__double_as_longlong(fma(w, scale, 0x1p52)) & 0x000fffffffffffffull;
-}
-
-// elements base .. base + 7 of a row, those past its end -inf
-template <typename T>
-__device__ __forceinline__ void load_vec(const T* row, int64_t base, int V, float (&x)[kVec]) {
-  constexpr int PER = 16 / sizeof(T);
-  if (((uintptr_t)row & 15) == 0 && base + kVec <= V) {
-    u32x4 w[kVec / PER];
-#pragma unroll
-    for (int l = 0; l < kVec / PER; ++l) w[l] = *reinterpret_cast<const u32x4*>(row + base + l * PER);
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) x[e] = Elem<T>::unpack(w[e / PER], e % PER);
-  } else {
-#pragma unroll
-    for (int e = 0; e < kVec; ++e) x[e] = base + e < V ? Elem<T>::get(row[base + e]) : -__builtin_inff();
-  }
-}
 
 // f(index, x) of every element of a row, a workgroup's threads together
 template <typename T, typename F>
@@ -155,40 +43,9 @@ __device__ __forceinline__ void each(const T* row, int V, F f) {
   }
 }
 
-// Inclusive scan over a wave's 64 lanes on the VALU: within rows of 16 by
-// shifts of 1, 2, 4 and 8 lanes, then the last lane of row 0 and 2 to the row
-// behind it, and of row 1 to rows 2 and 3 (what has no source adds 0).  A
-// sixth of the shuffles' time, whose every step is a round trip through LDS.
-template <int CTRL, int ROWS, typename T>
-__device__ __forceinline__ T dpp_or_zero(T v) {
-  if constexpr (sizeof(T) == 4) {
-    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
-  } else {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
-    return __builtin_bit_cast(T, ((uint64_t)hi << 32) | lo);
-  }
-}
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {
-  v += dpp_or_zero<0x111, 0xf>(v);
-  v += dpp_or_zero<0x112, 0xf>(v);
-  v += dpp_or_zero<0x114, 0xf>(v);
-  v += dpp_or_zero<0x118, 0xf>(v);
-  v += dpp_or_zero<0x142, 0xa>(v);
-  v += dpp_or_zero<0x143, 0xc>(v);
-  return v;
-}
-// lane l's value (l uniform), and the lane's before a lane's own
-__device__ __forceinline__ double lane_f64(double v, int l) {
-  return __longlong_as_double((long long)lane_u64((uint64_t)__double_as_longlong(v), l));
-}
-template <typename T>
-__device__ __forceinline__ T lane_before(T v) {
-  return dpp_or_zero<0x138, 0xf>(v);  // the whole wave one lane up, 0 into the first
-}
-
+// ---------------------------------------------------------------------------
+// radix descent
+// ---------------------------------------------------------------------------
 struct RowLds {
   uint32_t count[kBins];
   unsigned long long mass[kBins];
@@ -435,15 +292,110 @@ __device__ RowCut filter_row(const FilterArgs& a, int b, const T* row, bool samp
 
 
 // ---------------------------------------------------------------------------
+// rows in parts
+// ---------------------------------------------------------------------------
+constexpr int kAhead = 4;      // vectors a thread loads ahead of those it works on
+constexpr int kMaxParts = 32;  // of a row, by a workgroup each ..
+constexpr int kMaxSplit = 8;   // .. and this many at most where one would do
+constexpr int kSlab = 1024;    // parts of a launch: their counts take 128 MiB at most
+
+// A row as 16-byte vectors of N elements: vector g holds elements N g - skew ..
+// + N - 1; what lies outside the row counts as -inf.
+template <typename T>
+struct Row {
+  static constexpr int N = 16 / sizeof(T);
+  const T* at;
+  int V, skew, vecs;
+  __device__ Row(const T* row, int V_) : at(row), V(V_), skew((int)(((uintptr_t)row & 15) / sizeof(T))) {
+    vecs = (V + skew + N - 1) / N;
+  }
+  __device__ __forceinline__ u32x4 load(int g) const {
+    const int64_t e0 = (int64_t)N * g - skew;
+    if (e0 >= 0 && e0 + N <= V) return *reinterpret_cast<const u32x4*>(at + e0);
+    u32x4 v;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 2) {
+        const int64_t a = e0 + 2 * i, b = a + 1;
+        const uint32_t lo = a >= 0 && a < V ? at[a] : 0xff80u, hi = b >= 0 && b < V ? at[b] : 0xff80u;
+        v[i] = lo | (hi << 16);
+      } else {
+        const int64_t a = e0 + i;
+        v[i] = a >= 0 && a < V ? __float_as_uint(at[a]) : 0xff800000u;
+      }
+    }
+    return v;
+  }
+};
+template <typename T>
+__device__ __forceinline__ int part_vecs(const Row<T>& row, int parts) { return (row.vecs + parts - 1) / parts; }
+
+// f(step, vector, whether there is one) of the vectors lo .. hi - 1, a
+// workgroup's threads together, kAhead of them loaded ahead.  The loop stays
+// rolled: a row kept in registers (one unrolled body per vector) saved its
+// second reading, and cost more in instructions fetched once.
+template <typename T, typename F>
+__device__ __forceinline__ void each_vec(const Row<T>& row, int lo, int hi, F f) {
+  const int steps = (hi - lo + kRowThreads - 1) / kRowThreads;
+  u32x4 v[kAhead];
+  int g = lo + threadIdx.x;
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j) v[j] = row.load(min(g + j * kRowThreads, hi - 1));
+#pragma unroll 1
+  for (int it = 0; it < steps; it += kAhead) {
+    u32x4 w[kAhead] = {};
+    if (it + kAhead < steps) {
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) w[j] = row.load(min(g + (kAhead + j) * kRowThreads, hi - 1));
+    }
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (it + j < steps) f(it + j, v[j], g + j * kRowThreads < hi);
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) v[j] = w[j];
+    g += kAhead * kRowThreads;
+  }
+}
+
+// What the filters of a row are, and what is wanted of it.
+struct Settings {
+  float T, p, least, u;
+  int k;
+  bool sampled, ends;
+  double inv_t;
+};
+// (as vector loads: scalar ones would be waited for with the LDS writes)
+__device__ __forceinline__ Settings settings_of(const FilterArgs& a, int b, bool sampled, int64_t at_u, bool ends) {
+  int vb = b;
+  int64_t vu = at_u;
+  asm volatile("" : "+v"(vb), "+v"(vu));
+  Settings f;
+  f.T = a.temperature[vb];
+  f.k = a.top_k ? a.top_k[vb] : 0;
+  f.p = a.top_p ? a.top_p[vb] : 1.f;
+  f.least = a.min_p ? a.min_p[vb] : 0.f;
+  f.u = a.uniforms[vu];
+  f.sampled = sampled;
+  f.ends = ends;
+  return f;
+}
+
+// .. for scalar registers and uniform branches
+__device__ __forceinline__ void make_uniform(Settings& f) {
+  auto one = [](float x) { return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(x))); };
+  f.T = one(f.T);
+  f.p = one(f.p);
+  f.least = one(f.least);
+  f.u = one(f.u);
+  f.k = __builtin_amdgcn_readfirstlane(f.k);
+}
+
+// ---------------------------------------------------------------------------
 // bf16 rows by counts
 // ---------------------------------------------------------------------------
 constexpr int kGroups = 512;   // of 128 values each, along the order of the tokens: 64 words of two counts
-constexpr int kAhead = 4;      // vectors a thread loads ahead of those it counts
-constexpr int kSafeSteps = 7;  // steps whose 57,344 tokens fit a 16-bit count beside ..
-constexpr uint32_t kFull = 65536 - kSafeSteps * kStep;  // .. fewer than these
-constexpr int kMaxHeavy = kRowWaves + kMaxVocab / kFull + 1;
-constexpr int kMaxParts = 32;  // of a row, counted by a workgroup each ..
-constexpr int kMaxSplit = 8;  // .. for speed this many
+constexpr int kSafeSteps = 7;  // steps of a workgroup whose 57,344 tokens fit a 16-bit count
+constexpr int kMaxHeavy = kMaxVocab / 65536 + 1;
 
 struct CountLds {
   uint32_t bin[32768];         // counts of values 2i (low half) and 2i + 1
@@ -459,7 +411,6 @@ struct CountLds {
   uint32_t heavy[kMaxHeavy], heavy_count[kMaxHeavy];  // counts beside the bins
   uint32_t part_occurs[kMaxParts * kGroups / 32];
   int heavies;
-  uint32_t slots;              // tokens counted
   int nan, index;
   // what wave 0 decides
   float top, cut;
@@ -467,55 +418,6 @@ struct CountLds {
   uint32_t value, cut_value;   // bits
   double total;
 };
-
-// A row as vectors of 8 elements on 16 bytes: vector g holds elements 8 g -
-// skew .. + 7; what lies outside the row counts as -inf.
-struct Row {
-  const uint16_t* at;
-  int V, skew, vecs;
-  __device__ Row(const uint16_t* row, int V_) : at(row), V(V_), skew((int)(((uintptr_t)row & 15) >> 1)) {
-    vecs = (V + skew + 7) / 8;
-  }
-  __device__ __forceinline__ u32x4 load(int g) const {
-    const int64_t e0 = (int64_t)8 * g - skew;
-    if (e0 >= 0 && e0 + 8 <= V) return *reinterpret_cast<const u32x4*>(at + e0);
-    u32x4 v;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t a = e0 + 2 * i, b = a + 1;
-      const uint32_t lo = a >= 0 && a < V ? at[a] : 0xff80u, hi = b >= 0 && b < V ? at[b] : 0xff80u;
-      v[i] = lo | (hi << 16);
-    }
-    return v;
-  }
-};
-
-// f(step, vector, whether there is one) of the vectors lo .. hi - 1, a
-// workgroup's threads together, kAhead of them loaded ahead.  The loop stays
-// rolled: a row kept in registers (one unrolled body per vector) saved its
-// second reading, and cost more in instructions fetched once.
-template <typename F>
-__device__ __forceinline__ void each_vec(const Row& row, int lo, int hi, F f) {
-  const int steps = (hi - lo + kRowThreads - 1) / kRowThreads;
-  u32x4 v[kAhead];
-  int g = lo + threadIdx.x;
-#pragma unroll
-  for (int j = 0; j < kAhead; ++j) v[j] = row.load(min(g + j * kRowThreads, hi - 1));
-#pragma unroll 1
-  for (int it = 0; it < steps; it += kAhead) {
-    u32x4 w[kAhead];
-    if (it + kAhead < steps) {
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) w[j] = row.load(min(g + (kAhead + j) * kRowThreads, hi - 1));
-    }
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (it + j < steps) f(it + j, v[j], g + j * kRowThreads < hi);
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) v[j] = w[j];
-    g += kAhead * kRowThreads;
-  }
-}
 
 __device__ __forceinline__ void count_value(uint32_t* bin, uint32_t bits) {
   atomicAdd(&bin[bits >> 1], 1u << ((bits & 1) << 4));
@@ -545,26 +447,6 @@ __device__ __forceinline__ void count_vec(uint32_t* bin, const u32x4& v, uint32_
 
 __device__ __forceinline__ void clear_bins(uint32_t* bin) {
   for (int i = threadIdx.x; i < 32768 / 4; i += kRowThreads) reinterpret_cast<u32x4*>(bin)[i] = u32x4{0u, 0u, 0u, 0u};
-}
-
-// Counts that another kSafeSteps might carry over 16 bits, beside the bins.
-__device__ __forceinline__ void flush_full(CountLds& s) {
-  __syncthreads();
-#pragma unroll 1
-  for (int i = threadIdx.x; i < 32768; i += kRowThreads) {
-    uint32_t w = s.bin[i];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const uint32_t c = (w >> (16 * half)) & 0xffffu;
-      if (c < kFull) continue;
-      const int at = atomicAdd(&s.heavies, 1);
-      s.heavy[at] = 2 * i + half;
-      s.heavy_count[at] = c;
-      w -= c << (16 * half);
-    }
-    s.bin[i] = w;
-  }
-  __syncthreads();
 }
 
 // a lane's word of a group
@@ -708,7 +590,7 @@ __device__ __forceinline__ bool has_value(const u32x4& v, uint32_t both, uint32_
 
 // s.index = the index of the token of bits `value` with `rank` of them before
 // it among the vectors lo .. hi - 1
-__device__ __forceinline__ void find_token(const Row& row, int lo, int hi, uint32_t value, uint32_t rank, CountLds& s) {
+__device__ __forceinline__ void find_token(const Row<uint16_t>& row, int lo, int hi, uint32_t value, uint32_t rank, CountLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t mask = value ? ~0u : 0x7fff7fffu, both = value | (value << 16);  // (+0: -0 too)
   each_vec(row, lo, hi, [&](int it, const u32x4& v, bool in) {
@@ -757,28 +639,6 @@ __device__ __forceinline__ void find_token(const Row& row, int lo, int hi, uint3
   __syncthreads();
 }
 
-struct Settings {
-  float T, p, least, u;
-  int k;
-  bool sampled, ends;
-  double inv_t;
-};
-// (as vector loads: scalar ones would be waited for with the LDS writes)
-__device__ __forceinline__ Settings settings_of(const FilterArgs& a, int b, bool sampled, int64_t at_u, bool ends) {
-  int vb = b;
-  int64_t vu = at_u;
-  asm volatile("" : "+v"(vb), "+v"(vu));
-  Settings f;
-  f.T = a.temperature[vb];
-  f.k = a.top_k ? a.top_k[vb] : 0;
-  f.p = a.top_p ? a.top_p[vb] : 1.f;
-  f.least = a.min_p ? a.min_p[vb] : 0.f;
-  f.u = a.uniforms[vu];
-  f.sampled = sampled;
-  f.ends = ends;
-  return f;
-}
-
 // Counts and weights of the groups that occur, the waves in turn; their number.
 __device__ __forceinline__ int weigh_groups(double inv_t, int heavies, CountLds& s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -787,7 +647,6 @@ __device__ __forceinline__ int weigh_groups(double inv_t, int heavies, CountLds&
   if (lane == kGroups / 64 - 1 && (s.occurs[kGroups / 64] & 1)) occurs |= 1u << 31;
   const uint32_t upto = wave_scan((uint32_t)__popc(occurs));
   const int groups = (int)lane_u32(upto, 63);
-  uint32_t slots = 0;
 #pragma unroll 1
   for (int n = wave; n < groups; n += kRowWaves) {
     const int g = nth_group(n, occurs, upto);
@@ -800,14 +659,12 @@ __device__ __forceinline__ int weigh_groups(double inv_t, int heavies, CountLds&
     pair_weights(q, bf16_bits_to_f32(ref), inv_t, s.tab, w1, w2);
     const double m = wave_sum_dpp(q.c1 * w1 + q.c2 * w2);
     const uint32_t all = lane_u32(wave_scan(q.c1 + q.c2), 63);
-    slots += all;
     if (lane == 0) {
       s.count[n] = all;
       s.mass[n] = m;
       s.ref[n] = ((uint32_t)g << 16) | ref;
     }
   }
-  if (lane == 0) atomicAdd(&s.slots, slots);
   return groups;
 }
 
@@ -891,7 +748,7 @@ __device__ __forceinline__ void decide(const Settings& f, int V, int groups, int
 }
 
 // The first NaN of a row that has one.
-__device__ __forceinline__ RowCut nan_row(const Row& row, CountLds& s) {
+__device__ __forceinline__ RowCut nan_row(const Row<uint16_t>& row, CountLds& s) {
   if (threadIdx.x == 0) s.index = row.V;
   __syncthreads();
 #pragma unroll 1
@@ -923,78 +780,14 @@ __device__ __forceinline__ RowCut look_up(int V, const CountLds& s, F find) {
   return out;
 }
 
-// filter_row for bf16, by one workgroup.
-__device__ __forceinline__ RowCut count_row(const Row& row, Settings f, CountLds& s) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  clear_bins(s.bin);
-  if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
-  if (tid == 0) {
-    s.nan = s.heavies = 0;
-    s.slots = 0;
-  }
-  lds_barrier();
-  f.inv_t = is_greedy(f.T) ? 1.0 : 1.0 / (double)f.T;
-  // A bin runs over only where one value has more than 65,535 tokens: the
-  // counts then miss some, and are taken again with the full ones put aside
-  // in between.
-  int groups = 0, heavies = 0;
-#pragma unroll 1
-  for (int careful = 0; careful < 2; ++careful) {
-    uint32_t heavy = ~0u, many = 0;
-    const int whole = (row.vecs + kRowThreads - 1) / kRowThreads * kRowThreads;
-    const int run = careful ? kSafeSteps * kRowThreads : whole;
-#pragma unroll 1
-    for (int lo = 0; lo < row.vecs; lo += run) {
-      each_vec(row, lo, min(lo + run, row.vecs), [&](int, const u32x4& v, bool in) {
-        if (in) count_vec(s.bin, v, heavy, many);
-      });
-      if (careful) flush_full(s);
-    }
-    // (a wave's lanes count alike, but those without a last vector)
-    heavy = (uint32_t)__builtin_amdgcn_readfirstlane((int)heavy);
-    many = (uint32_t)__builtin_amdgcn_readfirstlane((int)many);
-    if (lane == 0 && many) {
-      const int at = atomicAdd(&s.heavies, 1);
-      s.heavy[at] = heavy;
-      s.heavy_count[at] = many;
-    }
-    __syncthreads();
-    heavies = s.heavies;
-    uint32_t has = own_groups(s.bin, [](int, uint32_t) {});
-    for (int i = 0; i < heavies; ++i) {
-      const int g = group_of(s.heavy[i]);
-      if (g >> 5 == wave) has |= 1u << (g & 31);
-    }
-    if (lane == 0) s.occurs[wave] = has;
-    __syncthreads();
-    groups = weigh_groups(f.inv_t, heavies, s);
-    __syncthreads();
-    if (s.slots == 8u * (uint32_t)row.vecs) break;  // uniform
-    __syncthreads();
-    clear_bins(s.bin);
-    if (tid == 0) {
-      s.heavies = 0;
-      s.slots = 0;
-    }
-    __syncthreads();
-  }
-  if (s.nan) return nan_row(row, s);  // uniform
-  if (wave == 0) decide(f, row.V, groups, heavies, s);
-  __syncthreads();
-  return look_up(row.V, s, [&](uint32_t value, uint32_t rank) { find_token(row, 0, row.vecs, value, rank, s); });
-}
-
-// A row in parts, each counted by a workgroup of its own (at most kSafeSteps
-// steps, so that 16 bits hold every count): which groups occur, and the words
-// of those that do.
+// What one workgroup counted of a row (at most kSafeSteps steps, so that 16
+// bits hold every count): which groups occur, and the words of those that do.
 struct Part {
   uint32_t occurs[kGroups / 32];
   uint32_t word[kGroups * 64];
 };
 
-__device__ __forceinline__ int part_vecs(const Row& row, int parts) { return (row.vecs + parts - 1) / parts; }
-
-__device__ __forceinline__ void count_part(const Row& row, int part, int parts, uint32_t* bin, Part* out) {
+__device__ __forceinline__ void count_part(const Row<uint16_t>& row, int part, int parts, uint32_t* bin, Part* out) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int per = part_vecs(row, parts), lo = part * per, hi = min(lo + per, row.vecs);
   clear_bins(bin);
@@ -1013,13 +806,12 @@ __device__ __forceinline__ void count_part(const Row& row, int part, int parts, 
 }
 
 // filter_row for bf16, from the counts of a row's parts.
-__device__ __forceinline__ RowCut merge_row(const Row& row, Settings f, const Part* in, int parts, CountLds& s) {
+__device__ __forceinline__ RowCut merge_row(const Row<uint16_t>& row, Settings f, const Part* in, int parts, CountLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid < kGroups / 32 * parts) s.part_occurs[tid] = in[tid / (kGroups / 32)].occurs[tid % (kGroups / 32)];
   if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
   if (tid == 0) {
     s.nan = s.heavies = 0;
-    s.slots = 0;
     s.bin[0x4000] = 0;  // (read with the word of +0, whether its own group occurs or not)
   }
   __syncthreads();
@@ -1062,6 +854,7 @@ __device__ __forceinline__ RowCut merge_row(const Row& row, Settings f, const Pa
     }
     s.bin[word] = lo | (hi << 16);
   }
+  make_uniform(f);
   f.inv_t = is_greedy(f.T) ? 1.0 : 1.0 / (double)f.T;
   __syncthreads();
   const int heavies = s.heavies;
@@ -1089,14 +882,540 @@ __device__ __forceinline__ RowCut merge_row(const Row& row, Settings f, const Pa
   });
 }
 
-// probability of token i of logit x
-__device__ __forceinline__ double prob_of(const RowCut& c, float x, int i, double inv_t, const double* tab) {
-  if (c.kept == 1) return i == c.token ? 1.0 : 0.0;
-  const bool in = x > c.cut || (x == c.cut && i <= c.last);
-  return in ? weight_of(x, c.top, inv_t, tab) / c.total : 0.0;
+
+// ---------------------------------------------------------------------------
+// fp32 rows by bins
+// ---------------------------------------------------------------------------
+constexpr int kBinShift = 19;           // a bin: the tokens of equal leading 13 bits of their order
+constexpr int kBins32 = 1 << (32 - kBinShift);
+constexpr int kBinGroups = kBins32 / 64;
+constexpr int kList = 4096;             // tokens looked at one by one
+constexpr int kSubBins = 1024;
+
+// What one workgroup added up of a row: its maximum, and the bins of the
+// groups of 64 that occur: tokens above -inf, and their weights as integers of
+// 2^-shift, of the bin's largest possible value (of the maximum in its own bin,
+// which at a low temperature lies far above what the others weigh).
+struct BinPart {
+  uint32_t occurs[kBinGroups / 32];
+  float top;
+  uint32_t nan, pad[2];
+  uint32_t count[kBins32];
+  unsigned long long mass[kBins32];
+};
+
+struct BinLds {
+  uint32_t count[kBins32];
+  unsigned long long mass[kBins32];
+  double tab[256];
+  float red[kRowWaves];
+  int nan;
+};
+
+__device__ __forceinline__ uint32_t bin_of(float x) { return order_bits(x) >> kBinShift; }
+__device__ __forceinline__ float bin_edge(uint32_t bin) { return order_value(bin << kBinShift); }
+
+__device__ __forceinline__ void bin_part(const Row<float>& row, int part, int parts, float T, int shift, BinLds& s, BinPart* out) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int per = part_vecs(row, parts), lo = part * per, hi = min(lo + per, row.vecs);
+  for (int i = tid; i < kBins32 / 4; i += kRowThreads) reinterpret_cast<u32x4*>(s.count)[i] = u32x4{0u, 0u, 0u, 0u};
+  for (int i = tid; i < kBins32 / 2; i += kRowThreads) reinterpret_cast<u32x4*>(s.mass)[i] = u32x4{0u, 0u, 0u, 0u};
+  if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
+  if (tid == 0) s.nan = 0;
+  float top = -__builtin_inff();
+  bool nan = false;
+  if (lo < hi)
+    each_vec(row, lo, hi, [&](int, const u32x4& v, bool) {  // (a vector past the end is the last one again)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __uint_as_float(v[e]);
+        top = fmaxf(top, x);
+        nan |= x != x;
+      }
+    });
+  top = wave_max_dpp(top);
+  if (lane == 0) s.red[wave] = top;
+  __syncthreads();
+  if (nan) s.nan = 1;
+  top = s.red[0];
+  for (int i = 1; i < kRowWaves; ++i) top = fmaxf(top, s.red[i]);
+  __syncthreads();
+  if (tid == 0) {
+    out->top = top;
+    out->nan = s.nan;
+  }
+  if (s.nan || top == -__builtin_inff()) {  // uniform
+    if (tid < kBinGroups / 32) out->occurs[tid] = 0;
+    return;
+  }
+  const double inv_t = is_greedy(T) ? 1.0 : 1.0 / (double)T, scale = (double)(1ull << shift);
+  const uint32_t top_bin = bin_of(top);
+  auto weigh = [&](float x, uint32_t bin) {
+    return fixed_weight(weight_of(x, bin == top_bin ? top : bin_edge(bin), inv_t, s.tab), scale);
+  };
+  uint32_t heavy = 0xff800000u, many = 0;  // (-inf: none)
+  each_vec(row, lo, hi, [&](int, const u32x4& v, bool in) {
+    if (!in) return;
+    // a value that many of a wave's lanes hold (a mask's) is added up beside the bins
+    const uint32_t some = (uint32_t)__builtin_amdgcn_readfirstlane((int)v[0]);
+    const bool crowd = some != 0xff800000u && __popcll(__ballot(v[0] == some)) >= 16 && (many == 0 || heavy == some);
+    if (crowd) heavy = some;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = __uint_as_float(v[e]);
+      const bool aside = crowd && v[e] == some;
+      if (crowd) many += __popcll(__ballot(aside));
+      if (x == -__builtin_inff() || aside) continue;
+      const uint32_t bin = bin_of(x);
+      atomicAdd(&s.count[bin], 1u);
+      const uint64_t q = weigh(x, bin);
+      if (q) atomicAdd(&s.mass[bin], (unsigned long long)q);
+    }
+  });
+  heavy = (uint32_t)__builtin_amdgcn_readfirstlane((int)heavy);
+  many = (uint32_t)__builtin_amdgcn_readfirstlane((int)many);
+  if (many && lane == 0) {
+    const float x = __uint_as_float(heavy);
+    const uint32_t bin = bin_of(x);
+    atomicAdd(&s.count[bin], many);
+    atomicAdd(&s.mass[bin], (unsigned long long)many * weigh(x, bin));
+  }
+  __syncthreads();
+  // the groups that occur: 8 each wave
+  uint32_t has = 0;
+#pragma unroll
+  for (int i = 0; i < kBinGroups / kRowWaves; ++i) {
+    const int at = (wave * (kBinGroups / kRowWaves) + i) * 64 + lane;
+    const uint32_t c = s.count[at];
+    if (!__ballot(c > 0)) continue;  // uniform
+    has |= 1u << i;
+    out->count[at] = c;
+    out->mass[at] = s.mass[at];
+  }
+  static_assert(kBinGroups / kRowWaves == 8, "a byte of bits per wave");
+  if (lane == 0) reinterpret_cast<uint8_t*>(out->occurs)[wave] = (uint8_t)has;
 }
 
-// The row of workgroup (r, b): where it lies, and what is wanted of it.
+struct ListLds {
+  uint32_t count[kBins32];     // tokens of a bin; at the end the indices of equal tokens
+  double weight[kBins32];      // their weights
+  // groups that occur, along the order
+  double gweight[kBinGroups], gbefore[kBinGroups];
+  uint32_t gcount[kBinGroups], gcbefore[kBinGroups], gid[kBinGroups];
+  uint32_t part_occurs[kMaxParts * kBinGroups / 32];
+  float part_top[kMaxParts];
+  double part_scale[kMaxParts];
+  uint64_t list[kList];        // order bits << 32 | index
+  uint32_t sub_count[kSubBins];
+  unsigned long long sub_mass[kSubBins];
+  double tab[256];
+  uint32_t red[kRowWaves];
+  uint64_t red2[kRowWaves];
+  int nan, listed, hit, index, equals;
+  uint32_t hit_count, hit_before;
+  uint64_t hit_mass, hit_mass_before;
+};
+union RowLds32 {
+  ListLds bins;
+  RowLds radix;
+};
+
+struct Bin {
+  uint32_t bin;
+  uint32_t before, count;  // tokens
+  double mass, weight;     // weights before; of its tokens
+};
+
+// The last bin with: tokens before it < goal (kByCount); weights before it <
+// goal (kReach) or <= goal (kBeyond), and a weight of its own; a largest
+// possible weight >= goal (kAbove).  By every wave alike.
+__device__ __forceinline__ Bin seek_bin(int kind, double goal, const ListLds& s, int groups, float top, double inv_t) {
+  const int lane = threadIdx.x & 63;
+  int n = -1;
+#pragma unroll 1
+  for (int i = (groups - 1) >> 6; i >= 0 && n < 0; --i) {
+    const int mine = min(64 * i + lane, groups - 1);
+    bool fits;
+    if (kind == kByCount) fits = (double)s.gcbefore[mine] < goal;
+    // (a group's first bin may be empty: whether another of it is heavy enough shows below)
+    else if (kind == kAbove) fits = weight_of(fminf(bin_edge(64 * s.gid[mine]), top), top, inv_t, s.tab) >= goal;
+    else fits = s.gweight[mine] > 0.0 && (kind == kReach ? s.gbefore[mine] < goal : s.gbefore[mine] <= goal);
+    const uint64_t yes = __ballot(fits && 64 * i + lane < groups);
+    if (yes) n = 64 * i + 63 - __clzll((long long)yes);
+  }
+  n = max(n, 0);
+  Bin at{};
+#pragma unroll 1
+  for (;; --n) {  // (kAbove: to a group before, where the bins that are heavy enough are empty)
+    const uint32_t bin = 64 * s.gid[n] + lane, c = s.count[bin];
+    const double w = s.weight[bin];
+    const double before = s.gbefore[n] + lane_before(wave_scan(w));
+    const uint32_t cbefore = s.gcbefore[n] + wave_scan(c) - c;
+    bool fits = c > 0;
+    if (kind == kByCount) fits = fits && (double)cbefore < goal;
+    else if (kind == kAbove) fits = fits && weight_of(fminf(bin_edge(bin), top), top, inv_t, s.tab) >= goal;
+    else fits = fits && w > 0.0 && (kind == kReach ? before < goal : before <= goal);
+    const uint64_t yes = __ballot(fits);
+    if (!yes && n > 0) continue;
+    const int l = yes ? 63 - __clzll((long long)yes) : 0;
+    at.bin = lane_u32(bin, l);
+    at.before = lane_u32(cbefore, l);
+    at.count = lane_u32(c, l);
+    at.mass = lane_f64(before, l);
+    at.weight = lane_f64(w, l);
+    return at;
+  }
+}
+
+// As seek, among the listed tokens of a bin.  mass, weight: integers of
+// 2^-shift of the bin's reference value.
+__device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, float ref, double inv_t, double scale, ListLds& s) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Spot at{bin << kBinShift, 0u, 0u, 0ull, 0ull};
+#pragma unroll 1
+  for (int level = 0; level < 2; ++level) {
+    const int sh = level ? 0 : 9, bits = level ? 9 : 10;
+    __syncthreads();
+    s.sub_count[tid] = 0;
+    s.sub_mass[tid] = 0;
+    if (tid == 0) s.hit = -1;
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < s.listed; i += kRowThreads) {
+      const uint32_t k = (uint32_t)(s.list[i] >> 32);
+      if ((k >> (sh + bits)) != (at.key >> (sh + bits))) continue;
+      const uint32_t sub = (k >> sh) & ((1u << bits) - 1);
+      atomicAdd(&s.sub_count[sub], 1u);
+      const uint64_t q = fixed_weight(weight_of(order_value(k), ref, inv_t, s.tab), scale);
+      if (q) atomicAdd(&s.sub_mass[sub], (unsigned long long)q);
+    }
+    __syncthreads();
+    const uint32_t c = s.sub_count[tid], cu = wave_scan(c);
+    const uint64_t m = s.sub_mass[tid], mu = wave_scan(m);
+    if (lane == 63) {
+      s.red[wave] = cu;
+      s.red2[wave] = mu;
+    }
+    __syncthreads();
+    uint32_t cb = at.before + cu - c;
+    uint64_t mb = at.mass + mu - m;
+    for (int i = 0; i < wave; ++i) {
+      cb += s.red[i];
+      mb += s.red2[i];
+    }
+    bool fits = c > 0;
+    if (kind == kByCount) fits = fits && (double)cb < goal;
+    else fits = fits && m > 0 && (kind == kReach ? (double)mb < goal : (double)mb <= goal);
+    if (fits) atomicMax(&s.hit, tid);
+    __syncthreads();
+    if (tid == max(s.hit, 0)) {
+      s.hit_count = c;
+      s.hit_before = cb;
+      s.hit_mass = m;
+      s.hit_mass_before = mb;
+    }
+    __syncthreads();
+    at.key |= (uint32_t)max(s.hit, 0) << sh;
+    at.before = s.hit_before;
+    at.mass = s.hit_mass_before;
+    at.count = s.hit_count;
+    at.weight = s.hit_mass;
+  }
+  at.weight /= max(at.count, 1u);  // (equal values have equal weights)
+  return at;
+}
+
+// index of the listed token of the value with `rank` of them before it (the
+// bins are overwritten)
+__device__ __forceinline__ int index_in_list(uint32_t key, uint32_t rank, ListLds& s) {
+  __syncthreads();
+  if (threadIdx.x == 0) s.equals = s.index = 0;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < s.listed; i += kRowThreads)
+    if ((uint32_t)(s.list[i] >> 32) == key) s.count[atomicAdd(&s.equals, 1)] = (uint32_t)s.list[i];
+  __syncthreads();
+#pragma unroll 1
+  for (int i = threadIdx.x; i < s.equals; i += kRowThreads) {
+    const uint32_t mine = s.count[i];
+    uint32_t before = 0;
+    for (int j = 0; j < s.equals; ++j) before += s.count[j] < mine;
+    if (before == rank) s.index = (int)mine;
+  }
+  __syncthreads();
+  return s.index;
+}
+
+// A row from its parts' bins.  Which bins the cuts and the sample lie in
+// follows from the sums, but for the weights inside the bin of the cut before:
+// so from the least and the most it may leave a range of bins is taken, the
+// tokens of all ranges are listed in one pass over the row, and the values
+// found among them.
+__device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, const BinPart* in, int parts, int shift, ListLds& s,
+                                           bool& fits) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = row.V;
+  constexpr int kWords = kBinGroups / 32;
+  fits = true;
+  if (tid < kWords * parts) s.part_occurs[tid] = in[tid / kWords].occurs[tid % kWords];
+  if (tid < parts) s.part_top[tid] = in[tid].top;
+  if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
+  if (tid == 0) s.nan = s.listed = 0;
+  __syncthreads();
+  if (tid < parts && in[tid].nan) s.nan = 1;
+  make_uniform(f);
+  float top = -__builtin_inff();
+  for (int c = 0; c < parts; ++c) top = fmaxf(top, s.part_top[c]);
+  const bool greedy = is_greedy(f.T);
+  const double inv_t = greedy ? 1.0 : 1.0 / (double)f.T, scale = (double)(1ull << shift);
+  if (tid < parts) s.part_scale[tid] = weight_of(s.part_top[tid], top, inv_t, s.tab) / scale;
+  __syncthreads();
+  RowCut out{top, top, V - 1, 1, 0, 0, 1.0};
+  if (s.nan) {  // uniform
+    fits = false;
+    return out;
+  }
+  if (top == -__builtin_inff()) {  // uniform: nothing above it, the first token
+    out.last = 0;
+    return out;
+  }
+  // the parts' bins added up: those of a part's maximum by that, the others as integers
+  uint32_t occurs = 0;
+  if (lane < kWords)
+    for (int c = 0; c < parts; ++c) occurs |= s.part_occurs[c * kWords + lane];
+  const uint32_t upto = wave_scan((uint32_t)__popc(occurs));
+  const int groups = (int)lane_u32(upto, 63);
+#pragma unroll 1
+  for (int n = wave; n < groups; n += kRowWaves) {
+    const int g = nth_group(n, occurs, upto);
+    const uint64_t have = __ballot(lane < parts && ((s.part_occurs[min(lane, parts - 1) * kWords + (g >> 5)] >> (g & 31)) & 1));
+    const uint32_t bin = 64 * g + lane;
+    uint32_t count = 0;
+    uint64_t mass = 0;
+    double weight = 0.0;
+#pragma unroll 1
+    for (int c0 = 0; c0 < parts; c0 += 4) {
+      uint32_t pc[4];
+      unsigned long long pm[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const BinPart& p = in[min(c0 + j, parts - 1)];
+        pc[j] = p.count[bin];
+        pm[j] = p.mass[bin];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (!((have >> (c0 + j)) & 1)) continue;  // uniform (what a part has not is whatever the memory held)
+        const uint32_t tb = bin_of(s.part_top[c0 + j]);
+        count += pc[j];
+        if ((tb >> 6) == (uint32_t)g && bin == tb) weight += (double)pm[j] * s.part_scale[c0 + j];
+        else mass += pm[j];
+      }
+    }
+    weight += (double)mass * (weight_of(fminf(bin_edge(bin), top), top, inv_t, s.tab) / scale);
+    s.count[bin] = count;
+    s.weight[bin] = weight;
+    const double all = wave_sum_dpp(weight);
+    const uint32_t many = lane_u32(wave_scan(count), 63);
+    if (lane == 0) {
+      s.gweight[n] = all;
+      s.gcount[n] = many;
+      s.gid[n] = g;
+    }
+  }
+  __syncthreads();
+  double total = 0.0;
+  uint32_t tokens = 0;  // above -inf
+  if (wave == 0) {
+#pragma unroll 1
+    for (int i = 0; i < groups; i += 64) {
+      const int n = min(i + lane, groups - 1);
+      const bool here = i + lane < groups;
+      const double w = here ? s.gweight[n] : 0.0, wu = wave_scan(w);
+      const uint32_t c = here ? s.gcount[n] : 0u, cu = wave_scan(c);
+      if (here) {
+        s.gbefore[n] = total + lane_before(wu);
+        s.gcbefore[n] = tokens + cu - c;
+      }
+      total += lane_f64(wu, 63);
+      tokens += lane_u32(cu, 63);
+    }
+  }
+  __syncthreads();
+  total = s.gbefore[groups - 1] + s.gweight[groups - 1];
+  tokens = s.gcbefore[groups - 1] + s.gcount[groups - 1];
+
+  // ranges of bins, from the least and the most that each cut may leave (all waves alike)
+  const double tiny = 0x1p-1000, slack = 0x1p-30;  // (the sums' own error is below 2^-40)
+  const bool by_count = !greedy && f.k > 0 && f.k < V && (uint32_t)f.k < tokens, reach = !greedy && f.p < 1.f,
+             above = !greedy && f.least > 0.f;
+  float hi[4], lo[4];
+  int ranges = 0;
+  auto take = [&](uint32_t first, uint32_t last) {
+    const float h = bin_edge(first), l = order_value(((last + 1) << kBinShift) - 1);
+    hi[0] = ranges == 0 ? h : hi[0];
+    lo[0] = ranges == 0 ? l : lo[0];
+    hi[1] = ranges == 1 ? h : hi[1];
+    lo[1] = ranges == 1 ? l : lo[1];
+    hi[2] = ranges == 2 ? h : hi[2];
+    lo[2] = ranges == 2 ? l : lo[2];
+    hi[3] = ranges == 3 ? h : hi[3];
+    lo[3] = ranges == 3 ? l : lo[3];
+    ++ranges;
+  };
+  double least = total, most = total;
+  if (greedy) take(bin_of(top), bin_of(top));
+  if (by_count) {
+    const Bin at = seek_bin(kByCount, (double)f.k, s, groups, top, inv_t);
+    take(at.bin, at.bin);
+    least = at.mass;
+    most = at.mass + at.weight;
+  }
+  if (reach) {
+    const Bin x = seek_bin(kReach, fmax((double)f.p * least * (1.0 - slack), tiny), s, groups, top, inv_t);
+    const Bin y = seek_bin(kReach, fmax((double)f.p * most * (1.0 + slack), tiny), s, groups, top, inv_t);
+    take(x.bin, y.bin);
+    least = x.mass;
+    most = y.mass + y.weight;
+  }
+  if (above) {
+    const Bin at = seek_bin(kAbove, fmin((double)f.least, 1.0), s, groups, top, inv_t);
+    take(at.bin, at.bin);
+    least = fmin(least, at.mass);
+    most = fmin(most, at.mass + at.weight);
+  }
+  if (f.sampled && !greedy) {
+    const Bin x = seek_bin(kBeyond, unit(f.u) * least * (1.0 - slack), s, groups, top, inv_t);
+    const Bin y = seek_bin(kBeyond, unit(f.u) * most * (1.0 + slack), s, groups, top, inv_t);
+    take(x.bin, y.bin);
+  }
+  // (bin_edge of the bins of infinity and of NaN is a NaN)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (i >= ranges) hi[i] = lo[i] = __builtin_nanf("");
+    else if (hi[i] != hi[i]) hi[i] = __builtin_inff();
+  }
+  if (ranges) each_vec(row, 0, row.vecs, [&](int it, const u32x4& v, bool here) {
+    if (!here) return;
+    const int64_t e0 = (int64_t)4 * (it * kRowThreads + tid) - row.skew;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float x = __uint_as_float(v[e]);
+      bool is = x <= hi[0] && x >= lo[0];
+      if (ranges > 1) is = is || (x <= hi[1] && x >= lo[1]);
+      if (ranges > 2) is = is || (x <= hi[2] && x >= lo[2]);
+      if (ranges > 3) is = is || (x <= hi[3] && x >= lo[3]);
+      if (!is || x == -__builtin_inff()) continue;
+      const int at = atomicAdd(&s.listed, 1);
+      if (at < kList) s.list[at] = ((uint64_t)order_bits(x) << 32) | (uint32_t)(e0 + e);
+    }
+  });
+  __syncthreads();
+  if (s.listed > kList) {  // uniform
+    fits = false;
+    return out;
+  }
+  // the cuts, one after another, among the listed tokens
+  uint32_t cut_key = order_bits(top), token_key = cut_key, token_rank = 0;
+  int cut_rank = -1;
+  bool cuts = false;  // cut_key is a value that stays in part at least
+  double W = greedy ? 1.0 : total;
+  int kept = greedy ? 1 : V;
+  if (greedy) cuts = true;
+  if (!greedy && f.k > 0 && f.k < V) kept = f.k;
+  out.cut = greedy ? top : -__builtin_inff();
+  auto ref_of = [&](uint32_t bin) { return fminf(bin_edge(bin), top); };
+  if (by_count) {
+    const Bin at = seek_bin(kByCount, (double)f.k, s, groups, top, inv_t);
+    const Spot x = seek_list(kByCount, (double)((uint32_t)f.k - at.before), at.bin, ref_of(at.bin), inv_t, scale, s);
+    const uint32_t n = (uint32_t)f.k - at.before - x.before;
+    W = at.mass + (double)(x.mass + n * x.weight) * (weight_of(ref_of(at.bin), top, inv_t, s.tab) / scale);
+    cut_key = x.key;
+    cut_rank = n < x.count ? (int)n - 1 : -1;
+    cuts = true;
+  }
+  if (reach) {
+    const double goal = fmax((double)f.p * W, tiny);
+    const Bin at = seek_bin(kReach, goal, s, groups, top, inv_t);
+    const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) / scale;
+    const double inside = fmax((goal - at.mass) / unit_w, 0.5);
+    const Spot x = seek_list(kReach, inside, at.bin, ref_of(at.bin), inv_t, scale, s);
+    const double need = ceil((inside - (double)x.mass) / (double)x.weight);
+    const uint32_t n = (uint32_t)fmin(fmax(need, 1.0), (double)x.count);
+    if ((int)(at.before + x.before + n) < kept) {
+      kept = (int)(at.before + x.before + n);
+      W = at.mass + (double)(x.mass + n * x.weight) * unit_w;
+      cut_key = x.key;
+      cut_rank = n < x.count ? (int)n - 1 : -1;
+      cuts = true;
+    }
+  }
+  if (above) {
+    const double goal = fmin((double)f.least, 1.0);
+    const Bin at = seek_bin(kAbove, goal, s, groups, top, inv_t);
+    const float ref = ref_of(at.bin);
+    // the bin's tokens that are heavy enough: how many, their weights, the lightest
+    __syncthreads();
+    if (tid == 0) {
+      s.hit_count = 0;
+      s.hit_mass = 0;
+      s.hit_before = 0;
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = tid; i < s.listed; i += kRowThreads) {
+      const uint32_t k = (uint32_t)(s.list[i] >> 32);
+      const float x = order_value(k);
+      if (k >> kBinShift != at.bin || !(weight_of(x, top, inv_t, s.tab) >= goal)) continue;
+      atomicAdd(&s.hit_count, 1u);
+      atomicMax(&s.hit_before, k);
+      atomicAdd((unsigned long long*)&s.hit_mass, (unsigned long long)fixed_weight(weight_of(x, ref, inv_t, s.tab), scale));
+    }
+    __syncthreads();
+    const uint32_t n = s.hit_count;
+    if ((int)(at.before + n) < kept) {
+      kept = (int)(at.before + n);
+      W = at.mass + (double)s.hit_mass * (weight_of(ref, top, inv_t, s.tab) / scale);
+      // (none: what lies before the bin, whose largest possible value none of its tokens has)
+      cut_key = n ? s.hit_before : at.bin << kBinShift;
+      cut_rank = -1;
+      cuts = true;
+    }
+  }
+  if (f.sampled && kept > 1) {
+    const double goal = unit(f.u) * W;
+    const Bin at = seek_bin(kBeyond, goal, s, groups, top, inv_t);
+    const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) / scale;
+    const double inside = fmax((goal - at.mass) / unit_w, 0.0);
+    const Spot x = seek_list(kBeyond, inside, at.bin, ref_of(at.bin), inv_t, scale, s);
+    const double j = fmin(floor((inside - (double)x.mass) / (double)x.weight),
+                          (double)min((int)x.count, kept - (int)(at.before + x.before)) - 1.0);
+    token_key = x.key;
+    token_rank = (uint32_t)fmax(j, 0.0);
+  }
+  out.kept = kept;
+  out.total = W;
+  if (cuts) out.cut = order_value(cut_key);
+  if (kept == 1 || f.sampled) out.token = index_in_list(token_key, token_rank, s);
+  if (kept == 1 && s.equals == 0) {  // uniform: alone because of a bin behind its own, which was not listed
+    if (tid == 0) s.index = V;
+    __syncthreads();
+    each<float>(row.at, V, [&](int i, float x) {
+      if (x == top) atomicMin(&s.index, i);
+    });
+    __syncthreads();
+    out.token = s.index;
+  }
+  if (kept == 1) out.last = out.token;
+  else if (f.ends && cut_rank >= 0) out.last = index_in_list(cut_key, (uint32_t)cut_rank, s);
+  return out;
+}
+
+
+// ---------------------------------------------------------------------------
+// kernels
+// ---------------------------------------------------------------------------
+
+// Row r of sequence b: where it lies, and what is wanted of it.
 struct Job {
   int64_t at;       // elements, from `target` or `draft`
   int64_t u;        // its number among the uniforms
@@ -1137,353 +1456,97 @@ __device__ __forceinline__ void put_row(const FilterArgs& a, int r, int b, const
   }
 }
 
-// grid (rows per sequence, B): target rows, then draft rows
-__global__ __launch_bounds__(kRowThreads) void filter_rows_f32_kernel(FilterArgs a) {
-  __shared__ RowLds s;
-  const int r = blockIdx.x, b = blockIdx.y;
-  const Job j = job_of(a, r, b);
-  if (!j.active) return;  // uniform
-  const float* row = (const float*)(j.is_draft ? a.draft : a.target) + j.at;
-  put_row(a, r, b, j, row, filter_row<float>(a, b, row, j.sampled, a.uniforms[j.u], j.ends, s));
-}
+// What a launch's n-th row is.
+template <typename T>
+struct Work {
+  int r, b;
+  Job j;
+  const T* row;
+  __device__ Work(const FilterArgs& a, int n) {
+    b = (a.row0 + n) / a.rows;
+    r = a.row0 + n - b * a.rows;
+    j = job_of(a, r, b);
+    row = (const T*)(j.is_draft ? a.draft : a.target) + j.at;
+  }
+};
 
-__global__ __launch_bounds__(kRowThreads) void filter_rows_bf16_kernel(FilterArgs a) {
-  __shared__ CountLds s;
-  const int r = blockIdx.x, b = blockIdx.y;
-  const Job j = job_of(a, r, b);
-  if (!j.active) return;  // uniform
-  const uint16_t* row = (const uint16_t*)(j.is_draft ? a.draft : a.target) + j.at;
-  put_row(a, r, b, j, row, count_row(Row(row, a.V), settings_of(a, b, j.sampled, j.u, j.ends), s));
-}
-
-// grid (parts, rows per sequence, B)
-__global__ __launch_bounds__(kRowThreads) void filter_parts_kernel(FilterArgs a) {
+// grid (parts, rows)
+__global__ __launch_bounds__(kRowThreads) void filter_count_kernel(FilterArgs a) {
   __shared__ uint32_t bin[32768];
-  const int r = blockIdx.y, b = blockIdx.z;
-  const Job j = job_of(a, r, b);
-  if (!j.active) return;  // uniform
-  const uint16_t* row = (const uint16_t*)(j.is_draft ? a.draft : a.target) + j.at;
-  count_part(Row(row, a.V), blockIdx.x, gridDim.x, bin, a.row_parts + ((int64_t)b * gridDim.y + r) * gridDim.x + blockIdx.x);
+  const Work<uint16_t> w(a, blockIdx.y);
+  if (!w.j.active) return;  // uniform
+  count_part(Row<uint16_t>(w.row, a.V), blockIdx.x, a.split, bin, (Part*)a.row_parts + (int64_t)blockIdx.y * a.split + blockIdx.x);
 }
-// grid (rows per sequence, B)
+__global__ __launch_bounds__(kRowThreads) void filter_bin_kernel(FilterArgs a) {
+  __shared__ BinLds s;
+  const Work<float> w(a, blockIdx.y);
+  if (!w.j.active) return;  // uniform
+  bin_part(Row<float>(w.row, a.V), blockIdx.x, a.split, a.temperature[w.b], a.shift, s,
+           (BinPart*)a.row_parts + (int64_t)blockIdx.y * a.split + blockIdx.x);
+}
+// grid rows
 __global__ __launch_bounds__(kRowThreads) void filter_merge_kernel(FilterArgs a) {
   __shared__ CountLds s;
-  const int r = blockIdx.x, b = blockIdx.y;
-  const Job j = job_of(a, r, b);
-  if (!j.active) return;  // uniform
-  const uint16_t* row = (const uint16_t*)(j.is_draft ? a.draft : a.target) + j.at;
-  const Part* in = a.row_parts + ((int64_t)b * gridDim.x + r) * a.split;
-  put_row(a, r, b, j, row, merge_row(Row(row, a.V), settings_of(a, b, j.sampled, j.u, j.ends), in, a.split, s));
+  const Work<uint16_t> w(a, blockIdx.x);
+  if (!w.j.active) return;  // uniform
+  const Part* in = (const Part*)a.row_parts + (int64_t)blockIdx.x * a.split;
+  put_row(a, w.r, w.b, w.j, w.row,
+          merge_row(Row<uint16_t>(w.row, a.V), settings_of(a, w.b, w.j.sampled, w.j.u, w.j.ends), in, a.split, s));
+}
+__global__ __launch_bounds__(kRowThreads) void filter_list_kernel(FilterArgs a) {
+  __shared__ RowLds32 s;
+  const Work<float> w(a, blockIdx.x);
+  if (!w.j.active) return;  // uniform
+  const BinPart* in = (const BinPart*)a.row_parts + (int64_t)blockIdx.x * a.split;
+  bool fits;
+  RowCut c = list_row(Row<float>(w.row, a.V), settings_of(a, w.b, w.j.sampled, w.j.u, w.j.ends), in, a.split, a.shift, s.bins, fits);
+  if (!fits) {  // uniform
+    __syncthreads();
+    c = filter_row<float>(a, w.b, w.row, w.j.sampled, a.uniforms[w.j.u], w.j.ends, s.radix);
+  }
+  put_row(a, w.r, w.b, w.j, w.row, c);
 }
 
-// drafts accepted before the first refused (a whole wave)
-__device__ __forceinline__ int accepted_by_rows(const FilterArgs& a, int b, int kb) {
-  const int i = threadIdx.x & 63;
-  bool refused = false;
-  if (i < kb) {
-    const double pt = a.probs[(int64_t)b * (2 * a.K + 1) + i], pd = a.probs[(int64_t)b * (2 * a.K + 1) + a.K + 1 + i];
-    refused = !((double)a.uniforms[(int64_t)b * (a.K + 1) + i] * pd < pt);
-  }
-  const uint64_t no = __ballot(refused);
-  return no ? __ffsll((long long)no) - 1 : kb;
-}
-
-// a thread's residuals max(p_target - p_draft, 0) and p_target of a chunk
-template <typename T>
-__device__ __forceinline__ void residuals(const FilterArgs& a, int b, int r, int ch, const double* tab, double (&left)[kVec],
-                                          double (&pt)[kVec]) {
-  const T* t = (const T*)a.target + (int64_t)b * a.t_seq + (int64_t)r * a.t_row;
-  const T* d = (const T*)a.draft + draft_at(a, b, r);
-  const RowCut ct = a.cuts[(int64_t)b * (2 * a.K + 1) + r], cd = a.cuts[(int64_t)b * (2 * a.K + 1) + a.K + 1 + r];
-  const double inv_t = 1.0 / (double)a.temperature[b];
-  const int64_t base = (int64_t)ch * kChunk + kVec * threadIdx.x;
-  float xt[kVec], xd[kVec];
-  if (base < a.V) {
-    load_vec<T>(t, base, a.V, xt);
-    load_vec<T>(d, base, a.V, xd);
-  }
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    left[e] = pt[e] = 0.0;
-    if (base + e >= a.V) continue;
-    pt[e] = prob_of(ct, xt[e], (int)(base + e), inv_t, tab);
-    if (pt[e] > 0.0) left[e] = fmax(pt[e] - prob_of(cd, xd[e], (int)(base + e), inv_t, tab), 0.0);
-  }
-}
-
-// grid (chunks, B): chunk sums of the refused row's residuals
-template <typename T>
-__global__ __launch_bounds__(kChunkThreads) void filter_residual_kernel(FilterArgs a) {
-  __shared__ double tab[256], red[2 * kChunkThreads / 64];
-  const int b = blockIdx.y, ch = blockIdx.x;
-  if (!by_rows(a, b)) return;  // uniform
-  const int kb = draft_count(a, b), n = accepted_by_rows(a, b, kb);
-  if (n == kb) return;  // uniform: every draft stays
-  tab[threadIdx.x] = kExp2Frac256[threadIdx.x];
-  __syncthreads();
-  double left[kVec], pt[kVec], sl = 0.0, sp = 0.0;
-  residuals<T>(a, b, n, ch, tab, left, pt);
-  for (int e = 0; e < kVec; ++e) {
-    sl += left[e];
-    sp += pt[e];
-  }
-  sl = wave_sum_dpp(sl);
-  sp = wave_sum_dpp(sp);
-  if ((threadIdx.x & 63) == 0) {
-    red[2 * (threadIdx.x >> 6)] = sl;
-    red[2 * (threadIdx.x >> 6) + 1] = sp;
-  }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    double r = 0.0;
-    for (int w = 0; w < kChunkThreads / 64; ++w) r += red[2 * w + threadIdx.x];
-    a.parts[((int64_t)b * a.chunks + ch) * 2 + threadIdx.x] = r;
-  }
-}
-
-// grid B: the sequence's tokens
-template <typename T>
-__global__ __launch_bounds__(kChunkThreads) void filter_finish_kernel(FilterArgs a) {
-  __shared__ double tab[256], red[kChunkThreads / 64], goal_s, before_s;
-  __shared__ int which, use_pt, token;
-  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int K = a.K, kb = draft_count(a, b);
-  const RowCut* cuts = a.cuts + (int64_t)b * (2 * K + 1);
-  int32_t* out = a.out_tokens + (int64_t)b * (K + 1);
-  const int32_t d = lane < kb ? a.drafts[(int64_t)b * K + lane] : -1;
-  if (!by_rows(a, b)) {  // uniform: every row was sampled
-    if (wave) return;
-    const int32_t t = lane <= kb ? cuts[lane].token : 0;
-    const uint64_t no = __ballot(lane < kb && t != d);
-    const int n = no ? __ffsll((long long)no) - 1 : kb;
-    if (lane <= n) out[lane] = t;
-    if (lane == 0) a.out_len[b] = n + 1;
-    return;
-  }
-  const int n = accepted_by_rows(a, b, kb);
-  if (wave == 0 && lane < n) out[lane] = d;
-  if (tid == 0) a.out_len[b] = n + 1;
-  if (n == kb) {  // uniform: the bonus token
-    if (tid == 0) out[n] = cuts[n].token;
-    return;
-  }
-  tab[tid] = kExp2Frac256[tid];
-  // the chunk that holds the token: the last with any weight whose sums before it do not exceed the goal
-  const double* parts = a.parts + (int64_t)b * a.chunks * 2;
-  if (wave == 0) {
-    double sl = 0.0;
-    for (int c = lane; c < a.chunks; c += 64) sl += parts[2 * c];
-    const int col = wave_sum_dpp(sl) > 0.0 ? 0 : 1;  // no residual: the target row itself
-    double total = 0.0;
-    for (int c0 = 0; c0 < a.chunks; c0 += 64) {
-      const double v = wave_scan(c0 + lane < a.chunks ? parts[2 * (c0 + lane) + col] : 0.0);
-      total += __shfl(v, 63);
-    }
-    const double goal = unit(a.uniforms[(int64_t)b * (K + 1) + K]) * total;
-    double run = 0.0, before = 0.0;
-    int at = 0;
-    for (int c0 = 0; c0 < a.chunks; c0 += 64) {
-      const double mine = c0 + lane < a.chunks ? parts[2 * (c0 + lane) + col] : 0.0;
-      const double v = wave_scan(mine);
-      double prev = __shfl_up(v, 1);
-      if (lane == 0) prev = 0.0;
-      const uint64_t yes = __ballot(mine > 0.0 && run + prev <= goal);
-      if (yes) {
-        const int l = 63 - __clzll((long long)yes);
-        at = c0 + l;
-        before = run + __shfl(prev, l);
-      }
-      run += __shfl(v, 63);
-    }
-    if (lane == 0) {
-      which = at;
-      use_pt = col;
-      goal_s = goal;
-      before_s = before;
-      token = -1;
-    }
-  }
-  __syncthreads();
-  double left[kVec], pt[kVec];
-  residuals<T>(a, b, n, which, tab, left, pt);
-  double mine = 0.0;
-  for (int e = 0; e < kVec; ++e) {
-    if (use_pt) left[e] = pt[e];
-    mine += left[e];
-  }
-  const double v = wave_scan(mine);
-  double run = __shfl_up(v, 1);
-  if (lane == 0) run = 0.0;
-  if (lane == 63) red[wave] = v;
-  __syncthreads();
-  double before = before_s;
-  for (int w = 0; w < wave; ++w) before += red[w];
-  run += before;
-  // the last element with any weight whose sums before it do not exceed the goal
-  int best = -1;
-  for (int e = 0; e < kVec; ++e) {
-    if (left[e] > 0.0 && run <= goal_s) best = which * kChunk + kVec * tid + e;
-    run += left[e];
-  }
-  if (best >= 0) atomicMax(&token, best);
-  __syncthreads();
-  if (tid == 0) out[n] = token;
-}
-
-bool bad_rows(int B, int V, int dtype) { return B < 0 || V <= 0 || (dtype != NSV_F32 && dtype != NSV_BF16); }
-
-// weights as integers: V of them, each at most 2^shift, stay below 2^62
-int weight_shift(int V) {
-  int bits = 0;
-  while ((1 << bits) < V) ++bits;
-  const int s = 62 - bits;
-  return s > 50 ? 50 : s;
-}
-
-size_t a256(size_t x) { return (x + 255) & ~(size_t)255; }
-int residual_chunks(int V) { return (V + kChunk - 1) / kChunk; }
-
-// Workgroups that count a bf16 row, each a part of it; 1: one workgroup does
-// the whole row.  Up to 256 workgroups share few rows (one row of 151,936
-// TIME1), as long as the parts' counts stay under 64 MiB.
+// Parts of a row, a workgroup each: more where the rows alone leave compute
+// units idle, as long as each takes a step of a workgroup, and in bf16 so many
+// that 16 bits hold a part's counts.
 int row_split(int rows, int V, int dtype) {
-  if (dtype != NSV_BF16 || rows <= 0) return 1;
-  const int least = (V + 7 + kSafeSteps * kStep - 1) / (kSafeSteps * kStep);
+  const int step = dtype == NSV_BF16 ? kStep : kStep / 2;
   int n = kMaxSplit;
-  while (n > 1 && (rows * n > 256 || V < n * kStep)) n >>= 1;
-  if (n < least) n = least;
-  return n > 1 && rows * n <= 512 && n <= kMaxParts ? n : 1;
+  while (n > 1 && (rows * n > 256 || V < n * step)) n >>= 1;
+  const int least = dtype == NSV_BF16 ? (V + 7 + kSafeSteps * kStep - 1) / (kSafeSteps * kStep) : 1;
+  return n < least ? least : n;
 }
-size_t parts_bytes(int rows, int V, int dtype) {
-  const int n = row_split(rows, V, dtype);
-  return n > 1 ? (size_t)rows * n * sizeof(Part) : 0;
-}
-
-struct Layout {
-  size_t cuts, probs, parts, row_parts, total;
-};
-Layout layout(int B, int K, int V, int dtype, bool draft_rows) {
-  Layout L;
-  const size_t rows = (size_t)B * (2 * (size_t)K + 1);
-  L.cuts = 0;
-  L.probs = a256(rows * sizeof(RowCut));
-  L.parts = L.probs + a256(rows * sizeof(double));
-  L.row_parts = L.parts + a256((size_t)B * residual_chunks(V) * 2 * sizeof(double));
-  L.total = L.row_parts + parts_bytes(B * (draft_rows ? 2 * K + 1 : K + 1), V, dtype);
-  return L;
-}
-
-int launch_rows(FilterArgs& a, int rows, int dtype, char* row_parts, hipStream_t s) {
-  a.split = row_split(rows * a.B, a.V, dtype);
-  a.row_parts = (Part*)row_parts;
-  const dim3 grid(rows, a.B), block(kRowThreads);
-  if (dtype == NSV_F32) {
-    hipLaunchKernelGGL(filter_rows_f32_kernel, grid, block, 0, s, a);
-  } else if (a.split == 1) {
-    hipLaunchKernelGGL(filter_rows_bf16_kernel, grid, block, 0, s, a);
-  } else {
-    hipLaunchKernelGGL(filter_parts_kernel, dim3(a.split, rows, a.B), block, 0, s, a);
-    const int rc = nsv_launch_status();
-    if (rc) return rc;
-    hipLaunchKernelGGL(filter_merge_kernel, grid, block, 0, s, a);
-  }
-  return nsv_launch_status();
-}
+size_t part_bytes(int dtype) { return dtype == NSV_BF16 ? sizeof(Part) : sizeof(BinPart); }
+static_assert(sizeof(Part) % 16 == 0 && sizeof(BinPart) % 16 == 0 && (kMaxVocab + 7) / (kSafeSteps * kStep) < kMaxParts, "parts");
 
 }  // namespace
 
-extern "C" {
+namespace nsv_filter {
 
-size_t nsv_sample_filtered_workspace_size(int B, int V, int dtype) {
-  if (bad_rows(B, V, dtype) || V > kMaxVocab || B > 65535) return 0;
-  return parts_bytes(B, V, dtype);
+size_t rows_bytes(int rows, int V, int dtype) {
+  if (rows <= 0) return 0;
+  const int n = row_split(rows, V, dtype), most = kSlab / n;
+  return (size_t)(rows < most ? rows : most) * n * part_bytes(dtype);
 }
 
-int nsv_sample_filtered(const void* logits, int64_t row_stride, const float* temperature, const int32_t* top_k,
-                        const float* top_p, const float* min_p, const float* uniforms, int B, int V, int dtype,
-                        int32_t* out_tokens, int64_t out_stride, int32_t* kept, void* workspace, size_t workspace_bytes,
-                        void* stream) {
-  if (bad_rows(B, V, dtype) || row_stride < V || out_stride < 1) return NSV_ERR_ARG;
-  if (V > kMaxVocab || B > 65535) return NSV_ERR_UNSUPPORTED;
-  if (B == 0) return NSV_OK;
-  if (!logits || !temperature || !uniforms || !out_tokens) return NSV_ERR_ARG;
-  const size_t need = parts_bytes(B, V, dtype);
-  if (need && (!workspace || workspace_bytes < need)) return NSV_ERR_WORKSPACE;
-  FilterArgs a{};
-  a.target = logits;
-  a.t_seq = row_stride;
-  a.B = B;
-  a.K = -1;
-  a.V = V;
-  a.shift = weight_shift(V);
-  a.temperature = temperature;
-  a.top_k = top_k;
-  a.top_p = top_p;
-  a.min_p = min_p;
-  a.uniforms = uniforms;
-  a.tokens = out_tokens;
-  a.out_stride = out_stride;
-  a.kept = kept;
-  return launch_rows(a, 1, dtype, (char*)workspace, (hipStream_t)stream);
-}
-
-size_t nsv_accept_filtered_workspace_size(int B, int K, int V, int dtype) {
-  if (bad_rows(B, V, dtype) || K < 0 || K > kMaxDrafts || V > kMaxVocab || B > 65535) return 0;
-  const size_t x = layout(B, K, V, dtype, false).total, y = layout(B, K, V, dtype, true).total;
-  return x > y ? x : y;  // (with draft rows or without)
-}
-
-int nsv_accept_filtered(const void* target_logits, int64_t target_seq_stride, const void* draft_logits,
-                        int64_t draft_seq_stride, int64_t draft_row_stride, const int32_t* draft_mode,
-                        const int32_t* drafts, const int32_t* num_drafts, const float* temperature, const int32_t* top_k,
-                        const float* top_p, const float* min_p, const float* uniforms, int B, int K, int V, int dtype,
-                        int32_t* out_tokens, int32_t* out_len, void* workspace, size_t workspace_bytes, void* stream) {
-  if (bad_rows(B, V, dtype) || K < 0 || K > kMaxDrafts || target_seq_stride < K + 1) return NSV_ERR_ARG;
-  if (draft_logits && (draft_row_stride < 1 || draft_seq_stride < 0)) return NSV_ERR_ARG;
-  if (draft_mode && !draft_logits) return NSV_ERR_ARG;
-  if (V > kMaxVocab || B > 65535) return NSV_ERR_UNSUPPORTED;
-  if (B == 0) return NSV_OK;
-  if (!target_logits || (!drafts && K > 0) || !num_drafts || !temperature || !uniforms || !out_tokens || !out_len)
-    return NSV_ERR_ARG;
-  const Layout L = layout(B, K, V, dtype, K > 0 && draft_logits);
-  if (!workspace || workspace_bytes < nsv_accept_filtered_workspace_size(B, K, V, dtype)) return NSV_ERR_WORKSPACE;
-  FilterArgs a{};
-  a.target = target_logits;
-  a.t_seq = target_seq_stride * V;
-  a.t_row = V;
-  a.draft = K > 0 ? draft_logits : nullptr;
-  a.d_seq = draft_seq_stride;
-  a.d_row = draft_row_stride;
-  a.B = B;
-  a.K = K;
-  a.V = V;
-  a.shift = weight_shift(V);
-  a.temperature = temperature;
-  a.top_k = top_k;
-  a.top_p = top_p;
-  a.min_p = min_p;
-  a.uniforms = uniforms;
-  a.drafts = drafts;
-  a.num_drafts = num_drafts;
-  a.mode = draft_mode;
-  a.cuts = (RowCut*)((char*)workspace + L.cuts);
-  a.probs = (double*)((char*)workspace + L.probs);
-  a.parts = (double*)((char*)workspace + L.parts);
-  a.chunks = residual_chunks(V);
-  a.out_tokens = out_tokens;
-  a.out_len = out_len;
-  hipStream_t s = (hipStream_t)stream;
-  int rc = launch_rows(a, a.draft ? 2 * K + 1 : K + 1, dtype, (char*)workspace + L.row_parts, s);
-  if (rc) return rc;
-  if (a.draft) {
-    const dim3 grid(a.chunks, B);
-    if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_residual_kernel<uint16_t>, grid, dim3(kChunkThreads), 0, s, a);
-    else hipLaunchKernelGGL(filter_residual_kernel<float>, grid, dim3(kChunkThreads), 0, s, a);
+int launch_rows(FilterArgs& a, int dtype, void* workspace, hipStream_t s) {
+  const int total = a.rows * a.B;
+  a.split = row_split(total, a.V, dtype);
+  a.row_parts = workspace;
+  const int most = kSlab / a.split;
+  for (a.row0 = 0; a.row0 < total; a.row0 += most) {
+    const int rows = total - a.row0 < most ? total - a.row0 : most;
+    const dim3 parts(a.split, rows), block(kRowThreads);
+    if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_count_kernel, parts, block, 0, s, a);
+    else hipLaunchKernelGGL(filter_bin_kernel, parts, block, 0, s, a);
+    int rc = nsv_launch_status();
+    if (rc) return rc;
+    if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_merge_kernel, dim3(rows), block, 0, s, a);
+    else hipLaunchKernelGGL(filter_list_kernel, dim3(rows), block, 0, s, a);
     if ((rc = nsv_launch_status())) return rc;
   }
-  if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_finish_kernel<uint16_t>, dim3(B), dim3(kChunkThreads), 0, s, a);
-  else hipLaunchKernelGGL(filter_finish_kernel<float>, dim3(B), dim3(kChunkThreads), 0, s, a);
-  return nsv_launch_status();
+  return NSV_OK;
 }
 
-}  // extern "C"
+}  // namespace nsv_filter

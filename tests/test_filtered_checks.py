@@ -36,7 +36,7 @@ def test_sample_shapes():
     assert _sample(B=0) == 0
     size = _lib.lib().nsv_sample_filtered_workspace_size
     need = size(2, 151936, 1)
-    assert need > 0 and size(2, 151936, 0) == size(2, (1 << 20) + 1, 1) == size(-1, 100, 1) == 0
+    assert need > 0 and size(2, (1 << 20) + 1, 1) == size(-1, 100, 1) == 0
     assert _sample(V=151936, pitch=151936, ws=None) == _sample(V=151936, pitch=151936, ws_bytes=need - 1) == WORKSPACE
 
 

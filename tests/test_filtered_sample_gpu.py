@@ -66,6 +66,31 @@ def test_many_draws_of_a_row(dtype, setting):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_cuts_between_close_values(dtype):
+    """A lone maximum whose next tokens lie in a range that might have passed;
+    more equal and close tokens than are looked at one by one; temperatures at
+    which one range of values spans many orders of weight."""
+    print(f"case: sample_filtered close values {dtype}", flush=True)
+    V = 30000
+    x = logits(3, 8, V, dtype)
+    x[0] = x[0].clamp_max(8.0)
+    x[0, 77] = 8.9
+    x[1] = x[1].clamp_max(8.0)
+    x[1, [99, 700]] = 8.9
+    x[2, ::3] = 5.0                                              # 10,000 equal ones
+    x[3] = 5.0 + logits(4, 1, V, "f32")[0].to(x.dtype) * 1e-3    # all within a few of the type's steps, or fp32's
+    x[4] = -5.0 - logits(5, 1, V, "f32")[0].abs().to(x.dtype) * 1e-4
+    x[5] = logits(6, 1, V, dtype)[0] * 1e-6
+    x[6, 5:] = -np.inf
+    x[7] = x[7] * 1000
+    for n, f in enumerate((dict(), dict(min_p=np.full(8, 0.5)), dict(top_p=np.full(8, 0.4)), dict(top_k=np.full(8, 1000)),
+                           dict(top_k=np.full(8, 5000), top_p=np.full(8, 0.9), min_p=np.full(8, 0.02)), dict(top_p=np.full(8, 1e-6)))):
+        f = {k: v.astype(np.int32 if k == "top_k" else np.float32) for k, v in f.items()}
+        for T in (1.0, 0.02, 30.0):
+            _check(x, dict(f, temperature=np.full(8, T, np.float32)), _uniforms(n, 8))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 def test_extreme_settings(dtype):
     print(f"case: sample_filtered extremes {dtype}", flush=True)
     V, nan, inf = 3001, np.nan, np.inf
@@ -145,12 +170,13 @@ def test_values_of_most_tokens(dtype):
         assert _check(x, dict(f, **more), _uniforms(n, 6), got[:6], kept[:6]) == 6
 
 
-@pytest.mark.parametrize("B,V", [(33, 16384), (65, 20011), (129, 20011), (300, 9001), (260, 70001)])
-def test_many_rows(B, V):
-    """Rows counted in parts, and whole ones."""
-    print(f"case: sample_filtered {B} rows of {V}", flush=True)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("B,V", [(33, 16384), (65, 20011), (129, 20011), (1100, 1201), (300, 70001)])
+def test_many_rows(B, V, dtype):
+    """Rows in one part and in several, of one launch and of several."""
+    print(f"case: sample_filtered {B} rows of {V} {dtype}", flush=True)
     for shape in ("peaked", "levels"):
-        assert _check(logits(B, B, V, "bf16", shape), settings(B, B), _uniforms(B, B)) == B
+        assert _check(logits(B, B, V, dtype, shape), settings(B, B), _uniforms(B, B)) == B
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
