@@ -67,7 +67,7 @@ struct FilterArgs {
   int rows;                // per sequence: target rows, then draft rows
   int row0;                // a launch's first row, of all B * rows
   void* row_parts;         // [rows of a launch, split]
-  int split;
+  int split, steps, share; // parts of a row, workgroup steps of a part, parts of a workgroup
   double* parts;           // [B, chunks, 2]: sums of the residual and of p_target
   int chunks;
   int32_t* tokens;         // sampler: row b's at b * out_stride

@@ -85,12 +85,12 @@ struct Spot {
   uint64_t mass;           // weights before
   uint64_t weight;
 };
-enum Seek { kByCount, kReach, kAbove, kBeyond };
+enum { kByCount, kReach, kAbove, kBeyond };
 
 // The last value with: tokens before it < goal (kByCount); weights before it
 // < goal (kReach) or <= goal (kBeyond), and a weight of its own.
 template <typename T>
-__device__ Spot seek(Seek kind, double goal, const T* row, int V, float top, double inv_t, double scale, RowLds& s) {
+__device__ __forceinline__ Spot seek(int kind, double goal, const T* row, int V, float top, double inv_t, double scale, RowLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   Spot at{0u, 0u, 0u, 0ull, 0ull};
   constexpr int kShift[3] = {21, 10, 0}, kWidth[3] = {11, 11, 10};
@@ -156,7 +156,7 @@ __device__ Spot seek(Seek kind, double goal, const T* row, int V, float top, dou
 
 // index of the token with j of its value before it
 template <typename T>
-__device__ int index_of(float value, uint32_t j, const T* row, int V, RowLds& s) {
+__device__ __forceinline__ int index_of(float value, uint32_t j, const T* row, int V, RowLds& s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int steps = (V + kStep - 1) / kStep;
   __syncthreads();
@@ -202,102 +202,12 @@ __device__ int index_of(float value, uint32_t j, const T* row, int V, RowLds& s)
   return (int)s.hit_cbefore;
 }
 
-// What the filters leave of a row, and its sample of u where one is wanted.
-template <typename T>
-__device__ RowCut filter_row(const FilterArgs& a, int b, const T* row, bool sampled, float u, bool ends, RowLds& s) {
-  const int V = a.V;
-  const float T_ = a.temperature[b];
-  RowCut out;
-  // the argmax: NaN above all, equal values by the lower index
-  uint64_t best = 0;
-  each<T>(row, V, [&](int i, float x) {
-    const uint32_t k = x != x ? 0xffffffffu : ~order_bits(x);
-    const uint64_t key = ((uint64_t)k << 32) | (uint32_t)~i;
-    best = key > best ? key : best;
-  });
-  best = block_max(best, s);
-  const int first = (int)~(uint32_t)best;
-  const bool nan = (uint32_t)(best >> 32) == 0xffffffffu;
-  out.top = nan ? __builtin_nanf("") : order_value(~(uint32_t)(best >> 32));
-  out.cut = out.top;
-  out.last = out.token = first;
-  out.kept = 1;
-  out.pad = 0;
-  out.total = 1.0;
-  if (is_greedy(T_) || nan || out.top == -__builtin_inff()) return out;  // uniform
-
-  const double inv_t = 1.0 / (double)T_, scale = (double)(1ull << a.shift);
-  const float top = out.top;
-  if (threadIdx.x < 256) s.tab[threadIdx.x] = kExp2Frac256[threadIdx.x];
-  const int k = a.top_k ? a.top_k[b] : 0;
-  const double p = a.top_p ? (double)a.top_p[b] : 1.0, m = a.min_p ? (double)a.min_p[b] : 0.0;
-  out.kept = V;
-  out.cut = -__builtin_inff();
-  out.last = V - 1;
-  __syncthreads();
-  uint64_t total;
-  if (k > 0 && k < V) {
-    const Spot at = seek<T>(kByCount, (double)k, row, V, top, inv_t, scale, s);
-    out.kept = k;
-    out.cut = order_value(at.key);
-    out.last = (uint32_t)k - at.before == at.count ? V - 1 : -(int)((uint32_t)k - at.before);  // (negative: to be looked up)
-    total = at.mass + (uint64_t)((uint32_t)k - at.before) * at.weight;
-  } else {
-    uint64_t sum = 0;
-    each<T>(row, V, [&](int, float x) { sum += fixed_weight(weight_of(x, top, inv_t, s.tab), scale); });
-    total = block_sum(sum, s);
-  }
-  if (p < 1.0) {
-    const double goal = fmax(p * (double)total, 0.5);  // (the first token stays)
-    const Spot at = seek<T>(kReach, goal, row, V, top, inv_t, scale, s);
-    const double need = ceil((goal - (double)at.mass) / (double)at.weight);
-    const uint32_t n = (uint32_t)fmin(fmax(need, 1.0), (double)at.count);
-    if ((int)(at.before + n) < out.kept) {
-      out.kept = (int)(at.before + n);
-      out.cut = order_value(at.key);
-      out.last = n == at.count ? V - 1 : -(int)n;
-      total = at.mass + (uint64_t)n * at.weight;
-    }
-  }
-  if (m > 0.0) {
-    uint64_t sum = 0, count = 0, low = 0;  // low: the furthest key along the order
-    each<T>(row, V, [&](int, float x) {
-      const double w = weight_of(x, top, inv_t, s.tab);
-      if (x != top && !(w >= m)) return;
-      sum += fixed_weight(w, scale);
-      ++count;
-      const uint64_t key = order_bits(x);
-      low = key > low ? key : low;
-    });
-    count = block_sum(count, s);
-    if ((int)count < out.kept) {
-      out.kept = (int)count;
-      out.last = V - 1;
-      total = block_sum(sum, s);
-      out.cut = order_value((uint32_t)block_max(low, s));
-    }
-  }
-  out.total = (double)total / scale;
-  if (sampled) {
-    const double goal = unit(u) * (double)total;
-    const Spot at = seek<T>(kBeyond, goal, row, V, top, inv_t, scale, s);
-    double j = floor((goal - (double)at.mass) / (double)at.weight);
-    j = fmin(fmax(j, 0.0), (double)(at.count - 1));
-    j = fmin(j, (double)(out.kept - 1 - (int)at.before));
-    out.token = index_of<T>(order_value(at.key), (uint32_t)j, row, V, s);
-  }
-  if (out.last < 0) out.last = ends ? index_of<T>(out.cut, (uint32_t)(-out.last - 1), row, V, s) : V - 1;
-  return out;
-}
-
-
 // ---------------------------------------------------------------------------
 // rows in parts
 // ---------------------------------------------------------------------------
-constexpr int kAhead = 4;      // vectors a thread loads ahead of those it works on
-constexpr int kMaxParts = 32;  // of a row, by a workgroup each ..
-constexpr int kMaxSplit = 8;   // .. and this many at most where one would do
-constexpr int kSlab = 1024;    // parts of a launch: their counts take 128 MiB at most
+constexpr int kMaxParts = 32;  // of a row ..
+constexpr int kFewParts = 8;   // .. where they may be as long as that takes: the second kernel reads them one after another
+constexpr int kSlab = 1024;    // parts of a launch: what they leave takes 128 MiB at most
 
 // A row as 16-byte vectors of N elements: vector g holds elements N g - skew ..
 // + N - 1; what lies outside the row counts as -inf.
@@ -306,7 +216,7 @@ struct Row {
   static constexpr int N = 16 / sizeof(T);
   const T* at;
   int V, skew, vecs;
-  __device__ Row(const T* row, int V_) : at(row), V(V_), skew((int)(((uintptr_t)row & 15) / sizeof(T))) {
+  __device__ __forceinline__ Row(const T* row, int V_) : at(row), V(V_), skew((int)(((uintptr_t)row & 15) / sizeof(T))) {
     vecs = (V + skew + N - 1) / N;
   }
   __device__ __forceinline__ u32x4 load(int g) const {
@@ -327,33 +237,32 @@ struct Row {
     return v;
   }
 };
-template <typename T>
-__device__ __forceinline__ int part_vecs(const Row<T>& row, int parts) { return (row.vecs + parts - 1) / parts; }
-
 // f(step, vector, whether there is one) of the vectors lo .. hi - 1, a
-// workgroup's threads together, kAhead of them loaded ahead.  The loop stays
-// rolled: a row kept in registers (one unrolled body per vector) saved its
-// second reading, and cost more in instructions fetched once.
-template <typename T, typename F>
+// workgroup's threads together, AHEAD of them loaded ahead (a step is 16 KiB,
+// and a compute unit takes some ten of them in the time of one's way from
+// memory).  The loop stays rolled: a row kept in registers (one unrolled body
+// per vector) saved its second reading, and cost more in instructions fetched
+// once.
+template <int AHEAD, typename T, typename F>
 __device__ __forceinline__ void each_vec(const Row<T>& row, int lo, int hi, F f) {
   const int steps = (hi - lo + kRowThreads - 1) / kRowThreads;
-  u32x4 v[kAhead];
+  u32x4 v[AHEAD];
   int g = lo + threadIdx.x;
 #pragma unroll
-  for (int j = 0; j < kAhead; ++j) v[j] = row.load(min(g + j * kRowThreads, hi - 1));
+  for (int j = 0; j < AHEAD; ++j) v[j] = row.load(min(g + j * kRowThreads, hi - 1));
 #pragma unroll 1
-  for (int it = 0; it < steps; it += kAhead) {
-    u32x4 w[kAhead] = {};
-    if (it + kAhead < steps) {
+  for (int it = 0; it < steps; it += AHEAD) {
+    u32x4 w[AHEAD] = {};
+    if (it + AHEAD < steps) {
 #pragma unroll
-      for (int j = 0; j < kAhead; ++j) w[j] = row.load(min(g + (kAhead + j) * kRowThreads, hi - 1));
+      for (int j = 0; j < AHEAD; ++j) w[j] = row.load(min(g + (AHEAD + j) * kRowThreads, hi - 1));
     }
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j)
+    for (int j = 0; j < AHEAD; ++j)
       if (it + j < steps) f(it + j, v[j], g + j * kRowThreads < hi);
 #pragma unroll
-    for (int j = 0; j < kAhead; ++j) v[j] = w[j];
-    g += kAhead * kRowThreads;
+    for (int j = 0; j < AHEAD; ++j) v[j] = w[j];
+    g += AHEAD * kRowThreads;
   }
 }
 
@@ -361,7 +270,7 @@ __device__ __forceinline__ void each_vec(const Row<T>& row, int lo, int hi, F f)
 struct Settings {
   float T, p, least, u;
   int k;
-  bool sampled, ends;
+  bool has_k, has_p, has_least, sampled, ends;
   double inv_t;
 };
 // (as vector loads: scalar ones would be waited for with the LDS writes)
@@ -369,25 +278,127 @@ __device__ __forceinline__ Settings settings_of(const FilterArgs& a, int b, bool
   int vb = b;
   int64_t vu = at_u;
   asm volatile("" : "+v"(vb), "+v"(vu));
+  // (no load in a branch: each would be waited for before the next is issued)
+  const int32_t* k = a.top_k ? a.top_k : (const int32_t*)a.temperature;
+  const float* p = a.top_p ? a.top_p : a.temperature;
+  const float* least = a.min_p ? a.min_p : a.temperature;
   Settings f;
   f.T = a.temperature[vb];
-  f.k = a.top_k ? a.top_k[vb] : 0;
-  f.p = a.top_p ? a.top_p[vb] : 1.f;
-  f.least = a.min_p ? a.min_p[vb] : 0.f;
+  f.k = k[vb];
+  f.p = p[vb];
+  f.least = least[vb];
   f.u = a.uniforms[vu];
+  f.has_k = a.top_k != nullptr;
+  f.has_p = a.top_p != nullptr;
+  f.has_least = a.min_p != nullptr;
   f.sampled = sampled;
   f.ends = ends;
   return f;
 }
 
-// .. for scalar registers and uniform branches
+// .. as they count, in scalar registers
 __device__ __forceinline__ void make_uniform(Settings& f) {
   auto one = [](float x) { return __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(x))); };
   f.T = one(f.T);
-  f.p = one(f.p);
-  f.least = one(f.least);
+  f.p = f.has_p ? one(f.p) : 1.f;
+  f.least = f.has_least ? one(f.least) : 0.f;
   f.u = one(f.u);
-  f.k = __builtin_amdgcn_readfirstlane(f.k);
+  f.k = f.has_k ? __builtin_amdgcn_readfirstlane(f.k) : 0;
+}
+
+// What the filters leave of a row, and its sample of u where one is wanted, by
+// radix descent.
+__device__ __forceinline__ RowCut radix_row(const float* row, int V, int shift, const Settings& f, RowLds& s) {
+  RowCut out;
+  // the argmax: NaN above all, equal values by the lower index
+  uint64_t best = 0;
+  each<float>(row, V, [&](int i, float x) {
+    const uint32_t k = x != x ? 0xffffffffu : ~order_bits(x);
+    const uint64_t key = ((uint64_t)k << 32) | (uint32_t)~i;
+    best = key > best ? key : best;
+  });
+  best = block_max(best, s);
+  const int first = (int)~(uint32_t)best;
+  const bool nan = (uint32_t)(best >> 32) == 0xffffffffu;
+  out.top = nan ? __builtin_nanf("") : order_value(~(uint32_t)(best >> 32));
+  out.cut = out.top;
+  out.last = out.token = first;
+  out.kept = 1;
+  out.pad = 0;
+  out.total = 1.0;
+  if (is_greedy(f.T) || nan || out.top == -__builtin_inff()) return out;  // uniform
+
+  const double inv_t = 1.0 / (double)f.T, scale = (double)(1ull << shift);
+  const float top = out.top;
+  if (threadIdx.x < 256) s.tab[threadIdx.x] = kExp2Frac256[threadIdx.x];
+  out.kept = V;
+  out.cut = -__builtin_inff();
+  out.last = V - 1;
+  __syncthreads();
+  uint64_t total = 0;
+  each<float>(row, V, [&](int, float x) { total += fixed_weight(weight_of(x, top, inv_t, s.tab), scale); });
+  total = block_sum(total, s);
+  uint32_t value = 0, rank = 0;
+  int cut_rank = -1;
+#pragma unroll 1
+  for (int kind = 0; kind < 4; ++kind) {
+    double goal = 0.0;
+    if (kind == kByCount) {
+      if (f.k <= 0 || f.k >= V) continue;
+      goal = (double)f.k;
+    } else if (kind == kReach) {
+      if (!(f.p < 1.f)) continue;
+      goal = fmax((double)f.p * (double)total, 0.5);  // (the first token stays)
+    } else if (kind == kAbove) {
+      if (!(f.least > 0.f)) continue;
+      uint64_t sum = 0, count = 0, low = 0;  // low: the furthest key along the order
+      each<float>(row, V, [&](int, float x) {
+        const double w = weight_of(x, top, inv_t, s.tab);
+        if (x != top && !(w >= (double)f.least)) return;
+        sum += fixed_weight(w, scale);
+        ++count;
+        const uint64_t key = order_bits(x);
+        low = key > low ? key : low;
+      });
+      count = block_sum(count, s);
+      if ((int)count >= out.kept) continue;
+      out.kept = (int)count;
+      cut_rank = -1;
+      total = block_sum(sum, s);
+      out.cut = order_value((uint32_t)block_max(low, s));
+      continue;
+    } else {
+      if (!f.sampled) continue;
+      goal = unit(f.u) * (double)total;
+    }
+    const Spot at = seek<float>(kind, goal, row, V, top, inv_t, scale, s);
+    if (kind == kBeyond) {
+      const double j = fmin(floor((goal - (double)at.mass) / (double)at.weight),
+                            (double)min((int)at.count, out.kept - (int)at.before) - 1.0);
+      value = at.key;
+      rank = (uint32_t)fmax(j, 0.0);
+      continue;
+    }
+    uint32_t stay = (uint32_t)f.k - at.before;
+    if (kind == kReach) {
+      const double need = ceil((goal - (double)at.mass) / (double)at.weight);
+      stay = (uint32_t)fmin(fmax(need, 1.0), (double)at.count);
+    }
+    if ((int)(at.before + stay) >= out.kept) continue;
+    out.kept = (int)(at.before + stay);
+    out.cut = order_value(at.key);
+    cut_rank = stay < at.count ? (int)stay - 1 : -1;
+    total = at.mass + (uint64_t)stay * at.weight;
+  }
+  out.total = (double)total / scale;
+#pragma unroll 1
+  for (int which = 0; which < 2; ++which) {
+    if (which ? !f.ends || cut_rank < 0 : !f.sampled) continue;  // uniform
+    const int at = index_of<float>(which ? out.cut : order_value(value), which ? (uint32_t)cut_rank : rank, row, V, s);
+    if (which) out.last = at;
+    else out.token = at;
+  }
+  return out;
 }
 
 // ---------------------------------------------------------------------------
@@ -399,13 +410,13 @@ constexpr int kMaxHeavy = kMaxVocab / 65536 + 1;
 
 struct CountLds {
   uint32_t bin[32768];         // counts of values 2i (low half) and 2i + 1
-  uint32_t occurs[kGroups / 32];
   // groups that occur, along the order
   double mass[kGroups];        // weights of a group, first of its first value's
   double before[kGroups];      // weights before a group
   uint32_t count[kGroups];
   uint32_t cbefore[kGroups];
   uint32_t ref[kGroups];       // group << 16 | bits of its first value that occurs
+  uint16_t gid[kGroups];       // the groups themselves
   uint32_t found[kMaxSteps * kRowWaves];
   double tab[256];
   uint32_t heavy[kMaxHeavy], heavy_count[kMaxHeavy];  // counts beside the bins
@@ -456,27 +467,6 @@ __device__ __forceinline__ uint32_t word_of(int g) {
 }
 __device__ __forceinline__ int group_of(uint32_t value) {
   return value & 0x8000u ? (int)(value >> 7) : kGroups / 2 - 1 - (int)(value >> 7);
-}
-
-// Which of a wave's 32 groups have values, as bits; f(group, a lane's word) of
-// each that has.
-template <typename F>
-__device__ __forceinline__ uint32_t own_groups(const uint32_t* bin, F f) {
-  const int wave = threadIdx.x >> 6;
-  uint32_t has = 0;
-#pragma unroll 1
-  for (int i = 0; i < 32; i += 8) {
-    uint32_t w[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) w[j] = bin[word_of(32 * wave + i + j)];
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (__ballot(w[j] != 0)) {  // uniform
-        has |= 1u << (i + j);
-        f(32 * wave + i + j, w[j]);
-      }
-  }
-  return has;
 }
 
 // The n-th group that occurs; lanes 0..15 hold the words of bits in `occurs`
@@ -593,7 +583,7 @@ __device__ __forceinline__ bool has_value(const u32x4& v, uint32_t both, uint32_
 __device__ __forceinline__ void find_token(const Row<uint16_t>& row, int lo, int hi, uint32_t value, uint32_t rank, CountLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const uint32_t mask = value ? ~0u : 0x7fff7fffu, both = value | (value << 16);  // (+0: -0 too)
-  each_vec(row, lo, hi, [&](int it, const u32x4& v, bool in) {
+  each_vec<kSafeSteps>(row, lo, hi, [&](int it, const u32x4& v, bool in) {
     uint32_t all = 0;
     if (__ballot(in && has_value(v, both, mask))) {
       const uint32_t n = in ? matches(v, both, mask) : 0u;
@@ -639,19 +629,16 @@ __device__ __forceinline__ void find_token(const Row<uint16_t>& row, int lo, int
   __syncthreads();
 }
 
-// Counts and weights of the groups that occur, the waves in turn; their number.
-__device__ __forceinline__ int weigh_groups(double inv_t, int heavies, CountLds& s) {
+// Counts and weights of the groups that occur (s.gid), the waves in turn.
+__device__ __forceinline__ void weigh_groups(double inv_t, int groups, int heavies, CountLds& s) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  uint32_t occurs = lane < kGroups / 32 ? s.occurs[lane] : 0u;
-  // (-0 counts with +0, the last value of the positive ones)
-  if (lane == kGroups / 64 - 1 && (s.occurs[kGroups / 64] & 1)) occurs |= 1u << 31;
-  const uint32_t upto = wave_scan((uint32_t)__popc(occurs));
-  const int groups = (int)lane_u32(upto, 63);
 #pragma unroll 1
   for (int n = wave; n < groups; n += kRowWaves) {
-    const int g = nth_group(n, occurs, upto);
+    const int g = __builtin_amdgcn_readfirstlane(s.gid[n]);
     const Pair q = pair_of(s, heavies, g);
-    if ((q.c1 && (q.v1 & 0x7fffu) > 0x7f80u) || (q.c2 && (q.v2 & 0x7fffu) > 0x7f80u)) s.nan = 1;
+    if (g == 0 || g == kGroups - 1) {  // uniform: infinities and NaNs
+      if ((q.c1 && (q.v1 & 0x7fffu) > 0x7f80u) || (q.c2 && (q.v2 & 0x7fffu) > 0x7f80u)) s.nan = 1;
+    }
     const uint64_t y1 = __ballot(q.c1 > 0), y2 = __ballot(q.c2 > 0);
     const int l1 = y1 ? __ffsll((long long)y1) - 1 : 64, l2 = y2 ? __ffsll((long long)y2) - 1 : 64;
     const uint32_t ref = lane_u32(l1 <= l2 ? q.v1 : q.v2, min(min(l1, l2), 63));
@@ -665,7 +652,6 @@ __device__ __forceinline__ int weigh_groups(double inv_t, int heavies, CountLds&
       s.ref[n] = ((uint32_t)g << 16) | ref;
     }
   }
-  return groups;
 }
 
 // What the filters leave, from the weighed groups, by one wave: into s.
@@ -780,33 +766,62 @@ __device__ __forceinline__ RowCut look_up(int V, const CountLds& s, F find) {
   return out;
 }
 
-// What one workgroup counted of a row (at most kSafeSteps steps, so that 16
-// bits hold every count): which groups occur, and the words of those that do.
+// What a part of a row holds (at most kSafeSteps steps of a workgroup, so that
+// 16 bits hold every count): which groups occur, and the words of those that do.
 struct Part {
   uint32_t occurs[kGroups / 32];
-  uint32_t word[kGroups * 64];
+  uint32_t word[32768];
 };
 
-__device__ __forceinline__ void count_part(const Row<uint16_t>& row, int part, int parts, uint32_t* bin, Part* out) {
+// A part's counts out of LDS, which is clear for the next one.  A wave takes
+// 2,048 words, four a lane at a time: the 16 lanes of a group write it whole or
+// not at all.
+__device__ __forceinline__ void put_part(uint32_t* bin, Part* out) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int per = part_vecs(row, parts), lo = part * per, hi = min(lo + per, row.vecs);
+  uint32_t has = 0;  // of groups in the order of their words
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int at = 2048 * wave + 256 * i + 4 * lane;
+    const u32x4 w = *reinterpret_cast<const u32x4*>(bin + at);
+    const uint64_t any = __ballot((w[0] | w[1] | w[2] | w[3]) != 0);
+    if ((any >> (lane & 48)) & 0xffffu) {
+      *reinterpret_cast<u32x4*>(out->word + at) = w;
+      *reinterpret_cast<u32x4*>(bin + at) = u32x4{0u, 0u, 0u, 0u};
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) has |= ((any >> (16 * g)) & 0xffffu ? 1u : 0u) << (4 * i + g);
+  }
+  // (positive values: the order is that of falling words)
+  if (lane == 0) out->occurs[wave < 8 ? 7 - wave : wave] = wave < 8 ? __brev(has) : has;
+}
+
+// Parts first .. last - 1 of `steps` steps each, counted by one workgroup one
+// after another; the next one's first vectors are on their way meanwhile.
+__device__ __forceinline__ void count_parts(const Row<uint16_t>& row, int first, int last, int steps, uint32_t* bin, Part* out) {
+  const int lane = threadIdx.x & 63;
+  const int lo = first * steps * kRowThreads, hi = min(last * steps * kRowThreads, row.vecs);
   clear_bins(bin);
   lds_barrier();
   uint32_t heavy = ~0u, many = 0;
-  if (lo < hi)
-    each_vec(row, lo, hi, [&](int, const u32x4& v, bool in) {
-      if (in) count_vec(bin, v, heavy, many);
-    });
-  heavy = (uint32_t)__builtin_amdgcn_readfirstlane((int)heavy);
-  many = (uint32_t)__builtin_amdgcn_readfirstlane((int)many);
-  if (lane == 0 && many) atomicAdd(&bin[heavy >> 1], many << ((heavy & 1) << 4));
-  __syncthreads();
-  const uint32_t has = own_groups(bin, [&](int g, uint32_t w) { out->word[64 * g + lane] = w; });
-  if (lane == 0) out->occurs[wave] = has;
+  int left = steps;
+  each_vec<4>(row, lo, hi, [&](int it, const u32x4& v, bool in) {
+    if (in) count_vec(bin, v, heavy, many);
+    if (--left && (it + 1) * kRowThreads < hi - lo) return;  // uniform
+    // (a wave's lanes count alike, but those without a last vector)
+    const uint32_t h = (uint32_t)__builtin_amdgcn_readfirstlane((int)heavy), m = (uint32_t)__builtin_amdgcn_readfirstlane((int)many);
+    if (lane == 0 && m) atomicAdd(&bin[h >> 1], m << ((h & 1) << 4));
+    lds_barrier();
+    put_part(bin, out);
+    lds_barrier();
+    ++out;
+    left = steps;
+    heavy = ~0u;
+    many = 0;
+  });
 }
 
-// filter_row for bf16, from the counts of a row's parts.
-__device__ __forceinline__ RowCut merge_row(const Row<uint16_t>& row, Settings f, const Part* in, int parts, CountLds& s) {
+// A bf16 row from the counts of its parts.
+__device__ __forceinline__ RowCut merge_row(const Row<uint16_t>& row, Settings f, const Part* in, int parts, int steps, CountLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (tid < kGroups / 32 * parts) s.part_occurs[tid] = in[tid / (kGroups / 32)].occurs[tid % (kGroups / 32)];
   if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
@@ -820,45 +835,70 @@ __device__ __forceinline__ RowCut merge_row(const Row<uint16_t>& row, Settings f
 #pragma unroll 8
     for (int c = 0; c < parts; ++c) occurs |= s.part_occurs[c * (kGroups / 32) + lane];
   }
-  if (wave == 0 && lane < kGroups / 32) s.occurs[lane] = occurs;
-  if (lane == kGroups / 64 - 1 && (lane_u32(occurs, kGroups / 64) & 1)) occurs |= 1u << 31;  // (+0's group where there is -0)
+  if (lane == kGroups / 64 - 1 && (lane_u32(occurs, kGroups / 64) & 1)) occurs |= 1u << 31;  // (-0 counts with +0, the last positive value)
   const uint32_t upto = wave_scan((uint32_t)__popc(occurs));
   const int groups = (int)lane_u32(upto, 63);
+  {  // a thread per group: its place among those that occur
+    const int l = (tid >> 5) & 15;
+    const uint32_t word = (uint32_t)__shfl((int)occurs, l), before = (uint32_t)__shfl((int)upto, l) - __popc(word);
+    if (tid < kGroups && ((word >> (tid & 31)) & 1)) s.gid[before + __popc(word & ((1u << (tid & 31)) - 1))] = (uint16_t)tid;
+  }
+  __syncthreads();
+  // the words of a wave's groups, those of three groups in eight parts on their way at once
+  constexpr int kAtOnce = 3, kBatch = 8;
+  const int last = max(groups - 1, 0);
 #pragma unroll 1
-  for (int n = wave; n < groups; n += kRowWaves) {
-    const int g = nth_group(n, occurs, upto);
-    // parts that have it (the word of one that has not is whatever the memory held)
-    const uint64_t have = __ballot(lane < parts && ((s.part_occurs[min(lane, parts - 1) * (kGroups / 32) + (g >> 5)] >> (g & 31)) & 1));
-    uint32_t lo = 0, hi = 0;
+  for (int n0 = wave; n0 < groups; n0 += kAtOnce * kRowWaves) {
+    const uint32_t gids = s.gid[min(n0 + min(lane, kAtOnce - 1) * kRowWaves, last)];
+    uint32_t lo[kAtOnce] = {}, hi[kAtOnce] = {};
 #pragma unroll 1
-    for (int c0 = 0; c0 < parts; c0 += 8) {
-      uint32_t w[8];
+    for (int c0 = 0; c0 < parts; c0 += kBatch) {
+      uint32_t w[kAtOnce][kBatch];
+      uint64_t have[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = in[min(c0 + j, parts - 1)].word[64 * g + lane];
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int g = (int)lane_u32(gids, i);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const bool has = (have >> (c0 + j)) & 1;
-        lo += has ? w[j] & 0xffffu : 0u;
-        hi += has ? w[j] >> 16 : 0u;
+        for (int j = 0; j < kBatch; ++j) w[i][j] = in[min(c0 + j, parts - 1)].word[word_of(g)];
       }
-    }
-    const int64_t word = g >= kGroups / 2 ? 64 * g + lane : 64 * (kGroups / 2 - 1 - g) + 63 - lane;
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      uint32_t& c = half ? hi : lo;
-      if (c < 65536) continue;  // (rows of one value mostly)
-      const int at = atomicAdd(&s.heavies, 1);
-      s.heavy[at] = 2 * (uint32_t)word + half;
-      s.heavy_count[at] = c;
-      c = 0;
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int g = (int)lane_u32(gids, i), c = c0 + min(lane, kBatch - 1);
+        have[i] = __ballot(c < parts && ((s.part_occurs[min(c, parts - 1) * (kGroups / 32) + (g >> 5)] >> (g & 31)) & 1));
+      }
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i)
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+          // (the word of a group that a part has not is whatever the memory held)
+          const uint32_t word = (have[i] >> j) & 1 ? w[i][j] : 0u;
+          lo[i] += word & 0xffffu;
+          hi[i] += word >> 16;
+        }
     }
-    s.bin[word] = lo | (hi << 16);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (n0 + i * kRowWaves >= groups) break;  // uniform
+      const uint32_t word = word_of((int)lane_u32(gids, i));
+      if (__ballot((lo[i] | hi[i]) >= 65536)) {  // (rows of one value mostly)
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          uint32_t& c = half ? hi[i] : lo[i];
+          if (c < 65536) continue;
+          const int at = atomicAdd(&s.heavies, 1);
+          s.heavy[at] = 2 * word + half;
+          s.heavy_count[at] = c;
+          c = 0;
+        }
+      }
+      s.bin[word] = lo[i] | (hi[i] << 16);
+    }
   }
   make_uniform(f);
   f.inv_t = is_greedy(f.T) ? 1.0 : 1.0 / (double)f.T;
   __syncthreads();
   const int heavies = s.heavies;
-  weigh_groups(f.inv_t, heavies, s);
+  weigh_groups(f.inv_t, groups, heavies, s);
   __syncthreads();
   if (s.nan) return nan_row(row, s);  // uniform
   if (wave == 0) decide(f, row.V, groups, heavies, s);
@@ -867,21 +907,19 @@ __device__ __forceinline__ RowCut merge_row(const Row<uint16_t>& row, Settings f
     // the part that holds the token, by its counts of the value
     uint32_t c = 0;
     auto count = [&](uint32_t v) {
-      const int g = group_of(v);
-      if (lane >= parts || !((s.part_occurs[lane * (kGroups / 32) + (g >> 5)] >> (g & 31)) & 1)) return;
-      const uint32_t w = v >> 1, at = g >= kGroups / 2 ? w & 63 : 63 - (w & 63);
-      const uint32_t both = in[lane].word[64 * g + at];
+      const int at = group_of(v);
+      if (lane >= parts || !((s.part_occurs[lane * (kGroups / 32) + (at >> 5)] >> (at & 31)) & 1)) return;
+      const uint32_t both = in[lane].word[v >> 1];
       c += (v & 1) ? both >> 16 : both & 0xffffu;
     };
     count(value);
     if (value == 0) count(0x8000u);
     const uint32_t upto_c = wave_scan(c);
     const int part = max(__ffsll((long long)__ballot(upto_c > rank)) - 1, 0);
-    const int per = part_vecs(row, parts), lo = part * per;
-    find_token(row, lo, min(lo + per, row.vecs), value, rank - lane_u32(upto_c - c, part), s);
+    const int lo = part * steps * kRowThreads;
+    find_token(row, lo, min(lo + steps * kRowThreads, row.vecs), value, rank - lane_u32(upto_c - c, part), s);
   });
 }
-
 
 // ---------------------------------------------------------------------------
 // fp32 rows by bins
@@ -891,6 +929,7 @@ constexpr int kBins32 = 1 << (32 - kBinShift);
 constexpr int kBinGroups = kBins32 / 64;
 constexpr int kList = 4096;             // tokens looked at one by one
 constexpr int kSubBins = 1024;
+constexpr int kHead = kBinGroups / 32 + 4;
 
 // What one workgroup added up of a row: its maximum, and the bins of the
 // groups of 64 that occur: tokens above -inf, and their weights as integers of
@@ -899,7 +938,7 @@ constexpr int kSubBins = 1024;
 struct BinPart {
   uint32_t occurs[kBinGroups / 32];
   float top;
-  uint32_t nan, pad[2];
+  uint32_t nan, pad[2];        // (kHead words up to here)
   uint32_t count[kBins32];
   unsigned long long mass[kBins32];
 };
@@ -915,24 +954,23 @@ struct BinLds {
 __device__ __forceinline__ uint32_t bin_of(float x) { return order_bits(x) >> kBinShift; }
 __device__ __forceinline__ float bin_edge(uint32_t bin) { return order_value(bin << kBinShift); }
 
-__device__ __forceinline__ void bin_part(const Row<float>& row, int part, int parts, float T, int shift, BinLds& s, BinPart* out) {
+__device__ __forceinline__ void bin_part(const Row<float>& row, int part, int steps, float T, int shift, BinLds& s, BinPart* out) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int per = part_vecs(row, parts), lo = part * per, hi = min(lo + per, row.vecs);
+  const int lo = part * steps * kRowThreads, hi = min(lo + steps * kRowThreads, row.vecs);
   for (int i = tid; i < kBins32 / 4; i += kRowThreads) reinterpret_cast<u32x4*>(s.count)[i] = u32x4{0u, 0u, 0u, 0u};
   for (int i = tid; i < kBins32 / 2; i += kRowThreads) reinterpret_cast<u32x4*>(s.mass)[i] = u32x4{0u, 0u, 0u, 0u};
   if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
   if (tid == 0) s.nan = 0;
   float top = -__builtin_inff();
   bool nan = false;
-  if (lo < hi)
-    each_vec(row, lo, hi, [&](int, const u32x4& v, bool) {  // (a vector past the end is the last one again)
+  each_vec<4>(row, lo, hi, [&](int, const u32x4& v, bool) {  // (a vector past the end is the last one again)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = __uint_as_float(v[e]);
-        top = fmaxf(top, x);
-        nan |= x != x;
-      }
-    });
+    for (int e = 0; e < 4; ++e) {
+      const float x = __uint_as_float(v[e]);
+      top = fmaxf(top, x);
+      nan |= x != x;
+    }
+  });
   top = wave_max_dpp(top);
   if (lane == 0) s.red[wave] = top;
   __syncthreads();
@@ -954,7 +992,7 @@ __device__ __forceinline__ void bin_part(const Row<float>& row, int part, int pa
     return fixed_weight(weight_of(x, bin == top_bin ? top : bin_edge(bin), inv_t, s.tab), scale);
   };
   uint32_t heavy = 0xff800000u, many = 0;  // (-inf: none)
-  each_vec(row, lo, hi, [&](int, const u32x4& v, bool in) {
+  each_vec<2>(row, lo, hi, [&](int, const u32x4& v, bool in) {
     if (!in) return;
     // a value that many of a wave's lanes hold (a mask's) is added up beside the bins
     const uint32_t some = (uint32_t)__builtin_amdgcn_readfirstlane((int)v[0]);
@@ -996,15 +1034,23 @@ __device__ __forceinline__ void bin_part(const Row<float>& row, int part, int pa
   if (lane == 0) reinterpret_cast<uint8_t*>(out->occurs)[wave] = (uint8_t)has;
 }
 
+struct Bin {
+  uint32_t bin;
+  uint32_t before, count;  // tokens
+  double mass, weight;     // weights before; of its tokens
+};
+
 struct ListLds {
   uint32_t count[kBins32];     // tokens of a bin; at the end the indices of equal tokens
   double weight[kBins32];      // their weights
   // groups that occur, along the order
   double gweight[kBinGroups], gbefore[kBinGroups];
   uint32_t gcount[kBinGroups], gcbefore[kBinGroups], gid[kBinGroups];
-  uint32_t part_occurs[kMaxParts * kBinGroups / 32];
-  float part_top[kMaxParts];
+  uint32_t head[kMaxParts * kHead];  // of the parts
   double part_scale[kMaxParts];
+  Bin at;                      // what wave 0 found
+  float high[4], low[4];       // ranges of values to list
+  int ranges;
   uint64_t list[kList];        // order bits << 32 | index
   uint32_t sub_count[kSubBins];
   unsigned long long sub_mass[kSubBins];
@@ -1020,15 +1066,9 @@ union RowLds32 {
   RowLds radix;
 };
 
-struct Bin {
-  uint32_t bin;
-  uint32_t before, count;  // tokens
-  double mass, weight;     // weights before; of its tokens
-};
-
 // The last bin with: tokens before it < goal (kByCount); weights before it <
 // goal (kReach) or <= goal (kBeyond), and a weight of its own; a largest
-// possible weight >= goal (kAbove).  By every wave alike.
+// possible weight >= goal (kAbove).  By one wave.
 __device__ __forceinline__ Bin seek_bin(int kind, double goal, const ListLds& s, int groups, float top, double inv_t) {
   const int lane = threadIdx.x & 63;
   int n = -1;
@@ -1067,6 +1107,16 @@ __device__ __forceinline__ Bin seek_bin(int kind, double goal, const ListLds& s,
   }
 }
 
+// .. for the whole workgroup
+__device__ __forceinline__ Bin find_bin(int kind, double goal, int groups, float top, double inv_t, ListLds& s) {
+  if (threadIdx.x < 64) {
+    const Bin at = seek_bin(kind, goal, s, groups, top, inv_t);
+    if (threadIdx.x == 0) s.at = at;
+  }
+  __syncthreads();
+  return s.at;
+}
+
 // As seek, among the listed tokens of a bin.  mass, weight: integers of
 // 2^-shift of the bin's reference value.
 __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, float ref, double inv_t, double scale, ListLds& s) {
@@ -1097,12 +1147,10 @@ __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, f
       s.red2[wave] = mu;
     }
     __syncthreads();
-    uint32_t cb = at.before + cu - c;
-    uint64_t mb = at.mass + mu - m;
-    for (int i = 0; i < wave; ++i) {
-      cb += s.red[i];
-      mb += s.red2[i];
-    }
+    const uint32_t cw = lane < kRowWaves ? s.red[lane] : 0u;
+    const uint64_t mw = lane < kRowWaves ? s.red2[lane] : 0ull;
+    const uint32_t cb = at.before + cu - c + lane_u32(wave_scan(cw) - cw, wave);
+    const uint64_t mb = at.mass + mu - m + lane_u64(wave_scan(mw) - mw, wave);
     bool fits = c > 0;
     if (kind == kByCount) fits = fits && (double)cb < goal;
     else fits = fits && m > 0 && (kind == kReach ? (double)mb < goal : (double)mb <= goal);
@@ -1156,21 +1204,19 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, V = row.V;
   constexpr int kWords = kBinGroups / 32;
   fits = true;
-  if (tid < kWords * parts) s.part_occurs[tid] = in[tid / kWords].occurs[tid % kWords];
-  if (tid < parts) s.part_top[tid] = in[tid].top;
+  if (tid < kHead * parts) s.head[tid] = reinterpret_cast<const uint32_t*>(&in[tid / kHead])[tid % kHead];
   if (tid < 256) s.tab[tid] = kExp2Frac256[tid];
-  if (tid == 0) s.nan = s.listed = 0;
+  if (tid == 0) s.listed = 0;
   __syncthreads();
-  if (tid < parts && in[tid].nan) s.nan = 1;
   make_uniform(f);
-  float top = -__builtin_inff();
-  for (int c = 0; c < parts; ++c) top = fmaxf(top, s.part_top[c]);
+  const float my_top = lane < parts ? __uint_as_float(s.head[lane * kHead + kWords]) : -__builtin_inff();
+  const float top = wave_max_dpp(my_top);
+  const bool nan = __ballot(lane < parts && s.head[min(lane, parts - 1) * kHead + kWords + 1]) != 0;
   const bool greedy = is_greedy(f.T);
   const double inv_t = greedy ? 1.0 : 1.0 / (double)f.T, scale = (double)(1ull << shift);
-  if (tid < parts) s.part_scale[tid] = weight_of(s.part_top[tid], top, inv_t, s.tab) / scale;
-  __syncthreads();
+  if (tid < parts) s.part_scale[tid] = weight_of(my_top, top, inv_t, s.tab) / scale;
   RowCut out{top, top, V - 1, 1, 0, 0, 1.0};
-  if (s.nan) {  // uniform
+  if (nan) {  // uniform
     fits = false;
     return out;
   }
@@ -1180,32 +1226,35 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   }
   // the parts' bins added up: those of a part's maximum by that, the others as integers
   uint32_t occurs = 0;
-  if (lane < kWords)
-    for (int c = 0; c < parts; ++c) occurs |= s.part_occurs[c * kWords + lane];
+  if (lane < kWords) {
+#pragma unroll 8
+    for (int c = 0; c < parts; ++c) occurs |= s.head[c * kHead + lane];
+  }
+  __syncthreads();  // part_scale
   const uint32_t upto = wave_scan((uint32_t)__popc(occurs));
   const int groups = (int)lane_u32(upto, 63);
 #pragma unroll 1
   for (int n = wave; n < groups; n += kRowWaves) {
     const int g = nth_group(n, occurs, upto);
-    const uint64_t have = __ballot(lane < parts && ((s.part_occurs[min(lane, parts - 1) * kWords + (g >> 5)] >> (g & 31)) & 1));
+    const uint64_t have = __ballot(lane < parts && ((s.head[min(lane, parts - 1) * kHead + (g >> 5)] >> (g & 31)) & 1));
     const uint32_t bin = 64 * g + lane;
     uint32_t count = 0;
     uint64_t mass = 0;
     double weight = 0.0;
 #pragma unroll 1
-    for (int c0 = 0; c0 < parts; c0 += 4) {
-      uint32_t pc[4];
-      unsigned long long pm[4];
+    for (int c0 = 0; c0 < parts; c0 += 8) {
+      uint32_t pc[8];
+      unsigned long long pm[8];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         const BinPart& p = in[min(c0 + j, parts - 1)];
         pc[j] = p.count[bin];
         pm[j] = p.mass[bin];
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int j = 0; j < 8; ++j) {
         if (!((have >> (c0 + j)) & 1)) continue;  // uniform (what a part has not is whatever the memory held)
-        const uint32_t tb = bin_of(s.part_top[c0 + j]);
+        const uint32_t tb = bin_of(__uint_as_float(lane_u32(__float_as_uint(my_top), c0 + j)));
         count += pc[j];
         if ((tb >> 6) == (uint32_t)g && bin == tb) weight += (double)pm[j] * s.part_scale[c0 + j];
         else mass += pm[j];
@@ -1244,71 +1293,88 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   total = s.gbefore[groups - 1] + s.gweight[groups - 1];
   tokens = s.gcbefore[groups - 1] + s.gcount[groups - 1];
 
-  // ranges of bins, from the least and the most that each cut may leave (all waves alike)
+  // ranges of bins, from the least and the most that each cut may leave
   const double tiny = 0x1p-1000, slack = 0x1p-30;  // (the sums' own error is below 2^-40)
   const bool by_count = !greedy && f.k > 0 && f.k < V && (uint32_t)f.k < tokens, reach = !greedy && f.p < 1.f,
-             above = !greedy && f.least > 0.f;
-  float hi[4], lo[4];
-  int ranges = 0;
-  auto take = [&](uint32_t first, uint32_t last) {
-    const float h = bin_edge(first), l = order_value(((last + 1) << kBinShift) - 1);
-    hi[0] = ranges == 0 ? h : hi[0];
-    lo[0] = ranges == 0 ? l : lo[0];
-    hi[1] = ranges == 1 ? h : hi[1];
-    lo[1] = ranges == 1 ? l : lo[1];
-    hi[2] = ranges == 2 ? h : hi[2];
-    lo[2] = ranges == 2 ? l : lo[2];
-    hi[3] = ranges == 3 ? h : hi[3];
-    lo[3] = ranges == 3 ? l : lo[3];
-    ++ranges;
-  };
-  double least = total, most = total;
-  if (greedy) take(bin_of(top), bin_of(top));
-  if (by_count) {
-    const Bin at = seek_bin(kByCount, (double)f.k, s, groups, top, inv_t);
-    take(at.bin, at.bin);
-    least = at.mass;
-    most = at.mass + at.weight;
-  }
-  if (reach) {
-    const Bin x = seek_bin(kReach, fmax((double)f.p * least * (1.0 - slack), tiny), s, groups, top, inv_t);
-    const Bin y = seek_bin(kReach, fmax((double)f.p * most * (1.0 + slack), tiny), s, groups, top, inv_t);
-    take(x.bin, y.bin);
-    least = x.mass;
-    most = y.mass + y.weight;
-  }
-  if (above) {
-    const Bin at = seek_bin(kAbove, fmin((double)f.least, 1.0), s, groups, top, inv_t);
-    take(at.bin, at.bin);
-    least = fmin(least, at.mass);
-    most = fmin(most, at.mass + at.weight);
-  }
-  if (f.sampled && !greedy) {
-    const Bin x = seek_bin(kBeyond, unit(f.u) * least * (1.0 - slack), s, groups, top, inv_t);
-    const Bin y = seek_bin(kBeyond, unit(f.u) * most * (1.0 + slack), s, groups, top, inv_t);
-    take(x.bin, y.bin);
-  }
-  // (bin_edge of the bins of infinity and of NaN is a NaN)
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (i >= ranges) hi[i] = lo[i] = __builtin_nanf("");
-    else if (hi[i] != hi[i]) hi[i] = __builtin_inff();
-  }
-  if (ranges) each_vec(row, 0, row.vecs, [&](int it, const u32x4& v, bool here) {
-    if (!here) return;
-    const int64_t e0 = (int64_t)4 * (it * kRowThreads + tid) - row.skew;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const float x = __uint_as_float(v[e]);
-      bool is = x <= hi[0] && x >= lo[0];
-      if (ranges > 1) is = is || (x <= hi[1] && x >= lo[1]);
-      if (ranges > 2) is = is || (x <= hi[2] && x >= lo[2]);
-      if (ranges > 3) is = is || (x <= hi[3] && x >= lo[3]);
-      if (!is || x == -__builtin_inff()) continue;
-      const int at = atomicAdd(&s.listed, 1);
-      if (at < kList) s.list[at] = ((uint64_t)order_bits(x) << 32) | (uint32_t)(e0 + e);
+             above = !greedy && f.least > 0.f, draws = !greedy && f.sampled;
+  if (wave == 0) {
+    double least = total, most = total;
+    int ranges = 0;
+#pragma unroll 1
+    for (int kind = 0; kind < 5; ++kind) {  // (4: the maximum's bin)
+      if (!(kind == kByCount ? by_count : kind == kReach ? reach : kind == kAbove ? above : kind == kBeyond ? draws : greedy)) continue;
+      double g0 = 0.0, g1 = 0.0;
+      if (kind == kByCount) g0 = g1 = (double)f.k;
+      if (kind == kAbove) g0 = g1 = fmin((double)f.least, 1.0);
+      if (kind == kReach) {
+        g0 = fmax((double)f.p * least * (1.0 - slack), tiny);
+        g1 = fmax((double)f.p * most * (1.0 + slack), tiny);
+      }
+      if (kind == kBeyond) {
+        g0 = unit(f.u) * least * (1.0 - slack);
+        g1 = unit(f.u) * most * (1.0 + slack);
+      }
+      uint32_t first = bin_of(top), last = first;
+      if (kind < 4) {
+        const Bin x = seek_bin(kind, g0, s, groups, top, inv_t);
+        first = x.bin;
+        double m0 = x.mass, m1 = x.mass + x.weight;
+        // (the bin reaches over both goals as a rule)
+        if (kind == kReach ? m1 < g1 : kind == kBeyond && m1 <= g1) {
+          const Bin y = seek_bin(kind, g1, s, groups, top, inv_t);
+          last = y.bin;
+          m1 = y.mass + y.weight;
+        } else {
+          last = first;
+        }
+        if (kind == kAbove) {
+          m0 = fmin(m0, least);
+          m1 = fmin(m1, most);
+        }
+        least = m0;
+        most = m1;
+      }
+      const float h = bin_edge(first);
+      if (lane == 0) {
+        s.high[ranges] = h == h ? h : __builtin_inff();  // (infinity's bin begins with NaNs)
+        s.low[ranges] = order_value(((last + 1) << kBinShift) - 1);
+      }
+      ++ranges;
     }
-  });
+    if (lane == 0) s.ranges = ranges;
+  }
+  __syncthreads();
+  const int ranges = __builtin_amdgcn_readfirstlane(s.ranges);
+  auto bound = [&](const float* at, int i) {
+    return i < ranges ? __uint_as_float((uint32_t)__builtin_amdgcn_readfirstlane((int)__float_as_uint(at[i]))) : __builtin_nanf("");
+  };
+  const float h0 = bound(s.high, 0), h1 = bound(s.high, 1), h2 = bound(s.high, 2), h3 = bound(s.high, 3);
+  const float l0 = bound(s.low, 0), l1 = bound(s.low, 1), l2 = bound(s.low, 2), l3 = bound(s.low, 3);
+  if (ranges)
+    each_vec<8>(row, 0, row.vecs, [&](int it, const u32x4& v, bool here) {
+      uint32_t is = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = __uint_as_float(v[e]);
+        bool in_range = x <= h0 && x >= l0;
+        if (ranges > 1) in_range |= x <= h1 && x >= l1;  // uniform
+        if (ranges > 2) in_range |= (x <= h2 && x >= l2) || (x <= h3 && x >= l3);
+        is |= (in_range ? 1u : 0u) << e;
+      }
+      if (!here) is = 0;
+      if (!__ballot(is != 0)) return;  // uniform
+      const uint32_t n = __popc(is), upto_n = wave_scan(n);
+      int base = 0;
+      if (lane == 63) base = atomicAdd(&s.listed, (int)upto_n);
+      int at = (int)lane_u32((uint32_t)base, 63) + (int)(upto_n - n);
+      const int64_t e0 = (int64_t)4 * (it * kRowThreads + tid) - row.skew;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if ((is >> e) & 1) {
+          if (at < kList) s.list[at] = ((uint64_t)order_bits(__uint_as_float(v[e])) << 32) | (uint32_t)(e0 + e);
+          ++at;
+        }
+    });
   __syncthreads();
   if (s.listed > kList) {  // uniform
     fits = false;
@@ -1325,7 +1391,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   out.cut = greedy ? top : -__builtin_inff();
   auto ref_of = [&](uint32_t bin) { return fminf(bin_edge(bin), top); };
   if (by_count) {
-    const Bin at = seek_bin(kByCount, (double)f.k, s, groups, top, inv_t);
+    const Bin at = find_bin(kByCount, (double)f.k, groups, top, inv_t, s);
     const Spot x = seek_list(kByCount, (double)((uint32_t)f.k - at.before), at.bin, ref_of(at.bin), inv_t, scale, s);
     const uint32_t n = (uint32_t)f.k - at.before - x.before;
     W = at.mass + (double)(x.mass + n * x.weight) * (weight_of(ref_of(at.bin), top, inv_t, s.tab) / scale);
@@ -1335,7 +1401,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   }
   if (reach) {
     const double goal = fmax((double)f.p * W, tiny);
-    const Bin at = seek_bin(kReach, goal, s, groups, top, inv_t);
+    const Bin at = find_bin(kReach, goal, groups, top, inv_t, s);
     const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) / scale;
     const double inside = fmax((goal - at.mass) / unit_w, 0.5);
     const Spot x = seek_list(kReach, inside, at.bin, ref_of(at.bin), inv_t, scale, s);
@@ -1351,7 +1417,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   }
   if (above) {
     const double goal = fmin((double)f.least, 1.0);
-    const Bin at = seek_bin(kAbove, goal, s, groups, top, inv_t);
+    const Bin at = find_bin(kAbove, goal, groups, top, inv_t, s);
     const float ref = ref_of(at.bin);
     // the bin's tokens that are heavy enough: how many, their weights, the lightest
     __syncthreads();
@@ -1383,7 +1449,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   }
   if (f.sampled && kept > 1) {
     const double goal = unit(f.u) * W;
-    const Bin at = seek_bin(kBeyond, goal, s, groups, top, inv_t);
+    const Bin at = find_bin(kBeyond, goal, groups, top, inv_t, s);
     const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) / scale;
     const double inside = fmax((goal - at.mass) / unit_w, 0.0);
     const Spot x = seek_list(kBeyond, inside, at.bin, ref_of(at.bin), inv_t, scale, s);
@@ -1456,13 +1522,19 @@ __device__ __forceinline__ void put_row(const FilterArgs& a, int r, int b, const
   }
 }
 
+// Parts of a row (one more than another's, maybe, where it starts off a 16-byte boundary).
+template <typename T>
+__device__ __forceinline__ int part_count(const Row<T>& row, int steps) {
+  return (row.vecs + steps * kRowThreads - 1) / (steps * kRowThreads);
+}
+
 // What a launch's n-th row is.
 template <typename T>
 struct Work {
   int r, b;
   Job j;
   const T* row;
-  __device__ Work(const FilterArgs& a, int n) {
+  __device__ __forceinline__ Work(const FilterArgs& a, int n) {
     b = (a.row0 + n) / a.rows;
     r = a.row0 + n - b * a.rows;
     j = job_of(a, r, b);
@@ -1475,14 +1547,18 @@ __global__ __launch_bounds__(kRowThreads) void filter_count_kernel(FilterArgs a)
   __shared__ uint32_t bin[32768];
   const Work<uint16_t> w(a, blockIdx.y);
   if (!w.j.active) return;  // uniform
-  count_part(Row<uint16_t>(w.row, a.V), blockIdx.x, a.split, bin, (Part*)a.row_parts + (int64_t)blockIdx.y * a.split + blockIdx.x);
+  const Row<uint16_t> row(w.row, a.V);
+  const int first = blockIdx.x * a.share, last = min(first + a.share, part_count(row, a.steps));
+  if (first < last) count_parts(row, first, last, a.steps, bin, (Part*)a.row_parts + (int64_t)blockIdx.y * a.split + first);
 }
 __global__ __launch_bounds__(kRowThreads) void filter_bin_kernel(FilterArgs a) {
   __shared__ BinLds s;
   const Work<float> w(a, blockIdx.y);
   if (!w.j.active) return;  // uniform
-  bin_part(Row<float>(w.row, a.V), blockIdx.x, a.split, a.temperature[w.b], a.shift, s,
-           (BinPart*)a.row_parts + (int64_t)blockIdx.y * a.split + blockIdx.x);
+  const Row<float> row(w.row, a.V);
+  if ((int)blockIdx.x < part_count(row, a.steps))
+    bin_part(row, blockIdx.x, a.steps, a.temperature[w.b], a.shift, s,
+             (BinPart*)a.row_parts + (int64_t)blockIdx.y * a.split + blockIdx.x);
 }
 // grid rows
 __global__ __launch_bounds__(kRowThreads) void filter_merge_kernel(FilterArgs a) {
@@ -1490,35 +1566,55 @@ __global__ __launch_bounds__(kRowThreads) void filter_merge_kernel(FilterArgs a)
   const Work<uint16_t> w(a, blockIdx.x);
   if (!w.j.active) return;  // uniform
   const Part* in = (const Part*)a.row_parts + (int64_t)blockIdx.x * a.split;
-  put_row(a, w.r, w.b, w.j, w.row,
-          merge_row(Row<uint16_t>(w.row, a.V), settings_of(a, w.b, w.j.sampled, w.j.u, w.j.ends), in, a.split, s));
+  const Row<uint16_t> row(w.row, a.V);
+  put_row(a, w.r, w.b, w.j, w.row, merge_row(row, settings_of(a, w.b, w.j.sampled, w.j.u, w.j.ends), in,
+                                             part_count(row, a.steps), a.steps, s));
 }
 __global__ __launch_bounds__(kRowThreads) void filter_list_kernel(FilterArgs a) {
   __shared__ RowLds32 s;
   const Work<float> w(a, blockIdx.x);
   if (!w.j.active) return;  // uniform
   const BinPart* in = (const BinPart*)a.row_parts + (int64_t)blockIdx.x * a.split;
+  const Row<float> row(w.row, a.V);
   bool fits;
-  RowCut c = list_row(Row<float>(w.row, a.V), settings_of(a, w.b, w.j.sampled, w.j.u, w.j.ends), in, a.split, a.shift, s.bins, fits);
+  RowCut c = list_row(row, settings_of(a, w.b, w.j.sampled, w.j.u, w.j.ends), in, part_count(row, a.steps), a.shift, s.bins, fits);
+  // (worked out anew: kept over all that, it would be spilled)
+  int n = blockIdx.x;
+  asm volatile("" : "+s"(n));
+  const Work<float> again(a, n);
   if (!fits) {  // uniform
+    Settings f = settings_of(a, again.b, again.j.sampled, again.j.u, again.j.ends);
+    make_uniform(f);
     __syncthreads();
-    c = filter_row<float>(a, w.b, w.row, w.j.sampled, a.uniforms[w.j.u], w.j.ends, s.radix);
+    c = radix_row(again.row, a.V, a.shift, f, s.radix);
   }
-  put_row(a, w.r, w.b, w.j, w.row, c);
+  put_row(a, again.r, again.b, again.j, again.row, c);
 }
 
-// Parts of a row, a workgroup each: more where the rows alone leave compute
-// units idle, as long as each takes a step of a workgroup, and in bf16 so many
-// that 16 bits hold a part's counts.
-int row_split(int rows, int V, int dtype) {
+// How rows are cut: parts of `steps` steps of a workgroup, `split` of them a
+// row, `share` a workgroup.  Few rows: a part a workgroup, and as short as
+// leaves 256 of them and 8 a row.  Many: bf16 parts as long as 16 bits count, so that less
+// is written and read again, and as many of them a workgroup as leave 256;
+// fp32 rows in one part, whose maximum its weights are relative to.
+struct Cut {
+  int steps, split, share;
+};
+Cut cut_rows(int rows, int V, int dtype) {
   const int step = dtype == NSV_BF16 ? kStep : kStep / 2;
-  int n = kMaxSplit;
-  while (n > 1 && (rows * n > 256 || V < n * step)) n >>= 1;
-  const int least = dtype == NSV_BF16 ? (V + 7 + kSafeSteps * kStep - 1) / (kSafeSteps * kStep) : 1;
-  return n < least ? least : n;
+  const int whole = (V + (dtype == NSV_BF16 ? 7 : 3) + step - 1) / step;  // steps of a row
+  const int longest = dtype == NSV_BF16 ? kSafeSteps : whole;
+  Cut c{1, whole, 1};
+  while (c.steps < longest && ((int64_t)rows * c.split > 256 || c.split > kFewParts)) {
+    ++c.steps;
+    c.split = (whole + c.steps - 1) / c.steps;
+  }
+  const int groups = rows >= 256 ? 1 : 256 / rows;
+  c.share = (c.split + groups - 1) / groups;
+  return c;
 }
 size_t part_bytes(int dtype) { return dtype == NSV_BF16 ? sizeof(Part) : sizeof(BinPart); }
-static_assert(sizeof(Part) % 16 == 0 && sizeof(BinPart) % 16 == 0 && (kMaxVocab + 7) / (kSafeSteps * kStep) < kMaxParts, "parts");
+static_assert(sizeof(Part) % 16 == 0 && sizeof(BinPart) % 16 == 0 && (kMaxVocab + 7) / (kSafeSteps * kStep) < kMaxParts &&
+              kHead * kMaxParts <= kRowThreads, "parts");
 
 }  // namespace
 
@@ -1526,20 +1622,23 @@ namespace nsv_filter {
 
 size_t rows_bytes(int rows, int V, int dtype) {
   if (rows <= 0) return 0;
-  const int n = row_split(rows, V, dtype), most = kSlab / n;
+  const int n = cut_rows(rows, V, dtype).split, most = kSlab / n;
   return (size_t)(rows < most ? rows : most) * n * part_bytes(dtype);
 }
 
 int launch_rows(FilterArgs& a, int dtype, void* workspace, hipStream_t s) {
   const int total = a.rows * a.B;
-  a.split = row_split(total, a.V, dtype);
+  const Cut c = cut_rows(total, a.V, dtype);
+  a.split = c.split;
+  a.steps = c.steps;
+  a.share = c.share;
   a.row_parts = workspace;
-  const int most = kSlab / a.split;
+  const int most = kSlab / c.split;
   for (a.row0 = 0; a.row0 < total; a.row0 += most) {
     const int rows = total - a.row0 < most ? total - a.row0 : most;
-    const dim3 parts(a.split, rows), block(kRowThreads);
+    const dim3 parts((c.split + c.share - 1) / c.share, rows), block(kRowThreads);
     if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_count_kernel, parts, block, 0, s, a);
-    else hipLaunchKernelGGL(filter_bin_kernel, parts, block, 0, s, a);
+    else hipLaunchKernelGGL(filter_bin_kernel, dim3(c.split, rows), block, 0, s, a);
     int rc = nsv_launch_status();
     if (rc) return rc;
     if (dtype == NSV_BF16) hipLaunchKernelGGL(filter_merge_kernel, dim3(rows), block, 0, s, a);
