@@ -205,8 +205,8 @@ __device__ __forceinline__ int index_of(float value, uint32_t j, const T* row, i
 // ---------------------------------------------------------------------------
 // rows in parts
 // ---------------------------------------------------------------------------
-constexpr int kMaxParts = 32;  // of a row ..
-constexpr int kFewParts = 8;   // .. where they may be as long as that takes: the second kernel reads them one after another
+constexpr int kFewParts = 8;   // workgroups that a row is cut over, at most ..
+constexpr int kMaxParts = 32;  // .. and parts
 constexpr int kSlab = 1024;    // parts of a launch: what they leave takes 128 MiB at most
 
 // A row as 16-byte vectors of N elements: vector g holds elements N g - skew ..
@@ -1052,7 +1052,7 @@ struct ListLds {
   float high[4], low[4];       // ranges of values to list
   int ranges;
   uint64_t list[kList];        // order bits << 32 | index
-  uint32_t sub_count[kSubBins];
+  uint32_t sub_count[kSubBins], sub_key[kSubBins];
   unsigned long long sub_mass[kSubBins];
   double tab[256];
   uint32_t red[kRowWaves];
@@ -1136,6 +1136,7 @@ __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, f
       if ((k >> (sh + bits)) != (at.key >> (sh + bits))) continue;
       const uint32_t sub = (k >> sh) & ((1u << bits) - 1);
       atomicAdd(&s.sub_count[sub], 1u);
+      s.sub_key[sub] = k;
       const uint64_t q = fixed_weight(weight_of(order_value(k), ref, inv_t, s.tab), scale);
       if (q) atomicAdd(&s.sub_mass[sub], (unsigned long long)q);
     }
@@ -1168,6 +1169,10 @@ __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, f
     at.mass = s.hit_mass_before;
     at.count = s.hit_count;
     at.weight = s.hit_mass;
+    if (at.count == 1) {  // uniform: that token itself (fp32 values are apart as a rule)
+      at.key = s.sub_key[max(s.hit, 0)];
+      break;
+    }
   }
   at.weight /= max(at.count, 1u);  // (equal values have equal weights)
   return at;
@@ -1591,29 +1596,26 @@ __global__ __launch_bounds__(kRowThreads) void filter_list_kernel(FilterArgs a) 
   put_row(a, again.r, again.b, again.j, again.row, c);
 }
 
-// How rows are cut: parts of `steps` steps of a workgroup, `split` of them a
-// row, `share` a workgroup.  Few rows: a part a workgroup, and as short as
-// leaves 256 of them and 8 a row.  Many: bf16 parts as long as 16 bits count, so that less
-// is written and read again, and as many of them a workgroup as leave 256;
-// fp32 rows in one part, whose maximum its weights are relative to.
+// How rows are cut: `split` parts of `steps` steps of a workgroup each, `share`
+// of them counted by one workgroup one after another.  As many workgroups a row
+// as the rows leave of 256, 8 at most (the second kernel reads every part), and
+// in bf16 so many parts that 16 bits count one.
 struct Cut {
   int steps, split, share;
 };
 Cut cut_rows(int rows, int V, int dtype) {
   const int step = dtype == NSV_BF16 ? kStep : kStep / 2;
   const int whole = (V + (dtype == NSV_BF16 ? 7 : 3) + step - 1) / step;  // steps of a row
-  const int longest = dtype == NSV_BF16 ? kSafeSteps : whole;
-  Cut c{1, whole, 1};
-  while (c.steps < longest && ((int64_t)rows * c.split > 256 || c.split > kFewParts)) {
-    ++c.steps;
-    c.split = (whole + c.steps - 1) / c.steps;
-  }
-  const int groups = rows >= 256 ? 1 : 256 / rows;
-  c.share = (c.split + groups - 1) / groups;
+  int groups = rows >= 256 ? 1 : 256 / rows;
+  if (groups > kFewParts) groups = kFewParts;
+  Cut c;
+  c.share = dtype == NSV_BF16 ? (whole + groups * kSafeSteps - 1) / (groups * kSafeSteps) : 1;
+  c.steps = (whole + groups * c.share - 1) / (groups * c.share);
+  c.split = (whole + c.steps - 1) / c.steps;
   return c;
 }
 size_t part_bytes(int dtype) { return dtype == NSV_BF16 ? sizeof(Part) : sizeof(BinPart); }
-static_assert(sizeof(Part) % 16 == 0 && sizeof(BinPart) % 16 == 0 && (kMaxVocab + 7) / (kSafeSteps * kStep) < kMaxParts &&
+static_assert(sizeof(Part) % 16 == 0 && sizeof(BinPart) % 16 == 0 && kMaxVocab / (kSafeSteps * kStep) + 1 + kFewParts < kMaxParts &&
               kHead * kMaxParts <= kRowThreads, "parts");
 
 }  // namespace
