@@ -22,6 +22,8 @@
 
 #include "filter.h"
 
+#include <type_traits>
+
 using namespace nsv_filter;
 
 namespace {
@@ -779,13 +781,16 @@ struct Part {
 __device__ __forceinline__ void put_part(uint32_t* bin, Part* out) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   uint32_t has = 0;  // of groups in the order of their words
+  u32x4 w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = *reinterpret_cast<const u32x4*>(bin + 2048 * wave + 256 * i + 4 * lane);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
+    const uint64_t any = __ballot((w[i][0] | w[i][1] | w[i][2] | w[i][3]) != 0);
+    if (!any) continue;  // uniform
     const int at = 2048 * wave + 256 * i + 4 * lane;
-    const u32x4 w = *reinterpret_cast<const u32x4*>(bin + at);
-    const uint64_t any = __ballot((w[0] | w[1] | w[2] | w[3]) != 0);
     if ((any >> (lane & 48)) & 0xffffu) {
-      *reinterpret_cast<u32x4*>(out->word + at) = w;
+      *reinterpret_cast<u32x4*>(out->word + at) = w[i];
       *reinterpret_cast<u32x4*>(bin + at) = u32x4{0u, 0u, 0u, 0u};
     }
 #pragma unroll
@@ -1355,19 +1360,20 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   };
   const float h0 = bound(s.high, 0), h1 = bound(s.high, 1), h2 = bound(s.high, 2), h3 = bound(s.high, 3);
   const float l0 = bound(s.low, 0), l1 = bound(s.low, 1), l2 = bound(s.low, 2), l3 = bound(s.low, 3);
-  if (ranges)
+  auto list = [&](auto four) {
     each_vec<8>(row, 0, row.vecs, [&](int it, const u32x4& v, bool here) {
-      uint32_t is = 0;
+      uint64_t in[4];  // of each element: the lanes whose is in a range (comparisons all, and no branch)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = __uint_as_float(v[e]);
-        bool in_range = x <= h0 && x >= l0;
-        if (ranges > 1) in_range |= x <= h1 && x >= l1;  // uniform
-        if (ranges > 2) in_range |= (x <= h2 && x >= l2) || (x <= h3 && x >= l3);
-        is |= (in_range ? 1u : 0u) << e;
+        bool is = ((x <= h0) & (x >= l0)) | ((x <= h1) & (x >= l1));
+        if constexpr (four) is = is | ((x <= h2) & (x >= l2)) | ((x <= h3) & (x >= l3));
+        in[e] = __ballot(is & here);
       }
-      if (!here) is = 0;
-      if (!__ballot(is != 0)) return;  // uniform
+      if (!(in[0] | in[1] | in[2] | in[3])) return;  // uniform
+      uint32_t is = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) is |= (uint32_t)((in[e] >> lane) & 1) << e;
       const uint32_t n = __popc(is), upto_n = wave_scan(n);
       int base = 0;
       if (lane == 63) base = atomicAdd(&s.listed, (int)upto_n);
@@ -1380,6 +1386,9 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
           ++at;
         }
     });
+  };
+  if (ranges > 2) list(std::true_type{});
+  else if (ranges) list(std::false_type{});
   __syncthreads();
   if (s.listed > kList) {  // uniform
     fits = false;
