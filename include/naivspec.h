@@ -291,7 +291,7 @@ int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights,
  * [num_blocks, block_size, Hkv, D]: one segment of Hkv * D elements per key;
  * key weights [num_blocks, Hkv, block_size]: Hkv segments of 4 bytes).
  * `pools` is a host array, read before the call returns.  key_bytes and base
- * even; num_blocks <= 524,288; pages under 2^30 bytes.  A table entry outside
+ * even; num_blocks <= 262,144; pages under 2^30 bytes.  A table entry outside
  * [0, num_blocks) is unmapped.  held [num_blocks] bytes (nullable): a page
  * with a nonzero byte is somebody else's and neither given out nor moved.
  *

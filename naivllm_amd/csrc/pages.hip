@@ -19,7 +19,7 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanWaves = kPlanThreads / 64;
-constexpr int kMaxPages = 1 << 19;            // two bits each in LDS: 128 KiB
+constexpr int kMaxPages = 1 << 18;            // two bits each in LDS, and two counts per 32: 128 KiB
 constexpr int kMaxWords = kMaxPages / 32;
 constexpr int kMaxRows = 4096;
 constexpr int kMoveThreads = 256;
@@ -40,6 +40,7 @@ struct Moves {
   const int32_t* keys;   // nullable: whole pages
   const int32_t* count;  // nullable
   int most;
+  const int32_t* via;    // nullable: dst holds places of this list
 };
 
 __device__ __forceinline__ uint32_t scan_u32(uint32_t v) {  // inclusive, over a wave
@@ -67,16 +68,45 @@ __device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* red, uint32
   return before + in - v;
 }
 
-__device__ __forceinline__ void mark_held(const uint8_t* held, int pages, uint32_t* bits) {
-  if (!held) return;
-  for (int i = threadIdx.x; i < pages; i += kPlanThreads)
-    if (held[i]) atomicOr(&bits[i >> 5], 1u << (i & 31));
-}
-
 // the pages of a word that exist
 __device__ __forceinline__ uint32_t word_mask(int w, int pages) {
   const int left = pages - 32 * w;
   return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
+}
+
+// bits of the held pages, a thread per word
+__device__ __forceinline__ void mark_held(const uint8_t* held, int pages, uint32_t* bits) {
+  if (!held) return;
+  for (int w = threadIdx.x; 32 * w < pages; w += kPlanThreads) {
+    const uint8_t* at = held + 32 * w;
+    uint32_t m = 0;
+    if (((uintptr_t)held & 15) == 0 && 32 * w + 32 <= pages) {
+      const u32x4 a = reinterpret_cast<const u32x4*>(at)[0], b = reinterpret_cast<const u32x4*>(at)[1];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        m |= ((a[i >> 2] >> (8 * (i & 3))) & 0xffu ? 1u : 0u) << i;
+        m |= ((b[i >> 2] >> (8 * (i & 3))) & 0xffu ? 1u : 0u) << (16 + i);
+      }
+    } else {
+      for (int i = 0; i < 32 && 32 * w + i < pages; ++i) m |= (at[i] ? 1u : 0u) << i;
+    }
+    if (m) atomicOr(&bits[w], m);
+  }
+}
+
+// before[w] = pages of the words before w that `pick` takes; their whole number
+template <typename F>
+__device__ __forceinline__ uint32_t count_before(int words, uint32_t* before, uint32_t* red, F pick) {
+  const int per = (words + kPlanThreads - 1) / kPlanThreads, w0 = threadIdx.x * per;
+  uint32_t mine = 0, all;
+  for (int w = w0; w < min(w0 + per, words); ++w) mine += __popc(pick(w));
+  uint32_t at = block_scan(mine, red, all);
+  for (int w = w0; w < min(w0 + per, words); ++w) {
+    before[w] = at;
+    at += __popc(pick(w));
+  }
+  __syncthreads();
+  return all;
 }
 
 // ---------------------------------------------------------------------------
@@ -94,122 +124,140 @@ struct ForkArgs {
   // workspace
   int32_t* count;         // moves
   int32_t* src;
-  int32_t* dst;
+  int32_t* dst;           // (places of `fresh`)
   int32_t* keys;          // [B] each
   int32_t* base;          // [B] a row's first place in `fresh`; -1: the row is empty; -2: it has its parent's pages
   int32_t* fresh;         // free pages, rising
 };
 
-// keys of row b's parent, and its whole pages among W columns
-__device__ __forceinline__ int64_t parent_keys(const ForkArgs& a, int p) {
-  const int64_t n = a.lens[p];
-  return n > 0 ? n : 0;
-}
-__device__ __forceinline__ int whole_pages(int64_t keys, int block_size, int W) {
-  const int64_t n = keys / block_size;
-  return n < W ? (int)n : W;
+// How keys fill a row of W pages: whole pages, and the keys of the one behind
+// them (0 where the row ends with them).
+struct Filled {
+  int whole, rest;
+};
+__device__ __forceinline__ Filled filled(int64_t keys, int block_size, int W) {
+  const int64_t room = (int64_t)W * block_size;
+  if (keys <= 0) return {0, 0};
+  if (keys >= room) return {W, 0};
+  if (room <= 0x7fffffff) {  // uniform (a 64-bit division is some 150 instructions)
+    const uint32_t k = (uint32_t)keys, q = k / (uint32_t)block_size;
+    return {(int)q, (int)(k - q * (uint32_t)block_size)};
+  }
+  return {(int)(keys / block_size), (int)(keys % block_size)};
 }
 
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkArgs a, int pages, int block_size) {
-  __shared__ uint32_t used[kMaxWords], red[kPlanWaves];
-  __shared__ int32_t first[kMaxRows];
+  __shared__ uint32_t used[kMaxWords], before[kMaxWords], red[kPlanWaves];
+  __shared__ int32_t first[kMaxRows], parent[kMaxRows], partly[kMaxRows], rest[kMaxRows];
   __shared__ uint32_t need[kMaxRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int words = (pages + 31) / 32;
-  for (int i = tid; i < words; i += kPlanThreads) used[i] = 0;
-  for (int b = tid; b < a.B; b += kPlanThreads) first[b] = a.B;
-  __syncthreads();
   for (int b = tid; b < a.B; b += kPlanThreads) {
     const int p = a.parents[b];
-    if (p >= 0 && p < a.B) atomicMin(&first[p], b);
+    parent[b] = p >= 0 && p < a.B ? p : -1;
+    first[b] = a.B;
   }
+  for (int i = tid; i < words; i += kPlanThreads) used[i] = 0;
+  __syncthreads();
+  for (int b = tid; b < a.B; b += kPlanThreads)
+    if (parent[b] >= 0) atomicMin(&first[parent[b]], b);
   mark_held(a.held, pages, used);
   __syncthreads();
-  // a first child keeps its parent's pages; the others need one for each that is not whole
-  for (int b = wave; b < a.B; b += kPlanWaves) {
-    const int p = a.parents[b];
-    const bool live = p >= 0 && p < a.B;
-    const int32_t* row = a.tables + (int64_t)(live ? p : 0) * a.W;
-    uint32_t n = 0;
-    if (live && first[p] == b) {
-      for (int j = lane; j < a.W; j += 64) {
-        const int e = row[j];
-        if (e >= 0 && e < pages) atomicOr(&used[e >> 5], 1u << (e & 31));
+  // a first child keeps its parent's pages; the others need one for each that
+  // is not whole.  Four rows of a wave and 128 columns at a time, their loads
+  // beside each other.
+  constexpr int kAtOnce = 4;
+  for (int b0 = wave; b0 < a.B; b0 += kAtOnce * kPlanWaves) {
+    int64_t keys[kAtOnce];
+    Filled fill[kAtOnce];
+    int p[kAtOnce], src[kAtOnce];  // src: the partly filled page that a row copies
+    uint32_t n[kAtOnce] = {};
+    for (int j0 = 0; j0 < a.W; j0 += 128) {
+      int e[kAtOnce][2];
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        const int b = b0 + i * kPlanWaves;
+        if (j0 == 0) {
+          p[i] = b < a.B ? parent[b] : -1;
+          src[i] = -1;
+        }
+        const int row = max(p[i], 0);
+        if (j0 == 0) keys[i] = a.lens[row];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) e[i][h] = a.tables[(int64_t)row * a.W + min(j0 + 64 * h + lane, a.W - 1)];
       }
-    } else if (live) {
-      for (int j = whole_pages(parent_keys(a, p), block_size, a.W) + lane; j < a.W; j += 64) {
-        const int e = row[j];
-        n += e >= 0 && e < pages;
+#pragma unroll
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (p[i] < 0) continue;  // uniform
+        const bool keeps = first[p[i]] == b0 + i * kPlanWaves;
+        if (j0 == 0) fill[i] = filled(keys[i], block_size, a.W);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int j = j0 + 64 * h + lane, id = e[i][h];
+          if (j >= a.W || id < 0 || id >= pages) continue;
+          if (keeps) atomicOr(&used[id >> 5], 1u << (id & 31));
+          else n[i] += j >= fill[i].whole;
+          if (!keeps && j == fill[i].whole && fill[i].rest) src[i] = id;
+        }
       }
-      n = (uint32_t)__shfl((int)scan_u32(n), 63);
     }
-    if (lane == 0) need[b] = n;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int b = b0 + i * kPlanWaves;
+      if (b >= a.B) break;  // uniform
+      const uint32_t all = lane_u32(scan_u32(n[i]), 63);
+      const uint64_t has = __ballot(src[i] >= 0);
+      const int one = has ? (int)lane_u32((uint32_t)src[i], __ffsll((long long)has) - 1) : -1;
+      if (lane == 0) {
+        need[b] = all;
+        partly[b] = one;
+        rest[b] = p[i] >= 0 ? fill[i].rest : 0;
+      }
+    }
   }
   __syncthreads();
-  // free pages before each thread's words
-  const int per = (words + kPlanThreads - 1) / kPlanThreads;
-  uint32_t mine = 0, free_pages, wanted = 0;
-  for (int i = 0; i < per; ++i) {
-    const int w = tid * per + i;
-    if (w < words) mine += __popc(~used[w] & word_mask(w, pages));
-  }
-  uint32_t rank = block_scan(mine, red, free_pages);
-  // places of the rows' pages among the free ones, row by row
-  const int rows = (a.B + kPlanThreads - 1) / kPlanThreads;
-  for (int i = 0; i < rows; ++i)
-    if (tid * rows + i < a.B) wanted += need[tid * rows + i];
-  uint32_t all;
+  auto is_free = [&](int w) { return ~used[w] & word_mask(w, pages); };
+  const uint32_t free_pages = count_before(words, before, red, is_free);
+  // places of the rows' pages among the free ones, row by row, and of the copies
+  const int rows = (a.B + kPlanThreads - 1) / kPlanThreads, r0 = tid * rows, r1 = min(r0 + rows, a.B);
+  uint32_t wanted = 0, copies = 0, all, many;
+  for (int b = r0; b < r1; ++b) wanted += need[b];
   uint32_t at = block_scan(wanted, red, all);
-  for (int i = 0; i < rows; ++i) {
-    const int b = tid * rows + i;
-    if (b >= a.B) break;
-    const int p = a.parents[b];
-    const bool live = p >= 0 && p < a.B;
+  const uint32_t start = at;
+  for (int b = r0; b < r1; ++b) {
+    at += need[b];
+    copies += partly[b] >= 0 && at <= free_pages;
+  }
+  uint32_t to = block_scan(copies, red, many);
+  at = start;
+  for (int b = r0; b < r1; ++b) {
     const uint32_t n = need[b];
-    a.base[b] = !live ? -1 : n == 0 ? -2 : at + n <= free_pages ? (int32_t)at : -1;
+    const bool fits = at + n <= free_pages;
+    a.base[b] = parent[b] < 0 ? -1 : n == 0 ? -2 : fits ? (int32_t)at : -1;
+    if (partly[b] >= 0 && fits) {  // the row's first new page, of its parent's partly filled one
+      a.src[to] = partly[b];
+      a.dst[to] = (int32_t)at;
+      a.keys[to++] = rest[b];
+    }
     at += n;
   }
   const uint32_t most = all < free_pages ? all : free_pages;
-  for (int i = 0; i < per && rank < most; ++i) {
-    const int w = tid * per + i;
-    if (w >= words) break;
-    for (uint32_t f = ~used[w] & word_mask(w, pages); f && rank < most; f &= f - 1) a.fresh[rank++] = 32 * w + __ffs((int)f) - 1;
+  for (int id = tid; id < pages && before[id >> 5] < most; id += kPlanThreads) {  // (rising: none behind the last that is wanted)
+    const uint32_t f = is_free(id >> 5), rank = before[id >> 5] + __popc(f & ((1u << (id & 31)) - 1));
+    if (((f >> (id & 31)) & 1) && rank < most) a.fresh[rank] = id;
   }
-  if (tid == 0) *a.lacking = (int32_t)(all > free_pages ? all - free_pages : 0);
-  __syncthreads();  // base and fresh, for the whole workgroup
-  // pages to copy: a row's first new page, where its parent's was partly filled
-  uint32_t copies = 0, many;
-  for (int i = 0; i < rows; ++i) {
-    const int b = tid * rows + i;
-    if (b >= a.B || a.base[b] < 0) continue;
-    const int64_t n = parent_keys(a, a.parents[b]);
-    const int j = whole_pages(n, block_size, a.W);
-    if (j >= a.W || n % block_size == 0) continue;
-    const int e = a.tables[(int64_t)a.parents[b] * a.W + j];
-    copies += e >= 0 && e < pages;
+  if (tid == 0) {
+    *a.lacking = (int32_t)(all > free_pages ? all - free_pages : 0);
+    *a.count = (int32_t)many;
   }
-  uint32_t to = block_scan(copies, red, many);
-  for (int i = 0; i < rows; ++i) {
-    const int b = tid * rows + i;
-    if (b >= a.B || a.base[b] < 0) continue;
-    const int64_t n = parent_keys(a, a.parents[b]);
-    const int j = whole_pages(n, block_size, a.W);
-    if (j >= a.W || n % block_size == 0) continue;
-    const int e = a.tables[(int64_t)a.parents[b] * a.W + j];
-    if (e < 0 || e >= pages) continue;
-    a.src[to] = e;
-    a.dst[to] = a.fresh[a.base[b]];
-    a.keys[to++] = (int32_t)(n % block_size);
-  }
-  if (tid == 0) *a.count = (int32_t)many;
 }
 
 // A row of the new tables, by one wave.
 __device__ __forceinline__ void fork_row(const ForkArgs& a, int b, int pages, int block_size) {
   const int lane = threadIdx.x & 63;
   const int base = a.base[b], p = a.parents[b];
-  const int64_t keys = base == -1 ? 0 : parent_keys(a, p);
-  const int whole = whole_pages(keys, block_size, a.W);
+  const int64_t keys = base == -1 ? 0 : a.lens[p] > 0 ? a.lens[p] : 0;
+  const int whole = filled(keys, block_size, a.W).whole;
   int at = base;
   for (int j0 = 0; j0 < a.W; j0 += 64) {
     const int j = j0 + lane;
@@ -246,64 +294,58 @@ struct CompactArgs {
 // lies before it: a page moves iff more holes lie below it than movable pages
 // above, a hole is filled iff more movable pages lie above it than holes below.
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactArgs a, int pages) {
-  __shared__ uint32_t used[kMaxWords], keep[kMaxWords], red[kPlanWaves];
+  __shared__ uint32_t used[kMaxWords], keep[kMaxWords], below_m[kMaxWords], below_h[kMaxWords], red[kPlanWaves];
   __shared__ int top;
   const int tid = threadIdx.x;
-  const int words = (pages + 31) / 32, per = (words + kPlanThreads - 1) / kPlanThreads;
+  const int words = (pages + 31) / 32;
   for (int i = tid; i < words; i += kPlanThreads) used[i] = keep[i] = 0;
   if (tid == 0) top = -1;
   __syncthreads();
+#pragma unroll 4
   for (int64_t i = tid; i < a.entries; i += kPlanThreads) {
     const int e = a.tables[i];
     if (e >= 0 && e < pages) atomicOr(&used[e >> 5], 1u << (e & 31));
   }
   mark_held(a.held, pages, keep);
   __syncthreads();
-  uint32_t mine = 0, empty = 0, movable, holes;
-  for (int i = 0; i < per; ++i) {
-    const int w = tid * per + i;
-    if (w >= words) break;
-    mine += __popc(used[w] & ~keep[w]);
-    empty += __popc(~(used[w] | keep[w]) & word_mask(w, pages));
-  }
-  uint32_t before = block_scan(mine, red, movable);  // movable pages below
-  uint32_t below = block_scan(empty, red, holes);    // holes below
+  const uint32_t movable = count_before(words, below_m, red, [&](int w) { return used[w] & ~keep[w]; });
+  count_before(words, below_h, red, [&](int w) { return ~(used[w] | keep[w]) & word_mask(w, pages); });
   int high = -1;
   uint32_t moved = 0, moves;
-  for (int i = 0; i < per; ++i) {
-    const int w = tid * per + i;
-    if (w >= words) break;
-    const uint32_t u = used[w], k = keep[w];
-    for (int bit = 0; bit < 32 && 32 * w + bit < pages; ++bit) {
-      const int id = 32 * w + bit;
-      const uint32_t m = 1u << bit;
-      int at = id;  // where the page's content is afterwards
-      if (u & m & ~k) {
-        const uint32_t above = movable - before - 1;
-        if (below > above) {
-          a.src[above] = id;
-          ++moved;
-        } else {
-          high = id;
+  for (int id = tid; id < pages; id += kPlanThreads) {
+    const int w = id >> 5;
+    const uint32_t u = used[w], k = keep[w], bit = 1u << (id & 31), low = bit - 1;
+    const uint32_t below = below_h[w] + __popc(~(u | k) & low);                 // holes
+    const uint32_t above = movable - below_m[w] - __popc(u & ~k & (low | bit));  // movable pages
+    int at = id;  // where the page's content is afterwards
+    bool taken = true;  // whether the place is in use then
+    if (u & bit & ~k) {
+      if (below > above) {
+        // hole number `above`: the last word with no more holes before it, then its bit
+        int lo = 0, hi = w + 1;
+        while (hi - lo > 1) {
+          const int mid = (lo + hi) >> 1;
+          if (below_h[mid] <= above) lo = mid;
+          else hi = mid;
         }
-        ++before;
-      } else if (k & m) {
-        high = id;
-      } else {
-        at = -1;
-        if (movable - before > below) {
-          a.dst[below] = id;
-          high = id;
-        }
-        ++below;
+        uint32_t f = ~(used[lo] | keep[lo]);
+        for (uint32_t skip = above - below_h[lo]; skip; --skip) f &= f - 1;
+        at = 32 * lo + __ffs((int)f) - 1;
+        a.src[above] = id;
+        a.dst[above] = at;
+        ++moved;
+        taken = false;
       }
-      a.new_ids[id] = at;
+    } else if (!(k & bit)) {
+      at = -1;
+      taken = above > below;
     }
+    if (taken) high = id;
+    a.new_ids[id] = at;
   }
   if (high >= 0) atomicMax(&top, high);
   block_scan(moved, red, moves);
-  __syncthreads();  // the lists and new_ids, for the whole workgroup
-  for (uint32_t i = tid; i < moves; i += kPlanThreads) a.new_ids[a.src[i]] = a.dst[i];
+  __syncthreads();  // top
   if (tid == 0) {
     *a.count = (int32_t)moves;
     *a.top = top + 1;
@@ -357,7 +399,7 @@ __device__ __forceinline__ void move_pages(const Pools& p, const Moves& m) {
       if (p.first[mid] <= unit) lo = mid;
       else hi = mid;
     }
-    const int src = m.src[move], dst = m.dst[move];
+    const int src = m.src[move], to = m.dst[move], dst = m.via ? m.via[to] : to;
     if (src < 0 || dst < 0 || src >= p.num_blocks || dst >= p.num_blocks || src == dst) continue;  // uniform
     const int keys = m.keys ? m.keys[move] : p.block_size;
     copy_unit(p.pool[lo], p.block_size, src, dst, keys, (int64_t)(unit - p.first[lo]) * kUnit);
@@ -446,7 +488,7 @@ int nsv_copy_pages(const nsv_pool* pools, int npools, int num_blocks, int block_
   if (moves < 0) return NSV_ERR_ARG;
   if (moves == 0 || npools == 0) return NSV_OK;
   if (!src || !dst) return NSV_ERR_ARG;
-  const Moves m{src, dst, keys, nullptr, moves};
+  const Moves m{src, dst, keys, nullptr, moves, nullptr};
   for (int at = 0; at < npools; at += kPoolsPerLaunch) {
     const Pools p = take_pools(pools, npools, at, num_blocks, block_size);
     hipLaunchKernelGGL(copy_pages_kernel, dim3(move_grid(p, moves, 1)), dim3(kMoveThreads), 0, (hipStream_t)stream, p, m);
@@ -498,7 +540,7 @@ int nsv_fork_pages(const nsv_pool* pools, int npools, int num_blocks, int block_
   hipLaunchKernelGGL(fork_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, a, num_blocks, block_size);
   int rc = nsv_launch_status();
   if (rc) return rc;
-  const Moves m{a.src, a.dst, a.keys, a.count, B};
+  const Moves m{a.src, a.dst, a.keys, a.count, B, a.fresh};
   for (int at = 0; at == 0 || at < npools; at += kPoolsPerLaunch) {
     const Pools p = take_pools(pools, npools, at, num_blocks, block_size);
     if (at == 0) hipLaunchKernelGGL(fork_move_kernel, dim3(move_grid(p, B, B)), dim3(kMoveThreads), 0, s, p, m, a);
@@ -542,7 +584,7 @@ int nsv_compact_pages(const nsv_pool* pools, int npools, int num_blocks, int blo
   int rc = nsv_launch_status();
   if (rc) return rc;
   // (at most half of the pages move)
-  const Moves m{a.src, a.dst, nullptr, a.count, num_blocks};
+  const Moves m{a.src, a.dst, nullptr, a.count, num_blocks, nullptr};
   for (int at = 0; at == 0 || at < npools; at += kPoolsPerLaunch) {
     const Pools p = take_pools(pools, npools, at, num_blocks, block_size);
     const int64_t moves = num_blocks / 2;

@@ -12,6 +12,7 @@ No counterpart in the reference, whose pages belong to one sequence each.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -24,13 +25,23 @@ class _Pool(ctypes.Structure):
     _fields_ = [("base", ctypes.c_void_p), ("segments", ctypes.c_int32), ("key_bytes", ctypes.c_int32)]
 
 
+@functools.lru_cache(maxsize=256)
+def _fork_bytes(*shape: int) -> int:
+    return int(_lib.lib().nsv_fork_pages_workspace_size(*shape))
+
+
+@functools.lru_cache(maxsize=256)
+def _compact_bytes(num_blocks: int) -> int:
+    return int(_lib.lib().nsv_compact_pages_workspace_size(num_blocks))
+
+
 class CachePages:
     """The pools of one page numbering.
 
     caches: K and V pools (num_blocks, block_size, Hkv, D), of any layers,
     bfloat16 or float32; key_weights: their (num_blocks, Hkv, block_size)
     float32 tables.  All contiguous, on one device, of one num_blocks (at most
-    524,288) and block_size.  The handle keeps the tensors; it holds no other
+    262,144) and block_size.  The handle keeps the tensors; it holds no other
     state, so several threads, streams and captured graphs may use it."""
 
     def __init__(self, caches, key_weights=()):
@@ -62,29 +73,24 @@ class CachePages:
         self._pools = (_Pool * len(pools))(*pools)
         self._shape = (ctypes.addressof(self._pools), len(pools), nb, bs)
 
-    def _ids(self, t: torch.Tensor, shape: tuple, name: str, dtype=torch.int32) -> torch.Tensor:
-        if t.dtype != dtype or tuple(t.shape) != shape or t.device != self.device:
+    def _like(self, t: torch.Tensor, shape: tuple, name: str, dtype=torch.int32) -> torch.Tensor:
+        if t.dtype is not dtype or t.shape != shape or t.device != self.device:
             raise ValueError(f"{name} must be a {dtype} {shape} tensor on {self.device}, got {t.dtype} {tuple(t.shape)}")
         return t if t.is_contiguous() else t.contiguous()
-
-    def _tables(self, t: torch.Tensor) -> tuple:
-        if t.dim() != 2 or t.shape[1] == 0:
-            raise ValueError("block_tables must be (batch, pages)")
-        return self._ids(t, tuple(t.shape), "block_tables"), *t.shape
 
     def _held(self, held: torch.Tensor | None) -> torch.Tensor | None:
         if held is None:
             return None
-        if held.dtype not in (torch.bool, torch.uint8):
+        if held.dtype is not torch.bool and held.dtype is not torch.uint8:
             raise ValueError(f"held must be bool or uint8, got {held.dtype}")
-        return self._ids(held, (self.num_blocks,), "held", held.dtype)
+        return self._like(held, (self.num_blocks,), "held", held.dtype)
 
     def _out(self, t: torch.Tensor | None, shape: tuple, name: str, dtype=torch.int32) -> torch.Tensor:
         if t is None:
             return torch.empty(shape, dtype=dtype, device=self.device)
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-        return self._ids(t, shape, name, dtype)
+        return self._like(t, shape, name, dtype)
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor, keys: torch.Tensor | None = None) -> None:
         """Page src[i] to page dst[i] (int32, on the device) in every pool: its
@@ -94,8 +100,8 @@ class CachePages:
         if src.dim() != 1:
             raise ValueError("src must be (pairs,)")
         n = src.shape[0]
-        src, dst = self._ids(src, (n,), "src"), self._ids(dst, (n,), "dst")
-        keys = None if keys is None else self._ids(keys, (n,), "keys")
+        src, dst = self._like(src, (n,), "src"), self._like(dst, (n,), "dst")
+        keys = None if keys is None else self._like(keys, (n,), "keys")
         with _lib.on_device(self.device):
             rc = _lib.lib().nsv_copy_pages(*self._shape, src.data_ptr(), dst.data_ptr(), _lib.ptr(keys), n,
                                            _lib.stream_ptr(self.device))
@@ -122,16 +128,18 @@ class CachePages:
         how many pages were short; then the first row that could not get its
         pages, and every later one that needs any, is empty.  ``out_tables``
         and ``out_lens`` may not overlap the old ones."""
-        block_tables, B, width = self._tables(block_tables)
-        context_lens = self._ids(context_lens, (B,), "context_lens", torch.int64)
-        parents, held = self._ids(parents, (B,), "parents"), self._held(held)
-        out_tables = self._out(out_tables, (B, width), "out_tables")
+        if block_tables.dim() != 2 or block_tables.shape[1] == 0:
+            raise ValueError("block_tables must be (batch, pages)")
+        shape = B, width = block_tables.shape
+        block_tables = self._like(block_tables, shape, "block_tables")
+        context_lens = self._like(context_lens, (B,), "context_lens", torch.int64)
+        parents, held = self._like(parents, (B,), "parents"), self._held(held)
+        out_tables = self._out(out_tables, shape, "out_tables")
         out_lens = self._out(out_lens, (B,), "out_lens", torch.int64)
         lacking = torch.empty((), dtype=torch.int32, device=self.device)
         if B == 0:
             return out_tables, out_lens, lacking.zero_()
-        h = _lib.lib()
-        nbytes = int(h.nsv_fork_pages_workspace_size(B, width, self.num_blocks))
+        h, nbytes = _lib.lib(), _fork_bytes(B, width, self.num_blocks)
         with _lib.on_device(self.device):
             stream = _lib.stream_ptr(self.device)
             scratch = _lib.stream_scratch(self.device, stream)
@@ -155,13 +163,15 @@ class CachePages:
         ``out_tables`` may be block_tables itself.  Block tables that are not
         given, a prefix cache's ids and the like follow by new_ids; pages that
         only they name must be held."""
-        block_tables, B, width = self._tables(block_tables)
+        if block_tables.dim() != 2 or block_tables.shape[1] == 0:
+            raise ValueError("block_tables must be (batch, pages)")
+        shape = B, width = block_tables.shape
+        block_tables = self._like(block_tables, shape, "block_tables")
         held = self._held(held)
-        out_tables = self._out(out_tables, (B, width), "out_tables")
+        out_tables = self._out(out_tables, shape, "out_tables")
         new_ids = torch.empty(self.num_blocks, dtype=torch.int32, device=self.device)
         top = torch.empty((), dtype=torch.int32, device=self.device)
-        h = _lib.lib()
-        nbytes = int(h.nsv_compact_pages_workspace_size(self.num_blocks))
+        h, nbytes = _lib.lib(), _compact_bytes(self.num_blocks)
         with _lib.on_device(self.device):
             stream = _lib.stream_ptr(self.device)
             scratch = _lib.stream_scratch(self.device, stream)

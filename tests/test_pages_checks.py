@@ -38,7 +38,7 @@ def test_pools(call):
     for bad in (dict(base=0), dict(base=0x1001), dict(segments=0), dict(key_bytes=0), dict(key_bytes=3), dict(key_bytes=-2)):
         assert call(pools=_pools(**bad)) == ARG, bad
     assert call(n=-1) == call(nb=0) == call(bs=0) == ARG
-    assert call(nb=(1 << 19) + 1) == call(pools=_pools(key_bytes=1 << 28)) == UNSUPPORTED
+    assert call(nb=(1 << 18) + 1) == call(pools=_pools(key_bytes=1 << 28)) == UNSUPPORTED
 
 
 def test_fork():

@@ -142,8 +142,8 @@ def test_many_rows_and_pages():
     parents = [b // 2 for b in range(B)]
     pools = _pools(nb, 4, heads=1, dim=8, layers=1)
     _check_fork(tables, lens, parents, nb, 4, held=range(15000, 15007), pools=pools)
-    print("case: compact 524288 pages", flush=True)
-    nb = 1 << 19
+    print("case: compact 262144 pages", flush=True)
+    nb = 1 << 18
     rng = np.random.default_rng(3)
     ids = rng.choice(nb, 30000, replace=False).tolist()
     _check_compact([ids[i:i + 100] for i in range(0, 30000, 100)], nb, 1, held=ids[:50] + [nb - 1], heads=1, dim=8, layers=1)
