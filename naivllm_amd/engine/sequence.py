@@ -42,12 +42,20 @@ class Sequence:
         self.max_tokens = sampling_params.max_tokens
         self.ignore_eos = sampling_params.ignore_eos
         self.max_model_length = sampling_params.max_model_length
+        self.top_k = sampling_params.top_k
+        self.top_p = sampling_params.top_p
+        self.min_p = sampling_params.min_p
 
     def __len__(self):
         return self.num_tokens
 
     def __getitem__(self, idx):
         return self.token_ids[idx]
+
+    @property
+    def filtered(self):
+        """Whether a top-k, top-p or min-p narrows what is sampled."""
+        return self.temperature > 1e-6 and (self.top_k > 0 or self.top_p < 1 or self.min_p > 0)
 
     @property
     def is_finished(self):

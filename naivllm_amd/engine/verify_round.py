@@ -18,7 +18,9 @@ Per round and batch bucket B (K drafts, R = K + 1 rows per sequence):
      stochastic) min(1, p_t/p_d) with residual resampling for model
      drafts and row sampling for n-gram drafts, per sequence, greedy for
      temperature <= 1e-6 (spec_llm_engine.py:224-247,
-     rejection_sampler.py:24-98);
+     rejection_sampler.py:24-98); built filtered, the same under each
+     sequence's top-k, top-p and min-p, drafts sampled under them too, from
+     one uniform number per draw;
   5. commit of the accepted tokens into the history, with the caps of
      spec_llm_engine.py:249-291.
 All of it runs on one stream from static buffers, random draws included
@@ -46,7 +48,8 @@ import torch
 from naivllm_amd import _lib
 from naivllm_amd.layers.qwen3 import Qwen3Verify
 from naivllm_amd.spec_engine.drafters import ngram_draft
-from naivllm_amd.spec_engine.rejection_sampler import accept_greedy, accept_stochastic, sample
+from naivllm_amd.spec_engine.rejection_sampler import (accept_filtered, accept_greedy, accept_stochastic, sample,
+                                                       sample_filtered)
 
 DEFAULT_BUCKETS = (1, 2, 4, 8, 16, 32)
 METHODS = ("ngram", "model", "hybrid", "none")
@@ -87,7 +90,8 @@ def commit(tokens, num_tokens, num_drafts, history, hist_len, prompt_len, max_to
 class VerifyRound:
     def __init__(self, model: Qwen3Verify, max_batch: int, num_spec_tokens: int, min_ngram: int, max_ngram: int,
                  history_len: int, max_blocks: int, eos_token_id: int = -1, method: str = "ngram",
-                 draft_model: Qwen3Verify | None = None, stochastic: bool = False, buckets=DEFAULT_BUCKETS):
+                 draft_model: Qwen3Verify | None = None, stochastic: bool = False, buckets=DEFAULT_BUCKETS,
+                 filtered: bool = False):
         if method not in METHODS:
             raise ValueError(f"unknown round method {method!r}; expected one of {METHODS}")
         if method in ("model", "hybrid"):
@@ -107,7 +111,8 @@ class VerifyRound:
         self.eos = eos_token_id
         self.max_batch = max_batch
         self.buckets = sorted({b for b in buckets if b <= max_batch} | {max_batch})
-        self.stochastic = stochastic
+        self.stochastic = stochastic or filtered
+        self.filtered = filtered
         K, R, V = self.K, self.R, model.cfg.vocab_size
         i32 = dict(dtype=torch.int32, device=dev)
         i64 = dict(dtype=torch.int64, device=dev)
@@ -151,10 +156,19 @@ class VerifyRound:
             self.dctx = torch.zeros(K * max_batch, **i64)
             self.step0_logits = torch.empty(2 * max_batch, V, dtype=model.dtype, device=dev)
             self.draft_logits = torch.empty(K, max_batch, V, dtype=model.dtype, device=dev)  # step i, sequence b
-            self.draft_noise = torch.ones(K, max_batch, V, dtype=torch.float32, device=dev)
+            if filtered:
+                self.draft_uniforms = torch.zeros(K, max_batch, dtype=torch.float32, device=dev)
+            else:
+                self.draft_noise = torch.ones(K, max_batch, V, dtype=torch.float32, device=dev)
             self.cu1 = {b: torch.arange(0, b + 1, **i32) for b in self.buckets}
             self.cu2 = {b: torch.arange(0, 2 * b + 1, 2, **i32) for b in self.buckets}
-        if stochastic:
+        # each slot's filters (a filtered round's; off)
+        self.top_k = torch.zeros(max_batch, **i32)
+        self.top_p = torch.ones(max_batch, dtype=torch.float32, device=dev)
+        self.min_p = torch.zeros(max_batch, dtype=torch.float32, device=dev)
+        if filtered:
+            self.uniforms = torch.zeros(max_batch, R, dtype=torch.float32, device=dev)
+        elif stochastic:
             self.uniforms = torch.zeros(max_batch, max(K, 1), dtype=torch.float32, device=dev)
             per_seq = (V,) if method == "model" else (R, V)  # model drafts only: one multinomial per sequence
             self.accept_noise = torch.ones(max_batch, *per_seq, dtype=model.dtype, device=dev)
@@ -175,6 +189,9 @@ class VerifyRound:
             t = table[B] = torch.arange(0, B * step + 1, step, dtype=torch.int32, device=self.model.device)
         return t
 
+    def _filters(self, B: int) -> dict:
+        return dict(top_k=self.top_k[:B], top_p=self.top_p[:B], min_p=self.min_p[:B])
+
     # ------------------------------------------------------------- drafting
     def _model_draft(self, B: int) -> None:
         """K decode steps of the draft model for slots 0..B-1: step 0 feeds
@@ -185,7 +202,9 @@ class VerifyRound:
         prepare_draft(self.history[:B], self.hist_len[:B], self.block_tables[:B], dm.block_size, self.active[:B], K,
                       self.ids0[:2 * B], self.pos0[:2 * B], self.slot0[:2 * B], self.dpos[:K * B],
                       self.dslot[:K * B], self.dctx[:K * B])
-        if self.stochastic:
+        if self.filtered:
+            self.draft_uniforms.uniform_()
+        elif self.stochastic:
             self.draft_noise[:, :B].exponential_(1).clamp_min_(1e-10)  # layers/sampler.py:23
         for i in range(K):
             if i == 0:
@@ -196,8 +215,12 @@ class VerifyRound:
                 s = slice(i * B, (i + 1) * B)
                 dm.forward(self.model_drafts[:B, i - 1], self.dpos[s], self.dslot[s], self.block_tables[:B],
                            self.dctx[s], self._cu_rows(self.cu1, B, 1), 1, logits_out=self.draft_logits[i, :B])
-            sample(self.draft_logits[i, :B], self.temperature[:B], self.draft_noise[i, :B],
-                   out=self.model_drafts[:B, i])
+            if self.filtered:
+                sample_filtered(self.draft_logits[i, :B], self.temperature[:B], self.draft_uniforms[i, :B],
+                                **self._filters(B), out=self.model_drafts[:B, i])
+            else:
+                sample(self.draft_logits[i, :B], self.temperature[:B], self.draft_noise[i, :B],
+                       out=self.model_drafts[:B, i])
 
     def _draft(self, B: int) -> None:
         K = self.K
@@ -234,7 +257,16 @@ class VerifyRound:
         self.model.forward(self.input_ids[:rows], self.positions[:rows], self.slot_mapping[:rows],
                            self.block_tables[:B], self.context_lens[:B], self._cu_rows(self.cu, B, R), R,
                            logits_out=self.logits[:rows])
-        if self.stochastic:
+        if self.filtered:
+            self.uniforms[:B].uniform_()
+            rows_of = {}
+            if self.draft_model is not None:
+                rows_of = dict(draft_logits=self.draft_logits, draft_seq_stride=1, draft_row_stride=self.max_batch,
+                               draft_mode=self.draft_mode[:B] if self.method == "hybrid" else None)
+            accept_filtered(self.logits[:rows], self.drafts[:B, :K], self.num_drafts[:B], self.temperature[:B],
+                            self.uniforms[:B], target_seq_stride=R, **rows_of, **self._filters(B),
+                            out_tokens=self.out_tokens[:B], out_len=self.out_len[:B])
+        elif self.stochastic:
             self.uniforms[:B].uniform_()
             self.accept_noise[:B].exponential_(1)
             with_rows = self.draft_model is not None

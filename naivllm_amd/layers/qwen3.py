@@ -38,6 +38,7 @@ import torch.nn.functional as F
 from naivllm_amd import _lib
 from naivllm_amd.layers.attention import (PrefillPlan, PrefillRows, paged_attention_verify, prefill_attention,
                                           verify_serves_prefill)
+from naivllm_amd.layers.pages import CachePages
 
 
 @dataclass
@@ -438,6 +439,11 @@ class Qwen3Verify:
         self.k_caches = [torch.zeros(shape, device=self.device, dtype=self.dtype) for _ in range(cfg.num_layers)]
         self.v_caches = [torch.zeros(shape, device=self.device, dtype=self.dtype) for _ in range(cfg.num_layers)]
         self.block_size = block_size
+
+    def cache_pages(self) -> CachePages:
+        """The pools of every layer, to copy, fork and compact their pages
+        together (of the caches as they are: again after allocate_kv_cache)."""
+        return CachePages(self.k_caches + self.v_caches)
 
     def forward(self, input_ids: torch.Tensor, positions: torch.Tensor, slot_mapping: torch.Tensor,
                 block_tables: torch.Tensor, context_lens: torch.Tensor, cu_seqlens_q: torch.Tensor,

@@ -304,6 +304,8 @@ class ModelDrafter:
         k = self.num_speculative_tokens
         if not seqs:
             return [], []
+        if any(seq.filtered for seq in seqs):
+            raise ValueError("ModelDrafter applies a temperature alone; top_k, top_p and min_p need SpecLLMEngine")
         for seq in seqs:
             self.block_manager.ensure_capacity(seq, len(seq) + k + 1)
         temps = torch.tensor([seq.temperature for seq in seqs], dtype=torch.float32)

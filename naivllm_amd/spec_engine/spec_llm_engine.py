@@ -39,7 +39,9 @@ round until it finishes, and its slot takes the next waiting request.
 Sampling: a request with temperature <= 1e-6 is decoded greedily; any
 other temperature samples the first token, the model drafts and the
 acceptance (min(1, p_t/p_d) with residual resampling) from torch's device
-generator, seeded from ``config["seed"]``.
+generator, seeded from ``config["seed"]``.  A request's ``top_k``, ``top_p``
+and ``min_p`` hold for all three; where a waiting request has one, the call
+runs the filtered round, whose draws are uniform numbers.
 """
 
 from __future__ import annotations
@@ -56,7 +58,7 @@ from naivllm_amd.engine.sequence import Sequence, SequenceStatus
 from naivllm_amd.engine.verify_round import VerifyRound
 from naivllm_amd.layers.qwen3 import Qwen3Config, Qwen3Verify
 from naivllm_amd.sampling_parameters import SamplingParams
-from naivllm_amd.spec_engine.rejection_sampler import GREEDY_TEMPERATURE, sample
+from naivllm_amd.spec_engine.rejection_sampler import GREEDY_TEMPERATURE, sample, sample_filtered
 
 
 def _exit_if_alive(ref) -> None:
@@ -102,7 +104,8 @@ class SpecLLMEngine:
         if self.draft_model is not None:
             self.draft_model.allocate_kv_cache(num_blocks, self.block_size)
         self.eager = config.get("enforce_eager", False) or not config.get("capture_verify", True)
-        self.rounds: dict[bool, VerifyRound] = {}  # greedy / stochastic round, built on first use
+        # greedy, stochastic and filtered round, built on first use
+        self.rounds: dict[bool | str, VerifyRound] = {}
         self.spec_stats = {"method": self.spec_method, "num_speculative_tokens": K, "rounds": 0,
                            "drafted_tokens": 0, "accepted_tokens": 0, "fallback_rounds": 0}
         if self.spec_method == "hybrid":
@@ -142,16 +145,18 @@ class SpecLLMEngine:
         """The greedy round."""
         return self._round(False)
 
-    def _round(self, stochastic: bool) -> VerifyRound:
-        """The greedy or the stochastic round, built and captured on first use."""
-        r = self.rounds.get(stochastic)
+    def _round(self, stochastic: bool, filtered: bool = False) -> VerifyRound:
+        """The greedy, the stochastic or the filtered round, built and captured
+        on first use."""
+        key = "filtered" if filtered else stochastic
+        r = self.rounds.get(key)
         if r is None:
             r = VerifyRound(self.model, self.max_num_sequences, self.num_speculative_tokens, self.min_ngram,
                             self.max_ngram, self.history_len, self.max_blocks, self.eos, method=self.spec_method,
-                            draft_model=self.draft_model, stochastic=stochastic)
+                            draft_model=self.draft_model, stochastic=stochastic, filtered=filtered)
             if not self.eager:
                 r.capture()
-            self.rounds[stochastic] = r
+            self.rounds[key] = r
         return r
 
     # ---------------------------------------------------------------- prefill
@@ -171,6 +176,11 @@ class SpecLLMEngine:
         temps = torch.tensor([float(s.temperature) for s in seqs], dtype=torch.float32, device=self.device)
         if all(s.temperature <= GREEDY_TEMPERATURE for s in seqs):
             return logits.argmax(-1).tolist()
+        if any(s.filtered for s in seqs):
+            column = lambda name, dtype: torch.tensor([getattr(s, name) for s in seqs], dtype=dtype, device=self.device)  # noqa: E731
+            return sample_filtered(logits, temps, torch.rand(len(seqs), device=self.device),
+                                   top_k=column("top_k", torch.int32), top_p=column("top_p", torch.float32),
+                                   min_p=column("min_p", torch.float32)).tolist()
         noise = torch.empty(len(seqs), logits.shape[-1], dtype=torch.float32,
                             device=self.device).exponential_(1).clamp_min_(1e-10)
         return sample(logits, temps, noise).tolist()
@@ -185,6 +195,9 @@ class SpecLLMEngine:
         r.max_len[slot] = seq.max_model_length or self.max_model_length
         r.ignore_eos[slot] = int(seq.ignore_eos)
         r.temperature[slot] = float(seq.temperature)
+        r.top_k[slot] = min(seq.top_k, 0x7fffffff)
+        r.top_p[slot] = float(seq.top_p)
+        r.min_p[slot] = float(seq.min_p)
         r.block_tables[slot].fill_(-1)
         r.block_tables[slot, :len(seq.block_table)] = torch.tensor(seq.block_table, dtype=torch.int32, device=dev)
         r.active[slot] = 1
@@ -237,7 +250,8 @@ class SpecLLMEngine:
     def _generate(self, requests: list[Sequence]) -> dict:
         self._check_open()
         K = self.num_speculative_tokens
-        r = self._round(any(s.temperature > GREEDY_TEMPERATURE for s in self.scheduler.waiting))
+        r = self._round(any(s.temperature > GREEDY_TEMPERATURE for s in self.scheduler.waiting),
+                        filtered=any(s.filtered for s in self.scheduler.waiting))
         slots: list[Sequence | None] = [None] * r.max_batch
         left: dict[int, int] = {}  # slot -> tokens its sequence may still commit
         t0 = time.perf_counter()

@@ -1,0 +1,27 @@
+"""SamplingParams' filters: their checks, and what a sequence takes from them."""
+
+import pytest
+
+from naivllm_amd.engine.sequence import Sequence
+from naivllm_amd.sampling_parameters import SamplingParams
+
+
+@pytest.mark.parametrize("bad", [dict(top_k=-1), dict(top_k=2.0), dict(top_k=True), dict(top_k=None), dict(top_p=0.0),
+                                 dict(top_p=1.01), dict(top_p=float("nan")), dict(min_p=-0.1), dict(min_p=1.5),
+                                 dict(min_p=float("nan"))])
+def test_refuses(bad):
+    with pytest.raises(ValueError, match=next(iter(bad))):
+        SamplingParams(temperature=1.0, **bad)
+
+
+@pytest.mark.parametrize("settings,filtered", [
+    (dict(temperature=1.0), False), (dict(temperature=1.0, top_k=5), True), (dict(temperature=0.5, top_p=0.9), True),
+    (dict(temperature=2.0, min_p=0.1), True), (dict(temperature=0.0, top_k=5, top_p=0.5, min_p=0.5), False)])
+def test_a_sequence_knows_whether_it_is_filtered(settings, filtered):
+    seq = Sequence([1, 2, 3], SamplingParams(**settings))
+    assert seq.filtered is filtered
+    assert (seq.top_k, seq.top_p, seq.min_p) == (settings.get("top_k", 0), settings.get("top_p", 1.0), settings.get("min_p", 0.0))
+
+
+def test_the_defaults_filter_nothing():
+    assert not Sequence([1]).filtered
