@@ -86,6 +86,7 @@ struct Spot {
   uint32_t before, count;  // tokens
   uint64_t mass;           // weights before
   uint64_t weight;
+  int only;                // seek_list's, of one token: its place in the list
 };
 enum { kByCount, kReach, kAbove, kBeyond };
 
@@ -94,7 +95,7 @@ enum { kByCount, kReach, kAbove, kBeyond };
 template <typename T>
 __device__ __forceinline__ Spot seek(int kind, double goal, const T* row, int V, float top, double inv_t, double scale, RowLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Spot at{0u, 0u, 0u, 0ull, 0ull};
+  Spot at{0u, 0u, 0u, 0ull, 0ull, 0};
   constexpr int kShift[3] = {21, 10, 0}, kWidth[3] = {11, 11, 10};
   for (int level = 0; level < 3; ++level) {
     const int sh = kShift[level], bits = kWidth[level];
@@ -265,6 +266,45 @@ __device__ __forceinline__ void each_vec(const Row<T>& row, int lo, int hi, F f)
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) v[j] = w[j];
     g += AHEAD * kRowThreads;
+  }
+}
+
+// The same of an fp32 row, in no order: f(its first element, vector, whether
+// there is one).  Vectors that the row fills in part are taken by themselves,
+// behind the others, not by a second path of every load.
+template <int AHEAD, typename F>
+__device__ __forceinline__ void each_vec32(const Row<float>& row, int lo, int hi, F f) {
+  const int tid = threadIdx.x;
+  const int a = max(lo, row.skew ? 1 : 0), b = min(hi, (row.V + row.skew) / 4);  // whole ones
+  const u32x4* at = reinterpret_cast<const u32x4*>(row.at - row.skew);
+  if (a < b) {  // uniform
+    const int steps = (b - a + kRowThreads - 1) / kRowThreads;
+    u32x4 v[AHEAD];
+    int g = a + tid;
+#pragma unroll
+    for (int j = 0; j < AHEAD; ++j) v[j] = at[min(g + j * kRowThreads, b - 1)];
+#pragma unroll 1
+    for (int it = 0; it < steps; it += AHEAD) {
+      u32x4 w[AHEAD] = {};
+      if (it + AHEAD < steps) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) w[j] = at[min(g + (AHEAD + j) * kRowThreads, b - 1)];
+      }
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j)
+        if (it + j < steps) f(4 * (g + j * kRowThreads) - row.skew, v[j], g + j * kRowThreads < b);
+#pragma unroll
+      for (int j = 0; j < AHEAD; ++j) v[j] = w[j];
+      g += AHEAD * kRowThreads;
+    }
+  }
+  const bool front = lo == 0 && row.skew, back = hi == row.vecs && (row.V + row.skew) % 4 && row.vecs - 1 >= a;
+  if ((front || back) && tid < 64) {  // uniform
+    const bool in = (tid == 0 && front) || (tid == 1 && back);
+    const int g = tid == 0 ? 0 : row.vecs - 1;
+    u32x4 v{0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u};
+    if (in) v = row.load(g);
+    f(4 * g - row.skew, v, in);
   }
 }
 
@@ -705,14 +745,16 @@ __device__ __forceinline__ void decide(const Settings& f, int V, int groups, int
       }
       const Place at = seek_counts(kind, goal, s, groups, heavies, top, f.inv_t);
       if (kind == kBeyond) {
-        const double j = fmin(floor((goal - at.mass) / at.weight), (double)min((int)at.count, kept - (int)at.before) - 1.0);
         value = at.value;
-        rank = (int)fmax(j, 0.0);
+        if (at.count > 1) {
+          const double j = fmin(floor((goal - at.mass) / at.weight), (double)min((int)at.count, kept - (int)at.before) - 1.0);
+          rank = (int)fmax(j, 0.0);
+        }
         continue;
       }
       uint32_t stay = at.count;  // tokens of the value that do
       if (kind == kByCount) stay = (uint32_t)f.k - at.before;
-      if (kind == kReach) stay = (uint32_t)fmin(fmax(ceil((goal - at.mass) / at.weight), 1.0), (double)at.count);
+      if (kind == kReach && at.count > 1) stay = (uint32_t)fmin(fmax(ceil((goal - at.mass) / at.weight), 1.0), (double)at.count);
       if ((int)(at.before + stay) >= kept) continue;
       kept = (int)(at.before + stay);
       cut = at.value;
@@ -968,7 +1010,7 @@ __device__ __forceinline__ void bin_part(const Row<float>& row, int part, int st
   if (tid == 0) s.nan = 0;
   float top = -__builtin_inff();
   bool nan = false;
-  each_vec<4>(row, lo, hi, [&](int, const u32x4& v, bool) {  // (a vector past the end is the last one again)
+  each_vec32<2>(row, lo, hi, [&](int, const u32x4& v, bool) {  // (a vector past the end is the last one again)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float x = __uint_as_float(v[e]);
@@ -997,7 +1039,7 @@ __device__ __forceinline__ void bin_part(const Row<float>& row, int part, int st
     return fixed_weight(weight_of(x, bin == top_bin ? top : bin_edge(bin), inv_t, s.tab), scale);
   };
   uint32_t heavy = 0xff800000u, many = 0;  // (-inf: none)
-  each_vec<2>(row, lo, hi, [&](int, const u32x4& v, bool in) {
+  each_vec32<2>(row, lo, hi, [&](int, const u32x4& v, bool in) {
     if (!in) return;
     // a value that many of a wave's lanes hold (a mask's) is added up beside the bins
     const uint32_t some = (uint32_t)__builtin_amdgcn_readfirstlane((int)v[0]);
@@ -1054,10 +1096,12 @@ struct ListLds {
   uint32_t head[kMaxParts * kHead];  // of the parts
   double part_scale[kMaxParts];
   Bin at;                      // what wave 0 found
+  Bin range_bin[4];            // by kind: the bin of a range of one bin
+  int one_bin[4];
   float high[4], low[4];       // ranges of values to list
   int ranges;
   uint64_t list[kList];        // order bits << 32 | index
-  uint32_t sub_count[kSubBins], sub_key[kSubBins];
+  uint32_t sub_count[kSubBins], sub_at[kSubBins];
   unsigned long long sub_mass[kSubBins];
   double tab[256];
   uint32_t red[kRowWaves];
@@ -1112,8 +1156,9 @@ __device__ __forceinline__ Bin seek_bin(int kind, double goal, const ListLds& s,
   }
 }
 
-// .. for the whole workgroup
+// .. for the whole workgroup: a range of one bin is that bin
 __device__ __forceinline__ Bin find_bin(int kind, double goal, int groups, float top, double inv_t, ListLds& s) {
+  if (__builtin_amdgcn_readfirstlane(s.one_bin[kind])) return s.range_bin[kind];
   if (threadIdx.x < 64) {
     const Bin at = seek_bin(kind, goal, s, groups, top, inv_t);
     if (threadIdx.x == 0) s.at = at;
@@ -1126,7 +1171,7 @@ __device__ __forceinline__ Bin find_bin(int kind, double goal, int groups, float
 // 2^-shift of the bin's reference value.
 __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, float ref, double inv_t, double scale, ListLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  Spot at{bin << kBinShift, 0u, 0u, 0ull, 0ull};
+  Spot at{bin << kBinShift, 0u, 0u, 0ull, 0ull, -1};
 #pragma unroll 1
   for (int level = 0; level < 2; ++level) {
     const int sh = level ? 0 : 9, bits = level ? 9 : 10;
@@ -1141,7 +1186,7 @@ __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, f
       if ((k >> (sh + bits)) != (at.key >> (sh + bits))) continue;
       const uint32_t sub = (k >> sh) & ((1u << bits) - 1);
       atomicAdd(&s.sub_count[sub], 1u);
-      s.sub_key[sub] = k;
+      s.sub_at[sub] = i;
       const uint64_t q = fixed_weight(weight_of(order_value(k), ref, inv_t, s.tab), scale);
       if (q) atomicAdd(&s.sub_mass[sub], (unsigned long long)q);
     }
@@ -1175,11 +1220,13 @@ __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, f
     at.count = s.hit_count;
     at.weight = s.hit_mass;
     if (at.count == 1) {  // uniform: that token itself (fp32 values are apart as a rule)
-      at.key = s.sub_key[max(s.hit, 0)];
+      at.only = s.sub_at[max(s.hit, 0)];
+      at.key = (uint32_t)(s.list[at.only] >> 32);
       break;
     }
   }
-  at.weight /= max(at.count, 1u);  // (equal values have equal weights)
+  // (equal values have equal weights, whole numbers below 2^51: the quotient of their sum is off by less than a half)
+  if (at.count > 1) at.weight = (uint64_t)rint((double)at.weight / (double)at.count);
   return at;
 }
 
@@ -1223,8 +1270,8 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   const float top = wave_max_dpp(my_top);
   const bool nan = __ballot(lane < parts && s.head[min(lane, parts - 1) * kHead + kWords + 1]) != 0;
   const bool greedy = is_greedy(f.T);
-  const double inv_t = greedy ? 1.0 : 1.0 / (double)f.T, scale = (double)(1ull << shift);
-  if (tid < parts) s.part_scale[tid] = weight_of(my_top, top, inv_t, s.tab) / scale;
+  const double inv_t = greedy ? 1.0 : 1.0 / (double)f.T, scale = (double)(1ull << shift), per = 1.0 / scale;
+  if (tid < parts) s.part_scale[tid] = weight_of(my_top, top, inv_t, s.tab) * per;
   RowCut out{top, top, V - 1, 1, 0, 0, 1.0};
   if (nan) {  // uniform
     fits = false;
@@ -1270,7 +1317,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
         else mass += pm[j];
       }
     }
-    weight += (double)mass * (weight_of(fminf(bin_edge(bin), top), top, inv_t, s.tab) / scale);
+    weight += (double)mass * (weight_of(fminf(bin_edge(bin), top), top, inv_t, s.tab) * per);
     s.count[bin] = count;
     s.weight[bin] = weight;
     const double all = wave_sum_dpp(weight);
@@ -1310,6 +1357,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   if (wave == 0) {
     double least = total, most = total;
     int ranges = 0;
+    uint32_t hull_first = kBins32, hull_last = 0, hull_before = 0, hull_upto = 0;  // bins, tokens
 #pragma unroll 1
     for (int kind = 0; kind < 5; ++kind) {  // (4: the maximum's bin)
       if (!(kind == kByCount ? by_count : kind == kReach ? reach : kind == kAbove ? above : kind == kBeyond ? draws : greedy)) continue;
@@ -1325,17 +1373,25 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
         g1 = unit(f.u) * most * (1.0 + slack);
       }
       uint32_t first = bin_of(top), last = first;
+      uint32_t before = 0, upto_last = 0;
       if (kind < 4) {
         const Bin x = seek_bin(kind, g0, s, groups, top, inv_t);
         first = x.bin;
+        before = x.before;
+        upto_last = x.before + x.count;
         double m0 = x.mass, m1 = x.mass + x.weight;
         // (the bin reaches over both goals as a rule)
         if (kind == kReach ? m1 < g1 : kind == kBeyond && m1 <= g1) {
           const Bin y = seek_bin(kind, g1, s, groups, top, inv_t);
           last = y.bin;
+          upto_last = y.before + y.count;
           m1 = y.mass + y.weight;
         } else {
           last = first;
+        }
+        if (lane == 0) {
+          s.one_bin[kind] = first == last;
+          s.range_bin[kind] = x;
         }
         if (kind == kAbove) {
           m0 = fmin(m0, least);
@@ -1344,12 +1400,28 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
         least = m0;
         most = m1;
       }
+      if (first < hull_first) {
+        hull_first = first;
+        hull_before = before;
+      }
+      hull_last = max(hull_last, last);
+      hull_upto = max(hull_upto, upto_last);
       const float h = bin_edge(first);
       if (lane == 0) {
         s.high[ranges] = h == h ? h : __builtin_inff();  // (infinity's bin begins with NaNs)
         s.low[ranges] = order_value(((last + 1) << kBinShift) - 1);
       }
       ++ranges;
+    }
+    // Ranges with few tokens between them are one: a row of 50,001 is listed in
+    // 9,500 cycles instead of 18,000 (comparisons, not memory, bound it).
+    if (ranges > 1 && hull_upto - hull_before <= kList / 2) {
+      const float h = bin_edge(hull_first);
+      if (lane == 0) {
+        s.high[0] = h == h ? h : __builtin_inff();
+        s.low[0] = order_value(((hull_last + 1) << kBinShift) - 1);
+      }
+      ranges = 1;
     }
     if (lane == 0) s.ranges = ranges;
   }
@@ -1360,34 +1432,34 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   };
   const float h0 = bound(s.high, 0), h1 = bound(s.high, 1), h2 = bound(s.high, 2), h3 = bound(s.high, 3);
   const float l0 = bound(s.low, 0), l1 = bound(s.low, 1), l2 = bound(s.low, 2), l3 = bound(s.low, 3);
-  auto list = [&](auto four) {
-    each_vec<8>(row, 0, row.vecs, [&](int it, const u32x4& v, bool here) {
+  auto list = [&](auto several) {
+    each_vec32<4>(row, 0, row.vecs, [&](int e0, const u32x4& v, bool here) {
+      const uint64_t some = __ballot(here);
       uint64_t in[4];  // of each element: the lanes whose is in a range (comparisons all, and no branch)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float x = __uint_as_float(v[e]);
-        bool is = ((x <= h0) & (x >= l0)) | ((x <= h1) & (x >= l1));
-        if constexpr (four) is = is | ((x <= h2) & (x >= l2)) | ((x <= h3) & (x >= l3));
-        in[e] = __ballot(is & here);
+        in[e] = __ballot(x <= h0) & __ballot(x >= l0);
+        if constexpr (several)
+          in[e] |= (__ballot(x <= h1) & __ballot(x >= l1)) | (__ballot(x <= h2) & __ballot(x >= l2)) | (__ballot(x <= h3) & __ballot(x >= l3));
+        in[e] &= some;
       }
-      if (!(in[0] | in[1] | in[2] | in[3])) return;  // uniform
-      uint32_t is = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) is |= (uint32_t)((in[e] >> lane) & 1) << e;
-      const uint32_t n = __popc(is), upto_n = wave_scan(n);
+      const int n = __popcll(in[0]) + __popcll(in[1]) + __popcll(in[2]) + __popcll(in[3]);
+      if (!n) return;  // uniform
       int base = 0;
-      if (lane == 63) base = atomicAdd(&s.listed, (int)upto_n);
-      int at = (int)lane_u32((uint32_t)base, 63) + (int)(upto_n - n);
-      const int64_t e0 = (int64_t)4 * (it * kRowThreads + tid) - row.skew;
+      if (lane == 0) base = atomicAdd(&s.listed, n);
+      base = __builtin_amdgcn_readfirstlane(base);
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if ((is >> e) & 1) {
+      for (int e = 0; e < 4; ++e) {
+        if (__builtin_amdgcn_inverse_ballot_w64(in[e])) {
+          const int at = base + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(in[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)in[e], 0));
           if (at < kList) s.list[at] = ((uint64_t)order_bits(__uint_as_float(v[e])) << 32) | (uint32_t)(e0 + e);
-          ++at;
         }
+        base += __popcll(in[e]);
+      }
     });
   };
-  if (ranges > 2) list(std::true_type{});
+  if (ranges > 1) list(std::true_type{});
   else if (ranges) list(std::false_type{});
   __syncthreads();
   if (s.listed > kList) {  // uniform
@@ -1396,7 +1468,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   }
   // the cuts, one after another, among the listed tokens
   uint32_t cut_key = order_bits(top), token_key = cut_key, token_rank = 0;
-  int cut_rank = -1;
+  int cut_rank = -1, only = -1;
   bool cuts = false;  // cut_key is a value that stays in part at least
   double W = greedy ? 1.0 : total;
   int kept = greedy ? 1 : V;
@@ -1408,7 +1480,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
     const Bin at = find_bin(kByCount, (double)f.k, groups, top, inv_t, s);
     const Spot x = seek_list(kByCount, (double)((uint32_t)f.k - at.before), at.bin, ref_of(at.bin), inv_t, scale, s);
     const uint32_t n = (uint32_t)f.k - at.before - x.before;
-    W = at.mass + (double)(x.mass + n * x.weight) * (weight_of(ref_of(at.bin), top, inv_t, s.tab) / scale);
+    W = at.mass + (double)(x.mass + n * x.weight) * (weight_of(ref_of(at.bin), top, inv_t, s.tab) * per);
     cut_key = x.key;
     cut_rank = n < x.count ? (int)n - 1 : -1;
     cuts = true;
@@ -1416,11 +1488,14 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   if (reach) {
     const double goal = fmax((double)f.p * W, tiny);
     const Bin at = find_bin(kReach, goal, groups, top, inv_t, s);
-    const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) / scale;
+    const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) * per;
     const double inside = fmax((goal - at.mass) / unit_w, 0.5);
     const Spot x = seek_list(kReach, inside, at.bin, ref_of(at.bin), inv_t, scale, s);
-    const double need = ceil((inside - (double)x.mass) / (double)x.weight);
-    const uint32_t n = (uint32_t)fmin(fmax(need, 1.0), (double)x.count);
+    uint32_t n = 1;
+    if (x.count > 1) {  // uniform
+      const double need = ceil((inside - (double)x.mass) / (double)x.weight);
+      n = (uint32_t)fmin(fmax(need, 1.0), (double)x.count);
+    }
     if ((int)(at.before + x.before + n) < kept) {
       kept = (int)(at.before + x.before + n);
       W = at.mass + (double)(x.mass + n * x.weight) * unit_w;
@@ -1454,7 +1529,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
     const uint32_t n = s.hit_count;
     if ((int)(at.before + n) < kept) {
       kept = (int)(at.before + n);
-      W = at.mass + (double)s.hit_mass * (weight_of(ref, top, inv_t, s.tab) / scale);
+      W = at.mass + (double)s.hit_mass * (weight_of(ref, top, inv_t, s.tab) * per);
       // (none: what lies before the bin, whose largest possible value none of its tokens has)
       cut_key = n ? s.hit_before : at.bin << kBinShift;
       cut_rank = -1;
@@ -1464,19 +1539,23 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   if (f.sampled && kept > 1) {
     const double goal = unit(f.u) * W;
     const Bin at = find_bin(kBeyond, goal, groups, top, inv_t, s);
-    const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) / scale;
+    const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) * per;
     const double inside = fmax((goal - at.mass) / unit_w, 0.0);
     const Spot x = seek_list(kBeyond, inside, at.bin, ref_of(at.bin), inv_t, scale, s);
-    const double j = fmin(floor((inside - (double)x.mass) / (double)x.weight),
-                          (double)min((int)x.count, kept - (int)(at.before + x.before)) - 1.0);
     token_key = x.key;
-    token_rank = (uint32_t)fmax(j, 0.0);
+    if (x.count > 1) {  // uniform
+      const double j = fmin(floor((inside - (double)x.mass) / (double)x.weight),
+                            (double)min((int)x.count, kept - (int)(at.before + x.before)) - 1.0);
+      token_rank = (uint32_t)fmax(j, 0.0);
+    }
+    only = x.only;
   }
   out.kept = kept;
   out.total = W;
   if (cuts) out.cut = order_value(cut_key);
-  if (kept == 1 || f.sampled) out.token = index_in_list(token_key, token_rank, s);
-  if (kept == 1 && s.equals == 0) {  // uniform: alone because of a bin behind its own, which was not listed
+  if (only >= 0) out.token = (int)(uint32_t)s.list[only];
+  else if (kept == 1 || f.sampled) out.token = index_in_list(token_key, token_rank, s);
+  if (kept == 1 && only < 0 && s.equals == 0) {  // uniform: alone because of a bin behind its own, which was not listed
     if (tid == 0) s.index = V;
     __syncthreads();
     each<float>(row.at, V, [&](int i, float x) {
