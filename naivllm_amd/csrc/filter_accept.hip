@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kChunkThreads = 256;
 constexpr int kChunk = kChunkThreads * kVec;     // of the residual passes
+constexpr int kMaxChunks = kMaxVocab / kChunk;
 
 // drafts accepted before the first refused (a whole wave)
 __device__ __forceinline__ int accepted_by_rows(const FilterArgs& a, int b, int kb) {
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(kChunkThreads) void filter_residual_kernel(FilterAr
 // grid B: the sequence's tokens
 template <typename T>
 __global__ __launch_bounds__(kChunkThreads) void filter_finish_kernel(FilterArgs a) {
-  __shared__ double tab[256], red[kChunkThreads / 64], goal_s, before_s;
+  __shared__ double tab[256], parts[2 * kMaxChunks], red[kChunkThreads / 64], goal_s, before_s;
   __shared__ int which, use_pt, token;
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int K = a.K, kb = draft_count(a, b);
@@ -102,6 +103,9 @@ __global__ __launch_bounds__(kChunkThreads) void filter_finish_kernel(FilterArgs
     if (lane == 0) a.out_len[b] = n + 1;
     return;
   }
+  // (on their way beside what says whether they are needed; a refused draft's
+  // chunks are there, else they are whatever the memory held)
+  for (int i = tid; i < 2 * a.chunks; i += kChunkThreads) parts[i] = a.parts[(int64_t)b * a.chunks * 2 + i];
   const int n = accepted_by_rows(a, b, kb);
   if (wave == 0 && lane < n) out[lane] = d;
   if (tid == 0) a.out_len[b] = n + 1;
@@ -110,8 +114,8 @@ __global__ __launch_bounds__(kChunkThreads) void filter_finish_kernel(FilterArgs
     return;
   }
   tab[tid] = kExp2Frac256[tid];
+  __syncthreads();
   // the chunk that holds the token: the last with any weight whose sums before it do not exceed the goal
-  const double* parts = a.parts + (int64_t)b * a.chunks * 2;
   if (wave == 0) {
     double sl = 0.0;
     for (int c = lane; c < a.chunks; c += 64) sl += parts[2 * c];
@@ -119,7 +123,7 @@ __global__ __launch_bounds__(kChunkThreads) void filter_finish_kernel(FilterArgs
     double total = 0.0;
     for (int c0 = 0; c0 < a.chunks; c0 += 64) {
       const double v = wave_scan(c0 + lane < a.chunks ? parts[2 * (c0 + lane) + col] : 0.0);
-      total += __shfl(v, 63);
+      total += lane_f64(v, 63);
     }
     const double goal = unit(a.uniforms[(int64_t)b * (K + 1) + K]) * total;
     double run = 0.0, before = 0.0;
@@ -127,15 +131,14 @@ __global__ __launch_bounds__(kChunkThreads) void filter_finish_kernel(FilterArgs
     for (int c0 = 0; c0 < a.chunks; c0 += 64) {
       const double mine = c0 + lane < a.chunks ? parts[2 * (c0 + lane) + col] : 0.0;
       const double v = wave_scan(mine);
-      double prev = __shfl_up(v, 1);
-      if (lane == 0) prev = 0.0;
+      const double prev = lane_before(v);
       const uint64_t yes = __ballot(mine > 0.0 && run + prev <= goal);
       if (yes) {
         const int l = 63 - __clzll((long long)yes);
         at = c0 + l;
-        before = run + __shfl(prev, l);
+        before = run + lane_f64(prev, l);
       }
-      run += __shfl(v, 63);
+      run += lane_f64(v, 63);
     }
     if (lane == 0) {
       which = at;
@@ -154,8 +157,7 @@ __global__ __launch_bounds__(kChunkThreads) void filter_finish_kernel(FilterArgs
     mine += left[e];
   }
   const double v = wave_scan(mine);
-  double run = __shfl_up(v, 1);
-  if (lane == 0) run = 0.0;
+  double run = lane_before(v);
   if (lane == 63) red[wave] = v;
   __syncthreads();
   double before = before_s;
