@@ -308,7 +308,7 @@ int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights,
  *   partly filled one's keys.  Free is what no new row keeps and nobody holds;
  *   the lowest ids go first, row by row, column by column.  Where they run
  *   out, a row that lacks one is empty; *lacking is how many were short (0:
- *   every row is there).  B <= 4,096.  The new tables [B, max_blocks] and
+ *   every row is there).  B <= 4,096, B * max_blocks < 2^31.  The new tables [B, max_blocks] and
  *   lengths [B] may not overlap the old.
  *
  * nsv_compact_pages: of the pages in block_tables that nobody holds, the

@@ -510,7 +510,7 @@ int nsv_fork_pages(const nsv_pool* pools, int npools, int num_blocks, int block_
   const int bad = check_pools(pools, npools, num_blocks, block_size);
   if (bad) return bad;
   if (B < 0 || max_blocks <= 0) return NSV_ERR_ARG;
-  if (B > kMaxRows) return NSV_ERR_UNSUPPORTED;
+  if (B > kMaxRows || (int64_t)B * max_blocks > 0x7fffffff) return NSV_ERR_UNSUPPORTED;  // (entries are counted in 32 bits)
   if (!lacking) return NSV_ERR_ARG;
   if (B > 0 && (!block_tables || !context_lens || !parents || !out_block_tables || !out_context_lens)) return NSV_ERR_ARG;
   // (a row of the new tables is written while others of the old are read)

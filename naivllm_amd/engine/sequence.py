@@ -42,9 +42,10 @@ class Sequence:
         self.max_tokens = sampling_params.max_tokens
         self.ignore_eos = sampling_params.ignore_eos
         self.max_model_length = sampling_params.max_model_length
-        self.top_k = sampling_params.top_k
-        self.top_p = sampling_params.top_p
-        self.min_p = sampling_params.min_p
+        # (a caller's own settings, of the reference's fields, have no filters)
+        self.top_k = min(getattr(sampling_params, "top_k", 0), 0x7fffffff)
+        self.top_p = getattr(sampling_params, "top_p", 1.0)
+        self.min_p = getattr(sampling_params, "min_p", 0.0)
 
     def __len__(self):
         return self.num_tokens

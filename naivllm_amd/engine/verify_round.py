@@ -162,11 +162,11 @@ class VerifyRound:
                 self.draft_noise = torch.ones(K, max_batch, V, dtype=torch.float32, device=dev)
             self.cu1 = {b: torch.arange(0, b + 1, **i32) for b in self.buckets}
             self.cu2 = {b: torch.arange(0, 2 * b + 1, 2, **i32) for b in self.buckets}
-        # each slot's filters (a filtered round's; off)
-        self.top_k = torch.zeros(max_batch, **i32)
-        self.top_p = torch.ones(max_batch, dtype=torch.float32, device=dev)
-        self.min_p = torch.zeros(max_batch, dtype=torch.float32, device=dev)
         if filtered:
+            # each slot's filters
+            self.top_k = torch.zeros(max_batch, **i32)
+            self.top_p = torch.ones(max_batch, dtype=torch.float32, device=dev)
+            self.min_p = torch.zeros(max_batch, dtype=torch.float32, device=dev)
             self.uniforms = torch.zeros(max_batch, R, dtype=torch.float32, device=dev)
         elif stochastic:
             self.uniforms = torch.zeros(max_batch, max(K, 1), dtype=torch.float32, device=dev)

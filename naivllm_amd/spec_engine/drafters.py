@@ -304,7 +304,7 @@ class ModelDrafter:
         k = self.num_speculative_tokens
         if not seqs:
             return [], []
-        if any(seq.filtered for seq in seqs):
+        if any(getattr(seq, "filtered", False) for seq in seqs):
             raise ValueError("ModelDrafter applies a temperature alone; top_k, top_p and min_p need SpecLLMEngine")
         for seq in seqs:
             self.block_manager.ensure_capacity(seq, len(seq) + k + 1)

@@ -195,9 +195,10 @@ class SpecLLMEngine:
         r.max_len[slot] = seq.max_model_length or self.max_model_length
         r.ignore_eos[slot] = int(seq.ignore_eos)
         r.temperature[slot] = float(seq.temperature)
-        r.top_k[slot] = min(seq.top_k, 0x7fffffff)
-        r.top_p[slot] = float(seq.top_p)
-        r.min_p[slot] = float(seq.min_p)
+        if r.filtered:
+            r.top_k[slot] = seq.top_k
+            r.top_p[slot] = float(seq.top_p)
+            r.min_p[slot] = float(seq.min_p)
         r.block_tables[slot].fill_(-1)
         r.block_tables[slot, :len(seq.block_table)] = torch.tensor(seq.block_table, dtype=torch.int32, device=dev)
         r.active[slot] = 1

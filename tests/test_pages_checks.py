@@ -45,7 +45,7 @@ def test_fork():
     for bad in (dict(tables=None), dict(lens=None), dict(parents=None), dict(out=None), dict(out_lens=None), dict(lacking=None),
                 dict(B=-1), dict(W=0), dict(out=0x1000), dict(out=0x1014), dict(out_lens=0x2008)):
         assert _fork(**bad) == ARG, bad
-    assert _fork(B=4097) == UNSUPPORTED
+    assert _fork(B=4097) == _fork(B=2048, W=1 << 20, out=1 << 40) == UNSUPPORTED
     need = _lib.lib().nsv_fork_pages_workspace_size(2, 3, 10)
     assert need > 0 and _fork(size=need - 1) == _fork(ws=None) == WORKSPACE
     assert _lib.lib().nsv_fork_pages_workspace_size(4097, 3, 10) == 0

@@ -25,3 +25,16 @@ def test_a_sequence_knows_whether_it_is_filtered(settings, filtered):
 
 def test_the_defaults_filter_nothing():
     assert not Sequence([1]).filtered
+
+
+def test_settings_of_the_references_fields():
+    class Plain:
+        temperature, max_tokens, ignore_eos, max_model_length = 0.8, 5, False, None
+
+    seq = Sequence([1, 2], Plain())
+    assert not seq.filtered and (seq.top_k, seq.top_p, seq.min_p) == (0, 1.0, 0.0)
+
+
+def test_a_top_k_beyond_32_bits_keeps_everything():
+    seq = Sequence([1], SamplingParams(temperature=1.0, top_k=1 << 40))
+    assert seq.top_k == 0x7fffffff
