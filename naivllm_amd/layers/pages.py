@@ -85,12 +85,12 @@ class CachePages:
             raise ValueError(f"held must be bool or uint8, got {held.dtype}")
         return self._like(held, (self.num_blocks,), "held", held.dtype)
 
-    def _out(self, t: torch.Tensor | None, shape: tuple, name: str, dtype=torch.int32) -> torch.Tensor:
+    def _out(self, t: torch.Tensor | None, like: torch.Tensor, name: str) -> torch.Tensor:
         if t is None:
-            return torch.empty(shape, dtype=dtype, device=self.device)
+            return torch.empty_like(like)
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-        return self._like(t, shape, name, dtype)
+        return self._like(t, like.shape, name, like.dtype)
 
     def copy(self, src: torch.Tensor, dst: torch.Tensor, keys: torch.Tensor | None = None) -> None:
         """Page src[i] to page dst[i] (int32, on the device) in every pool: its
@@ -134,9 +134,9 @@ class CachePages:
         block_tables = self._like(block_tables, shape, "block_tables")
         context_lens = self._like(context_lens, (B,), "context_lens", torch.int64)
         parents, held = self._like(parents, (B,), "parents"), self._held(held)
-        out_tables = self._out(out_tables, shape, "out_tables")
-        out_lens = self._out(out_lens, (B,), "out_lens", torch.int64)
-        lacking = torch.empty((), dtype=torch.int32, device=self.device)
+        out_tables = self._out(out_tables, block_tables, "out_tables")
+        out_lens = self._out(out_lens, context_lens, "out_lens")
+        lacking = parents.new_empty(())
         if B == 0:
             return out_tables, out_lens, lacking.zero_()
         h, nbytes = _lib.lib(), _fork_bytes(B, width, self.num_blocks)
@@ -168,9 +168,8 @@ class CachePages:
         shape = B, width = block_tables.shape
         block_tables = self._like(block_tables, shape, "block_tables")
         held = self._held(held)
-        out_tables = self._out(out_tables, shape, "out_tables")
-        new_ids = torch.empty(self.num_blocks, dtype=torch.int32, device=self.device)
-        top = torch.empty((), dtype=torch.int32, device=self.device)
+        out_tables = self._out(out_tables, block_tables, "out_tables")
+        new_ids, top = block_tables.new_empty(self.num_blocks), block_tables.new_empty(())
         h, nbytes = _lib.lib(), _compact_bytes(self.num_blocks)
         with _lib.on_device(self.device):
             stream = _lib.stream_ptr(self.device)
