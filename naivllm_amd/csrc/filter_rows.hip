@@ -699,7 +699,9 @@ __device__ __forceinline__ void weigh_groups(double inv_t, int groups, int heavi
 // What the filters leave, from the weighed groups, by one wave: into s.
 __device__ __forceinline__ void decide(const Settings& f, int V, int groups, int heavies, CountLds& s) {
   const int lane = threadIdx.x & 63;
-  const uint32_t top_bits = s.ref[0] & 0xffffu;  // the maximum: the first value
+  // the maximum: the first value (group 255 is there for -0 and empty where
+  // 256, which brought it, holds other values alone)
+  const uint32_t top_bits = s.ref[s.count[0] ? 0 : min(1, groups - 1)] & 0xffffu;
   const float top = bf16_bits_to_f32(top_bits);
   uint32_t cut = top_bits, value = top_bits;
   int kept = 1, rank = 0, cut_rank = -1;

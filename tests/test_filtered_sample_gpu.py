@@ -171,6 +171,24 @@ def test_values_of_most_tokens(dtype):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("V", [1, 2, 30, 9001])
+def test_values_next_to_zero(V, dtype):
+    """Maxima among the type's smallest numbers, below zero too, beside either
+    zero and beside nothing."""
+    print(f"case: sample_filtered next to zero V {V} {dtype}", flush=True)
+    least = 2.0 ** -133 if dtype == "bf16" else 2.0 ** -149  # the type's smallest
+    few = (-least, -3 * least, -100 * least, least, 5 * least, 0.0, -0.0, -2.0 ** -126, 2.0 ** -126, -1.0)
+    rng = np.random.default_rng(V)
+    rows = [np.full(V, v) for v in few] + [rng.choice(few[:n], V) for n in range(2, len(few) + 1)]
+    rows += [np.where(rng.random(V) < 0.5, -np.inf, r) for r in rows[:8]]
+    rows += [np.where(rng.random(V) < 0.9, -5.0, r) for r in rows[:8]]
+    x = torch.tensor(np.stack(rows)).float().to(logits(0, 1, 1, dtype).dtype)
+    for n, f in enumerate((dict(), dict(top_k=np.full(len(x), 3, np.int32)), dict(top_p=np.full(len(x), 0.6, np.float32)))):
+        for T in (0.0, 0.9):
+            assert _check(x, dict(f, temperature=np.full(len(x), T, np.float32)), _uniforms(n, len(x))) == len(x)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("B,V", [(33, 16384), (65, 20011), (129, 20011), (1100, 1201), (300, 70001)])
 def test_many_rows(B, V, dtype):
     """Rows in one part and in several, of one launch and of several."""
