@@ -1,5 +1,7 @@
 """sample_filtered against the oracle."""
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -255,3 +257,43 @@ def test_captured_and_on_another_stream(dtype):
         torch.cuda.synchronize()
         assert _check(new, nf, nu, out, kept) == B
         assert torch.equal(o2, out) and torch.equal(k2, kept)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_rows_behind_32_bits(dtype):
+    """Rows whose first element is the 2^31-th and later of their storage."""
+    print(f"case: sample_filtered rows behind 32 bits {dtype}", flush=True)
+    B, V, pitch = 3, 5003, 2 ** 30 + 2 ** 28 + 7
+    x, f, u = logits(7, B, V, dtype), settings(7, B), _uniforms(7, B)
+    view = torch.empty((B - 1) * pitch + V, dtype=x.dtype, device="cuda").as_strided((B, V), (pitch, 1))
+    view.copy_(x)
+    kept = torch.zeros(B, dtype=torch.int32, device="cuda")
+    got = sample_filtered(view, uniforms=torch.from_numpy(u).cuda(), kept=kept, **on_gpu(f))
+    assert _check(x, f, u, got, kept) == B
+
+
+def test_two_threads_on_a_stream():
+    """Calls of two threads on one stream, which share its scratch."""
+    print("case: sample_filtered from two threads", flush=True)
+    jobs = []
+    for n, (B, V, dtype) in enumerate(((9, 20001, "bf16"), (5, 30001, "f32"))):
+        x, f, u = logits(n, B, V, dtype), settings(n, B), _uniforms(n, B)
+        kept = [torch.zeros(B, dtype=torch.int32, device="cuda") for _ in range(40)]
+        jobs.append((x, f, u, x.cuda(), torch.from_numpy(u).cuda(), on_gpu(f), kept, []))
+    torch.cuda.synchronize()
+
+    def run(job):
+        for kept in job[6]:
+            job[7].append(sample_filtered(job[3], uniforms=job[4], kept=kept, **job[5]))
+
+    threads = [threading.Thread(target=run, args=(job,)) for job in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for x, f, u, _, _, _, kept, got in jobs:
+        assert len(got) == 40
+        for k, g in zip(kept, got):
+            assert torch.equal(g, got[0]) and torch.equal(k, kept[0])
+        assert _check(x, f, u, got[0], kept[0]) == len(x)

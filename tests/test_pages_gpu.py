@@ -264,3 +264,26 @@ def test_refused_pools():
                 lambda: CachePages([kv[0].cpu()]), lambda: CachePages([kv[0][:0]])):
         with pytest.raises(ValueError):
             bad()
+
+
+def test_pages_behind_32_bits():
+    print("case: pages past 4 GiB of a pool", flush=True)
+    nb, bs = 70000, 16
+    kv = [torch.empty((nb, bs, 8, 256), dtype=torch.bfloat16, device="cuda") for _ in range(2)]  # 64 KiB a page
+    pages = CachePages(kv)
+    marks = [69999, 69000, 66000]
+    for n, t in enumerate(kv):
+        for page in marks:
+            t[page] = torch.randn(t.shape[1:], device="cuda").bfloat16() + n
+    was = [[t[page].clone() for page in marks] for t in kv]
+    tables, lens, lacking = pages.fork(_i32([[69999, 69000], [-1, -1]]), torch.tensor([20, 0], device="cuda"), _i32([0, 0]),
+                                       held=_held(nb, range(68000)))
+    assert tables.tolist() == [[69999, 69000], [69999, 68000]] and lens.tolist() == [20, 20] and lacking.item() == 0
+    for t, w in zip(kv, was):
+        assert torch.equal(t[68000, :4], w[1][:4])
+    pages.copy(_i32([66000]), _i32([67000]))
+    tables, _, top = pages.compact(_i32([[69999, 69000, 67000]]), held=_held(nb, range(65999)))
+    assert tables.tolist() == [[65999, 66000, 66001]] and top.item() == 66002
+    for t, w in zip(kv, was):
+        for page, content in zip((65999, 66000, 66001), w):
+            assert torch.equal(t[page], content)
