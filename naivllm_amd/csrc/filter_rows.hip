@@ -1637,7 +1637,12 @@ struct Work {
   }
 };
 
-// grid (parts, rows)
+// grid (workgroups of a row, rows).  Counting: 151,936 tokens in 7 workgroups
+// 5.8 us, 256 such rows (77.8 MB) by a workgroup each 20.4 us, 3.7 TB/s.  Bound
+// by the LDS: 8,192 additions at random words are 1,200 cycles, 0.6 of them bank
+// conflicts.  Up to 8 workgroups a row, because one CU takes in some 50 GB/s
+// however many loads are under way; not more, because the row's second
+// workgroup reads what each leaves.
 __global__ __launch_bounds__(kRowThreads) void filter_count_kernel(FilterArgs a) {
   __shared__ uint32_t bin[32768];
   const Work<uint16_t> w(a, blockIdx.y);
@@ -1646,6 +1651,10 @@ __global__ __launch_bounds__(kRowThreads) void filter_count_kernel(FilterArgs a)
   const int first = blockIdx.x * a.share, last = min(first + a.share, part_count(row, a.steps));
   if (first < last) count_parts(row, first, last, a.steps, bin, (Part*)a.row_parts + (int64_t)blockIdx.y * a.split + first);
 }
+// grid (parts, rows).  21 rows of 50,001 (4.2 MB) 7.9 us, 45 such rows 11.2: the
+// maximum, then an exponential and two LDS additions per token, the bins cleared
+// before and put away behind (2,000 to 4,500 cycles each); its waves wait for
+// 0.56 of their cycles.
 __global__ __launch_bounds__(kRowThreads) void filter_bin_kernel(FilterArgs a) {
   __shared__ BinLds s;
   const Work<float> w(a, blockIdx.y);
@@ -1655,7 +1664,11 @@ __global__ __launch_bounds__(kRowThreads) void filter_bin_kernel(FilterArgs a) {
     bin_part(row, blockIdx.x, a.steps, a.temperature[w.b], a.shift, s,
              (BinPart*)a.row_parts + (int64_t)blockIdx.y * a.split + blockIdx.x);
 }
-// grid rows
+// grid rows.  1 row of 151,936 11.7 us, 88 rows 15.3, 256 rows 17.6: a chain of
+// dependent steps in one workgroup (parts read and added 8,500 cycles, groups
+// weighed 6,000, cuts and sample by one wave 4,800, its index 5,700 in a part of 3
+// steps and 11,900 in one of 7, at 5.4 TB/s over the chip).  One workgroup a row,
+// since the steps are too short to hand over.
 __global__ __launch_bounds__(kRowThreads) void filter_merge_kernel(FilterArgs a) {
   __shared__ CountLds s;
   const Work<uint16_t> w(a, blockIdx.x);
@@ -1665,6 +1678,9 @@ __global__ __launch_bounds__(kRowThreads) void filter_merge_kernel(FilterArgs a)
   put_row(a, w.r, w.b, w.j, w.row, merge_row(row, settings_of(a, w.b, w.j.sampled, w.j.u, w.j.ends), in,
                                              part_count(row, a.steps), a.steps, s));
 }
+// grid rows.  21 rows of 50,001 24.0 us, 45 rows 33.8, as long as the row with
+// the most filters takes: parts added 10,500 cycles, a bin found 2,500, the row
+// listed 9,500 (18,000 with several ranges), each cut and the sample 4,500.
 __global__ __launch_bounds__(kRowThreads) void filter_list_kernel(FilterArgs a) {
   __shared__ RowLds32 s;
   const Work<float> w(a, blockIdx.x);

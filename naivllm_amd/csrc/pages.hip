@@ -146,6 +146,9 @@ __device__ __forceinline__ Filled filled(int64_t keys, int block_size, int W) {
   return {(int)(keys / block_size), (int)(keys % block_size)};
 }
 
+// 4 rows 6.8 us, 64 rows of 128 pages 10.6: some ten barriers and two round trips
+// to memory.  One workgroup, since places among the free pages follow from all
+// rows before; a wave per row, four rows of loads at a time.
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkArgs a, int pages, int block_size) {
   __shared__ uint32_t used[kMaxWords], before[kMaxWords], red[kPlanWaves];
   __shared__ int32_t first[kMaxRows], parent[kMaxRows], partly[kMaxRows], rest[kMaxRows];
@@ -293,6 +296,8 @@ struct CompactArgs {
 // The i-th movable page from above goes to the i-th hole from below while that
 // lies before it: a page moves iff more holes lie below it than movable pages
 // above, a hole is filled iff more movable pages lie above it than holes below.
+// 8 sequences of some 40 pages 8.0 us: ten barriers and a round trip; a thread per
+// page, its move worked out from the counts per word without a list of holes.
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactArgs a, int pages) {
   __shared__ uint32_t used[kMaxWords], keep[kMaxWords], below_m[kMaxWords], below_h[kMaxWords], red[kPlanWaves];
   __shared__ int top;
@@ -406,6 +411,9 @@ __device__ __forceinline__ void move_pages(const Pools& p, const Moves& m) {
   }
 }
 
+// Bound by memory where there is much to move: 41.7 MB compacted in 15.0 us, 5.6
+// TB/s read and written; 22 MB of a fork in 6.3, 1.5 MB in 3.7.  A workgroup
+// copies 8 KiB at a time, so few pages still spread over the chip.
 __global__ __launch_bounds__(kMoveThreads) void copy_pages_kernel(Pools p, Moves m) { move_pages(p, m); }
 
 __global__ __launch_bounds__(kMoveThreads) void fork_move_kernel(Pools p, Moves m, ForkArgs a) {
