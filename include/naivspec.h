@@ -318,7 +318,8 @@ int nsv_evict_kv(void* k_cache, void* v_cache, float* key_weights,
  *   out_block_tables: the tables with the new ids (block_tables itself, or
  *   apart from it).
  *
- * Workspaces: of any content; calls that share one must not run concurrently.
+ * Workspaces: on 16 bytes, of any content; calls that share one must not run
+ * concurrently.
  */
 typedef struct nsv_pool {
   void* base;

@@ -170,6 +170,8 @@ size_t rows_bytes(int rows, int V, int dtype);
 int launch_rows(FilterArgs& a, int dtype, void* workspace, hipStream_t s);
 
 inline size_t a256(size_t x) { return (x + 255) & ~(size_t)255; }
+inline bool off_by(const void* at, int bytes) { return ((uintptr_t)at & (bytes - 1)) != 0; }
+inline int elem_bytes(int dtype) { return dtype == NSV_BF16 ? 2 : 4; }
 inline bool bad_rows(int B, int V, int dtype) { return B < 0 || V <= 0 || (dtype != NSV_F32 && dtype != NSV_BF16); }
 // weights as integers: V of them, each at most 2^shift, stay below 2^62
 inline int weight_shift(int V) {

@@ -210,9 +210,9 @@ int nsv_sample_filtered(const void* logits, int64_t row_stride, const float* tem
   if (bad_rows(B, V, dtype) || row_stride < V || out_stride < 1) return NSV_ERR_ARG;
   if (V > kMaxVocab || B > 65535) return NSV_ERR_UNSUPPORTED;
   if (B == 0) return NSV_OK;
-  if (!logits || !temperature || !uniforms || !out_tokens) return NSV_ERR_ARG;
+  if (!logits || !temperature || !uniforms || !out_tokens || off_by(logits, elem_bytes(dtype))) return NSV_ERR_ARG;
   const size_t need = rows_bytes(B, V, dtype);
-  if (!workspace || workspace_bytes < need) return NSV_ERR_WORKSPACE;
+  if (!workspace || off_by(workspace, 16) || workspace_bytes < need) return NSV_ERR_WORKSPACE;
   FilterArgs a{};
   a.target = logits;
   a.t_seq = row_stride;
@@ -248,10 +248,12 @@ int nsv_accept_filtered(const void* target_logits, int64_t target_seq_stride, co
   if (draft_mode && !draft_logits) return NSV_ERR_ARG;
   if (V > kMaxVocab || B > 65535) return NSV_ERR_UNSUPPORTED;
   if (B == 0) return NSV_OK;
-  if (!target_logits || (!drafts && K > 0) || !num_drafts || !temperature || !uniforms || !out_tokens || !out_len)
+  if (!target_logits || (!drafts && K > 0) || !num_drafts || !temperature || !uniforms || !out_tokens || !out_len ||
+      off_by(target_logits, elem_bytes(dtype)) || off_by(draft_logits, elem_bytes(dtype)))
     return NSV_ERR_ARG;
   const Layout L = layout(B, K, V, dtype, K > 0 && draft_logits);
-  if (!workspace || workspace_bytes < nsv_accept_filtered_workspace_size(B, K, V, dtype)) return NSV_ERR_WORKSPACE;
+  if (!workspace || off_by(workspace, 16) || workspace_bytes < nsv_accept_filtered_workspace_size(B, K, V, dtype))
+    return NSV_ERR_WORKSPACE;
   FilterArgs a{};
   a.target = target_logits;
   a.t_seq = target_seq_stride * V;

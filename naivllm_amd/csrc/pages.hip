@@ -526,7 +526,7 @@ int nsv_fork_pages(const nsv_pool* pools, int npools, int num_blocks, int block_
   if (B > 0 && (out_block_tables < block_tables + entries && block_tables < out_block_tables + entries)) return NSV_ERR_ARG;
   if (B > 0 && (out_context_lens < context_lens + B && context_lens < out_context_lens + B)) return NSV_ERR_ARG;
   const ForkLayout L = fork_layout(B, max_blocks, num_blocks);
-  if (!workspace || workspace_bytes < L.total) return NSV_ERR_WORKSPACE;
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < L.total) return NSV_ERR_WORKSPACE;
   char* ws = (char*)workspace;
   ForkArgs a{};
   a.tables = block_tables;
@@ -575,7 +575,8 @@ int nsv_compact_pages(const nsv_pool* pools, int npools, int num_blocks, int blo
   if (out_block_tables != block_tables && out_block_tables < block_tables + entries &&
       block_tables < out_block_tables + entries)
     return NSV_ERR_ARG;
-  if (!workspace || workspace_bytes < nsv_compact_pages_workspace_size(num_blocks)) return NSV_ERR_WORKSPACE;
+  if (!workspace || ((uintptr_t)workspace & 15) || workspace_bytes < nsv_compact_pages_workspace_size(num_blocks))
+    return NSV_ERR_WORKSPACE;
   char* ws = (char*)workspace;
   CompactArgs a{};
   a.tables = block_tables;

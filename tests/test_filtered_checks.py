@@ -63,3 +63,9 @@ def test_tensors_on_the_cpu_are_refused():
         sample_filtered(x, 1.0, torch.zeros(2))
     with pytest.raises(ValueError, match="GPU"):
         accept_filtered(x, torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32), 1.0, torch.zeros(1, 2))
+
+
+def test_alignment():
+    odd, two, eight = (ctypes.c_void_p(0x1000 + n) for n in (1, 2, 8))
+    assert _sample(logits=odd) == _sample(logits=two, dtype=0) == _accept(target=odd) == _accept(draft=two, dtype=0) == ARG
+    assert _sample(ws=eight) == _accept(ws=eight) == WORKSPACE

@@ -47,7 +47,7 @@ def test_fork():
         assert _fork(**bad) == ARG, bad
     assert _fork(B=4097) == _fork(B=2048, W=1 << 20, out=1 << 40) == UNSUPPORTED
     need = _lib.lib().nsv_fork_pages_workspace_size(2, 3, 10)
-    assert need > 0 and _fork(size=need - 1) == _fork(ws=None) == WORKSPACE
+    assert need > 0 and _fork(size=need - 1) == _fork(ws=None) == _fork(ws=0x7008) == WORKSPACE
     assert _lib.lib().nsv_fork_pages_workspace_size(4097, 3, 10) == 0
 
 
@@ -55,7 +55,7 @@ def test_compact():
     for bad in (dict(tables=None), dict(out=None), dict(ids=None), dict(top=None), dict(B=-1), dict(W=0), dict(out=0x1004)):
         assert _compact(**bad) == ARG, bad
     need = _lib.lib().nsv_compact_pages_workspace_size(10)
-    assert need > 0 and _compact(size=need - 1) == _compact(ws=None) == WORKSPACE
+    assert need > 0 and _compact(size=need - 1) == _compact(ws=None) == _compact(ws=0x7008) == WORKSPACE
     assert _lib.lib().nsv_compact_pages_workspace_size(1 << 20) == 0
 
 
