@@ -123,31 +123,6 @@ __device__ __forceinline__ void load_vec(const T* row, int64_t base, int V, floa
   }
 }
 
-// Inclusive scan over a wave's 64 lanes on the VALU: within rows of 16 by
-// shifts of 1, 2, 4 and 8 lanes, then the last lane of row 0 and 2 to the row
-// behind it, and of row 1 to rows 2 and 3 (what has no source adds 0).  A
-// sixth of the shuffles' time, whose every step is a round trip through LDS.
-template <int CTRL, int ROWS, typename T>
-__device__ __forceinline__ T dpp_or_zero(T v) {
-  if constexpr (sizeof(T) == 4) {
-    return __builtin_bit_cast(T, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, ROWS, 0xf, false));
-  } else {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, ROWS, 0xf, false);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
-    return __builtin_bit_cast(T, ((uint64_t)hi << 32) | lo);
-  }
-}
-template <typename T>
-__device__ __forceinline__ T wave_scan(T v) {
-  v += dpp_or_zero<0x111, 0xf>(v);
-  v += dpp_or_zero<0x112, 0xf>(v);
-  v += dpp_or_zero<0x114, 0xf>(v);
-  v += dpp_or_zero<0x118, 0xf>(v);
-  v += dpp_or_zero<0x142, 0xa>(v);
-  v += dpp_or_zero<0x143, 0xc>(v);
-  return v;
-}
 // lane l's value (l uniform), and the lane's before a lane's own
 __device__ __forceinline__ double lane_f64(double v, int l) {
   return __longlong_as_double((long long)lane_u64((uint64_t)__double_as_longlong(v), l));

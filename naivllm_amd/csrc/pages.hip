@@ -43,29 +43,17 @@ struct Moves {
   const int32_t* via;    // nullable: dst holds places of this list
 };
 
-__device__ __forceinline__ uint32_t scan_u32(uint32_t v) {  // inclusive, over a wave
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t o = __shfl_up(v, d);
-    if (lane >= d) v += o;
-  }
-  return v;
-}
-
 // exclusive prefix over the workgroup, and the whole sum
-__device__ __forceinline__ uint32_t block_scan(uint32_t v, uint32_t* red, uint32_t& total) {
-  const uint32_t in = scan_u32(v);
+template <typename T>
+__device__ __forceinline__ T block_scan(T v, uint64_t* red, T& total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const T in = wave_scan(v);
   __syncthreads();
-  if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = in;
+  if (lane == 63) red[wave] = in;
   __syncthreads();
-  uint32_t before = 0, all = 0;
-  for (int w = 0; w < kPlanWaves; ++w) {
-    if (w < (int)(threadIdx.x >> 6)) before += red[w];
-    all += red[w];
-  }
-  total = all;
-  return before + in - v;
+  const uint64_t waves = lane < kPlanWaves ? red[lane] : 0ull, upto = wave_scan(waves);
+  total = (T)lane_u64(upto, 63);
+  return (T)lane_u64(upto - waves, wave) + in - v;
 }
 
 // the pages of a word that exist
@@ -74,39 +62,31 @@ __device__ __forceinline__ uint32_t word_mask(int w, int pages) {
   return left >= 32 ? ~0u : left <= 0 ? 0u : (1u << left) - 1;
 }
 
-// bits of the held pages, a thread per word
+// bits of the held pages, 64 of a wave at a time
 __device__ __forceinline__ void mark_held(const uint8_t* held, int pages, uint32_t* bits) {
   if (!held) return;
-  for (int w = threadIdx.x; 32 * w < pages; w += kPlanThreads) {
-    const uint8_t* at = held + 32 * w;
-    uint32_t m = 0;
-    if (((uintptr_t)held & 15) == 0 && 32 * w + 32 <= pages) {
-      const u32x4 a = reinterpret_cast<const u32x4*>(at)[0], b = reinterpret_cast<const u32x4*>(at)[1];
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        m |= ((a[i >> 2] >> (8 * (i & 3))) & 0xffu ? 1u : 0u) << i;
-        m |= ((b[i >> 2] >> (8 * (i & 3))) & 0xffu ? 1u : 0u) << (16 + i);
-      }
-    } else {
-      for (int i = 0; i < 32 && 32 * w + i < pages; ++i) m |= (at[i] ? 1u : 0u) << i;
-    }
-    if (m) atomicOr(&bits[w], m);
+  const int lane = threadIdx.x & 63;
+#pragma unroll 4
+  for (int first = threadIdx.x - lane; first < pages; first += kPlanThreads) {
+    const uint64_t m = __ballot(held[min(first + lane, pages - 1)] != 0 && first + lane < pages);
+    const uint32_t half = lane ? (uint32_t)(m >> 32) : (uint32_t)m;
+    if (lane < 2 && half) atomicOr(&bits[(first >> 5) + lane], half);
   }
 }
 
-// before[w] = pages of the words before w that `pick` takes; their whole number
-template <typename F>
-__device__ __forceinline__ uint32_t count_before(int words, uint32_t* before, uint32_t* red, F pick) {
-  const int per = (words + kPlanThreads - 1) / kPlanThreads, w0 = threadIdx.x * per;
-  uint32_t mine = 0, all;
-  for (int w = w0; w < min(w0 + per, words); ++w) mine += __popc(pick(w));
-  uint32_t at = block_scan(mine, red, all);
-  for (int w = w0; w < min(w0 + per, words); ++w) {
-    before[w] = at;
-    at += __popc(pick(w));
+// the n-th set bit
+__device__ __forceinline__ int nth_bit(uint32_t f, uint32_t n) {
+  int at = 0;
+#pragma unroll
+  for (int h = 16; h; h >>= 1) {
+    const uint32_t c = __popc(f & ((1u << h) - 1));
+    if (n >= c) {
+      n -= c;
+      at += h;
+      f >>= h;
+    }
   }
-  __syncthreads();
-  return all;
+  return at;
 }
 
 // ---------------------------------------------------------------------------
@@ -146,11 +126,12 @@ __device__ __forceinline__ Filled filled(int64_t keys, int block_size, int W) {
   return {(int)(keys / block_size), (int)(keys % block_size)};
 }
 
-// 4 rows 6.8 us, 64 rows of 128 pages 10.6: some ten barriers and two round trips
+// 4 rows 4.2 us, 64 rows of 128 pages 7.0: some ten barriers and three round trips
 // to memory.  One workgroup, since places among the free pages follow from all
 // rows before; a wave per row, four rows of loads at a time.
 __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkArgs a, int pages, int block_size) {
-  __shared__ uint32_t used[kMaxWords], before[kMaxWords], red[kPlanWaves];
+  __shared__ uint32_t used[kMaxWords], before[kMaxWords];
+  __shared__ uint64_t red[kPlanWaves];
   __shared__ int32_t first[kMaxRows], parent[kMaxRows], partly[kMaxRows], rest[kMaxRows];
   __shared__ uint32_t need[kMaxRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -208,7 +189,7 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkArgs a, int
     for (int i = 0; i < kAtOnce; ++i) {
       const int b = b0 + i * kPlanWaves;
       if (b >= a.B) break;  // uniform
-      const uint32_t all = lane_u32(scan_u32(n[i]), 63);
+      const uint32_t all = lane_u32(wave_scan(n[i]), 63);
       const uint64_t has = __ballot(src[i] >= 0);
       const int one = has ? (int)lane_u32((uint32_t)src[i], __ffsll((long long)has) - 1) : -1;
       if (lane == 0) {
@@ -220,12 +201,19 @@ __global__ __launch_bounds__(kPlanThreads) void fork_plan_kernel(ForkArgs a, int
   }
   __syncthreads();
   auto is_free = [&](int w) { return ~used[w] & word_mask(w, pages); };
-  const uint32_t free_pages = count_before(words, before, red, is_free);
-  // places of the rows' pages among the free ones, row by row, and of the copies
+  // the free pages before each word, and places of the rows' pages among them, row by row
+  const int per = (words + kPlanThreads - 1) / kPlanThreads, w0 = tid * per, w1 = min(w0 + per, words);
   const int rows = (a.B + kPlanThreads - 1) / kPlanThreads, r0 = tid * rows, r1 = min(r0 + rows, a.B);
-  uint32_t wanted = 0, copies = 0, all, many;
-  for (int b = r0; b < r1; ++b) wanted += need[b];
-  uint32_t at = block_scan(wanted, red, all);
+  uint64_t mine = 0, both;
+  for (int w = w0; w < w1; ++w) mine += __popc(is_free(w));
+  for (int b = r0; b < r1; ++b) mine += (uint64_t)need[b] << 32;
+  const uint64_t places = block_scan(mine, red, both);
+  const uint32_t free_pages = (uint32_t)both, all = (uint32_t)(both >> 32);
+  uint32_t below = (uint32_t)places, at = (uint32_t)(places >> 32), copies = 0, many;
+  for (int w = w0; w < w1; ++w) {
+    before[w] = below;
+    below += __popc(is_free(w));
+  }
   const uint32_t start = at;
   for (int b = r0; b < r1; ++b) {
     at += need[b];
@@ -296,15 +284,19 @@ struct CompactArgs {
 // The i-th movable page from above goes to the i-th hole from below while that
 // lies before it: a page moves iff more holes lie below it than movable pages
 // above, a hole is filled iff more movable pages lie above it than holes below.
-// 8 sequences of some 40 pages 8.0 us: ten barriers and a round trip; a thread per
+// 8 sequences of some 40 pages 4.0 us: six barriers and two round trips; a thread per
 // page, its move worked out from the counts per word without a list of holes.
 __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactArgs a, int pages) {
-  __shared__ uint32_t used[kMaxWords], keep[kMaxWords], below_m[kMaxWords], below_h[kMaxWords], red[kPlanWaves];
-  __shared__ int top;
+  __shared__ uint32_t used[kMaxWords], keep[kMaxWords], below_m[kMaxWords], below_h[kMaxWords];
+  __shared__ uint64_t red[kPlanWaves];
+  __shared__ int top, moves;
   const int tid = threadIdx.x;
   const int words = (pages + 31) / 32;
   for (int i = tid; i < words; i += kPlanThreads) used[i] = keep[i] = 0;
-  if (tid == 0) top = -1;
+  if (tid == 0) {
+    top = -1;
+    moves = 0;
+  }
   __syncthreads();
 #pragma unroll 4
   for (int64_t i = tid; i < a.entries; i += kPlanThreads) {
@@ -313,10 +305,22 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactArgs 
   }
   mark_held(a.held, pages, keep);
   __syncthreads();
-  const uint32_t movable = count_before(words, below_m, red, [&](int w) { return used[w] & ~keep[w]; });
-  count_before(words, below_h, red, [&](int w) { return ~(used[w] | keep[w]) & word_mask(w, pages); });
-  int high = -1;
-  uint32_t moved = 0, moves;
+  // movable pages and holes before each word
+  const int per = (words + kPlanThreads - 1) / kPlanThreads, w0 = tid * per, w1 = min(w0 + per, words);
+  auto counts = [&](int w) {
+    return ((uint64_t)__popc(used[w] & ~keep[w]) << 32) | __popc(~(used[w] | keep[w]) & word_mask(w, pages));
+  };
+  uint64_t mine = 0, all;
+  for (int w = w0; w < w1; ++w) mine += counts(w);
+  uint64_t below_w = block_scan(mine, red, all);
+  for (int w = w0; w < w1; ++w) {
+    below_m[w] = (uint32_t)(below_w >> 32);
+    below_h[w] = (uint32_t)below_w;
+    below_w += counts(w);
+  }
+  __syncthreads();
+  const uint32_t movable = (uint32_t)(all >> 32);
+  int high = -1, moved = 0;  // of the wave
   for (int id = tid; id < pages; id += kPlanThreads) {
     const int w = id >> 5;
     const uint32_t u = used[w], k = keep[w], bit = 1u << (id & 31), low = bit - 1;
@@ -333,26 +337,27 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(CompactArgs 
           if (below_h[mid] <= above) lo = mid;
           else hi = mid;
         }
-        uint32_t f = ~(used[lo] | keep[lo]);
-        for (uint32_t skip = above - below_h[lo]; skip; --skip) f &= f - 1;
-        at = 32 * lo + __ffs((int)f) - 1;
+        at = 32 * lo + nth_bit(~(used[lo] | keep[lo]), above - below_h[lo]);
         a.src[above] = id;
         a.dst[above] = at;
-        ++moved;
         taken = false;
       }
     } else if (!(k & bit)) {
       at = -1;
       taken = above > below;
     }
-    if (taken) high = id;
     a.new_ids[id] = at;
+    const uint64_t t = __ballot(taken);
+    if (t) high = (id & ~63) + 63 - __clzll((long long)t);
+    moved += __popcll(__ballot(at >= 0 && at != id));
   }
-  if (high >= 0) atomicMax(&top, high);
-  block_scan(moved, red, moves);
-  __syncthreads();  // top
+  if ((tid & 63) == 0) {
+    if (high >= 0) atomicMax(&top, high);
+    if (moved) atomicAdd(&moves, moved);
+  }
+  __syncthreads();
   if (tid == 0) {
-    *a.count = (int32_t)moves;
+    *a.count = moves;
     *a.top = top + 1;
   }
 }
