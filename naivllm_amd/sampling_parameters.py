@@ -7,6 +7,7 @@ rejection_sampler.sample_filtered, off by default."""
 
 from __future__ import annotations
 
+import numbers
 from dataclasses import dataclass
 
 
@@ -22,7 +23,7 @@ class SamplingParams:
 
     def __post_init__(self):
         assert self.temperature == 0 or self.temperature >= 1e-6, "temperature must be 0 (greedy) or >= 1e-6"
-        if isinstance(self.top_k, bool) or not isinstance(self.top_k, int) or self.top_k < 0:
+        if isinstance(self.top_k, bool) or not isinstance(self.top_k, numbers.Integral) or self.top_k < 0:
             raise ValueError(f"top_k must be an integer from 0 on, got {self.top_k!r}")
         if not 0 < self.top_p <= 1:
             raise ValueError(f"top_p must be above 0 and at most 1, got {self.top_p!r}")
