@@ -91,9 +91,12 @@ struct Spot {
 enum { kByCount, kReach, kAbove, kBeyond };
 
 // The last value with: tokens before it < goal (kByCount); weights before it
-// < goal (kReach) or <= goal (kBeyond), and a weight of its own.
+// < goal (kReach) or <= goal (kBeyond), and a weight of its own; kBeyond: with
+// fewer than `limit` tokens before it too (what lies behind the kept ones has
+// all their weights before it, which a goal of u = 1 does not exclude).
 template <typename T>
-__device__ __forceinline__ Spot seek(int kind, double goal, const T* row, int V, float top, double inv_t, double scale, RowLds& s) {
+__device__ __forceinline__ Spot seek(int kind, double goal, uint32_t limit, const T* row, int V, float top, double inv_t,
+                                     double scale, RowLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   Spot at{0u, 0u, 0u, 0ull, 0ull, 0};
   constexpr int kShift[3] = {21, 10, 0}, kWidth[3] = {11, 11, 10};
@@ -132,7 +135,7 @@ __device__ __forceinline__ Spot seek(int kind, double goal, const T* row, int V,
     }
     auto fits = [&](uint32_t n, uint64_t w, uint32_t before, uint64_t mass) {
       if (kind == kByCount) return n > 0 && (double)before < goal;
-      return w > 0 && (kind == kReach ? (double)mass < goal : (double)mass <= goal);
+      return w > 0 && (kind == kReach ? (double)mass < goal : (double)mass <= goal && before < limit);
     };
     int best = -1;
     if (fits(c0, m0, cb, mb)) best = 2 * tid;
@@ -413,7 +416,7 @@ __device__ __forceinline__ RowCut radix_row(const float* row, int V, int shift, 
       if (!f.sampled) continue;
       goal = unit(f.u) * (double)total;
     }
-    const Spot at = seek<float>(kind, goal, row, V, top, inv_t, scale, s);
+    const Spot at = seek<float>(kind, goal, (uint32_t)out.kept, row, V, top, inv_t, scale, s);
     if (kind == kBeyond) {
       const double j = fmin(floor((goal - (double)at.mass) / (double)at.weight),
                             (double)min((int)at.count, out.kept - (int)at.before) - 1.0);
@@ -563,8 +566,8 @@ struct Place {
 
 // As seek, from the counts of `groups` groups, by one wave.  kAbove: the last
 // value of weight >= goal.
-__device__ __forceinline__ Place seek_counts(int kind, double goal, const CountLds& s, int groups, int heavies, float top,
-                                             double inv_t) {
+__device__ __forceinline__ Place seek_counts(int kind, double goal, uint32_t limit, const CountLds& s, int groups, int heavies,
+                                             float top, double inv_t) {
   const int lane = threadIdx.x & 63;
   int at_group = -1;
 #pragma unroll 1
@@ -573,7 +576,7 @@ __device__ __forceinline__ Place seek_counts(int kind, double goal, const CountL
     bool fits;
     if (kind == kByCount) fits = (double)s.cbefore[mine] < goal;
     else if (kind == kAbove) fits = weight_of(bf16_bits_to_f32(s.ref[mine] & 0xffffu), top, inv_t, s.tab) >= goal;
-    else fits = s.mass[mine] > 0.0 && (kind == kReach ? s.before[mine] < goal : s.before[mine] <= goal);
+    else fits = s.mass[mine] > 0.0 && (kind == kReach ? s.before[mine] < goal : s.before[mine] <= goal && s.cbefore[mine] < limit);
     const uint64_t yes = __ballot(fits && s.count[mine] > 0 && 64 * i + lane < groups);  // (a group of -0 alone is empty)
     if (yes) at_group = 64 * i + 63 - __clzll((long long)yes);
   }
@@ -587,7 +590,7 @@ __device__ __forceinline__ Place seek_counts(int kind, double goal, const CountL
   auto fits = [&](uint32_t c, double w, uint32_t cb, double mb) {
     if (kind == kByCount) return c && (double)cb < goal;
     if (kind == kAbove) return c && w >= goal;
-    return c && w > 0.0 && (kind == kReach ? mb < goal : mb <= goal);
+    return c && w > 0.0 && (kind == kReach ? mb < goal : mb <= goal && cb < limit);
   };
   const uint64_t y1 = __ballot(fits(p.c1, w1, cbefore, before)), y2 = __ballot(fits(p.c2, w2, cbefore + p.c1, before + m1));
   const int l1 = y1 ? 63 - __clzll((long long)y1) : -1, l2 = y2 ? 63 - __clzll((long long)y2) : -1;
@@ -745,7 +748,7 @@ __device__ __forceinline__ void decide(const Settings& f, int V, int groups, int
         if (!f.sampled || kept == 1) continue;
         goal = unit(f.u) * total;
       }
-      const Place at = seek_counts(kind, goal, s, groups, heavies, top, f.inv_t);
+      const Place at = seek_counts(kind, goal, (uint32_t)kept, s, groups, heavies, top, f.inv_t);
       if (kind == kBeyond) {
         value = at.value;
         if (at.count > 1) {
@@ -1118,9 +1121,9 @@ union RowLds32 {
 };
 
 // The last bin with: tokens before it < goal (kByCount); weights before it <
-// goal (kReach) or <= goal (kBeyond), and a weight of its own; a largest
-// possible weight >= goal (kAbove).  By one wave.
-__device__ __forceinline__ Bin seek_bin(int kind, double goal, const ListLds& s, int groups, float top, double inv_t) {
+// goal (kReach) or <= goal (kBeyond, and tokens before it < limit), and a weight
+// of its own; a largest possible weight >= goal (kAbove).  By one wave.
+__device__ __forceinline__ Bin seek_bin(int kind, double goal, uint32_t limit, const ListLds& s, int groups, float top, double inv_t) {
   const int lane = threadIdx.x & 63;
   int n = -1;
 #pragma unroll 1
@@ -1130,14 +1133,15 @@ __device__ __forceinline__ Bin seek_bin(int kind, double goal, const ListLds& s,
     if (kind == kByCount) fits = (double)s.gcbefore[mine] < goal;
     // (a group's first bin may be empty: whether another of it is heavy enough shows below)
     else if (kind == kAbove) fits = weight_of(fminf(bin_edge(64 * s.gid[mine]), top), top, inv_t, s.tab) >= goal;
-    else fits = s.gweight[mine] > 0.0 && (kind == kReach ? s.gbefore[mine] < goal : s.gbefore[mine] <= goal);
+    else if (kind == kReach) fits = s.gweight[mine] > 0.0 && s.gbefore[mine] < goal;
+    else fits = s.gweight[mine] > 0.0 && s.gbefore[mine] <= goal && s.gcbefore[mine] < limit;
     const uint64_t yes = __ballot(fits && 64 * i + lane < groups);
     if (yes) n = 64 * i + 63 - __clzll((long long)yes);
   }
   n = max(n, 0);
   Bin at{};
 #pragma unroll 1
-  for (;; --n) {  // (kAbove: to a group before, where the bins that are heavy enough are empty)
+  for (;; --n) {  // (to a group before, where the bins that are heavy enough are empty, or those with a weight past the limit)
     const uint32_t bin = 64 * s.gid[n] + lane, c = s.count[bin];
     const double w = s.weight[bin];
     const double before = s.gbefore[n] + lane_before(wave_scan(w));
@@ -1145,7 +1149,7 @@ __device__ __forceinline__ Bin seek_bin(int kind, double goal, const ListLds& s,
     bool fits = c > 0;
     if (kind == kByCount) fits = fits && (double)cbefore < goal;
     else if (kind == kAbove) fits = fits && weight_of(fminf(bin_edge(bin), top), top, inv_t, s.tab) >= goal;
-    else fits = fits && w > 0.0 && (kind == kReach ? before < goal : before <= goal);
+    else fits = fits && w > 0.0 && (kind == kReach ? before < goal : before <= goal && cbefore < limit);
     const uint64_t yes = __ballot(fits);
     if (!yes && n > 0) continue;
     const int l = yes ? 63 - __clzll((long long)yes) : 0;
@@ -1158,11 +1162,12 @@ __device__ __forceinline__ Bin seek_bin(int kind, double goal, const ListLds& s,
   }
 }
 
-// .. for the whole workgroup: a range of one bin is that bin
-__device__ __forceinline__ Bin find_bin(int kind, double goal, int groups, float top, double inv_t, ListLds& s) {
+// .. for the whole workgroup: a range of one bin is that bin (kBeyond's begins
+// with a bin that holds kept tokens: its goal is below the weights before the cut's)
+__device__ __forceinline__ Bin find_bin(int kind, double goal, uint32_t limit, int groups, float top, double inv_t, ListLds& s) {
   if (__builtin_amdgcn_readfirstlane(s.one_bin[kind])) return s.range_bin[kind];
   if (threadIdx.x < 64) {
-    const Bin at = seek_bin(kind, goal, s, groups, top, inv_t);
+    const Bin at = seek_bin(kind, goal, limit, s, groups, top, inv_t);
     if (threadIdx.x == 0) s.at = at;
   }
   __syncthreads();
@@ -1171,7 +1176,8 @@ __device__ __forceinline__ Bin find_bin(int kind, double goal, int groups, float
 
 // As seek, among the listed tokens of a bin.  mass, weight: integers of
 // 2^-shift of the bin's reference value.
-__device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, float ref, double inv_t, double scale, ListLds& s) {
+__device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t limit, uint32_t bin, float ref, double inv_t, double scale,
+                                          ListLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   Spot at{bin << kBinShift, 0u, 0u, 0ull, 0ull, -1};
 #pragma unroll 1
@@ -1206,7 +1212,7 @@ __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t bin, f
     const uint64_t mb = at.mass + mu - m + lane_u64(wave_scan(mw) - mw, wave);
     bool fits = c > 0;
     if (kind == kByCount) fits = fits && (double)cb < goal;
-    else fits = fits && m > 0 && (kind == kReach ? (double)mb < goal : (double)mb <= goal);
+    else fits = fits && m > 0 && (kind == kReach ? (double)mb < goal : (double)mb <= goal && cb < limit);
     if (fits) atomicMax(&s.hit, tid);
     __syncthreads();
     if (tid == max(s.hit, 0)) {
@@ -1377,14 +1383,14 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
       uint32_t first = bin_of(top), last = first;
       uint32_t before = 0, upto_last = 0;
       if (kind < 4) {
-        const Bin x = seek_bin(kind, g0, s, groups, top, inv_t);
+        const Bin x = seek_bin(kind, g0, V, s, groups, top, inv_t);
         first = x.bin;
         before = x.before;
         upto_last = x.before + x.count;
         double m0 = x.mass, m1 = x.mass + x.weight;
         // (the bin reaches over both goals as a rule)
         if (kind == kReach ? m1 < g1 : kind == kBeyond && m1 <= g1) {
-          const Bin y = seek_bin(kind, g1, s, groups, top, inv_t);
+          const Bin y = seek_bin(kind, g1, V, s, groups, top, inv_t);
           last = y.bin;
           upto_last = y.before + y.count;
           m1 = y.mass + y.weight;
@@ -1479,8 +1485,8 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   out.cut = greedy ? top : -__builtin_inff();
   auto ref_of = [&](uint32_t bin) { return fminf(bin_edge(bin), top); };
   if (by_count) {
-    const Bin at = find_bin(kByCount, (double)f.k, groups, top, inv_t, s);
-    const Spot x = seek_list(kByCount, (double)((uint32_t)f.k - at.before), at.bin, ref_of(at.bin), inv_t, scale, s);
+    const Bin at = find_bin(kByCount, (double)f.k, V, groups, top, inv_t, s);
+    const Spot x = seek_list(kByCount, (double)((uint32_t)f.k - at.before), V, at.bin, ref_of(at.bin), inv_t, scale, s);
     const uint32_t n = (uint32_t)f.k - at.before - x.before;
     W = at.mass + (double)(x.mass + n * x.weight) * (weight_of(ref_of(at.bin), top, inv_t, s.tab) * per);
     cut_key = x.key;
@@ -1489,10 +1495,10 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   }
   if (reach) {
     const double goal = fmax((double)f.p * W, tiny);
-    const Bin at = find_bin(kReach, goal, groups, top, inv_t, s);
+    const Bin at = find_bin(kReach, goal, V, groups, top, inv_t, s);
     const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) * per;
     const double inside = fmax((goal - at.mass) / unit_w, 0.5);
-    const Spot x = seek_list(kReach, inside, at.bin, ref_of(at.bin), inv_t, scale, s);
+    const Spot x = seek_list(kReach, inside, V, at.bin, ref_of(at.bin), inv_t, scale, s);
     uint32_t n = 1;
     if (x.count > 1) {  // uniform
       const double need = ceil((inside - (double)x.mass) / (double)x.weight);
@@ -1508,7 +1514,7 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   }
   if (above) {
     const double goal = fmin((double)f.least, 1.0);
-    const Bin at = find_bin(kAbove, goal, groups, top, inv_t, s);
+    const Bin at = find_bin(kAbove, goal, V, groups, top, inv_t, s);
     const float ref = ref_of(at.bin);
     // the bin's tokens that are heavy enough: how many, their weights, the lightest
     __syncthreads();
@@ -1540,10 +1546,10 @@ __device__ __forceinline__ RowCut list_row(const Row<float>& row, Settings f, co
   }
   if (f.sampled && kept > 1) {
     const double goal = unit(f.u) * W;
-    const Bin at = find_bin(kBeyond, goal, groups, top, inv_t, s);
+    const Bin at = find_bin(kBeyond, goal, (uint32_t)kept, groups, top, inv_t, s);
     const double unit_w = weight_of(ref_of(at.bin), top, inv_t, s.tab) * per;
     const double inside = fmax((goal - at.mass) / unit_w, 0.0);
-    const Spot x = seek_list(kBeyond, inside, at.bin, ref_of(at.bin), inv_t, scale, s);
+    const Spot x = seek_list(kBeyond, inside, (uint32_t)kept - at.before, at.bin, ref_of(at.bin), inv_t, scale, s);
     token_key = x.key;
     if (x.count > 1) {  // uniform
       const double j = fmin(floor((inside - (double)x.mass) / (double)x.weight),

@@ -1,0 +1,58 @@
+"""Filtered sampling and acceptance by uniform numbers at and next to the end
+of their range, against the oracle."""
+
+import numpy as np
+import pytest
+import torch
+
+from naivllm_amd.spec_engine.rejection_sampler import sample_filtered
+from tests.filtered_util import logits
+from tests.test_filtered_accept_gpu import _case, _run, _want
+from tests.test_filtered_sample_gpu import _check
+
+pytestmark = pytest.mark.gpu
+
+
+def _settings(B, **kw):
+    f = dict(temperature=np.ones(B, np.float32))
+    return f | {k: np.full(B, v, np.int32 if k == "top_k" else np.float32) for k, v in kw.items()}
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_one_behind_two_kept(dtype):
+    """1 takes the last token kept, not the first behind it."""
+    print(f"case: sample_filtered of 1, three tokens {dtype}", flush=True)
+    x = logits(0, 1, 3, dtype).copy_(torch.tensor([[2.0, 1.0, 0.0]]))
+    for kw in (dict(top_k=2), dict(top_p=0.8), dict(min_p=0.2)):
+        for u in (1.0, 7.0):
+            assert _check(x, _settings(1, **kw), np.full(1, u, np.float32)) == 1, (kw, u)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("shift", [0.0, 200.0])
+@pytest.mark.parametrize("setting", [dict(top_k=2), dict(top_k=300), dict(top_p=0.5), dict(top_p=0.9), dict(min_p=0.3),
+                                     dict(min_p=2e-3), dict(top_k=400, top_p=0.8, min_p=0.01)])
+def test_one_under_filters(dtype, shift, setting):
+    """The same of long rows, whose cuts lie between distinct and between equal
+    values; rows around 200 have more fp32 tokens next to a cut than are listed."""
+    print(f"case: sample_filtered of 1, {setting} around {shift} {dtype}", flush=True)
+    B, V = 4, 20011
+    for n, shape in enumerate(("flat", "peaked", "levels", "equal")):
+        x = (logits(50 + n, B, V, "f32", shape) + shift).to(logits(0, 1, 1, dtype).dtype)
+        assert _check(x, _settings(B, **setting), np.ones(B, np.float32)) == B, shape
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("mode", ["model", "ngram", "hybrid"])
+def test_one_in_rounds(mode, dtype):
+    """Every number of a round 1: samples, refused drafts, residuals, bonus rows."""
+    print(f"case: accept_filtered of 1, {mode} {dtype}", flush=True)
+    target, draft, f, drafts, live, u = _case(61, 9, 4, 2049, dtype, near=0.02)
+    f = dict(temperature=np.full(9, 0.9, np.float32), top_k=np.where(np.arange(9) % 3 == 0, 40, 0).astype(np.int32),
+             top_p=np.where(np.arange(9) % 3 == 1, 0.8, 1.0).astype(np.float32),
+             min_p=np.where(np.arange(9) % 3 == 2, 0.02, 0.0).astype(np.float32))
+    u[:] = 1.0
+    u[::2, 0] = 0.0  # (1 refuses a draft more likely in the draft row)
+    draft = None if mode == "ngram" else draft
+    modes = (np.arange(9) % 2).astype(np.int32) if mode == "hybrid" else None
+    assert _run(target, draft, f, drafts, live, u, modes) == _want(target, draft, f, drafts, live, u, modes)
