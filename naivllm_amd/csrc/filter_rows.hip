@@ -1175,7 +1175,9 @@ __device__ __forceinline__ Bin find_bin(int kind, double goal, uint32_t limit, i
 }
 
 // As seek, among the listed tokens of a bin.  mass, weight: integers of
-// 2^-shift of the bin's reference value.
+// 2^-shift of the bin's reference value.  The first value always fits: the bin
+// itself does, also where its tokens weigh nothing beside its reference (the
+// bin's weight can come from the maximum of a part, weighed by that).
 __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t limit, uint32_t bin, float ref, double inv_t, double scale,
                                           ListLds& s) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -1212,7 +1214,7 @@ __device__ __forceinline__ Spot seek_list(int kind, double goal, uint32_t limit,
     const uint64_t mb = at.mass + mu - m + lane_u64(wave_scan(mw) - mw, wave);
     bool fits = c > 0;
     if (kind == kByCount) fits = fits && (double)cb < goal;
-    else fits = fits && m > 0 && (kind == kReach ? (double)mb < goal : (double)mb <= goal && cb < limit);
+    else fits = fits && (cb == at.before || (m > 0 && (kind == kReach ? (double)mb < goal : (double)mb <= goal && cb < limit)));
     if (fits) atomicMax(&s.hit, tid);
     __syncthreads();
     if (tid == max(s.hit, 0)) {

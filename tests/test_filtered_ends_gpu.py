@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from naivllm_amd.spec_engine.rejection_sampler import sample_filtered
-from tests.filtered_util import logits
+from tests.filtered_util import logits, on_gpu
 from tests.test_filtered_accept_gpu import _case, _run, _want
 from tests.test_filtered_sample_gpu import _check
 
@@ -56,3 +56,22 @@ def test_one_in_rounds(mode, dtype):
     draft = None if mode == "ngram" else draft
     modes = (np.arange(9) % 2).astype(np.int32) if mode == "hybrid" else None
     assert _run(target, draft, f, drafts, live, u, modes) == _want(target, draft, f, drafts, live, u, modes)
+
+
+@pytest.mark.parametrize("setting", [dict(), dict(top_k=900), dict(top_p=1 - 2.0 ** -24, top_k=4000)])
+@pytest.mark.parametrize("count", [1, 3, 700])
+def test_one_behind_a_far_maximum(count, setting):
+    """At a low temperature tokens of 3 weigh e^-150 beside a maximum of 3.3 in
+    another stretch of the row, and e^-62 of the largest value next to them: the
+    sample of 1 is the maximum or one of them, never a masked token."""
+    print(f"case: sample_filtered of 1 behind a far maximum, {count} tokens, {setting}", flush=True)
+    B, V = 2, 20000
+    x = torch.full((B, V), -np.inf)
+    x[:, 5000] = 3.3
+    x[0, 10000:10000 + count] = 3.0
+    x[1, 10000:10000 + count] = 3.0 + 2.0 ** -20 * torch.arange(count)
+    f = _settings(B, **setting) | dict(temperature=np.full(B, 0.002, np.float32))
+    kept = torch.zeros(B, dtype=torch.int32, device="cuda")
+    got = sample_filtered(x.cuda(), uniforms=torch.ones(B, device="cuda"), kept=kept, **on_gpu(f))
+    assert torch.isfinite(x.gather(1, got.cpu().long()[:, None])).all()
+    assert _check(x, f, np.ones(B, np.float32), got, kept) is not None
