@@ -29,6 +29,7 @@ import torch
 from naivllm_amd import _lib
 
 GREEDY_TEMPERATURE = 1e-6  # temperature <= this selects greedy (rejection_sampler.py:95)
+_BELOW_ONE = 1 - 2.0 ** -24  # the largest float32 below 1
 
 
 def _i32(x, device) -> torch.Tensor:
@@ -221,6 +222,14 @@ def _per_row(x, rows: int, dtype: torch.dtype, device, name: str) -> torch.Tenso
     return x if x.is_contiguous() else x.contiguous()
 
 
+def _uniforms32(x):
+    """Uniform numbers as float32, in which those of 64 bits next to 1 would
+    round to 1: they stay below it."""
+    if isinstance(x, torch.Tensor):
+        return x.to(torch.float32).clamp_(max=_BELOW_ONE) if x.dtype == torch.float64 else x
+    return min(x, _BELOW_ONE) if isinstance(x, float) else x
+
+
 def _check_out(t: torch.Tensor, shape: tuple, device, name: str, strided: bool = False) -> None:
     if t.dtype != torch.int32 or tuple(t.shape) != shape or t.device != device:
         raise ValueError(f"{name} must be an int32 {shape} tensor on {device}")
@@ -270,7 +279,7 @@ def sample_filtered(logits: torch.Tensor, temperature, uniforms: torch.Tensor, t
     temperature = _per_row(temperature, B, torch.float32, dev, "temperature")
     if temperature is None or uniforms is None:
         raise ValueError("sample_filtered needs a temperature and uniforms")
-    uniforms = _per_row(uniforms, B, torch.float32, dev, "uniforms")
+    uniforms = _per_row(_uniforms32(uniforms), B, torch.float32, dev, "uniforms")
     top_k = _per_row(top_k, B, torch.int32, dev, "top_k")
     top_p = _per_row(top_p, B, torch.float32, dev, "top_p")
     min_p = _per_row(min_p, B, torch.float32, dev, "min_p")
@@ -344,7 +353,7 @@ def accept_filtered(target_logits: torch.Tensor, drafts: torch.Tensor, num_draft
                 raise ValueError("draft_mode must hold one flag per sequence")
     if uniforms is None or tuple(uniforms.shape) != (B, K + 1):
         raise ValueError(f"uniforms must be ({B}, {K + 1})")
-    uniforms = uniforms.to(device=dev, dtype=torch.float32).contiguous()
+    uniforms = _uniforms32(uniforms).to(device=dev, dtype=torch.float32).contiguous()
     temperature = _per_row(temperature, B, torch.float32, dev, "temperature")
     if temperature is None:
         raise ValueError("accept_filtered needs a temperature")

@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 import torch
 
-from naivllm_amd.spec_engine.rejection_sampler import sample_filtered
+from naivllm_amd.spec_engine.rejection_sampler import accept_filtered, sample_filtered
 from tests.filtered_util import logits, on_gpu
 from tests.test_filtered_accept_gpu import _case, _run, _want
 from tests.test_filtered_sample_gpu import _check
@@ -75,3 +75,20 @@ def test_one_behind_a_far_maximum(count, setting):
     got = sample_filtered(x.cuda(), uniforms=torch.ones(B, device="cuda"), kept=kept, **on_gpu(f))
     assert torch.isfinite(x.gather(1, got.cpu().long()[:, None])).all()
     assert _check(x, f, np.ones(B, np.float32), got, kept) is not None
+
+
+def test_wide_numbers_below_one():
+    """64-bit numbers below 1 that round to 1 in 32 bits, and such a number for
+    every row: a draft as likely in both rows stays, a sample is a kept token."""
+    print("case: filtered draws of 64-bit numbers next to 1", flush=True)
+    B, K, V = 3, 2, 64
+    near = torch.tensor([1 - 2.0 ** -26, 1 - 2.0 ** -40, 1 - 2.0 ** -53], dtype=torch.float64, device="cuda")
+    rows = logits(5, B * (K + 1), V, "f32").cuda()
+    draft = rows.view(B, K + 1, V)[:, :K].reshape(-1, V).contiguous()
+    drafts = draft.argmax(1).view(B, K).int()
+    tokens, lens = accept_filtered(rows, drafts, torch.full((B,), K, dtype=torch.int32), 1.0, near[:, None].expand(B, K + 1),
+                                   draft_logits=draft, draft_seq_stride=K, top_k=5)
+    assert lens.tolist() == [K + 1] * B and torch.equal(tokens[:, :K], drafts)
+    x = torch.tensor([[2.0, 1.0, 0.0]], device="cuda").expand(B, 3).contiguous()
+    for u in (near, 1 - 2.0 ** -30):
+        assert sample_filtered(x, 1.0, u, top_k=2).tolist() == [1] * B
