@@ -313,16 +313,17 @@ def accept_filtered(target_logits: torch.Tensor, drafts: torch.Tensor, num_draft
     which hold for a sequence's target and draft rows alike: the accepted
     tokens are distributed as the filtered target's samples.
 
-    Rows, drafts, draft_mode and outputs as accept_stochastic's; temperature
-    and the filters (B,) tensors, numbers, or None.  uniforms (B, K + 1)
-    float32.  With draft rows and a temperature above 1e-6 a draft stays if
-    its uniform number times its draft probability is below its target
-    probability; at the first that does not, the last uniform number draws
-    from max(p_target - p_draft, 0) in the order of the indices; behind kept
-    drafts it samples the bonus row.  Otherwise uniform number r samples row
-    r, and drafts stay while they equal the samples.  Returns (tokens
-    (B, K + 1) int32, lengths (B,) int32) on the device; entries past a
-    sequence's tokens are not written.  No counterpart in the reference."""
+    Rows, drafts, draft_mode and outputs as accept_stochastic's, target and
+    draft logits contiguous; temperature and the filters (B,) tensors, numbers,
+    or None. uniforms (B, K + 1) float32. With draft rows and a temperature
+    above 1e-6 a draft stays if its uniform number times its draft probability
+    is below its target probability; at the first that does not, the last
+    uniform number draws from max(p_target - p_draft, 0) in the order of the
+    indices; behind kept drafts it samples the bonus row. Otherwise uniform
+    number r samples row r, and drafts stay while they equal the samples.
+    Returns (tokens (B, K + 1) int32, lengths (B,) int32) on the device;
+    entries past a sequence's tokens are not written. No counterpart in the
+    reference."""
     _check_logits(target_logits, "target_logits")
     dev = target_logits.device
     V = target_logits.shape[-1]
@@ -343,6 +344,8 @@ def accept_filtered(target_logits: torch.Tensor, drafts: torch.Tensor, num_draft
         _check_logits(draft_logits, "draft_logits")
         if draft_logits.dtype != target_logits.dtype or draft_logits.device != dev or draft_logits.shape[-1] != V:
             raise ValueError("draft and target logits must share dtype, device and vocabulary")
+        if not draft_logits.is_contiguous():
+            raise ValueError("draft_logits must be contiguous (its rows are counted from the first)")
         if draft_row_stride < 1 or draft_seq_stride < 0:
             raise ValueError("bad draft strides")
         if B and K:

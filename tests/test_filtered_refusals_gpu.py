@@ -59,3 +59,22 @@ def test_what_is_allowed_runs():
     assert _sample(top_k=torch.full((3,), 2 ** 40, device="cuda"), out=_i32(3, 2)[:, 1]).shape == (3,)
     tokens, lens = _accept()
     assert tokens.shape == (2, 3) and lens.tolist() == [1, 1]
+
+
+@pytest.mark.parametrize("draft", [lambda: torch.zeros(4, 128, device="cuda")[:, :64], lambda: torch.zeros(8, 64, device="cuda")[::2],
+                                   lambda: torch.zeros(2, 3, 64, device="cuda")[:, :2],
+                                   lambda: torch.zeros(1, 64, device="cuda").expand(4, 64)])
+def test_draft_rows_apart(draft):
+    """Rows of draft logits that do not lie one behind another: whatever lies
+    between them would be taken for rows."""
+    with pytest.raises(ValueError, match="draft_logits must be contiguous"):
+        _accept(draft_logits=draft())
+
+
+def test_draft_rows_of_a_larger_buffer():
+    """Contiguous ones of it are taken, whatever lies before and behind."""
+    buf = torch.full((7, 64), 9.0, device="cuda")
+    buf[2:6] = 0.0
+    buf[2, 5] = 3.0
+    got, want = _accept(draft_logits=buf[2:6], top_k=4), _accept(draft_logits=buf[2:6].clone(), top_k=4)
+    assert torch.equal(got[1], want[1]) and torch.equal(got[0][:, 0], want[0][:, 0])
