@@ -274,6 +274,12 @@ class DraftRunner:
         return host, b["logits"][:, :B]
 
 
+def refuse_filters(seqs) -> None:
+    """The draft model's tokens are sampled with a temperature alone."""
+    if any(getattr(seq, "filtered", False) for seq in seqs):
+        raise ValueError("ModelDrafter applies a temperature alone; top_k, top_p and min_p need SpecLLMEngine")
+
+
 class ModelDrafter:
     """Draft with a small model running K autoregressive decode steps
     (drafters.py:86-154): same constructor, ``can_draft``, ``prefill`` and
@@ -304,8 +310,7 @@ class ModelDrafter:
         k = self.num_speculative_tokens
         if not seqs:
             return [], []
-        if any(getattr(seq, "filtered", False) for seq in seqs):
-            raise ValueError("ModelDrafter applies a temperature alone; top_k, top_p and min_p need SpecLLMEngine")
+        refuse_filters(seqs)
         for seq in seqs:
             self.block_manager.ensure_capacity(seq, len(seq) + k + 1)
         temps = torch.tensor([seq.temperature for seq in seqs], dtype=torch.float32)
@@ -339,6 +344,7 @@ class HybridDrafter:
         return True
 
     def draft(self, seqs) -> tuple[list[list[int]], list]:
+        refuse_filters(seqs)  # (before the lookup appends its drafts; any of them may fall to the model)
         rows = [None] * len(seqs)
         self.ngram.draft(seqs)
         rest_idx = [i for i, seq in enumerate(seqs) if not seq.draft_tokens]
