@@ -512,7 +512,7 @@ int nsv_copy_pages(const nsv_pool* pools, int npools, int num_blocks, int block_
 }
 
 size_t nsv_fork_pages_workspace_size(int B, int max_blocks, int num_blocks) {
-  if (B <= 0 || B > kMaxRows || max_blocks <= 0 || num_blocks <= 0) return 0;
+  if (B < 0 || B > kMaxRows || max_blocks <= 0 || num_blocks <= 0) return 0;
   return fork_layout(B, max_blocks, num_blocks).total;
 }
 

@@ -67,3 +67,10 @@ def test_copy():
 def test_pools_on_the_cpu_are_refused():
     with pytest.raises(ValueError, match="GPU"):
         CachePages([torch.zeros(4, 2, 1, 8)])
+
+
+def test_fork_of_an_empty_batch_says_what_it_needs():
+    size = _lib.lib().nsv_fork_pages_workspace_size
+    need = size(0, 3, 10)
+    assert need > 0 and size(-1, 3, 10) == size(0, 0, 10) == size(0, 3, 0) == 0
+    assert _fork(B=0, size=need - 1) == _fork(B=0, ws=None) == WORKSPACE

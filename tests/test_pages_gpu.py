@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 import torch
 
+from naivllm_amd import _lib
 from naivllm_amd.layers.pages import CachePages
 from oracle import pages as op
 
@@ -287,3 +288,25 @@ def test_pages_behind_32_bits():
     for t, w in zip(kv, was):
         for page, content in zip((65999, 66000, 66001), w):
             assert torch.equal(t[page], content)
+
+
+def test_empty_batches_of_the_library():
+    """The entries themselves, by the workspace sizes that they name: nothing is
+    short, nothing but held pages is in use."""
+    print("case: pages of empty batches, library entries", flush=True)
+    kv, kw = _pools(6, 4)
+    before = [t.clone() for t in kv + kw]
+    pages = CachePages(kv, kw)  # (holds the array of pools)
+    h, shape, stream = _lib.lib(), pages._shape, torch.cuda.current_stream().cuda_stream
+    lacking, top, ids, held = _i32(7), _i32(7), _i32([7] * 6), _held(6, [1, 4])
+    need = h.nsv_fork_pages_workspace_size(0, 3, 6)
+    ws = torch.empty(max(need, 16), dtype=torch.uint8, device="cuda")
+    assert h.nsv_fork_pages(*shape, None, None, None, held.data_ptr(), 0, 3, None, None, lacking.data_ptr(), ws.data_ptr(), need,
+                            stream) == 0
+    need = h.nsv_compact_pages_workspace_size(6)
+    ws2 = torch.empty(need, dtype=torch.uint8, device="cuda")
+    assert h.nsv_compact_pages(*shape, None, held.data_ptr(), 0, 3, None, ids.data_ptr(), top.data_ptr(), ws2.data_ptr(), need,
+                               stream) == 0
+    torch.cuda.synchronize()
+    assert lacking.item() == 0 and top.item() == 5 and ids.tolist() == [-1, 1, -1, -1, 4, -1]
+    _same(kv + kw, before)
