@@ -40,9 +40,9 @@ class CachePages:
 
     caches: K and V pools (num_blocks, block_size, Hkv, D), of any layers,
     bfloat16 or float32; key_weights: their (num_blocks, Hkv, block_size)
-    float32 tables.  All contiguous, on one device, of one num_blocks (at most
-    262,144) and block_size.  The handle keeps the tensors; it holds no other
-    state, so several threads, streams and captured graphs may use it."""
+    float32 tables.  All contiguous and apart, on one device, of one num_blocks
+    (at most 262,144) and block_size.  The handle keeps the tensors; it holds no
+    other state, so several threads, streams and captured graphs may use it."""
 
     def __init__(self, caches, key_weights=()):
         caches, key_weights = list(caches), list(key_weights)
@@ -65,9 +65,9 @@ class CachePages:
                 raise ValueError(f"key weights must be ({nb}, num_kv_heads, {bs}), got {tuple(t.shape)}")
         self.device, self.num_blocks, self.block_size = first.device, nb, bs
         self._tensors = caches + key_weights
-        at = [t.data_ptr() for t in self._tensors]
-        if len(set(at)) < len(at):
-            raise ValueError("a pool is given twice")
+        at = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in self._tensors)
+        if any(end > start for (_, end), (start, _) in zip(at, at[1:])):
+            raise ValueError("pools overlap (their pages are moved at once)")
         pools = [_Pool(t.data_ptr(), 1, t.shape[2] * t.shape[3] * t.element_size()) for t in caches]
         pools += [_Pool(t.data_ptr(), t.shape[1], 4) for t in key_weights]
         self._pools = (_Pool * len(pools))(*pools)

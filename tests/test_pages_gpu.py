@@ -310,3 +310,16 @@ def test_empty_batches_of_the_library():
     torch.cuda.synchronize()
     assert lacking.item() == 0 and top.item() == 5 and ids.tolist() == [-1, 1, -1, -1, 4, -1]
     _same(kv + kw, before)
+
+
+def test_pools_that_overlap_are_refused():
+    """Views of one allocation are pools of their own only where they are apart."""
+    print("case: pools that overlap", flush=True)
+    kv = torch.zeros((2, 12, 4, 1, 8), device="cuda")
+    kw = torch.zeros((13, 2, 4), device="cuda")
+    CachePages([kv[0], kv[1]], [kw[:12]])
+    CachePages([kv[1, 6:], kv[0, :6], kv[0, 6:], kv[1, :6]], [kw[:6], kw[7:]])
+    for caches, weights in (([kv[0, :8], kv[0, 4:]], []), ([kv[0, 1:9], kv[1, :8], kv[0, :8]], []), ([kv[0, :6]], [kw[:6], kw[5:11]]),
+                            ([kv[0]], [kv[0, :6].view(12, 4, 4)])):
+        with pytest.raises(ValueError):
+            CachePages(caches, weights)
