@@ -43,7 +43,7 @@ class Sequence:
         self.ignore_eos = sampling_params.ignore_eos
         self.max_model_length = sampling_params.max_model_length
         # (a caller's own settings, of the reference's fields, have no filters)
-        self.top_k = min(int(getattr(sampling_params, "top_k", 0)), 0x7fffffff)
+        self.top_k = max(0, min(int(getattr(sampling_params, "top_k", 0)), 0x7fffffff))
         self.top_p = getattr(sampling_params, "top_p", 1.0)
         self.min_p = getattr(sampling_params, "min_p", 0.0)
 

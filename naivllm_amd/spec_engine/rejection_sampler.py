@@ -208,7 +208,7 @@ def _per_row(x, rows: int, dtype: torch.dtype, device, name: str) -> torch.Tenso
     if not isinstance(x, torch.Tensor):
         if isinstance(x, bool) or not isinstance(x, int if whole else (int, float)):
             raise ValueError(f"{name} must be a tensor or {'an integer' if whole else 'a number'}, got {x!r}")
-        return torch.full((rows,), min(x, 0x7fffffff) if whole else float(x), dtype=dtype, device=device)
+        return torch.full((rows,), max(-1, min(x, 0x7fffffff)) if whole else float(x), dtype=dtype, device=device)
     if tuple(x.shape) != (rows,):
         raise ValueError(f"{name} must have {rows} entries, got {tuple(x.shape)}")
     if x.dtype != dtype:

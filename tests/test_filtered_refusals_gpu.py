@@ -78,3 +78,11 @@ def test_draft_rows_of_a_larger_buffer():
     buf[2, 5] = 3.0
     got, want = _accept(draft_logits=buf[2:6], top_k=4), _accept(draft_logits=buf[2:6].clone(), top_k=4)
     assert torch.equal(got[1], want[1]) and torch.equal(got[0][:, 0], want[0][:, 0])
+
+
+@pytest.mark.parametrize("top_k", [-2 ** 31 - 1, -2 ** 40, -10 ** 30, 10 ** 30])
+def test_whole_numbers_past_32_bits(top_k):
+    """As top_k: all stay."""
+    kept = _i32(3)
+    _sample(top_k=top_k, kept=kept)
+    assert kept.tolist() == [64] * 3

@@ -38,3 +38,13 @@ def test_settings_of_the_references_fields():
 def test_a_top_k_beyond_32_bits_keeps_everything():
     seq = Sequence([1], SamplingParams(temperature=1.0, top_k=1 << 40))
     assert seq.top_k == 0x7fffffff
+
+
+@pytest.mark.parametrize("top_k", [-1, -2 ** 31 - 1, -2 ** 40])
+def test_a_callers_own_settings_below_zero_keep_everything(top_k):
+    class Own:
+        temperature, max_tokens, ignore_eos, max_model_length = 0.8, 5, False, None
+
+    Own.top_k = top_k
+    seq = Sequence([1], Own())
+    assert seq.top_k == 0 and not seq.filtered
