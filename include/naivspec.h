@@ -517,8 +517,11 @@ int nsv_sample(const void* logits, int64_t row_stride, const float* temperature,
  *   min_p  those with w >= min_p, every maximum at least (<= 0 or NaN: all)
  * What all three leave has the sum W; p(token) = w / W in it, 0 outside.  The
  * sample of u is the first token of the order whose running sum exceeds u W.
- * Sums are exact to 2^-44 of the largest weight per token.  top_k, top_p and
- * min_p are [B] and may be NULL (all stay); uniforms are in [0, 1).
+ * A running sum of V weights is within V 2^-(s+1) of the largest, s the lesser
+ * of 50 and 62 - ceil(log2 V) (2^-27.8 at 151,936 tokens), beside an
+ * exponential's rounding, 2^-47 of each.  top_k, top_p and min_p are [B]
+ * and may be NULL (all stay); uniforms are in [0, 1); 1 and more is taken for
+ * the last kept token with a weight, less than 0 and NaN for 0.
  * V <= 2^20, B <= 65,535; K <= 63.
  *
  * nsv_sample_filtered: row b at b * row_stride elements (any row_stride >= V),

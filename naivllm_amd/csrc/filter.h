@@ -78,7 +78,8 @@ struct FilterArgs {
 };
 
 __device__ __forceinline__ bool is_greedy(float T) { return !(T > 1e-6f); }
-// u of the sample's goal u W: what is no number in [0, 1] is taken to its end
+// u of the sample's goal u W: what is no number in [0, 1] is taken to its end (1,
+// which no running sum exceeds: the last token kept that has a weight)
 __device__ __forceinline__ double unit(float u) { return fmin(fmax((double)u, 0.0), 1.0); }
 // sequence b's drafts are decided by their probabilities
 __device__ __forceinline__ bool by_rows(const FilterArgs& a, int b) {

@@ -255,7 +255,7 @@ def sample_filtered(logits: torch.Tensor, temperature, uniforms: torch.Tensor, t
     logits (B, V) bfloat16 or float32 (rows contiguous, any pitch); V at most
     2^20.  temperature, top_k, top_p and min_p are (B,) tensors, or numbers
     for every row; None leaves a filter off, as do top_k <= 0, top_p >= 1 and
-    min_p <= 0.  uniforms (B,) float32.
+    min_p <= 0.  uniforms (B,) float32 (64-bit ones stay below 1).
 
     Of a row's tokens in falling order of their logits (equal ones by rising
     index) top-k leaves the first k, top-p the fewest whose probabilities
