@@ -45,7 +45,7 @@ def test_one_under_filters(dtype, shift, setting):
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("mode", ["model", "ngram", "hybrid"])
 def test_one_in_rounds(mode, dtype):
-    """Every number of a round 1: samples, refused drafts, residuals, bonus rows."""
+    """Nearly all numbers are 1: samples, refused drafts, residuals, bonus rows."""
     print(f"case: accept_filtered of 1, {mode} {dtype}", flush=True)
     target, draft, f, drafts, live, u = _case(61, 9, 4, 2049, dtype, near=0.02)
     f = dict(temperature=np.full(9, 0.9, np.float32), top_k=np.where(np.arange(9) % 3 == 0, 40, 0).astype(np.int32),
